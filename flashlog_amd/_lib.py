@@ -12,7 +12,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libflashlog_hip.so")
-ABI_VERSION = 25
+ABI_VERSION = 26
 FL_SEG = 32
 FL_SUP = 16
 
@@ -80,6 +80,33 @@ class FlGroundGraph(ctypes.Structure):
         ("nodes", ctypes.c_int64), ("num_relations", ctypes.c_int64), ("max_groups", ctypes.c_int64),
         ("nhub", ctypes.c_int64), ("hub_options", ctypes.c_int64), ("hub_id", ctypes.c_void_p),
         ("hub_node", ctypes.c_void_p), ("hub_off", ctypes.c_void_p),
+    ]
+
+
+class FlLinear(ctypes.Structure):
+    """Mirror of ``fl_linear`` (include/flashlog_hip.h)."""
+    _fields_ = [
+        ("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("groups", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("ldw", ctypes.c_int64), ("w_group", ctypes.c_int64),
+        ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("ldres", ctypes.c_int64),
+        ("order", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("tiles", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32), ("act", ctypes.c_int32), ("bias_f32", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class FlLogits(ctypes.Structure):
+    """Mirror of ``fl_logits`` (include/flashlog_hip.h)."""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("ldx", ctypes.c_int64),
+        ("inner", ctypes.c_int64),
+        ("allowed", ctypes.c_void_p), ("allowed_rows", ctypes.c_int64), ("allowed_ld", ctypes.c_int64),
+        ("group", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("bias_rows", ctypes.c_int64),
+        ("history", ctypes.c_void_p), ("history_ptr", ctypes.c_void_p), ("history_len", ctypes.c_int64),
+        ("repetition", ctypes.c_float), ("presence", ctypes.c_float), ("frequency", ctypes.c_float),
+        ("temperature", ctypes.c_float), ("fill", ctypes.c_float), ("dtype", ctypes.c_int32),
     ]
 
 
@@ -222,6 +249,31 @@ _SIGS = {
     "fl_filter_expand_fill": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_int64, ctypes.c_void_p,
                                                                     ctypes.c_void_p, ctypes.c_int64] +
                               [ctypes.c_void_p] * 3),
+    "fl_group_block": (ctypes.c_int64, [ctypes.c_int64] * 2),
+    "fl_group_tiles": (ctypes.c_int64, [ctypes.c_int64] * 2),
+    "fl_group_rows_bytes": (ctypes.c_size_t, [ctypes.c_int64] * 2),
+    "fl_group_rows": (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_void_p] * 4 +
+                      [ctypes.c_size_t]),
+    "fl_linear_op_bytes": (ctypes.c_size_t, []),
+    "fl_linear_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 2),
+    "fl_linear_act_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                          ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "fl_linear_input_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 2),
+    "fl_linear_weight_grad_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLinear)]),
+    "fl_linear_weight_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 3 +
+                              [ctypes.c_size_t]),
+    "fl_linear_bias_grad_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLinear)]),
+    "fl_linear_bias_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 2 +
+                            [ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t]),
+    "fl_logits_op_bytes": (ctypes.c_size_t, []),
+    "fl_pack_bits": (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_void_p]),
+    "fl_logits_constrain": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLogits), ctypes.c_void_p]),
+    "fl_logits_softmax_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLogits)]),
+    "fl_logits_softmax": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLogits)] + [ctypes.c_void_p] * 2 +
+                          [ctypes.c_size_t]),
+    "fl_logits_grad_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLogits)] + [ctypes.c_int] * 2),
+    "fl_logits_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLogits)] + [ctypes.c_void_p] * 7 +
+                       [ctypes.c_size_t]),
     "fl_prof_enable": (ctypes.c_int, [ctypes.c_int]),
     "fl_prof_read": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),
                                     ctypes.POINTER(ctypes.c_int64)]),
@@ -247,7 +299,8 @@ def exported_symbols():
 
 # each argument struct and the entry point returning the library's sizeof
 STRUCT_SIZES = ((FlSide, "fl_side_bytes"), (FlSparseHop, "fl_sparse_hop_bytes"),
-                (FlGroundGraph, "fl_ground_graph_bytes"))
+                (FlGroundGraph, "fl_ground_graph_bytes"), (FlLinear, "fl_linear_op_bytes"),
+                (FlLogits, "fl_logits_op_bytes"))
 
 
 def lib():

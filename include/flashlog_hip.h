@@ -824,6 +824,120 @@ int fl_ground_count(void *stream, const uint64_t *keys,
                     const int64_t *budgets, void *ws, size_t ws_bytes,
                     int64_t *rows, int64_t row_cap, int64_t *info);
 
+/* ------------------------------------------------------------------------
+ * The products that make relation logits of a generator's hidden states, and
+ * the constraints on logits and scores (no counterpart in the reference,
+ * whose model files do both with torch: src/model_DRUM_kernel.py:90-117).
+ * ------------------------------------------------------------------------ */
+
+/* Operand types. */
+#define FL_F32 0
+#define FL_BF16 1
+#define FL_F16 2
+
+#define FL_ACT_NONE 0
+#define FL_ACT_RELU 1
+#define FL_ACT_GELU 2 /* p (1 + erf(p / sqrt 2)) / 2 */
+#define FL_ACT_SILU 3
+#define FL_ACT_TANH 4
+#define FL_ACT_SIGMOID 5
+
+/* Rows grouped by index[i] in [0, groups): order [rows] receives the rows,
+ * those of a group together and in their own order, offsets [groups + 1] the
+ * groups' first places; ids outside the range come behind offsets[groups]
+ * (rows of no group).  tiles [fl_group_tiles][2], optional: (group, first
+ * place) of every run of fl_group_block rows, the entries behind the last one
+ * with group -1; the products of fl_linear take them. */
+int64_t fl_group_block(int64_t rows, int64_t groups);
+int64_t fl_group_tiles(int64_t rows, int64_t groups);
+size_t fl_group_rows_bytes(int64_t rows, int64_t groups);
+int fl_group_rows(void *stream, const int64_t *index, int64_t rows,
+                  int64_t groups, int32_t *order, int32_t *offsets,
+                  int32_t *tiles, void *ws, size_t ws_bytes);
+
+/* y [M, N] = act(x W_g^T + b_g) + residual over the rows' groups; strides in
+ * elements, y and the gradients contiguous.  order, offsets and tiles are
+ * fl_group_rows' (null: one group of all rows).  A row of no group gets its
+ * residual (or 0), and its dx is 0. */
+typedef struct fl_linear {
+    int64_t M, N, K;          /* rows, outputs, inputs                     */
+    int64_t groups;
+    const void *x;            /* [M, K], row stride ldx                    */
+    int64_t ldx;
+    const void *weight;       /* [groups, N, K], row stride ldw            */
+    int64_t ldw, w_group;
+    const void *bias;         /* [groups, N] contiguous, or null           */
+    const void *residual;     /* [M, N], row stride ldres, or null         */
+    int64_t ldres;
+    const int32_t *order, *offsets, *tiles;
+    int32_t dtype, act, bias_f32, reserved;
+} fl_linear;
+
+size_t fl_linear_op_bytes(void);
+/* pre [M, N], optional: the activation's argument, for the backward. */
+int fl_linear_forward(void *stream, const fl_linear *op, void *y, void *pre);
+/* d [n] = gy * act'(pre). */
+int fl_linear_act_grad(void *stream, int dtype, int act, const void *gy,
+                       const void *pre, int64_t n, void *d);
+/* dx [M, K] = d W_g. */
+int fl_linear_input_grad(void *stream, const fl_linear *op, const void *d,
+                         void *dx);
+/* dw [groups, N, K] = d^T x over each group's rows (0 for an empty group). */
+size_t fl_linear_weight_grad_bytes(const fl_linear *op);
+int fl_linear_weight_grad(void *stream, const fl_linear *op, const void *d,
+                          void *dw, void *ws, size_t ws_bytes);
+/* db [groups, N] = column sums of d over each group's rows. */
+size_t fl_linear_bias_grad_bytes(const fl_linear *op);
+int fl_linear_bias_grad(void *stream, const fl_linear *op, const void *d,
+                        void *db, int db_f32, void *ws, size_t ws_bytes);
+
+/* Constraints on the rows x [rows, cols] (row stride ldx, columns
+ * contiguous).  Every `inner` rows in a row share an owner (a query's steps);
+ * per owner: group[owner] picks the row of the tables that have several, and
+ * a history of column ids, history_len of them
+ * padded with ids outside [0, cols), or with history_ptr [owners + 1] the
+ * ids of [ptr[o], ptr[o+1]) in a list of history_len.  An owner whose group
+ * is outside a table has nothing allowed.  With c = how often a column is in
+ * the history:
+ *   u = x + bias; if c: u = u > 0 ? u / repetition : u * repetition,
+ *   u -= presence + frequency c;  v = u / temperature; not allowed: fill. */
+typedef struct fl_logits {
+    const void *x;
+    int64_t rows, cols, ldx, inner;
+    const int32_t *allowed;   /* [allowed_rows, allowed_ld] words, column
+                                 32 w + b in bit b of word w; null: all    */
+    int64_t allowed_rows, allowed_ld;
+    const int64_t *group;     /* [owners] or null                          */
+    const float *bias;        /* [bias_rows, cols] or null                 */
+    int64_t bias_rows;
+    const int64_t *history;   /* null: none                                */
+    const int64_t *history_ptr;
+    int64_t history_len;
+    float repetition, presence, frequency, temperature, fill;
+    int32_t dtype;
+} fl_logits;
+
+size_t fl_logits_op_bytes(void);
+/* words [rows, ceil(cols / 32)] of a byte mask [rows, cols] (nonzero: 1). */
+int fl_pack_bits(void *stream, const uint8_t *mask, int64_t rows, int64_t cols,
+                 int32_t *words);
+/* out [rows, cols] of x's type. */
+int fl_logits_constrain(void *stream, const fl_logits *op, void *out);
+/* w [rows, cols] = softmax of the constrained row over its allowed columns,
+ * 0 elsewhere and in rows with nothing left: a hop's attention. */
+size_t fl_logits_softmax_bytes(const fl_logits *op);
+int fl_logits_softmax(void *stream, const fl_logits *op, float *w, void *ws,
+                      size_t ws_bytes);
+/* Gradients of fl_logits_constrain (w null, grad of x's type) or of
+ * fl_logits_softmax (w its output, grad fp32): dx [rows, cols] of x's type,
+ * or null, and dbias [bias_rows, cols], or null.  order, offsets: the owners
+ * grouped by group (fl_group_rows), for a dbias of several rows. */
+size_t fl_logits_grad_bytes(const fl_logits *op, int softmax, int with_dbias);
+int fl_logits_grad(void *stream, const fl_logits *op, const float *w,
+                   const void *grad, const int32_t *order,
+                   const int32_t *offsets, void *dx, float *dbias, void *ws,
+                   size_t ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif
