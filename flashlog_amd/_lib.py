@@ -256,15 +256,9 @@ _SIGS = {
                       [ctypes.c_size_t]),
     "fl_linear_op_bytes": (ctypes.c_size_t, []),
     "fl_linear_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 2),
-    "fl_linear_act_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
-                                          ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
-    "fl_linear_input_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 2),
-    "fl_linear_weight_grad_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLinear)]),
-    "fl_linear_weight_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 3 +
-                              [ctypes.c_size_t]),
-    "fl_linear_bias_grad_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLinear)]),
-    "fl_linear_bias_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 2 +
-                            [ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t]),
+    "fl_linear_backward_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLinear)] + [ctypes.c_int] * 2),
+    "fl_linear_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 5 +
+                           [ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t]),
     "fl_logits_op_bytes": (ctypes.c_size_t, []),
     "fl_pack_bits": (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_void_p]),
     "fl_logits_constrain": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLogits), ctypes.c_void_p]),

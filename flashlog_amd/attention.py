@@ -66,6 +66,8 @@ def _need_gpu(what, *tensors):
 
 
 def _integers(what, name, t):
+    if t.dtype is torch.int64 and t.is_contiguous():
+        return t
     if t.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8):
         raise TypeError("%s: %s must hold integers" % (what, name))
     return t.long().contiguous()
@@ -120,118 +122,111 @@ def group_rows(index, groups):
 
 def _rows_of(t, cols):
     """t as [rows, cols] with contiguous columns (a copy where its strides allow no such view)."""
-    t = t.reshape(math.prod(t.shape[:-1]), cols)
+    if t.dim() != 2:
+        t = t.reshape(math.prod(t.shape[:-1]), cols)
     return t if cols <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
 def _linear_op(x, weight, bias, residual, plan, act):
     M, K = x.shape
     N = weight.shape[-2]
-    grouped = plan is not None
-    return FlLinear(M, N, K, plan.groups if grouped else 1, x.data_ptr(), x.stride(0), weight.data_ptr(),
-                    weight.stride(-2), weight.stride(0) if grouped else 0,
-                    bias.data_ptr() if bias is not None else None,
-                    residual.data_ptr() if residual is not None else None,
-                    residual.stride(0) if residual is not None else 0,
-                    plan.order.data_ptr() if grouped else None, plan.offsets.data_ptr() if grouped else None,
-                    plan.tiles.data_ptr() if grouped else None, _TYPES[x.dtype], act,
-                    int(bias is not None and bias.dtype == torch.float32), 0)
+    if plan is None:
+        groups, w_group, order, offsets, tiles = 1, 0, None, None, None
+    else:
+        groups, w_group = plan.groups, weight.stride(0)
+        order, offsets, tiles = plan.order.data_ptr(), plan.offsets.data_ptr(), plan.tiles.data_ptr()
+    return FlLinear(M, N, K, groups, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(-2), w_group,
+                    None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
+                    0 if residual is None else residual.stride(0), order, offsets, tiles, _TYPES[x.dtype], act,
+                    int(bias is not None and bias.dtype is torch.float32), 0)
 
 
 def _linear_forward(x, weight, bias, residual, plan, act, keep):
-    """(y, the activation's argument or None)."""
+    """(y, the laid out x and weight, the activation's argument or None)."""
     dev = x.device
-    y = torch.empty((x.shape[0], weight.shape[-2]), dtype=x.dtype, device=dev)
-    pre = torch.empty_like(y) if keep else None
+    N, K = weight.shape[-2:]
+    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=dev)
+    x = _rows_of(x, K)
+    if K > 1 and weight.stride(-1) != 1:
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if residual is not None:
+        residual = _rows_of(residual, N)
+    pre = torch.empty((x.shape[0], N), dtype=torch.float32, device=dev) if keep else None
     op = _linear_op(x, weight, bias, residual, plan, act)
     with _on(dev):
         check(_lib.lib().fl_linear_forward(stream_handle(dev), op, ptr(y), ptr(pre)), "linear")
-    return y, pre
+    return y, x, weight, pre
 
 
 class _LinearFunction(autograd.Function):
-    """act(x W_g^T + b_g) + residual of 2D rows; plan None: one group."""
+    """act(x W_g^T + b_g) + residual; plan None: one group."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, plan, act):
-        slopes = act != 0 and any(ctx.needs_input_grad[:3])
-        y, pre = _linear_forward(x, weight, bias, residual, plan, act, slopes)
-        ctx.save_for_backward(x, weight, pre)
-        ctx.plan, ctx.act = plan, act
-        ctx.bias_dtype = bias.dtype if bias is not None else None
+        keep = act != 0 and any(ctx.needs_input_grad[:3])
+        y, x2, w2, pre = _linear_forward(x, weight, bias, residual, plan, act, keep)
+        ctx.save_for_backward(x2, w2, pre)
+        ctx.plan, ctx.act, ctx.shapes = plan, act, (x.shape, bias.dtype if bias is not None else None)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         x, weight, pre = ctx.saved_tensors
-        need = ctx.needs_input_grad
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
-        if any(need[:3]):
+        if need_x or need_w or need_b:
             dev, lib = x.device, _lib.lib()
-            d = grad.contiguous()
+            (shape, bias_dtype), g = ctx.shapes, grad.contiguous()
             op = _linear_op(x, weight, None, None, ctx.plan, ctx.act)
+            if need_x:
+                dx = torch.empty(shape, dtype=x.dtype, device=dev)
+            if need_w:
+                dw = torch.empty(weight.shape, dtype=x.dtype, device=dev)
+            if need_b:
+                db = torch.empty(weight.shape[:-1], dtype=bias_dtype, device=dev)
+            nbytes = lib.fl_linear_backward_bytes(op, need_w, need_b)
+            ws = _workspace(nbytes, dev)
             with _on(dev):
-                st = stream_handle(dev)
-                if pre is not None:
-                    g, d = d, torch.empty_like(pre)
-                    check(lib.fl_linear_act_grad(st, _TYPES[x.dtype], ctx.act, ptr(g), ptr(pre), d.numel(), ptr(d)),
-                          "linear")
-                if need[0]:
-                    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-                    check(lib.fl_linear_input_grad(st, op, ptr(d), ptr(dx)), "linear")
-                if need[1]:
-                    dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev)
-                    nbytes = lib.fl_linear_weight_grad_bytes(op)
-                    ws = _workspace(nbytes, dev)
-                    check(lib.fl_linear_weight_grad(st, op, ptr(d), ptr(dw), ptr(ws), nbytes), "linear")
-                if need[2]:
-                    db = torch.empty(weight.shape[:-1], dtype=ctx.bias_dtype, device=dev)
-                    nbytes = lib.fl_linear_bias_grad_bytes(op)
-                    ws = _workspace(nbytes, dev)
-                    check(lib.fl_linear_bias_grad(st, op, ptr(d), ptr(db), int(db.dtype == torch.float32), ptr(ws),
-                                                  nbytes), "linear")
-        return dx, dw, db, grad if need[3] else None, None, None
+                check(lib.fl_linear_backward(stream_handle(dev), op, ptr(g), ptr(pre), ptr(dx), ptr(dw), ptr(db),
+                                             int(bias_dtype is torch.float32), ptr(ws), nbytes), "linear")
+        return dx, dw, db, grad if need_r else None, None, None
 
 
 def _product(what, x, plan, weight, bias, activation, residual):
     _need_gpu(what, x, weight, bias, residual, plan.order if plan is not None else None)
-    if activation not in _ACTIVATIONS:
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError("%s: activation must be one of %s" % (what, ", ".join(map(repr, _ACTIVATIONS))))
-    if x.dtype not in _TYPES:
+    dtype, wshape, xshape = x.dtype, weight.shape, x.shape
+    if dtype not in _TYPES:
         raise TypeError("%s: x must be float32, bfloat16 or float16" % what)
-    if weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype):
+    if weight.dtype is not dtype or (residual is not None and residual.dtype is not dtype):
         raise TypeError("%s: x, weight and residual must be of one type" % what)
-    if bias is not None and bias.dtype not in (x.dtype, torch.float32):
-        raise TypeError("%s: bias must be of x's type or float32" % what)
-    dims = 2 if plan is None else 3
-    if weight.dim() != dims or x.dim() < 1:
-        raise ValueError("%s: weight must be [%soutputs, inputs] and x [..., inputs]" % (what, "groups, " * (dims - 2)))
-    N, K = weight.shape[-2:]
-    if x.shape[-1] != K:
-        raise ValueError("%s: x has %d inputs, weight %d" % (what, x.shape[-1], K))
-    if plan is not None and weight.shape[0] != plan.groups:
-        raise ValueError("%s: weight has %d groups, the plan %d" % (what, weight.shape[0], plan.groups))
-    if bias is not None and bias.shape != weight.shape[:-1]:
-        raise ValueError("%s: bias must be %s" % (what, list(weight.shape[:-1])))
-    shape = x.shape[:-1] + (N,)
-    if residual is not None and residual.shape != shape:
-        raise ValueError("%s: residual must be %s" % (what, list(shape)))
-    x = _rows_of(x, K)
-    if plan is not None and x.shape[0] != plan.rows:
-        raise ValueError("%s: x has %d rows, the plan %d" % (what, x.shape[0], plan.rows))
-    if K > 1 and weight.stride(-1) != 1:
-        weight = weight.contiguous()
+    if len(wshape) != (2 if plan is None else 3) or len(xshape) < 1:
+        raise ValueError("%s: weight must be [%soutputs, inputs] and x [..., inputs]"
+                         % (what, "" if plan is None else "groups, "))
+    if xshape[-1] != wshape[-1]:
+        raise ValueError("%s: x has %d inputs, weight %d" % (what, xshape[-1], wshape[-1]))
     if bias is not None:
-        bias = bias.contiguous()
-    if residual is not None:
-        residual = _rows_of(residual, N)
-    act = _ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        y = _LinearFunction.apply(x, weight, bias, residual, plan, act)
-    else:
-        y = _linear_forward(x, weight, bias, residual, plan, act, False)[0]
-    return y.view(shape)
+        if bias.dtype is not dtype and bias.dtype is not torch.float32:
+            raise TypeError("%s: bias must be of x's type or float32" % what)
+        if bias.shape != wshape[:-1]:
+            raise ValueError("%s: bias must be %s" % (what, list(wshape[:-1])))
+    if residual is not None and residual.shape != xshape[:-1] + wshape[-2:-1]:
+        raise ValueError("%s: residual must be %s" % (what, list(xshape[:-1] + wshape[-2:-1])))
+    if plan is not None:
+        if wshape[0] != plan.groups:
+            raise ValueError("%s: weight has %d groups, the plan %d" % (what, wshape[0], plan.groups))
+        if math.prod(xshape[:-1]) != plan.rows:
+            raise ValueError("%s: x has %d rows, the plan %d" % (what, math.prod(xshape[:-1]), plan.rows))
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
+        return _LinearFunction.apply(x, weight, bias, residual, plan, act)
+    return _linear_forward(x, weight, bias, residual, plan, act, False)[0]
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
@@ -243,8 +238,9 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     operands whose last dimension is not contiguous are copied.  Sums are
     float32 and the result is rounded once; with float32 operands products
     are as exact as float32 ones, except that a sum which an infinity or NaN
-    enters is NaN.  For the gradients of bfloat16 and float16 operands the
-    activation's argument and its gradient are kept in their type."""
+    enters is NaN.  For the backward the
+    activation's argument is kept in float32; its gradient is rounded to the
+    operands' type, as an operand of two products."""
     return _product("linear", x, None, weight, bias, activation, residual)
 
 
@@ -293,21 +289,18 @@ def history_from_pairs(rows, ids, count):
 
 
 class _Constraints:
-    """The checked arguments of one call."""
+    """The checked arguments of one call, laid out."""
 
-    __slots__ = ("rows", "cols", "inner", "allowed", "group", "bias", "history", "history_ptr", "scalars")
+    __slots__ = ("rows", "cols", "inner", "allowed", "group", "history", "history_ptr", "scalars")
 
     def op(self, x, bias):
-        a, h = self.allowed, self.history
-        return FlLogits(x.data_ptr() if x is not None else None, self.rows, self.cols,
-                        x.stride(0) if x is not None else 0, self.inner,
-                        a.data_ptr() if a is not None else None, a.shape[0] if a is not None else 0,
-                        a.stride(0) if a is not None else 0,
-                        self.group.data_ptr() if self.group is not None else None,
-                        bias.data_ptr() if bias is not None else None, bias.shape[0] if bias is not None else 0,
-                        h.data_ptr() if h is not None else None,
-                        self.history_ptr.data_ptr() if self.history_ptr is not None else None,
-                        h.shape[-1] if h is not None else 0, *self.scalars)
+        a, h, g, p = self.allowed, self.history, self.group, self.history_ptr
+        return FlLogits(x.data_ptr(), self.rows, self.cols, x.stride(0), self.inner,
+                        None if a is None else a.data_ptr(), 0 if a is None else a.shape[0],
+                        0 if a is None else a.shape[1], None if g is None else g.data_ptr(),
+                        None if bias is None else bias.data_ptr(), 0 if bias is None else bias.shape[0],
+                        None if h is None else h.data_ptr(), None if p is None else p.data_ptr(),
+                        0 if h is None else h.shape[-1], *self.scalars)
 
 
 def _spread(t, count):
@@ -315,7 +308,20 @@ def _spread(t, count):
     return t if t.shape[0] == count else t.repeat_interleave(count // max(t.shape[0], 1), 0)
 
 
-def _constraints(what, logits, allowed, group, bias, history, repetition, presence, frequency, temperature, fill):
+def _table(what, name, t, width, group):
+    """A table [width] or [groups, width] as [groups, width]."""
+    if t.dim() not in (1, 2) or t.shape[-1] != width:
+        raise ValueError("%s: %s must be [%d] or [groups, %d]" % (what, name, width, width))
+    if t.dim() == 1:
+        t = t.reshape(1, width)
+    if t.shape[0] != 1 and group is None:
+        raise ValueError("%s: %s has %d rows; group says which of them a row takes" % (what, name, t.shape[0]))
+    if t.shape[0] == 0:
+        raise ValueError("%s: %s has no rows" % (what, name))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _constraints(what, logits, allowed, group, bias, history, *scalars):
     past, offsets = history, None
     if isinstance(history, (tuple, list)):
         if len(history) != 2:
@@ -324,118 +330,113 @@ def _constraints(what, logits, allowed, group, bias, history, repetition, presen
     _need_gpu(what, logits, allowed, group, bias, past, offsets)
     if logits.dtype not in _TYPES:
         raise TypeError("%s: logits must be float32, bfloat16 or float16" % what)
+    lead = logits.shape[:-1]
     if logits.dim() < 1:
         raise ValueError("%s: logits must be [..., columns]" % what)
-    for name, v, least in (("repetition", repetition, 0.0), ("temperature", temperature, 0.0),
-                           ("presence", presence, None), ("frequency", frequency, None)):
-        if not math.isfinite(v) or (least is not None and not v > least):
-            raise ValueError("%s: %s must be %s" % (what, name, "finite" if least is None else "positive"))
-    lead, n = logits.shape[:-1], logits.shape[-1]
+    scalars = [float(v) for v in scalars]
+    for name, v in zip(("repetition", "presence", "frequency", "temperature"), scalars):
+        if not math.isfinite(v) or (v <= 0.0 and name in ("repetition", "temperature")):
+            raise ValueError("%s: %s must be finite%s" % (what, name, "" if name[-4:] in ("ence", "ency") else
+                                                          " and positive"))
     c = _Constraints()
-    c.rows, c.cols = math.prod(lead), n
+    c.rows, c.cols = math.prod(lead), logits.shape[-1]
 
     def owners_of(shape, name):
-        if tuple(shape) != tuple(lead[:len(shape)]):
+        if shape != lead[:len(shape)]:
             raise ValueError("%s: %s is for rows %s, the logits have %s" % (what, name, list(shape), list(lead)))
         return math.prod(shape)
 
-    counts = []
+    owners = None
     if group is not None:
-        counts.append(owners_of(group.shape, "group"))
-        group = _integers(what, "group", group).reshape(-1)
+        owners = owners_of(group.shape, "group")
+        group = _integers(what, "group", group)
+        if group.dim() != 1:
+            group = group.reshape(-1)
     if past is not None:
         past = _integers(what, "history", past)
         if offsets is not None:
             if past.dim() != 1 or offsets.dim() != 1 or offsets.numel() < 1:
                 raise ValueError("%s: a ragged history is 1D offsets and 1D ids" % what)
             offsets = _integers(what, "history", offsets)
-            owners = offsets.numel() - 1
-            if owners not in [math.prod(lead[:k]) for k in range(len(lead) + 1)]:
-                raise ValueError("%s: history is for %d rows, the logits have %s" % (what, owners, list(lead)))
+            listed = offsets.numel() - 1
+            if listed not in [math.prod(lead[:k]) for k in range(len(lead) + 1)]:
+                raise ValueError("%s: history is for %d rows, the logits have %s" % (what, listed, list(lead)))
         else:
             if past.dim() < 1:
                 raise ValueError("%s: history must be [..., ids]" % what)
-            owners = owners_of(past.shape[:-1], "history")
-            past = past.reshape(owners, past.shape[-1])
-        counts.append(owners)
-    owners = max(counts) if counts else c.rows
+            listed = owners_of(past.shape[:-1], "history")
+            if past.dim() != 2:
+                past = past.reshape(listed, past.shape[-1])
+        if owners is None or listed > owners:
+            owners = listed
+        if offsets is None:
+            past = _spread(past, owners)
+        elif listed != owners:
+            raise ValueError("%s: a ragged history needs as many rows as group has" % what)
     if group is not None:
         group = _spread(group, owners)
-    if past is not None and offsets is None:
-        past = _spread(past, owners)
-    elif past is not None and offsets.numel() - 1 != owners:
-        raise ValueError("%s: a ragged history needs as many rows as group has" % what)
     c.inner = max(c.rows // owners, 1) if owners else 1
     if allowed is not None:
-        if allowed.dtype == torch.bool:
-            if allowed.shape[-1:] != (n,):
-                raise ValueError("%s: allowed must be [..., %d]" % (what, n))
+        if allowed.dtype is torch.bool:
+            if allowed.shape[-1:] != (c.cols,):
+                raise ValueError("%s: allowed must be [..., %d]" % (what, c.cols))
             allowed = pack_allowed(allowed)
-        elif allowed.dtype != torch.int32:
+        elif allowed.dtype is not torch.int32:
             raise TypeError("%s: allowed must be a bool mask or pack_allowed's words" % what)
-        if allowed.dim() not in (1, 2) or allowed.shape[-1] != (n + 31) // 32:
-            raise ValueError("%s: allowed must be [%d words] or [groups, %d words]" % ((what,) + ((n + 31) // 32,) * 2))
-        allowed = allowed.reshape(-1, allowed.shape[-1]).contiguous()
+        allowed = _table(what, "allowed", allowed, (c.cols + 31) // 32, group)
     if bias is not None:
         if bias.dtype not in _TYPES:
             raise TypeError("%s: bias must be float32, bfloat16 or float16" % what)
-        if bias.dim() not in (1, 2) or bias.shape[-1] != n:
-            raise ValueError("%s: bias must be [%d] or [groups, %d]" % (what, n, n))
-        bias = bias.float().reshape(-1, n).contiguous()
-    for name, t in (("allowed", allowed), ("bias", bias)):
-        if t is not None and t.shape[0] != 1 and group is None:
-            raise ValueError("%s: %s has %d rows; group says which of them a row takes" % (what, name, t.shape[0]))
-    if allowed is not None and bias is not None and 1 not in (allowed.shape[0], bias.shape[0]) and \
-            allowed.shape[0] != bias.shape[0]:
-        raise ValueError("%s: allowed and bias have different numbers of groups" % what)
-    if (allowed is not None and allowed.shape[0] == 0) or (bias is not None and bias.shape[0] == 0):
-        raise ValueError("%s: a table without rows" % what)
+        bias = _table(what, "bias", bias.float(), c.cols, group)
+        if allowed is not None and 1 not in (allowed.shape[0], bias.shape[0]) and allowed.shape[0] != bias.shape[0]:
+            raise ValueError("%s: allowed and bias have different numbers of groups" % what)
     c.allowed, c.group, c.history, c.history_ptr = allowed, group, past, offsets
-    c.scalars = (repetition, presence, frequency, temperature, fill, _TYPES[logits.dtype])
-    return c, bias, _rows_of(logits, n)
+    c.scalars = (*scalars, _TYPES[logits.dtype])
+    return c, bias
 
 
-def _logits_forward(c, x, bias, softmax):
-    dev, lib = x.device, _lib.lib()
-    out = torch.empty((c.rows, c.cols), dtype=torch.float32 if softmax else x.dtype, device=dev)
+def _logits_forward(c, logits, bias, softmax):
+    """(output, the laid out logits)."""
+    dev, lib = logits.device, _lib.lib()
+    out = torch.empty(logits.shape, dtype=torch.float32 if softmax else logits.dtype, device=dev)
+    x = _rows_of(logits, c.cols)
     op = c.op(x, bias)
+    nbytes = lib.fl_logits_softmax_bytes(op) if softmax else 0
+    ws = _workspace(nbytes, dev)
     with _on(dev):
         st = stream_handle(dev)
         if softmax:
-            nbytes = lib.fl_logits_softmax_bytes(op)
-            ws = _workspace(nbytes, dev)
             check(lib.fl_logits_softmax(st, op, ptr(out), ptr(ws), nbytes), "hop_attention")
         else:
             check(lib.fl_logits_constrain(st, op, ptr(out)), "constrain_logits")
-    return out
+    return out, x
 
 
 class _LogitsFunction(autograd.Function):
     @staticmethod
-    def forward(ctx, x, bias, c, softmax):
-        out = _logits_forward(c, x, bias, softmax)
-        signs = c.history is not None and c.scalars[0] != 1.0  # the slopes go by the sign of x + bias
+    def forward(ctx, logits, bias, c, softmax):
+        out, x = _logits_forward(c, logits, bias, softmax)
+        signs = c.history is not None and c.scalars[0] != 1.0  # the slopes go by the sign of logits + bias
         ctx.save_for_backward(x if signs else None, bias, out if softmax else None, c.allowed, c.group, c.history,
                               c.history_ptr)
-        ctx.c, ctx.softmax, ctx.x = c, softmax, (x.dtype, x.device)
+        ctx.c, ctx.softmax, ctx.dtype = c, softmax, logits.dtype
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         x, bias, w = ctx.saved_tensors[:3]
-        c, (dtype, dev) = ctx.c, ctx.x
-        lib = _lib.lib()
-        grad = grad.contiguous()
+        c, lib, dev = ctx.c, _lib.lib(), grad.device
         need_x, need_b = ctx.needs_input_grad[:2]
-        dx = torch.empty((c.rows, c.cols), dtype=dtype, device=dev) if need_x else None
+        shape, grad = grad.shape, grad.contiguous()
+        dx = torch.empty(shape, dtype=ctx.dtype, device=dev) if need_x else None
         db = torch.empty_like(bias) if need_b else None
         plan = group_rows(c.group, bias.shape[0]) if need_b and bias.shape[0] > 1 else None
-        # without their signs the logits are not read: any row stands for them
-        op = c.op(x if x is not None else grad, bias)
+        # without their signs the logits are not read: the gradient's rows stand for them
+        op = c.op(x if x is not None else _rows_of(grad, c.cols), bias)
+        nbytes = lib.fl_logits_grad_bytes(op, ctx.softmax, need_b)
+        ws = _workspace(nbytes, dev)
         with _on(dev):
-            nbytes = lib.fl_logits_grad_bytes(op, int(ctx.softmax), int(need_b))
-            ws = _workspace(nbytes, dev)
             check(lib.fl_logits_grad(stream_handle(dev), op, ptr(w), ptr(grad),
                                      ptr(plan.order) if plan is not None else None,
                                      ptr(plan.offsets) if plan is not None else None, ptr(dx), ptr(db), ptr(ws),
@@ -443,12 +444,10 @@ class _LogitsFunction(autograd.Function):
         return dx, db, None, None
 
 
-def _apply(logits, c, bias, x, softmax):
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-        out = _LogitsFunction.apply(x, bias, c, softmax)
-    else:
-        out = _logits_forward(c, x, bias, softmax)
-    return out.view(logits.shape)
+def _apply(logits, c, bias, softmax):
+    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+        return _LogitsFunction.apply(logits, bias, c, softmax)
+    return _logits_forward(c, logits, bias, softmax)[0]
 
 
 def constrain_logits(logits, allowed=None, group=None, bias=None, history=None, repetition=1.0, presence=0.0,
@@ -471,9 +470,8 @@ def constrain_logits(logits, allowed=None, group=None, bias=None, history=None, 
 
     Masked logits are not read into anything: they may be infinite or NaN.
     Gradients reach logits and bias; masked columns have none."""
-    return _apply(logits, *_constraints("constrain_logits", logits, allowed, group, bias, history, float(repetition),
-                                        float(presence), float(frequency), float(temperature), float(fill)),
-                  softmax=False)
+    return _apply(logits, *_constraints("constrain_logits", logits, allowed, group, bias, history, repetition, presence,
+                                        frequency, temperature, fill), softmax=False)
 
 
 def hop_attention(logits, allowed=None, group=None, bias=None, history=None, repetition=1.0, presence=0.0,
@@ -482,5 +480,5 @@ def hop_attention(logits, allowed=None, group=None, bias=None, history=None, rep
     columns, float32 [..., n], with the same arguments.  Masked columns are
     exactly 0; a row with nothing left (no column allowed, or every allowed
     logit -inf) is all zeros and has no gradient."""
-    return _apply(logits, *_constraints("hop_attention", logits, allowed, group, bias, history, float(repetition),
-                                        float(presence), float(frequency), float(temperature), 0.0), softmax=True)
+    return _apply(logits, *_constraints("hop_attention", logits, allowed, group, bias, history, repetition, presence,
+                                        frequency, temperature, 0.0), softmax=True)

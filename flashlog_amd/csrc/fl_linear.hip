@@ -125,31 +125,36 @@ __device__ __forceinline__ int lds_at(int r, int c) {
     return r * BK + ((c ^ f) << 3);
 }
 
-// Operand rows with k contiguous: row pointers are fixed, 8 k a load.
+// Operand rows with k contiguous: a pointer a row, 8 k a load.  The part of K
+// that is no whole tile is taken first (fetch_tail, guarded), the whole tiles
+// without guards.
 template <typename T, int BR, int BK>
 struct ContigTile {
     static constexpr int CPR = BK / 8, RP = LN_NT / CPR, PASSES = BR / RP;
     static_assert(BR % RP == 0, "whole passes");
     const T *row[PASSES];
     Vec<T, 8> raw[PASSES];
-    int64_t K;
 
     template <typename F>
-    __device__ __forceinline__ void init(F &&row_ptr, int64_t k) {
-        K = k;
+    __device__ __forceinline__ void init(F &&row_ptr) {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) row[i] = row_ptr(threadIdx.x / CPR + i * RP);
+        for (int i = 0; i < PASSES; ++i) row[i] = row_ptr(threadIdx.x / CPR + i * RP) + (threadIdx.x % CPR) * 8;
     }
-    __device__ __forceinline__ void fetch(int64_t k0) {
-        const int64_t kk = k0 + (threadIdx.x % CPR) * 8;
-        if (kk + 8 <= K) {
+    // The first `left` < BK values of every row.
+    __device__ __forceinline__ void fetch_tail(int64_t left) {
+        const int have = (int)left - (int)(threadIdx.x % CPR) * 8;
 #pragma unroll
-            for (int i = 0; i < PASSES; ++i) raw[i] = load_vec<T, 8>(row[i] + kk);
-        } else {
+        for (int i = 0; i < PASSES; ++i) {
 #pragma unroll
-            for (int i = 0; i < PASSES; ++i)
+            for (int j = 0; j < 8; ++j) raw[i].v[j] = j < have ? row[i][j] : (T)0.0f;
+            row[i] += left;
+        }
+    }
+    __device__ __forceinline__ void fetch() {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) raw[i].v[j] = kk + j < K ? row[i][kk + j] : (T)0.0f;
+        for (int i = 0; i < PASSES; ++i) {
+            raw[i] = load_vec<T, 8>(row[i]);
+            row[i] += BK;
         }
     }
     __device__ __forceinline__ void stage(uint16_t *lds, int plane) const {
@@ -166,54 +171,67 @@ struct ContigTile {
 };
 
 // Operand rows with k strided: element (k, r) at base + row_of(k) * ld + r.
-// Lanes take consecutive r (a word's worth of them each), a thread 8 k.
+// Lanes take consecutive r, a word's worth of them each, a thread 8 k.  Lanes
+// behind the last of the R columns read it again: their products are not
+// stored.  (Two columns a word need R >= 2; at an odd end the pair before it
+// is read and shifted.)
 template <typename T, int BR, int BK>
 struct StridedTile {
     static constexpr int V = BR >= 128 ? 4 / (int)sizeof(T) : 1;
     static constexpr int LR = BR / V < FL_WAVE ? BR / V : FL_WAVE;  // lanes along r
     static constexpr int RPASS = BR / (LR * V), SLOTS = LN_NT / LR, CPR = BK / 8, CP = CPR / SLOTS;
     static_assert(CP >= 1 && CPR % SLOTS == 0 && BR % (LR * V) == 0, "whole passes");
-    const T *base;
+    const T *col[RPASS];
     const int32_t *order;
-    int64_t ld, K, R;  // K, R: extents (positions of k; columns from base)
+    int64_t ld, k;  // k: first place of the thread's slot
     uint32_t raw[CP][RPASS][8];
-    int slot, col;
+    int slot, shift[RPASS];
 
-    __device__ __forceinline__ void init(const T *b, int64_t stride, int64_t k, int64_t r, const int32_t *ord) {
-        base = b;
+    __device__ __forceinline__ void init(const T *base, int64_t stride, int64_t R, const int32_t *ord) {
         ld = stride;
-        K = k;
-        R = r;
         order = ord;
+        k = 0;
         slot = threadIdx.x / LR;
         if (LR == FL_WAVE) slot = __builtin_amdgcn_readfirstlane(slot);
-        col = (threadIdx.x % LR) * V;
-    }
-    // V values from column r on, those beyond R as 0.
-    __device__ __forceinline__ uint32_t load(const T *p, int64_t r) const {
-        if constexpr (sizeof(T) == 4) {
-            return r < R ? __builtin_bit_cast(uint32_t, p[r]) : 0u;
-        } else {
-            if (V == 2 && r + 2 <= R) {
-                uint32_t w;
-                __builtin_memcpy(&w, p + r, 4);
-                return w;
-            }
-            return r < R ? (uint32_t)__builtin_bit_cast(uint16_t, p[r]) : 0u;
+#pragma unroll
+        for (int i = 0; i < RPASS; ++i) {
+            const int64_t r = (threadIdx.x % LR) * V + i * LR * V;
+            col[i] = base + (r < R - V ? r : R - V);
+            shift[i] = V == 2 && r == R - 1 ? 16 : 0;
         }
     }
-    __device__ __forceinline__ void fetch(int64_t k0) {
+    __device__ __forceinline__ uint32_t load(const T *p) const {
+        if constexpr (sizeof(T) == 2 && V == 1) return __builtin_bit_cast(uint16_t, *p);
+        uint32_t w;
+        __builtin_memcpy(&w, p, 4);
+        return w;
+    }
+    __device__ __forceinline__ int64_t at(int64_t place) const { return (order ? (int64_t)order[place] : place) * ld; }
+    __device__ __forceinline__ void fetch_tail(int64_t left) {
 #pragma unroll
-        for (int cp = 0; cp < CP; ++cp) {
-            const int64_t kk = k0 + (slot + cp * SLOTS) * 8;
+        for (int cp = 0; cp < CP; ++cp)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int64_t k = kk + j;
-                const T *p = base + (k < K ? (order ? (int64_t)order[k] : k) * ld : 0);
+                const int64_t q = (slot + cp * SLOTS) * 8 + j;
+                const int64_t o = at(q < left ? q : left - 1);
 #pragma unroll
-                for (int i = 0; i < RPASS; ++i) raw[cp][i][j] = k < K ? load(p, col + i * LR * V) : 0u;
+                for (int i = 0; i < RPASS; ++i) {
+                    const uint32_t w = load(col[i] + o);
+                    raw[cp][i][j] = q < left ? w : 0u;
+                }
             }
-        }
+        k = left;
+    }
+    __device__ __forceinline__ void fetch() {
+#pragma unroll
+        for (int cp = 0; cp < CP; ++cp)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t o = at(k + (slot + cp * SLOTS) * 8 + j);
+#pragma unroll
+                for (int i = 0; i < RPASS; ++i) raw[cp][i][j] = load(col[i] + o);
+            }
+        k += BK;
     }
     __device__ __forceinline__ void stage(uint16_t *lds, int plane) const {
 #pragma unroll
@@ -221,7 +239,7 @@ struct StridedTile {
 #pragma unroll
             for (int i = 0; i < RPASS; ++i) {
                 const uint32_t(&w)[8] = raw[cp][i];
-                const int r = col + i * LR * V, c = slot + cp * SLOTS;
+                const int r = (threadIdx.x % LR) * V + i * LR * V, c = slot + cp * SLOTS;
                 if constexpr (sizeof(T) == 4) {
                     float one[8];
 #pragma unroll
@@ -235,8 +253,9 @@ struct StridedTile {
                     u32x4 lo, hi;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        lo[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
-                        hi[j] = upper_halves(w[2 * j], w[2 * j + 1]);
+                        const uint32_t w0 = w[2 * j] >> shift[i], w1 = w[2 * j + 1] >> shift[i];
+                        lo[j] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+                        hi[j] = upper_halves(w0, w1);
                     }
                     *reinterpret_cast<u32x4 *>(lds + lds_at<BK>(r, c)) = lo;
                     if (V == 2) *reinterpret_cast<u32x4 *>(lds + lds_at<BK>(r + 1, c)) = hi;
@@ -298,19 +317,25 @@ struct Product {
 #pragma unroll
             for (int j = 0; j < NTL; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
         uint16_t *la = lds, *lb = lds + P * PLANE_A;
-        if (K > 0) {
-            ta.fetch(0);
-            tb.fetch(0);
+        if (K <= 0) return;
+        const int64_t left = K % BK;
+        if (left) {
+            ta.fetch_tail(left);
+            tb.fetch_tail(left);
+        } else {
+            ta.fetch();
+            tb.fetch();
         }
-        for (int64_t k0 = 0; k0 < K; k0 += BK) {
+        for (int64_t more = (K - 1) / BK;; --more) {
             ta.stage(la, PLANE_A);
             tb.stage(lb, PLANE_B);
             __syncthreads();
-            if (k0 + BK < K) {
-                ta.fetch(k0 + BK);
-                tb.fetch(k0 + BK);
+            if (more > 0) {
+                ta.fetch();
+                tb.fetch();
             }
             step(la, lb);
+            if (more == 0) break;
             __syncthreads();
         }
     }
@@ -358,7 +383,7 @@ struct RowsArgs {
     const int32_t *order, *offsets, *tiles;
     const void *bias, *residual;
     int64_t bias_group, ldres;
-    void *pre;
+    float *pre;
     int act, bias_f32;
 };
 
@@ -386,17 +411,16 @@ __global__ __launch_bounds__(LN_NT) void k_lin_rows(RowsArgs a) {
         [&](int r) {
             int64_t p = pos0 + r < end ? pos0 + r : end - 1;
             return A + (a.order ? (int64_t)a.order[p] : p) * a.lda;
-        },
-        a.K);
+        });
     Prod prod;
     const int64_t K = none ? 0 : a.K;
     if constexpr (B_CONTIG) {
         ContigTile<T, BN, BK> tb;
-        tb.init([&](int r) { return B + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldb; }, a.K);
+        tb.init([&](int r) { return B + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldb; });
         prod.run(ta, tb, K, lds);
     } else {
         StridedTile<T, BN, BK> tb;
-        tb.init(B + n0, a.ldb, a.K, a.N - n0, nullptr);
+        tb.init(B + n0, a.ldb, a.N - n0, nullptr);
         prod.run(ta, tb, K, lds);
     }
     const int lane = fl_lane();
@@ -419,16 +443,15 @@ __global__ __launch_bounds__(LN_NT) void k_lin_rows(RowsArgs a) {
                 for (int e = 0; e < 4; ++e)
                     if (e < m) v[e] += a.bias_f32 ? ((const float *)a.bias)[at + e] : (float)((const T *)a.bias)[at + e];
             }
-            Vec<T, 4> o;
             if (a.pre) {
-                // the activation's argument is kept in the operands' type: its rounding (half a step) moves
-                // the slope by less than the rounding of the gradients that use it
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o.v[e] = (T)v[e];
-                T *q = (T *)a.pre + row * a.N + n;
-                if (m == 4) store_vec<T, 4>(q, o);
-                else store_some<T, 4>(q, o, m);
+                // kept in 32 bits: rounded to the operands' type it would move the slopes by as much as the
+                // gradients' own rounding does
+                const Vec<float, 4> f{{v[0], v[1], v[2], v[3]}};
+                float *q = a.pre + row * a.N + n;
+                if (m == 4) store_vec<float, 4>(q, f);
+                else store_some<float, 4>(q, f, m);
             }
+            Vec<T, 4> o;
             if (!none)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = act_value(v[e], a.act);
@@ -495,8 +518,8 @@ __global__ __launch_bounds__(LN_NT) void k_lin_outer(OuterArgs a) {
     }
     StridedTile<T, BM, BK> ta;
     StridedTile<T, BN, BK> tb;
-    ta.init(D, a.ldd, len, a.N - m0, ord);
-    tb.init(X, a.ldx, len, a.K - c0, ord);
+    ta.init(D, a.ldd, a.N - m0, ord);
+    tb.init(X, a.ldx, a.K - c0, ord);
     Prod prod;
     prod.run(ta, tb, len, lds);
     const int lane = fl_lane();
@@ -527,21 +550,21 @@ __global__ __launch_bounds__(LN_NT) void k_lin_outer(OuterArgs a) {
     }
 }
 
-// d = gy * act'(p).
+// d = gy * act'(p), rounded to the operands' type: it is an operand of two products.
 template <typename T>
-__global__ __launch_bounds__(LN_NT) void k_act_grad(const T *__restrict__ gy, const T *__restrict__ pre, int64_t n,
+__global__ __launch_bounds__(LN_NT) void k_act_grad(const T *__restrict__ gy, const float *__restrict__ pre, int64_t n,
                                                     int act, T *__restrict__ d) {
-    constexpr int V = 16 / (int)sizeof(T);
-    const int64_t i = ((int64_t)blockIdx.x * LN_NT + threadIdx.x) * V;
+    const int64_t i = ((int64_t)blockIdx.x * LN_NT + threadIdx.x) * 4;
     if (i >= n) return;
-    if (i + V <= n) {
-        const Vec<T, V> g = load_vec<T, V>(gy + i), p = load_vec<T, V>(pre + i);
-        Vec<T, V> o;
+    if (i + 4 <= n) {
+        const Vec<T, 4> g = load_vec<T, 4>(gy + i);
+        const Vec<float, 4> p = load_vec<float, 4>(pre + i);
+        Vec<T, 4> o;
 #pragma unroll
-        for (int e = 0; e < V; ++e) o.v[e] = (T)((float)g.v[e] * act_slope((float)p.v[e], act));
-        store_vec<T, V>(d + i, o);
+        for (int e = 0; e < 4; ++e) o.v[e] = (T)((float)g.v[e] * act_slope(p.v[e], act));
+        store_vec<T, 4>(d + i, o);
     } else
-        for (int64_t e = i; e < n; ++e) d[e] = (T)((float)gy[e] * act_slope((float)pre[e], act));
+        for (int64_t e = i; e < n; ++e) d[e] = (T)((float)gy[e] * act_slope(pre[e], act));
 }
 
 // Column sums of a group's rows (a part of them), one thread a column.
@@ -600,14 +623,17 @@ template <typename T, bool B_CONTIG>
 int launch_rows(hipStream_t st, const fl_linear *op, RowsArgs &a, const char *what) {
     const int bm = tile_rows(op, a.N);
     constexpr int BIG_K = sizeof(T) == 4 ? 32 : 64;
-    const int bn = bm == 128 ? 128 : 64;
+    const int bn = bm == 128 && a.N > 64 ? 128 : 64;
     const int64_t m_tiles = op->offsets ? fl_group_tiles(op->M, op->groups) : ceil_div(op->M, bm);
     a.n_tiles = (uint32_t)ceil_div(a.N, bn);
     const int64_t grid = m_tiles * a.n_tiles;
     if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "%s: too many tiles for one launch (shape)", what);
     if (grid == 0) return FL_OK;
-    if (bm == 128)
+    if (bn == 128)
         FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 128, 128, BIG_K>), dim3((unsigned)grid), dim3(LN_NT), 0, st,
+                  a);
+    else if (bm == 128)
+        FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 128, 64, BIG_K>), dim3((unsigned)grid), dim3(LN_NT), 0, st,
                   a);
     else
         FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 32, 64, 64>), dim3((unsigned)grid), dim3(LN_NT), 0, st, a);
@@ -649,7 +675,7 @@ int check_op(const fl_linear *op, const char *what) {
 }
 
 template <typename T>
-int forward(hipStream_t st, const fl_linear *op, void *y, void *pre) {
+int forward(hipStream_t st, const fl_linear *op, void *y, float *pre) {
     RowsArgs a{};
     a.a = op->x;
     a.lda = op->ldx;
@@ -739,12 +765,51 @@ int bias_grad(hipStream_t st, const fl_linear *op, const void *d, void *db, int 
 }
 
 template <typename T>
-int act_grad(hipStream_t st, int act, const void *gy, const void *pre, int64_t n, void *d) {
-    const int64_t grid = ceil_div(n, LN_NT * (16 / (int)sizeof(T)));
-    if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "linear_act_grad: too many values for one launch (shape)");
-    FL_LAUNCH("k_act_grad", k_act_grad<T>, dim3((unsigned)grid), dim3(LN_NT), 0, st, (const T *)gy, (const T *)pre, n,
-              act, (T *)d);
-    return fl_check_launch("linear_act_grad");
+int act_grad(hipStream_t st, int act, const void *gy, const float *pre, int64_t n, void *d) {
+    const int64_t grid = ceil_div(n, LN_NT * 4);
+    if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "linear_backward: too many values for one launch (shape)");
+    FL_LAUNCH("k_act_grad", k_act_grad<T>, dim3((unsigned)grid), dim3(LN_NT), 0, st, (const T *)gy, pre, n, act,
+              (T *)d);
+    return fl_check_launch("linear_backward");
+}
+
+// The backward's workspace: d (when there is an activation), the parts of dW
+// and those of db.
+struct BackwardSpace {
+    size_t d, dw, db, bytes;
+};
+
+BackwardSpace backward_space(const fl_linear *op, int with_dw, int with_db) {
+    BackwardSpace s{0, 0, 0, 0};
+    const auto take = [&](size_t n) {
+        const size_t at = s.bytes;
+        s.bytes += (n + 255) / 256 * 256;
+        return at;
+    };
+    if (op->act != FL_ACT_NONE) s.d = take((size_t)op->M * op->N * (op->dtype == FL_F32 ? 4 : 2));
+    const int64_t tiles = outer_tiles(op);
+    if (with_dw && tiles) {
+        const int parts = outer_parts(op->M, op->groups, tiles);
+        s.dw = take(parts > 1 ? (size_t)parts * op->groups * op->N * op->K * 4 : 0);
+    }
+    if (with_db && op->N) s.db = take((size_t)sum_parts(op->M, op->N, op->groups) * op->groups * op->N * 4);
+    return s;
+}
+
+template <typename T>
+int backward(hipStream_t st, const fl_linear *op, const void *gy, const float *pre, void *dx, void *dw, void *db,
+             int db_f32, char *ws) {
+    const BackwardSpace s = backward_space(op, dw != nullptr, db != nullptr);
+    const void *d = gy;
+    int rc = FL_OK;
+    if (op->act != FL_ACT_NONE && op->M && op->N) {
+        rc = act_grad<T>(st, op->act, gy, pre, op->M * op->N, ws + s.d);
+        d = ws + s.d;
+    }
+    if (!rc && dx && op->M && op->K) rc = input_grad<T>(st, op, d, dx);
+    if (!rc && dw && op->N && op->K) rc = weight_grad<T>(st, op, d, dw, (float *)(ws + s.dw));
+    if (!rc && db && op->N) rc = bias_grad<T>(st, op, d, db, db_f32, (float *)(ws + s.db));
+    return rc;
 }
 
 }  // namespace
@@ -761,7 +826,7 @@ extern "C" {
 
 size_t fl_linear_op_bytes(void) { return sizeof(fl_linear); }
 
-int fl_linear_forward(void *stream, const fl_linear *op, void *y, void *pre) {
+int fl_linear_forward(void *stream, const fl_linear *op, void *y, float *pre) {
     const int rc = fl::check_op(op, "linear_forward");
     if (rc) return rc;
     if (op->M == 0 || op->N == 0) return FL_OK;
@@ -770,53 +835,22 @@ int fl_linear_forward(void *stream, const fl_linear *op, void *y, void *pre) {
     FL_BY_TYPE(op->dtype, fl::forward<T>((hipStream_t)stream, op, y, pre))
 }
 
-int fl_linear_act_grad(void *stream, int dtype, int act, const void *gy, const void *pre, int64_t n, void *d) {
-    if (dtype < FL_F32 || dtype > FL_F16 || act < FL_ACT_NONE || act > FL_ACT_SIGMOID || n < 0)
-        return fl::fl_fail(FL_ERR_ARG, "linear_act_grad: bad type, activation or shape");
-    if (n == 0) return FL_OK;
-    if (!gy || !pre || !d) return fl::fl_fail(FL_ERR_ARG, "linear_act_grad: null pointer");
-    FL_BY_TYPE(dtype, fl::act_grad<T>((hipStream_t)stream, act, gy, pre, n, d))
+size_t fl_linear_backward_bytes(const fl_linear *op, int with_dw, int with_db) {
+    if (!op || op->M < 0 || op->N < 0 || op->K < 0 || op->groups < 1) return 0;
+    return fl::backward_space(op, with_dw, with_db).bytes;
 }
 
-int fl_linear_input_grad(void *stream, const fl_linear *op, const void *d, void *dx) {
-    const int rc = fl::check_op(op, "linear_input_grad");
+int fl_linear_backward(void *stream, const fl_linear *op, const void *gy, const float *pre, void *dx, void *dw,
+                       void *db, int db_f32, void *ws, size_t ws_bytes) {
+    const int rc = fl::check_op(op, "linear_backward");
     if (rc) return rc;
-    if (op->M == 0 || op->K == 0) return FL_OK;
-    if (!dx || (op->N > 0 && (!d || !op->weight)))
-        return fl::fl_fail(FL_ERR_ARG, "linear_input_grad: null pointer");
-    FL_BY_TYPE(op->dtype, fl::input_grad<T>((hipStream_t)stream, op, d, dx))
-}
-
-size_t fl_linear_weight_grad_bytes(const fl_linear *op) {
-    if (!op || op->groups < 1) return 0;
-    const int parts = fl::outer_parts(op->M, op->groups, fl::outer_tiles(op) < 1 ? 1 : fl::outer_tiles(op));
-    return parts > 1 ? (size_t)parts * op->groups * op->N * op->K * 4 : 0;
-}
-
-int fl_linear_weight_grad(void *stream, const fl_linear *op, const void *d, void *dw, void *ws, size_t ws_bytes) {
-    const int rc = fl::check_op(op, "linear_weight_grad");
-    if (rc) return rc;
-    if (op->N == 0 || op->K == 0) return FL_OK;
-    if (!dw || (op->M > 0 && (!d || !op->x))) return fl::fl_fail(FL_ERR_ARG, "linear_weight_grad: null pointer");
-    const size_t need = fl_linear_weight_grad_bytes(op);
-    if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "linear_weight_grad: workspace too small");
-    FL_BY_TYPE(op->dtype, fl::weight_grad<T>((hipStream_t)stream, op, d, dw, (float *)ws))
-}
-
-size_t fl_linear_bias_grad_bytes(const fl_linear *op) {
-    if (!op || op->groups < 1 || op->N < 1) return 0;
-    return (size_t)fl::sum_parts(op->M, op->N, op->groups) * op->groups * op->N * 4;
-}
-
-int fl_linear_bias_grad(void *stream, const fl_linear *op, const void *d, void *db, int db_f32, void *ws,
-                        size_t ws_bytes) {
-    const int rc = fl::check_op(op, "linear_bias_grad");
-    if (rc) return rc;
-    if (op->N == 0) return FL_OK;
-    if (!db || (op->M > 0 && !d)) return fl::fl_fail(FL_ERR_ARG, "linear_bias_grad: null pointer");
-    if (!ws || ws_bytes < fl_linear_bias_grad_bytes(op))
-        return fl::fl_fail(FL_ERR_ARG, "linear_bias_grad: workspace too small");
-    FL_BY_TYPE(op->dtype, fl::bias_grad<T>((hipStream_t)stream, op, d, db, db_f32, (float *)ws))
+    const bool any = op->M > 0 && op->N > 0;
+    if ((any && (!gy || (op->act != FL_ACT_NONE && !pre))) || (any && dx && op->K > 0 && !op->weight) ||
+        (any && dw && op->K > 0 && !op->x))
+        return fl::fl_fail(FL_ERR_ARG, "linear_backward: null pointer");
+    const size_t need = fl_linear_backward_bytes(op, dw != nullptr, db != nullptr);
+    if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "linear_backward: workspace too small");
+    FL_BY_TYPE(op->dtype, fl::backward<T>((hipStream_t)stream, op, gy, pre, dx, dw, db, db_f32, (char *)ws))
 }
 
 }  // extern "C"

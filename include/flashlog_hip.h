@@ -875,21 +875,16 @@ typedef struct fl_linear {
 
 size_t fl_linear_op_bytes(void);
 /* pre [M, N], optional: the activation's argument, for the backward. */
-int fl_linear_forward(void *stream, const fl_linear *op, void *y, void *pre);
-/* d [n] = gy * act'(pre). */
-int fl_linear_act_grad(void *stream, int dtype, int act, const void *gy,
-                       const void *pre, int64_t n, void *d);
-/* dx [M, K] = d W_g. */
-int fl_linear_input_grad(void *stream, const fl_linear *op, const void *d,
-                         void *dx);
-/* dw [groups, N, K] = d^T x over each group's rows (0 for an empty group). */
-size_t fl_linear_weight_grad_bytes(const fl_linear *op);
-int fl_linear_weight_grad(void *stream, const fl_linear *op, const void *d,
-                          void *dw, void *ws, size_t ws_bytes);
-/* db [groups, N] = column sums of d over each group's rows. */
-size_t fl_linear_bias_grad_bytes(const fl_linear *op);
-int fl_linear_bias_grad(void *stream, const fl_linear *op, const void *d,
-                        void *db, int db_f32, void *ws, size_t ws_bytes);
+int fl_linear_forward(void *stream, const fl_linear *op, void *y, float *pre);
+/* With d = gy * act'(pre) (gy [M, N] contiguous; pre unused without an
+ * activation), those of the gradients that are not null: dx [M, K] = d W_g,
+ * dw [groups, N, K] = d^T x and db [groups, N] = the sums of d over each
+ * group's rows (0 for an empty group; db fp32 when db_f32, else of the
+ * operands' type). */
+size_t fl_linear_backward_bytes(const fl_linear *op, int with_dw, int with_db);
+int fl_linear_backward(void *stream, const fl_linear *op, const void *gy,
+                       const float *pre, void *dx, void *dw, void *db,
+                       int db_f32, void *ws, size_t ws_bytes);
 
 /* Constraints on the rows x [rows, cols] (row stride ldx, columns
  * contiguous).  Every `inner` rows in a row share an owner (a query's steps);

@@ -64,13 +64,16 @@ def test_linear_arguments():
     assert "plan" in fwd(_linear_op(groups=2, offsets=1))
     assert "null" in fwd(_linear_op(x=None))
     assert "null" in fwd(_linear_op(), None)
-    assert "null" in _error(lib.fl_linear_input_grad(None, _linear_op(), None, one))
-    assert "null" in _error(lib.fl_linear_weight_grad(None, _linear_op(), None, one, None, 0))
-    assert "workspace" in _error(lib.fl_linear_bias_grad(None, _linear_op(), one, one, 0, None, 0))
+    back = lambda op, gy, pre, dx, dw, db, ws, n: _error(lib.fl_linear_backward(None, op, gy, pre, dx, dw, db, 0, ws, n))
+    assert "null" in back(_linear_op(), None, None, one, None, None, None, 0)
+    assert "null" in back(_linear_op(act=2), one, None, one, None, None, one, 1 << 20)
+    assert "null" in back(_linear_op(weight=None), one, None, one, None, None, None, 0)
+    assert "null" in back(_linear_op(x=None), one, None, None, one, None, None, 0)
+    assert "workspace" in back(_linear_op(), one, None, None, None, one, None, 0)
+    assert "workspace" in back(_linear_op(act=2), one, one, one, None, None, None, 0)
     long = _linear_op(M=100_000)
-    need = lib.fl_linear_weight_grad_bytes(long)
-    assert need > 0 and "workspace" in _error(lib.fl_linear_weight_grad(None, long, one, one, one, need - 1))
-    assert "shape" in _error(lib.fl_linear_act_grad(None, 0, 1, one, one, -1, one))
+    need = lib.fl_linear_backward_bytes(long, 1, 0)
+    assert need > 0 and "workspace" in back(long, one, None, None, one, None, one, need - 1)
     # nothing to do is no error
     assert lib.fl_linear_forward(None, _linear_op(M=0), None, None) == 0
 
