@@ -180,6 +180,8 @@ class _LinearFunction(autograd.Function):
         if need_x or need_w or need_b:
             dev, lib = x.device, _lib.lib()
             (shape, bias_dtype), g = ctx.shapes, grad.contiguous()
+            if g.data_ptr() % 16:
+                g = g.clone()
             op = _linear_op(x, weight, None, None, ctx.plan, ctx.act)
             if need_x:
                 dx = torch.empty(shape, dtype=x.dtype, device=dev)

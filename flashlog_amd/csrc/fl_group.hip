@@ -252,7 +252,7 @@ bool one_launch(int64_t rows, int64_t groups) { return rows <= GR_BLOCK_ROWS && 
 
 extern "C" {
 
-int64_t fl_group_block(int64_t rows, int64_t groups) { return rows >= 64 * groups ? 128 : 32; }
+int64_t fl_group_block(int64_t rows, int64_t groups) { return rows >= 512 * groups ? 128 : rows >= 32 * groups ? 64 : 32; }
 
 int64_t fl_group_tiles(int64_t rows, int64_t groups) {
     if (rows <= 0) return 0;

@@ -27,6 +27,7 @@
 // that such a value enters are NaN.
 #include "fl_abi.h"
 #include "fl_common.h"
+#include <type_traits>
 
 namespace fl {
 namespace {
@@ -117,11 +118,16 @@ __device__ __forceinline__ void chunk_planes<float>(const float (&v)[8], u32x4 (
     }
 }
 
-// LDS element offset of chunk c of row r in a tile of BK values a row: the
-// permutation spreads both 8 and 16 consecutive rows' chunks over the banks.
+// LDS element offset of chunk c of row r in a tile of BK values a row.  A
+// 128-bit LDS read takes 16 lanes a cycle, lanes 0-3, 12-15, 20-23, 24-27 of
+// each half wave together and then the rest, so an MFMA operand read has 8
+// rows at chunk c and 8 others at chunk c ^ 1 in one cycle; the permutation of
+// a row's chunks keeps those 16 in different banks, and 16 consecutive rows at
+// one chunk (the stores of k-strided operands) too.  (Permuted by r ^ (r >> 3)
+// a third of the LDS cycles were conflicts.)
 template <int BK>
 __device__ __forceinline__ int lds_at(int r, int c) {
-    const int f = BK == 32 ? ((r >> 1) ^ (r >> 3)) & 3 : (r ^ (r >> 3)) & 7;
+    const int f = BK == 32 ? (0x78 >> (2 * ((r >> 2) & 3))) & 3 : (r >> 1) & 7;
     return r * BK + ((c ^ f) << 3);
 }
 
@@ -341,13 +347,38 @@ struct Product {
     }
 };
 
+// exp by the hardware's 2^x: off by |x| 2^-24 of itself besides its own step.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+// Phi(p) = erfc(-p / sqrt 2) / 2 by Abramowitz and Stegun 7.1.26 (off by at
+// most 1.5e-7; the factor exp(-p^2/2) keeps the lower tail's own scale).
+__device__ __forceinline__ float normal_cdf(float p) {
+    const float x = fabsf(p) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+    float q = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+    q = __builtin_fmaf(t, q, 1.421413741f);
+    q = __builtin_fmaf(t, q, -0.284496736f);
+    q = __builtin_fmaf(t, q, 0.254829592f);
+    const float tail = 0.5f * t * q * fast_exp(-x * x);
+    return p < 0.0f ? tail : 1.0f - tail;
+}
+
+// The activations of the epilogue, in a few instructions each: with the
+// library's erff the epilogue of a 128 x 128 tile took a third of a product
+// over 2048 inputs (9000 vector instructions a wave).
 __device__ __forceinline__ float act_value(float p, int act) {
     switch (act) {
         case FL_ACT_RELU: return p > 0.0f ? p : (p != p ? p : 0.0f);
-        case FL_ACT_GELU: return 0.5f * p * (1.0f + erff(p * 0.70710678118654752f));
-        case FL_ACT_SILU: return p / (1.0f + expf(-p));
-        case FL_ACT_TANH: return tanhf(p);
-        case FL_ACT_SIGMOID: return 1.0f / (1.0f + expf(-p));
+        case FL_ACT_GELU: return p * normal_cdf(p);
+        case FL_ACT_SILU: return p * __builtin_amdgcn_rcpf(1.0f + fast_exp(-p));
+        case FL_ACT_TANH: {
+            // near 0 the odd series, off by 4e-7 of itself at 1/4
+            const float s = p * p;
+            const float near = p + p * s * (-0.33333333f + s * (0.13333333f + s * -0.053968254f));
+            const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + fast_exp(2.0f * p));
+            return s < 0.0625f ? near : far;
+        }
+        case FL_ACT_SIGMOID: return __builtin_amdgcn_rcpf(1.0f + fast_exp(-p));
         default: return p;
     }
 }
@@ -384,59 +415,53 @@ struct RowsArgs {
     const void *bias, *residual;
     int64_t bias_group, ldres;
     float *pre;
-    int act, bias_f32;
+    int act, bias_f32, block;
 };
 
-// Products whose C rows are the batch's rows (the forward, and dx): a tile is
-// BM rows of one group.
-template <typename T, bool B_CONTIG, int BM, int BN, int BK>
-__global__ __launch_bounds__(LN_NT) void k_lin_rows(RowsArgs a) {
-    using Prod = Product<T, BM, BN, BK>;
-    __shared__ __align__(16) uint16_t lds[Prod::LDS_ELEMS];
-    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
-    const int64_t mt = w / a.n_tiles, nt = w % a.n_tiles;
-    int64_t g = 0, pos0 = mt * BM, end = a.M;
-    if (a.tiles) {
-        g = a.tiles[2 * mt];
-        if (g < 0) return;
-        pos0 = a.tiles[2 * mt + 1];
-        end = g < a.groups ? (int64_t)a.offsets[g + 1] : a.M;
+// A tile of a product: its group (`none`: the rows of no group) and the places
+// pos0 .. end of its rows.
+struct RowTile {
+    int64_t g, pos0, end;
+    bool none;
+};
+
+// The BM rows of tile mt; the plan's tiles are `block` rows.
+template <int BM>
+__device__ __forceinline__ bool row_tile(const RowsArgs &a, uint32_t mt, RowTile *t) {
+    if (!a.tiles) {
+        *t = RowTile{0, (int64_t)mt * BM, a.M, false};
+        return true;
     }
-    const bool none = g >= a.groups;  // rows of no group
-    const int64_t n0 = nt * BN;
-    const T *A = (const T *)a.a;
-    const T *B = (const T *)a.b + (none ? 0 : g * a.b_group);
-    ContigTile<T, BM, BK> ta;
-    ta.init(
-        [&](int r) {
-            int64_t p = pos0 + r < end ? pos0 + r : end - 1;
-            return A + (a.order ? (int64_t)a.order[p] : p) * a.lda;
-        });
-    Prod prod;
-    const int64_t K = none ? 0 : a.K;
-    if constexpr (B_CONTIG) {
-        ContigTile<T, BN, BK> tb;
-        tb.init([&](int r) { return B + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldb; });
-        prod.run(ta, tb, K, lds);
-    } else {
-        StridedTile<T, BN, BK> tb;
-        tb.init(B + n0, a.ldb, a.N - n0, nullptr);
-        prod.run(ta, tb, K, lds);
-    }
+    const uint32_t sub = a.block / BM;
+    const int32_t *e = a.tiles + 2 * (int64_t)(mt / sub);
+    const int64_t g = e[0];
+    if (g < 0) return false;
+    const int64_t end = g < a.groups ? (int64_t)a.offsets[g + 1] : a.M;
+    *t = RowTile{g, e[1] + (int64_t)(mt % sub) * BM, end, g >= a.groups};
+    return t->pos0 < end;
+}
+
+// Stores a wave's tiles, whose first row is at place `pos` and first column
+// `col`: bias, activation, residual, one rounding.
+template <typename T, int MT, int NTL>
+__device__ __forceinline__ void store_rows(const RowsArgs &a, const f32x4 (&acc)[MT][NTL], const RowTile &t,
+                                           int64_t pos, int64_t col) {
+    const int64_t g = t.g, end = t.end;
+    const bool none = t.none;
     const int lane = fl_lane();
 #pragma unroll
-    for (int i = 0; i < Prod::MT; ++i) {
-        const int64_t p = pos0 + prod.wave_m() + i * 16 + (lane & 15);
+    for (int i = 0; i < MT; ++i) {
+        const int64_t p = pos + i * 16 + (lane & 15);
         if (p >= end) continue;
         const int64_t row = a.order ? (int64_t)a.order[p] : p;
 #pragma unroll
-        for (int j = 0; j < Prod::NTL; ++j) {
-            const int64_t n = n0 + prod.wave_n() + j * 16 + (lane >> 4) * 4;
+        for (int j = 0; j < NTL; ++j) {
+            const int64_t n = col + j * 16 + (lane >> 4) * 4;
             if (n >= a.N) continue;
             const int m = a.N - n < 4 ? (int)(a.N - n) : 4;
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = prod.acc[i][j][e];
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
             if (a.bias && !none) {
                 const int64_t at = g * a.bias_group + n;
 #pragma unroll
@@ -475,6 +500,37 @@ __global__ __launch_bounds__(LN_NT) void k_lin_rows(RowsArgs a) {
     }
 }
 
+// Products whose C rows are the batch's rows (the forward, and dx): a tile is
+// BM rows of one group.
+template <typename T, bool B_CONTIG, int BM, int BN, int BK>
+__global__ __launch_bounds__(LN_NT) void k_lin_rows(RowsArgs a) {
+    using Prod = Product<T, BM, BN, BK>;
+    __shared__ __align__(16) uint16_t lds[Prod::LDS_ELEMS];
+    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    RowTile t;
+    if (!row_tile<BM>(a, w / a.n_tiles, &t)) return;
+    const int64_t n0 = (int64_t)(w % a.n_tiles) * BN;
+    const T *A = (const T *)a.a;
+    const T *B = (const T *)a.b + (t.none ? 0 : t.g * a.b_group);
+    ContigTile<T, BM, BK> ta;
+    ta.init([&](int r) {
+        const int64_t p = t.pos0 + r < t.end ? t.pos0 + r : t.end - 1;
+        return A + (a.order ? (int64_t)a.order[p] : p) * a.lda;
+    });
+    Prod prod;
+    const int64_t K = t.none ? 0 : a.K;
+    if constexpr (B_CONTIG) {
+        ContigTile<T, BN, BK> tb;
+        tb.init([&](int r) { return B + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldb; });
+        prod.run(ta, tb, K, lds);
+    } else {
+        StridedTile<T, BN, BK> tb;
+        tb.init(B + n0, a.ldb, a.N - n0, nullptr);
+        prod.run(ta, tb, K, lds);
+    }
+    store_rows<T>(a, prod.acc, t, t.pos0 + prod.wave_m(), n0 + prod.wave_n());
+}
+
 struct OuterArgs {
     const void *d, *x;
     int64_t ldd, ldx;
@@ -493,6 +549,38 @@ __device__ __forceinline__ void part_range(const int32_t *offsets, int64_t M, in
     const int64_t n = (offsets ? (int64_t)offsets[g + 1] : M) - b;
     *begin = b + n * p / parts;
     *end = b + n * (p + 1) / parts;
+}
+
+// Stores a wave's tiles of dW_g, or of a part of its sum.
+template <typename T, int MT, int NTL>
+__device__ __forceinline__ void store_outer(const OuterArgs &a, const f32x4 (&acc)[MT][NTL], int64_t g, int part,
+                                            int64_t row, int64_t col) {
+    const int lane = fl_lane();
+    const int64_t NK = a.N * a.K;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t m = row + i * 16 + (lane & 15);
+        if (m >= a.N) continue;
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) {
+            const int64_t c = col + j * 16 + (lane >> 4) * 4;
+            if (c >= a.K) continue;
+            const int n = a.K - c < 4 ? (int)(a.K - c) : 4;
+            if (a.part) {
+                float *q = a.part + ((int64_t)part * a.groups + g) * NK + m * a.K + c;
+                const Vec<float, 4> f{{acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]}};
+                if (n == 4) store_vec<float, 4>(q, f);
+                else store_some<float, 4>(q, f, n);
+            } else {
+                T *q = (T *)a.dw + g * NK + m * a.K + c;
+                Vec<T, 4> o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o.v[e] = (T)acc[i][j][e];
+                if (n == 4) store_vec<T, 4>(q, o);
+                else store_some<T, 4>(q, o, n);
+            }
+        }
+    }
 }
 
 // dW_g = sum over the group's rows (a part of them) of d^T x.
@@ -522,32 +610,256 @@ __global__ __launch_bounds__(LN_NT) void k_lin_outer(OuterArgs a) {
     tb.init(X, a.ldx, a.K - c0, ord);
     Prod prod;
     prod.run(ta, tb, len, lds);
-    const int lane = fl_lane();
-    const int64_t NK = a.N * a.K;
+    store_outer<T>(a, prod.acc, g, part, m0 + prod.wave_m(), c0 + prod.wave_n());
+}
+
+// The same products for large 16-bit operands at the matrix unit's pace.  512
+// threads take BM x 256 outputs, 8 waves of BM/2 x 64; BK = 64 values of k
+// per step.  Operands go from memory to LDS without registers
+// (global_load_lds, 16 bytes a lane), into one of STAGES buffers while another
+// is multiplied: one barrier a step, and the loads have STAGES - 1 steps to
+// arrive.  A wave's load fills 1 KB of LDS in lane order, so the permutation
+// of the chunks that spreads the later reads over the banks is made on the
+// memory side: a lane loads the chunk that belongs to its place.
+// k-strided operands lie in LDS as they do in memory, rows of k, and are read
+// transposed (ds_read_b64_tr_b16: of 16 lanes, lane s gives the address of
+// row s/4, columns 4 (s%4)..+3, and lane i receives column i of the 4 rows).
+// Needs 16-byte aligned rows of whole 8-value chunks.  With 256 x 256 tiles
+// the LDS reads of a step take 1536 cycles a CU and its multiplications 2048.
+constexpr int WD_NT = 512;
+constexpr int WD_WAVES = WD_NT / FL_WAVE;
+constexpr int WD_BN = 256;
+constexpr int WD_BK = 64;
+
+// What lanes outside an operand load.
+__device__ __align__(16) const uint32_t wd_zeros[4] = {0, 0, 0, 0};
+
+typedef __attribute__((address_space(3))) void lds_ptr;
+typedef __attribute__((address_space(1))) const void mem_ptr;
+
+__device__ __forceinline__ void load_lds(const void *p, uint16_t *lds) {
+    __builtin_amdgcn_global_load_lds((mem_ptr *)p, (lds_ptr *)lds, 16, 0, 0);
+}
+
+template <int BR>
+struct WideContig {
+    static constexpr int LOADS = BR / 8 / WD_WAVES;  // 8 rows of 64 values a load
+    static constexpr int ELEMS = BR * WD_BK;
+    const uint16_t *p[LOADS];
+
+    // The row and the chunk that this lane loads i-th.
+    static __device__ __forceinline__ int row(int i) { return (fl_wave_id() * LOADS + i) * 8 + (fl_lane() >> 3); }
+    static __device__ __forceinline__ int chunk(int i) { return (fl_lane() & 7) ^ ((row(i) >> 1) & 7); }
+
+    template <typename F>
+    __device__ __forceinline__ void init(F &&row_ptr) {
 #pragma unroll
-    for (int i = 0; i < Prod::MT; ++i) {
-        const int64_t m = m0 + prod.wave_m() + i * 16 + (lane & 15);
-        if (m >= a.N) continue;
+        for (int i = 0; i < LOADS; ++i) p[i] = row_ptr(row(i)) + chunk(i) * 8;
+    }
+    // The next `count` <= 64 values of k.
+    __device__ __forceinline__ void issue(uint16_t *lds, int count) {
 #pragma unroll
-        for (int j = 0; j < Prod::NTL; ++j) {
-            const int64_t c = c0 + prod.wave_n() + j * 16 + (lane >> 4) * 4;
-            if (c >= a.K) continue;
-            const int n = a.K - c < 4 ? (int)(a.K - c) : 4;
-            if (a.part) {
-                float *q = a.part + ((int64_t)part * a.groups + g) * NK + m * a.K + c;
-                #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < n) q[e] = prod.acc[i][j][e];
-            } else {
-                T *q = (T *)a.dw + g * NK + m * a.K + c;
-                Vec<T, 4> o;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o.v[e] = (T)prod.acc[i][j][e];
-                if (n == 4) store_vec<T, 4>(q, o);
-                else store_some<T, 4>(q, o, n);
-            }
+        for (int i = 0; i < LOADS; ++i) {
+            const void *q = chunk(i) * 8 < count ? (const void *)p[i] : (const void *)wd_zeros;
+            load_lds(q, lds + (fl_wave_id() * LOADS + i) * 512);
+            p[i] += count;
         }
     }
+    __device__ __forceinline__ u32x4 frag(const uint16_t *lds, int row0, int ks) const {
+        const int r = row0 + (fl_lane() & 15), q = fl_lane() >> 4;
+        return *reinterpret_cast<const u32x4 *>(lds + r * WD_BK + (((ks * 4 + q) ^ ((r >> 1) & 7)) << 3));
+    }
+};
+
+template <int BR>
+struct WideStrided {
+    static constexpr int CH = BR / 8;                // chunks a row of k
+    static constexpr int RPL = FL_WAVE / CH;         // rows of k a load
+    static constexpr int LOADS = WD_BK / RPL / WD_WAVES;
+    static constexpr int ELEMS = BR * WD_BK;
+    const uint16_t *col[LOADS];
+    const int32_t *order;
+    int32_t next[LOADS];
+    int64_t ld, place;
+
+    // The permutation of a row's chunks, in steps of the two chunks that a
+    // transposed read takes of each of 4 rows.
+    static __device__ __forceinline__ int turn(int k) { return 2 * ((k & 3) | ((((k >> 3) ^ (k >> 4)) & 1) << 2)); }
+    __device__ __forceinline__ int row(int i) const { return (fl_wave_id() * LOADS + i) * RPL + fl_lane() / CH; }
+
+    __device__ __forceinline__ void init(const uint16_t *base, int64_t stride, int64_t R, const int32_t *ord,
+                                         int first) {
+        ld = stride;
+        order = ord;
+        place = 0;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int64_t c = ((fl_lane() % CH) ^ turn(row(i))) * 8;
+            col[i] = base + (c <= R - 8 ? c : R - 8);
+        }
+        look(first);
+    }
+    // The rows of the step that begins at `place`, of `count` rows.
+    __device__ __forceinline__ void look(int count) {
+        if (order)
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) next[i] = row(i) < count ? order[place + row(i)] : 0;
+    }
+    __device__ __forceinline__ void issue(uint16_t *lds, int count, int after) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int64_t r = order ? (int64_t)next[i] : place + row(i);
+            const void *q = row(i) < count ? (const void *)(col[i] + r * ld) : (const void *)wd_zeros;
+            load_lds(q, lds + (fl_wave_id() * LOADS + i) * 512);
+        }
+        place += count;
+        look(after);
+    }
+    __device__ __forceinline__ u32x4 frag(const uint16_t *lds, int col0, int ks) const {
+        const int s = fl_lane() & 15, q = fl_lane() >> 4;
+        u32x4 out;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = ks * 32 + q * 8 + h * 4 + (s >> 2);
+            const int c = (col0 >> 3) + ((s & 3) >> 1);
+            const uint16_t *a = lds + k * BR + ((c ^ turn(k)) << 3) + (s & 1) * 4;
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4 *)const_cast<uint16_t *>(a));
+            const uint64_t u = __builtin_bit_cast(uint64_t, v);
+            out[2 * h] = (uint32_t)u;
+            out[2 * h + 1] = (uint32_t)(u >> 32);
+        }
+        return out;
+    }
+};
+
+template <typename T, int BM, int STAGES, typename TA, typename TB>
+struct WideProduct {
+    static constexpr int MT = BM / 2 / 16, NTL = 4;
+    static constexpr int ELEMS = TA::ELEMS + TB::ELEMS;
+    static constexpr int LOADS = TA::LOADS + TB::LOADS;
+    f32x4 acc[MT][NTL];
+
+    static __device__ __forceinline__ int wave_m() { return (fl_wave_id() >> 2) * (BM / 2); }
+    static __device__ __forceinline__ int wave_n() { return (fl_wave_id() & 3) * 64; }
+
+    // count(i): values of step i; feed(lds_a, lds_b, i) issues its loads.
+    template <typename F>
+    __device__ __forceinline__ void run(const TA &ta, const TB &tb, int64_t steps, uint16_t *lds, F &&feed) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+        if (steps <= 0) return;
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s)
+            if (s < steps) feed(lds + s * ELEMS, lds + s * ELEMS + TA::ELEMS, s);
+        int at = 0;
+        for (int64_t s = 0; s < steps; ++s) {
+            // this step's loads have landed when at most those of the later steps are under way
+            if (STAGES == 2 || s + 1 >= steps) __builtin_amdgcn_s_waitcnt(0x0f70);
+            else __builtin_amdgcn_s_waitcnt(wait_imm());
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            if (s + STAGES - 1 < steps) {
+                const int to = at + STAGES - 1 >= STAGES ? at - 1 : at + STAGES - 1;
+                feed(lds + to * ELEMS, lds + to * ELEMS + TA::ELEMS, s + STAGES - 1);
+            }
+            const uint16_t *la = lds + at * ELEMS, *lb = la + TA::ELEMS;
+#pragma unroll
+            for (int ks = 0; ks < WD_BK / 32; ++ks) {
+                u32x4 b[NTL];
+#pragma unroll
+                for (int j = 0; j < NTL; ++j) b[j] = tb.frag(lb, wave_n() + j * 16, ks);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const u32x4 f = ta.frag(la, wave_m() + i * 16, ks);
+#pragma unroll
+                    for (int j = 0; j < NTL; ++j) acc[i][j] = mfma<T>(b[j], f, acc[i][j]);
+                }
+            }
+            at = at + 1 == STAGES ? 0 : at + 1;
+        }
+    }
+    // s_waitcnt vmcnt(LOADS (STAGES - 2)), nothing else (vmcnt: bits 0-3 and 14-15)
+    static constexpr int wait_imm() {
+        constexpr int n = LOADS * (STAGES - 2);
+        return (n & 15) | ((n >> 4) << 14) | 0x0f70;
+    }
+};
+
+// The forward (B_CONTIG) and dx.
+template <typename T, bool B_CONTIG, int BM, int STAGES>
+__global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
+    using TA = WideContig<BM>;
+    using TB = std::conditional_t<B_CONTIG, WideContig<WD_BN>, WideStrided<WD_BN>>;
+    using Prod = WideProduct<T, BM, STAGES, TA, TB>;
+    extern __shared__ __align__(16) uint16_t wide_lds[];
+    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    RowTile t;
+    if (!row_tile<BM>(a, w / a.n_tiles, &t)) return;
+    const int64_t n0 = (int64_t)(w % a.n_tiles) * WD_BN;
+    const uint16_t *A = (const uint16_t *)a.a;
+    const uint16_t *B = (const uint16_t *)a.b + (t.none ? 0 : t.g * a.b_group);
+    const int64_t steps = t.none ? 0 : (a.K + WD_BK - 1) / WD_BK;
+    const int first = (int)(a.K - (steps - 1) * WD_BK);  // the step that is no whole one comes first
+    TA ta;
+    TB tb;
+    ta.init([&](int r) {
+        const int64_t p = t.pos0 + r < t.end ? t.pos0 + r : t.end - 1;
+        return A + (a.order ? (int64_t)a.order[p] : p) * a.lda;
+    });
+    if constexpr (B_CONTIG) tb.init([&](int r) { return B + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldb; });
+    else tb.init(B + n0, a.ldb, a.N - n0, nullptr, first);
+    Prod prod;
+    prod.run(ta, tb, steps, wide_lds, [&](uint16_t *la, uint16_t *lb, int64_t s) {
+        const int count = s ? WD_BK : first;
+        ta.issue(la, count);
+        if constexpr (B_CONTIG) tb.issue(lb, count);
+        else tb.issue(lb, count, WD_BK);
+    });
+    store_rows<T>(a, prod.acc, t, t.pos0 + prod.wave_m(), n0 + prod.wave_n());
+}
+
+// dW.
+template <typename T, int BM, int STAGES>
+__global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
+    using TA = WideStrided<BM>;
+    using TB = WideStrided<WD_BN>;
+    using Prod = WideProduct<T, BM, STAGES, TA, TB>;
+    extern __shared__ __align__(16) uint16_t wide_lds[];
+    uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    const int64_t nt = w % a.n_tiles;
+    w /= a.n_tiles;
+    const int64_t kt = w % a.k_tiles;
+    w /= a.k_tiles;
+    const int part = (int)(w % a.parts);
+    const int64_t g = w / a.parts;
+    int64_t begin, end;
+    part_range(a.offsets, a.M, g, (int)a.parts, part, &begin, &end);
+    const int64_t m0 = nt * BM, c0 = kt * WD_BN, len = end - begin;
+    const uint16_t *D = (const uint16_t *)a.d + m0, *X = (const uint16_t *)a.x + c0;
+    const int32_t *ord = a.order ? a.order + begin : nullptr;
+    if (!ord) {
+        D += begin * a.ldd;
+        X += begin * a.ldx;
+    }
+    const int64_t steps = (len + WD_BK - 1) / WD_BK;
+    const int first = (int)(len - (steps - 1) * WD_BK);
+    TA ta;
+    TB tb;
+    const int look = len > 0 ? first : 0;
+    ta.init(D, a.ldd, a.N - m0, ord, look);
+    tb.init(X, a.ldx, a.K - c0, ord, look);
+    Prod prod;
+    prod.run(ta, tb, steps, wide_lds, [&](uint16_t *la, uint16_t *lb, int64_t s) {
+        const int count = s ? WD_BK : first, after = s + 1 < steps ? WD_BK : 0;
+        ta.issue(la, count, after);
+        tb.issue(lb, count, after);
+    });
+    store_outer<T>(a, prod.acc, g, part, m0 + prod.wave_m(), c0 + prod.wave_n());
 }
 
 // d = gy * act'(p), rounded to the operands' type: it is an operand of two products.
@@ -612,38 +924,58 @@ void part_sums(hipStream_t st, const float *part, int parts, int64_t n, void *ou
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Rows of a tile: the plan's, or for one group 128 where that gives the chip
-// enough workgroups.
+// Rows of a tile: the plan's, or for one group the largest tile that gives
+// every CU one and a half workgroups, down to 32.
 int tile_rows(const fl_linear *op, int64_t cols) {
     if (op->offsets) return (int)fl_group_block(op->M, op->groups);
-    return ceil_div(op->M, 128) * ceil_div(cols, 128) >= 128 ? 128 : 32;
+    if (ceil_div(op->M, 128) * ceil_div(cols, 128) >= 384) return 128;
+    return ceil_div(op->M, 64) * ceil_div(cols, 64) >= 128 ? 64 : 32;
+}
+
+bool aligned(const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+
+// Rows of the wide kernels' tiles, 0: the operands or the sizes are not for them.
+int wide_rows(const fl_linear *op, const RowsArgs &a, bool b_contig) {
+    if (op->dtype == FL_F32 || !aligned(a.a, a.lda) || !aligned(a.b, a.ldb) || a.b_group % 8 || a.K % 8 || a.K < 64 ||
+        (!b_contig && a.N % 8) || a.N < 192)
+        return 0;
+    const int64_t cols = ceil_div(a.N, WD_BN);
+    if (op->offsets) return fl_group_block(op->M, op->groups) == 128 && ceil_div(op->M, 128) * cols >= 128 ? 128 : 0;
+    if (ceil_div(op->M, 256) * cols >= 192) return 256;
+    return ceil_div(op->M, 128) * cols >= 128 ? 128 : 0;
 }
 
 template <typename T, bool B_CONTIG>
 int launch_rows(hipStream_t st, const fl_linear *op, RowsArgs &a, const char *what) {
-    const int bm = tile_rows(op, a.N);
+    a.block = (int)fl_group_block(op->M, op->groups);
+    const int wide = sizeof(T) == 2 ? wide_rows(op, a, B_CONTIG) : 0;
+    const int bm = wide ? wide : tile_rows(op, a.N);
     constexpr int BIG_K = sizeof(T) == 4 ? 32 : 64;
-    const int bn = bm == 128 && a.N > 64 ? 128 : 64;
-    const int64_t m_tiles = op->offsets ? fl_group_tiles(op->M, op->groups) : ceil_div(op->M, bm);
+    const int bn = wide ? WD_BN : bm == 128 && a.N > 64 ? 128 : 64;
+    const int64_t m_tiles = op->offsets ? fl_group_tiles(op->M, op->groups) * (a.block / bm) : ceil_div(op->M, bm);
     a.n_tiles = (uint32_t)ceil_div(a.N, bn);
     const int64_t grid = m_tiles * a.n_tiles;
     if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "%s: too many tiles for one launch (shape)", what);
     if (grid == 0) return FL_OK;
-    if (bn == 128)
-        FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 128, 128, BIG_K>), dim3((unsigned)grid), dim3(LN_NT), 0, st,
-                  a);
-    else if (bm == 128)
-        FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 128, 64, BIG_K>), dim3((unsigned)grid), dim3(LN_NT), 0, st,
-                  a);
-    else
-        FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 32, 64, 64>), dim3((unsigned)grid), dim3(LN_NT), 0, st, a);
+    const dim3 g((unsigned)grid), nt(LN_NT);
+    if constexpr (sizeof(T) == 2) {
+        if (wide == 256)
+            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 256, 2>), g, dim3(WD_NT), 2 * 512 * WD_BK * 2, st, a);
+        else if (wide)
+            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 128, 3>), g, dim3(WD_NT), 3 * 384 * WD_BK * 2, st, a);
+        if (wide) return fl_check_launch(what);
+    }
+    if (bn == 128) FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 128, 128, BIG_K>), g, nt, 0, st, a);
+    else if (bm == 128) FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 128, 64, BIG_K>), g, nt, 0, st, a);
+    else if (bm == 64) FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 64, 64, BIG_K>), g, nt, 0, st, a);
+    else FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 32, 64, 64>), g, nt, 0, st, a);
     return fl_check_launch(what);
 }
 
 // Parts of a group's rows in dW and db: enough workgroups for the chip where
 // the tiles alone are few, of at least 256 rows on average.
-int outer_parts(int64_t M, int64_t groups, int64_t tiles) {
-    int64_t want = ceil_div(512, tiles * groups), most = M / (256 * groups);
+int outer_parts(int64_t M, int64_t groups, int64_t tiles, int64_t workgroups) {
+    int64_t want = workgroups / (tiles * groups), most = M / (256 * groups);
     int64_t p = want < most ? want : most;
     return (int)(p < 1 ? 1 : p > 64 ? 64 : p);
 }
@@ -654,11 +986,34 @@ int sum_parts(int64_t M, int64_t N, int64_t groups) {
     return (int)(p < 1 ? 1 : p > 256 ? 256 : p);
 }
 
-int outer_tile(const fl_linear *op) { return op->N >= 128 && op->K >= 128 ? 128 : 64; }
+// Tiles of dW: N and K extents, and the parts of the rows.  Wide ones where
+// the operands allow it and a part keeps 256 rows; 64 x 64 where 128 x 128
+// would leave CUs idle.
+struct OuterPlan {
+    int tn, tk, parts;
+    bool wide;
+    int64_t tiles;
+};
 
-int64_t outer_tiles(const fl_linear *op) {
-    const int t = outer_tile(op);
-    return ceil_div(op->N, t) * ceil_div(op->K, t);
+OuterPlan outer_plan(const fl_linear *op) {
+    OuterPlan p{};
+    const auto fill = [&](int tn, int tk) {
+        p.tn = tn;
+        p.tk = tk;
+        p.tiles = ceil_div(op->N, tn) * ceil_div(op->K, tk);
+    };
+    // d is contiguous [M, N], on a 256-byte boundary of the workspace or the caller's gradient
+    if (op->dtype != FL_F32 && op->N % 8 == 0 && aligned(op->x, op->ldx) && op->K % 8 == 0 && op->N >= 192 &&
+        op->K >= 192) {
+        fill(256, 256);
+        p.parts = outer_parts(op->M, op->groups, p.tiles, 256);
+        p.wide = p.tiles * op->groups * p.parts >= 128;
+        if (p.wide) return p;
+    }
+    fill(128, 128);
+    if (op->N < 128 || op->K < 128 || p.tiles * op->groups < 384) fill(64, 64);
+    p.parts = outer_parts(op->M, op->groups, p.tiles < 1 ? 1 : p.tiles, 1024);
+    return p;
 }
 
 int check_op(const fl_linear *op, const char *what) {
@@ -724,7 +1079,8 @@ int input_grad(hipStream_t st, const fl_linear *op, const void *d, void *dx) {
 template <typename T>
 int weight_grad(hipStream_t st, const fl_linear *op, const void *d, void *dw, float *ws) {
     OuterArgs a{};
-    const int t = outer_tile(op);
+    OuterPlan p = outer_plan(op);
+    if (p.wide && (uintptr_t)d % 16) return fl_fail(FL_ERR_ARG, "linear_backward: gy must be 16-byte aligned");
     a.d = d;
     a.x = op->x;
     a.ldd = op->N;
@@ -733,23 +1089,27 @@ int weight_grad(hipStream_t st, const fl_linear *op, const void *d, void *dw, fl
     a.N = op->N;
     a.K = op->K;
     a.groups = op->groups;
-    a.n_tiles = (uint32_t)ceil_div(op->N, t);
-    a.k_tiles = (uint32_t)ceil_div(op->K, t);
-    a.parts = (uint32_t)outer_parts(op->M, op->groups, outer_tiles(op));
+    a.n_tiles = (uint32_t)ceil_div(op->N, p.tn);
+    a.k_tiles = (uint32_t)ceil_div(op->K, p.tk);
+    a.parts = (uint32_t)p.parts;
     a.order = op->order;
     a.offsets = op->offsets;
     a.dw = dw;
     a.part = a.parts > 1 ? ws : nullptr;
-    const int64_t grid = outer_tiles(op) * a.parts * a.groups;
-    if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "linear_weight_grad: too many tiles for one launch (shape)");
+    const int64_t grid = p.tiles * a.parts * a.groups;
+    if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "linear_backward: too many tiles for one launch (shape)");
     if (grid == 0) return FL_OK;
     constexpr int BIG_K = sizeof(T) == 4 ? 32 : 64;
-    if (t == 128)
-        FL_LAUNCH("k_lin_outer", (k_lin_outer<T, 128, 128, BIG_K>), dim3((unsigned)grid), dim3(LN_NT), 0, st, a);
-    else
-        FL_LAUNCH("k_lin_outer", (k_lin_outer<T, 64, 64, 64>), dim3((unsigned)grid), dim3(LN_NT), 0, st, a);
+    const dim3 g((unsigned)grid), nt(LN_NT);
+    if constexpr (sizeof(T) == 2) {
+        if (p.wide)
+            FL_LAUNCH("k_wide_outer", (k_wide_outer<T, 256, 2>), g, dim3(WD_NT), 2 * 512 * WD_BK * 2, st, a);
+    }
+    if (p.wide) {
+    } else if (p.tn == 128) FL_LAUNCH("k_lin_outer", (k_lin_outer<T, 128, 128, BIG_K>), g, nt, 0, st, a);
+    else FL_LAUNCH("k_lin_outer", (k_lin_outer<T, 64, 64, BIG_K>), g, nt, 0, st, a);
     if (a.part) part_sums<T>(st, ws, (int)a.parts, a.groups * a.N * a.K, dw);
-    return fl_check_launch("linear_weight_grad");
+    return fl_check_launch("linear_backward");
 }
 
 template <typename T>
@@ -787,9 +1147,8 @@ BackwardSpace backward_space(const fl_linear *op, int with_dw, int with_db) {
         return at;
     };
     if (op->act != FL_ACT_NONE) s.d = take((size_t)op->M * op->N * (op->dtype == FL_F32 ? 4 : 2));
-    const int64_t tiles = outer_tiles(op);
-    if (with_dw && tiles) {
-        const int parts = outer_parts(op->M, op->groups, tiles);
+    if (with_dw && op->N && op->K) {
+        const int parts = outer_plan(op).parts;
         s.dw = take(parts > 1 ? (size_t)parts * op->groups * op->N * op->K * 4 : 0);
     }
     if (with_db && op->N) s.db = take((size_t)sum_parts(op->M, op->N, op->groups) * op->groups * op->N * 4);
@@ -850,6 +1209,7 @@ int fl_linear_backward(void *stream, const fl_linear *op, const void *gy, const 
         return fl::fl_fail(FL_ERR_ARG, "linear_backward: null pointer");
     const size_t need = fl_linear_backward_bytes(op, dw != nullptr, db != nullptr);
     if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "linear_backward: workspace too small");
+    if ((uintptr_t)ws % 16) return fl::fl_fail(FL_ERR_ARG, "linear_backward: workspace must be 16-byte aligned");
     FL_BY_TYPE(op->dtype, fl::backward<T>((hipStream_t)stream, op, gy, pre, dx, dw, db, db_f32, (char *)ws))
 }
 

@@ -880,7 +880,7 @@ int fl_linear_forward(void *stream, const fl_linear *op, void *y, float *pre);
  * activation), those of the gradients that are not null: dx [M, K] = d W_g,
  * dw [groups, N, K] = d^T x and db [groups, N] = the sums of d over each
  * group's rows (0 for an empty group; db fp32 when db_f32, else of the
- * operands' type). */
+ * operands' type).  gy and ws lie on 16-byte boundaries. */
 size_t fl_linear_backward_bytes(const fl_linear *op, int with_dw, int with_db);
 int fl_linear_backward(void *stream, const fl_linear *op, const void *gy,
                        const float *pre, void *dx, void *dw, void *db,

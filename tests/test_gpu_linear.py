@@ -166,6 +166,37 @@ def test_linear_large_tiles(shape, t):
     _check(*_make(M, K, N, t, 5), act="silu")
 
 
+@pytest.mark.parametrize("t", TYPES[1:])
+@pytest.mark.parametrize("shape", [(6100, 72, 2048), (6100, 2048, 72), (2000, 136, 2041), (2000, 2048, 264),
+                                   (32800, 256, 200)])
+def test_linear_half_precision_tiles(shape, t):
+    """Shapes and alignments of the wide tiles: the forward, dx and dW of each, ends of K and of the columns."""
+    M, K, N = shape
+    _check(*_make(M, K, N, t, 15), act="relu")
+
+
+@pytest.mark.parametrize("t", TYPES[1:])
+@pytest.mark.parametrize("K,N", [(200, 1024), (264, 520)])
+def test_relation_linear_half_precision_tiles(K, N, t):
+    g = torch.Generator().manual_seed(1)
+    index = torch.randint(-1, 4, (8200,), generator=g)
+    index[2000:5000] = 3
+    _check(*_make(8200, K, N, t, 16, groups=4), act="tanh", index=index)
+
+
+def test_misaligned_gradient():
+    """A contiguous gradient that begins inside a tensor, off the 16-byte boundaries."""
+    fa = _fa()
+    x, w, b, r, gy = _make(33000, 256, 200, torch.bfloat16, 17)
+    flat = torch.zeros(33000 * 200 + 3, dtype=torch.bfloat16, device="cuda")
+    flat[3:] = gy.cuda().view(-1)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    y = fa.linear(*leaves)
+    for p, q in zip(torch.autograd.grad(y, leaves, flat[3:].view(33000, 200), retain_graph=True),
+                    torch.autograd.grad(y, leaves, gy.cuda())):
+        assert torch.equal(p, q)
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("rows,groups,K,N", [(1, 3, 8, 4), (96, 474, 32, 25), (50, 7, 100, 33), (700, 5, 130, 140),
                                              (513, 4, 129, 257)])
