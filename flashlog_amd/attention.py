@@ -26,7 +26,6 @@ anything between calls, so they can be captured into a graph.  A captured
 backward needs leaves whose gradient graph was not begun outside the capture,
 as everywhere in torch.
 """
-import contextlib
 import math
 
 import torch
@@ -34,19 +33,38 @@ from torch import autograd
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import FlLinear, FlLogits, check, ptr, stream_handle
+from ._lib import FlLinear, FlLogits, check
 
 __all__ = ["RowGroups", "group_rows", "linear", "relation_linear", "pack_allowed", "history_from_pairs",
            "constrain_logits", "hop_attention"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3, "tanh": 4, "sigmoid": 5}
-_HERE = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without a Stream object
+_LIB = None
 
 
-def _on(dev):
-    """The device that a call's tensors are on, as the current one."""
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _lib_handle():
+    global _LIB
+    if _LIB is None:
+        _LIB = _lib.lib()
+    return _LIB
+
+
+def _launch(what, fn, dev, *args):
+    """Calls an entry point on the device's current stream, with the device current."""
+    i = dev.index
+    if i == torch.cuda.current_device():
+        rc = fn(_raw_stream(i), *args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(_raw_stream(i), *args)
+    if rc:
+        check(rc, what)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _need_gpu(what, *tensors):
@@ -87,10 +105,24 @@ class RowGroups:
     [groups + 1], where each group begins.  Rows whose id was outside
     [0, groups) come behind ``offsets[groups]``."""
 
-    __slots__ = ("rows", "groups", "order", "offsets", "tiles")
+    __slots__ = ("rows", "groups", "_plan", "_at")
 
-    def __init__(self, rows, groups, order, offsets, tiles):
-        self.rows, self.groups, self.order, self.offsets, self.tiles = rows, groups, order, offsets, tiles
+    def __init__(self, rows, groups, plan):
+        self.rows, self.groups, self._plan = rows, groups, plan  # order, offsets, the products' tiles
+        base = plan.data_ptr()
+        self._at = (base, base + 4 * rows, base + 4 * (rows + groups + 1))
+
+    @property
+    def order(self):
+        return self._plan[:self.rows]
+
+    @property
+    def offsets(self):
+        return self._plan[self.rows:self.rows + self.groups + 1]
+
+    @property
+    def tiles(self):
+        return self._plan[self.rows + self.groups + 1:]
 
 
 def group_rows(index, groups):
@@ -103,17 +135,13 @@ def group_rows(index, groups):
         raise ValueError("group_rows: at least one group")
     index = _integers("group_rows", "index", index)
     rows = index.numel()
-    lib = _lib.lib()
-    ntiles = lib.fl_group_tiles(rows, groups)
-    # one allocation: order, offsets, tiles
-    buf = torch.empty(rows + groups + 1 + 2 * ntiles, dtype=torch.int32, device=dev)
-    order, offsets, tiles = buf[:rows], buf[rows:rows + groups + 1], buf[rows + groups + 1:]
+    lib = _lib_handle()
+    plan = torch.empty(rows + groups + 1 + 2 * lib.fl_group_tiles(rows, groups), dtype=torch.int32, device=dev)
     nbytes = lib.fl_group_rows_bytes(rows, groups)
     ws = _workspace(nbytes, dev)
-    with _on(dev):
-        check(lib.fl_group_rows(stream_handle(dev), ptr(index), rows, groups, ptr(order), ptr(offsets), ptr(tiles),
-                                ptr(ws), nbytes), "group_rows")
-    return RowGroups(rows, groups, order, offsets, tiles)
+    out = RowGroups(rows, groups, plan)
+    _launch("group_rows", lib.fl_group_rows, dev, index.data_ptr(), rows, groups, *out._at, _ptr(ws), nbytes)
+    return out
 
 
 # ---------------------------------------------------------------------------
@@ -134,7 +162,7 @@ def _linear_op(x, weight, bias, residual, plan, act):
         groups, w_group, order, offsets, tiles = 1, 0, None, None, None
     else:
         groups, w_group = plan.groups, weight.stride(0)
-        order, offsets, tiles = plan.order.data_ptr(), plan.offsets.data_ptr(), plan.tiles.data_ptr()
+        order, offsets, tiles = plan._at
     return FlLinear(M, N, K, groups, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(-2), w_group,
                     None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
                     0 if residual is None else residual.stride(0), order, offsets, tiles, _TYPES[x.dtype], act,
@@ -155,8 +183,7 @@ def _linear_forward(x, weight, bias, residual, plan, act, keep):
         residual = _rows_of(residual, N)
     pre = torch.empty((x.shape[0], N), dtype=torch.float32, device=dev) if keep else None
     op = _linear_op(x, weight, bias, residual, plan, act)
-    with _on(dev):
-        check(_lib.lib().fl_linear_forward(stream_handle(dev), op, ptr(y), ptr(pre)), "linear")
+    _launch("linear", _lib_handle().fl_linear_forward, dev, op, y.data_ptr(), _ptr(pre))
     return y, x, weight, pre
 
 
@@ -178,7 +205,7 @@ class _LinearFunction(autograd.Function):
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if need_x or need_w or need_b:
-            dev, lib = x.device, _lib.lib()
+            dev, lib = x.device, _lib_handle()
             (shape, bias_dtype), g = ctx.shapes, grad.contiguous()
             if g.data_ptr() % 16:
                 g = g.clone()
@@ -191,14 +218,13 @@ class _LinearFunction(autograd.Function):
                 db = torch.empty(weight.shape[:-1], dtype=bias_dtype, device=dev)
             nbytes = lib.fl_linear_backward_bytes(op, need_w, need_b)
             ws = _workspace(nbytes, dev)
-            with _on(dev):
-                check(lib.fl_linear_backward(stream_handle(dev), op, ptr(g), ptr(pre), ptr(dx), ptr(dw), ptr(db),
-                                             int(bias_dtype is torch.float32), ptr(ws), nbytes), "linear")
+            _launch("linear", lib.fl_linear_backward, dev, op, g.data_ptr(), _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db),
+                    bias_dtype is torch.float32, _ptr(ws), nbytes)
         return dx, dw, db, grad if need_r else None, None, None
 
 
 def _product(what, x, plan, weight, bias, activation, residual):
-    _need_gpu(what, x, weight, bias, residual, plan.order if plan is not None else None)
+    _need_gpu(what, x, weight, bias, residual, None if plan is None else plan._plan)
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError("%s: activation must be one of %s" % (what, ", ".join(map(repr, _ACTIVATIONS))))
@@ -273,8 +299,7 @@ def pack_allowed(mask):
     rows = math.prod(mask.shape[:-1])
     words = torch.empty(mask.shape[:-1] + ((n + 31) // 32,), dtype=torch.int32, device=dev)
     mask = mask.contiguous()
-    with _on(dev):
-        check(_lib.lib().fl_pack_bits(stream_handle(dev), ptr(mask), rows, n, ptr(words)), "pack_allowed")
+    _launch("pack_allowed", _lib_handle().fl_pack_bits, dev, mask.data_ptr(), rows, n, words.data_ptr())
     return words
 
 
@@ -399,18 +424,15 @@ def _constraints(what, logits, allowed, group, bias, history, *scalars):
 
 def _logits_forward(c, logits, bias, softmax):
     """(output, the laid out logits)."""
-    dev, lib = logits.device, _lib.lib()
+    dev, lib = logits.device, _lib_handle()
     out = torch.empty(logits.shape, dtype=torch.float32 if softmax else logits.dtype, device=dev)
     x = _rows_of(logits, c.cols)
     op = c.op(x, bias)
-    nbytes = lib.fl_logits_softmax_bytes(op) if softmax else 0
-    ws = _workspace(nbytes, dev)
-    with _on(dev):
-        st = stream_handle(dev)
-        if softmax:
-            check(lib.fl_logits_softmax(st, op, ptr(out), ptr(ws), nbytes), "hop_attention")
-        else:
-            check(lib.fl_logits_constrain(st, op, ptr(out)), "constrain_logits")
+    if softmax:
+        nbytes = lib.fl_logits_softmax_bytes(op)
+        _launch("hop_attention", lib.fl_logits_softmax, dev, op, out.data_ptr(), _ptr(_workspace(nbytes, dev)), nbytes)
+    else:
+        _launch("constrain_logits", lib.fl_logits_constrain, dev, op, out.data_ptr())
     return out, x
 
 
@@ -428,21 +450,17 @@ class _LogitsFunction(autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         x, bias, w = ctx.saved_tensors[:3]
-        c, lib, dev = ctx.c, _lib.lib(), grad.device
+        c, lib, dev = ctx.c, _lib_handle(), grad.device
         need_x, need_b = ctx.needs_input_grad[:2]
         shape, grad = grad.shape, grad.contiguous()
         dx = torch.empty(shape, dtype=ctx.dtype, device=dev) if need_x else None
         db = torch.empty_like(bias) if need_b else None
-        plan = group_rows(c.group, bias.shape[0]) if need_b and bias.shape[0] > 1 else None
         # without their signs the logits are not read: the gradient's rows stand for them
         op = c.op(x if x is not None else _rows_of(grad, c.cols), bias)
         nbytes = lib.fl_logits_grad_bytes(op, ctx.softmax, need_b)
         ws = _workspace(nbytes, dev)
-        with _on(dev):
-            check(lib.fl_logits_grad(stream_handle(dev), op, ptr(w), ptr(grad),
-                                     ptr(plan.order) if plan is not None else None,
-                                     ptr(plan.offsets) if plan is not None else None, ptr(dx), ptr(db), ptr(ws),
-                                     nbytes), "hop_attention" if ctx.softmax else "constrain_logits")
+        _launch("hop_attention" if ctx.softmax else "constrain_logits", lib.fl_logits_grad, dev, op, _ptr(w),
+                grad.data_ptr(), _ptr(dx), _ptr(db), _ptr(ws), nbytes)
         return dx, db, None, None
 
 

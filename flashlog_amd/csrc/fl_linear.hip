@@ -27,6 +27,7 @@
 // that such a value enters are NaN.
 #include "fl_abi.h"
 #include "fl_common.h"
+#include "fl_parts.h"
 #include <type_traits>
 
 namespace fl {
@@ -904,24 +905,6 @@ __global__ __launch_bounds__(LN_NT) void k_col_sums(const T *__restrict__ d, int
     out[((int64_t)part * groups + g) * N + c] = s;
 }
 
-// out[i] = sum over the parts, in order.
-template <typename TO>
-__global__ __launch_bounds__(LN_NT) void k_part_sums(const float *__restrict__ part, int parts, int64_t n,
-                                                     TO *__restrict__ out) {
-    for (int64_t i = (int64_t)blockIdx.x * LN_NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * LN_NT) {
-        float s = 0.0f;
-        for (int p = 0; p < parts; ++p) s += part[(int64_t)p * n + i];
-        out[i] = (TO)s;
-    }
-}
-
-template <typename TO>
-void part_sums(hipStream_t st, const float *part, int parts, int64_t n, void *out) {
-    int64_t grid = (n + LN_NT - 1) / LN_NT;
-    if (grid > 65536) grid = 65536;
-    FL_LAUNCH("k_part_sums", k_part_sums<TO>, dim3((unsigned)grid), dim3(LN_NT), 0, st, part, parts, n, (TO *)out);
-}
-
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Rows of a tile: the plan's, or for one group the largest tile that gives
@@ -1108,7 +1091,7 @@ int weight_grad(hipStream_t st, const fl_linear *op, const void *d, void *dw, fl
     if (p.wide) {
     } else if (p.tn == 128) FL_LAUNCH("k_lin_outer", (k_lin_outer<T, 128, 128, BIG_K>), g, nt, 0, st, a);
     else FL_LAUNCH("k_lin_outer", (k_lin_outer<T, 64, 64, BIG_K>), g, nt, 0, st, a);
-    if (a.part) part_sums<T>(st, ws, (int)a.parts, a.groups * a.N * a.K, dw);
+    if (a.part) fold_parts<T>(st, ws, (int)a.parts, a.groups * a.N * a.K, (T *)dw);
     return fl_check_launch("linear_backward");
 }
 
@@ -1119,8 +1102,8 @@ int bias_grad(hipStream_t st, const fl_linear *op, const void *d, void *db, int 
     if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "linear_bias_grad: too many groups for one launch (shape)");
     FL_LAUNCH("k_col_sums", k_col_sums<T>, dim3((unsigned)grid), dim3(LN_NT), 0, st,
               (const T *)d, op->N, op->M, op->N, op->groups, parts, op->order, op->offsets, ws);
-    if (db_f32) part_sums<float>(st, ws, parts, op->groups * op->N, db);
-    else part_sums<T>(st, ws, parts, op->groups * op->N, db);
+    if (db_f32) fold_parts<float>(st, ws, parts, op->groups * op->N, (float *)db);
+    else fold_parts<T>(st, ws, parts, op->groups * op->N, (T *)db);
     return fl_check_launch("linear_bias_grad");
 }
 

@@ -14,27 +14,37 @@
 //   sign of x + bias; dbias[g] = the sum of the dx of the group's rows
 //
 // All of it is one pass over the rows: HBM-bound, bytes = one read and one
-// write of the rows (the gradients: what the slopes need besides).  A
-// workgroup takes one row's segment of NT * 4 * VPT columns in registers
-// (rows of up to 8192 columns whole; the softmax of longer rows joins the
-// segments' maxima and sums in a second launch), a thread groups of 4 columns
-// (16 or 8 bytes a load).  Masks are one bit a column; the repeats of the
-// segment's columns are counted with LDS atomics (integers, so the order does
-// not matter), once per segment.
+// write of the rows.  Rows of up to 2048 columns are a wave's each, held in
+// registers (up to 8 groups of 4 columns a lane), so that nothing waits for
+// other waves; longer ones are cut into segments of 4096 columns, a workgroup
+// each (the softmax: up to 8192 whole, beyond that the segments' maxima and
+// sums are joined by a second launch).
 //
-// dbias adds fp32 terms in a fixed order: a workgroup keeps one table row's
-// segment in registers and walks the group's rows, writing their dx on the
-// way; groups of many rows are cut into parts whose sums are joined in order.
-// The terms are the unrounded ones, so half-precision logits give the same
-// dbias as fp32 ones.
+// Masks are one bit a column.  Histories are short next to the rows: up to 8
+// ids are compared with the columns in registers, more are looked at first and
+// only a segment that holds some of them counts them in LDS (integers, so the
+// order does not matter); the slopes read the logits of repeated columns only.
+//
+// dbias adds fp32 terms in a fixed order.  A workgroup keeps one table row's
+// columns in registers and walks the group's rows, writing their dx on the
+// way (rows of up to 2048 columns: four waves, a row each, joined in LDS);
+// groups of many rows are cut into parts.  The terms are the unrounded ones,
+// so half-precision logits give the same dbias as fp32 ones.
 #include "fl_abi.h"
 #include "fl_common.h"
+#include "fl_parts.h"
+#include <type_traits>
 
 namespace fl {
 namespace {
 
-constexpr int LG_LONG = 8192;      // longest row held by one workgroup
-constexpr int LG_SEG_VPT = 4;      // columns of a segment of longer rows: 256 * 4 * 4
+constexpr int LG_WAVE_COLS = 2048;  // longest row held by a wave
+constexpr int LG_LONG = 8192;       // longest row held by a workgroup
+constexpr int LG_NT = 256;
+constexpr int LG_WAVES = LG_NT / FL_WAVE;
+constexpr int LG_VPT = 4;           // groups of 4 columns a thread of a segment
+constexpr int LG_SEG = LG_NT * 4 * LG_VPT;
+constexpr int LG_FEW = 8;           // ids compared in registers
 
 enum { LG_CONSTRAIN = 0, LG_SOFTMAX = 1, LG_STATS = 2, LG_JOINED = 3 };
 
@@ -101,8 +111,24 @@ __device__ __forceinline__ RowView row_view(const fl_logits &op, int64_t row) {
     return r;
 }
 
+// Threads that share a row: a wave (nothing to wait for) or a workgroup.
 template <int NT>
-__device__ __forceinline__ float block_max(float v, float *red) {
+__device__ __forceinline__ void team_sync() {
+    if (NT == FL_WAVE) fl_wave_sync();
+    else __syncthreads();
+}
+template <int NT>
+__device__ __forceinline__ bool team_any(bool v) {
+    if (NT == FL_WAVE) return __any(v);
+    return __syncthreads_or(v);
+}
+template <int NT>
+__device__ __forceinline__ int team_thread() {
+    return NT == FL_WAVE ? fl_lane() : (int)threadIdx.x;
+}
+
+template <int NT>
+__device__ __forceinline__ float team_max(float v, float *red) {
 #pragma unroll
     for (int o = FL_WAVE / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, FL_WAVE));
     if (NT == FL_WAVE) return v;
@@ -116,7 +142,7 @@ __device__ __forceinline__ float block_max(float v, float *red) {
 }
 
 template <int NT>
-__device__ __forceinline__ float block_sum(float v, float *red) {
+__device__ __forceinline__ float team_sum(float v, float *red) {
     v = fl_wave_sum_f32(v);
     if (NT == FL_WAVE) return v;
     if (fl_lane() == 0) red[fl_wave_id()] = v;
@@ -128,18 +154,72 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
     return v;
 }
 
-// Counts the ids of the row's history that fall into [base, base + SEG).
+// How often the row's history holds the columns [base, base + SEG).
 template <int NT, int SEG>
-__device__ __forceinline__ void count_repeats(const RowView &r, int64_t base, int64_t cols, int *cnt) {
-    __syncthreads();  // the last row's counts are read
-    for (int i = threadIdx.x; i < SEG; i += NT) cnt[i] = 0;
-    __syncthreads();
-    for (int64_t i = threadIdx.x; i < r.nids; i += NT) {
-        const int64_t id = r.ids[i];
-        if (id >= base && id < base + SEG && id < cols) atomicAdd(&cnt[id - base], 1);
+struct Repeats {
+    enum { NONE, FEW, BYTES, WORDS };
+    int mode;
+    int rel[LG_FEW];  // FEW: the ids' places in the segment, far below it for those outside
+    const int *cnt;   // BYTES: a byte a column; WORDS: a word
+
+    // lds: SEG words of the team.
+    __device__ __forceinline__ void begin(const RowView &r, int64_t base, int64_t cols, int *lds) {
+        const int64_t end = base + SEG < cols ? base + SEG : cols;
+        const int t = team_thread<NT>();
+        cnt = lds;
+        mode = NONE;
+        if (r.nids <= LG_FEW) {
+            if (r.nids == 0) return;
+            mode = FEW;
+#pragma unroll
+            for (int k = 0; k < LG_FEW; ++k) {
+                const int64_t id = k < r.nids ? r.ids[k] : -1;
+                rel[k] = id >= base && id < end ? (int)(id - base) : -8;
+            }
+            return;
+        }
+        bool hit = false;
+        for (int64_t i = t; i < r.nids; i += NT) {
+            const int64_t id = r.ids[i];
+            hit |= id >= base && id < end;
+        }
+        if (!team_any<NT>(hit)) return;  // (behind it the last row's counts are read)
+        const bool bytes = r.nids <= 255;
+        mode = bytes ? BYTES : WORDS;
+        const int words = bytes ? SEG / 4 : SEG;
+        for (int i = t; i < words; i += NT) lds[i] = 0;
+        team_sync<NT>();
+        for (int64_t i = t; i < r.nids; i += NT) {
+            const int64_t id = r.ids[i];
+            if (id >= base && id < end) {
+                const int c = (int)(id - base);
+                if (bytes) atomicAdd(&lds[c >> 2], 1 << (8 * (c & 3)));
+                else atomicAdd(&lds[c], 1);
+            }
+        }
+        team_sync<NT>();
     }
-    __syncthreads();
-}
+    // The counts of the columns local .. local + 3; whether any is not 0.
+    __device__ __forceinline__ bool quad(int local, int (&c)[4]) const {
+        if (mode == NONE) return false;
+        if (mode == WORDS) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[e] = cnt[local + e];
+            return (c[0] | c[1] | c[2] | c[3]) != 0;
+        }
+        unsigned w = 0;
+        if (mode == BYTES) w = (unsigned)cnt[local >> 2];
+        else
+#pragma unroll
+            for (int k = 0; k < LG_FEW; ++k) {
+                const unsigned d = (unsigned)(rel[k] - local);
+                w += d < 4 ? 1u << (8 * d) : 0u;
+            }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = (int)((w >> (8 * e)) & 255u);
+        return w != 0;
+    }
+};
 
 // The allowed bits of columns c .. c + 3 (those below cols).
 __device__ __forceinline__ unsigned quad_bits(const RowView &r, int64_t c, int64_t cols) {
@@ -148,98 +228,143 @@ __device__ __forceinline__ unsigned quad_bits(const RowView &r, int64_t c, int64
     return cols - c < 4 ? b & ((1u << (cols - c)) - 1) : b;
 }
 
-__device__ __forceinline__ float constrained(const LogitArgs &a, float x, float b, int c) {
-    float u = x + b;
-    if (c > 0) {
-        u = u > 0.0f ? u * a.inv_repetition : u * a.op.repetition;
-        u -= a.op.presence + a.op.frequency * (float)c;
-    }
-    return u * a.inv_temperature;
-}
-
-// Forward of one row's segment.  LG_STATS: the segment's maximum and sum to
-// stats; LG_JOINED: the softmax with the row's joined statistics.
-template <typename T, int NT, int VPT, int MODE, bool HIST>
-__global__ __launch_bounds__(NT) void k_logits(LogitArgs a, void *out, float2 *stats) {
-    constexpr int SEG = NT * 4 * VPT;
-    __shared__ float red[NT / FL_WAVE];
-    __shared__ int cnt[HIST ? SEG : 1];
-    const int64_t cols = a.op.cols;
-    const int64_t row = blockIdx.x / a.segments;
-    const int64_t base = (int64_t)(blockIdx.x % a.segments) * SEG;
-    const RowView r = row_view(a.op, row);
-    const T *x = (const T *)a.op.x + row * a.op.ldx;
+// A row's segment in a team's registers: the constrained values v and the
+// allowed bits.
+template <typename T, int NT, int VPT, bool HIST>
+struct Segment {
+    static constexpr int SEG = NT * 4 * VPT;
     float v[VPT][4];
-    unsigned ok = 0;
-    if (HIST) count_repeats<NT, SEG>(r, base, cols, cnt);
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int local = (i * NT + threadIdx.x) * 4;
-        const int64_t c = base + local;
-        const unsigned bits = quad_bits(r, c, cols);
-        ok |= bits << (4 * i);
-        if (c >= cols) continue;
-        const Quad<T> q = load_quad(x + c, cols - c);
-        Quad<float> b{{0, 0, 0, 0}};
-        if (r.bias) b = load_quad(r.bias + c, cols - c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            v[i][e] = constrained(a, (float)q.v[e], b.v[e], HIST ? cnt[local + e] : 0);
-    }
-    if constexpr (MODE == LG_CONSTRAIN) {
-        T *y = (T *)out + row * cols;
+    unsigned ok;
+
+    static __device__ __forceinline__ int local(int i) { return (i * NT + team_thread<NT>()) * 4; }
+
+    __device__ __forceinline__ void load(const LogitArgs &a, int64_t row, int64_t base, int *cnt) {
+        const int64_t cols = a.op.cols;
+        const RowView r = row_view(a.op, row);
+        const T *x = (const T *)a.op.x + row * a.op.ldx;
+        Quad<T> q[VPT];
+        ok = 0;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int64_t c = base + (i * NT + threadIdx.x) * 4;
-            if (c >= cols) continue;
-            Quad<T> q;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q.v[e] = (T)((ok >> (4 * i + e)) & 1 ? v[i][e] : a.op.fill);
-            store_quad(y + c, q, cols - c);
+            const int64_t c = base + local(i);
+            if (c < cols) q[i] = load_quad(x + c, cols - c);
+            ok |= quad_bits(r, c, cols) << (4 * i);
         }
-        return;
+        Repeats<NT, SEG> rep;
+        if (HIST) rep.begin(r, base, cols, cnt);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int64_t c = base + local(i);
+            if (c >= cols) continue;
+            Quad<float> b{{0, 0, 0, 0}};
+            if (r.bias) b = load_quad(r.bias + c, cols - c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = (float)q[i].v[e] + b.v[e];
+            int n[4];
+            if (HIST && rep.quad(local(i), n)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n[e] > 0) {
+                        v[i][e] *= v[i][e] > 0.0f ? a.inv_repetition : a.op.repetition;
+                        v[i][e] -= a.op.presence + a.op.frequency * (float)n[e];
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] *= a.inv_temperature;
+        }
     }
-    float m = -__builtin_inff(), s = 0.0f;
-    if constexpr (MODE == LG_JOINED) {
-        const float2 *st = stats + row * a.segments;
-        for (int64_t i = threadIdx.x; i < a.segments; i += NT) m = fmaxf(m, st[i].x);
-        m = block_max<NT>(m, red);
-        if (m == -__builtin_inff()) m = 0.0f;
-        for (int64_t i = threadIdx.x; i < a.segments; i += NT) s += st[i].y * expf(st[i].x - m);
-        s = block_sum<NT>(s, red);
-    } else {
+    __device__ __forceinline__ bool allowed(int i, int e) const { return (ok >> (4 * i + e)) & 1; }
+    __device__ __forceinline__ float largest(float *red) const {
+        float m = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if ((ok >> (4 * i + e)) & 1) m = fmaxf(m, v[i][e]);
-        m = block_max<NT>(m, red);
-        if (m == -__builtin_inff()) m = MODE == LG_STATS ? m : 0.0f;
+                if (allowed(i, e)) m = fmaxf(m, v[i][e]);
+        return team_max<NT>(m, red);
     }
-    const float shift = m == -__builtin_inff() ? 0.0f : m;
+    // v = exp(v - shift) where allowed, 0 elsewhere; this thread's sum.
+    __device__ __forceinline__ float exponentials(float shift) {
+        float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+        for (int i = 0; i < VPT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[i][e] = (ok >> (4 * i + e)) & 1 ? expf(v[i][e] - shift) : 0.0f;
-            if (MODE != LG_JOINED) s += v[i][e];
+            for (int e = 0; e < 4; ++e) {
+                v[i][e] = allowed(i, e) ? expf(v[i][e] - shift) : 0.0f;
+                s += v[i][e];
+            }
+        return s;
+    }
+    __device__ __forceinline__ void store_weights(float *y, int64_t base, int64_t cols, float inv) const {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int64_t c = base + local(i);
+            if (c < cols)
+                store_quad(y + c, Quad<float>{{v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv}}, cols - c);
         }
-    if (MODE != LG_JOINED) s = block_sum<NT>(s, red);
-    if constexpr (MODE == LG_STATS) {
-        // a segment of nothing but NaN keeps its sum: a maximum of 0 lets it through
-        if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(m == -__builtin_inff() && s != s ? 0.0f : m, s);
-        return;
     }
-    const float inv = 1.0f / (s == 0.0f ? 1.0f : s);
-    float *y = (float *)out + row * cols;
+    __device__ __forceinline__ void store_values(T *y, int64_t base, int64_t cols, float fill) const {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int64_t c = base + (i * NT + threadIdx.x) * 4;
-        if (c >= cols) continue;
-        Quad<float> q;
+        for (int i = 0; i < VPT; ++i) {
+            const int64_t c = base + local(i);
+            if (c >= cols) continue;
+            Quad<T> q;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) q.v[e] = v[i][e] * inv;
-        store_quad(y + c, q, cols - c);
+            for (int e = 0; e < 4; ++e) q.v[e] = (T)(allowed(i, e) ? v[i][e] : fill);
+            store_quad(y + c, q, cols - c);
+        }
+    }
+};
+
+// Forward of rows held whole by a wave (NT = 64: a wave each) or a workgroup.
+template <typename T, int NT, int VPT, bool SOFTMAX, bool HIST>
+__global__ __launch_bounds__(LG_NT) void k_logits_rows(LogitArgs a, void *out) {
+    using Seg = Segment<T, NT, VPT, HIST>;
+    __shared__ float red[LG_WAVES];
+    __shared__ int cnt[HIST ? LG_NT / NT : 1][HIST ? Seg::SEG : 1];
+    const int team = NT == FL_WAVE ? fl_wave_id() : 0;
+    const int64_t row = NT == FL_WAVE ? (int64_t)blockIdx.x * (blockDim.x / FL_WAVE) + team : (int64_t)blockIdx.x;
+    if (row >= a.op.rows) return;  // NT = 64: no workgroup barriers
+    const int64_t cols = a.op.cols;
+    Seg s;
+    s.load(a, row, 0, cnt[HIST ? team : 0]);
+    if constexpr (!SOFTMAX) {
+        s.store_values((T *)out + row * cols, 0, cols, a.op.fill);
+    } else {
+        const float m = s.largest(red);
+        const float sum = team_sum<NT>(s.exponentials(m == -__builtin_inff() ? 0.0f : m), red);
+        s.store_weights((float *)out + row * cols, 0, cols, 1.0f / (sum == 0.0f ? 1.0f : sum));
+    }
+}
+
+// Forward of one segment of a longer row.  LG_STATS: its maximum and sum;
+// LG_JOINED: the softmax with the row's joined ones.
+template <typename T, int MODE, bool HIST>
+__global__ __launch_bounds__(LG_NT) void k_logits_seg(LogitArgs a, void *out, float2 *stats) {
+    using Seg = Segment<T, LG_NT, LG_VPT, HIST>;
+    __shared__ float red[LG_WAVES];
+    __shared__ int cnt[HIST ? LG_SEG : 1];
+    const int64_t cols = a.op.cols, row = blockIdx.x / a.segments;
+    const int64_t base = (int64_t)(blockIdx.x % a.segments) * LG_SEG;
+    Seg s;
+    s.load(a, row, base, cnt);
+    if constexpr (MODE == LG_CONSTRAIN) {
+        s.store_values((T *)out + row * cols, base, cols, a.op.fill);
+    } else if constexpr (MODE == LG_STATS) {
+        const float m = s.largest(red);
+        const float sum = team_sum<LG_NT>(s.exponentials(m == -__builtin_inff() ? 0.0f : m), red);
+        // a segment of nothing but NaN keeps its sum: a maximum of 0 lets it through
+        if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(m == -__builtin_inff() && sum != sum ? 0.0f : m, sum);
+    } else {
+        const float2 *st = stats + row * a.segments;
+        float m = -__builtin_inff(), sum = 0.0f;
+        for (uint32_t i = threadIdx.x; i < a.segments; i += LG_NT) m = fmaxf(m, st[i].x);
+        m = team_max<LG_NT>(m, red);
+        if (m == -__builtin_inff()) m = 0.0f;
+        for (uint32_t i = threadIdx.x; i < a.segments; i += LG_NT) sum += st[i].y * expf(st[i].x - m);
+        sum = team_sum<LG_NT>(sum, red);
+        s.exponentials(m);
+        s.store_weights((float *)out + row * cols, base, cols, 1.0f / (sum == 0.0f ? 1.0f : sum));
     }
 }
 
@@ -247,34 +372,216 @@ struct GradArgs {
     LogitArgs l;
     const void *g;        // gradient of the output (T; the softmax: float)
     const float *w;       // the softmax's output
-    const float *dots;    // [rows] sum w g, of rows longer than a segment
+    const float *dots;    // [rows] sum w g, of rows longer than a workgroup holds
     void *dx;
-    float *dbias;         // [parts][bias_rows][cols], or null
-    const int32_t *order, *offsets;  // owners by group (null: every row its own list, or one list of all)
-    int64_t lists;        // row lists (groups and one of no group; without dbias the rows)
+    float *dbias;         // [parts][bias_rows][cols], or null: every row is a list of its own
+    const int32_t *order, *offsets;  // owners by group (null: one list of all)
+    int64_t lists;        // row lists: groups and one of no group
     uint32_t parts;
 };
 
+// The rows of a list, cut into parts.
+struct RowList {
+    int64_t first, q0, q1;
+    __device__ __forceinline__ RowList(const GradArgs &a, int64_t list, uint32_t part) {
+        const fl_logits &op = a.l.op;
+        first = a.order ? (int64_t)a.offsets[list] : 0;
+        const int64_t end = a.order && list + 1 < a.lists ? (int64_t)a.offsets[list + 1] : op.rows / op.inner;
+        const int64_t n = (end - first) * op.inner;
+        q0 = n * part / a.parts;
+        q1 = n * (part + 1) / a.parts;
+    }
+    __device__ __forceinline__ int64_t row(const GradArgs &a, int64_t q) const {
+        const uint32_t inner = (uint32_t)a.l.op.inner, at = (uint32_t)q / inner;
+        const int64_t place = first + at;
+        return (a.order ? (int64_t)a.order[place] : place) * inner + ((uint32_t)q - at * inner);
+    }
+};
+
+// The gradient of a row's segment: what it reads, and its terms.
+template <typename T, int NT, int VPT, bool SOFTMAX, bool HIST>
+struct GradSegment {
+    using TG = std::conditional_t<SOFTMAX, float, T>;
+    static constexpr int SEG = NT * 4 * VPT;
+    Quad<TG> g[VPT];
+    Quad<float> w[SOFTMAX ? VPT : 1];
+    int64_t row;
+
+    static __device__ __forceinline__ int local(int i) { return (i * NT + team_thread<NT>()) * 4; }
+
+    __device__ __forceinline__ void load(const GradArgs &a, int64_t at, int64_t base) {
+        row = at;
+        const int64_t cols = a.l.op.cols;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int64_t c = base + local(i);
+            if (c >= cols) continue;
+            g[i] = load_quad((const TG *)a.g + row * cols + c, cols - c);
+            if (SOFTMAX) w[i] = load_quad(a.w + row * cols + c, cols - c);
+        }
+    }
+    // Writes the row's dx and adds its terms to acc.
+    template <bool WHOLE>
+    __device__ __forceinline__ void apply(const GradArgs &a, int64_t base, int *cnt, float *red, float (&acc)[VPT][4]) {
+        const fl_logits &op = a.l.op;
+        const int64_t cols = op.cols;
+        const RowView r = row_view(op, row);
+        unsigned ok = 0;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int64_t c = base + local(i);
+            const unsigned bits = quad_bits(r, c, cols);
+            ok |= bits << (4 * i);
+            if (SOFTMAX && WHOLE && c < cols)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s += (bits >> e) & 1 ? w[i].v[e] * (float)g[i].v[e] : 0.0f;
+        }
+        Repeats<NT, SEG> rep;
+        if (HIST) rep.begin(r, base, cols, cnt);
+        if (SOFTMAX) s = WHOLE ? team_sum<NT>(s, red) : a.dots[row];
+        const T *x = (const T *)op.x + row * op.ldx;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int64_t c = base + local(i);
+            if (c >= cols) continue;
+            float u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                u[e] = SOFTMAX ? w[i].v[e] * ((float)g[i].v[e] - s) : (float)g[i].v[e];
+                u[e] *= a.l.inv_temperature;
+            }
+            int n[4];
+            if (HIST && rep.quad(local(i), n)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n[e] > 0) {
+                        const float z = (float)x[c + e] + (r.bias ? r.bias[c + e] : 0.0f);
+                        u[e] *= z > 0.0f ? a.l.inv_repetition : op.repetition;
+                    }
+            }
+            Quad<T> o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                u[e] = (ok >> (4 * i + e)) & 1 ? u[e] : 0.0f;
+                acc[i][e] += u[e];
+                o.v[e] = (T)u[e];
+            }
+            if (a.dx) store_quad((T *)a.dx + row * cols + c, o, cols - c);
+        }
+    }
+};
+
+// Rows held whole by a wave.  Without dbias a wave takes one row; with it a
+// workgroup's waves take the rows of a list in turn, each loading its next
+// row while it works on one, and join their sums.
+template <typename T, int VPT, bool SOFTMAX, bool HIST>
+__global__ __launch_bounds__(LG_NT) void k_logits_rows_grad(GradArgs a) {
+    using Grad = GradSegment<T, FL_WAVE, VPT, SOFTMAX, HIST>;
+    constexpr int SEG = Grad::SEG;
+    __shared__ int cnt[HIST ? LG_WAVES : 1][HIST ? SEG : 1];
+    __shared__ float sums[SEG];
+    const int64_t cols = a.l.op.cols;
+    const int wave = fl_wave_id(), waves = blockDim.x / FL_WAVE;
+    int *mine = cnt[HIST ? wave : 0];
+    float acc[VPT][4];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
+    if (!a.dbias) {
+        const int64_t row = (int64_t)blockIdx.x * waves + wave;
+        if (row >= a.l.op.rows) return;
+        Grad g;
+        g.load(a, row, 0);
+        g.template apply<true>(a, 0, mine, nullptr, acc);
+        return;
+    }
+    const int64_t list = blockIdx.x / a.parts;
+    const uint32_t part = blockIdx.x % a.parts;
+    const RowList rows(a, list, part);
+    Grad g;
+    if (rows.q0 + wave < rows.q1) g.load(a, rows.row(a, rows.q0 + wave), 0);
+    for (int64_t q = rows.q0 + wave; q < rows.q1; q += LG_WAVES) {
+        Grad next = g;
+        if (q + LG_WAVES < rows.q1) next.load(a, rows.row(a, q + LG_WAVES), 0);
+        g.template apply<true>(a, 0, mine, nullptr, acc);
+        g = next;
+    }
+    if (list >= a.l.op.bias_rows) return;
+    // in wave order
+    for (int w = 0; w < LG_WAVES; ++w) {
+        if (wave == w)
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float *at = sums + Grad::local(i) + e;
+                    *at = w == 0 ? acc[i][e] : *at + acc[i][e];
+                }
+        __syncthreads();
+    }
+    float *b = a.dbias + ((int64_t)part * a.l.op.bias_rows + list) * cols;
+    for (int64_t c = threadIdx.x; c < cols; c += LG_NT) b[c] = sums[c];
+}
+
+// One segment of the rows of a list (or of one row).  WHOLE: it is the row.
+template <typename T, int VPT, bool SOFTMAX, bool HIST, bool WHOLE>
+__global__ __launch_bounds__(LG_NT) void k_logits_seg_grad(GradArgs a) {
+    using Grad = GradSegment<T, LG_NT, VPT, SOFTMAX, HIST>;
+    __shared__ float red[LG_WAVES];
+    __shared__ int cnt[HIST ? Grad::SEG : 1];
+    const int64_t cols = a.l.op.cols;
+    const uint32_t item = blockIdx.x / a.l.segments;
+    const int64_t base = (int64_t)(blockIdx.x % a.l.segments) * Grad::SEG;
+    float acc[VPT][4];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
+    Grad g;
+    if (!a.dbias) {
+        g.load(a, item, base);
+        g.template apply<WHOLE>(a, base, cnt, red, acc);
+        return;
+    }
+    const uint32_t part = item % a.parts;
+    const int64_t list = item / a.parts;
+    const RowList rows(a, list, part);
+    if (rows.q0 < rows.q1) g.load(a, rows.row(a, rows.q0), base);
+    for (int64_t q = rows.q0; q < rows.q1; ++q) {
+        Grad next = g;
+        if (q + 1 < rows.q1) next.load(a, rows.row(a, q + 1), base);
+        g.template apply<WHOLE>(a, base, cnt, red, acc);
+        g = next;
+    }
+    if (list >= a.l.op.bias_rows) return;
+    float *b = a.dbias + ((int64_t)part * a.l.op.bias_rows + list) * cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int64_t c = base + Grad::local(i);
+        if (c < cols) store_quad(b + c, Quad<float>{{acc[i][0], acc[i][1], acc[i][2], acc[i][3]}}, cols - c);
+    }
+}
+
 // sum w g of one segment of a row.
-template <int NT, int VPT>
-__global__ __launch_bounds__(NT) void k_logits_dot(LogitArgs a, const float *__restrict__ g,
-                                                   const float *__restrict__ w, float *__restrict__ dots) {
-    constexpr int SEG = NT * 4 * VPT;
-    __shared__ float red[NT / FL_WAVE];
+__global__ __launch_bounds__(LG_NT) void k_logits_dot(LogitArgs a, const float *__restrict__ g,
+                                                      const float *__restrict__ w, float *__restrict__ dots) {
+    __shared__ float red[LG_WAVES];
     const int64_t cols = a.op.cols, row = blockIdx.x / a.segments;
-    const int64_t base = (int64_t)(blockIdx.x % a.segments) * SEG;
+    const int64_t base = (int64_t)(blockIdx.x % a.segments) * LG_SEG;
     const RowView r = row_view(a.op, row);
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int64_t c = base + (i * NT + threadIdx.x) * 4;
+    for (int i = 0; i < LG_VPT; ++i) {
+        const int64_t c = base + (i * LG_NT + threadIdx.x) * 4;
         const unsigned bits = quad_bits(r, c, cols);
         if (!bits) continue;
         const Quad<float> p = load_quad(w + row * cols + c, cols - c), q = load_quad(g + row * cols + c, cols - c);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s += (bits >> e) & 1 ? p.v[e] * q.v[e] : 0.0f;
     }
-    s = block_sum<NT>(s, red);
+    s = team_sum<LG_NT>(s, red);
     if (threadIdx.x == 0) dots[blockIdx.x] = s;
 }
 
@@ -285,113 +592,6 @@ __global__ __launch_bounds__(FL_WAVE) void k_logits_join(const float *__restrict
     for (int64_t i = threadIdx.x; i < segments; i += FL_WAVE) s += part[row * segments + i];
     s = fl_wave_sum_f32(s);
     if (threadIdx.x == 0) dots[row] = s;
-}
-
-// Gradients of the rows of a list (a part of them), one segment of columns.
-template <typename T, int NT, int VPT, bool SOFTMAX, bool HIST, bool WHOLE>
-__global__ __launch_bounds__(NT) void k_logits_grad(GradArgs a) {
-    constexpr int SEG = NT * 4 * VPT;
-    __shared__ float red[NT / FL_WAVE];
-    __shared__ int cnt[HIST ? SEG : 1];
-    const fl_logits &op = a.l.op;
-    const int64_t cols = op.cols;
-    const uint32_t item = blockIdx.x / a.l.segments;
-    const int64_t base = (int64_t)(blockIdx.x % a.l.segments) * SEG;
-    const uint32_t part = item % a.parts;
-    const int64_t list = item / a.parts;
-    int64_t first = list, count = 1;  // rows (without a plan) or places of owners
-    if (a.dbias) {
-        const int64_t owners = op.rows / op.inner;
-        first = a.order ? (int64_t)a.offsets[list] : 0;
-        count = ((a.order && list + 1 < a.lists ? (int64_t)a.offsets[list + 1] : owners) - first) * op.inner;
-    }
-    const int64_t q0 = count * part / a.parts, q1 = count * (part + 1) / a.parts;
-    float acc[VPT][4];
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
-    for (int64_t q = q0; q < q1; ++q) {
-        int64_t row = first;
-        if (a.dbias) {
-            const uint32_t inner = (uint32_t)op.inner, at = (uint32_t)q / inner;
-            const int64_t place = first + at;
-            row = (a.order ? (int64_t)a.order[place] : place) * inner + ((uint32_t)q - at * inner);
-        }
-        const RowView r = row_view(op, row);
-        if (HIST) count_repeats<NT, SEG>(r, base, cols, cnt);
-        float d[VPT][4];
-        Quad<float> w[VPT];
-        unsigned ok = 0;
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t c = base + (i * NT + threadIdx.x) * 4;
-            const unsigned bits = quad_bits(r, c, cols);
-            ok |= bits << (4 * i);
-            if (c >= cols) continue;
-            if (SOFTMAX) {
-                const Quad<float> g = load_quad((const float *)a.g + row * cols + c, cols - c);
-                w[i] = load_quad(a.w + row * cols + c, cols - c);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    d[i][e] = g.v[e];
-                    if (WHOLE) s += (bits >> e) & 1 ? w[i].v[e] * g.v[e] : 0.0f;
-                }
-            } else {
-                const Quad<T> g = load_quad((const T *)a.g + row * cols + c, cols - c);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) d[i][e] = (float)g.v[e];
-            }
-        }
-        if (SOFTMAX) s = WHOLE ? block_sum<NT>(s, red) : a.dots[row];
-        const T *x = (const T *)op.x + row * op.ldx;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int local = (i * NT + threadIdx.x) * 4;
-            const int64_t c = base + local;
-            if (c >= cols) continue;
-            float slope[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) slope[e] = a.l.inv_temperature;
-            if (HIST) {
-                const Quad<T> xq = load_quad(x + c, cols - c);
-                Quad<float> b{{0, 0, 0, 0}};
-                if (r.bias) b = load_quad(r.bias + c, cols - c);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (cnt[local + e] > 0)
-                        slope[e] *= (float)xq.v[e] + b.v[e] > 0.0f ? a.l.inv_repetition : op.repetition;
-            }
-            Quad<T> o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float t = SOFTMAX ? w[i].v[e] * (d[i][e] - s) : d[i][e];
-                const float u = (ok >> (4 * i + e)) & 1 ? t * slope[e] : 0.0f;
-                acc[i][e] += u;
-                o.v[e] = (T)u;
-            }
-            if (a.dx) store_quad((T *)a.dx + row * cols + c, o, cols - c);
-        }
-    }
-    if (a.dbias && list < op.bias_rows) {
-        float *b = a.dbias + ((int64_t)part * op.bias_rows + list) * cols;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t c = base + (i * NT + threadIdx.x) * 4;
-            if (c >= cols) continue;
-            store_quad(b + c, Quad<float>{{acc[i][0], acc[i][1], acc[i][2], acc[i][3]}}, cols - c);
-        }
-    }
-}
-
-__global__ __launch_bounds__(256) void k_logits_parts(const float *__restrict__ part, int parts, int64_t n,
-                                                      float *__restrict__ out) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float s = 0.0f;
-        for (int p = 0; p < parts; ++p) s += part[(int64_t)p * n + i];
-        out[i] = s;
-    }
 }
 
 // One bit a column of a byte mask, 32 columns a word.
@@ -408,16 +608,6 @@ __global__ __launch_bounds__(256) void k_pack_bits(const uint8_t *__restrict__ m
 
 int64_t lg_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-int64_t seg_cols(int64_t cols, bool softmax) {
-    if (cols <= 256) return 256;
-    if (cols <= 1024) return 1024;
-    if (cols <= 2048) return 2048;
-    if (softmax && cols <= LG_LONG) return LG_LONG;
-    return 256 * 4 * LG_SEG_VPT;
-}
-
-bool lg_long(int64_t cols) { return cols > LG_LONG; }
-
 int lg_check(const fl_logits *op, const char *what) {
     if (!op) return fl_fail(FL_ERR_ARG, "%s: null operator", what);
     if (op->dtype < FL_F32 || op->dtype > FL_F16) return fl_fail(FL_ERR_ARG, "%s: unknown type", what);
@@ -432,8 +622,7 @@ int lg_check(const fl_logits *op, const char *what) {
         return fl_fail(FL_ERR_ARG, "%s: bad shape of the bias table", what);
     if (op->history && op->history_len < 0) return fl_fail(FL_ERR_ARG, "%s: bad shape of the history", what);
     if (op->rows > 0 && op->cols > 0 && !op->x) return fl_fail(FL_ERR_ARG, "%s: null pointer", what);
-    const int64_t seg = seg_cols(op->cols, false);
-    if (op->cols && op->rows > 0x7fffffffll / lg_ceil(op->cols, seg))
+    if (op->cols && op->rows > 0x7fffffffll / lg_ceil(op->cols, LG_SEG))
         return fl_fail(FL_ERR_ARG, "%s: too many rows for one launch (shape)", what);
     return FL_OK;
 }
@@ -449,84 +638,145 @@ LogitArgs lg_args(const fl_logits *op, int64_t seg) {
     return a;
 }
 
-template <typename T, int NT, int VPT, int MODE>
-void launch_fwd(hipStream_t st, const fl_logits *op, void *out, float2 *stats) {
+// Waves of a workgroup whose waves take a row each: one where there are too
+// few rows to give every CU a workgroup of four.
+int row_waves(int64_t rows) { return rows < 1024 ? 1 : LG_WAVES; }
+
+template <typename T, int NT, int VPT, bool SOFTMAX>
+void launch_rows(hipStream_t st, const fl_logits *op, void *out) {
     const LogitArgs a = lg_args(op, NT * 4 * VPT);
-    const dim3 grid((unsigned)(op->rows * a.segments));
-    if (op->history)
-        FL_LAUNCH("k_logits", (k_logits<T, NT, VPT, MODE, true>), grid, dim3(NT), 0, st, a, out, stats);
-    else
-        FL_LAUNCH("k_logits", (k_logits<T, NT, VPT, MODE, false>), grid, dim3(NT), 0, st, a, out, stats);
+    const int waves = NT == FL_WAVE ? row_waves(op->rows) : LG_WAVES;
+    const dim3 grid((unsigned)(NT == FL_WAVE ? lg_ceil(op->rows, waves) : op->rows)), nt(waves * FL_WAVE);
+    if (op->history) FL_LAUNCH("k_logits_rows", (k_logits_rows<T, NT, VPT, SOFTMAX, true>), grid, nt, 0, st, a, out);
+    else FL_LAUNCH("k_logits_rows", (k_logits_rows<T, NT, VPT, SOFTMAX, false>), grid, nt, 0, st, a, out);
 }
 
 template <typename T, int MODE>
+void launch_seg(hipStream_t st, const fl_logits *op, void *out, float2 *stats) {
+    const LogitArgs a = lg_args(op, LG_SEG);
+    const dim3 grid((unsigned)(op->rows * a.segments)), nt(LG_NT);
+    if (op->history) FL_LAUNCH("k_logits_seg", (k_logits_seg<T, MODE, true>), grid, nt, 0, st, a, out, stats);
+    else FL_LAUNCH("k_logits_seg", (k_logits_seg<T, MODE, false>), grid, nt, 0, st, a, out, stats);
+}
+
+template <typename T, bool SOFTMAX>
 int forward(hipStream_t st, const fl_logits *op, void *out, float2 *stats, const char *what) {
-    const int64_t seg = seg_cols(op->cols, MODE == LG_SOFTMAX);
-    if (seg == 256) launch_fwd<T, 64, 1, MODE>(st, op, out, stats);
-    else if (seg == 1024) launch_fwd<T, 256, 1, MODE>(st, op, out, stats);
-    else if (seg == 2048) launch_fwd<T, 256, 2, MODE>(st, op, out, stats);
-    else if constexpr (MODE == LG_CONSTRAIN) launch_fwd<T, 256, LG_SEG_VPT, MODE>(st, op, out, stats);
-    else if (seg == LG_LONG) launch_fwd<T, 256, LG_LONG / 1024, MODE>(st, op, out, stats);
+    if (op->cols <= 256) launch_rows<T, FL_WAVE, 1, SOFTMAX>(st, op, out);
+    else if (op->cols <= 512) launch_rows<T, FL_WAVE, 2, SOFTMAX>(st, op, out);
+    else if (op->cols <= 1024) launch_rows<T, FL_WAVE, 4, SOFTMAX>(st, op, out);
+    else if (op->cols <= LG_WAVE_COLS) launch_rows<T, FL_WAVE, 8, SOFTMAX>(st, op, out);
+    else if constexpr (!SOFTMAX) launch_seg<T, LG_CONSTRAIN>(st, op, out, stats);
+    else if (op->cols <= LG_LONG) launch_rows<T, LG_NT, LG_LONG / LG_NT / 4, true>(st, op, out);
     else {
-        launch_fwd<T, 256, LG_SEG_VPT, LG_STATS>(st, op, out, stats);
-        launch_fwd<T, 256, LG_SEG_VPT, LG_JOINED>(st, op, out, stats);
+        launch_seg<T, LG_STATS>(st, op, out, stats);
+        launch_seg<T, LG_JOINED>(st, op, out, stats);
     }
     return fl_check_launch(what);
 }
 
-// Row lists of the gradient with a bias table: its groups and, with a plan,
-// the owners of no group.
+// Row lists of a bias table's gradient: its groups and, when there are
+// several, the owners of none.
 int64_t grad_lists(const fl_logits *op) { return op->bias_rows > 1 ? op->bias_rows + 1 : 1; }
 
+int64_t grad_segments(const fl_logits *op, bool softmax) {
+    return op->cols <= LG_WAVE_COLS || (softmax && op->cols <= LG_LONG) ? 1 : lg_ceil(op->cols, LG_SEG);
+}
+
+// Parts of a list: some 2048 workgroups in all, of at least 8 rows on average.
 int grad_parts(const fl_logits *op, int64_t lists, int64_t segments) {
     const int64_t want = lg_ceil(2048, lists * segments), most = op->rows / (8 * lists);
     const int64_t p = want < most ? want : most;
     return (int)(p < 1 ? 1 : p > 256 ? 256 : p);
 }
 
-template <typename T, int NT, int VPT, bool SOFTMAX, bool WHOLE>
-void launch_grad(hipStream_t st, GradArgs &a, const fl_logits *op, float *dbias, float *ws) {
-    a.l = lg_args(op, NT * 4 * VPT);
-    const bool table = dbias != nullptr;
-    a.lists = table ? grad_lists(op) : op->rows;
-    a.parts = table ? (uint32_t)grad_parts(op, a.lists, a.l.segments) : 1;
-    a.dbias = a.parts > 1 ? ws : dbias;
-    const dim3 grid((unsigned)(a.lists * a.parts * a.l.segments));
-    if (op->history && op->repetition != 1.0f)  // the slopes need the repeats
-        FL_LAUNCH("k_logits_grad", (k_logits_grad<T, NT, VPT, SOFTMAX, true, WHOLE>), grid, dim3(NT), 0, st, a);
-    else
-        FL_LAUNCH("k_logits_grad", (k_logits_grad<T, NT, VPT, SOFTMAX, false, WHOLE>), grid, dim3(NT), 0, st, a);
-    if (a.parts > 1) {
-        const int64_t n = op->bias_rows * op->cols;
-        FL_LAUNCH("k_logits_parts", k_logits_parts, dim3((unsigned)(lg_ceil(n, 256) < 8192 ? lg_ceil(n, 256) : 8192)),
-                  dim3(256), 0, st, ws, (int)a.parts, n, dbias);
+template <typename T, int VPT, bool SOFTMAX>
+void launch_rows_grad(hipStream_t st, const GradArgs &a) {
+    const fl_logits &op = a.l.op;
+    const int waves = a.dbias ? LG_WAVES : row_waves(op.rows);
+    const dim3 grid((unsigned)(a.dbias ? a.lists * a.parts : lg_ceil(op.rows, waves))), nt(waves * FL_WAVE);
+    if (op.history && op.repetition != 1.0f)  // the slopes need the repeats
+        FL_LAUNCH("k_logits_rows_grad", (k_logits_rows_grad<T, VPT, SOFTMAX, true>), grid, nt, 0, st, a);
+    else FL_LAUNCH("k_logits_rows_grad", (k_logits_rows_grad<T, VPT, SOFTMAX, false>), grid, nt, 0, st, a);
+}
+
+template <typename T, int VPT, bool SOFTMAX, bool WHOLE>
+void launch_seg_grad(hipStream_t st, const GradArgs &a) {
+    const fl_logits &op = a.l.op;
+    const dim3 grid((unsigned)((a.dbias ? a.lists * a.parts : op.rows) * a.l.segments)), nt(LG_NT);
+    if (op.history && op.repetition != 1.0f)
+        FL_LAUNCH("k_logits_seg_grad", (k_logits_seg_grad<T, VPT, SOFTMAX, true, WHOLE>), grid, nt, 0, st, a);
+    else FL_LAUNCH("k_logits_seg_grad", (k_logits_seg_grad<T, VPT, SOFTMAX, false, WHOLE>), grid, nt, 0, st, a);
+}
+
+// The gradient's workspace: the parts of dbias, the segments' dots and the
+// rows' (long softmax), and the owners by group.
+struct GradSpace {
+    size_t parts, dots, order, offsets, group, group_bytes, bytes;
+};
+
+GradSpace grad_space(const fl_logits *op, bool softmax, bool with_dbias) {
+    GradSpace s{};
+    const auto take = [&](size_t n) {
+        const size_t at = s.bytes;
+        s.bytes += (n + 255) / 256 * 256;
+        return at;
+    };
+    const int64_t segments = grad_segments(op, softmax);
+    if (with_dbias) {
+        const int parts = grad_parts(op, grad_lists(op), segments);
+        if (parts > 1) s.parts = take((size_t)parts * op->bias_rows * op->cols * 4);
+        if (op->bias_rows > 1) {
+            const int64_t owners = op->rows / op->inner;
+            s.order = take((size_t)owners * 4 + 4);
+            s.offsets = take((size_t)(op->bias_rows + 1) * 4);
+            s.group_bytes = fl_group_rows_bytes(owners, op->bias_rows);
+            s.group = take(s.group_bytes);
+        }
     }
+    if (softmax && op->cols > LG_LONG) s.dots = take((size_t)op->rows * (segments + 1) * 4);
+    return s;
 }
 
 template <typename T, bool SOFTMAX>
-int gradient(hipStream_t st, GradArgs &a, const fl_logits *op, float *dbias, float *ws, const char *what) {
-    const int64_t seg = seg_cols(op->cols, SOFTMAX);
-    if (seg == 256) launch_grad<T, 64, 1, SOFTMAX, true>(st, a, op, dbias, ws);
-    else if (seg == 1024) launch_grad<T, 256, 1, SOFTMAX, true>(st, a, op, dbias, ws);
-    else if (seg == 2048) launch_grad<T, 256, 2, SOFTMAX, true>(st, a, op, dbias, ws);
-    else if constexpr (!SOFTMAX) launch_grad<T, 256, LG_SEG_VPT, false, true>(st, a, op, dbias, ws);
-    else if (seg == LG_LONG) launch_grad<T, 256, LG_LONG / 1024, true, true>(st, a, op, dbias, ws);
-    else launch_grad<T, 256, LG_SEG_VPT, true, false>(st, a, op, dbias, ws);
-    return fl_check_launch(what);
-}
-
-// Floats of workspace: the parts of dbias, then (long softmax) the segments'
-// dots and the rows'.
-size_t grad_floats(const fl_logits *op, int softmax, int with_dbias, int64_t *dots_at) {
-    const int64_t segments = lg_ceil(op->cols, seg_cols(op->cols, softmax != 0));
-    size_t n = 0;
-    if (with_dbias) {
-        const int parts = grad_parts(op, grad_lists(op), segments);
-        if (parts > 1) n += (size_t)parts * op->bias_rows * op->cols;
+int gradient(hipStream_t st, const fl_logits *op, const float *w, const void *grad, void *dx, float *dbias, char *ws) {
+    const GradSpace sp = grad_space(op, SOFTMAX, dbias != nullptr);
+    GradArgs a{};
+    a.l = lg_args(op, LG_SEG);
+    a.l.segments = (uint32_t)grad_segments(op, SOFTMAX);
+    a.g = grad;
+    a.w = w;
+    a.dx = dx;
+    a.parts = 1;
+    if (dbias) {
+        a.lists = grad_lists(op);
+        a.parts = (uint32_t)grad_parts(op, a.lists, a.l.segments);
+        a.dbias = a.parts > 1 ? (float *)(ws + sp.parts) : dbias;
+        if (op->bias_rows > 1) {
+            int32_t *order = (int32_t *)(ws + sp.order), *offsets = (int32_t *)(ws + sp.offsets);
+            const int rc = fl_group_rows(st, op->group, op->rows / op->inner, op->bias_rows, order, offsets, nullptr,
+                                         ws + sp.group, sp.group_bytes);
+            if (rc) return rc;
+            a.order = order;
+            a.offsets = offsets;
+        }
+    } else if (op->rows == 0) return FL_OK;
+    if (SOFTMAX && op->cols > LG_LONG && op->rows > 0) {
+        float *part = (float *)(ws + sp.dots), *dots = part + op->rows * a.l.segments;
+        FL_LAUNCH("k_logits_dot", k_logits_dot, dim3((unsigned)(op->rows * a.l.segments)), dim3(LG_NT), 0, st, a.l,
+                  (const float *)grad, w, part);
+        FL_LAUNCH("k_logits_join", k_logits_join, dim3((unsigned)op->rows), dim3(FL_WAVE), 0, st, part,
+                  (int64_t)a.l.segments, dots);
+        a.dots = dots;
     }
-    *dots_at = (int64_t)n;
-    if (softmax && lg_long(op->cols)) n += (size_t)op->rows * (segments + 1);
-    return n;
+    if (op->cols <= 256) launch_rows_grad<T, 1, SOFTMAX>(st, a);
+    else if (op->cols <= 512) launch_rows_grad<T, 2, SOFTMAX>(st, a);
+    else if (op->cols <= 1024) launch_rows_grad<T, 4, SOFTMAX>(st, a);
+    else if (op->cols <= LG_WAVE_COLS) launch_rows_grad<T, 8, SOFTMAX>(st, a);
+    else if constexpr (!SOFTMAX) launch_seg_grad<T, LG_VPT, false, true>(st, a);
+    else if (op->cols <= LG_LONG) launch_seg_grad<T, LG_LONG / LG_NT / 4, true, true>(st, a);
+    else launch_seg_grad<T, LG_VPT, true, false>(st, a);
+    if (a.parts > 1) fold_parts<float>(st, a.dbias, (int)a.parts, op->bias_rows * op->cols, dbias);
+    return fl_check_launch("logits_grad");
 }
 
 }  // namespace
@@ -559,13 +809,13 @@ int fl_logits_constrain(void *stream, const fl_logits *op, void *out) {
     if (rc) return rc;
     if (op->rows == 0 || op->cols == 0) return FL_OK;
     if (!out) return fl::fl_fail(FL_ERR_ARG, "logits_constrain: null pointer");
-    FL_BY_TYPE(op->dtype, (fl::forward<T, fl::LG_CONSTRAIN>((hipStream_t)stream, op, out, nullptr,
+    FL_BY_TYPE(op->dtype, (fl::forward<T, false>((hipStream_t)stream, op, out, nullptr,
                                                             "logits_constrain")))
 }
 
 size_t fl_logits_softmax_bytes(const fl_logits *op) {
-    if (!op || !fl::lg_long(op->cols)) return 0;
-    return (size_t)op->rows * fl::lg_ceil(op->cols, 256 * 4 * fl::LG_SEG_VPT) * sizeof(float2);
+    if (!op || op->cols <= fl::LG_LONG || op->rows < 1) return 0;
+    return (size_t)op->rows * fl::lg_ceil(op->cols, fl::LG_SEG) * sizeof(float2);
 }
 
 int fl_logits_softmax(void *stream, const fl_logits *op, float *w, void *ws, size_t ws_bytes) {
@@ -575,51 +825,30 @@ int fl_logits_softmax(void *stream, const fl_logits *op, float *w, void *ws, siz
     if (!w) return fl::fl_fail(FL_ERR_ARG, "logits_softmax: null pointer");
     const size_t need = fl_logits_softmax_bytes(op);
     if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "logits_softmax: workspace too small");
-    FL_BY_TYPE(op->dtype, (fl::forward<T, fl::LG_SOFTMAX>((hipStream_t)stream, op, w, (float2 *)ws,
+    FL_BY_TYPE(op->dtype, (fl::forward<T, true>((hipStream_t)stream, op, w, (float2 *)ws,
                                                           "logits_softmax")))
 }
 
 size_t fl_logits_grad_bytes(const fl_logits *op, int softmax, int with_dbias) {
-    if (!op || op->rows < 1 || op->cols < 1) return 0;
-    int64_t at;
-    return fl::grad_floats(op, softmax, with_dbias, &at) * 4;
+    if (!op || op->rows < 0 || op->cols < 1 || op->inner < 1) return 0;
+    return fl::grad_space(op, softmax != 0, with_dbias != 0 && op->bias && op->bias_rows > 0).bytes;
 }
 
-int fl_logits_grad(void *stream, const fl_logits *op, const float *w, const void *grad, const int32_t *order,
-                   const int32_t *offsets, void *dx, float *dbias, void *ws, size_t ws_bytes) {
+int fl_logits_grad(void *stream, const fl_logits *op, const float *w, const void *grad, void *dx, float *dbias,
+                   void *ws, size_t ws_bytes) {
     const int rc = fl::lg_check(op, "logits_grad");
     if (rc) return rc;
     if (op->cols == 0) return FL_OK;
-    if (dbias && (!op->bias || (op->bias_rows > 1 && (!order || !offsets))))
-        return fl::fl_fail(FL_ERR_ARG, "logits_grad: the gradient of a bias table needs the owners by group");
+    if (dbias && !op->bias) return fl::fl_fail(FL_ERR_ARG, "logits_grad: the gradient of no bias table");
     if (op->rows > 0 && !grad) return fl::fl_fail(FL_ERR_ARG, "logits_grad: null pointer");
     const size_t need = fl_logits_grad_bytes(op, w != nullptr, dbias != nullptr);
     if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "logits_grad: workspace too small");
-    if (op->rows == 0 && !dbias) return FL_OK;
+    if ((uintptr_t)ws % 16) return fl::fl_fail(FL_ERR_ARG, "logits_grad: workspace must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
-    fl::GradArgs a{};
-    a.g = grad;
-    a.w = w;
-    a.dx = dx;
-    if (dbias && op->bias_rows > 1) {
-        a.order = order;
-        a.offsets = offsets;
-    }
-    if (w && fl::lg_long(op->cols) && op->rows > 0) {
-        int64_t at;
-        fl::grad_floats(op, 1, dbias != nullptr, &at);
-        const fl::LogitArgs l = fl::lg_args(op, 256 * 4 * fl::LG_SEG_VPT);
-        float *part = (float *)ws + at, *dots = part + op->rows * l.segments;
-        FL_LAUNCH("k_logits_dot", (fl::k_logits_dot<256, fl::LG_SEG_VPT>), dim3((unsigned)(op->rows * l.segments)),
-                  dim3(256), 0, st, l, (const float *)grad, w, part);
-        FL_LAUNCH("k_logits_join", fl::k_logits_join, dim3((unsigned)op->rows), dim3(FL_WAVE), 0, st, part,
-                  (int64_t)l.segments, dots);
-        a.dots = dots;
-    }
     if (w) {
-        FL_BY_TYPE(op->dtype, (fl::gradient<T, true>(st, a, op, dbias, (float *)ws, "logits_grad")))
+        FL_BY_TYPE(op->dtype, (fl::gradient<T, true>(st, op, w, grad, dx, dbias, (char *)ws)))
     }
-    FL_BY_TYPE(op->dtype, (fl::gradient<T, false>(st, a, op, dbias, (float *)ws, "logits_grad")))
+    FL_BY_TYPE(op->dtype, (fl::gradient<T, false>(st, op, w, grad, dx, dbias, (char *)ws)))
 }
 
 }  // extern "C"

@@ -925,12 +925,11 @@ int fl_logits_softmax(void *stream, const fl_logits *op, float *w, void *ws,
                       size_t ws_bytes);
 /* Gradients of fl_logits_constrain (w null, grad of x's type) or of
  * fl_logits_softmax (w its output, grad fp32): dx [rows, cols] of x's type,
- * or null, and dbias [bias_rows, cols], or null.  order, offsets: the owners
- * grouped by group (fl_group_rows), for a dbias of several rows. */
+ * or null, and dbias [bias_rows, cols], or null.  grad contiguous; ws on a
+ * 16-byte boundary. */
 size_t fl_logits_grad_bytes(const fl_logits *op, int softmax, int with_dbias);
 int fl_logits_grad(void *stream, const fl_logits *op, const float *w,
-                   const void *grad, const int32_t *order,
-                   const int32_t *offsets, void *dx, float *dbias, void *ws,
+                   const void *grad, void *dx, float *dbias, void *ws,
                    size_t ws_bytes);
 
 #ifdef __cplusplus

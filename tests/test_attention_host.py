@@ -104,12 +104,12 @@ def test_logits_arguments():
     long = _logits_op(cols=20000, ldx=20000)
     need = lib.fl_logits_softmax_bytes(long)
     assert need > 0 and "workspace" in _error(lib.fl_logits_softmax(None, long, one, one, need - 1))
-    table = _logits_op(bias=1, bias_rows=2, group=1)
-    assert "group" in _error(lib.fl_logits_grad(None, table, None, one, None, None, one, one, None, 0))
-    assert "null" in _error(lib.fl_logits_grad(None, _logits_op(), None, None, None, None, one, None, None, 0))
-    many = _logits_op(rows=100_000, bias=1, bias_rows=1)
-    need = lib.fl_logits_grad_bytes(many, 0, 1)
-    assert need > 0 and "workspace" in _error(lib.fl_logits_grad(None, many, None, one, None, None, one, one, one,
-                                                                  need - 1))
+    back = lambda op, w, g, dx, db, ws, n: _error(lib.fl_logits_grad(None, op, w, g, dx, db, ws, n))
+    assert "bias" in back(_logits_op(), None, one, one, one, None, 0)
+    assert "null" in back(_logits_op(), None, None, one, None, None, 0)
+    for op in (_logits_op(rows=100_000, bias=1, bias_rows=1), _logits_op(bias=1, bias_rows=2, group=1)):
+        need = lib.fl_logits_grad_bytes(op, 0, 1)
+        assert need > 0 and "workspace" in back(op, None, one, one, one, one, need - 1)
+        assert "aligned" in back(op, None, one, one, one, one, need)
     assert "shape" in _error(lib.fl_pack_bits(None, one, -1, 3, one))
     assert lib.fl_logits_constrain(None, _logits_op(rows=0), None) == 0
