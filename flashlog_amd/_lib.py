@@ -265,7 +265,7 @@ _SIGS = {
     "fl_logits_softmax_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLogits)]),
     "fl_logits_softmax": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLogits)] + [ctypes.c_void_p] * 2 +
                           [ctypes.c_size_t]),
-    "fl_logits_grad_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLogits)] + [ctypes.c_int] * 2),
+    "fl_logits_grad_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLogits)] + [ctypes.c_int] * 3),
     "fl_logits_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLogits)] + [ctypes.c_void_p] * 5 +
                        [ctypes.c_size_t]),
     "fl_prof_enable": (ctypes.c_int, [ctypes.c_int]),

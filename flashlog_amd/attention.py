@@ -457,7 +457,7 @@ class _LogitsFunction(autograd.Function):
         db = torch.empty_like(bias) if need_b else None
         # without their signs the logits are not read: the gradient's rows stand for them
         op = c.op(x if x is not None else _rows_of(grad, c.cols), bias)
-        nbytes = lib.fl_logits_grad_bytes(op, ctx.softmax, need_b)
+        nbytes = lib.fl_logits_grad_bytes(op, ctx.softmax, need_x, need_b)
         ws = _workspace(nbytes, dev)
         _launch("hop_attention" if ctx.softmax else "constrain_logits", lib.fl_logits_grad, dev, op, _ptr(w),
                 grad.data_ptr(), _ptr(dx), _ptr(db), _ptr(ws), nbytes)

@@ -14,22 +14,24 @@
 //   sign of x + bias; dbias[g] = the sum of the dx of the group's rows
 //
 // All of it is one pass over the rows: HBM-bound, bytes = one read and one
-// write of the rows.  Rows of up to 2048 columns are a wave's each, held in
-// registers (up to 8 groups of 4 columns a lane), so that nothing waits for
-// other waves; longer ones are cut into segments of 4096 columns, a workgroup
-// each (the softmax: up to 8192 whole, beyond that the segments' maxima and
-// sums are joined by a second launch).
+// write of the rows.  A wave takes a row's segment of up to 2048 columns in
+// registers, 16 bytes a lane and load, so that nothing waits for other waves;
+// rows of up to 2048 columns are one segment, the softmax of longer ones
+// joins the segments' maxima and sums in a second launch.
 //
-// Masks are one bit a column.  Histories are short next to the rows: up to 8
-// ids are compared with the columns in registers, more are looked at first and
-// only a segment that holds some of them counts them in LDS (integers, so the
-// order does not matter); the slopes read the logits of repeated columns only.
+// Masks are one bit a column.  Histories are short next to the rows: a wave
+// looks at the ids 64 at a time, and every one that falls into its segment is
+// counted by the lane that holds the column (a byte each; rows with more than
+// 255 ids are counted in LDS, 16 bits each -- integers, so the order does not
+// matter).  The
+// slopes read the logits of repeated columns only.
 //
-// dbias adds fp32 terms in a fixed order.  A workgroup keeps one table row's
-// columns in registers and walks the group's rows, writing their dx on the
-// way (rows of up to 2048 columns: four waves, a row each, joined in LDS);
-// groups of many rows are cut into parts.  The terms are the unrounded ones,
-// so half-precision logits give the same dbias as fp32 ones.
+// dbias adds fp32 terms in a fixed order: of longer rows a wave keeps one
+// table row's segment in registers and walks the group's rows, writing their
+// dx on the way; of rows of one segment, where that leaves too few waves, the
+// terms are read back (fp32 dx as they are, of 16-bit logits a copy).  Groups
+// of many rows are cut into parts.  The terms are the unrounded ones, so
+// half-precision logits give the same dbias as fp32 ones.
 #include "fl_abi.h"
 #include "fl_common.h"
 #include "fl_parts.h"
@@ -38,36 +40,51 @@
 namespace fl {
 namespace {
 
-constexpr int LG_WAVE_COLS = 2048;  // longest row held by a wave
-constexpr int LG_LONG = 8192;       // longest row held by a workgroup
-constexpr int LG_NT = 256;
-constexpr int LG_WAVES = LG_NT / FL_WAVE;
-constexpr int LG_VPT = 4;           // groups of 4 columns a thread of a segment
-constexpr int LG_SEG = LG_NT * 4 * LG_VPT;
-constexpr int LG_FEW = 8;           // ids compared in registers
+constexpr int LG_SEG = 2048;  // columns of a wave
+constexpr int LG_WAVES = 4;   // of a workgroup
+constexpr int LG_NT = LG_WAVES * FL_WAVE;
 
-enum { LG_CONSTRAIN = 0, LG_SOFTMAX = 1, LG_STATS = 2, LG_JOINED = 3 };
-
+// Columns of a lane's load.
 template <typename T>
-struct Quad {
-    T v[4];
+constexpr int group_cols() {
+    return 16 / (int)sizeof(T);
+}
+
+template <typename U, int G>
+struct Group {
+    U v[G];
 };
-template <typename T>
-__device__ __forceinline__ Quad<T> load_quad(const T *p, int64_t left) {
-    Quad<T> r;
-    if (left >= 4) __builtin_memcpy(&r, p, sizeof(r));
-    else
+
+// Columns c .. c + G - 1 of a row of `cols`.  A group that the row ends in is
+// read from its last G columns and shifted; lanes behind the row read those
+// too and use nothing of it.
+template <typename U, int G>
+__device__ __forceinline__ Group<U, G> load_group(const U *row, int c, int cols) {
+    Group<U, G> r;
+    if (cols < G) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r.v[e] = e < left ? p[e] : (T)0.0f;
+        for (int e = 0; e < G; ++e) r.v[e] = c + e < cols ? row[c + e] : (U)0.0f;
+        return r;
+    }
+    const int at = c + G <= cols ? c : cols - G;
+    __builtin_memcpy(&r, reinterpret_cast<const char *>(row) + (uint32_t)at * (uint32_t)sizeof(U), sizeof(r));
+    const int shift = c - at < G ? c - at : 0;
+    if (__any(shift)) {
+#pragma unroll
+        for (int s = 1; s < G; s *= 2)
+            if (shift & s)
+#pragma unroll
+                for (int e = 0; e + s < G; ++e) r.v[e] = r.v[e + s];
+    }
     return r;
 }
-template <typename T>
-__device__ __forceinline__ void store_quad(T *p, const Quad<T> &r, int64_t left) {
-    if (left >= 4) __builtin_memcpy(p, &r, sizeof(r));
+template <typename U, int G>
+__device__ __forceinline__ void store_group(U *row, int c, int cols, const Group<U, G> &r) {
+    if (c + G <= cols) __builtin_memcpy(reinterpret_cast<char *>(row) + (uint32_t)c * (uint32_t)sizeof(U), &r, sizeof(r));
     else
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < left) p[e] = r.v[e];
+        for (int e = 0; e < G; ++e)
+            if (c + e < cols) row[c + e] = r.v[e];
 }
 
 struct LogitArgs {
@@ -111,260 +128,210 @@ __device__ __forceinline__ RowView row_view(const fl_logits &op, int64_t row) {
     return r;
 }
 
-// Threads that share a row: a wave (nothing to wait for) or a workgroup.
-template <int NT>
-__device__ __forceinline__ void team_sync() {
-    if (NT == FL_WAVE) fl_wave_sync();
-    else __syncthreads();
-}
-template <int NT>
-__device__ __forceinline__ bool team_any(bool v) {
-    if (NT == FL_WAVE) return __any(v);
-    return __syncthreads_or(v);
-}
-template <int NT>
-__device__ __forceinline__ int team_thread() {
-    return NT == FL_WAVE ? fl_lane() : (int)threadIdx.x;
-}
-
-template <int NT>
-__device__ __forceinline__ float team_max(float v, float *red) {
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int o = FL_WAVE / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, FL_WAVE));
-    if (NT == FL_WAVE) return v;
-    if (fl_lane() == 0) red[fl_wave_id()] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < NT / FL_WAVE; ++w) v = fmaxf(v, red[w]);
-    __syncthreads();
     return v;
 }
 
-template <int NT>
-__device__ __forceinline__ float team_sum(float v, float *red) {
-    v = fl_wave_sum_f32(v);
-    if (NT == FL_WAVE) return v;
-    if (fl_lane() == 0) red[fl_wave_id()] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < NT / FL_WAVE; ++w) v += red[w];
-    __syncthreads();
-    return v;
-}
+// A wave's columns of a row: VPT groups of G a lane from column `base` on.
+template <int G, int VPT>
+struct Columns {
+    static constexpr int SEG = FL_WAVE * G * VPT;
+    static __device__ __forceinline__ int local(int i) { return (i * FL_WAVE + fl_lane()) * G; }
 
-// How often the row's history holds the columns [base, base + SEG).
-template <int NT, int SEG>
-struct Repeats {
-    enum { NONE, FEW, BYTES, WORDS };
-    int mode;
-    int rel[LG_FEW];  // FEW: the ids' places in the segment, far below it for those outside
-    const int *cnt;   // BYTES: a byte a column; WORDS: a word
-
-    // lds: SEG words of the team.
-    __device__ __forceinline__ void begin(const RowView &r, int64_t base, int64_t cols, int *lds) {
-        const int64_t end = base + SEG < cols ? base + SEG : cols;
-        const int t = team_thread<NT>();
-        cnt = lds;
-        mode = NONE;
-        if (r.nids <= LG_FEW) {
-            if (r.nids == 0) return;
-            mode = FEW;
-#pragma unroll
-            for (int k = 0; k < LG_FEW; ++k) {
-                const int64_t id = k < r.nids ? r.ids[k] : -1;
-                rel[k] = id >= base && id < end ? (int)(id - base) : -8;
-            }
-            return;
-        }
-        bool hit = false;
-        for (int64_t i = t; i < r.nids; i += NT) {
-            const int64_t id = r.ids[i];
-            hit |= id >= base && id < end;
-        }
-        if (!team_any<NT>(hit)) return;  // (behind it the last row's counts are read)
-        const bool bytes = r.nids <= 255;
-        mode = bytes ? BYTES : WORDS;
-        const int words = bytes ? SEG / 4 : SEG;
-        for (int i = t; i < words; i += NT) lds[i] = 0;
-        team_sync<NT>();
-        for (int64_t i = t; i < r.nids; i += NT) {
-            const int64_t id = r.ids[i];
-            if (id >= base && id < end) {
-                const int c = (int)(id - base);
-                if (bytes) atomicAdd(&lds[c >> 2], 1 << (8 * (c & 3)));
-                else atomicAdd(&lds[c], 1);
-            }
-        }
-        team_sync<NT>();
-    }
-    // The counts of the columns local .. local + 3; whether any is not 0.
-    __device__ __forceinline__ bool quad(int local, int (&c)[4]) const {
-        if (mode == NONE) return false;
-        if (mode == WORDS) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[e] = cnt[local + e];
-            return (c[0] | c[1] | c[2] | c[3]) != 0;
-        }
-        unsigned w = 0;
-        if (mode == BYTES) w = (unsigned)cnt[local >> 2];
-        else
-#pragma unroll
-            for (int k = 0; k < LG_FEW; ++k) {
-                const unsigned d = (unsigned)(rel[k] - local);
-                w += d < 4 ? 1u << (8 * d) : 0u;
-            }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = (int)((w >> (8 * e)) & 255u);
-        return w != 0;
+    // The allowed bits of the lane's i-th group (those of columns below cols).
+    static __device__ __forceinline__ unsigned bits(const RowView &r, int c, int cols) {
+        if (c >= cols || r.none) return 0;
+        const unsigned all = (1u << G) - 1;
+        const unsigned b = r.allowed ? (r.allowed[c >> 5] >> (c & 31)) & all : all;
+        return cols - c < G ? b & ((1u << (cols - c)) - 1) : b;
     }
 };
 
-// The allowed bits of columns c .. c + 3 (those below cols).
-__device__ __forceinline__ unsigned quad_bits(const RowView &r, int64_t c, int64_t cols) {
-    if (c >= cols || r.none) return 0;
-    unsigned b = r.allowed ? (r.allowed[c >> 5] >> (c & 31)) & 15u : 15u;
-    return cols - c < 4 ? b & ((1u << (cols - c)) - 1) : b;
-}
+// How often the row's history holds the wave's columns.
+template <int G, int VPT>
+struct Repeats {
+    using C = Columns<G, VPT>;
+    using Pack = std::conditional_t<G == 4, uint32_t, uint64_t>;
+    Pack pack[VPT];         // a byte a column
+    const uint32_t *halves;  // rows with more ids than a byte counts: LDS, 16 bits a column of the wave
 
-// A row's segment in a team's registers: the constrained values v and the
-// allowed bits.
-template <typename T, int NT, int VPT, bool HIST>
-struct Segment {
-    static constexpr int SEG = NT * 4 * VPT;
-    float v[VPT][4];
-    unsigned ok;
-
-    static __device__ __forceinline__ int local(int i) { return (i * NT + team_thread<NT>()) * 4; }
-
-    __device__ __forceinline__ void load(const LogitArgs &a, int64_t row, int64_t base, int *cnt) {
-        const int64_t cols = a.op.cols;
-        const RowView r = row_view(a.op, row);
-        const T *x = (const T *)a.op.x + row * a.op.ldx;
-        Quad<T> q[VPT];
-        ok = 0;
+    // head: this lane's id of the first 64.
+    __device__ __forceinline__ void count(const RowView &r, int64_t head, int base, int cols, uint32_t *lds) {
+        const int end = cols - base < C::SEG ? cols : base + C::SEG;
+        halves = nullptr;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t c = base + local(i);
-            if (c < cols) q[i] = load_quad(x + c, cols - c);
-            ok |= quad_bits(r, c, cols) << (4 * i);
-        }
-        Repeats<NT, SEG> rep;
-        if (HIST) rep.begin(r, base, cols, cnt);
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t c = base + local(i);
-            if (c >= cols) continue;
-            Quad<float> b{{0, 0, 0, 0}};
-            if (r.bias) b = load_quad(r.bias + c, cols - c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] = (float)q[i].v[e] + b.v[e];
-            int n[4];
-            if (HIST && rep.quad(local(i), n)) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n[e] > 0) {
-                        v[i][e] *= v[i][e] > 0.0f ? a.inv_repetition : a.op.repetition;
-                        v[i][e] -= a.op.presence + a.op.frequency * (float)n[e];
-                    }
+        for (int i = 0; i < VPT; ++i) pack[i] = 0;
+        if (r.nids > 255) {
+            halves = lds;
+            fl_wave_sync();  // the last row's counts are read
+            for (int i = fl_lane(); i < C::SEG / 2; i += FL_WAVE) lds[i] = 0;
+            fl_wave_sync();
+            for (int64_t j = fl_lane(); j < r.nids; j += FL_WAVE) {
+                const int64_t id = r.ids[j];
+                if (id >= base && id < end) {
+                    const int c = (int)(id - base), up = 16 * (c & 1);
+                    // at most 64 more a turn: a column that has come up 65000 times is counted no further
+                    if (((volatile uint32_t *)lds)[c >> 1] >> up << 16 < 65000u << 16) atomicAdd(&lds[c >> 1], 1u << up);
+                }
             }
+            fl_wave_sync();
+            return;
+        }
+        for (int j = 0; j < (int)r.nids; j += FL_WAVE) {
+            const int64_t id = j == 0 ? head : j + fl_lane() < (int)r.nids ? r.ids[j + fl_lane()] : -1;
+            const int o = (int)(id - base);
+            unsigned long long m = __ballot(id >= base && id < end);
+            while (m) {
+                const int at = __builtin_amdgcn_readlane(o, __builtin_ctzll(m));
+                m &= m - 1;
+                const Pack one = fl_lane() == (at / G) % FL_WAVE ? (Pack)1 << (8 * (at % G)) : (Pack)0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] *= a.inv_temperature;
+                for (int i = 0; i < VPT; ++i)
+                    if (at / (G * FL_WAVE) == i) pack[i] += one;
+            }
         }
     }
-    __device__ __forceinline__ bool allowed(int i, int e) const { return (ok >> (4 * i + e)) & 1; }
-    __device__ __forceinline__ float largest(float *red) const {
+    __device__ __forceinline__ bool any(int i) const {
+        if (halves) {
+            uint32_t n = 0;
+#pragma unroll
+            for (int e = 0; e < G; e += 2) n |= halves[(C::local(i) + e) / 2];
+            return n != 0;
+        }
+        return pack[i] != 0;
+    }
+    __device__ __forceinline__ int at(int i, int e) const {
+        if (halves) return (int)(halves[(C::local(i) + e) / 2] >> (16 * (e & 1))) & 0xffff;
+        return (int)((pack[i] >> (8 * e)) & 255);
+    }
+};
+
+// This lane's id of the first 64 of the row's history.
+__device__ __forceinline__ int64_t head_id(const RowView &r) {
+    return fl_lane() < r.nids && r.nids <= 255 ? r.ids[fl_lane()] : -1;
+}
+
+// The constrained values v of a wave's segment and their allowed bits.
+template <typename T, int VPT, bool HIST>
+struct Segment : Columns<group_cols<T>(), VPT> {
+    static constexpr int G = group_cols<T>();
+    using C = Columns<G, VPT>;
+    float v[VPT][G];
+    unsigned ok[VPT];
+
+    __device__ __forceinline__ void load(const LogitArgs &a, int64_t row, int base, uint32_t *lds) {
+        const int cols = (int)a.op.cols;
+        const RowView r = row_view(a.op, row);
+        const T *x = (const T *)a.op.x + row * a.op.ldx;
+        Group<T, G> q[VPT];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) q[i] = load_group<T, G>(x, base + C::local(i), cols);
+        Repeats<G, VPT> rep;
+        if (HIST) rep.count(r, head_id(r), base, cols, lds);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = base + C::local(i);
+            ok[i] = C::bits(r, c, cols);
+#pragma unroll
+            for (int e = 0; e < G; ++e) v[i][e] = (float)q[i].v[e];
+            if (r.bias) {
+                const Group<float, G> b = load_group<float, G>(r.bias, c, cols);
+#pragma unroll
+                for (int e = 0; e < G; ++e) v[i][e] += b.v[e];
+            }
+            if (HIST && rep.any(i)) {
+#pragma unroll
+                for (int e = 0; e < G; ++e) {
+                    const int n = rep.at(i, e);
+                    if (n > 0) {
+                        v[i][e] *= v[i][e] > 0.0f ? a.inv_repetition : a.op.repetition;
+                        v[i][e] -= a.op.presence + a.op.frequency * (float)n;
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < G; ++e) v[i][e] *= a.inv_temperature;
+        }
+    }
+    __device__ __forceinline__ bool allowed(int i, int e) const { return (ok[i] >> e) & 1; }
+    __device__ __forceinline__ float largest() const {
         float m = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < G; ++e)
                 if (allowed(i, e)) m = fmaxf(m, v[i][e]);
-        return team_max<NT>(m, red);
+        return wave_max(m);
     }
-    // v = exp(v - shift) where allowed, 0 elsewhere; this thread's sum.
+    // v = exp(v - shift) where allowed, 0 elsewhere; their sum.
     __device__ __forceinline__ float exponentials(float shift) {
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < G; ++e) {
                 v[i][e] = allowed(i, e) ? expf(v[i][e] - shift) : 0.0f;
                 s += v[i][e];
             }
-        return s;
+        return fl_wave_sum_f32(s);
     }
-    __device__ __forceinline__ void store_weights(float *y, int64_t base, int64_t cols, float inv) const {
+    __device__ __forceinline__ void store_weights(float *y, int base, int cols, float inv) const {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int64_t c = base + local(i);
-            if (c < cols)
-                store_quad(y + c, Quad<float>{{v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv}}, cols - c);
+            Group<float, G> q;
+#pragma unroll
+            for (int e = 0; e < G; ++e) q.v[e] = v[i][e] * inv;
+            store_group<float, G>(y, base + C::local(i), cols, q);
         }
     }
-    __device__ __forceinline__ void store_values(T *y, int64_t base, int64_t cols, float fill) const {
+    __device__ __forceinline__ void store_values(T *y, int base, int cols, float fill) const {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int64_t c = base + local(i);
-            if (c >= cols) continue;
-            Quad<T> q;
+            Group<T, G> q;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) q.v[e] = (T)(allowed(i, e) ? v[i][e] : fill);
-            store_quad(y + c, q, cols - c);
+            for (int e = 0; e < G; ++e) q.v[e] = (T)(allowed(i, e) ? v[i][e] : fill);
+            store_group<T, G>(y, base + C::local(i), cols, q);
         }
     }
 };
 
-// Forward of rows held whole by a wave (NT = 64: a wave each) or a workgroup.
-template <typename T, int NT, int VPT, bool SOFTMAX, bool HIST>
-__global__ __launch_bounds__(LG_NT) void k_logits_rows(LogitArgs a, void *out) {
-    using Seg = Segment<T, NT, VPT, HIST>;
-    __shared__ float red[LG_WAVES];
-    __shared__ int cnt[HIST ? LG_NT / NT : 1][HIST ? Seg::SEG : 1];
-    const int team = NT == FL_WAVE ? fl_wave_id() : 0;
-    const int64_t row = NT == FL_WAVE ? (int64_t)blockIdx.x * (blockDim.x / FL_WAVE) + team : (int64_t)blockIdx.x;
-    if (row >= a.op.rows) return;  // NT = 64: no workgroup barriers
-    const int64_t cols = a.op.cols;
-    Seg s;
-    s.load(a, row, 0, cnt[HIST ? team : 0]);
-    if constexpr (!SOFTMAX) {
-        s.store_values((T *)out + row * cols, 0, cols, a.op.fill);
-    } else {
-        const float m = s.largest(red);
-        const float sum = team_sum<NT>(s.exponentials(m == -__builtin_inff() ? 0.0f : m), red);
-        s.store_weights((float *)out + row * cols, 0, cols, 1.0f / (sum == 0.0f ? 1.0f : sum));
-    }
-}
+enum { LG_CONSTRAIN = 0, LG_SOFTMAX = 1, LG_STATS = 2, LG_JOINED = 3 };
 
-// Forward of one segment of a longer row.  LG_STATS: its maximum and sum;
-// LG_JOINED: the softmax with the row's joined ones.
-template <typename T, int MODE, bool HIST>
-__global__ __launch_bounds__(LG_NT) void k_logits_seg(LogitArgs a, void *out, float2 *stats) {
-    using Seg = Segment<T, LG_NT, LG_VPT, HIST>;
-    __shared__ float red[LG_WAVES];
-    __shared__ int cnt[HIST ? LG_SEG : 1];
-    const int64_t cols = a.op.cols, row = blockIdx.x / a.segments;
-    const int64_t base = (int64_t)(blockIdx.x % a.segments) * LG_SEG;
+// Forward of a wave's segment.  LG_SOFTMAX: it is the row.  LG_STATS: its
+// maximum and sum; LG_JOINED: the softmax with the row's joined ones.
+template <typename T, int VPT, int MODE, bool HIST>
+__global__ __launch_bounds__(LG_NT) void k_logits(LogitArgs a, void *out, float2 *stats) {
+    using Seg = Segment<T, VPT, HIST>;
+    __shared__ uint32_t words[HIST ? LG_WAVES : 1][HIST ? Seg::SEG / 2 : 1];
+    const uint32_t item = blockIdx.x * (blockDim.x / FL_WAVE) + fl_wave_id();
+    const int64_t row = item / a.segments, cols = a.op.cols;
+    const int base = (int)(item % a.segments) * Seg::SEG;
+    if (row >= a.op.rows) return;
     Seg s;
-    s.load(a, row, base, cnt);
+    s.load(a, row, base, words[HIST ? fl_wave_id() : 0]);
     if constexpr (MODE == LG_CONSTRAIN) {
-        s.store_values((T *)out + row * cols, base, cols, a.op.fill);
-    } else if constexpr (MODE == LG_STATS) {
-        const float m = s.largest(red);
-        const float sum = team_sum<LG_NT>(s.exponentials(m == -__builtin_inff() ? 0.0f : m), red);
-        // a segment of nothing but NaN keeps its sum: a maximum of 0 lets it through
-        if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(m == -__builtin_inff() && sum != sum ? 0.0f : m, sum);
-    } else {
+        s.store_values((T *)out + row * cols, base, (int)cols, a.op.fill);
+    } else if constexpr (MODE == LG_JOINED) {
         const float2 *st = stats + row * a.segments;
         float m = -__builtin_inff(), sum = 0.0f;
-        for (uint32_t i = threadIdx.x; i < a.segments; i += LG_NT) m = fmaxf(m, st[i].x);
-        m = team_max<LG_NT>(m, red);
+        for (uint32_t i = fl_lane(); i < a.segments; i += FL_WAVE) m = fmaxf(m, st[i].x);
+        m = wave_max(m);
         if (m == -__builtin_inff()) m = 0.0f;
-        for (uint32_t i = threadIdx.x; i < a.segments; i += LG_NT) sum += st[i].y * expf(st[i].x - m);
-        sum = team_sum<LG_NT>(sum, red);
+        for (uint32_t i = fl_lane(); i < a.segments; i += FL_WAVE) sum += st[i].y * expf(st[i].x - m);
+        sum = fl_wave_sum_f32(sum);
         s.exponentials(m);
-        s.store_weights((float *)out + row * cols, base, cols, 1.0f / (sum == 0.0f ? 1.0f : sum));
+        s.store_weights((float *)out + row * cols, base, (int)cols, 1.0f / (sum == 0.0f ? 1.0f : sum));
+    } else {
+        const float m = s.largest();
+        const float sum = s.exponentials(m == -__builtin_inff() ? 0.0f : m);
+        if constexpr (MODE == LG_STATS) {
+            // a segment of nothing but NaN keeps its sum: a maximum of 0 lets it through
+            if (fl_lane() == 0) stats[item] = make_float2(m == -__builtin_inff() && sum != sum ? 0.0f : m, sum);
+        } else {
+            s.store_weights((float *)out + row * cols, base, (int)cols, 1.0f / (sum == 0.0f ? 1.0f : sum));
+        }
     }
 }
 
@@ -372,9 +339,10 @@ struct GradArgs {
     LogitArgs l;
     const void *g;        // gradient of the output (T; the softmax: float)
     const float *w;       // the softmax's output
-    const float *dots;    // [rows] sum w g, of rows longer than a workgroup holds
+    const float *dots;    // [rows] sum w g, of rows of several segments
     void *dx;
-    float *dbias;         // [parts][bias_rows][cols], or null: every row is a list of its own
+    float *terms;         // [rows, cols] fp32 terms of dbias (rows of one segment), or null
+    float *dbias;         // [parts][bias_rows][cols]
     const int32_t *order, *offsets;  // owners by group (null: one list of all)
     int64_t lists;        // row lists: groups and one of no group
     uint32_t parts;
@@ -398,191 +366,188 @@ struct RowList {
     }
 };
 
-// The gradient of a row's segment: what it reads, and its terms.
-template <typename T, int NT, int VPT, bool SOFTMAX, bool HIST>
+// What the gradient of a row's segment reads, and its terms.
+template <typename T, int VPT, bool SOFTMAX, bool HIST>
 struct GradSegment {
+    static constexpr int G = group_cols<T>();
+    using C = Columns<G, VPT>;
     using TG = std::conditional_t<SOFTMAX, float, T>;
-    static constexpr int SEG = NT * 4 * VPT;
-    Quad<TG> g[VPT];
-    Quad<float> w[SOFTMAX ? VPT : 1];
-    int64_t row;
+    Group<TG, G> g[VPT];
+    Group<float, G> w[SOFTMAX ? VPT : 1];
+    int64_t row, head;
+    RowView r;
 
-    static __device__ __forceinline__ int local(int i) { return (i * NT + team_thread<NT>()) * 4; }
-
-    __device__ __forceinline__ void load(const GradArgs &a, int64_t at, int64_t base) {
+    __device__ __forceinline__ void load(const GradArgs &a, int64_t at, int base) {
         row = at;
+        r = row_view(a.l.op, row);
         const int64_t cols = a.l.op.cols;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int64_t c = base + local(i);
-            if (c >= cols) continue;
-            g[i] = load_quad((const TG *)a.g + row * cols + c, cols - c);
-            if (SOFTMAX) w[i] = load_quad(a.w + row * cols + c, cols - c);
+            g[i] = load_group<TG, G>((const TG *)a.g + row * cols, base + C::local(i), (int)cols);
+            if (SOFTMAX) w[i] = load_group<float, G>(a.w + row * cols, base + C::local(i), (int)cols);
         }
+        if (HIST) head = head_id(r);
     }
     // Writes the row's dx and adds its terms to acc.
     template <bool WHOLE>
-    __device__ __forceinline__ void apply(const GradArgs &a, int64_t base, int *cnt, float *red, float (&acc)[VPT][4]) {
+    __device__ __forceinline__ void apply(const GradArgs &a, int base, uint32_t *lds, float (&acc)[VPT][G]) {
         const fl_logits &op = a.l.op;
-        const int64_t cols = op.cols;
-        const RowView r = row_view(op, row);
-        unsigned ok = 0;
+        const int cols = (int)op.cols;
+        unsigned ok[VPT];
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int64_t c = base + local(i);
-            const unsigned bits = quad_bits(r, c, cols);
-            ok |= bits << (4 * i);
-            if (SOFTMAX && WHOLE && c < cols)
+            ok[i] = C::bits(r, base + C::local(i), cols);
+            if (SOFTMAX && WHOLE)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s += (bits >> e) & 1 ? w[i].v[e] * (float)g[i].v[e] : 0.0f;
+                for (int e = 0; e < G; ++e) s += (ok[i] >> e) & 1 ? w[i].v[e] * (float)g[i].v[e] : 0.0f;
         }
-        Repeats<NT, SEG> rep;
-        if (HIST) rep.begin(r, base, cols, cnt);
-        if (SOFTMAX) s = WHOLE ? team_sum<NT>(s, red) : a.dots[row];
+        if (SOFTMAX) s = WHOLE ? fl_wave_sum_f32(s) : a.dots[row];
+        Repeats<G, VPT> rep;
+        if (HIST) rep.count(r, head, base, cols, lds);
         const T *x = (const T *)op.x + row * op.ldx;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int64_t c = base + local(i);
-            if (c >= cols) continue;
-            float u[4];
+            const int c = base + C::local(i);
+            float u[G];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < G; ++e) {
                 u[e] = SOFTMAX ? w[i].v[e] * ((float)g[i].v[e] - s) : (float)g[i].v[e];
                 u[e] *= a.l.inv_temperature;
             }
-            int n[4];
-            if (HIST && rep.quad(local(i), n)) {
+            if (HIST && rep.any(i)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n[e] > 0) {
+                for (int e = 0; e < G; ++e)
+                    if (rep.at(i, e) > 0 && c + e < cols) {
                         const float z = (float)x[c + e] + (r.bias ? r.bias[c + e] : 0.0f);
                         u[e] *= z > 0.0f ? a.l.inv_repetition : op.repetition;
                     }
             }
-            Quad<T> o;
+            Group<T, G> o;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                u[e] = (ok >> (4 * i + e)) & 1 ? u[e] : 0.0f;
+            for (int e = 0; e < G; ++e) {
+                u[e] = (ok[i] >> e) & 1 ? u[e] : 0.0f;
                 acc[i][e] += u[e];
                 o.v[e] = (T)u[e];
             }
-            if (a.dx) store_quad((T *)a.dx + row * cols + c, o, cols - c);
+            if (a.dx) store_group<T, G>((T *)a.dx + row * op.cols, c, cols, o);
+            if (a.terms) {
+                Group<float, G> f;
+#pragma unroll
+                for (int e = 0; e < G; ++e) f.v[e] = u[e];
+                store_group<float, G>(a.terms + row * op.cols, c, cols, f);
+            }
         }
     }
 };
 
-// Rows held whole by a wave.  Without dbias a wave takes one row; with it a
-// workgroup's waves take the rows of a list in turn, each loading its next
-// row while it works on one, and join their sums.
-template <typename T, int VPT, bool SOFTMAX, bool HIST>
-__global__ __launch_bounds__(LG_NT) void k_logits_rows_grad(GradArgs a) {
-    using Grad = GradSegment<T, FL_WAVE, VPT, SOFTMAX, HIST>;
-    constexpr int SEG = Grad::SEG;
-    __shared__ int cnt[HIST ? LG_WAVES : 1][HIST ? SEG : 1];
-    __shared__ float sums[SEG];
-    const int64_t cols = a.l.op.cols;
-    const int wave = fl_wave_id(), waves = blockDim.x / FL_WAVE;
-    int *mine = cnt[HIST ? wave : 0];
-    float acc[VPT][4];
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
-    if (!a.dbias) {
-        const int64_t row = (int64_t)blockIdx.x * waves + wave;
-        if (row >= a.l.op.rows) return;
-        Grad g;
-        g.load(a, row, 0);
-        g.template apply<true>(a, 0, mine, nullptr, acc);
-        return;
-    }
-    const int64_t list = blockIdx.x / a.parts;
-    const uint32_t part = blockIdx.x % a.parts;
-    const RowList rows(a, list, part);
+// Gradients of the rows: a wave a segment.  WHOLE: it is the row.
+template <typename T, int VPT, bool SOFTMAX, bool HIST, bool WHOLE>
+__global__ __launch_bounds__(LG_NT) void k_logits_grad(GradArgs a) {
+    using Grad = GradSegment<T, VPT, SOFTMAX, HIST>;
+    __shared__ uint32_t words[HIST ? LG_WAVES : 1][HIST ? Grad::C::SEG / 2 : 1];
+    const uint32_t item = blockIdx.x * (blockDim.x / FL_WAVE) + fl_wave_id();
+    const int64_t row = item / a.l.segments;
+    const int base = (int)(item % a.l.segments) * Grad::C::SEG;
+    if (row >= a.l.op.rows) return;
+    float acc[VPT][Grad::G] = {};
     Grad g;
-    if (rows.q0 + wave < rows.q1) g.load(a, rows.row(a, rows.q0 + wave), 0);
-    for (int64_t q = rows.q0 + wave; q < rows.q1; q += LG_WAVES) {
-        Grad next = g;
-        if (q + LG_WAVES < rows.q1) next.load(a, rows.row(a, q + LG_WAVES), 0);
-        g.template apply<true>(a, 0, mine, nullptr, acc);
-        g = next;
-    }
-    if (list >= a.l.op.bias_rows) return;
-    // in wave order
-    for (int w = 0; w < LG_WAVES; ++w) {
-        if (wave == w)
-#pragma unroll
-            for (int i = 0; i < VPT; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float *at = sums + Grad::local(i) + e;
-                    *at = w == 0 ? acc[i][e] : *at + acc[i][e];
-                }
-        __syncthreads();
-    }
-    float *b = a.dbias + ((int64_t)part * a.l.op.bias_rows + list) * cols;
-    for (int64_t c = threadIdx.x; c < cols; c += LG_NT) b[c] = sums[c];
+    g.load(a, row, base);
+    g.template apply<WHOLE>(a, base, words[HIST ? fl_wave_id() : 0], acc);
 }
 
-// One segment of the rows of a list (or of one row).  WHOLE: it is the row.
-template <typename T, int VPT, bool SOFTMAX, bool HIST, bool WHOLE>
-__global__ __launch_bounds__(LG_NT) void k_logits_seg_grad(GradArgs a) {
-    using Grad = GradSegment<T, LG_NT, VPT, SOFTMAX, HIST>;
-    __shared__ float red[LG_WAVES];
-    __shared__ int cnt[HIST ? Grad::SEG : 1];
+// Gradients of rows of several segments with dbias: a wave takes one segment
+// of all the rows of a list.  (Loading the next row's values ahead took 256
+// registers and was slower than the twice as many waves without.)
+template <typename T, int VPT, bool SOFTMAX, bool HIST>
+__global__ __launch_bounds__(LG_NT) void k_logits_table_grad(GradArgs a) {
+    using Grad = GradSegment<T, VPT, SOFTMAX, HIST>;
+    constexpr int G = Grad::G, SEG = Grad::C::SEG;
+    __shared__ uint32_t words[HIST ? LG_WAVES : 1][HIST ? SEG / 2 : 1];
     const int64_t cols = a.l.op.cols;
-    const uint32_t item = blockIdx.x / a.l.segments;
-    const int64_t base = (int64_t)(blockIdx.x % a.l.segments) * Grad::SEG;
-    float acc[VPT][4];
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
-    Grad g;
-    if (!a.dbias) {
-        g.load(a, item, base);
-        g.template apply<WHOLE>(a, base, cnt, red, acc);
-        return;
-    }
+    const uint32_t segments = (uint32_t)((cols + SEG - 1) / SEG);
+    uint32_t item = blockIdx.x * LG_WAVES + fl_wave_id();
+    const int base = (int)(item % segments) * SEG;
+    item /= segments;
     const uint32_t part = item % a.parts;
     const int64_t list = item / a.parts;
+    if (list >= a.lists) return;
+    float acc[VPT][G] = {};
     const RowList rows(a, list, part);
-    if (rows.q0 < rows.q1) g.load(a, rows.row(a, rows.q0), base);
     for (int64_t q = rows.q0; q < rows.q1; ++q) {
-        Grad next = g;
-        if (q + 1 < rows.q1) next.load(a, rows.row(a, q + 1), base);
-        g.template apply<WHOLE>(a, base, cnt, red, acc);
-        g = next;
+        Grad g;
+        g.load(a, rows.row(a, q), base);
+        g.template apply<false>(a, base, words[HIST ? fl_wave_id() : 0], acc);
     }
-    if (list >= a.l.op.bias_rows) return;
+    if (list >= a.l.op.bias_rows) return;  // the rows of no group
     float *b = a.dbias + ((int64_t)part * a.l.op.bias_rows + list) * cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        const int64_t c = base + Grad::local(i);
-        if (c < cols) store_quad(b + c, Quad<float>{{acc[i][0], acc[i][1], acc[i][2], acc[i][3]}}, cols - c);
+        Group<float, G> o;
+#pragma unroll
+        for (int e = 0; e < G; ++e) o.v[e] = acc[i][e];
+        store_group<float, G>(b, base + Grad::C::local(i), (int)cols, o);
     }
+}
+
+// dbias of rows of one segment, from their fp32 terms: four columns a thread,
+// the rows of a list (a part of them) in order.
+__global__ __launch_bounds__(LG_NT) void k_logits_sums(GradArgs a) {
+    const int64_t cols = a.l.op.cols;
+    const uint32_t blocks = (uint32_t)((cols + 4 * LG_NT - 1) / (4 * LG_NT)), item = blockIdx.x / blocks;
+    const int c = (int)((blockIdx.x % blocks) * LG_NT + threadIdx.x) * 4;
+    const uint32_t part = item % a.parts;
+    const int64_t list = item / a.parts;
+    if (c >= cols) return;
+    const RowList rows(a, list, part);
+    const float *terms = a.terms ? a.terms : (const float *)a.dx;  // fp32 dx are the terms themselves
+    float s[4] = {0, 0, 0, 0};
+    int64_t q = rows.q0;
+    for (; q + 4 <= rows.q1; q += 4) {
+        Group<float, 4> t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float *row = terms + rows.row(a, q + j) * cols;
+            if (c + 4 <= cols) __builtin_memcpy(&t[j], row + c, 16);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[j].v[e] = c + e < cols ? row[c + e] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += t[j].v[e];
+    }
+    for (; q < rows.q1; ++q) {
+        const float *row = terms + rows.row(a, q) * cols;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += c + e < cols ? row[c + e] : 0.0f;
+    }
+    float *b = a.dbias + ((int64_t)part * a.l.op.bias_rows + list) * cols;
+    store_group<float, 4>(b, c, (int)cols, Group<float, 4>{{s[0], s[1], s[2], s[3]}});
 }
 
 // sum w g of one segment of a row.
 __global__ __launch_bounds__(LG_NT) void k_logits_dot(LogitArgs a, const float *__restrict__ g,
                                                       const float *__restrict__ w, float *__restrict__ dots) {
-    __shared__ float red[LG_WAVES];
-    const int64_t cols = a.op.cols, row = blockIdx.x / a.segments;
-    const int64_t base = (int64_t)(blockIdx.x % a.segments) * LG_SEG;
+    using C = Columns<4, LG_SEG / FL_WAVE / 4>;
+    const uint32_t item = blockIdx.x * LG_WAVES + fl_wave_id();
+    const int64_t row = item / a.segments;
+    const int cols = (int)a.op.cols, base = (int)(item % a.segments) * LG_SEG;
+    if (row >= a.op.rows) return;
     const RowView r = row_view(a.op, row);
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < LG_VPT; ++i) {
-        const int64_t c = base + (i * LG_NT + threadIdx.x) * 4;
-        const unsigned bits = quad_bits(r, c, cols);
-        if (!bits) continue;
-        const Quad<float> p = load_quad(w + row * cols + c, cols - c), q = load_quad(g + row * cols + c, cols - c);
+    for (int i = 0; i < C::SEG / FL_WAVE / 4; ++i) {
+        const int c = base + C::local(i);
+        const unsigned bits = C::bits(r, c, cols);
+        const Group<float, 4> p = load_group<float, 4>(w + row * a.op.cols, c, cols);
+        const Group<float, 4> q = load_group<float, 4>(g + row * a.op.cols, c, cols);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s += (bits >> e) & 1 ? p.v[e] * q.v[e] : 0.0f;
     }
-    s = team_sum<LG_NT>(s, red);
-    if (threadIdx.x == 0) dots[blockIdx.x] = s;
+    s = fl_wave_sum_f32(s);
+    if (fl_lane() == 0) dots[item] = s;
 }
 
 __global__ __launch_bounds__(FL_WAVE) void k_logits_join(const float *__restrict__ part, int64_t segments,
@@ -622,54 +587,59 @@ int lg_check(const fl_logits *op, const char *what) {
         return fl_fail(FL_ERR_ARG, "%s: bad shape of the bias table", what);
     if (op->history && op->history_len < 0) return fl_fail(FL_ERR_ARG, "%s: bad shape of the history", what);
     if (op->rows > 0 && op->cols > 0 && !op->x) return fl_fail(FL_ERR_ARG, "%s: null pointer", what);
+    if (op->cols >= 1ll << 29) return fl_fail(FL_ERR_ARG, "%s: rows of fewer than 2^29 columns (shape)", what);
     if (op->cols && op->rows > 0x7fffffffll / lg_ceil(op->cols, LG_SEG))
         return fl_fail(FL_ERR_ARG, "%s: too many rows for one launch (shape)", what);
     return FL_OK;
 }
 
-LogitArgs lg_args(const fl_logits *op, int64_t seg) {
+int64_t segments_of(const fl_logits *op) { return lg_ceil(op->cols, LG_SEG); }
+
+LogitArgs lg_args(const fl_logits *op) {
     LogitArgs a;
     a.op = *op;
     if (!op->allowed) a.op.allowed_rows = 0;
     if (!op->bias) a.op.bias_rows = 0;
     a.inv_temperature = 1.0f / op->temperature;
     a.inv_repetition = 1.0f / op->repetition;
-    a.segments = (uint32_t)lg_ceil(op->cols, seg);
+    a.segments = (uint32_t)segments_of(op);
     return a;
 }
 
-// Waves of a workgroup whose waves take a row each: one where there are too
-// few rows to give every CU a workgroup of four.
-int row_waves(int64_t rows) { return rows < 1024 ? 1 : LG_WAVES; }
+// Waves of a workgroup whose waves work alone: one where there are too few to
+// give every CU a workgroup of four.
+int lone_waves(int64_t items) { return items < 1024 ? 1 : LG_WAVES; }
 
-template <typename T, int NT, int VPT, bool SOFTMAX>
-void launch_rows(hipStream_t st, const fl_logits *op, void *out) {
-    const LogitArgs a = lg_args(op, NT * 4 * VPT);
-    const int waves = NT == FL_WAVE ? row_waves(op->rows) : LG_WAVES;
-    const dim3 grid((unsigned)(NT == FL_WAVE ? lg_ceil(op->rows, waves) : op->rows)), nt(waves * FL_WAVE);
-    if (op->history) FL_LAUNCH("k_logits_rows", (k_logits_rows<T, NT, VPT, SOFTMAX, true>), grid, nt, 0, st, a, out);
-    else FL_LAUNCH("k_logits_rows", (k_logits_rows<T, NT, VPT, SOFTMAX, false>), grid, nt, 0, st, a, out);
+template <typename T, int VPT, int MODE>
+void launch(hipStream_t st, const fl_logits *op, void *out, float2 *stats) {
+    const LogitArgs a = lg_args(op);
+    const int64_t items = op->rows * a.segments;
+    const int waves = lone_waves(items);
+    const dim3 grid((unsigned)lg_ceil(items, waves)), nt(waves * FL_WAVE);
+    if (op->history) FL_LAUNCH("k_logits", (k_logits<T, VPT, MODE, true>), grid, nt, 0, st, a, out, stats);
+    else FL_LAUNCH("k_logits", (k_logits<T, VPT, MODE, false>), grid, nt, 0, st, a, out, stats);
 }
 
-template <typename T, int MODE>
-void launch_seg(hipStream_t st, const fl_logits *op, void *out, float2 *stats) {
-    const LogitArgs a = lg_args(op, LG_SEG);
-    const dim3 grid((unsigned)(op->rows * a.segments)), nt(LG_NT);
-    if (op->history) FL_LAUNCH("k_logits_seg", (k_logits_seg<T, MODE, true>), grid, nt, 0, st, a, out, stats);
-    else FL_LAUNCH("k_logits_seg", (k_logits_seg<T, MODE, false>), grid, nt, 0, st, a, out, stats);
+// The instance whose wave takes the columns: f(VPT), VPT in 1, 2, 4 (and 8).
+template <typename T, typename F>
+void by_columns(int64_t cols, F &&f) {
+    constexpr int lane = FL_WAVE * group_cols<T>();
+    if (cols <= lane) f(std::integral_constant<int, 1>{});
+    else if (cols <= 2 * lane) f(std::integral_constant<int, 2>{});
+    else if (LG_SEG == 4 * lane || cols <= 4 * lane) f(std::integral_constant<int, 4>{});
+    else f(std::integral_constant<int, LG_SEG / lane>{});
 }
 
 template <typename T, bool SOFTMAX>
 int forward(hipStream_t st, const fl_logits *op, void *out, float2 *stats, const char *what) {
-    if (op->cols <= 256) launch_rows<T, FL_WAVE, 1, SOFTMAX>(st, op, out);
-    else if (op->cols <= 512) launch_rows<T, FL_WAVE, 2, SOFTMAX>(st, op, out);
-    else if (op->cols <= 1024) launch_rows<T, FL_WAVE, 4, SOFTMAX>(st, op, out);
-    else if (op->cols <= LG_WAVE_COLS) launch_rows<T, FL_WAVE, 8, SOFTMAX>(st, op, out);
-    else if constexpr (!SOFTMAX) launch_seg<T, LG_CONSTRAIN>(st, op, out, stats);
-    else if (op->cols <= LG_LONG) launch_rows<T, LG_NT, LG_LONG / LG_NT / 4, true>(st, op, out);
-    else {
-        launch_seg<T, LG_STATS>(st, op, out, stats);
-        launch_seg<T, LG_JOINED>(st, op, out, stats);
+    if (SOFTMAX && op->cols > LG_SEG) {
+        constexpr int V = LG_SEG / FL_WAVE / group_cols<T>();
+        launch<T, V, LG_STATS>(st, op, out, stats);
+        launch<T, V, LG_JOINED>(st, op, out, stats);
+    } else {
+        by_columns<T>(op->cols, [&](auto v) {
+            launch<T, decltype(v)::value, SOFTMAX ? LG_SOFTMAX : LG_CONSTRAIN>(st, op, out, stats);
+        });
     }
     return fl_check_launch(what);
 }
@@ -678,53 +648,61 @@ int forward(hipStream_t st, const fl_logits *op, void *out, float2 *stats, const
 // several, the owners of none.
 int64_t grad_lists(const fl_logits *op) { return op->bias_rows > 1 ? op->bias_rows + 1 : 1; }
 
-int64_t grad_segments(const fl_logits *op, bool softmax) {
-    return op->cols <= LG_WAVE_COLS || (softmax && op->cols <= LG_LONG) ? 1 : lg_ceil(op->cols, LG_SEG);
-}
-
-// Parts of a list: some 2048 workgroups in all, of at least 8 rows on average.
-int grad_parts(const fl_logits *op, int64_t lists, int64_t segments) {
-    const int64_t want = lg_ceil(2048, lists * segments), most = op->rows / (8 * lists);
+// Parts of a list: some 8192 waves in all, of at least 8 rows on average.
+int grad_parts(const fl_logits *op, int64_t lists) {
+    const int64_t waves = op->cols <= LG_SEG ? lg_ceil(op->cols, 256) : lg_ceil(op->cols, LG_SEG / 2);
+    const int64_t want = lg_ceil(8192, lists * waves), most = op->rows / (8 * lists);
     const int64_t p = want < most ? want : most;
     return (int)(p < 1 ? 1 : p > 256 ? 256 : p);
 }
 
-template <typename T, int VPT, bool SOFTMAX>
-void launch_rows_grad(hipStream_t st, const GradArgs &a) {
+template <typename T, int VPT, bool SOFTMAX, bool HIST>
+void launch_grad(hipStream_t st, const GradArgs &a) {
     const fl_logits &op = a.l.op;
-    const int waves = a.dbias ? LG_WAVES : row_waves(op.rows);
-    const dim3 grid((unsigned)(a.dbias ? a.lists * a.parts : lg_ceil(op.rows, waves))), nt(waves * FL_WAVE);
-    if (op.history && op.repetition != 1.0f)  // the slopes need the repeats
-        FL_LAUNCH("k_logits_rows_grad", (k_logits_rows_grad<T, VPT, SOFTMAX, true>), grid, nt, 0, st, a);
-    else FL_LAUNCH("k_logits_rows_grad", (k_logits_rows_grad<T, VPT, SOFTMAX, false>), grid, nt, 0, st, a);
+    constexpr bool LONG = VPT == LG_SEG / FL_WAVE / group_cols<T>();
+    const bool whole = op.cols <= LG_SEG;
+    if constexpr (LONG) {
+        if (!whole && a.dbias) {  // half as many columns a wave: more waves, fewer registers
+            const int64_t waves = a.lists * a.parts * lg_ceil(op.cols, LG_SEG / 2);
+            FL_LAUNCH("k_logits_table_grad", (k_logits_table_grad<T, VPT / 2, SOFTMAX, HIST>),
+                      dim3((unsigned)lg_ceil(waves, LG_WAVES)), dim3(LG_NT), 0, st, a);
+            return;
+        }
+    }
+    const int64_t items = op.rows * a.l.segments;
+    if (items > 0) {
+        const int waves = lone_waves(items);
+        const dim3 grid((unsigned)lg_ceil(items, waves)), nt(waves * FL_WAVE);
+        if constexpr (SOFTMAX && LONG) {
+            if (!whole) FL_LAUNCH("k_logits_grad", (k_logits_grad<T, VPT, true, HIST, false>), grid, nt, 0, st, a);
+        }
+        if (!SOFTMAX || whole)
+            FL_LAUNCH("k_logits_grad", (k_logits_grad<T, VPT, SOFTMAX, HIST, true>), grid, nt, 0, st, a);
+    }
+    if (a.dbias) {
+        const int64_t sums = op.bias_rows * a.parts * lg_ceil(op.cols, 4 * LG_NT);
+        FL_LAUNCH("k_logits_sums", k_logits_sums, dim3((unsigned)sums), dim3(LG_NT), 0, st, a);
+    }
 }
 
-template <typename T, int VPT, bool SOFTMAX, bool WHOLE>
-void launch_seg_grad(hipStream_t st, const GradArgs &a) {
-    const fl_logits &op = a.l.op;
-    const dim3 grid((unsigned)((a.dbias ? a.lists * a.parts : op.rows) * a.l.segments)), nt(LG_NT);
-    if (op.history && op.repetition != 1.0f)
-        FL_LAUNCH("k_logits_seg_grad", (k_logits_seg_grad<T, VPT, SOFTMAX, true, WHOLE>), grid, nt, 0, st, a);
-    else FL_LAUNCH("k_logits_seg_grad", (k_logits_seg_grad<T, VPT, SOFTMAX, false, WHOLE>), grid, nt, 0, st, a);
-}
-
-// The gradient's workspace: the parts of dbias, the segments' dots and the
-// rows' (long softmax), and the owners by group.
+// The gradient's workspace: the parts of dbias, its terms (rows of one segment
+// whose dx does not hold them), the segments' dots and the rows' (softmax of
+// several segments), and the owners by group.
 struct GradSpace {
-    size_t parts, dots, order, offsets, group, group_bytes, bytes;
+    size_t parts, terms, dots, order, offsets, group, group_bytes, bytes;
 };
 
-GradSpace grad_space(const fl_logits *op, bool softmax, bool with_dbias) {
+GradSpace grad_space(const fl_logits *op, bool softmax, bool with_dx, bool with_dbias) {
     GradSpace s{};
     const auto take = [&](size_t n) {
         const size_t at = s.bytes;
         s.bytes += (n + 255) / 256 * 256;
         return at;
     };
-    const int64_t segments = grad_segments(op, softmax);
     if (with_dbias) {
-        const int parts = grad_parts(op, grad_lists(op), segments);
+        const int parts = grad_parts(op, grad_lists(op));
         if (parts > 1) s.parts = take((size_t)parts * op->bias_rows * op->cols * 4);
+        if (op->cols <= LG_SEG && !(with_dx && op->dtype == FL_F32)) s.terms = take((size_t)op->rows * op->cols * 4);
         if (op->bias_rows > 1) {
             const int64_t owners = op->rows / op->inner;
             s.order = take((size_t)owners * 4 + 4);
@@ -733,24 +711,24 @@ GradSpace grad_space(const fl_logits *op, bool softmax, bool with_dbias) {
             s.group = take(s.group_bytes);
         }
     }
-    if (softmax && op->cols > LG_LONG) s.dots = take((size_t)op->rows * (segments + 1) * 4);
+    if (softmax && op->cols > LG_SEG) s.dots = take((size_t)op->rows * (segments_of(op) + 1) * 4);
     return s;
 }
 
 template <typename T, bool SOFTMAX>
 int gradient(hipStream_t st, const fl_logits *op, const float *w, const void *grad, void *dx, float *dbias, char *ws) {
-    const GradSpace sp = grad_space(op, SOFTMAX, dbias != nullptr);
+    const GradSpace sp = grad_space(op, SOFTMAX, dx != nullptr, dbias != nullptr);
     GradArgs a{};
-    a.l = lg_args(op, LG_SEG);
-    a.l.segments = (uint32_t)grad_segments(op, SOFTMAX);
+    a.l = lg_args(op);
     a.g = grad;
     a.w = w;
     a.dx = dx;
     a.parts = 1;
     if (dbias) {
         a.lists = grad_lists(op);
-        a.parts = (uint32_t)grad_parts(op, a.lists, a.l.segments);
+        a.parts = (uint32_t)grad_parts(op, a.lists);
         a.dbias = a.parts > 1 ? (float *)(ws + sp.parts) : dbias;
+        if (op->cols <= LG_SEG && !(std::is_same_v<T, float> && dx)) a.terms = (float *)(ws + sp.terms);
         if (op->bias_rows > 1) {
             int32_t *order = (int32_t *)(ws + sp.order), *offsets = (int32_t *)(ws + sp.offsets);
             const int rc = fl_group_rows(st, op->group, op->rows / op->inner, op->bias_rows, order, offsets, nullptr,
@@ -760,21 +738,19 @@ int gradient(hipStream_t st, const fl_logits *op, const float *w, const void *gr
             a.offsets = offsets;
         }
     } else if (op->rows == 0) return FL_OK;
-    if (SOFTMAX && op->cols > LG_LONG && op->rows > 0) {
+    if (SOFTMAX && op->cols > LG_SEG && op->rows > 0) {
         float *part = (float *)(ws + sp.dots), *dots = part + op->rows * a.l.segments;
-        FL_LAUNCH("k_logits_dot", k_logits_dot, dim3((unsigned)(op->rows * a.l.segments)), dim3(LG_NT), 0, st, a.l,
-                  (const float *)grad, w, part);
+        FL_LAUNCH("k_logits_dot", k_logits_dot, dim3((unsigned)lg_ceil(op->rows * a.l.segments, LG_WAVES)),
+                  dim3(LG_NT), 0, st, a.l, (const float *)grad, w, part);
         FL_LAUNCH("k_logits_join", k_logits_join, dim3((unsigned)op->rows), dim3(FL_WAVE), 0, st, part,
                   (int64_t)a.l.segments, dots);
         a.dots = dots;
     }
-    if (op->cols <= 256) launch_rows_grad<T, 1, SOFTMAX>(st, a);
-    else if (op->cols <= 512) launch_rows_grad<T, 2, SOFTMAX>(st, a);
-    else if (op->cols <= 1024) launch_rows_grad<T, 4, SOFTMAX>(st, a);
-    else if (op->cols <= LG_WAVE_COLS) launch_rows_grad<T, 8, SOFTMAX>(st, a);
-    else if constexpr (!SOFTMAX) launch_seg_grad<T, LG_VPT, false, true>(st, a);
-    else if (op->cols <= LG_LONG) launch_seg_grad<T, LG_LONG / LG_NT / 4, true, true>(st, a);
-    else launch_seg_grad<T, LG_VPT, true, false>(st, a);
+    const bool signs = op->history && op->repetition != 1.0f;  // the slopes need the repeats
+    by_columns<T>(op->cols, [&](auto v) {
+        if (signs) launch_grad<T, decltype(v)::value, SOFTMAX, true>(st, a);
+        else launch_grad<T, decltype(v)::value, SOFTMAX, false>(st, a);
+    });
     if (a.parts > 1) fold_parts<float>(st, a.dbias, (int)a.parts, op->bias_rows * op->cols, dbias);
     return fl_check_launch("logits_grad");
 }
@@ -814,7 +790,7 @@ int fl_logits_constrain(void *stream, const fl_logits *op, void *out) {
 }
 
 size_t fl_logits_softmax_bytes(const fl_logits *op) {
-    if (!op || op->cols <= fl::LG_LONG || op->rows < 1) return 0;
+    if (!op || op->cols <= fl::LG_SEG || op->rows < 1) return 0;
     return (size_t)op->rows * fl::lg_ceil(op->cols, fl::LG_SEG) * sizeof(float2);
 }
 
@@ -829,9 +805,9 @@ int fl_logits_softmax(void *stream, const fl_logits *op, float *w, void *ws, siz
                                                           "logits_softmax")))
 }
 
-size_t fl_logits_grad_bytes(const fl_logits *op, int softmax, int with_dbias) {
+size_t fl_logits_grad_bytes(const fl_logits *op, int softmax, int with_dx, int with_dbias) {
     if (!op || op->rows < 0 || op->cols < 1 || op->inner < 1) return 0;
-    return fl::grad_space(op, softmax != 0, with_dbias != 0 && op->bias && op->bias_rows > 0).bytes;
+    return fl::grad_space(op, softmax != 0, with_dx != 0, with_dbias != 0 && op->bias && op->bias_rows > 0).bytes;
 }
 
 int fl_logits_grad(void *stream, const fl_logits *op, const float *w, const void *grad, void *dx, float *dbias,
@@ -841,7 +817,7 @@ int fl_logits_grad(void *stream, const fl_logits *op, const float *w, const void
     if (op->cols == 0) return FL_OK;
     if (dbias && !op->bias) return fl::fl_fail(FL_ERR_ARG, "logits_grad: the gradient of no bias table");
     if (op->rows > 0 && !grad) return fl::fl_fail(FL_ERR_ARG, "logits_grad: null pointer");
-    const size_t need = fl_logits_grad_bytes(op, w != nullptr, dbias != nullptr);
+    const size_t need = fl_logits_grad_bytes(op, w != nullptr, dx != nullptr, dbias != nullptr);
     if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "logits_grad: workspace too small");
     if ((uintptr_t)ws % 16) return fl::fl_fail(FL_ERR_ARG, "logits_grad: workspace must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;

@@ -927,7 +927,8 @@ int fl_logits_softmax(void *stream, const fl_logits *op, float *w, void *ws,
  * fl_logits_softmax (w its output, grad fp32): dx [rows, cols] of x's type,
  * or null, and dbias [bias_rows, cols], or null.  grad contiguous; ws on a
  * 16-byte boundary. */
-size_t fl_logits_grad_bytes(const fl_logits *op, int softmax, int with_dbias);
+size_t fl_logits_grad_bytes(const fl_logits *op, int softmax, int with_dx,
+                            int with_dbias);
 int fl_logits_grad(void *stream, const fl_logits *op, const float *w,
                    const void *grad, void *dx, float *dbias, void *ws,
                    size_t ws_bytes);

@@ -108,7 +108,7 @@ def test_logits_arguments():
     assert "bias" in back(_logits_op(), None, one, one, one, None, 0)
     assert "null" in back(_logits_op(), None, None, one, None, None, 0)
     for op in (_logits_op(rows=100_000, bias=1, bias_rows=1), _logits_op(bias=1, bias_rows=2, group=1)):
-        need = lib.fl_logits_grad_bytes(op, 0, 1)
+        need = lib.fl_logits_grad_bytes(op, 0, 1, 1)
         assert need > 0 and "workspace" in back(op, None, one, one, one, one, need - 1)
         assert "aligned" in back(op, None, one, one, one, one, need)
     assert "shape" in _error(lib.fl_pack_bits(None, one, -1, 3, one))

@@ -421,3 +421,43 @@ def test_same_bits_and_graph():
         torch.cuda.synchronize()
         for p, q in zip(step(*args), out):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("softmax", [False, True])
+@pytest.mark.parametrize("t", TYPES)
+def test_long_histories(t, softmax):
+    """More ids than a byte counts: short rows, rows of several segments, an id many times over."""
+    g = torch.Generator().manual_seed(50)
+    for n in (30, 1645, 5000):
+        c = _case((2, 3), n, t, 51, groups=2, bias="table")
+        c["history"] = torch.randint(-2, n + 2, (2, 700), generator=g)
+        c["history"][0, :400] = n // 2
+        _check(c, dict(OPTIONS, frequency=0.01), softmax)
+
+
+def test_a_history_that_outgrows_its_counters():
+    """Past 65,000 repeats a column is counted no further, and its neighbours stay right."""
+    fa = _fa()
+    ids = torch.full((1, 150_000), 11)
+    ids[0, :3] = torch.tensor([10, 12, 12])
+    y = fa.constrain_logits(torch.zeros(1, 300).cuda(), history=ids.cuda(), frequency=1.0).cpu()[0]
+    assert y[10] == -1 and y[12] == -2 and -65_100 <= y[11] <= -65_000
+    y[[10, 11, 12]] = 0
+    assert (y == 0).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n", [70, 3000])
+def test_gradient_of_the_bias_alone(n, t):
+    fa = _fa()
+    c = _gpu(_case((40,), n, t, 60, groups=5, bias="table", past=2))
+    gy = torch.randn(40, n).cuda()
+    both, alone = [], []
+    for keep in (True, False):
+        x, b = c["x"].detach().requires_grad_(keep), c["bias"].detach().requires_grad_(True)
+        kw = dict(allowed=c["allowed"], group=c["group"], bias=b, history=c["history"], **OPTIONS)
+        for fn in (fa.hop_attention, fa.constrain_logits):
+            y = fn(x, **kw)
+            (both if keep else alone).append(torch.autograd.grad(y, [b], gy.to(y.dtype))[0])
+    for p, q in zip(both, alone):
+        assert torch.equal(p, q)
