@@ -43,56 +43,77 @@ __device__ __forceinline__ int64_t group_key(const GroupArgs &a, int64_t row) {
     return k >= 0 && k < a.groups ? k : a.groups;
 }
 
-// Digit of the row at place p of the pass's input.
-__device__ __forceinline__ int digit_at(const GroupArgs &a, int64_t p, int64_t *row) {
-    *row = a.in_order ? (int64_t)a.in_order[p] : p;
-    return (int)((group_key(a, *row) >> a.shift) & (a.digits - 1));
-}
-
 // Lanes whose digit equals this one's (among the active rows).
 __device__ __forceinline__ unsigned long long equal_lanes(int d, bool active, int bits) {
-    unsigned long long m = __ballot(active);
+    const unsigned long long m = __ballot(active);
+    unsigned lo = (unsigned)m, hi = (unsigned)(m >> 32);
     for (int b = 0; b < bits; ++b) {
-        const unsigned long long s = __ballot((d >> b) & 1);
-        m &= ((d >> b) & 1) ? s : ~s;
+        const int mine = (d << (31 - b)) >> 31;  // the bit, in every place
+        const unsigned long long s = __ballot(mine != 0);
+        lo &= ~((unsigned)s ^ (unsigned)mine);
+        hi &= ~((unsigned)(s >> 32) ^ (unsigned)mine);
     }
-    return m;
+    return ((unsigned long long)hi << 32) | lo;
 }
 
-// A wave's counts of its rows' digits; with `local`, each row's rank within
-// the wave's rows of its digit instead of nothing.
-template <typename F>
-__device__ __forceinline__ void wave_rows(const GroupArgs &a, int64_t begin, int64_t end, uint16_t *cnt, F &&f) {
-    const int lane = fl_lane();
-    for (int64_t p0 = begin; p0 < end; p0 += FL_WAVE) {
-        const int64_t p = p0 + lane;
-        const bool active = p < end;
-        int64_t row = 0;
-        const int d = active ? digit_at(a, p, &row) : 0;
-        const unsigned long long eq = equal_lanes(d, active, a.bits);
-        if (active) {
-            const int before = __popcll(eq & ((1ull << lane) - 1));
-            const int old = cnt[d];
-            f(row, d, old + before);
-            if (before == 0) cnt[d] = (uint16_t)(old + __popcll(eq));
+// The rows of a wave's run, a strip of 64 at a time: all loaded before the
+// first is worked on (one strip's loads after another's took 25 us for 15000
+// rows, nothing but their latency).
+struct WaveRows {
+    static constexpr int STRIPS = (int)(GR_WAVE_ROWS / FL_WAVE);
+    int32_t row[STRIPS];
+    int digit[STRIPS], rank[STRIPS];
+    int strips;
+    int64_t begin, end;
+
+    __device__ __forceinline__ void load(const GroupArgs &a) {
+        // the workgroup's rows in equal contiguous runs of whole strips
+        const int64_t b0 = (int64_t)blockIdx.x * GR_BLOCK_ROWS;
+        const int64_t n = a.rows - b0 < GR_BLOCK_ROWS ? a.rows - b0 : GR_BLOCK_ROWS;
+        const int64_t per = ((n + GR_WAVES - 1) / GR_WAVES + FL_WAVE - 1) / FL_WAVE * FL_WAVE;
+        const int64_t s = fl_wave_id() * per;
+        begin = b0 + (s < n ? s : n);
+        end = b0 + (s + per < n ? s + per : n);
+        strips = (int)((end - begin + FL_WAVE - 1) / FL_WAVE);
+#pragma unroll
+        for (int i = 0; i < STRIPS; ++i) {
+            const int64_t p = begin + i * FL_WAVE + fl_lane();
+            row[i] = p < end ? (a.in_order ? a.in_order[p] : (int32_t)p) : 0;
         }
-        fl_wave_sync();
+#pragma unroll
+        for (int i = 0; i < STRIPS; ++i)
+            digit[i] = i < strips ? (int)((group_key(a, row[i]) >> a.shift) & (a.digits - 1)) : 0;
     }
-}
+    // Counts the digits in cnt (0 before); every row's rank among the wave's
+    // rows of its digit.
+    __device__ __forceinline__ void count(const GroupArgs &a, uint16_t *cnt) {
+#pragma unroll
+        for (int i = 0; i < STRIPS; ++i) {
+            rank[i] = 0;
+            if (i < strips) {
+                const bool active = begin + i * FL_WAVE + fl_lane() < end;
+                const unsigned long long eq = equal_lanes(digit[i], active, a.bits);
+                if (active) {
+                    const int before = __popcll(eq & ((1ull << fl_lane()) - 1));
+                    const int old = cnt[digit[i]];
+                    rank[i] = old + before;
+                    if (before == 0) cnt[digit[i]] = (uint16_t)(old + __popcll(eq));
+                }
+                fl_wave_sync();
+            }
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F &&f) const {
+#pragma unroll
+        for (int i = 0; i < STRIPS; ++i)
+            if (begin + i * FL_WAVE + fl_lane() < end) f(row[i], digit[i], rank[i]);
+    }
+};
 
 __device__ __forceinline__ void clear_counts(uint16_t *cnt, int digits) {
     uint32_t *c = reinterpret_cast<uint32_t *>(cnt);
     for (int i = threadIdx.x; i < GR_WAVES * digits / 2; i += GR_NT) c[i] = 0;
-}
-
-__device__ __forceinline__ void wave_range(const GroupArgs &a, int64_t *begin, int64_t *end) {
-    // the workgroup's rows in equal contiguous runs of whole strips
-    const int64_t b0 = (int64_t)blockIdx.x * GR_BLOCK_ROWS;
-    const int64_t n = a.rows - b0 < GR_BLOCK_ROWS ? a.rows - b0 : GR_BLOCK_ROWS;
-    const int64_t per = ((n + GR_WAVES - 1) / GR_WAVES + FL_WAVE - 1) / FL_WAVE * FL_WAVE;
-    const int64_t s = fl_wave_id() * per;
-    *begin = b0 + (s < n ? s : n);
-    *end = b0 + (s + per < n ? s + per : n);
 }
 
 // Exclusive scan, by one workgroup, of f(i) for i < n; g(i, prefix) takes it.
@@ -137,12 +158,12 @@ __global__ __launch_bounds__(GR_NT) void k_group_one(GroupArgs a) {
     extern __shared__ uint16_t cnt[];
     __shared__ int lds[GR_WAVES + 1];
     __shared__ int first[GR_DIGITS];
+    WaveRows rows;
+    rows.load(a);
     clear_counts(cnt, a.digits);
     __syncthreads();
-    int64_t begin, end;
-    wave_range(a, &begin, &end);
     uint16_t *mine = cnt + fl_wave_id() * a.digits;
-    wave_rows(a, begin, end, mine, [](int64_t, int, int) {});
+    rows.count(a, mine);
     __syncthreads();
     block_scan(
         a.digits, lds,
@@ -160,7 +181,7 @@ __global__ __launch_bounds__(GR_NT) void k_group_one(GroupArgs a) {
             if (d <= a.groups) a.offsets[d] = pre;
         });
     __syncthreads();
-    wave_rows(a, begin, end, mine, [&](int64_t row, int d, int rank) { a.out_order[first[d] + rank] = (int32_t)row; });
+    rows.each([&](int32_t row, int d, int rank) { a.out_order[first[d] + mine[d] + rank] = row; });
     __threadfence_block();
     __syncthreads();
     if (a.tiles) write_tiles(a, lds);
@@ -168,11 +189,11 @@ __global__ __launch_bounds__(GR_NT) void k_group_one(GroupArgs a) {
 
 __global__ __launch_bounds__(GR_NT) void k_group_count(GroupArgs a) {
     extern __shared__ uint16_t cnt[];
+    WaveRows rows;
+    rows.load(a);
     clear_counts(cnt, a.digits);
     __syncthreads();
-    int64_t begin, end;
-    wave_range(a, &begin, &end);
-    wave_rows(a, begin, end, cnt + fl_wave_id() * a.digits, [](int64_t, int, int) {});
+    rows.count(a, cnt + fl_wave_id() * a.digits);
     __syncthreads();
     for (int d = threadIdx.x; d < a.digits; d += GR_NT) {
         int run = 0;
@@ -201,12 +222,12 @@ __global__ __launch_bounds__(GR_NT) void k_group_scan(GroupArgs a) {
 
 __global__ __launch_bounds__(GR_NT) void k_group_place(GroupArgs a) {
     extern __shared__ uint16_t cnt[];
+    WaveRows rows;
+    rows.load(a);
     clear_counts(cnt, a.digits);
     __syncthreads();
-    int64_t begin, end;
-    wave_range(a, &begin, &end);
     uint16_t *mine = cnt + fl_wave_id() * a.digits;
-    wave_rows(a, begin, end, mine, [](int64_t, int, int) {});
+    rows.count(a, mine);
     __syncthreads();
     for (int d = threadIdx.x; d < a.digits; d += GR_NT) {
         int run = 0;
@@ -218,7 +239,7 @@ __global__ __launch_bounds__(GR_NT) void k_group_place(GroupArgs a) {
     }
     __syncthreads();
     const int32_t *first = a.hist + (int64_t)blockIdx.x * a.digits;
-    wave_rows(a, begin, end, mine, [&](int64_t row, int d, int rank) { a.out_order[first[d] + rank] = (int32_t)row; });
+    rows.each([&](int32_t row, int d, int rank) { a.out_order[first[d] + mine[d] + rank] = row; });
 }
 
 // Offsets by binary search in the sorted rows (the multi-launch forms).

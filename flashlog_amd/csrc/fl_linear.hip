@@ -84,6 +84,18 @@ __device__ __forceinline__ void store_some(T *p, const Vec<T, N> &r, int m) {
         if (e < m) p[e] = r.v[e];
 }
 
+// Up to four values as floats, the others 0.
+template <typename T>
+__device__ __forceinline__ void load_some(const T *p, int have, float (&out)[4]) {
+    if (have == 4) {
+        const Vec<T, 4> r = load_vec<T, 4>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = (float)r.v[e];
+    } else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = e < have ? (float)p[e] : 0.0f;
+}
+
 // The upper halves of two words, lo's first.
 __device__ __forceinline__ uint32_t upper_halves(uint32_t lo, uint32_t hi) {
     return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
@@ -447,56 +459,58 @@ __device__ __forceinline__ bool row_tile(const RowsArgs &a, uint32_t mt, RowTile
 template <typename T, int MT, int NTL>
 __device__ __forceinline__ void store_rows(const RowsArgs &a, const f32x4 (&acc)[MT][NTL], const RowTile &t,
                                            int64_t pos, int64_t col) {
-    const int64_t g = t.g, end = t.end;
-    const bool none = t.none;
     const int lane = fl_lane();
+    const int64_t n0 = col + (lane >> 4) * 4;
+    int have[NTL];  // columns of the lane's j-th four
+    float bias[NTL][4];
+#pragma unroll
+    for (int j = 0; j < NTL; ++j) {
+        const int64_t left = a.N - (n0 + j * 16);
+        have[j] = left < 0 ? 0 : left < 4 ? (int)left : 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bias[j][e] = 0.0f;
+        if (a.bias && !t.none) {
+            const int64_t at = t.g * a.bias_group + n0 + j * 16;
+            if (a.bias_f32) load_some<float>((const float *)a.bias + at, have[j], bias[j]);
+            else load_some<T>((const T *)a.bias + at, have[j], bias[j]);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int64_t p = pos + i * 16 + (lane & 15);
-        if (p >= end) continue;
+        if (p >= t.end) continue;
         const int64_t row = a.order ? (int64_t)a.order[p] : p;
+        float res[NTL][4];
+        if (a.residual)
+#pragma unroll
+            for (int j = 0; j < NTL; ++j)
+                load_some<T>((const T *)a.residual + row * a.ldres + n0 + j * 16, have[j], res[j]);
 #pragma unroll
         for (int j = 0; j < NTL; ++j) {
-            const int64_t n = col + j * 16 + (lane >> 4) * 4;
-            if (n >= a.N) continue;
-            const int m = a.N - n < 4 ? (int)(a.N - n) : 4;
+            if (!have[j]) continue;
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
-            if (a.bias && !none) {
-                const int64_t at = g * a.bias_group + n;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < m) v[e] += a.bias_f32 ? ((const float *)a.bias)[at + e] : (float)((const T *)a.bias)[at + e];
-            }
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] + bias[j][e];
             if (a.pre) {
                 // kept in 32 bits: rounded to the operands' type it would move the slopes by as much as the
                 // gradients' own rounding does
                 const Vec<float, 4> f{{v[0], v[1], v[2], v[3]}};
-                float *q = a.pre + row * a.N + n;
-                if (m == 4) store_vec<float, 4>(q, f);
-                else store_some<float, 4>(q, f, m);
+                float *q = a.pre + row * a.N + n0 + j * 16;
+                if (have[j] == 4) store_vec<float, 4>(q, f);
+                else store_some<float, 4>(q, f, have[j]);
             }
-            Vec<T, 4> o;
-            if (!none)
+            if (!t.none)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = act_value(v[e], a.act);
-            if (a.residual) {
-                const T *q = (const T *)a.residual + row * a.ldres + n;
-                if (m == 4) {
-                    const Vec<T, 4> r = load_vec<T, 4>(q);
+            if (a.residual)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += (float)r.v[e];
-                } else
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < m) v[e] += (float)q[e];
-            }
+                for (int e = 0; e < 4; ++e) v[e] += res[j][e];
+            Vec<T, 4> o;
 #pragma unroll
             for (int e = 0; e < 4; ++e) o.v[e] = (T)v[e];
-            T *q = (T *)a.c + row * a.ldc + n;
-            if (m == 4) store_vec<T, 4>(q, o);
-            else store_some<T, 4>(q, o, m);
+            T *q = (T *)a.c + row * a.ldc + n0 + j * 16;
+            if (have[j] == 4) store_vec<T, 4>(q, o);
+            else store_some<T, 4>(q, o, have[j]);
         }
     }
 }
@@ -615,22 +629,23 @@ __global__ __launch_bounds__(LN_NT) void k_lin_outer(OuterArgs a) {
 }
 
 // The same products for large 16-bit operands at the matrix unit's pace.  512
-// threads take BM x 256 outputs, 8 waves of BM/2 x 64; BK = 64 values of k
-// per step.  Operands go from memory to LDS without registers
-// (global_load_lds, 16 bytes a lane), into one of STAGES buffers while another
-// is multiplied: one barrier a step, and the loads have STAGES - 1 steps to
-// arrive.  A wave's load fills 1 KB of LDS in lane order, so the permutation
+// threads take BM x 256 outputs, 8 waves of BM/2 x 64; BK values of k a step.
+// Operands go from memory to LDS without registers (global_load_lds, 16 bytes
+// a lane), into one of STAGES buffers while others are multiplied, so that a
+// load has STAGES - 1 steps to arrive.  The waves work in two halves, one wave
+// of each on every SIMD, half a step apart: while one half reads its operands
+// from LDS (and issues its share of the loads), the other multiplies; barriers
+// keep them in turn.  (With all waves in step the matrix unit was busy 45% of
+// the time.)  A wave's load fills 1 KB of LDS in lane order, so the permutation
 // of the chunks that spreads the later reads over the banks is made on the
 // memory side: a lane loads the chunk that belongs to its place.
 // k-strided operands lie in LDS as they do in memory, rows of k, and are read
 // transposed (ds_read_b64_tr_b16: of 16 lanes, lane s gives the address of
 // row s/4, columns 4 (s%4)..+3, and lane i receives column i of the 4 rows).
-// Needs 16-byte aligned rows of whole 8-value chunks.  With 256 x 256 tiles
-// the LDS reads of a step take 1536 cycles a CU and its multiplications 2048.
+// Needs 16-byte aligned rows of whole 8-value chunks.
 constexpr int WD_NT = 512;
 constexpr int WD_WAVES = WD_NT / FL_WAVE;
 constexpr int WD_BN = 256;
-constexpr int WD_BK = 64;
 
 // What lanes outside an operand load.
 __device__ __align__(16) const uint32_t wd_zeros[4] = {0, 0, 0, 0};
@@ -642,22 +657,23 @@ __device__ __forceinline__ void load_lds(const void *p, uint16_t *lds) {
     __builtin_amdgcn_global_load_lds((mem_ptr *)p, (lds_ptr *)lds, 16, 0, 0);
 }
 
-template <int BR>
+template <int BR, int BK>
 struct WideContig {
-    static constexpr int LOADS = BR / 8 / WD_WAVES;  // 8 rows of 64 values a load
-    static constexpr int ELEMS = BR * WD_BK;
+    static constexpr int CPR = BK / 8, RPL = FL_WAVE / CPR;  // chunks of a row, rows of a load
+    static constexpr int LOADS = BR / RPL / WD_WAVES;
+    static constexpr int ELEMS = BR * BK;
     const uint16_t *p[LOADS];
 
     // The row and the chunk that this lane loads i-th.
-    static __device__ __forceinline__ int row(int i) { return (fl_wave_id() * LOADS + i) * 8 + (fl_lane() >> 3); }
-    static __device__ __forceinline__ int chunk(int i) { return (fl_lane() & 7) ^ ((row(i) >> 1) & 7); }
+    static __device__ __forceinline__ int row(int i) { return (fl_wave_id() * LOADS + i) * RPL + fl_lane() / CPR; }
+    static __device__ __forceinline__ int chunk(int i) { return (lds_at<BK>(row(i), fl_lane() % CPR) % BK) / 8; }
 
     template <typename F>
     __device__ __forceinline__ void init(F &&row_ptr) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) p[i] = row_ptr(row(i)) + chunk(i) * 8;
     }
-    // The next `count` <= 64 values of k.
+    // The next `count` <= BK values of k.
     __device__ __forceinline__ void issue(uint16_t *lds, int count) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
@@ -667,20 +683,19 @@ struct WideContig {
         }
     }
     __device__ __forceinline__ u32x4 frag(const uint16_t *lds, int row0, int ks) const {
-        const int r = row0 + (fl_lane() & 15), q = fl_lane() >> 4;
-        return *reinterpret_cast<const u32x4 *>(lds + r * WD_BK + (((ks * 4 + q) ^ ((r >> 1) & 7)) << 3));
+        return *reinterpret_cast<const u32x4 *>(lds + lds_at<BK>(row0 + (fl_lane() & 15), ks * 4 + (fl_lane() >> 4)));
     }
 };
 
-template <int BR>
+template <int BR, int BK>
 struct WideStrided {
     static constexpr int CH = BR / 8;                // chunks a row of k
     static constexpr int RPL = FL_WAVE / CH;         // rows of k a load
-    static constexpr int LOADS = WD_BK / RPL / WD_WAVES;
-    static constexpr int ELEMS = BR * WD_BK;
+    static constexpr int LOADS = BK / RPL / WD_WAVES;
+    static constexpr int ELEMS = BR * BK;
     const uint16_t *col[LOADS];
     const int32_t *order;
-    int32_t next[LOADS];
+    int32_t next[LOADS][RPL];
     int64_t ld, place;
 
     // The permutation of a row's chunks, in steps of the two chunks that a
@@ -700,16 +715,29 @@ struct WideStrided {
         }
         look(first);
     }
-    // The rows of the step that begins at `place`, of `count` rows.
+    // The rows of the step that begins at `place`, of `count` rows.  (Scalar
+    // loads: vector ones would be waited for together with the operands'.)
     __device__ __forceinline__ void look(int count) {
-        if (order)
+        if (!order) return;
+        const auto *o = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)order;
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) next[i] = row(i) < count ? order[place + row(i)] : 0;
+        for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+            for (int j = 0; j < RPL; ++j) {
+                const int r = (fl_wave_id() * LOADS + i) * RPL + j;
+                next[i][j] = r < count ? o[place + r] : 0;
+            }
     }
     __device__ __forceinline__ void issue(uint16_t *lds, int count, int after) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int64_t r = order ? (int64_t)next[i] : place + row(i);
+            int64_t r = place + row(i);
+            if (order) {
+                int32_t n = next[i][0];
+#pragma unroll
+                for (int j = 1; j < RPL; ++j) n = fl_lane() / CH == j ? next[i][j] : n;
+                r = n;
+            }
             const void *q = row(i) < count ? (const void *)(col[i] + r * ld) : (const void *)wd_zeros;
             load_lds(q, lds + (fl_wave_id() * LOADS + i) * 512);
         }
@@ -735,7 +763,7 @@ struct WideStrided {
     }
 };
 
-template <typename T, int BM, int STAGES, typename TA, typename TB>
+template <typename T, int BM, int BK, int STAGES, typename TA, typename TB>
 struct WideProduct {
     static constexpr int MT = BM / 2 / 16, NTL = 4;
     static constexpr int ELEMS = TA::ELEMS + TB::ELEMS;
@@ -745,7 +773,7 @@ struct WideProduct {
     static __device__ __forceinline__ int wave_m() { return (fl_wave_id() >> 2) * (BM / 2); }
     static __device__ __forceinline__ int wave_n() { return (fl_wave_id() & 3) * 64; }
 
-    // count(i): values of step i; feed(lds_a, lds_b, i) issues its loads.
+    // feed(lds_a, lds_b, i) issues the loads of step i.
     template <typename F>
     __device__ __forceinline__ void run(const TA &ta, const TB &tb, int64_t steps, uint16_t *lds, F &&feed) {
 #pragma unroll
@@ -753,50 +781,65 @@ struct WideProduct {
 #pragma unroll
             for (int j = 0; j < NTL; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
         if (steps <= 0) return;
+        const bool second = fl_wave_id() >= WD_WAVES / 2;
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s)
             if (s < steps) feed(lds + s * ELEMS, lds + s * ELEMS + TA::ELEMS, s);
+        if (steps < STAGES - 1) wait<0>();
+        else wait<LOADS *(STAGES - 2)>();
+        meet();
+        if (second) meet();
         int at = 0;
         for (int64_t s = 0; s < steps; ++s) {
-            // this step's loads have landed when at most those of the later steps are under way
-            if (STAGES == 2 || s + 1 >= steps) __builtin_amdgcn_s_waitcnt(0x0f70);
-            else __builtin_amdgcn_s_waitcnt(wait_imm());
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            if (s + STAGES - 1 < steps) {
-                const int to = at + STAGES - 1 >= STAGES ? at - 1 : at + STAGES - 1;
-                feed(lds + to * ELEMS, lds + to * ELEMS + TA::ELEMS, s + STAGES - 1);
-            }
+            // this half reads step s while the other multiplies
             const uint16_t *la = lds + at * ELEMS, *lb = la + TA::ELEMS;
+            u32x4 fa[BK / 32][MT], fb[BK / 32][NTL];
 #pragma unroll
-            for (int ks = 0; ks < WD_BK / 32; ++ks) {
-                u32x4 b[NTL];
+            for (int ks = 0; ks < BK / 32; ++ks) {
 #pragma unroll
-                for (int j = 0; j < NTL; ++j) b[j] = tb.frag(lb, wave_n() + j * 16, ks);
+                for (int j = 0; j < NTL; ++j) fb[ks][j] = tb.frag(lb, wave_n() + j * 16, ks);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const u32x4 f = ta.frag(la, wave_m() + i * 16, ks);
-#pragma unroll
-                    for (int j = 0; j < NTL; ++j) acc[i][j] = mfma<T>(b[j], f, acc[i][j]);
-                }
+                for (int i = 0; i < MT; ++i) fa[ks][i] = ta.frag(la, wave_m() + i * 16, ks);
             }
+            if (s + STAGES - 1 < steps) {
+                // over step s - 1, which both halves have read
+                const int to = at == 0 ? STAGES - 1 : at - 1;
+                feed(lds + to * ELEMS, lds + to * ELEMS + TA::ELEMS, s + STAGES - 1);
+                wait<LOADS *(STAGES - 2)>();  // step s + 1 has landed
+            } else wait<0>();
+            meet();
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int ks = 0; ks < BK / 32; ++ks)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NTL; ++j) acc[i][j] = mfma<T>(fb[ks][j], fa[ks][i], acc[i][j]);
+            __builtin_amdgcn_s_setprio(0);
+            meet();
             at = at + 1 == STAGES ? 0 : at + 1;
         }
+        if (!second) meet();
     }
-    // s_waitcnt vmcnt(LOADS (STAGES - 2)), nothing else (vmcnt: bits 0-3 and 14-15)
-    static constexpr int wait_imm() {
-        constexpr int n = LOADS * (STAGES - 2);
-        return (n & 15) | ((n >> 4) << 14) | 0x0f70;
+    // Waits for this wave's LDS reads and for all but its last VM memory loads
+    // (s_waitcnt: vmcnt in bits 0-3 and 14-15, expcnt 4-6, lgkmcnt 8-11).
+    template <int VM>
+    static __device__ __forceinline__ void wait() {
+        __builtin_amdgcn_s_waitcnt((VM & 15) | ((VM >> 4) << 14) | 0x0070);
+    }
+    static __device__ __forceinline__ void meet() {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 };
 
 // The forward (B_CONTIG) and dx.
-template <typename T, bool B_CONTIG, int BM, int STAGES>
+template <typename T, bool B_CONTIG, int BM, int BK, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
-    using TA = WideContig<BM>;
-    using TB = std::conditional_t<B_CONTIG, WideContig<WD_BN>, WideStrided<WD_BN>>;
-    using Prod = WideProduct<T, BM, STAGES, TA, TB>;
+    using TA = WideContig<BM, BK>;
+    using TB = std::conditional_t<B_CONTIG, WideContig<WD_BN, BK>, WideStrided<WD_BN, BK>>;
+    using Prod = WideProduct<T, BM, BK, STAGES, TA, TB>;
     extern __shared__ __align__(16) uint16_t wide_lds[];
     const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
     RowTile t;
@@ -804,8 +847,8 @@ __global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
     const int64_t n0 = (int64_t)(w % a.n_tiles) * WD_BN;
     const uint16_t *A = (const uint16_t *)a.a;
     const uint16_t *B = (const uint16_t *)a.b + (t.none ? 0 : t.g * a.b_group);
-    const int64_t steps = t.none ? 0 : (a.K + WD_BK - 1) / WD_BK;
-    const int first = (int)(a.K - (steps - 1) * WD_BK);  // the step that is no whole one comes first
+    const int64_t steps = t.none ? 0 : (a.K + BK - 1) / BK;
+    const int first = (int)(a.K - (steps - 1) * BK);  // the step that is no whole one comes first
     TA ta;
     TB tb;
     ta.init([&](int r) {
@@ -816,20 +859,20 @@ __global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
     else tb.init(B + n0, a.ldb, a.N - n0, nullptr, first);
     Prod prod;
     prod.run(ta, tb, steps, wide_lds, [&](uint16_t *la, uint16_t *lb, int64_t s) {
-        const int count = s ? WD_BK : first;
+        const int count = s ? BK : first;
         ta.issue(la, count);
         if constexpr (B_CONTIG) tb.issue(lb, count);
-        else tb.issue(lb, count, WD_BK);
+        else tb.issue(lb, count, BK);
     });
     store_rows<T>(a, prod.acc, t, t.pos0 + prod.wave_m(), n0 + prod.wave_n());
 }
 
 // dW.
-template <typename T, int BM, int STAGES>
+template <typename T, int BM, int BK, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
-    using TA = WideStrided<BM>;
-    using TB = WideStrided<WD_BN>;
-    using Prod = WideProduct<T, BM, STAGES, TA, TB>;
+    using TA = WideStrided<BM, BK>;
+    using TB = WideStrided<WD_BN, BK>;
+    using Prod = WideProduct<T, BM, BK, STAGES, TA, TB>;
     extern __shared__ __align__(16) uint16_t wide_lds[];
     uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
     const int64_t nt = w % a.n_tiles;
@@ -847,8 +890,8 @@ __global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
         D += begin * a.ldd;
         X += begin * a.ldx;
     }
-    const int64_t steps = (len + WD_BK - 1) / WD_BK;
-    const int first = (int)(len - (steps - 1) * WD_BK);
+    const int64_t steps = (len + BK - 1) / BK;
+    const int first = (int)(len - (steps - 1) * BK);
     TA ta;
     TB tb;
     const int look = len > 0 ? first : 0;
@@ -856,7 +899,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
     tb.init(X, a.ldx, a.K - c0, ord, look);
     Prod prod;
     prod.run(ta, tb, steps, wide_lds, [&](uint16_t *la, uint16_t *lb, int64_t s) {
-        const int count = s ? WD_BK : first, after = s + 1 < steps ? WD_BK : 0;
+        const int count = s ? BK : first, after = s + 1 < steps ? BK : 0;
         ta.issue(la, count, after);
         tb.issue(lb, count, after);
     });
@@ -943,9 +986,9 @@ int launch_rows(hipStream_t st, const fl_linear *op, RowsArgs &a, const char *wh
     const dim3 g((unsigned)grid), nt(LN_NT);
     if constexpr (sizeof(T) == 2) {
         if (wide == 256)
-            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 256, 2>), g, dim3(WD_NT), 2 * 512 * WD_BK * 2, st, a);
+            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 256, 32, 4>), g, dim3(WD_NT), 4 * 512 * 32 * 2, st, a);
         else if (wide)
-            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 128, 3>), g, dim3(WD_NT), 3 * 384 * WD_BK * 2, st, a);
+            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 128, 64, 3>), g, dim3(WD_NT), 3 * 384 * 64 * 2, st, a);
         if (wide) return fl_check_launch(what);
     }
     if (bn == 128) FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 128, 128, BIG_K>), g, nt, 0, st, a);
@@ -1086,7 +1129,7 @@ int weight_grad(hipStream_t st, const fl_linear *op, const void *d, void *dw, fl
     const dim3 g((unsigned)grid), nt(LN_NT);
     if constexpr (sizeof(T) == 2) {
         if (p.wide)
-            FL_LAUNCH("k_wide_outer", (k_wide_outer<T, 256, 2>), g, dim3(WD_NT), 2 * 512 * WD_BK * 2, st, a);
+            FL_LAUNCH("k_wide_outer", (k_wide_outer<T, 256, 32, 4>), g, dim3(WD_NT), 4 * 512 * 32 * 2, st, a);
     }
     if (p.wide) {
     } else if (p.tn == 128) FL_LAUNCH("k_lin_outer", (k_lin_outer<T, 128, 128, BIG_K>), g, nt, 0, st, a);
