@@ -782,17 +782,24 @@ struct WideProduct {
             for (int j = 0; j < NTL; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
         if (steps <= 0) return;
         const bool second = fl_wave_id() >= WD_WAVES / 2;
+        const auto load = [&](int64_t step) {
+            uint16_t *to = lds + (int)(step % STAGES) * ELEMS;
+            feed(to, to + TA::ELEMS, step);
+        };
 #pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s)
-            if (s < steps) feed(lds + s * ELEMS, lds + s * ELEMS + TA::ELEMS, s);
-        if (steps < STAGES - 1) wait<0>();
-        else wait<LOADS *(STAGES - 2)>();
+        for (int s = 0; s < STAGES; ++s)
+            if (s < steps) load(s);
+        if (steps < STAGES) wait<0>();
+        else wait<LOADS *(STAGES - 1)>();
         meet();
         if (second) meet();
-        int at = 0;
+        // Phase 2s: the first half reads step s, phase 2s + 1: it multiplies;
+        // the second half one phase later.  In phase 2s + 2 both have read
+        // step s and both load step s + STAGES over it; step s + 1 has to
+        // have landed when phase 2s + 1 ends.
         for (int64_t s = 0; s < steps; ++s) {
-            // this half reads step s while the other multiplies
-            const uint16_t *la = lds + at * ELEMS, *lb = la + TA::ELEMS;
+            const uint16_t *la = lds + (int)(s % STAGES) * ELEMS, *lb = la + TA::ELEMS;
+            const bool full = s + STAGES - 1 < steps;  // as many steps under way as there can be
             u32x4 fa[BK / 32][MT], fb[BK / 32][NTL];
 #pragma unroll
             for (int ks = 0; ks < BK / 32; ++ks) {
@@ -801,13 +808,13 @@ struct WideProduct {
 #pragma unroll
                 for (int i = 0; i < MT; ++i) fa[ks][i] = ta.frag(la, wave_m() + i * 16, ks);
             }
-            if (s + STAGES - 1 < steps) {
-                // over step s - 1, which both halves have read
-                const int to = at == 0 ? STAGES - 1 : at - 1;
-                feed(lds + to * ELEMS, lds + to * ELEMS + TA::ELEMS, s + STAGES - 1);
-                wait<LOADS *(STAGES - 2)>();  // step s + 1 has landed
-            } else wait<0>();
+            if (!second && s > 0 && full) load(s + STAGES - 1);
+            if (second) {
+                if (full) wait<LOADS *(STAGES - 2)>();
+                else wait<0>();
+            } else wait_lds();
             meet();
+            if (second && s + STAGES < steps) load(s + STAGES);
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int ks = 0; ks < BK / 32; ++ks)
@@ -816,11 +823,15 @@ struct WideProduct {
 #pragma unroll
                     for (int j = 0; j < NTL; ++j) acc[i][j] = mfma<T>(fb[ks][j], fa[ks][i], acc[i][j]);
             __builtin_amdgcn_s_setprio(0);
+            if (!second) {
+                if (full) wait<LOADS *(STAGES - 2)>();
+                else wait<0>();
+            }
             meet();
-            at = at + 1 == STAGES ? 0 : at + 1;
         }
         if (!second) meet();
     }
+    static __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xc07f); }
     // Waits for this wave's LDS reads and for all but its last VM memory loads
     // (s_waitcnt: vmcnt in bits 0-3 and 14-15, expcnt 4-6, lgkmcnt 8-11).
     template <int VM>
@@ -986,7 +997,7 @@ int launch_rows(hipStream_t st, const fl_linear *op, RowsArgs &a, const char *wh
     const dim3 g((unsigned)grid), nt(LN_NT);
     if constexpr (sizeof(T) == 2) {
         if (wide == 256)
-            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 256, 32, 4>), g, dim3(WD_NT), 4 * 512 * 32 * 2, st, a);
+            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 256, 64, 2>), g, dim3(WD_NT), 2 * 512 * 64 * 2, st, a);
         else if (wide)
             FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 128, 64, 3>), g, dim3(WD_NT), 3 * 384 * 64 * 2, st, a);
         if (wide) return fl_check_launch(what);
@@ -1129,7 +1140,7 @@ int weight_grad(hipStream_t st, const fl_linear *op, const void *d, void *dw, fl
     const dim3 g((unsigned)grid), nt(LN_NT);
     if constexpr (sizeof(T) == 2) {
         if (p.wide)
-            FL_LAUNCH("k_wide_outer", (k_wide_outer<T, 256, 32, 4>), g, dim3(WD_NT), 4 * 512 * 32 * 2, st, a);
+            FL_LAUNCH("k_wide_outer", (k_wide_outer<T, 256, 64, 2>), g, dim3(WD_NT), 2 * 512 * 64 * 2, st, a);
     }
     if (p.wide) {
     } else if (p.tn == 128) FL_LAUNCH("k_lin_outer", (k_lin_outer<T, 128, 128, BIG_K>), g, nt, 0, st, a);
