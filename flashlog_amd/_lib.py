@@ -255,8 +255,10 @@ _SIGS = {
     "fl_group_rows": (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_void_p] * 4 +
                       [ctypes.c_size_t]),
     "fl_linear_op_bytes": (ctypes.c_size_t, []),
-    "fl_linear_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 2),
-    "fl_linear_backward_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLinear)] + [ctypes.c_int] * 2),
+    "fl_linear_forward_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLinear)]),
+    "fl_linear_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 3 +
+                          [ctypes.c_size_t]),
+    "fl_linear_backward_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLinear)] + [ctypes.c_int] * 3),
     "fl_linear_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLinear)] + [ctypes.c_void_p] * 5 +
                            [ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t]),
     "fl_logits_op_bytes": (ctypes.c_size_t, []),

@@ -183,7 +183,10 @@ def _linear_forward(x, weight, bias, residual, plan, act, keep):
         residual = _rows_of(residual, N)
     pre = torch.empty((x.shape[0], N), dtype=torch.float32, device=dev) if keep else None
     op = _linear_op(x, weight, bias, residual, plan, act)
-    _launch("linear", _lib_handle().fl_linear_forward, dev, op, y.data_ptr(), _ptr(pre))
+    lib = _lib_handle()
+    nbytes = lib.fl_linear_forward_bytes(op)
+    ws = _workspace(nbytes, dev)
+    _launch("linear", lib.fl_linear_forward, dev, op, y.data_ptr(), _ptr(pre), _ptr(ws), nbytes)
     return y, x, weight, pre
 
 
@@ -216,7 +219,7 @@ class _LinearFunction(autograd.Function):
                 dw = torch.empty(weight.shape, dtype=x.dtype, device=dev)
             if need_b:
                 db = torch.empty(weight.shape[:-1], dtype=bias_dtype, device=dev)
-            nbytes = lib.fl_linear_backward_bytes(op, need_w, need_b)
+            nbytes = lib.fl_linear_backward_bytes(op, need_x, need_w, need_b)
             ws = _workspace(nbytes, dev)
             _launch("linear", lib.fl_linear_backward, dev, op, g.data_ptr(), _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db),
                     bias_dtype is torch.float32, _ptr(ws), nbytes)
@@ -430,7 +433,8 @@ def _logits_forward(c, logits, bias, softmax):
     op = c.op(x, bias)
     if softmax:
         nbytes = lib.fl_logits_softmax_bytes(op)
-        _launch("hop_attention", lib.fl_logits_softmax, dev, op, out.data_ptr(), _ptr(_workspace(nbytes, dev)), nbytes)
+        ws = _workspace(nbytes, dev)
+        _launch("hop_attention", lib.fl_logits_softmax, dev, op, out.data_ptr(), _ptr(ws), nbytes)
     else:
         _launch("constrain_logits", lib.fl_logits_constrain, dev, op, out.data_ptr())
     return out, x

@@ -429,6 +429,8 @@ struct RowsArgs {
     int64_t bias_group, ldres;
     float *pre;
     int act, bias_f32, block;
+    uint32_t parts;  // of K
+    float *part;     // [parts][M][N] sums without the epilogue, when parts > 1
 };
 
 // A tile of a product: its group (`none`: the rows of no group) and the places
@@ -515,6 +517,64 @@ __device__ __forceinline__ void store_rows(const RowsArgs &a, const f32x4 (&acc)
     }
 }
 
+// The sums of a part of K (one group of all rows).
+template <int MT, int NTL>
+__device__ __forceinline__ void store_part(const RowsArgs &a, const f32x4 (&acc)[MT][NTL], uint32_t part, int64_t pos,
+                                           int64_t col) {
+    const int lane = fl_lane();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t row = pos + i * 16 + (lane & 15);
+        if (row >= a.M) continue;
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) {
+            const int64_t n = col + j * 16 + (lane >> 4) * 4;
+            if (n >= a.N) continue;
+            float *q = a.part + ((int64_t)part * a.M + row) * a.N + n;
+            const Vec<float, 4> f{{acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]}};
+            if (a.N - n >= 4) store_vec<float, 4>(q, f);
+            else store_some<float, 4>(q, f, (int)(a.N - n));
+        }
+    }
+}
+
+// Joins the parts of K in order and finishes as store_rows does, four columns
+// a thread.
+template <typename T>
+__global__ __launch_bounds__(LN_NT) void k_lin_finish(RowsArgs a) {
+    const uint32_t quads = (uint32_t)((a.N + 3) / 4);
+    const int64_t i = (int64_t)blockIdx.x * LN_NT + threadIdx.x;
+    if (i >= a.M * quads) return;
+    const int64_t row = i / quads, n = (i % quads) * 4;
+    const int have = a.N - n < 4 ? (int)(a.N - n) : 4;
+    float v[4] = {0, 0, 0, 0}, t[4];
+    for (uint32_t p = 0; p < a.parts; ++p) {
+        load_some<float>(a.part + ((int64_t)p * a.M + row) * a.N + n, have, t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += t[e];
+    }
+    if (a.bias) {
+        if (a.bias_f32) load_some<float>((const float *)a.bias + n, have, t);
+        else load_some<T>((const T *)a.bias + n, have, t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += t[e];
+    }
+    if (a.pre) store_some<float, 4>(a.pre + row * a.N + n, Vec<float, 4>{{v[0], v[1], v[2], v[3]}}, have);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = act_value(v[e], a.act);
+    if (a.residual) {
+        load_some<T>((const T *)a.residual + row * a.ldres + n, have, t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += t[e];
+    }
+    Vec<T, 4> o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o.v[e] = (T)v[e];
+    T *q = (T *)a.c + row * a.ldc + n;
+    if (have == 4) store_vec<T, 4>(q, o);
+    else store_some<T, 4>(q, o, have);
+}
+
 // Products whose C rows are the batch's rows (the forward, and dx): a tile is
 // BM rows of one group.
 template <typename T, bool B_CONTIG, int BM, int BN, int BK>
@@ -522,28 +582,33 @@ __global__ __launch_bounds__(LN_NT) void k_lin_rows(RowsArgs a) {
     using Prod = Product<T, BM, BN, BK>;
     __shared__ __align__(16) uint16_t lds[Prod::LDS_ELEMS];
     const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    const uint32_t tile = w / a.parts, part = w % a.parts;
     RowTile t;
-    if (!row_tile<BM>(a, w / a.n_tiles, &t)) return;
-    const int64_t n0 = (int64_t)(w % a.n_tiles) * BN;
+    if (!row_tile<BM>(a, tile / a.n_tiles, &t)) return;
+    const int64_t n0 = (int64_t)(tile % a.n_tiles) * BN;
+    // whole steps of K a part; the last has the end of K
+    const int64_t steps = (a.K + BK - 1) / BK, k0 = steps * part / a.parts * BK;
+    const int64_t k1 = part + 1 == a.parts ? a.K : steps * (part + 1) / a.parts * BK;
     const T *A = (const T *)a.a;
     const T *B = (const T *)a.b + (t.none ? 0 : t.g * a.b_group);
     ContigTile<T, BM, BK> ta;
     ta.init([&](int r) {
         const int64_t p = t.pos0 + r < t.end ? t.pos0 + r : t.end - 1;
-        return A + (a.order ? (int64_t)a.order[p] : p) * a.lda;
+        return A + (a.order ? (int64_t)a.order[p] : p) * a.lda + k0;
     });
     Prod prod;
-    const int64_t K = t.none ? 0 : a.K;
+    const int64_t K = t.none ? 0 : k1 - k0;
     if constexpr (B_CONTIG) {
         ContigTile<T, BN, BK> tb;
-        tb.init([&](int r) { return B + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldb; });
+        tb.init([&](int r) { return B + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldb + k0; });
         prod.run(ta, tb, K, lds);
     } else {
         StridedTile<T, BN, BK> tb;
-        tb.init(B + n0, a.ldb, a.N - n0, nullptr);
+        tb.init(B + k0 * a.ldb + n0, a.ldb, a.N - n0, nullptr);
         prod.run(ta, tb, K, lds);
     }
-    store_rows<T>(a, prod.acc, t, t.pos0 + prod.wave_m(), n0 + prod.wave_n());
+    if (a.part) store_part(a, prod.acc, part, t.pos0 + prod.wave_m(), n0 + prod.wave_n());
+    else store_rows<T>(a, prod.acc, t, t.pos0 + prod.wave_m(), n0 + prod.wave_n());
 }
 
 struct OuterArgs {
@@ -961,12 +1026,42 @@ __global__ __launch_bounds__(LN_NT) void k_col_sums(const T *__restrict__ d, int
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Rows of a tile: the plan's, or for one group the largest tile that gives
-// every CU one and a half workgroups, down to 32.
-int tile_rows(const fl_linear *op, int64_t cols) {
-    if (op->offsets) return (int)fl_group_block(op->M, op->groups);
-    if (ceil_div(op->M, 128) * ceil_div(cols, 128) >= 384) return 128;
-    return ceil_div(op->M, 64) * ceil_div(cols, 64) >= 128 ? 64 : 32;
+// How a product is cut: tiles of `rows` rows (and 128 or 64 columns), and
+// parts of its inner dimension whose sums a second launch joins.
+struct Cut {
+    int rows, parts;
+};
+
+// The fastest cut of an [M, N] product over K, by what the kernels measured.
+// A 32-value step of a tile takes `alone` microseconds where CUs hold one
+// workgroup, `shared` times the workgroups of a CU where they hold more (fp32:
+// [1536 x 2048 -> 1645] takes 147 us in 156 tiles of 128, 101 us in 624 tiles
+// of 64; [8192 x 2048 -> 2048] 370 us in tiles of 128); joining parts takes a
+// launch and their traffic.
+Cut best_cut(int64_t M, int64_t N, int64_t K, bool f32, bool small_tiles) {
+    struct Tile {
+        int rows, cols;
+        double alone, shared;
+    };
+    static const Tile wide[3] = {{128, 128, 2.3, 1.45}, {64, 64, 1.2, 0.52}, {32, 64, 0.52, 0.3}};
+    const double scale = f32 ? 1.0 : 0.35;
+    const double steps = (double)ceil_div(K, 32);
+    Cut best{64, 1};
+    double least = 1e30;
+    for (const Tile &t : wide) {
+        if (t.rows == 32 && !small_tiles) continue;
+        const int64_t tiles = ceil_div(M, t.rows) * ceil_div(N, t.rows == 128 && N <= 64 ? 64 : t.cols);
+        for (int parts = 1; parts <= 16 && (parts == 1 || K / parts >= 128); ++parts) {
+            const double shared = t.shared * (double)ceil_div(tiles * parts, 256);
+            double us = steps / parts * scale * (shared > t.alone ? shared : t.alone);
+            if (parts > 1) us += 4.0 + (double)parts * M * N * 8e-6 / 4.0;
+            if (us < least) {
+                least = us;
+                best = Cut{t.rows, parts};
+            }
+        }
+    }
+    return best;
 }
 
 bool aligned(const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
@@ -982,16 +1077,30 @@ int wide_rows(const fl_linear *op, const RowsArgs &a, bool b_contig) {
     return ceil_div(op->M, 128) * cols >= 128 ? 128 : 0;
 }
 
+// The cut of y's or dx's product that the wide kernels do not take.
+Cut rows_cut(const fl_linear *op, int64_t N, int64_t K) {
+    if (op->offsets) return Cut{(int)fl_group_block(op->M, op->groups), 1};
+    return best_cut(op->M, N, K, op->dtype == FL_F32, true);
+}
+
+size_t rows_bytes(const fl_linear *op, int64_t N, int64_t K) {
+    const Cut c = rows_cut(op, N, K);
+    return c.parts > 1 ? (size_t)c.parts * op->M * N * 4 : 0;
+}
+
 template <typename T, bool B_CONTIG>
-int launch_rows(hipStream_t st, const fl_linear *op, RowsArgs &a, const char *what) {
+int launch_rows(hipStream_t st, const fl_linear *op, RowsArgs &a, float *ws, const char *what) {
     a.block = (int)fl_group_block(op->M, op->groups);
     const int wide = sizeof(T) == 2 ? wide_rows(op, a, B_CONTIG) : 0;
-    const int bm = wide ? wide : tile_rows(op, a.N);
+    const Cut cut = wide ? Cut{wide, 1} : rows_cut(op, a.N, a.K);
+    const int bm = cut.rows;
+    a.parts = (uint32_t)cut.parts;
+    a.part = cut.parts > 1 ? ws : nullptr;
     constexpr int BIG_K = sizeof(T) == 4 ? 32 : 64;
     const int bn = wide ? WD_BN : bm == 128 && a.N > 64 ? 128 : 64;
     const int64_t m_tiles = op->offsets ? fl_group_tiles(op->M, op->groups) * (a.block / bm) : ceil_div(op->M, bm);
     a.n_tiles = (uint32_t)ceil_div(a.N, bn);
-    const int64_t grid = m_tiles * a.n_tiles;
+    const int64_t grid = m_tiles * a.n_tiles * a.parts;
     if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "%s: too many tiles for one launch (shape)", what);
     if (grid == 0) return FL_OK;
     const dim3 g((unsigned)grid), nt(LN_NT);
@@ -1006,6 +1115,9 @@ int launch_rows(hipStream_t st, const fl_linear *op, RowsArgs &a, const char *wh
     else if (bm == 128) FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 128, 64, BIG_K>), g, nt, 0, st, a);
     else if (bm == 64) FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 64, 64, BIG_K>), g, nt, 0, st, a);
     else FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 32, 64, 64>), g, nt, 0, st, a);
+    if (a.part)
+        FL_LAUNCH("k_lin_finish", k_lin_finish<T>, dim3((unsigned)ceil_div(a.M * ceil_div(a.N, 4), LN_NT)), nt, 0, st,
+                  a);
     return fl_check_launch(what);
 }
 
@@ -1047,6 +1159,13 @@ OuterPlan outer_plan(const fl_linear *op) {
         p.wide = p.tiles * op->groups * p.parts >= 128;
         if (p.wide) return p;
     }
+    if (op->groups == 1) {
+        const Cut c = best_cut(op->N, op->K, op->M, op->dtype == FL_F32, false);
+        const int t = c.rows == 128 && op->N >= 2 && op->K >= 2 ? 128 : 64;
+        fill(t, t);
+        p.parts = c.parts;
+        return p;
+    }
     fill(128, 128);
     if (op->N < 128 || op->K < 128 || p.tiles * op->groups < 384) fill(64, 64);
     p.parts = outer_parts(op->M, op->groups, p.tiles < 1 ? 1 : p.tiles, 1024);
@@ -1067,7 +1186,7 @@ int check_op(const fl_linear *op, const char *what) {
 }
 
 template <typename T>
-int forward(hipStream_t st, const fl_linear *op, void *y, float *pre) {
+int forward(hipStream_t st, const fl_linear *op, void *y, float *pre, float *ws) {
     RowsArgs a{};
     a.a = op->x;
     a.lda = op->ldx;
@@ -1090,11 +1209,11 @@ int forward(hipStream_t st, const fl_linear *op, void *y, float *pre) {
     a.ldres = op->ldres;
     a.pre = pre;
     a.act = op->act;
-    return launch_rows<T, true>(st, op, a, "linear_forward");
+    return launch_rows<T, true>(st, op, a, ws, "linear_forward");
 }
 
 template <typename T>
-int input_grad(hipStream_t st, const fl_linear *op, const void *d, void *dx) {
+int input_grad(hipStream_t st, const fl_linear *op, const void *d, void *dx, float *ws) {
     RowsArgs a{};
     a.a = d;
     a.lda = op->N;
@@ -1110,7 +1229,7 @@ int input_grad(hipStream_t st, const fl_linear *op, const void *d, void *dx) {
     a.order = op->order;
     a.offsets = op->offsets;
     a.tiles = op->tiles;
-    return launch_rows<T, false>(st, op, a, "linear_input_grad");
+    return launch_rows<T, false>(st, op, a, ws, "linear_backward");
 }
 
 template <typename T>
@@ -1170,41 +1289,46 @@ int act_grad(hipStream_t st, int act, const void *gy, const float *pre, int64_t 
     return fl_check_launch("linear_backward");
 }
 
-// The backward's workspace: d (when there is an activation), the parts of dW
-// and those of db.
+// The backward's workspace: d (when there is an activation), and the parts of
+// dx, dW and db, one after the other in the same place.
 struct BackwardSpace {
-    size_t d, dw, db, bytes;
+    size_t d, parts, bytes;
 };
 
-BackwardSpace backward_space(const fl_linear *op, int with_dw, int with_db) {
-    BackwardSpace s{0, 0, 0, 0};
+BackwardSpace backward_space(const fl_linear *op, int with_dx, int with_dw, int with_db) {
+    BackwardSpace s{0, 0, 0};
     const auto take = [&](size_t n) {
         const size_t at = s.bytes;
         s.bytes += (n + 255) / 256 * 256;
         return at;
     };
     if (op->act != FL_ACT_NONE) s.d = take((size_t)op->M * op->N * (op->dtype == FL_F32 ? 4 : 2));
+    size_t most = 0;
+    const auto need = [&](size_t n) { most = n > most ? n : most; };
+    if (with_dx && op->M && op->K) need(rows_bytes(op, op->K, op->N));
     if (with_dw && op->N && op->K) {
         const int parts = outer_plan(op).parts;
-        s.dw = take(parts > 1 ? (size_t)parts * op->groups * op->N * op->K * 4 : 0);
+        if (parts > 1) need((size_t)parts * op->groups * op->N * op->K * 4);
     }
-    if (with_db && op->N) s.db = take((size_t)sum_parts(op->M, op->N, op->groups) * op->groups * op->N * 4);
+    if (with_db && op->N) need((size_t)sum_parts(op->M, op->N, op->groups) * op->groups * op->N * 4);
+    s.parts = take(most);
     return s;
 }
 
 template <typename T>
 int backward(hipStream_t st, const fl_linear *op, const void *gy, const float *pre, void *dx, void *dw, void *db,
              int db_f32, char *ws) {
-    const BackwardSpace s = backward_space(op, dw != nullptr, db != nullptr);
+    const BackwardSpace s = backward_space(op, dx != nullptr, dw != nullptr, db != nullptr);
+    float *parts = (float *)(ws + s.parts);
     const void *d = gy;
     int rc = FL_OK;
     if (op->act != FL_ACT_NONE && op->M && op->N) {
         rc = act_grad<T>(st, op->act, gy, pre, op->M * op->N, ws + s.d);
         d = ws + s.d;
     }
-    if (!rc && dx && op->M && op->K) rc = input_grad<T>(st, op, d, dx);
-    if (!rc && dw && op->N && op->K) rc = weight_grad<T>(st, op, d, dw, (float *)(ws + s.dw));
-    if (!rc && db && op->N) rc = bias_grad<T>(st, op, d, db, db_f32, (float *)(ws + s.db));
+    if (!rc && dx && op->M && op->K) rc = input_grad<T>(st, op, d, dx, parts);
+    if (!rc && dw && op->N && op->K) rc = weight_grad<T>(st, op, d, dw, parts);
+    if (!rc && db && op->N) rc = bias_grad<T>(st, op, d, db, db_f32, parts);
     return rc;
 }
 
@@ -1222,18 +1346,25 @@ extern "C" {
 
 size_t fl_linear_op_bytes(void) { return sizeof(fl_linear); }
 
-int fl_linear_forward(void *stream, const fl_linear *op, void *y, float *pre) {
+size_t fl_linear_forward_bytes(const fl_linear *op) {
+    if (!op || op->M < 1 || op->N < 1 || op->K < 0 || op->groups < 1) return 0;
+    return fl::rows_bytes(op, op->N, op->K);
+}
+
+int fl_linear_forward(void *stream, const fl_linear *op, void *y, float *pre, void *ws, size_t ws_bytes) {
     const int rc = fl::check_op(op, "linear_forward");
     if (rc) return rc;
     if (op->M == 0 || op->N == 0) return FL_OK;
     if (!y || (op->K > 0 && (!op->x || !op->weight)))
         return fl::fl_fail(FL_ERR_ARG, "linear_forward: null pointer");
-    FL_BY_TYPE(op->dtype, fl::forward<T>((hipStream_t)stream, op, y, pre))
+    const size_t need = fl_linear_forward_bytes(op);
+    if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "linear_forward: workspace too small");
+    FL_BY_TYPE(op->dtype, fl::forward<T>((hipStream_t)stream, op, y, pre, (float *)ws))
 }
 
-size_t fl_linear_backward_bytes(const fl_linear *op, int with_dw, int with_db) {
+size_t fl_linear_backward_bytes(const fl_linear *op, int with_dx, int with_dw, int with_db) {
     if (!op || op->M < 0 || op->N < 0 || op->K < 0 || op->groups < 1) return 0;
-    return fl::backward_space(op, with_dw, with_db).bytes;
+    return fl::backward_space(op, with_dx, with_dw, with_db).bytes;
 }
 
 int fl_linear_backward(void *stream, const fl_linear *op, const void *gy, const float *pre, void *dx, void *dw,
@@ -1244,7 +1375,7 @@ int fl_linear_backward(void *stream, const fl_linear *op, const void *gy, const 
     if ((any && (!gy || (op->act != FL_ACT_NONE && !pre))) || (any && dx && op->K > 0 && !op->weight) ||
         (any && dw && op->K > 0 && !op->x))
         return fl::fl_fail(FL_ERR_ARG, "linear_backward: null pointer");
-    const size_t need = fl_linear_backward_bytes(op, dw != nullptr, db != nullptr);
+    const size_t need = fl_linear_backward_bytes(op, dx != nullptr, dw != nullptr, db != nullptr);
     if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "linear_backward: workspace too small");
     if ((uintptr_t)ws % 16) return fl::fl_fail(FL_ERR_ARG, "linear_backward: workspace must be 16-byte aligned");
     FL_BY_TYPE(op->dtype, fl::backward<T>((hipStream_t)stream, op, gy, pre, dx, dw, db, db_f32, (char *)ws))

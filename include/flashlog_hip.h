@@ -875,13 +875,16 @@ typedef struct fl_linear {
 
 size_t fl_linear_op_bytes(void);
 /* pre [M, N], optional: the activation's argument, for the backward. */
-int fl_linear_forward(void *stream, const fl_linear *op, void *y, float *pre);
+size_t fl_linear_forward_bytes(const fl_linear *op);
+int fl_linear_forward(void *stream, const fl_linear *op, void *y, float *pre,
+                      void *ws, size_t ws_bytes);
 /* With d = gy * act'(pre) (gy [M, N] contiguous; pre unused without an
  * activation), those of the gradients that are not null: dx [M, K] = d W_g,
  * dw [groups, N, K] = d^T x and db [groups, N] = the sums of d over each
  * group's rows (0 for an empty group; db fp32 when db_f32, else of the
  * operands' type).  gy and ws lie on 16-byte boundaries. */
-size_t fl_linear_backward_bytes(const fl_linear *op, int with_dw, int with_db);
+size_t fl_linear_backward_bytes(const fl_linear *op, int with_dx, int with_dw,
+                                int with_db);
 int fl_linear_backward(void *stream, const fl_linear *op, const void *gy,
                        const float *pre, void *dx, void *dw, void *db,
                        int db_f32, void *ws, size_t ws_bytes);

@@ -55,7 +55,7 @@ def _linear_op(**kw):
 def test_linear_arguments():
     lib = _lib.lib()
     one = ctypes.c_void_p(1)
-    fwd = lambda op, y=one: _error(lib.fl_linear_forward(None, op, y, None))
+    fwd = lambda op, y=one: _error(lib.fl_linear_forward(None, op, y, None, None, 0))
     assert "type" in fwd(_linear_op(dtype=3))
     assert "activation" in fwd(_linear_op(act=6))
     assert "shape" in fwd(_linear_op(M=-1))
@@ -72,10 +72,10 @@ def test_linear_arguments():
     assert "workspace" in back(_linear_op(), one, None, None, None, one, None, 0)
     assert "workspace" in back(_linear_op(act=2), one, one, one, None, None, None, 0)
     long = _linear_op(M=100_000)
-    need = lib.fl_linear_backward_bytes(long, 1, 0)
+    need = lib.fl_linear_backward_bytes(long, 0, 1, 0)
     assert need > 0 and "workspace" in back(long, one, None, None, one, None, one, need - 1)
     # nothing to do is no error
-    assert lib.fl_linear_forward(None, _linear_op(M=0), None, None) == 0
+    assert lib.fl_linear_forward(None, _linear_op(M=0), None, None, None, 0) == 0
 
 
 def _logits_op(**kw):
