@@ -153,38 +153,54 @@ __device__ __forceinline__ void write_tiles(const GroupArgs &a, int *lds) {
     for (int64_t t = used + threadIdx.x; t < a.ntiles; t += GR_NT) a.tiles[2 * t] = -1;
 }
 
-// All rows in one workgroup and one digit.
+// One launch: every workgroup takes GR_NT rows, and counts the groups of all
+// rows itself, those before its own apart, so that none waits for another
+// (16384 rows in 16 workgroups; in one the ranks alone took 20 us).
 __global__ __launch_bounds__(GR_NT) void k_group_one(GroupArgs a) {
-    extern __shared__ uint16_t cnt[];
+    extern __shared__ uint8_t mine[];  // [waves][digits] of the workgroup's own rows
     __shared__ int lds[GR_WAVES + 1];
-    __shared__ int first[GR_DIGITS];
-    WaveRows rows;
-    rows.load(a);
-    clear_counts(cnt, a.digits);
+    __shared__ int first[GR_DIGITS], rest[GR_DIGITS];
+    const int64_t b0 = (int64_t)blockIdx.x * GR_NT, own = b0 + threadIdx.x;
+    for (int i = threadIdx.x; i < a.digits; i += GR_NT) first[i] = rest[i] = 0;
+    uint32_t *m32 = reinterpret_cast<uint32_t *>(mine);
+    for (int i = threadIdx.x; i < GR_WAVES * a.digits / 4; i += GR_NT) m32[i] = 0;
+    int key[GR_BLOCK_ROWS / GR_NT], digit = 0;
+#pragma unroll
+    for (int j = 0; j < (int)(GR_BLOCK_ROWS / GR_NT); ++j) {
+        const int64_t p = (int64_t)j * GR_NT + threadIdx.x;
+        key[j] = p < a.rows ? (int)group_key(a, p) : -1;
+        if (p == own) digit = key[j];
+    }
     __syncthreads();
-    uint16_t *mine = cnt + fl_wave_id() * a.digits;
-    rows.count(a, mine);
+#pragma unroll
+    for (int j = 0; j < (int)(GR_BLOCK_ROWS / GR_NT); ++j)
+        if (key[j] >= 0) atomicAdd(j < (int)blockIdx.x ? &first[key[j]] : &rest[key[j]], 1);
+    const bool active = own < a.rows;
+    const int wave = fl_wave_id();
+    const unsigned long long eq = equal_lanes(digit, active, a.bits);
+    int rank = 0;
+    if (active) {
+        rank = __popcll(eq & ((1ull << fl_lane()) - 1));
+        if (rank == 0) mine[wave * a.digits + digit] = (uint8_t)__popcll(eq);
+    }
     __syncthreads();
     block_scan(
-        a.digits, lds,
-        [&](int64_t d) {
-            int run = 0;
-            for (int w = 0; w < GR_WAVES; ++w) {
-                const int c = cnt[w * a.digits + d];
-                cnt[w * a.digits + d] = (uint16_t)run;
-                run += c;
-            }
-            return run;
-        },
+        a.digits, lds, [&](int64_t d) { return first[d] + rest[d]; },
         [&](int64_t d, int pre) {
-            first[d] = pre;
-            if (d <= a.groups) a.offsets[d] = pre;
+            first[d] += pre;
+            if (blockIdx.x == 0 && d <= a.groups) a.offsets[d] = pre;
         });
     __syncthreads();
-    rows.each([&](int32_t row, int d, int rank) { a.out_order[first[d] + mine[d] + rank] = row; });
-    __threadfence_block();
-    __syncthreads();
-    if (a.tiles) write_tiles(a, lds);
+    if (active) {
+        int at = first[digit] + rank;
+        for (int w = 0; w < wave; ++w) at += mine[w * a.digits + digit];
+        a.out_order[at] = (int32_t)own;
+    }
+    if (blockIdx.x == 0 && a.tiles) {
+        __threadfence_block();
+        __syncthreads();
+        write_tiles(a, lds);
+    }
 }
 
 __global__ __launch_bounds__(GR_NT) void k_group_count(GroupArgs a) {
@@ -273,7 +289,7 @@ bool one_launch(int64_t rows, int64_t groups) { return rows <= GR_BLOCK_ROWS && 
 
 extern "C" {
 
-int64_t fl_group_block(int64_t rows, int64_t groups) { return rows >= 512 * groups ? 128 : rows >= 32 * groups ? 64 : 32; }
+int64_t fl_group_block(int64_t rows, int64_t groups) { return rows >= 512 * groups ? 256 : rows >= 32 * groups ? 64 : 32; }
 
 int64_t fl_group_tiles(int64_t rows, int64_t groups) {
     if (rows <= 0) return 0;
@@ -310,9 +326,9 @@ int fl_group_rows(void *stream, const int64_t *index, int64_t rows, int64_t grou
     if (fl::one_launch(rows, groups)) {
         a.bits = bits;
         a.digits = 1 << bits;
-        a.nblocks = 1;
-        const size_t lds = (size_t)fl::GR_WAVES * a.digits * sizeof(uint16_t);
-        FL_LAUNCH("k_group_one", fl::k_group_one, dim3(1), dim3(fl::GR_NT), lds, st, a);
+        const int64_t nb = rows > 0 ? (rows + fl::GR_NT - 1) / fl::GR_NT : 1;
+        const size_t lds = (size_t)fl::GR_WAVES * (a.digits < 4 ? 4 : a.digits);
+        FL_LAUNCH("k_group_one", fl::k_group_one, dim3((unsigned)nb), dim3(fl::GR_NT), lds, st, a);
         return fl::fl_check_launch("group_rows");
     }
     a.nblocks = (rows + fl::GR_BLOCK_ROWS - 1) / fl::GR_BLOCK_ROWS;

@@ -910,6 +910,104 @@ struct WideProduct {
     }
 };
 
+// A wave's tiles through its own slice of the LDS, 64 rows at a time, so that
+// eight lanes store (and read the residual of) a whole 128-byte line of a row:
+// straight from the accumulators a store has 32 bytes a row, and the epilogue
+// took 15 us of a 256 x 256 tile.  f(row, col, v): eight columns of one row of
+// the wave's tile.
+constexpr int WD_SLICE = 64 * 68;  // floats: 64 rows, 4 floats apart in the banks
+
+template <int MT, typename F>
+__device__ __forceinline__ void wide_rows_out(const f32x4 (&acc)[MT][4], float *slice, F &&f) {
+    const int lane = fl_lane();
+#pragma unroll
+    for (int h = 0; h < MT / 4; ++h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<f32x4 *>(slice + (i * 16 + (lane & 15)) * 68 + j * 16 + (lane >> 4) * 4) =
+                    acc[h * 4 + i][j];
+        fl_wave_sync();
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int row = r * 8 + (lane >> 3), col = (lane & 7) * 8;
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(slice + row * 68 + col);
+            const f32x4 hi = *reinterpret_cast<const f32x4 *>(slice + row * 68 + col + 4);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = lo[e];
+                v[4 + e] = hi[e];
+            }
+            f(h * 64 + row, col, v);
+        }
+        fl_wave_sync();
+    }
+}
+
+// The first `have` of eight values as floats, the others 0.
+template <typename U>
+__device__ __forceinline__ void load_eight(const U *p, int have, float (&out)[8]) {
+    if (have >= 8) {
+        const Vec<U, 8> r = load_vec<U, 8>(p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = (float)r.v[e];
+    } else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = e < have ? (float)p[e] : 0.0f;
+}
+template <typename U>
+__device__ __forceinline__ void store_eight(U *p, int have, const float (&v)[8]) {
+    Vec<U, 8> o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o.v[e] = (U)v[e];
+    if (have >= 8) store_vec<U, 8>(p, o);
+    else store_some<U, 8>(p, o, have);
+}
+
+template <typename T, int MT>
+__device__ __forceinline__ void wide_store_rows(const RowsArgs &a, const f32x4 (&acc)[MT][4], const RowTile &t,
+                                                int64_t pos, int64_t col, float *slice) {
+    const int64_t n = col + (fl_lane() & 7) * 8;
+    const int have = a.N - n < 8 ? (int)(a.N - n) : 8;
+    float bias[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (a.bias && !t.none && have > 0) {
+        if (a.bias_f32) load_eight<float>((const float *)a.bias + t.g * a.bias_group + n, have, bias);
+        else load_eight<T>((const T *)a.bias + t.g * a.bias_group + n, have, bias);
+    }
+    wide_rows_out<MT>(acc, slice, [&](int r, int, float (&v)[8]) {
+        const int64_t p = pos + r;
+        if (p >= t.end || have <= 0) return;
+        const int64_t row = a.order ? (int64_t)a.order[p] : p;
+        float res[8];
+        if (a.residual) load_eight<T>((const T *)a.residual + row * a.ldres + n, have, res);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += bias[e];
+        if (a.pre) store_eight<float>(a.pre + row * a.N + n, have, v);
+        if (!t.none)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = act_value(v[e], a.act);
+        if (a.residual)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += res[e];
+        store_eight<T>((T *)a.c + row * a.ldc + n, have, v);
+    });
+}
+
+template <typename T, int MT>
+__device__ __forceinline__ void wide_store_outer(const OuterArgs &a, const f32x4 (&acc)[MT][4], int64_t g, int part,
+                                                 int64_t row, int64_t col, float *slice) {
+    const int64_t NK = a.N * a.K, c = col + (fl_lane() & 7) * 8;
+    const int have = a.K - c < 8 ? (int)(a.K - c) : 8;
+    wide_rows_out<MT>(acc, slice, [&](int r, int, float (&v)[8]) {
+        const int64_t m = row + r;
+        if (m >= a.N || have <= 0) return;
+        if (a.part) store_eight<float>(a.part + ((int64_t)part * a.groups + g) * NK + m * a.K + c, have, v);
+        else store_eight<T>((T *)a.dw + g * NK + m * a.K + c, have, v);
+    });
+}
+
 // The forward (B_CONTIG) and dx.
 template <typename T, bool B_CONTIG, int BM, int BK, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
@@ -940,7 +1038,9 @@ __global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
         if constexpr (B_CONTIG) tb.issue(lb, count);
         else tb.issue(lb, count, BK);
     });
-    store_rows<T>(a, prod.acc, t, t.pos0 + prod.wave_m(), n0 + prod.wave_n());
+    __syncthreads();  // the operands in the LDS are read
+    wide_store_rows<T>(a, prod.acc, t, t.pos0 + prod.wave_m(), n0 + prod.wave_n(),
+                       reinterpret_cast<float *>(wide_lds) + fl_wave_id() * WD_SLICE);
 }
 
 // dW.
@@ -979,7 +1079,9 @@ __global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
         ta.issue(la, count, after);
         tb.issue(lb, count, after);
     });
-    store_outer<T>(a, prod.acc, g, part, m0 + prod.wave_m(), c0 + prod.wave_n());
+    __syncthreads();  // the operands in the LDS are read
+    wide_store_outer<T>(a, prod.acc, g, part, m0 + prod.wave_m(), c0 + prod.wave_n(),
+                        reinterpret_cast<float *>(wide_lds) + fl_wave_id() * WD_SLICE);
 }
 
 // d = gy * act'(p), rounded to the operands' type: it is an operand of two products.
@@ -1064,6 +1166,12 @@ Cut best_cut(int64_t M, int64_t N, int64_t K, bool f32, bool small_tiles) {
     return best;
 }
 
+// LDS of a wide kernel: its operands' buffers, or the waves' slices behind them.
+constexpr unsigned wide_bytes(int bm, int bk, int stages) {
+    const int operands = stages * (bm + WD_BN) * bk * 2, slices = WD_WAVES * WD_SLICE * 4;
+    return (unsigned)(operands > slices ? operands : slices);
+}
+
 bool aligned(const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
 
 // Rows of the wide kernels' tiles, 0: the operands or the sizes are not for them.
@@ -1072,14 +1180,17 @@ int wide_rows(const fl_linear *op, const RowsArgs &a, bool b_contig) {
         (!b_contig && a.N % 8) || a.N < 192)
         return 0;
     const int64_t cols = ceil_div(a.N, WD_BN);
-    if (op->offsets) return fl_group_block(op->M, op->groups) == 128 && ceil_div(op->M, 128) * cols >= 128 ? 128 : 0;
+    if (op->offsets) return fl_group_block(op->M, op->groups) == 256 && ceil_div(op->M, 256) * cols >= 64 ? 256 : 0;
     if (ceil_div(op->M, 256) * cols >= 192) return 256;
     return ceil_div(op->M, 128) * cols >= 128 ? 128 : 0;
 }
 
 // The cut of y's or dx's product that the wide kernels do not take.
 Cut rows_cut(const fl_linear *op, int64_t N, int64_t K) {
-    if (op->offsets) return Cut{(int)fl_group_block(op->M, op->groups), 1};
+    if (op->offsets) {
+        const int block = (int)fl_group_block(op->M, op->groups);
+        return Cut{block < 128 ? block : 128, 1};
+    }
     return best_cut(op->M, N, K, op->dtype == FL_F32, true);
 }
 
@@ -1106,9 +1217,9 @@ int launch_rows(hipStream_t st, const fl_linear *op, RowsArgs &a, float *ws, con
     const dim3 g((unsigned)grid), nt(LN_NT);
     if constexpr (sizeof(T) == 2) {
         if (wide == 256)
-            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 256, 64, 2>), g, dim3(WD_NT), 2 * 512 * 64 * 2, st, a);
+            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 256, 64, 2>), g, dim3(WD_NT), wide_bytes(256, 64, 2), st, a);
         else if (wide)
-            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 128, 64, 3>), g, dim3(WD_NT), 3 * 384 * 64 * 2, st, a);
+            FL_LAUNCH("k_wide_rows", (k_wide_rows<T, B_CONTIG, 128, 64, 3>), g, dim3(WD_NT), wide_bytes(128, 64, 3), st, a);
         if (wide) return fl_check_launch(what);
     }
     if (bn == 128) FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 128, 128, BIG_K>), g, nt, 0, st, a);
@@ -1259,7 +1370,7 @@ int weight_grad(hipStream_t st, const fl_linear *op, const void *d, void *dw, fl
     const dim3 g((unsigned)grid), nt(LN_NT);
     if constexpr (sizeof(T) == 2) {
         if (p.wide)
-            FL_LAUNCH("k_wide_outer", (k_wide_outer<T, 256, 64, 2>), g, dim3(WD_NT), 2 * 512 * 64 * 2, st, a);
+            FL_LAUNCH("k_wide_outer", (k_wide_outer<T, 256, 64, 2>), g, dim3(WD_NT), wide_bytes(256, 64, 2), st, a);
     }
     if (p.wide) {
     } else if (p.tn == 128) FL_LAUNCH("k_lin_outer", (k_lin_outer<T, 128, 128, BIG_K>), g, nt, 0, st, a);
