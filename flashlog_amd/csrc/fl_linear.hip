@@ -396,6 +396,22 @@ __device__ __forceinline__ float act_value(float p, int act) {
     }
 }
 
+template <int N>
+__device__ __forceinline__ void act_values(float (&v)[N], int act) {
+    const auto each = [&](auto known) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = act_value(v[e], decltype(known)::value);
+    };
+    switch (act) {
+        case FL_ACT_RELU: return each(std::integral_constant<int, FL_ACT_RELU>());
+        case FL_ACT_GELU: return each(std::integral_constant<int, FL_ACT_GELU>());
+        case FL_ACT_SILU: return each(std::integral_constant<int, FL_ACT_SILU>());
+        case FL_ACT_TANH: return each(std::integral_constant<int, FL_ACT_TANH>());
+        case FL_ACT_SIGMOID: return each(std::integral_constant<int, FL_ACT_SIGMOID>());
+        default: return;
+    }
+}
+
 __device__ __forceinline__ float act_slope(float p, int act) {
     switch (act) {
         case FL_ACT_RELU: return p > 0.0f ? 1.0f : (p != p ? p : 0.0f);
@@ -738,93 +754,140 @@ struct WideContig {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) p[i] = row_ptr(row(i)) + chunk(i) * 8;
     }
-    // The next `count` <= BK values of k.
+    // The next `count` values of k, BK if WHOLE.
+    template <bool WHOLE>
     __device__ __forceinline__ void issue(uint16_t *lds, int count) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const void *q = chunk(i) * 8 < count ? (const void *)p[i] : (const void *)wd_zeros;
+            const void *q = WHOLE || chunk(i) * 8 < count ? (const void *)p[i] : (const void *)wd_zeros;
             load_lds(q, lds + (fl_wave_id() * LOADS + i) * 512);
             p[i] += count;
         }
     }
-    __device__ __forceinline__ u32x4 frag(const uint16_t *lds, int row0, int ks) const {
-        return *reinterpret_cast<const u32x4 *>(lds + lds_at<BK>(row0 + (fl_lane() & 15), ks * 4 + (fl_lane() >> 4)));
+    // The operands of N 16-row tiles from row0 on.
+    template <int N>
+    __device__ __forceinline__ void read(const uint16_t *lds, int row0, u32x4 (&f)[BK / 32][N]) const {
+#pragma unroll
+        for (int ks = 0; ks < BK / 32; ++ks)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                f[ks][i] = *reinterpret_cast<const u32x4 *>(
+                    lds + lds_at<BK>(row0 + i * 16 + (fl_lane() & 15), ks * 4 + (fl_lane() >> 4)));
     }
 };
 
-template <int BR, int BK>
+// k-strided: the rows of k one after the other, or in an order if GATHER.
+template <int BR, int BK, bool GATHER>
 struct WideStrided {
     static constexpr int CH = BR / 8;                // chunks a row of k
     static constexpr int RPL = FL_WAVE / CH;         // rows of k a load
     static constexpr int LOADS = BK / RPL / WD_WAVES;
     static constexpr int ELEMS = BR * BK;
-    const uint16_t *col[LOADS];
-    const int32_t *order;
-    int32_t next[LOADS][RPL];
-    int64_t ld, place;
+    const uint16_t *base;  // of the next step, if not GATHER
+    int64_t ld;
+    uint32_t at[LOADS];  // bytes from there, or from a row's first column
 
     // The permutation of a row's chunks, in steps of the two chunks that a
     // transposed read takes of each of 4 rows.
     static __device__ __forceinline__ int turn(int k) { return 2 * ((k & 3) | ((((k >> 3) ^ (k >> 4)) & 1) << 2)); }
-    __device__ __forceinline__ int row(int i) const { return (fl_wave_id() * LOADS + i) * RPL + fl_lane() / CH; }
+    static __device__ __forceinline__ int row(int i) { return (fl_wave_id() * LOADS + i) * RPL + fl_lane() / CH; }
 
-    __device__ __forceinline__ void init(const uint16_t *base, int64_t stride, int64_t R, const int32_t *ord,
-                                         int first) {
+    __device__ __forceinline__ void init(const uint16_t *b, int64_t stride, int64_t R) {
+        base = b;
         ld = stride;
-        order = ord;
-        place = 0;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int64_t c = ((fl_lane() % CH) ^ turn(row(i))) * 8;
-            col[i] = base + (c <= R - 8 ? c : R - 8);
+            at[i] = (uint32_t)((c <= R - 8 ? c : R - 8) * 2);
+            if constexpr (!GATHER) at[i] += (uint32_t)(row(i) * stride * 2);
         }
-        look(first);
     }
-    // The rows of the step that begins at `place`, of `count` rows.  (Scalar
-    // loads: vector ones would be waited for together with the operands'.)
-    __device__ __forceinline__ void look(int count) {
-        if (!order) return;
-        const auto *o = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)order;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-            for (int j = 0; j < RPL; ++j) {
-                const int r = (fl_wave_id() * LOADS + i) * RPL + j;
-                next[i][j] = r < count ? o[place + r] : 0;
-            }
-    }
-    __device__ __forceinline__ void issue(uint16_t *lds, int count, int after) {
+    // The next `count` rows of k, BK if WHOLE; r: this lane's, if GATHER.
+    template <bool WHOLE>
+    __device__ __forceinline__ void issue(uint16_t *lds, int count, const int (&r)[LOADS]) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            int64_t r = place + row(i);
-            if (order) {
-                int32_t n = next[i][0];
-#pragma unroll
-                for (int j = 1; j < RPL; ++j) n = fl_lane() / CH == j ? next[i][j] : n;
-                r = n;
-            }
-            const void *q = row(i) < count ? (const void *)(col[i] + r * ld) : (const void *)wd_zeros;
+            const char *q = (const char *)base + at[i];
+            if constexpr (GATHER) q += (int64_t)r[i] * ld * 2;
+            if (!WHOLE && row(i) >= count) q = (const char *)wd_zeros;
             load_lds(q, lds + (fl_wave_id() * LOADS + i) * 512);
         }
-        place += count;
-        look(after);
+        if constexpr (!GATHER) base += count * ld;
     }
-    __device__ __forceinline__ u32x4 frag(const uint16_t *lds, int col0, int ks) const {
-        const int s = fl_lane() & 15, q = fl_lane() >> 4;
-        u32x4 out;
+    // The operands of N 16-column tiles from col0 on.  In asm, with the wait:
+    // the builtin's reads are made to wait for every load to LDS under way, so
+    // the half of the waves that has just issued some began each step by
+    // waiting for them.
+    template <int N>
+    __device__ __forceinline__ void read(const uint16_t *lds, int col0, u32x4 (&f)[BK / 32][N]) const {
+        static_assert(BK == 64 && N % 4 == 0, "four tiles of two k steps a block");
+        const int s = fl_lane() & 15, k = (fl_lane() >> 4) * 8 + (s >> 2);  // turn() is that of k's multiples of 4 and 32 on
+        const uint32_t base =
+            (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t *)lds + k * (BR * 2) + (s & 1) * 8;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int k = ks * 32 + q * 8 + h * 4 + (s >> 2);
-            const int c = (col0 >> 3) + ((s & 3) >> 1);
-            const uint16_t *a = lds + k * BR + ((c ^ turn(k)) << 3) + (s & 1) * 4;
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4 *)const_cast<uint16_t *>(a));
-            const uint64_t u = __builtin_bit_cast(uint64_t, v);
-            out[2 * h] = (uint32_t)u;
-            out[2 * h + 1] = (uint32_t)(u >> 32);
+        for (int i = 0; i < N; i += 4) {
+            uint32_t at[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                at[t] = base + ((((col0 >> 3) + (i + t) * 2 + ((s & 3) >> 1)) ^ turn(k)) << 4);
+            uint64_t v[4][4];  // [tile][4 rows, the next 4, those of k + 32]
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %16\n"
+                "ds_read_b64_tr_b16 %1, %16 offset:%20\n"
+                "ds_read_b64_tr_b16 %2, %16 offset:%21\n"
+                "ds_read_b64_tr_b16 %3, %16 offset:%22\n"
+                "ds_read_b64_tr_b16 %4, %17\n"
+                "ds_read_b64_tr_b16 %5, %17 offset:%20\n"
+                "ds_read_b64_tr_b16 %6, %17 offset:%21\n"
+                "ds_read_b64_tr_b16 %7, %17 offset:%22\n"
+                "ds_read_b64_tr_b16 %8, %18\n"
+                "ds_read_b64_tr_b16 %9, %18 offset:%20\n"
+                "ds_read_b64_tr_b16 %10, %18 offset:%21\n"
+                "ds_read_b64_tr_b16 %11, %18 offset:%22\n"
+                "ds_read_b64_tr_b16 %12, %19\n"
+                "ds_read_b64_tr_b16 %13, %19 offset:%20\n"
+                "ds_read_b64_tr_b16 %14, %19 offset:%21\n"
+                "ds_read_b64_tr_b16 %15, %19 offset:%22\n"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[0][2]), "=&v"(v[0][3]), "=&v"(v[1][0]), "=&v"(v[1][1]),
+                  "=&v"(v[1][2]), "=&v"(v[1][3]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[2][2]), "=&v"(v[2][3]),
+                  "=&v"(v[3][0]), "=&v"(v[3][1]), "=&v"(v[3][2]), "=&v"(v[3][3])
+                : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(4 * BR * 2), "n"(32 * BR * 2), "n"(36 * BR * 2)
+                : "memory");
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+                    f[ks][i + t] = u32x4{(uint32_t)v[t][2 * ks], (uint32_t)(v[t][2 * ks] >> 32),
+                                         (uint32_t)v[t][2 * ks + 1], (uint32_t)(v[t][2 * ks + 1] >> 32)};
         }
-        return out;
+    }
+};
+
+// The rows of k that a lane loads for strided operands, in the order `order`.
+template <typename Tile>
+struct WideRows {
+    static constexpr int LOADS = Tile::LOADS, RPL = Tile::RPL, OWN = LOADS * RPL;
+    const int32_t *order;  // of the next step
+    int32_t next;          // lane j: the index of the wave's j-th row of that step
+
+    __device__ __forceinline__ void init(const int32_t *ord, int first) {
+        order = ord;
+        look(first);
+    }
+    // One load of a wave, which arrives with the operands issued before it.
+    // (Scalar loads of the eight rows were waited for with the LDS reads of
+    // the same phase.)
+    __device__ __forceinline__ void look(int count) {
+        const int r = fl_wave_id() * OWN + fl_lane() % OWN;
+        next = r < count ? order[r] : 0;
+    }
+    // The step of `count` rows, which `after` more follow.
+    __device__ __forceinline__ void step(int count, int after, int (&r)[LOADS]) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) r[i] = __shfl(next, i * RPL + fl_lane() / Tile::CH);
+        order += count;
+        look(after);
     }
 };
 
@@ -838,7 +901,8 @@ struct WideProduct {
     static __device__ __forceinline__ int wave_m() { return (fl_wave_id() >> 2) * (BM / 2); }
     static __device__ __forceinline__ int wave_n() { return (fl_wave_id() & 3) * 64; }
 
-    // feed(lds_a, lds_b, i) issues the loads of step i.
+    // feed(lds_a, lds_b, i, whole) issues the loads of step i, a whole one of
+    // BK values or the first.
     template <typename F>
     __device__ __forceinline__ void run(const TA &ta, const TB &tb, int64_t steps, uint16_t *lds, F &&feed) {
 #pragma unroll
@@ -849,10 +913,11 @@ struct WideProduct {
         const bool second = fl_wave_id() >= WD_WAVES / 2;
         const auto load = [&](int64_t step) {
             uint16_t *to = lds + (int)(step % STAGES) * ELEMS;
-            feed(to, to + TA::ELEMS, step);
+            feed(to, to + TA::ELEMS, step, std::true_type());
         };
+        feed(lds, lds + TA::ELEMS, (int64_t)0, std::false_type());
 #pragma unroll
-        for (int s = 0; s < STAGES; ++s)
+        for (int s = 1; s < STAGES; ++s)
             if (s < steps) load(s);
         if (steps < STAGES) wait<0>();
         else wait<LOADS *(STAGES - 1)>();
@@ -866,13 +931,8 @@ struct WideProduct {
             const uint16_t *la = lds + (int)(s % STAGES) * ELEMS, *lb = la + TA::ELEMS;
             const bool full = s + STAGES - 1 < steps;  // as many steps under way as there can be
             u32x4 fa[BK / 32][MT], fb[BK / 32][NTL];
-#pragma unroll
-            for (int ks = 0; ks < BK / 32; ++ks) {
-#pragma unroll
-                for (int j = 0; j < NTL; ++j) fb[ks][j] = tb.frag(lb, wave_n() + j * 16, ks);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) fa[ks][i] = ta.frag(la, wave_m() + i * 16, ks);
-            }
+            tb.read(lb, wave_n(), fb);
+            ta.read(la, wave_m(), fa);
             if (!second && s > 0 && full) load(s + STAGES - 1);
             if (second) {
                 if (full) wait<LOADS *(STAGES - 2)>();
@@ -915,7 +975,9 @@ struct WideProduct {
 // straight from the accumulators a store has 32 bytes a row, and the epilogue
 // took 15 us of a 256 x 256 tile.  f(row, col, v): eight columns of one row of
 // the wave's tile.
-constexpr int WD_SLICE = 64 * 68;  // floats: 64 rows, 4 floats apart in the banks
+constexpr int WD_SLICE = 64 * 64;  // floats; a row's 16-byte chunks turned by the row
+
+__device__ __forceinline__ int slice_at(int row, int chunk) { return row * 64 + ((chunk ^ row) & 15) * 4; }
 
 template <int MT, typename F>
 __device__ __forceinline__ void wide_rows_out(const f32x4 (&acc)[MT][4], float *slice, F &&f) {
@@ -926,14 +988,14 @@ __device__ __forceinline__ void wide_rows_out(const f32x4 (&acc)[MT][4], float *
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<f32x4 *>(slice + (i * 16 + (lane & 15)) * 68 + j * 16 + (lane >> 4) * 4) =
+                *reinterpret_cast<f32x4 *>(slice + slice_at(i * 16 + (lane & 15), j * 4 + (lane >> 4))) =
                     acc[h * 4 + i][j];
         fl_wave_sync();
-#pragma unroll
+#pragma unroll 1
         for (int r = 0; r < 8; ++r) {
             const int row = r * 8 + (lane >> 3), col = (lane & 7) * 8;
-            const f32x4 lo = *reinterpret_cast<const f32x4 *>(slice + row * 68 + col);
-            const f32x4 hi = *reinterpret_cast<const f32x4 *>(slice + row * 68 + col + 4);
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(slice + slice_at(row, col / 4));
+            const f32x4 hi = *reinterpret_cast<const f32x4 *>(slice + slice_at(row, col / 4 + 1));
             float v[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -985,9 +1047,7 @@ __device__ __forceinline__ void wide_store_rows(const RowsArgs &a, const f32x4 (
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += bias[e];
         if (a.pre) store_eight<float>(a.pre + row * a.N + n, have, v);
-        if (!t.none)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = act_value(v[e], a.act);
+        if (!t.none) act_values(v, a.act);
         if (a.residual)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += res[e];
@@ -1012,7 +1072,7 @@ __device__ __forceinline__ void wide_store_outer(const OuterArgs &a, const f32x4
 template <typename T, bool B_CONTIG, int BM, int BK, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
     using TA = WideContig<BM, BK>;
-    using TB = std::conditional_t<B_CONTIG, WideContig<WD_BN, BK>, WideStrided<WD_BN, BK>>;
+    using TB = std::conditional_t<B_CONTIG, WideContig<WD_BN, BK>, WideStrided<WD_BN, BK, false>>;
     using Prod = WideProduct<T, BM, BK, STAGES, TA, TB>;
     extern __shared__ __align__(16) uint16_t wide_lds[];
     const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
@@ -1030,13 +1090,13 @@ __global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
         return A + (a.order ? (int64_t)a.order[p] : p) * a.lda;
     });
     if constexpr (B_CONTIG) tb.init([&](int r) { return B + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldb; });
-    else tb.init(B + n0, a.ldb, a.N - n0, nullptr, first);
+    else tb.init(B + n0, a.ldb, a.N - n0);
     Prod prod;
-    prod.run(ta, tb, steps, wide_lds, [&](uint16_t *la, uint16_t *lb, int64_t s) {
-        const int count = s ? BK : first;
-        ta.issue(la, count);
-        if constexpr (B_CONTIG) tb.issue(lb, count);
-        else tb.issue(lb, count, BK);
+    prod.run(ta, tb, steps, wide_lds, [&](uint16_t *la, uint16_t *lb, int64_t, auto whole) {
+        const int count = decltype(whole)::value ? BK : first;
+        ta.template issue<decltype(whole)::value>(la, count);
+        if constexpr (B_CONTIG) tb.template issue<decltype(whole)::value>(lb, count);
+        else tb.template issue<decltype(whole)::value>(lb, count, {});
     });
     __syncthreads();  // the operands in the LDS are read
     wide_store_rows<T>(a, prod.acc, t, t.pos0 + prod.wave_m(), n0 + prod.wave_n(),
@@ -1044,11 +1104,10 @@ __global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
 }
 
 // dW.
-template <typename T, int BM, int BK, int STAGES>
+template <typename T, bool GATHER, int BK, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
-    using TA = WideStrided<BM, BK>;
-    using TB = WideStrided<WD_BN, BK>;
-    using Prod = WideProduct<T, BM, BK, STAGES, TA, TB>;
+    using Tile = WideStrided<WD_BN, BK, GATHER>;
+    using Prod = WideProduct<T, WD_BN, BK, STAGES, Tile, Tile>;
     extern __shared__ __align__(16) uint16_t wide_lds[];
     uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
     const int64_t nt = w % a.n_tiles;
@@ -1059,25 +1118,26 @@ __global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
     const int64_t g = w / a.parts;
     int64_t begin, end;
     part_range(a.offsets, a.M, g, (int)a.parts, part, &begin, &end);
-    const int64_t m0 = nt * BM, c0 = kt * WD_BN, len = end - begin;
+    const int64_t m0 = nt * WD_BN, c0 = kt * WD_BN, len = end - begin;
     const uint16_t *D = (const uint16_t *)a.d + m0, *X = (const uint16_t *)a.x + c0;
-    const int32_t *ord = a.order ? a.order + begin : nullptr;
-    if (!ord) {
+    if constexpr (!GATHER) {
         D += begin * a.ldd;
         X += begin * a.ldx;
     }
     const int64_t steps = (len + BK - 1) / BK;
     const int first = (int)(len - (steps - 1) * BK);
-    TA ta;
-    TB tb;
-    const int look = len > 0 ? first : 0;
-    ta.init(D, a.ldd, a.N - m0, ord, look);
-    tb.init(X, a.ldx, a.K - c0, ord, look);
+    Tile ta, tb;
+    ta.init(D, a.ldd, a.N - m0);
+    tb.init(X, a.ldx, a.K - c0);
+    WideRows<Tile> rows;
+    if constexpr (GATHER) rows.init(a.order + begin, len > 0 ? first : 0);
     Prod prod;
-    prod.run(ta, tb, steps, wide_lds, [&](uint16_t *la, uint16_t *lb, int64_t s) {
-        const int count = s ? BK : first, after = s + 1 < steps ? BK : 0;
-        ta.issue(la, count, after);
-        tb.issue(lb, count, after);
+    prod.run(ta, tb, steps, wide_lds, [&](uint16_t *la, uint16_t *lb, int64_t s, auto whole) {
+        const int count = decltype(whole)::value ? BK : first;
+        int r[Tile::LOADS] = {};
+        if constexpr (GATHER) rows.step(count, s + 1 < steps ? BK : 0, r);
+        ta.template issue<decltype(whole)::value>(la, count, r);
+        tb.template issue<decltype(whole)::value>(lb, count, r);
     });
     __syncthreads();  // the operands in the LDS are read
     wide_store_outer<T>(a, prod.acc, g, part, m0 + prod.wave_m(), c0 + prod.wave_n(),
@@ -1172,7 +1232,8 @@ constexpr unsigned wide_bytes(int bm, int bk, int stages) {
     return (unsigned)(operands > slices ? operands : slices);
 }
 
-bool aligned(const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+// For the wide kernels: rows on 16 bytes, and offsets of a step's rows of k in 32 bits.
+bool aligned(const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld < (1 << 24); }
 
 // Rows of the wide kernels' tiles, 0: the operands or the sizes are not for them.
 int wide_rows(const fl_linear *op, const RowsArgs &a, bool b_contig) {
@@ -1241,7 +1302,7 @@ int outer_parts(int64_t M, int64_t groups, int64_t tiles, int64_t workgroups) {
 }
 
 int sum_parts(int64_t M, int64_t N, int64_t groups) {
-    int64_t want = ceil_div(1024, ceil_div(N, LN_NT) * groups), most = M / (32 * groups);
+    int64_t want = ceil_div(4096, ceil_div(N, LN_NT) * groups), most = M / (32 * groups);
     int64_t p = want < most ? want : most;
     return (int)(p < 1 ? 1 : p > 256 ? 256 : p);
 }
@@ -1263,7 +1324,7 @@ OuterPlan outer_plan(const fl_linear *op) {
         p.tiles = ceil_div(op->N, tn) * ceil_div(op->K, tk);
     };
     // d is contiguous [M, N], on a 256-byte boundary of the workspace or the caller's gradient
-    if (op->dtype != FL_F32 && op->N % 8 == 0 && aligned(op->x, op->ldx) && op->K % 8 == 0 && op->N >= 192 &&
+    if (op->dtype != FL_F32 && aligned(nullptr, op->N) && aligned(op->x, op->ldx) && op->K % 8 == 0 && op->N >= 192 &&
         op->K >= 192) {
         fill(256, 256);
         p.parts = outer_parts(op->M, op->groups, p.tiles, 256);
@@ -1369,8 +1430,10 @@ int weight_grad(hipStream_t st, const fl_linear *op, const void *d, void *dw, fl
     constexpr int BIG_K = sizeof(T) == 4 ? 32 : 64;
     const dim3 g((unsigned)grid), nt(LN_NT);
     if constexpr (sizeof(T) == 2) {
-        if (p.wide)
-            FL_LAUNCH("k_wide_outer", (k_wide_outer<T, 256, 64, 2>), g, dim3(WD_NT), wide_bytes(256, 64, 2), st, a);
+        if (p.wide && a.order)
+            FL_LAUNCH("k_wide_outer", (k_wide_outer<T, true, 64, 2>), g, dim3(WD_NT), wide_bytes(256, 64, 2), st, a);
+        else if (p.wide)
+            FL_LAUNCH("k_wide_outer", (k_wide_outer<T, false, 64, 2>), g, dim3(WD_NT), wide_bytes(256, 64, 2), st, a);
     }
     if (p.wide) {
     } else if (p.tn == 128) FL_LAUNCH("k_lin_outer", (k_lin_outer<T, 128, 128, BIG_K>), g, nt, 0, st, a);
