@@ -21,7 +21,8 @@ so its order within one query is not fixed; every consumer uniques the keys).
 Ranks.  calculate_hits_full_sparse and calculate_hits_full_with_filter_indices
 compute the filtered tie-aware ranks on the GPU (sparse2d_filtered_ranks_cuda,
 dense_filtered_ranks_cuda) and accumulate Hits@k and the reciprocal-rank sum
-as the reference does (src/main.py:391-512).  Everything here runs on the GPU;
+as the reference does (src/main.py:391-512); calculate_hits_constrained ranks
+among the entities that a relation's answers may be.  Everything here runs on the GPU;
 CPU inputs are moved to the lookup's GPU and results returned on the input's
 device, as the reference returns them.
 """
@@ -30,7 +31,7 @@ import collections
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, attention
 from ._lib import check, ptr
 from .flashlog_kernel import flashlog_kernel as fk
 
@@ -324,3 +325,18 @@ def calculate_hits_full_with_filter_indices(state, batches, filter_indices, hits
     (src/main.py:468-512) on the GPU rank kernel."""
     ranks = fk.dense_filtered_ranks_cuda(state, _targets(batches, state.device), filter_indices, use_eql=use_eql)
     return _hits_and_mrr(ranks, hits, False)
+
+
+def calculate_hits_constrained(state, batches, filter_indices, hits, allowed=None, bias=None, use_eql=False):
+    """calculate_hits_full_with_filter_indices over the entities that a query
+    may have as its answer: ``allowed`` is a bool mask of the entities [E], or
+    one row for every relation id of the batches [relations, E] (or
+    attention.pack_allowed of it), ``bias`` an entity prior of either shape
+    that the scores take.  An entity that is not allowed ranks behind all that
+    are, the target too."""
+    relation = None
+    if any(t is not None and t.dim() == 2 for t in (allowed, bias)):
+        relation = torch.tensor([int(it["r"]) for it in batches], dtype=torch.long, device=state.device)
+    with torch.no_grad():
+        scores = attention.constrain_logits(state, allowed=allowed, group=relation, bias=bias)
+    return calculate_hits_full_with_filter_indices(scores, batches, filter_indices, hits, use_eql=use_eql)
