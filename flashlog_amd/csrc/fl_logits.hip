@@ -78,10 +78,20 @@ __device__ __forceinline__ Group<U, G> load_group(const U *row, int c, int cols)
     }
     return r;
 }
-template <typename U, int G>
+// PAST: past the caches.
+template <bool PAST = false, typename U, int G>
 __device__ __forceinline__ void store_group(U *row, int c, int cols, const Group<U, G> &r) {
-    if (c + G <= cols) __builtin_memcpy(reinterpret_cast<char *>(row) + (uint32_t)c * (uint32_t)sizeof(U), &r, sizeof(r));
-    else
+    typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+    constexpr int N = (int)sizeof(r) / 16;
+    static_assert(sizeof(r) == 16 * N, "whole 16-byte words");
+    if (c + G <= cols) {
+        Words *to = reinterpret_cast<Words *>(reinterpret_cast<char *>(row) + (uint32_t)c * (uint32_t)sizeof(U)), q[N];
+        __builtin_memcpy(q, &r, sizeof(r));
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if constexpr (PAST) __builtin_nontemporal_store(q[i], to + i);
+            else to[i] = q[i];
+    } else
 #pragma unroll
         for (int e = 0; e < G; ++e)
             if (c + e < cols) row[c + e] = r.v[e];
@@ -283,24 +293,25 @@ struct Segment : Columns<group_cols<T>(), VPT> {
             Group<float, G> q;
 #pragma unroll
             for (int e = 0; e < G; ++e) q.v[e] = v[i][e] * inv;
-            store_group<float, G>(y, base + C::local(i), cols, q);
+            store_group(y, base + C::local(i), cols, q);
         }
     }
+    template <bool PAST>
     __device__ __forceinline__ void store_values(T *y, int base, int cols, float fill) const {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             Group<T, G> q;
 #pragma unroll
             for (int e = 0; e < G; ++e) q.v[e] = (T)(allowed(i, e) ? v[i][e] : fill);
-            store_group<T, G>(y, base + C::local(i), cols, q);
+            store_group<PAST>(y, base + C::local(i), cols, q);
         }
     }
 };
 
-enum { LG_CONSTRAIN = 0, LG_SOFTMAX = 1, LG_STATS = 2, LG_JOINED = 3 };
+enum { LG_CONSTRAIN, LG_PAST, LG_SOFTMAX, LG_STATS, LG_JOINED };
 
 // Forward of a wave's segment.  LG_SOFTMAX: it is the row.  LG_STATS: its
-// maximum and sum; LG_JOINED: the softmax with the row's joined ones.
+// maximum and sum; LG_PAST: stores past the caches; LG_JOINED: the softmax with the row's joined ones.
 template <typename T, int VPT, int MODE, bool HIST>
 __global__ __launch_bounds__(LG_NT) void k_logits(LogitArgs a, void *out, float2 *stats) {
     using Seg = Segment<T, VPT, HIST>;
@@ -311,8 +322,8 @@ __global__ __launch_bounds__(LG_NT) void k_logits(LogitArgs a, void *out, float2
     if (row >= a.op.rows) return;
     Seg s;
     s.load(a, row, base, words[HIST ? fl_wave_id() : 0]);
-    if constexpr (MODE == LG_CONSTRAIN) {
-        s.store_values((T *)out + row * cols, base, (int)cols, a.op.fill);
+    if constexpr (MODE == LG_CONSTRAIN || MODE == LG_PAST) {
+        s.template store_values<MODE == LG_PAST>((T *)out + row * cols, base, (int)cols, a.op.fill);
     } else if constexpr (MODE == LG_JOINED) {
         const float2 *st = stats + row * a.segments;
         float m = -__builtin_inff(), sum = 0.0f;
@@ -389,7 +400,7 @@ struct GradSegment {
         if (HIST) head = head_id(r);
     }
     // Writes the row's dx and adds its terms to acc.
-    template <bool WHOLE>
+    template <bool WHOLE, bool PAST>
     __device__ __forceinline__ void apply(const GradArgs &a, int base, uint32_t *lds, float (&acc)[VPT][G]) {
         const fl_logits &op = a.l.op;
         const int cols = (int)op.cols;
@@ -430,12 +441,12 @@ struct GradSegment {
                 acc[i][e] += u[e];
                 o.v[e] = (T)u[e];
             }
-            if (a.dx) store_group<T, G>((T *)a.dx + row * op.cols, c, cols, o);
+            if (a.dx) store_group<PAST>((T *)a.dx + row * op.cols, c, cols, o);
             if (a.terms) {
                 Group<float, G> f;
 #pragma unroll
                 for (int e = 0; e < G; ++e) f.v[e] = u[e];
-                store_group<float, G>(a.terms + row * op.cols, c, cols, f);
+                store_group(a.terms + row * op.cols, c, cols, f);
             }
         }
     }
@@ -453,12 +464,13 @@ __global__ __launch_bounds__(LG_NT) void k_logits_grad(GradArgs a) {
     float acc[VPT][Grad::G] = {};
     Grad g;
     g.load(a, row, base);
-    g.template apply<WHOLE>(a, base, words[HIST ? fl_wave_id() : 0], acc);
+    g.template apply<WHOLE, false>(a, base, words[HIST ? fl_wave_id() : 0], acc);
 }
 
 // Gradients of rows of several segments with dbias: a wave takes one segment
 // of all the rows of a list.  (Loading the next row's values ahead took 256
-// registers and was slower than the twice as many waves without.)
+// registers and was slower than the twice as many waves without.)  Its
+// outputs go past the caches ([509 x 123000] bf16 with 74 table rows 122 -> 107 us).
 template <typename T, int VPT, bool SOFTMAX, bool HIST>
 __global__ __launch_bounds__(LG_NT) void k_logits_table_grad(GradArgs a) {
     using Grad = GradSegment<T, VPT, SOFTMAX, HIST>;
@@ -477,7 +489,7 @@ __global__ __launch_bounds__(LG_NT) void k_logits_table_grad(GradArgs a) {
     for (int64_t q = rows.q0; q < rows.q1; ++q) {
         Grad g;
         g.load(a, rows.row(a, q), base);
-        g.template apply<false>(a, base, words[HIST ? fl_wave_id() : 0], acc);
+        g.template apply<false, true>(a, base, words[HIST ? fl_wave_id() : 0], acc);
     }
     if (list >= a.l.op.bias_rows) return;  // the rows of no group
     float *b = a.dbias + ((int64_t)part * a.l.op.bias_rows + list) * cols;
@@ -486,7 +498,7 @@ __global__ __launch_bounds__(LG_NT) void k_logits_table_grad(GradArgs a) {
         Group<float, G> o;
 #pragma unroll
         for (int e = 0; e < G; ++e) o.v[e] = acc[i][e];
-        store_group<float, G>(b, base + Grad::C::local(i), (int)cols, o);
+        store_group<true>(b, base + Grad::C::local(i), (int)cols, o);
     }
 }
 
@@ -524,7 +536,7 @@ __global__ __launch_bounds__(LG_NT) void k_logits_sums(GradArgs a) {
         for (int e = 0; e < 4; ++e) s[e] += c + e < cols ? row[c + e] : 0.0f;
     }
     float *b = a.dbias + ((int64_t)part * a.l.op.bias_rows + list) * cols;
-    store_group<float, 4>(b, c, (int)cols, Group<float, 4>{{s[0], s[1], s[2], s[3]}});
+    store_group(b, c, (int)cols, Group<float, 4>{{s[0], s[1], s[2], s[3]}});
 }
 
 // sum w g of one segment of a row.
@@ -612,7 +624,10 @@ int lone_waves(int64_t items) { return items < 1024 ? 1 : LG_WAVES; }
 
 template <typename T, int VPT, int MODE>
 void launch(hipStream_t st, const fl_logits *op, void *out, float2 *stats) {
-    const LogitArgs a = lg_args(op);
+    LogitArgs a = lg_args(op);
+    // without a softmax a row is cut anywhere: segments of half the columns take
+    // fewer registers ([509 x 123000] bf16 79 -> 73 us)
+    if (MODE == LG_CONSTRAIN || MODE == LG_PAST) a.segments = (uint32_t)lg_ceil(op->cols, FL_WAVE * group_cols<T>() * VPT);
     const int64_t items = op->rows * a.segments;
     const int waves = lone_waves(items);
     const dim3 grid((unsigned)lg_ceil(items, waves)), nt(waves * FL_WAVE);
@@ -638,7 +653,13 @@ int forward(hipStream_t st, const fl_logits *op, void *out, float2 *stats, const
         launch<T, V, LG_JOINED>(st, op, out, stats);
     } else {
         by_columns<T>(op->cols, [&](auto v) {
-            launch<T, decltype(v)::value, SOFTMAX ? LG_SOFTMAX : LG_CONSTRAIN>(st, op, out, stats);
+            constexpr int V = decltype(v)::value, HALF = LG_SEG / 2 / FL_WAVE / group_cols<T>();
+            if constexpr (SOFTMAX) launch<T, V, LG_SOFTMAX>(st, op, out, stats);
+            // an output that the L2s (32 MB) do not keep for its reader goes past
+            // them ([32 x 4600000] fp32 254 -> 246 us)
+            else if (op->cols > LG_SEG && op->rows * op->cols * (int64_t)sizeof(T) > (32 << 20))
+                launch<T, HALF, LG_PAST>(st, op, out, stats);
+            else launch<T, V < HALF ? V : HALF, LG_CONSTRAIN>(st, op, out, stats);
         });
     }
     return fl_check_launch(what);
