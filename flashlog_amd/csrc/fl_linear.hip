@@ -1019,13 +1019,21 @@ __device__ __forceinline__ void load_eight(const U *p, int have, float (&out)[8]
 #pragma unroll
         for (int e = 0; e < 8; ++e) out[e] = e < have ? (float)p[e] : 0.0f;
 }
-template <typename U>
+template <bool PAST, typename U>
 __device__ __forceinline__ void store_eight(U *p, int have, const float (&v)[8]) {
     Vec<U, 8> o;
 #pragma unroll
     for (int e = 0; e < 8; ++e) o.v[e] = (U)v[e];
-    if (have >= 8) store_vec<U, 8>(p, o);
-    else store_some<U, 8>(p, o, have);
+    if (have >= 8) {
+        typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+        Words q[sizeof(o) / 16];
+        __builtin_memcpy(q, &o, sizeof(o));
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(o) / 16; ++i) {
+            if constexpr (PAST) __builtin_nontemporal_store(q[i], reinterpret_cast<Words *>(p) + i);
+            else reinterpret_cast<Words *>(p)[i] = q[i];
+        }
+    } else store_some<U, 8>(p, o, have);
 }
 
 template <typename T, int MT>
@@ -1046,12 +1054,12 @@ __device__ __forceinline__ void wide_store_rows(const RowsArgs &a, const f32x4 (
         if (a.residual) load_eight<T>((const T *)a.residual + row * a.ldres + n, have, res);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += bias[e];
-        if (a.pre) store_eight<float>(a.pre + row * a.N + n, have, v);
+        if (a.pre) store_eight<true, float>(a.pre + row * a.N + n, have, v);
         if (!t.none) act_values(v, a.act);
         if (a.residual)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += res[e];
-        store_eight<T>((T *)a.c + row * a.ldc + n, have, v);
+        store_eight<false, T>((T *)a.c + row * a.ldc + n, have, v);
     });
 }
 
@@ -1063,8 +1071,8 @@ __device__ __forceinline__ void wide_store_outer(const OuterArgs &a, const f32x4
     wide_rows_out<MT>(acc, slice, [&](int r, int, float (&v)[8]) {
         const int64_t m = row + r;
         if (m >= a.N || have <= 0) return;
-        if (a.part) store_eight<float>(a.part + ((int64_t)part * a.groups + g) * NK + m * a.K + c, have, v);
-        else store_eight<T>((T *)a.dw + g * NK + m * a.K + c, have, v);
+        if (a.part) store_eight<false, float>(a.part + ((int64_t)part * a.groups + g) * NK + m * a.K + c, have, v);
+        else store_eight<false, T>((T *)a.dw + g * NK + m * a.K + c, have, v);
     });
 }
 
