@@ -1072,7 +1072,7 @@ __device__ __forceinline__ void wide_store_outer(const OuterArgs &a, const f32x4
         const int64_t m = row + r;
         if (m >= a.N || have <= 0) return;
         if (a.part) store_eight<false, float>(a.part + ((int64_t)part * a.groups + g) * NK + m * a.K + c, have, v);
-        else store_eight<false, T>((T *)a.dw + g * NK + m * a.K + c, have, v);
+        else store_eight<true, T>((T *)a.dw + g * NK + m * a.K + c, have, v);
     });
 }
 
@@ -1111,13 +1111,25 @@ __global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
                        reinterpret_cast<float *>(wide_lds) + fl_wave_id() * WD_SLICE);
 }
 
+// The tile of a workgroup of dW of several groups: an XCD takes whole groups
+// (or parts of them) in turn, there and back, so that the large ones spread
+// over all.  (16384 rows in 24 groups, the size falling with the root of the
+// group's number: 105 us, 144 where an XCD takes groups that lie together;
+// sizes in no order: 119 and 115.)
+__device__ __forceinline__ uint32_t outer_item(const OuterArgs &a) {
+    const uint32_t unit = a.n_tiles * a.k_tiles, whole = gridDim.x / unit / FL_XCDS * FL_XCDS * unit;
+    if (blockIdx.x >= whole) return blockIdx.x;
+    const uint32_t x = blockIdx.x % FL_XCDS, p = blockIdx.x / FL_XCDS, j = p / unit;
+    return (j * FL_XCDS + (j & 1 ? FL_XCDS - 1 - x : x)) * unit + p % unit;
+}
+
 // dW.
 template <typename T, bool GATHER, int BK, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
     using Tile = WideStrided<WD_BN, BK, GATHER>;
     using Prod = WideProduct<T, WD_BN, BK, STAGES, Tile, Tile>;
     extern __shared__ __align__(16) uint16_t wide_lds[];
-    uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    uint32_t w = GATHER ? outer_item(a) : (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
     const int64_t nt = w % a.n_tiles;
     w /= a.n_tiles;
     const int64_t kt = w % a.k_tiles;
