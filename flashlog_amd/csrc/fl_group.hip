@@ -155,7 +155,7 @@ __device__ __forceinline__ void write_tiles(const GroupArgs &a, int *lds) {
 
 // One launch: every workgroup takes GR_NT rows, and counts the groups of all
 // rows itself, those before its own apart, so that none waits for another
-// (16384 rows in 16 workgroups; in one the ranks alone took 20 us).
+// (16384 rows in 24 groups 13 us; in one workgroup 20 to 25).
 __global__ __launch_bounds__(GR_NT) void k_group_one(GroupArgs a) {
     extern __shared__ uint8_t mine[];  // [waves][digits] of the workgroup's own rows
     __shared__ int lds[GR_WAVES + 1];
