@@ -338,5 +338,5 @@ def calculate_hits_constrained(state, batches, filter_indices, hits, allowed=Non
     if any(t is not None and t.dim() == 2 for t in (allowed, bias)):
         relation = torch.tensor([int(it["r"]) for it in batches], dtype=torch.long, device=state.device)
     with torch.no_grad():
-        scores = attention.constrain_logits(state, allowed=allowed, group=relation, bias=bias)
+        scores = attention.constrain_logits(state.float(), allowed=allowed, group=relation, bias=bias)
     return calculate_hits_full_with_filter_indices(scores, batches, filter_indices, hits, use_eql=use_eql)

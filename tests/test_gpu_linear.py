@@ -406,3 +406,14 @@ def test_another_stream_and_graph():
         torch.cuda.synchronize()
         for p, q in zip(step(x, w, b, gy, index), out):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("t", TYPES[1:])
+@pytest.mark.parametrize("groups,rows,sort", [(11, 8200, False), (24, 12300, True)])
+def test_relation_linear_groups_over_xcds(groups, rows, sort, t):
+    """More groups than XCDs, not a multiple of them: skewed, with empty ones, in parts of the rows."""
+    g = torch.Generator().manual_seed(2)
+    index = (torch.rand(rows, generator=g) ** 2 * (groups + 1)).long() - 1
+    index[index == 3] = 4
+    index = index.sort().values if sort else index
+    _check(*_make(rows, 264, 520, t, 18, groups=groups), act="silu", index=index)

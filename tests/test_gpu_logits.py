@@ -461,3 +461,10 @@ def test_gradient_of_the_bias_alone(n, t):
             (both if keep else alone).append(torch.autograd.grad(y, [b], gy.to(y.dtype))[0])
     for p, q in zip(both, alone):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("t,rows", [(torch.float32, 35), (torch.bfloat16, 70), (torch.float16, 70)])
+def test_outputs_larger_than_the_caches(t, rows):
+    """Rows of an odd length whose output is stored past the caches, off the 16-byte boundaries."""
+    c = _case((rows,), 250001, t, 21, groups=3, bias="table", past="ragged")
+    _check(c, dict(presence=0.3, frequency=0.2, temperature=0.8), False)
