@@ -417,3 +417,23 @@ def test_relation_linear_groups_over_xcds(groups, rows, sort, t):
     index[index == 3] = 4
     index = index.sort().values if sort else index
     _check(*_make(rows, 264, 520, t, 18, groups=groups), act="silu", index=index)
+
+
+def test_more_elements_than_32_bits_count():
+    """Rows behind the 2^31st element of x, dx and the gradient: the last rows and the first, zeros between them."""
+    fa = _fa()
+    M, K, N = 1_100_000, 2048, 256
+    x0, w, _, _, g0 = _make(128, K, N, torch.bfloat16, 19, bias=False, residual=False)
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    gy = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    ends = torch.cat([torch.arange(64), torch.arange(M - 64, M)]).cuda()
+    x[ends], gy[ends] = x0.cuda(), g0.cuda()
+    x.requires_grad_(True)
+    wg = w.cuda().requires_grad_(True)
+    y = fa.linear(x, wg)
+    dx, dw = torch.autograd.grad(y, [x, wg], gy)
+    ref = _reference(x0, w, None, None, g0, None, None)
+    _close("y", y[ends], *ref["y"])
+    _close("dx", dx[ends], *ref["dx"])
+    _close("dw", dw, *ref["dw"])
+    assert not y[64:M - 64].any() and not dx[64:M - 64].any()

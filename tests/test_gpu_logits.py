@@ -468,3 +468,19 @@ def test_outputs_larger_than_the_caches(t, rows):
     """Rows of an odd length whose output is stored past the caches, off the 16-byte boundaries."""
     c = _case((rows,), 250001, t, 21, groups=3, bias="table", past="ragged")
     _check(c, dict(presence=0.3, frequency=0.2, temperature=0.8), False)
+
+
+def test_more_elements_than_32_bits_count():
+    """Rows behind the 2^31st element; sums of ones are exact."""
+    fa = _fa()
+    rows, n = 480, 4_600_001
+    x = torch.empty(rows, n, device="cuda").normal_().requires_grad_(True)
+    ok = torch.rand(n, device="cuda") < 0.5
+    bias = torch.randn(n, device="cuda").requires_grad_(True)
+    out = fa.constrain_logits(x, allowed=ok, bias=bias)
+    for i in (0, 300, rows - 1):
+        assert torch.equal(out[i], torch.where(ok, x[i] + bias, -math.inf))
+    dx, db = torch.autograd.grad(out, [x, bias], torch.ones_like(out))
+    for i in (0, 300, rows - 1):
+        assert torch.equal(dx[i], ok.float())
+    assert torch.equal(db, ok.float() * rows)
