@@ -396,41 +396,55 @@ __device__ __forceinline__ float act_value(float p, int act) {
     }
 }
 
-template <int N>
-__device__ __forceinline__ void act_values(float (&v)[N], int act) {
-    const auto each = [&](auto known) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = act_value(v[e], decltype(known)::value);
-    };
+// f with the activation as a constant.
+template <typename F>
+__device__ __forceinline__ void by_act(int act, F &&f) {
     switch (act) {
-        case FL_ACT_RELU: return each(std::integral_constant<int, FL_ACT_RELU>());
-        case FL_ACT_GELU: return each(std::integral_constant<int, FL_ACT_GELU>());
-        case FL_ACT_SILU: return each(std::integral_constant<int, FL_ACT_SILU>());
-        case FL_ACT_TANH: return each(std::integral_constant<int, FL_ACT_TANH>());
-        case FL_ACT_SIGMOID: return each(std::integral_constant<int, FL_ACT_SIGMOID>());
+        case FL_ACT_RELU: return f(std::integral_constant<int, FL_ACT_RELU>());
+        case FL_ACT_GELU: return f(std::integral_constant<int, FL_ACT_GELU>());
+        case FL_ACT_SILU: return f(std::integral_constant<int, FL_ACT_SILU>());
+        case FL_ACT_TANH: return f(std::integral_constant<int, FL_ACT_TANH>());
+        case FL_ACT_SIGMOID: return f(std::integral_constant<int, FL_ACT_SIGMOID>());
         default: return;
     }
 }
 
+template <int N>
+__device__ __forceinline__ void act_values(float (&v)[N], int act) {
+    by_act(act, [&](auto known) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = act_value(v[e], decltype(known)::value);
+    });
+}
+
+// act'(p), from the same pieces (gelu's of [16384 x 2048] bf16 44 us, 48 with
+// the library's erff and expf).
 __device__ __forceinline__ float act_slope(float p, int act) {
     switch (act) {
         case FL_ACT_RELU: return p > 0.0f ? 1.0f : (p != p ? p : 0.0f);
-        case FL_ACT_GELU:
-            return 0.5f * (1.0f + erff(p * 0.70710678118654752f)) + p * (0.39894228040143268f * expf(-0.5f * p * p));
+        case FL_ACT_GELU: return normal_cdf(p) + p * (0.39894228040143268f * fast_exp(-0.5f * p * p));
         case FL_ACT_SILU: {
-            const float q = 1.0f / (1.0f + expf(-p));
+            const float q = __builtin_amdgcn_rcpf(1.0f + fast_exp(-p));
             return q * (1.0f + p * (1.0f - q));
         }
         case FL_ACT_TANH: {
-            const float t = tanhf(p);
+            const float t = act_value(p, FL_ACT_TANH);
             return 1.0f - t * t;
         }
         case FL_ACT_SIGMOID: {
-            const float q = 1.0f / (1.0f + expf(-p));
+            const float q = act_value(p, FL_ACT_SIGMOID);
             return q * (1.0f - q);
         }
         default: return 1.0f;
     }
+}
+
+template <int N>
+__device__ __forceinline__ void act_slopes(float (&v)[N], int act) {
+    by_act(act, [&](auto known) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = act_slope(v[e], decltype(known)::value);
+    });
 }
 
 struct RowsArgs {
@@ -1173,7 +1187,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
 }
 
 // d = gy * act'(p), rounded to the operands' type: it is an operand of two
-// products.  HBM-bound: [16384 x 2048] fp16 45 us = 6.0 TB/s.
+// products.  HBM-bound: [16384 x 2048] bf16 44 us = 6.1 TB/s.
 template <typename T>
 __global__ __launch_bounds__(LN_NT) void k_act_grad(const T *__restrict__ gy, const float *__restrict__ pre, int64_t n,
                                                     int act, T *__restrict__ d) {
@@ -1188,6 +1202,59 @@ __global__ __launch_bounds__(LN_NT) void k_act_grad(const T *__restrict__ gy, co
         store_vec<T, 4>(d + i, o);
     } else
         for (int64_t e = i; e < n; ++e) d[e] = (T)((float)gy[e] * act_slope(pre[e], act));
+}
+
+// The same and the column sums of a part of the rows in one pass: a workgroup
+// takes 512 columns, eight a lane, each wave a quarter of its rows.  [16384 x
+// 2048] fp16: 57 us = 4.7 TB/s, 63 in two passes; of rows gathered for 24 groups
+// 84, 75 in two, so those take two.
+constexpr int AS_COLS = 8 * FL_WAVE;
+constexpr int AS_GROUPS = 2048;  // workgroups, where the rows give as many
+
+template <typename T>
+__global__ __launch_bounds__(LN_NT) void k_act_sums(const T *__restrict__ gy, const float *__restrict__ pre, int64_t M,
+                                                    int64_t N, int parts, int act, T *__restrict__ d,
+                                                    float *__restrict__ out) {
+    constexpr int AHEAD = 4;
+    constexpr int WAVES = LN_NT / FL_WAVE;
+    __shared__ float sums[WAVES][AS_COLS];
+    const uint32_t blocks = (uint32_t)((N + AS_COLS - 1) / AS_COLS), item = blockIdx.x;
+    const int64_t c0 = (int64_t)(item % blocks) * AS_COLS, c = c0 + fl_lane() * 8, part = item / blocks;
+    const int have = N - c < 8 ? (int)(N - c) : 8;
+    const int64_t run = part * WAVES + fl_wave_id(), begin = M * run / (parts * WAVES),
+                  end = M * (run + 1) / (parts * WAVES);
+    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int64_t p = begin; p < end && have > 0; p += AHEAD) {
+        float v[AHEAD][8], q[AHEAD][8];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int64_t row = p + j < end ? p + j : end - 1;
+            load_eight<T>(gy + row * N + c, have, v[j]);
+            load_eight<float>(pre + row * N + c, have, q[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (p + j >= end) break;
+            act_slopes(q[j], act);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[j][e] *= q[j][e];
+                s[e] += (float)(T)v[j][e];
+            }
+            store_eight<false, T>(d + (p + j) * N + c, have, v[j]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[fl_wave_id()][fl_lane() * 8 + e] = s[e];
+    __syncthreads();
+#pragma unroll
+    for (int i = threadIdx.x; i < AS_COLS; i += LN_NT)
+        if (c0 + i < N) {
+            float t = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) t += sums[w][i];
+            out[part * N + c0 + i] = t;
+        }
 }
 
 // Column sums of a group's rows (a part of them), one thread a column: [16384 x
@@ -1331,7 +1398,18 @@ int outer_parts(int64_t M, int64_t groups, int64_t tiles, int64_t workgroups) {
     return (int)(p < 1 ? 1 : p > 64 ? 64 : p);
 }
 
-int sum_parts(int64_t M, int64_t N, int64_t groups) {
+// Whether d and db are made in one pass: with few columns most lanes of its
+// waves would have none, and gathered rows are faster in two.
+bool act_and_sums(const fl_linear *op) { return op->act != FL_ACT_NONE && op->N >= 256 && !op->offsets; }
+
+// Parts of a group's rows in db's sums.
+int sum_parts(const fl_linear *op) {
+    const int64_t M = op->M, N = op->N, groups = op->groups;
+    if (act_and_sums(op)) {
+        const int64_t want = ceil_div(AS_GROUPS, ceil_div(N, AS_COLS)), most = M / 8;
+        const int64_t p = want < most ? want : most;
+        return (int)(p < 1 ? 1 : p > 512 ? 512 : p);
+    }
     int64_t want = ceil_div(4096, ceil_div(N, LN_NT) * groups), most = M / (32 * groups);
     int64_t p = want < most ? want : most;
     return (int)(p < 1 ? 1 : p > 256 ? 256 : p);
@@ -1474,7 +1552,7 @@ int weight_grad(hipStream_t st, const fl_linear *op, const void *d, void *dw, fl
 
 template <typename T>
 int bias_grad(hipStream_t st, const fl_linear *op, const void *d, void *db, int db_f32, float *ws) {
-    const int parts = sum_parts(op->M, op->N, op->groups);
+    const int parts = sum_parts(op);
     const int64_t grid = (int64_t)parts * op->groups * ceil_div(op->N, LN_NT);
     if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "linear_bias_grad: too many groups for one launch (shape)");
     FL_LAUNCH("k_col_sums", k_col_sums<T>, dim3((unsigned)grid), dim3(LN_NT), 0, st,
@@ -1482,6 +1560,18 @@ int bias_grad(hipStream_t st, const fl_linear *op, const void *d, void *db, int 
     if (db_f32) fold_parts<float>(st, ws, parts, op->groups * op->N, (float *)db);
     else fold_parts<T>(st, ws, parts, op->groups * op->N, (T *)db);
     return fl_check_launch("linear_bias_grad");
+}
+
+template <typename T>
+int act_and_bias_grad(hipStream_t st, const fl_linear *op, const void *gy, const float *pre, void *d, void *db,
+                      int db_f32, float *ws) {
+    const int parts = sum_parts(op);
+    const int64_t grid = parts * ceil_div(op->N, AS_COLS);
+    FL_LAUNCH("k_act_sums", k_act_sums<T>, dim3((unsigned)grid), dim3(LN_NT), 0, st, (const T *)gy, pre, op->M, op->N,
+              parts, op->act, (T *)d, ws);
+    if (db_f32) fold_parts<float>(st, ws, parts, op->N, (float *)db);
+    else fold_parts<T>(st, ws, parts, op->N, (T *)db);
+    return fl_check_launch("linear_backward");
 }
 
 template <typename T>
@@ -1514,7 +1604,7 @@ BackwardSpace backward_space(const fl_linear *op, int with_dx, int with_dw, int 
         const int parts = outer_plan(op).parts;
         if (parts > 1) need((size_t)parts * op->groups * op->N * op->K * 4);
     }
-    if (with_db && op->N) need((size_t)sum_parts(op->M, op->N, op->groups) * op->groups * op->N * 4);
+    if (with_db && op->N) need((size_t)sum_parts(op) * op->groups * op->N * 4);
     s.parts = take(most);
     return s;
 }
@@ -1526,13 +1616,15 @@ int backward(hipStream_t st, const fl_linear *op, const void *gy, const float *p
     float *parts = (float *)(ws + s.parts);
     const void *d = gy;
     int rc = FL_OK;
+    const bool both = db && act_and_sums(op) && op->M;
     if (op->act != FL_ACT_NONE && op->M && op->N) {
-        rc = act_grad<T>(st, op->act, gy, pre, op->M * op->N, ws + s.d);
         d = ws + s.d;
+        if (both) rc = act_and_bias_grad<T>(st, op, gy, pre, ws + s.d, db, db_f32, parts);
+        else rc = act_grad<T>(st, op->act, gy, pre, op->M * op->N, ws + s.d);
     }
     if (!rc && dx && op->M && op->K) rc = input_grad<T>(st, op, d, dx, parts);
     if (!rc && dw && op->N && op->K) rc = weight_grad<T>(st, op, d, dw, parts);
-    if (!rc && db && op->N) rc = bias_grad<T>(st, op, d, db, db_f32, parts);
+    if (!rc && db && op->N && !both) rc = bias_grad<T>(st, op, d, db, db_f32, parts);
     return rc;
 }
 
