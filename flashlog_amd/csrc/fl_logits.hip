@@ -231,7 +231,15 @@ struct Segment : Columns<group_cols<T>(), VPT> {
     float v[VPT][G];
     unsigned ok[VPT];
 
-    __device__ __forceinline__ void load(const LogitArgs &a, int64_t row, int base, uint32_t *lds) {
+    using Bias = Group<float, G>[VPT];
+
+    static __device__ __forceinline__ void load_bias(const float *bias, int base, int cols, Bias &b) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) b[i] = load_group<float, G>(bias, base + C::local(i), cols);
+    }
+    // kept: the bias, if KEPT.
+    template <bool KEPT>
+    __device__ __forceinline__ void load(const LogitArgs &a, int64_t row, int base, uint32_t *lds, const Bias &kept) {
         const int cols = (int)a.op.cols;
         const RowView r = row_view(a.op, row);
         const T *x = (const T *)a.op.x + row * a.op.ldx;
@@ -246,8 +254,8 @@ struct Segment : Columns<group_cols<T>(), VPT> {
             ok[i] = C::bits(r, c, cols);
 #pragma unroll
             for (int e = 0; e < G; ++e) v[i][e] = (float)q[i].v[e];
-            if (r.bias) {
-                const Group<float, G> b = load_group<float, G>(r.bias, c, cols);
+            if (KEPT || r.bias) {
+                const Group<float, G> b = KEPT ? kept[i] : load_group<float, G>(r.bias, c, cols);
 #pragma unroll
                 for (int e = 0; e < G; ++e) v[i][e] += b.v[e];
             }
@@ -308,10 +316,11 @@ struct Segment : Columns<group_cols<T>(), VPT> {
     }
 };
 
-enum { LG_CONSTRAIN, LG_PAST, LG_SOFTMAX, LG_STATS, LG_JOINED };
+enum { LG_CONSTRAIN, LG_PAST, LG_SHARED, LG_SOFTMAX, LG_STATS, LG_JOINED };
+constexpr int LG_SHARE = 4;  // rows of a wave, LG_SHARED
 
-// Forward of a wave's segment.  LG_PAST: stores past the caches.  LG_SOFTMAX: it
-// is the row.  LG_STATS: its maximum and sum; LG_JOINED: the softmax with the
+// Forward of a wave's segment.  LG_PAST: stores past the caches; LG_SHARED: so, of
+// LG_SHARE rows with one bias, which is loaded once.  LG_SOFTMAX: it is the row.  LG_STATS: its maximum and sum; LG_JOINED: the softmax with the
 // row's joined ones.  [32 x 4600000] fp32 with 60 ids a row 247 us = 4.9 TB/s,
 // [509 x 123000] bf16 72 us = 3.5 TB/s of the rows (and as many bytes of the bias
 // rows from the caches), the softmax of [4608 x 1645] 21 us = 2.9 TB/s: with 7
@@ -322,11 +331,22 @@ __global__ __launch_bounds__(LG_NT) void k_logits(LogitArgs a, void *out, float2
     using Seg = Segment<T, VPT, HIST>;
     __shared__ uint32_t words[HIST ? LG_WAVES : 1][HIST ? Seg::SEG / 2 : 1];
     const uint32_t item = blockIdx.x * (blockDim.x / FL_WAVE) + fl_wave_id();
-    const int64_t row = item / a.segments, cols = a.op.cols;
+    const int64_t row = item / a.segments * (MODE == LG_SHARED ? LG_SHARE : 1), cols = a.op.cols;
     const int base = (int)(item % a.segments) * Seg::SEG;
     if (row >= a.op.rows) return;
     Seg s;
-    s.load(a, row, base, words[HIST ? fl_wave_id() : 0]);
+    typename Seg::Bias bias;
+    uint32_t *lds = words[HIST ? fl_wave_id() : 0];
+    if constexpr (MODE == LG_SHARED) {
+        Seg::load_bias(a.op.bias, base, (int)cols, bias);
+        const int64_t end = row + LG_SHARE < a.op.rows ? row + LG_SHARE : a.op.rows;
+        for (int64_t r = row; r < end; ++r) {
+            s.template load<true>(a, r, base, lds, bias);
+            s.template store_values<true>((T *)out + r * cols, base, (int)cols, a.op.fill);
+        }
+        return;
+    }
+    s.template load<false>(a, row, base, lds, bias);
     if constexpr (MODE == LG_CONSTRAIN || MODE == LG_PAST) {
         s.template store_values<MODE == LG_PAST>((T *)out + row * cols, base, (int)cols, a.op.fill);
     } else if constexpr (MODE == LG_JOINED) {
@@ -634,8 +654,8 @@ void launch(hipStream_t st, const fl_logits *op, void *out, float2 *stats) {
     LogitArgs a = lg_args(op);
     // without a softmax a row is cut anywhere: segments of half the columns take
     // fewer registers ([509 x 123000] bf16 79 -> 73 us)
-    if (MODE == LG_CONSTRAIN || MODE == LG_PAST) a.segments = (uint32_t)lg_ceil(op->cols, FL_WAVE * group_cols<T>() * VPT);
-    const int64_t items = op->rows * a.segments;
+    if (MODE <= LG_SHARED) a.segments = (uint32_t)lg_ceil(op->cols, FL_WAVE * group_cols<T>() * VPT);
+    const int64_t items = (MODE == LG_SHARED ? lg_ceil(op->rows, LG_SHARE) : op->rows) * a.segments;
     const int waves = lone_waves(items);
     const dim3 grid((unsigned)lg_ceil(items, waves)), nt(waves * FL_WAVE);
     if (op->history) FL_LAUNCH("k_logits", (k_logits<T, VPT, MODE, true>), grid, nt, 0, st, a, out, stats);
@@ -664,8 +684,10 @@ int forward(hipStream_t st, const fl_logits *op, void *out, float2 *stats, const
             if constexpr (SOFTMAX) launch<T, V, LG_SOFTMAX>(st, op, out, stats);
             // an output that the L2s (32 MB) do not keep for its reader goes past
             // them ([32 x 4600000] fp32 254 -> 246 us)
-            else if (op->cols > LG_SEG && op->rows * op->cols * (int64_t)sizeof(T) > (32 << 20))
-                launch<T, HALF, LG_PAST>(st, op, out, stats);
+            else if (op->cols > LG_SEG && op->rows * op->cols * (int64_t)sizeof(T) > (32 << 20)) {
+                if (op->bias && op->bias_rows == 1) launch<T, HALF, LG_SHARED>(st, op, out, stats);
+                else launch<T, HALF, LG_PAST>(st, op, out, stats);
+            }
             else launch<T, V < HALF ? V : HALF, LG_CONSTRAIN>(st, op, out, stats);
         });
     }
