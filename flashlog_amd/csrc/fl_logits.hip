@@ -321,7 +321,7 @@ constexpr int LG_SHARE = 4;  // rows of a wave, LG_SHARED
 
 // Forward of a wave's segment.  LG_PAST: stores past the caches; LG_SHARED: so, of
 // LG_SHARE rows with one bias, which is loaded once.  LG_SOFTMAX: it is the row.  LG_STATS: its maximum and sum; LG_JOINED: the softmax with the
-// row's joined ones.  [32 x 4600000] fp32 with 60 ids a row 247 us = 4.9 TB/s,
+// row's joined ones.  [32 x 4600000] fp32 with 60 ids a row 224 us = 5.3 TB/s,
 // [509 x 123000] bf16 72 us = 3.5 TB/s of the rows (and as many bytes of the bias
 // rows from the caches), the softmax of [4608 x 1645] 21 us = 2.9 TB/s: with 7
 // or 8 waves a SIMD bound by how many loads are under way (bias loads ahead of
@@ -683,7 +683,10 @@ int forward(hipStream_t st, const fl_logits *op, void *out, float2 *stats, const
             constexpr int V = decltype(v)::value, HALF = LG_SEG / 2 / FL_WAVE / group_cols<T>();
             if constexpr (SOFTMAX) launch<T, V, LG_SOFTMAX>(st, op, out, stats);
             // an output that the L2s (32 MB) do not keep for its reader goes past
-            // them ([32 x 4600000] fp32 254 -> 246 us)
+            // them ([32 x 4600000] fp32 254 -> 246 us); one bias for all rows is
+            // loaded once for four (246 -> 224; two or eight: 228; rows taken in
+            // the order of a table's groups left the rows' streams: 71 -> 92 us
+            // for [509 x 123000] bf16)
             else if (op->cols > LG_SEG && op->rows * op->cols * (int64_t)sizeof(T) > (32 << 20)) {
                 if (op->bias && op->bias_rows == 1) launch<T, HALF, LG_SHARED>(st, op, out, stats);
                 else launch<T, HALF, LG_PAST>(st, op, out, stats);

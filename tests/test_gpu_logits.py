@@ -484,3 +484,11 @@ def test_more_elements_than_32_bits_count():
     for i in (0, 300, rows - 1):
         assert torch.equal(dx[i], ok.float())
     assert torch.equal(db, ok.float() * rows)
+
+
+@pytest.mark.parametrize("rows,inner,groups", [(70, 1, 3), (72, 8, 40), (69, 3, 20)])
+def test_long_rows_by_their_bias(rows, inner, groups):
+    """Large outputs with a table of biases: few, with steps of one owner, with owners of none, and too many to share."""
+    c = _case((rows // inner, inner), 250001, torch.bfloat16, 22, groups=groups, bias="table", past=3)
+    c["group"][::7] = groups
+    _check(c, dict(presence=0.3, frequency=0.2, temperature=0.8), False)
