@@ -9,8 +9,8 @@
 // (16 bits each: a wave takes at most GR_WAVE_ROWS rows).  The counts are then
 // scanned over the waves of a workgroup and over the workgroups, so that a
 // row's place is the same on every run.  Up to GR_BLOCK_ROWS rows and 4095
-// groups are one launch (latency-bound: 15000 rows in 74 groups are 120 KB);
-// more rows take three launches a digit.
+// groups are one launch, whose workgroups count all rows each (latency-bound:
+// 15000 rows in 74 groups are 120 KB); more rows take three launches a digit.
 //
 // Ids outside [0, groups) come last, behind offsets[groups]: rows of no group.
 #include "fl_abi.h"

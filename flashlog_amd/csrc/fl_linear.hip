@@ -1332,15 +1332,20 @@ constexpr unsigned wide_bytes(int bm, int bk, int stages) {
 // For the wide kernels: rows on 16 bytes, and offsets of a step's rows of k in 32 bits.
 bool aligned(const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld < (1 << 24); }
 
-// Rows of the wide kernels' tiles, 0: the operands or the sizes are not for them.
+// Rows of the wide kernels' tiles, 0: the operands or the sizes are not for
+// them.  bf16 [M x 2048 -> 2048], us with other tiles, 128 rows and 256 rows:
+// M = 1024 24, 32, 47; 2048 43, 34, 49; 4096 65, 41, 51; 6144 96, 74, 55; 8192
+// 115, 77, 62.  So 128 rows from half the CUs on, and 256 where the tiles of 128
+// would be more than the CUs.  Groups: 256 rows (16384 rows in 24 groups, bf16
+// [1024 -> 2048]: 137 us, 165 with 128 rows).
 int wide_rows(const fl_linear *op, const RowsArgs &a, bool b_contig) {
     if (op->dtype == FL_F32 || !aligned(a.a, a.lda) || !aligned(a.b, a.ldb) || a.b_group % 8 || a.K % 8 || a.K < 64 ||
         (!b_contig && a.N % 8) || a.N < 192)
         return 0;
     const int64_t cols = ceil_div(a.N, WD_BN);
     if (op->offsets) return fl_group_block(op->M, op->groups) == 256 && ceil_div(op->M, 256) * cols >= 64 ? 256 : 0;
-    if (ceil_div(op->M, 256) * cols >= 192) return 256;
-    return ceil_div(op->M, 128) * cols >= 128 ? 128 : 0;
+    const int64_t tiles = ceil_div(op->M, 128) * cols;
+    return tiles < 128 ? 0 : tiles <= 256 ? 128 : 256;
 }
 
 // The cut of y's or dx's product that the wide kernels do not take.

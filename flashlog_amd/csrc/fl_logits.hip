@@ -319,9 +319,10 @@ struct Segment : Columns<group_cols<T>(), VPT> {
 enum { LG_CONSTRAIN, LG_PAST, LG_SHARED, LG_SOFTMAX, LG_STATS, LG_JOINED };
 constexpr int LG_SHARE = 4;  // rows of a wave, LG_SHARED
 
-// Forward of a wave's segment.  LG_PAST: stores past the caches; LG_SHARED: so, of
-// LG_SHARE rows with one bias, which is loaded once.  LG_SOFTMAX: it is the row.  LG_STATS: its maximum and sum; LG_JOINED: the softmax with the
-// row's joined ones.  [32 x 4600000] fp32 with 60 ids a row 224 us = 5.3 TB/s,
+// Forward of a wave's segment.  LG_PAST: stores past the caches; LG_SHARED: so,
+// of LG_SHARE rows with one bias, which is loaded once.  LG_SOFTMAX: it is the
+// row.  LG_STATS: its maximum and sum; LG_JOINED: the softmax with the row's
+// joined ones.  [32 x 4600000] fp32 with 60 ids a row 224 us = 5.3 TB/s,
 // [509 x 123000] bf16 72 us = 3.5 TB/s of the rows (and as many bytes of the bias
 // rows from the caches), the softmax of [4608 x 1645] 21 us = 2.9 TB/s: with 7
 // or 8 waves a SIMD bound by how many loads are under way (bias loads ahead of
