@@ -1337,7 +1337,8 @@ bool aligned(const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 
 // M = 1024 24, 32, 47; 2048 43, 34, 49; 4096 65, 41, 51; 6144 96, 74, 55; 8192
 // 115, 77, 62.  So 128 rows from half the CUs on, and 256 where the tiles of 128
 // would be more than the CUs.  Groups: 256 rows (16384 rows in 24 groups, bf16
-// [1024 -> 2048]: 137 us, 165 with 128 rows).
+// [1024 -> 2048]: 137 us, 165 with 128 rows) from 64 tiles on (8192 rows in 4
+// groups, [1024 -> 512], 64 tiles: 34 us, 38 with others; [1024 -> 256] 33, 30).
 int wide_rows(const fl_linear *op, const RowsArgs &a, bool b_contig) {
     if (op->dtype == FL_F32 || !aligned(a.a, a.lda) || !aligned(a.b, a.ldb) || a.b_group % 8 || a.K % 8 || a.K < 64 ||
         (!b_contig && a.N % 8) || a.N < 192)
@@ -1421,7 +1422,9 @@ int sum_parts(const fl_linear *op) {
 }
 
 // Tiles of dW: N and K extents, and the parts of the rows.  Wide ones where
-// the operands allow it and a part keeps 256 rows; 64 x 64 where 128 x 128
+// the operands allow it, a part keeps 256 rows and they are 64 or more (bf16,
+// us, other tiles and wide ones: 256 x 256 over 16384 rows 34, 30; 1024 x 1024
+// over 1024 rows 33, 31, over 4096 68, 42); 64 x 64 where 128 x 128
 // would leave CUs idle.
 struct OuterPlan {
     int tn, tk, parts;
@@ -1441,7 +1444,7 @@ OuterPlan outer_plan(const fl_linear *op) {
         op->K >= 192) {
         fill(256, 256);
         p.parts = outer_parts(op->M, op->groups, p.tiles, 256);
-        p.wide = p.tiles * op->groups * p.parts >= 128;
+        p.wide = p.tiles * op->groups * p.parts >= 64;
         if (p.wide) return p;
     }
     if (op->groups == 1) {
