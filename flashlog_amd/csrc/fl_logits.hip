@@ -621,9 +621,9 @@ int lg_check(const fl_logits *op, const char *what) {
     if (!(op->temperature > 0.0f) || !(op->repetition > 0.0f))
         return fl_fail(FL_ERR_ARG, "%s: temperature and repetition must lie in the range (0, inf)", what);
     if (op->allowed && (op->allowed_rows < 1 || op->allowed_ld < lg_ceil(op->cols, 32) ||
-                        (op->allowed_rows > 1 && !op->group)))
+                        (op->allowed_rows > 1 && op->rows > 0 && !op->group)))
         return fl_fail(FL_ERR_ARG, "%s: bad shape of the allowed table", what);
-    if (op->bias && (op->bias_rows < 1 || (op->bias_rows > 1 && !op->group)))
+    if (op->bias && (op->bias_rows < 1 || (op->bias_rows > 1 && op->rows > 0 && !op->group)))
         return fl_fail(FL_ERR_ARG, "%s: bad shape of the bias table", what);
     if (op->history && op->history_len < 0) return fl_fail(FL_ERR_ARG, "%s: bad shape of the history", what);
     if (op->rows > 0 && op->cols > 0 && !op->x) return fl_fail(FL_ERR_ARG, "%s: null pointer", what);

@@ -1,0 +1,44 @@
+"""Calls of the attention operators that their documentation allows at the
+ends of their ranges: no rows, non-finite values beside masks and in
+gradients, more work items than one dimension of a launch holds."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+HALVES = [torch.bfloat16, torch.float16]
+
+
+def _fa():
+    from flashlog_amd import attention
+    return attention
+
+
+@pytest.mark.parametrize("n", [7, 3000])
+@pytest.mark.parametrize("softmax", [False, True])
+def test_no_rows_with_tables(softmax, n):
+    """An empty batch beside tables of several rows: empty outputs, a zero gradient for the biases."""
+    fa = _fa()
+    fn = fa.hop_attention if softmax else fa.constrain_logits
+    group = torch.zeros(0, dtype=torch.long, device="cuda")
+    allowed = torch.ones(3, n, dtype=torch.bool, device="cuda")
+    for lead in ((0,), (0, 4)):
+        x = torch.zeros(*lead, n, device="cuda", requires_grad=True)
+        b = torch.randn(3, n, device="cuda", requires_grad=True)
+        y = fn(x, allowed=allowed, group=group, bias=b)
+        assert y.shape == x.shape
+        gx, gb = torch.autograd.grad(y, [x, b], torch.ones_like(y))
+        assert gx.shape == x.shape and gb.shape == b.shape and not gb.any()
+
+
+def test_ranks_of_no_queries():
+    from flashlog_amd import evaluation as ev
+    hits = np.zeros(10)
+    none = torch.zeros(0, dtype=torch.long, device="cuda")
+    mrr = ev.calculate_hits_constrained(torch.zeros(0, 50, device="cuda"), [], (none, none), hits,
+                                        allowed=torch.ones(3, 50, dtype=torch.bool, device="cuda"))
+    assert mrr == 0 and not hits.any()
