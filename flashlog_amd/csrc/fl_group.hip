@@ -323,10 +323,15 @@ int fl_group_rows(void *stream, const int64_t *index, int64_t rows, int64_t grou
     a.ntiles = fl_group_tiles(rows, groups);
     a.block = (int)fl_group_block(rows, groups);
     const int bits = fl::bits_for(groups + 1);
+    if (rows == 0) {  // every group begins at 0, and there are no tiles
+        FL_LAUNCH("k_group_offsets", fl::k_group_offsets, dim3((unsigned)((groups + fl::GR_NT) / fl::GR_NT)),
+                  dim3(fl::GR_NT), 0, st, a);
+        return fl::fl_check_launch("group_rows");
+    }
     if (fl::one_launch(rows, groups)) {
         a.bits = bits;
         a.digits = 1 << bits;
-        const int64_t nb = rows > 0 ? (rows + fl::GR_NT - 1) / fl::GR_NT : 1;
+        const int64_t nb = (rows + fl::GR_NT - 1) / fl::GR_NT;
         const size_t lds = (size_t)fl::GR_WAVES * (a.digits < 4 ? 4 : a.digits);
         FL_LAUNCH("k_group_one", fl::k_group_one, dim3((unsigned)nb), dim3(fl::GR_NT), lds, st, a);
         return fl::fl_check_launch("group_rows");

@@ -42,3 +42,24 @@ def test_ranks_of_no_queries():
     mrr = ev.calculate_hits_constrained(torch.zeros(0, 50, device="cuda"), [], (none, none), hits,
                                         allowed=torch.ones(3, 50, dtype=torch.bool, device="cuda"))
     assert mrr == 0 and not hits.any()
+
+
+@pytest.mark.parametrize("groups", [1, 4095, 4096, 65534, (1 << 24) - 1])
+def test_no_rows_in_many_groups(groups):
+    """Every group of no rows begins at 0, however many passes more rows would take."""
+    fa = _fa()
+    none = torch.zeros(0, dtype=torch.long, device="cuda")
+    plan = fa.group_rows(none, groups)
+    assert plan.order.numel() == 0 and plan.tiles.numel() == 0
+    assert plan.offsets.shape == (groups + 1,) and not plan.offsets.any()
+    off, ids = fa.history_from_pairs(none, none, groups)
+    assert off.shape == (groups + 1,) and not off.any() and ids.numel() == 0
+
+
+def test_no_rows_beside_a_large_bias_table():
+    fa = _fa()
+    x = torch.zeros(0, 6, device="cuda", requires_grad=True)
+    b = torch.randn(5000, 6, device="cuda", requires_grad=True)
+    w = fa.hop_attention(x, group=torch.zeros(0, dtype=torch.long, device="cuda"), bias=b)
+    gx, gb = torch.autograd.grad(w, [x, b], torch.ones_like(w))
+    assert gx.shape == (0, 6) and gb.shape == b.shape and not gb.any()
