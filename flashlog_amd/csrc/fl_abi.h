@@ -14,6 +14,17 @@ int fl_check_launch(const char *what);
 // prof_end records the matching stop event.
 int prof_begin(const char *kernel, hipStream_t stream);
 void prof_end(int token, hipStream_t stream);
+
+// A dimension of a launch has fewer than 2^32 threads.
+inline bool launch_fits(int64_t blocks, int64_t threads) { return blocks < (1ll << 32) / threads; }
+
+// Any number of workgroups (of up to 512 threads), in two dimensions where one
+// does not hold them: kernels take fl_block() for their index and leave out
+// what lies behind the last.
+inline dim3 grid_of(int64_t blocks) {
+    const int64_t most = 1 << 22;
+    return blocks <= most ? dim3((unsigned)blocks) : dim3((unsigned)most, (unsigned)((blocks + most - 1) / most));
+}
 }  // namespace fl
 
 // Launch `kernel` on `stream`, bracketed by timing events when profiling.

@@ -10,6 +10,9 @@
 __device__ __forceinline__ float fl_mul(float a, float b) { return __fmul_rn(a, b); }
 __device__ __forceinline__ float fl_add(float a, float b) { return __fadd_rn(a, b); }
 
+// A workgroup's index in a grid of one or two dimensions.
+__device__ __forceinline__ int64_t fl_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 __device__ __forceinline__ int fl_lane() { return threadIdx.x & (FL_WAVE - 1); }
 
 // Workgroups of a launch go to the 8 XCDs round robin (workgroup g on XCD

@@ -573,7 +573,7 @@ __device__ __forceinline__ void store_part(const RowsArgs &a, const f32x4 (&acc)
 template <typename T>
 __global__ __launch_bounds__(LN_NT) void k_lin_finish(RowsArgs a) {
     const uint32_t quads = (uint32_t)((a.N + 3) / 4);
-    const int64_t i = (int64_t)blockIdx.x * LN_NT + threadIdx.x;
+    const int64_t i = fl_block() * LN_NT + threadIdx.x;
     if (i >= a.M * quads) return;
     const int64_t row = i / quads, n = (i % quads) * 4;
     const int have = a.N - n < 4 ? (int)(a.N - n) : 4;
@@ -1376,7 +1376,8 @@ int launch_rows(hipStream_t st, const fl_linear *op, RowsArgs &a, float *ws, con
     const int64_t m_tiles = op->offsets ? fl_group_tiles(op->M, op->groups) * (a.block / bm) : ceil_div(op->M, bm);
     a.n_tiles = (uint32_t)ceil_div(a.N, bn);
     const int64_t grid = m_tiles * a.n_tiles * a.parts;
-    if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "%s: too many tiles for one launch (shape)", what);
+    if (!launch_fits(grid, wide ? WD_NT : LN_NT))
+        return fl_fail(FL_ERR_ARG, "%s: too many tiles for one launch (shape)", what);
     if (grid == 0) return FL_OK;
     const dim3 g((unsigned)grid), nt(LN_NT);
     if constexpr (sizeof(T) == 2) {
@@ -1391,8 +1392,7 @@ int launch_rows(hipStream_t st, const fl_linear *op, RowsArgs &a, float *ws, con
     else if (bm == 64) FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 64, 64, BIG_K>), g, nt, 0, st, a);
     else FL_LAUNCH("k_lin_rows", (k_lin_rows<T, B_CONTIG, 32, 64, 64>), g, nt, 0, st, a);
     if (a.part)
-        FL_LAUNCH("k_lin_finish", k_lin_finish<T>, dim3((unsigned)ceil_div(a.M * ceil_div(a.N, 4), LN_NT)), nt, 0, st,
-                  a);
+        FL_LAUNCH("k_lin_finish", k_lin_finish<T>, grid_of(ceil_div(a.M * ceil_div(a.N, 4), LN_NT)), nt, 0, st, a);
     return fl_check_launch(what);
 }
 
@@ -1541,7 +1541,8 @@ int weight_grad(hipStream_t st, const fl_linear *op, const void *d, void *dw, fl
     a.dw = dw;
     a.part = a.parts > 1 ? ws : nullptr;
     const int64_t grid = p.tiles * a.parts * a.groups;
-    if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "linear_backward: too many tiles for one launch (shape)");
+    if (!launch_fits(grid, p.wide ? WD_NT : LN_NT))
+        return fl_fail(FL_ERR_ARG, "linear_backward: too many tiles for one launch (shape)");
     if (grid == 0) return FL_OK;
     constexpr int BIG_K = sizeof(T) == 4 ? 32 : 64;
     const dim3 g((unsigned)grid), nt(LN_NT);
@@ -1562,7 +1563,8 @@ template <typename T>
 int bias_grad(hipStream_t st, const fl_linear *op, const void *d, void *db, int db_f32, float *ws) {
     const int parts = sum_parts(op);
     const int64_t grid = (int64_t)parts * op->groups * ceil_div(op->N, LN_NT);
-    if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "linear_bias_grad: too many groups for one launch (shape)");
+    if (!launch_fits(grid, LN_NT))
+        return fl_fail(FL_ERR_ARG, "linear_bias_grad: too many groups for one launch (shape)");
     FL_LAUNCH("k_col_sums", k_col_sums<T>, dim3((unsigned)grid), dim3(LN_NT), 0, st,
               (const T *)d, op->N, op->M, op->N, op->groups, parts, op->order, op->offsets, ws);
     if (db_f32) fold_parts<float>(st, ws, parts, op->groups * op->N, (float *)db);
@@ -1575,6 +1577,8 @@ int act_and_bias_grad(hipStream_t st, const fl_linear *op, const void *gy, const
                       int db_f32, float *ws) {
     const int parts = sum_parts(op);
     const int64_t grid = parts * ceil_div(op->N, AS_COLS);
+    if (!launch_fits(grid, LN_NT))
+        return fl_fail(FL_ERR_ARG, "linear_backward: too many columns for one launch (shape)");
     FL_LAUNCH("k_act_sums", k_act_sums<T>, dim3((unsigned)grid), dim3(LN_NT), 0, st, (const T *)gy, pre, op->M, op->N,
               parts, op->act, (T *)d, ws);
     if (db_f32) fold_parts<float>(st, ws, parts, op->N, (float *)db);
@@ -1585,7 +1589,8 @@ int act_and_bias_grad(hipStream_t st, const fl_linear *op, const void *gy, const
 template <typename T>
 int act_grad(hipStream_t st, int act, const void *gy, const float *pre, int64_t n, void *d) {
     const int64_t grid = ceil_div(n, LN_NT * 4);
-    if (grid > 0x7fffffffll) return fl_fail(FL_ERR_ARG, "linear_backward: too many values for one launch (shape)");
+    if (!launch_fits(grid, LN_NT))
+        return fl_fail(FL_ERR_ARG, "linear_backward: too many values for one launch (shape)");
     FL_LAUNCH("k_act_grad", k_act_grad<T>, dim3((unsigned)grid), dim3(LN_NT), 0, st, (const T *)gy, pre, n, act,
               (T *)d);
     return fl_check_launch("linear_backward");

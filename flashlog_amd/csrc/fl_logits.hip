@@ -331,7 +331,7 @@ template <typename T, int VPT, int MODE, bool HIST>
 __global__ __launch_bounds__(LG_NT) void k_logits(LogitArgs a, void *out, float2 *stats) {
     using Seg = Segment<T, VPT, HIST>;
     __shared__ uint32_t words[HIST ? LG_WAVES : 1][HIST ? Seg::SEG / 2 : 1];
-    const uint32_t item = blockIdx.x * (blockDim.x / FL_WAVE) + fl_wave_id();
+    const uint32_t item = (uint32_t)fl_block() * (blockDim.x / FL_WAVE) + fl_wave_id();
     const int64_t row = item / a.segments * (MODE == LG_SHARED ? LG_SHARE : 1), cols = a.op.cols;
     const int base = (int)(item % a.segments) * Seg::SEG;
     if (row >= a.op.rows) return;
@@ -484,7 +484,7 @@ template <typename T, int VPT, bool SOFTMAX, bool HIST, bool WHOLE>
 __global__ __launch_bounds__(LG_NT) void k_logits_grad(GradArgs a) {
     using Grad = GradSegment<T, VPT, SOFTMAX, HIST>;
     __shared__ uint32_t words[HIST ? LG_WAVES : 1][HIST ? Grad::C::SEG / 2 : 1];
-    const uint32_t item = blockIdx.x * (blockDim.x / FL_WAVE) + fl_wave_id();
+    const uint32_t item = (uint32_t)fl_block() * (blockDim.x / FL_WAVE) + fl_wave_id();
     const int64_t row = item / a.l.segments;
     const int base = (int)(item % a.l.segments) * Grad::C::SEG;
     if (row >= a.l.op.rows) return;
@@ -505,7 +505,7 @@ __global__ __launch_bounds__(LG_NT) void k_logits_table_grad(GradArgs a) {
     __shared__ uint32_t words[HIST ? LG_WAVES : 1][HIST ? SEG / 2 : 1];
     const int64_t cols = a.l.op.cols;
     const uint32_t segments = (uint32_t)((cols + SEG - 1) / SEG);
-    uint32_t item = blockIdx.x * LG_WAVES + fl_wave_id();
+    uint32_t item = (uint32_t)fl_block() * LG_WAVES + fl_wave_id();
     const int base = (int)(item % segments) * SEG;
     item /= segments;
     const uint32_t part = item % a.parts;
@@ -534,11 +534,12 @@ __global__ __launch_bounds__(LG_NT) void k_logits_table_grad(GradArgs a) {
 // 20 us = 2.0 TB/s).
 __global__ __launch_bounds__(LG_NT) void k_logits_sums(GradArgs a) {
     const int64_t cols = a.l.op.cols;
-    const uint32_t blocks = (uint32_t)((cols + 4 * LG_NT - 1) / (4 * LG_NT)), item = blockIdx.x / blocks;
-    const int c = (int)((blockIdx.x % blocks) * LG_NT + threadIdx.x) * 4;
+    const uint32_t blocks = (uint32_t)((cols + 4 * LG_NT - 1) / (4 * LG_NT)), block = (uint32_t)fl_block(),
+                   item = block / blocks;
+    const int c = (int)((block % blocks) * LG_NT + threadIdx.x) * 4;
     const uint32_t part = item % a.parts;
     const int64_t list = item / a.parts;
-    if (c >= cols) return;
+    if (c >= cols || list >= a.l.op.bias_rows) return;
     const RowList rows(a, list, part);
     const float *terms = a.terms ? a.terms : (const float *)a.dx;  // fp32 dx are the terms themselves
     float s[4] = {0, 0, 0, 0};
@@ -571,7 +572,7 @@ __global__ __launch_bounds__(LG_NT) void k_logits_sums(GradArgs a) {
 __global__ __launch_bounds__(LG_NT) void k_logits_dot(LogitArgs a, const float *__restrict__ g,
                                                       const float *__restrict__ w, float *__restrict__ dots) {
     using C = Columns<4, LG_SEG / FL_WAVE / 4>;
-    const uint32_t item = blockIdx.x * LG_WAVES + fl_wave_id();
+    const uint32_t item = (uint32_t)fl_block() * LG_WAVES + fl_wave_id();
     const int64_t row = item / a.segments;
     const int cols = (int)a.op.cols, base = (int)(item % a.segments) * LG_SEG;
     if (row >= a.op.rows) return;
@@ -590,9 +591,10 @@ __global__ __launch_bounds__(LG_NT) void k_logits_dot(LogitArgs a, const float *
     if (fl_lane() == 0) dots[item] = s;
 }
 
-__global__ __launch_bounds__(FL_WAVE) void k_logits_join(const float *__restrict__ part, int64_t segments,
-                                                         float *__restrict__ dots) {
-    const int64_t row = blockIdx.x;
+__global__ __launch_bounds__(FL_WAVE) void k_logits_join(const float *__restrict__ part, int64_t rows,
+                                                         int64_t segments, float *__restrict__ dots) {
+    const int64_t row = fl_block();
+    if (row >= rows) return;
     float s = 0.0f;
     for (int64_t i = threadIdx.x; i < segments; i += FL_WAVE) s += part[row * segments + i];
     s = fl_wave_sum_f32(s);
@@ -603,7 +605,7 @@ __global__ __launch_bounds__(FL_WAVE) void k_logits_join(const float *__restrict
 __global__ __launch_bounds__(256) void k_pack_bits(const uint8_t *__restrict__ mask, int64_t rows, int64_t cols,
                                                    int64_t words, uint32_t *__restrict__ out) {
     const int64_t per = (cols + FL_WAVE - 1) / FL_WAVE;  // ballots a row
-    const int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) / FL_WAVE;
+    const int64_t t = (fl_block() * 256 + threadIdx.x) / FL_WAVE;
     if (t >= rows * per) return;
     const int64_t row = t / per, c = (t % per) * FL_WAVE + fl_lane();
     const unsigned long long b = __ballot(c < cols && mask[row * cols + c] != 0);
@@ -658,7 +660,7 @@ void launch(hipStream_t st, const fl_logits *op, void *out, float2 *stats) {
     if (MODE <= LG_SHARED) a.segments = (uint32_t)lg_ceil(op->cols, FL_WAVE * group_cols<T>() * VPT);
     const int64_t items = (MODE == LG_SHARED ? lg_ceil(op->rows, LG_SHARE) : op->rows) * a.segments;
     const int waves = lone_waves(items);
-    const dim3 grid((unsigned)lg_ceil(items, waves)), nt(waves * FL_WAVE);
+    const dim3 grid = grid_of(lg_ceil(items, waves)), nt(waves * FL_WAVE);
     if (op->history) FL_LAUNCH("k_logits", (k_logits<T, VPT, MODE, true>), grid, nt, 0, st, a, out, stats);
     else FL_LAUNCH("k_logits", (k_logits<T, VPT, MODE, false>), grid, nt, 0, st, a, out, stats);
 }
@@ -719,14 +721,14 @@ void launch_grad(hipStream_t st, const GradArgs &a) {
         if (!whole && a.dbias) {  // half as many columns a wave: more waves, fewer registers
             const int64_t waves = a.lists * a.parts * lg_ceil(op.cols, LG_SEG / 2);
             FL_LAUNCH("k_logits_table_grad", (k_logits_table_grad<T, VPT / 2, SOFTMAX, HIST>),
-                      dim3((unsigned)lg_ceil(waves, LG_WAVES)), dim3(LG_NT), 0, st, a);
+                      grid_of(lg_ceil(waves, LG_WAVES)), dim3(LG_NT), 0, st, a);
             return;
         }
     }
     const int64_t items = op.rows * a.l.segments;
     if (items > 0) {
         const int waves = lone_waves(items);
-        const dim3 grid((unsigned)lg_ceil(items, waves)), nt(waves * FL_WAVE);
+        const dim3 grid = grid_of(lg_ceil(items, waves)), nt(waves * FL_WAVE);
         if constexpr (SOFTMAX && LONG) {
             if (!whole) FL_LAUNCH("k_logits_grad", (k_logits_grad<T, VPT, true, HIST, false>), grid, nt, 0, st, a);
         }
@@ -735,7 +737,7 @@ void launch_grad(hipStream_t st, const GradArgs &a) {
     }
     if (a.dbias) {
         const int64_t sums = op.bias_rows * a.parts * lg_ceil(op.cols, 4 * LG_NT);
-        FL_LAUNCH("k_logits_sums", k_logits_sums, dim3((unsigned)sums), dim3(LG_NT), 0, st, a);
+        FL_LAUNCH("k_logits_sums", k_logits_sums, grid_of(sums), dim3(LG_NT), 0, st, a);
     }
 }
 
@@ -794,9 +796,9 @@ int gradient(hipStream_t st, const fl_logits *op, const float *w, const void *gr
     } else if (op->rows == 0) return FL_OK;
     if (SOFTMAX && op->cols > LG_SEG && op->rows > 0) {
         float *part = (float *)(ws + sp.dots), *dots = part + op->rows * a.l.segments;
-        FL_LAUNCH("k_logits_dot", k_logits_dot, dim3((unsigned)lg_ceil(op->rows * a.l.segments, LG_WAVES)),
-                  dim3(LG_NT), 0, st, a.l, (const float *)grad, w, part);
-        FL_LAUNCH("k_logits_join", k_logits_join, dim3((unsigned)op->rows), dim3(FL_WAVE), 0, st, part,
+        FL_LAUNCH("k_logits_dot", k_logits_dot, grid_of(lg_ceil(op->rows * a.l.segments, LG_WAVES)), dim3(LG_NT),
+                  0, st, a.l, (const float *)grad, w, part);
+        FL_LAUNCH("k_logits_join", k_logits_join, grid_of(op->rows), dim3(FL_WAVE), 0, st, part, op->rows,
                   (int64_t)a.l.segments, dots);
         a.dots = dots;
     }
@@ -829,7 +831,7 @@ int fl_pack_bits(void *stream, const uint8_t *mask, int64_t rows, int64_t cols, 
     if (waves == 0) return FL_OK;
     if (!mask || !words) return fl::fl_fail(FL_ERR_ARG, "pack_bits: null pointer");
     if (fl::lg_ceil(waves, 4) > 0x7fffffffll) return fl::fl_fail(FL_ERR_ARG, "pack_bits: too many bits (shape)");
-    FL_LAUNCH("k_pack_bits", fl::k_pack_bits, dim3((unsigned)fl::lg_ceil(waves, 4)), dim3(256), 0,
+    FL_LAUNCH("k_pack_bits", fl::k_pack_bits, fl::grid_of(fl::lg_ceil(waves, 4)), dim3(256), 0,
               (hipStream_t)stream, mask, rows, cols, fl::lg_ceil(cols, 32), (uint32_t *)words);
     return fl::fl_check_launch("pack_bits");
 }

@@ -13,7 +13,7 @@ __global__ __launch_bounds__(256) void k_fold_parts(const float *__restrict__ pa
                                                     TO *__restrict__ out) {
     __shared__ float runs[4][64];
     const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
-    const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t i = fl_block() * 64 + lane;
     const int p1 = parts * (run + 1) / 4;
     float s = 0.0f;
     if (i < n) {
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void k_fold_parts(const float *__restrict__ pa
 template <typename TO>
 __global__ __launch_bounds__(256) void k_fold_few(const float *__restrict__ part, int parts, int64_t n,
                                                   TO *__restrict__ out) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    const int64_t i = (fl_block() * 256 + threadIdx.x) * 4;
     if (i >= n) return;
     if (i + 4 <= n) {
         float s[4] = {0, 0, 0, 0};
@@ -58,15 +58,13 @@ __global__ __launch_bounds__(256) void k_fold_few(const float *__restrict__ part
         }
 }
 
-// n up to 2^31 * 64; by the number of parts.
+// By the number of parts.
 template <typename TO>
 inline void fold_parts(hipStream_t st, const float *part, int parts, int64_t n, TO *out) {
     if (parts > 8)
-        FL_LAUNCH("k_fold_parts", k_fold_parts<TO>, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, part, parts, n,
-                  out);
+        FL_LAUNCH("k_fold_parts", k_fold_parts<TO>, grid_of((n + 63) / 64), dim3(256), 0, st, part, parts, n, out);
     else
-        FL_LAUNCH("k_fold_few", k_fold_few<TO>, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st, part, parts, n,
-                  out);
+        FL_LAUNCH("k_fold_few", k_fold_few<TO>, grid_of((n + 1023) / 1024), dim3(256), 0, st, part, parts, n, out);
 }
 
 }  // namespace fl

@@ -25,3 +25,24 @@ def test_no_rows_need_no_group(table):
     assert lib.fl_logits_grad(None, op, None, None, None, None, None, 0) == 0
     op.rows = 1
     assert lib.fl_logits_constrain(None, op, ctypes.c_void_p(1)) == 1
+
+
+def test_more_tiles_than_a_launch_holds():
+    """A launch has fewer than 2^32 threads along a dimension; the products' tiles lie along one."""
+    lib = _lib.lib()
+    one, ws = ctypes.c_void_p(1), ctypes.c_void_p(4096)
+
+    def refused(rc):
+        assert rc == 1 and "shape" in lib.fl_last_error().decode()
+
+    op = _lib.FlLinear(M=(1 << 31) - 1, N=64, K=1, groups=1, x=1, ldx=1, weight=1, ldw=1)
+    refused(lib.fl_linear_forward(None, op, one, None, None, 0))
+    # the activation's gradient of 2^34 values, the weight gradient of 2^31 x 256, the bias gradients of 2^24 groups
+    op = _lib.FlLinear(M=1 << 20, N=1 << 14, K=0, groups=1, act=2)
+    refused(lib.fl_linear_backward(None, op, one, one, None, None, None, 0, ws, 1 << 60))
+    op = _lib.FlLinear(M=1, N=(1 << 31) - 1, K=256, groups=1, x=1, ldx=256, weight=1, ldw=256)
+    refused(lib.fl_linear_backward(None, op, one, None, None, one, None, 0, ws, 1 << 60))
+    op = _lib.FlLinear(M=1, N=1, K=0, groups=1 << 24, order=1, offsets=1, tiles=1)
+    refused(lib.fl_linear_backward(None, op, one, None, None, None, one, 0, ws, 1 << 60))
+    op = _lib.FlLinear(M=5000, N=1 << 24, K=0, groups=1, act=2)
+    refused(lib.fl_linear_backward(None, op, one, one, None, None, one, 0, ws, 1 << 60))

@@ -63,3 +63,48 @@ def test_no_rows_beside_a_large_bias_table():
     w = fa.hop_attention(x, group=torch.zeros(0, dtype=torch.long, device="cuda"), bias=b)
     gx, gb = torch.autograd.grad(w, [x, b], torch.ones_like(w))
     assert gx.shape == (0, 6) and gb.shape == b.shape and not gb.any()
+
+
+def test_mask_of_more_than_2_to_the_32_entries():
+    fa = _fa()
+    rows, n = 65537, 65600
+    base = torch.rand(n, device="cuda") < 0.5
+    turn = torch.arange(rows, device="cuda") % 3 == 1
+    words = fa.pack_allowed(base[None] ^ turn[:, None])
+    assert words.shape == (rows, n // 32)
+    for rest, row in ((~turn, base), (turn, ~base)):
+        want = fa.pack_allowed(row)
+        got = words[rest]
+        assert (got == want).all()
+    bits = (fa.pack_allowed(base)[:, None] >> torch.arange(32, device="cuda")) & 1
+    assert torch.equal(bits.reshape(-1).bool(), base)
+
+
+@pytest.mark.parametrize("softmax", [False, True])
+def test_rows_of_more_than_2_to_the_32_work_items(softmax):
+    """A wave a row: rows behind the 2^26th, forward and backward, with the sums of a bias."""
+    fa = _fa()
+    rows, n = (1 << 26) + 77, 3
+    x = torch.zeros(rows, n, device="cuda")
+    g = torch.Generator().manual_seed(3)
+    at = torch.tensor([0, 5, 1 << 25, (1 << 26) - 1, 1 << 26, (1 << 26) + 1, rows - 1]).cuda()
+    x[at] = torch.randn(len(at), n, generator=g).cuda()
+    bias = torch.randn(n, generator=g).cuda()
+    gy = torch.zeros(rows, n, device="cuda")
+    gy[at] = torch.randn(len(at), n, generator=g).cuda()
+    fn = fa.hop_attention if softmax else fa.constrain_logits
+
+    def run(x, gy):
+        x, b = x.detach().requires_grad_(True), bias.detach().requires_grad_(True)
+        y = fn(x, bias=b)
+        return [y.detach(), *torch.autograd.grad(y, [x, b], gy)]
+
+    many, few = run(x, gy), run(x[at], gy[at])
+    assert torch.equal(many[0][at], few[0]) and torch.equal(many[1][at], few[1])
+    rest = fn(torch.zeros(1, n, device="cuda"), bias=bias)
+    same = (many[0] == rest).all(1)
+    same[at] = True
+    assert same.all()
+    assert int(torch.count_nonzero(many[1].any(1))) <= len(at)
+    bound = 2 * (len(at) + 8) * E * few[1].double().abs().sum(0)
+    assert ((many[2].double() - few[1].double().sum(0)).abs() <= bound).all()
