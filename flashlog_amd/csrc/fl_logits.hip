@@ -300,7 +300,7 @@ struct Segment : Columns<group_cols<T>(), VPT> {
         for (int i = 0; i < VPT; ++i) {
             Group<float, G> q;
 #pragma unroll
-            for (int e = 0; e < G; ++e) q.v[e] = v[i][e] * inv;
+            for (int e = 0; e < G; ++e) q.v[e] = allowed(i, e) ? v[i][e] * inv : 0.0f;  // inv may be NaN
             store_group(y, base + C::local(i), cols, q);
         }
     }

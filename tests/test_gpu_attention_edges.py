@@ -108,3 +108,20 @@ def test_rows_of_more_than_2_to_the_32_work_items(softmax):
     assert int(torch.count_nonzero(many[1].any(1))) <= len(at)
     bound = 2 * (len(at) + 8) * E * few[1].double().abs().sum(0)
     assert ((many[2].double() - few[1].double().sum(0)).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("n", [30, 1500, 9000])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_masked_columns_are_zero_beside_bad_values(bad, n):
+    """A NaN or an infinity among the allowed logits does not reach the masked columns."""
+    fa = _fa()
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(4, n, generator=g).cuda()
+    ok = (torch.rand(n, generator=g) < 0.5).cuda()
+    ok[n // 2] = True
+    x[1, n // 2] = bad
+    w = fa.hop_attention(x, allowed=ok)
+    assert (w[:, ~ok] == 0).all()
+    assert torch.isnan(w[1, n // 2])
+    clean = fa.hop_attention(x[[0, 2, 3]], allowed=ok)
+    assert torch.equal(w[[0, 2, 3]], clean)
