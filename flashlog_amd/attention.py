@@ -20,16 +20,17 @@ src/model_DRUM_kernel.py:90-117); it has no constraints on either.  Here:
 
 Operands are float32, bfloat16 or float16 tensors on the GPU (CPU tensors
 raise); sums, softmax statistics and gradients of tables are float32.  All
-four are differentiable (once: a second derivative raises), run on torch's
-current stream, allocate with torch, and neither synchronise nor keep
-anything between calls, so they can be captured into a graph.  A captured
-backward needs leaves whose gradient graph was not begun outside the capture,
-as everywhere in torch.
+four are differentiable (once and backward: a second derivative and
+forward-mode tangents raise), run on torch's current stream, allocate with
+torch, and neither synchronise nor keep anything between calls, so they can be
+captured into a graph.  A captured backward needs leaves whose gradient graph
+was not begun outside the capture, as everywhere in torch.
 """
 import math
 
 import torch
 from torch import autograd
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -81,6 +82,15 @@ def _need_gpu(what, *tensors):
         elif t.device != dev:
             raise RuntimeError("%s: tensors on different devices" % what)
     return dev
+
+
+def _differentiated(*operands):
+    """Whether a call has to go through its autograd function: for the
+    backward, or, inside a forward-mode level, to have it refuse tangents
+    (dual tensors need not require gradients)."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands)
 
 
 def _integers(what, name, t):
@@ -253,9 +263,7 @@ def _product(what, x, plan, weight, bias, activation, residual):
             raise ValueError("%s: weight has %d groups, the plan %d" % (what, wshape[0], plan.groups))
         if math.prod(xshape[:-1]) != plan.rows:
             raise ValueError("%s: x has %d rows, the plan %d" % (what, math.prod(xshape[:-1]), plan.rows))
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
-                                    (bias is not None and bias.requires_grad) or
-                                    (residual is not None and residual.requires_grad)):
+    if _differentiated(x, weight, bias, residual):
         return _LinearFunction.apply(x, weight, bias, residual, plan, act)
     return _linear_forward(x, weight, bias, residual, plan, act, False)[0]
 
@@ -469,7 +477,7 @@ class _LogitsFunction(autograd.Function):
 
 
 def _apply(logits, c, bias, softmax):
-    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+    if _differentiated(logits, bias):
         return _LogitsFunction.apply(logits, bias, c, softmax)
     return _logits_forward(c, logits, bias, softmax)[0]
 

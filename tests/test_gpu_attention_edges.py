@@ -125,3 +125,21 @@ def test_masked_columns_are_zero_beside_bad_values(bad, n):
     assert torch.isnan(w[1, n // 2])
     clean = fa.hop_attention(x[[0, 2, 3]], allowed=ok)
     assert torch.equal(w[[0, 2, 3]], clean)
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+    fa = _fa()
+    x, w, b, r = torch.randn(4, 5).cuda(), torch.randn(3, 5).cuda(), torch.randn(3).cuda(), torch.randn(4, 3).cuda()
+    plan = fa.group_rows(torch.zeros(4, dtype=torch.long).cuda(), 1)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: fa.linear(dual(x), w), lambda: fa.linear(x, dual(w)), lambda: fa.linear(x, w, dual(b)),
+                 lambda: fa.linear(x, w, residual=dual(r)), lambda: fa.relation_linear(dual(x), plan, w[None]),
+                 lambda: fa.constrain_logits(dual(x)), lambda: fa.constrain_logits(x, bias=dual(x[0].clone())),
+                 lambda: fa.hop_attention(dual(x)), lambda: fa.hop_attention(x, bias=dual(x[0].clone()))]
+        for call in calls:
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    call()
+        assert fa.linear(x, w).shape == (4, 3)
