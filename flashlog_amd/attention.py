@@ -279,7 +279,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     are as exact as float32 ones, except that a sum which an infinity or NaN
     enters is NaN.  For the backward the
     activation's argument is kept in float32; its gradient is rounded to the
-    operands' type, as an operand of two products."""
+    operands' type as an operand of two products, but not as a term of the
+    bias's."""
     return _product("linear", x, None, weight, bias, activation, residual)
 
 

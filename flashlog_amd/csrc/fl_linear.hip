@@ -1204,33 +1204,43 @@ __global__ __launch_bounds__(LN_NT) void k_act_grad(const T *__restrict__ gy, co
         for (int64_t e = i; e < n; ++e) d[e] = (T)((float)gy[e] * act_slope(pre[e], act));
 }
 
-// The same and the column sums of a part of the rows in one pass: a workgroup
-// takes 512 columns, eight a lane, each wave a quarter of its rows.  [16384 x
-// 2048] fp16: 57 us = 4.7 TB/s, 63 in two passes; of rows gathered for 24 groups
-// 84, 75 in two, so those take two.
+// The same and the column sums of a part of a group's rows in one pass, added
+// before d is rounded: a workgroup takes 512 columns, eight a lane, each wave a
+// quarter of its rows, in the plan's order if GATHER (rows of no group have no
+// d).  [16384 x 2048] fp16: 54 us = 5.0 TB/s, 63 in two passes; bf16 in 24
+// groups 60 us.
 constexpr int AS_COLS = 8 * FL_WAVE;
 constexpr int AS_GROUPS = 2048;  // workgroups, where the rows give as many
 
-template <typename T>
+template <typename T, bool GATHER>
 __global__ __launch_bounds__(LN_NT) void k_act_sums(const T *__restrict__ gy, const float *__restrict__ pre, int64_t M,
-                                                    int64_t N, int parts, int act, T *__restrict__ d,
+                                                    int64_t N, int64_t groups, int parts, int act,
+                                                    const int32_t *__restrict__ order,
+                                                    const int32_t *__restrict__ offsets, T *__restrict__ d,
                                                     float *__restrict__ out) {
     constexpr int AHEAD = 4;
     constexpr int WAVES = LN_NT / FL_WAVE;
     __shared__ float sums[WAVES][AS_COLS];
-    const uint32_t blocks = (uint32_t)((N + AS_COLS - 1) / AS_COLS), item = blockIdx.x;
-    const int64_t c0 = (int64_t)(item % blocks) * AS_COLS, c = c0 + fl_lane() * 8, part = item / blocks;
+    const uint32_t blocks = (uint32_t)((N + AS_COLS - 1) / AS_COLS), item = blockIdx.x / blocks;
+    const int64_t c0 = (int64_t)(blockIdx.x % blocks) * AS_COLS, c = c0 + fl_lane() * 8;
+    const int64_t g = GATHER ? item / parts : 0, part = GATHER ? item % parts : item;
     const int have = N - c < 8 ? (int)(N - c) : 8;
-    const int64_t run = part * WAVES + fl_wave_id(), begin = M * run / (parts * WAVES),
-                  end = M * (run + 1) / (parts * WAVES);
+    int64_t begin, end;
+    part_range(GATHER ? offsets : nullptr, M, g, parts * WAVES, (int)part * WAVES + fl_wave_id(), &begin, &end);
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int64_t p = begin; p < end && have > 0; p += AHEAD) {
+    for (int64_t p = begin; p < end; p += AHEAD) {
         float v[AHEAD][8], q[AHEAD][8];
+        int64_t row[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            const int64_t row = p + j < end ? p + j : end - 1;
-            load_eight<T>(gy + row * N + c, have, v[j]);
-            load_eight<float>(pre + row * N + c, have, q[j]);
+            row[j] = p + j < end ? p + j : end - 1;
+            if constexpr (GATHER) row[j] = order[row[j]];
+        }
+        if (have <= 0) continue;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            load_eight<T>(gy + row[j] * N + c, have, v[j]);
+            load_eight<float>(pre + row[j] * N + c, have, q[j]);
         }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
@@ -1239,9 +1249,9 @@ __global__ __launch_bounds__(LN_NT) void k_act_sums(const T *__restrict__ gy, co
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 v[j][e] *= q[j][e];
-                s[e] += (float)(T)v[j][e];
+                s[e] += v[j][e];
             }
-            store_eight<false, T>(d + (p + j) * N + c, have, v[j]);
+            store_eight<false, T>(d + row[j] * N + c, have, v[j]);
         }
     }
 #pragma unroll
@@ -1253,15 +1263,17 @@ __global__ __launch_bounds__(LN_NT) void k_act_sums(const T *__restrict__ gy, co
             float t = 0.0f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) t += sums[w][i];
-            out[part * N + c0 + i] = t;
+            out[(part * groups + g) * N + c0 + i] = t;
         }
 }
 
 // Column sums of a group's rows (a part of them), one thread a column: [16384 x
-// 2048] fp16 18 us = 3.7 TB/s, of rows gathered for 24 groups 27 us.
-template <typename T>
-__global__ __launch_bounds__(LN_NT) void k_col_sums(const T *__restrict__ d, int64_t ldd, int64_t M, int64_t N,
-                                                    int64_t groups, int parts, const int32_t *__restrict__ order,
+// 2048] fp16 18 us = 3.7 TB/s.  With an activation (ACT) d's terms are made
+// again from the gradient gy and the argument, unrounded.
+template <typename T, bool ACT>
+__global__ __launch_bounds__(LN_NT) void k_col_sums(const T *__restrict__ d, const float *__restrict__ pre, int act,
+                                                    int64_t M, int64_t N, int64_t groups, int parts,
+                                                    const int32_t *__restrict__ order,
                                                     const int32_t *__restrict__ offsets, float *__restrict__ out) {
     const int64_t blocks = (N + LN_NT - 1) / LN_NT, w = blockIdx.x / blocks;
     const int64_t c = (blockIdx.x % blocks) * LN_NT + threadIdx.x;
@@ -1273,13 +1285,22 @@ __global__ __launch_bounds__(LN_NT) void k_col_sums(const T *__restrict__ d, int
     float s = 0.0f;
     int64_t p = begin;
     for (; p + 8 <= end; p += 8) {
-        float v[8];
+        float v[8], q[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = (float)d[(order ? (int64_t)order[p + j] : p + j) * ldd + c];
+        for (int j = 0; j < 8; ++j) {
+            const int64_t at = (order ? (int64_t)order[p + j] : p + j) * N + c;
+            v[j] = (float)d[at];
+            if (ACT) q[j] = pre[at];
+        }
+        if (ACT) act_slopes(q, act);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += v[j];
+        for (int j = 0; j < 8; ++j) s += ACT ? v[j] * q[j] : v[j];
     }
-    for (; p < end; ++p) s += (float)d[(order ? (int64_t)order[p] : p) * ldd + c];
+    for (; p < end; ++p) {
+        const int64_t at = (order ? (int64_t)order[p] : p) * N + c;
+        const float v = (float)d[at];
+        s += ACT ? v * act_slope(pre[at], act) : v;
+    }
     out[((int64_t)part * groups + g) * N + c] = s;
 }
 
@@ -1405,14 +1426,22 @@ int outer_parts(int64_t M, int64_t groups, int64_t tiles, int64_t workgroups) {
 }
 
 // Whether d and db are made in one pass: with few columns most lanes of its
-// waves would have none, and gathered rows are faster in two.
-bool act_and_sums(const fl_linear *op) { return op->act != FL_ACT_NONE && op->N >= 256 && !op->offsets; }
+// waves would have none.  In several groups where d is rounded, so that db's
+// terms would be made twice otherwise, from 32 rows a group on (bf16 gelu, us
+// in one pass and in two, sizes falling with the group's number: 16384 rows of
+// 475 in 100 groups 68, 101; 4000 rows in 100 groups 60, 104, in 300 groups 225,
+// 92, where a part is a whole group and the largest one's rows are walked by
+// one workgroup).
+bool act_and_sums(const fl_linear *op) {
+    if (op->act == FL_ACT_NONE || op->N < 256) return false;
+    return !op->offsets || (op->dtype != FL_F32 && op->M >= 32 * op->groups);
+}
 
 // Parts of a group's rows in db's sums.
 int sum_parts(const fl_linear *op) {
     const int64_t M = op->M, N = op->N, groups = op->groups;
     if (act_and_sums(op)) {
-        const int64_t want = ceil_div(AS_GROUPS, ceil_div(N, AS_COLS)), most = M / 8;
+        const int64_t want = ceil_div(AS_GROUPS, ceil_div(N, AS_COLS) * groups), most = M / (8 * groups);
         const int64_t p = want < most ? want : most;
         return (int)(p < 1 ? 1 : p > 512 ? 512 : p);
     }
@@ -1560,13 +1589,19 @@ int weight_grad(hipStream_t st, const fl_linear *op, const void *d, void *dw, fl
 }
 
 template <typename T>
-int bias_grad(hipStream_t st, const fl_linear *op, const void *d, void *db, int db_f32, float *ws) {
+int bias_grad(hipStream_t st, const fl_linear *op, const void *gy, const float *pre, const void *d, void *db,
+              int db_f32, float *ws) {
     const int parts = sum_parts(op);
     const int64_t grid = (int64_t)parts * op->groups * ceil_div(op->N, LN_NT);
     if (!launch_fits(grid, LN_NT))
         return fl_fail(FL_ERR_ARG, "linear_bias_grad: too many groups for one launch (shape)");
-    FL_LAUNCH("k_col_sums", k_col_sums<T>, dim3((unsigned)grid), dim3(LN_NT), 0, st,
-              (const T *)d, op->N, op->M, op->N, op->groups, parts, op->order, op->offsets, ws);
+    const dim3 g((unsigned)grid), nt(LN_NT);
+    if (sizeof(T) == 2 && op->act != FL_ACT_NONE)
+        FL_LAUNCH("k_col_sums", (k_col_sums<T, true>), g, nt, 0, st, (const T *)gy, pre, op->act, op->M, op->N,
+                  op->groups, parts, op->order, op->offsets, ws);
+    else
+        FL_LAUNCH("k_col_sums", (k_col_sums<T, false>), g, nt, 0, st, (const T *)d, pre, op->act, op->M, op->N,
+                  op->groups, parts, op->order, op->offsets, ws);
     if (db_f32) fold_parts<float>(st, ws, parts, op->groups * op->N, (float *)db);
     else fold_parts<T>(st, ws, parts, op->groups * op->N, (T *)db);
     return fl_check_launch("linear_bias_grad");
@@ -1576,13 +1611,18 @@ template <typename T>
 int act_and_bias_grad(hipStream_t st, const fl_linear *op, const void *gy, const float *pre, void *d, void *db,
                       int db_f32, float *ws) {
     const int parts = sum_parts(op);
-    const int64_t grid = parts * ceil_div(op->N, AS_COLS);
+    const int64_t grid = parts * op->groups * ceil_div(op->N, AS_COLS);
     if (!launch_fits(grid, LN_NT))
-        return fl_fail(FL_ERR_ARG, "linear_backward: too many columns for one launch (shape)");
-    FL_LAUNCH("k_act_sums", k_act_sums<T>, dim3((unsigned)grid), dim3(LN_NT), 0, st, (const T *)gy, pre, op->M, op->N,
-              parts, op->act, (T *)d, ws);
-    if (db_f32) fold_parts<float>(st, ws, parts, op->N, (float *)db);
-    else fold_parts<T>(st, ws, parts, op->N, (T *)db);
+        return fl_fail(FL_ERR_ARG, "linear_backward: too many columns or groups for one launch (shape)");
+    const dim3 g((unsigned)grid), nt(LN_NT);
+    if (op->offsets)
+        FL_LAUNCH("k_act_sums", (k_act_sums<T, true>), g, nt, 0, st, (const T *)gy, pre, op->M, op->N, op->groups,
+                  parts, op->act, op->order, op->offsets, (T *)d, ws);
+    else
+        FL_LAUNCH("k_act_sums", (k_act_sums<T, false>), g, nt, 0, st, (const T *)gy, pre, op->M, op->N, op->groups,
+                  parts, op->act, op->order, op->offsets, (T *)d, ws);
+    if (db_f32) fold_parts<float>(st, ws, parts, op->groups * op->N, (float *)db);
+    else fold_parts<T>(st, ws, parts, op->groups * op->N, (T *)db);
     return fl_check_launch("linear_backward");
 }
 
@@ -1637,7 +1677,7 @@ int backward(hipStream_t st, const fl_linear *op, const void *gy, const float *p
     }
     if (!rc && dx && op->M && op->K) rc = input_grad<T>(st, op, d, dx, parts);
     if (!rc && dw && op->N && op->K) rc = weight_grad<T>(st, op, d, dw, parts);
-    if (!rc && db && op->N && !both) rc = bias_grad<T>(st, op, d, db, db_f32, parts);
+    if (!rc && db && op->N && !both) rc = bias_grad<T>(st, op, gy, pre, d, db, db_f32, parts);
     return rc;
 }
 

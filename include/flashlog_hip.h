@@ -880,9 +880,10 @@ int fl_linear_forward(void *stream, const fl_linear *op, void *y, float *pre,
                       void *ws, size_t ws_bytes);
 /* With d = gy * act'(pre) (gy [M, N] contiguous; pre unused without an
  * activation), those of the gradients that are not null: dx [M, K] = d W_g,
- * dw [groups, N, K] = d^T x and db [groups, N] = the sums of d over each
- * group's rows (0 for an empty group; db fp32 when db_f32, else of the
- * operands' type).  gy and ws lie on 16-byte boundaries. */
+ * dw [groups, N, K] = d^T x, both of the d that is rounded to the operands'
+ * type, and db [groups, N] = the sums of the unrounded d over each group's
+ * rows (0 for an empty group; db fp32 when db_f32, else of the operands'
+ * type).  gy and ws lie on 16-byte boundaries. */
 size_t fl_linear_backward_bytes(const fl_linear *op, int with_dx, int with_dw,
                                 int with_db);
 int fl_linear_backward(void *stream, const fl_linear *op, const void *gy,

@@ -143,3 +143,49 @@ def test_forward_mode_is_refused():
                 with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
                     call()
         assert fa.linear(x, w).shape == (4, 3)
+
+
+def _slope(p, act):
+    if act == "relu":
+        return (p > 0).double()
+    if act == "gelu":
+        return 0.5 * torch.erfc(-p / 2 ** 0.5) + p * torch.exp(-p * p / 2) / (2 * math.pi) ** 0.5
+    if act == "tanh":
+        return 1 - torch.tanh(p) ** 2
+    q = torch.sigmoid(p)
+    return q * (1 + p * (1 - q))
+
+
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu", "tanh"])
+@pytest.mark.parametrize("M,N,groups", [(24, 512, None), (24, 70, None), (120, 520, 5), (200, 520, 5),
+                                        (120, 70, 5)])
+def test_bias_gradient_adds_unrounded_terms(M, N, groups, act, t):
+    """A float32 bias of half-precision operands: neither the activation's argument nor d = g act'(p) is rounded to
+    the operands' type on the way.  The bound has, besides the sum's own, only the argument's float32 error (no
+    second derivative exceeds 1) and 16 e of the slope's evaluation."""
+    K = 8
+    fa = _fa()
+    g = torch.Generator().manual_seed(N)
+    G = groups or 1
+    x, w = torch.randn(M, K, generator=g).to(t), (torch.randn(G, N, K, generator=g) / K ** 0.5).to(t)
+    b, gy = torch.randn(G, N, generator=g), torch.randn(M, N, generator=g).to(t)
+    index = torch.randint(-1, G, (M,), generator=g) if groups else torch.zeros(M, dtype=torch.long)
+    index[index == 3] = 2  # an empty group
+    leaf = b.cuda().requires_grad_(True)
+    if groups:
+        y = fa.relation_linear(x.cuda(), fa.group_rows(index.cuda(), G), w.cuda(), leaf, act)
+    else:
+        y = fa.linear(x.cuda(), w[0].cuda(), leaf[0], act)
+    (db,) = torch.autograd.grad(y, [leaf], gy.cuda())
+    for k in range(G):
+        rows = (index == k).nonzero()[:, 0]
+        xr, wk, gr = x[rows].double(), w[k].double(), gy[rows].double()
+        p = xr @ wk.T + b[k].double()
+        dp = (K + 16) * E * (xr.abs() @ wk.abs().T + b[k].abs().double())
+        d = gr * _slope(p, act)
+        off = gr.abs() * (dp + 16 * E)
+        if act == "relu":
+            off = torch.where(p.abs() <= dp, gr.abs(), 0.0)
+        bound = off.sum(0) + (len(rows) + 16) * E * d.abs().sum(0)
+        assert ((db[k].double().cpu() - d.sum(0)).abs() <= bound).all()
