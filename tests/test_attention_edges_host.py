@@ -44,5 +44,5 @@ def test_more_tiles_than_a_launch_holds():
     refused(lib.fl_linear_backward(None, op, one, None, None, one, None, 0, ws, 1 << 60))
     op = _lib.FlLinear(M=1, N=1, K=0, groups=1 << 24, order=1, offsets=1, tiles=1)
     refused(lib.fl_linear_backward(None, op, one, None, None, None, one, 0, ws, 1 << 60))
-    op = _lib.FlLinear(M=5000, N=1 << 24, K=0, groups=1, act=2)
+    op = _lib.FlLinear(M=1 << 24, N=1 << 14, K=0, groups=1 << 19, act=2, dtype=1, order=1, offsets=1, tiles=1)
     refused(lib.fl_linear_backward(None, op, one, one, None, None, one, 0, ws, 1 << 60))
