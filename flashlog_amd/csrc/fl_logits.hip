@@ -9,7 +9,8 @@
 //
 //   softmax: w = exp(v - max) / sum over the allowed columns; a row with
 //   nothing left (no column allowed, or all of them -inf) is all zeros
-//   gradients: dv = g (softmax: w (g - sum w g)), dx = dv allowed slope with
+//   gradients: dv = g (softmax: w (g - sum w g), 0 and no part of the sum where
+//   w is 0, whatever g is), dx = dv allowed slope with
 //   slope = 1/temperature, for c > 0 times 1/repetition or repetition by the
 //   sign of x + bias; dbias[g] = the sum of the dx of the group's rows
 //
@@ -437,7 +438,8 @@ struct GradSegment {
             ok[i] = C::bits(r, base + C::local(i), cols);
             if (SOFTMAX && WHOLE)
 #pragma unroll
-                for (int e = 0; e < G; ++e) s += (ok[i] >> e) & 1 ? w[i].v[e] * (float)g[i].v[e] : 0.0f;
+                for (int e = 0; e < G; ++e)
+                    s += ((ok[i] >> e) & 1) && w[i].v[e] != 0.0f ? w[i].v[e] * (float)g[i].v[e] : 0.0f;
         }
         if (SOFTMAX) s = WHOLE ? fl_wave_sum_f32(s) : a.dots[row];
         Repeats<G, VPT> rep;
@@ -450,6 +452,7 @@ struct GradSegment {
 #pragma unroll
             for (int e = 0; e < G; ++e) {
                 u[e] = SOFTMAX ? w[i].v[e] * ((float)g[i].v[e] - s) : (float)g[i].v[e];
+                if (SOFTMAX && w[i].v[e] == 0.0f) u[e] = 0.0f;
                 u[e] *= a.l.inv_temperature;
             }
             if (HIST && rep.any(i)) {
@@ -585,7 +588,7 @@ __global__ __launch_bounds__(LG_NT) void k_logits_dot(LogitArgs a, const float *
         const Group<float, 4> p = load_group<float, 4>(w + row * a.op.cols, c, cols);
         const Group<float, 4> q = load_group<float, 4>(g + row * a.op.cols, c, cols);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s += (bits >> e) & 1 ? p.v[e] * q.v[e] : 0.0f;
+        for (int e = 0; e < 4; ++e) s += ((bits >> e) & 1) && p.v[e] != 0.0f ? p.v[e] * q.v[e] : 0.0f;
     }
     s = fl_wave_sum_f32(s);
     if (fl_lane() == 0) dots[item] = s;

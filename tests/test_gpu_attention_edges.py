@@ -189,3 +189,28 @@ def test_bias_gradient_adds_unrounded_terms(M, N, groups, act, t):
             off = torch.where(p.abs() <= dp, gr.abs(), 0.0)
         bound = off.sum(0) + (len(rows) + 16) * E * d.abs().sum(0)
         assert ((db[k].double().cpu() - d.sum(0)).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("n", [40, 9000])
+def test_rows_with_nothing_left_have_no_gradient(n):
+    """Nor have single columns of weight 0: what comes back for them may be anything."""
+    fa = _fa()
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(4, n, generator=g)
+    x[1] = -math.inf
+    x[2, : n // 2] = -math.inf
+    gy = torch.randn(4, n, generator=g)
+    for bias in (None, torch.zeros(n)):
+        clean = gy.clone()
+        dirty = gy.clone()
+        clean[2, : n // 2] = 0
+        dirty[1] = torch.tensor([math.nan, math.inf, -math.inf, 1.0])[torch.arange(n) % 4]
+        dirty[2, : n // 2] = math.nan
+        out = []
+        for up in (clean, dirty):
+            leaves = [x.cuda().requires_grad_(True)] + ([] if bias is None else [bias.cuda().requires_grad_(True)])
+            w = fa.hop_attention(leaves[0], bias=leaves[1] if bias is not None else None)
+            out.append(torch.autograd.grad(w, leaves, up.cuda()))
+        assert (out[1][0][1] == 0).all()
+        for p, q in zip(*out):
+            assert torch.equal(p, q)
