@@ -36,6 +36,7 @@
 #include "fl_abi.h"
 #include "fl_common.h"
 #include "fl_parts.h"
+#include <math.h>
 #include <type_traits>
 
 namespace fl {
@@ -623,8 +624,12 @@ int lg_check(const fl_logits *op, const char *what) {
     if (op->dtype < FL_F32 || op->dtype > FL_F16) return fl_fail(FL_ERR_ARG, "%s: unknown type", what);
     if (op->rows < 0 || op->cols < 0 || op->inner < 1 || op->rows % op->inner)
         return fl_fail(FL_ERR_ARG, "%s: bad shape", what);
-    if (!(op->temperature > 0.0f) || !(op->repetition > 0.0f))
-        return fl_fail(FL_ERR_ARG, "%s: temperature and repetition must lie in the range (0, inf)", what);
+    // the kernels multiply by their reciprocals, which have to be normal numbers as well
+    const auto divides = [](float v) { return v >= 0x1p-126f && v <= 0x1p126f; };
+    if (!divides(op->temperature) || !divides(op->repetition))
+        return fl_fail(FL_ERR_ARG, "%s: temperature and repetition must lie in the range [2^-126, 2^126]", what);
+    if (!(fabsf(op->presence) < INFINITY) || !(fabsf(op->frequency) < INFINITY))
+        return fl_fail(FL_ERR_ARG, "%s: presence and frequency must lie in float32's range", what);
     if (op->allowed && (op->allowed_rows < 1 || op->allowed_ld < lg_ceil(op->cols, 32) ||
                         (op->allowed_rows > 1 && op->rows > 0 && !op->group)))
         return fl_fail(FL_ERR_ARG, "%s: bad shape of the allowed table", what);

@@ -912,7 +912,9 @@ typedef struct fl_logits {
     const int64_t *history;   /* null: none                                */
     const int64_t *history_ptr;
     int64_t history_len;
-    float repetition, presence, frequency, temperature, fill;
+    float repetition, presence, frequency; /* repetition in [2^-126, 2^126],
+                                 the others finite                         */
+    float temperature, fill;  /* temperature in [2^-126, 2^126]            */
     int32_t dtype;
 } fl_logits;
 

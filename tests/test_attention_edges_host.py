@@ -46,3 +46,18 @@ def test_more_tiles_than_a_launch_holds():
     refused(lib.fl_linear_backward(None, op, one, None, None, None, one, 0, ws, 1 << 60))
     op = _lib.FlLinear(M=1 << 24, N=1 << 14, K=0, groups=1 << 19, act=2, dtype=1, order=1, offsets=1, tiles=1)
     refused(lib.fl_linear_backward(None, op, one, one, None, None, one, 0, ws, 1 << 60))
+
+
+@pytest.mark.parametrize("name,bad,good", [("temperature", 1e39, 2.0 ** 126), ("temperature", 1e-39, 2.0 ** -126),
+                                           ("repetition", 1e39, 2.0 ** 126), ("repetition", 1e-40, 2.0 ** -126),
+                                           ("presence", 1e39, 3e38), ("frequency", -1e39, -3e38),
+                                           ("frequency", float("nan"), 0.0)])
+def test_scalars_that_float32_cannot_divide_by(name, bad, good):
+    """Finite numbers of 64 bits that are infinite, or have an infinite reciprocal, in 32."""
+    lib = _lib.lib()
+    one = ctypes.c_void_p(1)
+    op = _logits_op(**{name: bad})
+    for rc in (lib.fl_logits_constrain(None, op, one), lib.fl_logits_softmax(None, op, one, None, 0),
+               lib.fl_logits_grad(None, op, None, one, one, None, None, 0)):
+        assert rc == 1 and "range" in lib.fl_last_error().decode()
+    assert lib.fl_logits_constrain(None, _logits_op(rows=0, **{name: good}), one) == 0

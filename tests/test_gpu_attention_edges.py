@@ -214,3 +214,13 @@ def test_rows_with_nothing_left_have_no_gradient(n):
         assert (out[1][0][1] == 0).all()
         for p, q in zip(*out):
             assert torch.equal(p, q)
+
+
+def test_scalars_out_of_float32():
+    fa = _fa()
+    x = torch.zeros(2, 5).cuda()
+    for kw in (dict(temperature=1e39), dict(temperature=1e-39), dict(repetition=1e39), dict(repetition=1e-40),
+               dict(presence=1e39), dict(frequency=-1e39)):
+        for fn in (fa.constrain_logits, fa.hop_attention):
+            with pytest.raises(ValueError):
+                fn(x, **kw)
