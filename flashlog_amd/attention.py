@@ -322,9 +322,11 @@ def history_from_pairs(rows, ids, count):
     _need_gpu("history_from_pairs", rows, ids)
     if rows.dim() != 1 or rows.shape != ids.shape:
         raise ValueError("history_from_pairs: rows and ids must be 1D and equally long")
-    ids = _integers("history_from_pairs", "ids", ids)
-    plan = group_rows(rows, max(int(count), 1))
-    return plan.offsets[:int(count) + 1].long(), ids[plan.order.long()]
+    ids, count = _integers("history_from_pairs", "ids", ids), int(count)
+    if count < 0:
+        raise ValueError("history_from_pairs: count must be nonnegative")
+    plan = group_rows(rows, max(count, 1))
+    return plan.offsets[:count + 1].long(), ids[plan.order.long()]
 
 
 class _Constraints:

@@ -224,3 +224,16 @@ def test_scalars_out_of_float32():
         for fn in (fa.constrain_logits, fa.hop_attention):
             with pytest.raises(ValueError):
                 fn(x, **kw)
+
+
+def test_history_of_a_count_of_rows():
+    fa = _fa()
+    rows, ids = torch.tensor([0, 2, 0]).cuda(), torch.tensor([7, 8, 9]).cuda()
+    for count in (-1, -2):
+        with pytest.raises(ValueError):
+            fa.history_from_pairs(rows, ids, count)
+    off, got = fa.history_from_pairs(rows, ids, 0)
+    assert off.tolist() == [0]
+    assert fa.constrain_logits(torch.zeros(0, 20).cuda(), history=(off, got), presence=1.0).shape == (0, 20)
+    off, got = fa.history_from_pairs(rows, ids, 1)
+    assert off.tolist() == [0, 2] and got[:2].tolist() == [7, 9]
