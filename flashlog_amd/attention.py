@@ -275,9 +275,10 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     float32), residual [..., outputs]; activation None, "relu", "gelu" (the
     erf form), "silu", "tanh" or "sigmoid".  Rows and weights may be strided;
     operands whose last dimension is not contiguous are copied.  Sums are
-    float32 and the result is rounded once; with float32 operands products
-    are as exact as float32 ones, except that a sum which an infinity or NaN
-    enters is NaN.  For the backward the
+    float32 and the result is rounded once; with float32 operands every
+    product is off by less than 2^-22 of itself, to either side (a float32
+    product by up to 2^-24), and a sum which an infinity or NaN enters is NaN.
+    Activations are evaluated to 2^-20 of 1 + |argument|.  For the backward the
     activation's argument is kept in float32; its gradient is rounded to the
     operands' type as an operand of two products, but not as a term of the
     bias's."""

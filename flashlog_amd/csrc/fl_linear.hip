@@ -18,10 +18,13 @@
 // once per 16 rows.
 //
 // bfloat16 and half operands feed the instruction as they are, sums are fp32.
-// fp32 operands are cut into three bfloat16 planes by truncation, v = v0 + v1
-// + v2 exactly (24 significant bits in 8 + 8 + 8), and the six products whose
-// weight is at least 2^-16 are added: what is dropped is below 2^-22 of a
-// product (2^-24 on average), as near as fp32 products are.  The matrix unit
+// fp32 operands are cut into three bfloat16 planes, v = v0 + v1 + v2 exactly: v0
+// truncated (no value overflows), v1 the rest rounded to the nearest, so that
+// |v1| is below 2^-7 and |v2| at most 2^-16 of |v|, of either sign.  The six
+// products whose weight is at least 2^-16 are added; what is dropped, mostly
+// v1 w2 + v2 w1, is below 2^-22 of a product and as often above 0 as below
+// (with both planes truncated it was up to 2^-21, always towards 0).  An fp32
+// product is rounded by up to 2^-24 of itself.  The matrix unit
 // takes bfloat16 16 times faster than fp32, so the six products run at 2.7 times the
 // fp32 instruction's rate.  The planes of an infinity or NaN hold a NaN: sums
 // that such a value enters are NaN.
@@ -115,19 +118,18 @@ __device__ __forceinline__ void chunk_planes(const T (&v)[8], u32x4 (&out)[Plane
 }
 template <>
 __device__ __forceinline__ void chunk_planes<float>(const float (&v)[8], u32x4 (&out)[3]) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        uint32_t w[2][3];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float x = v[2 * j + i];
-            w[i][0] = __float_as_uint(x);
-            const float r1 = x - __uint_as_float(w[i][0] & 0xffff0000u);
-            w[i][1] = __float_as_uint(r1);
-            w[i][2] = __float_as_uint(r1 - __uint_as_float(w[i][1] & 0xffff0000u));
-        }
-#pragma unroll
-        for (int p = 0; p < 3; ++p) out[p][j] = upper_halves(w[0][p], w[1][p]);
+        const uint32_t x0 = __float_as_uint(v[2 * j]), x1 = __float_as_uint(v[2 * j + 1]);
+        const float r0 = v[2 * j] - __uint_as_float(x0 & 0xffff0000u);
+        const float r1 = v[2 * j + 1] - __uint_as_float(x1 & 0xffff0000u);
+        const uint32_t m = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{r0, r1}), bf16x2));
+        out[0][j] = upper_halves(x0, x1);
+        out[1][j] = m;
+        out[2][j] = upper_halves(__float_as_uint(r0 - __uint_as_float(m << 16)),
+                                 __float_as_uint(r1 - __uint_as_float(m & 0xffff0000u)));
     }
 }
 

@@ -237,3 +237,20 @@ def test_history_of_a_count_of_rows():
     assert fa.constrain_logits(torch.zeros(0, 20).cuda(), history=(off, got), presence=1.0).shape == (0, 20)
     off, got = fa.history_from_pairs(rows, ids, 1)
     assert off.tolist() == [0, 2] and got[:2].tolist() == [7, 9]
+
+
+def test_products_of_float32():
+    """Single products: what the planes drop is below 2^-22 of each (values whose lower planes are all ones are the
+    worst), the last addition is off by at most a step of 2^-23, those before it by 2^-28 in all."""
+    g = torch.Generator().manual_seed(8)
+    low = torch.randint(1 << 23, (2048,), generator=g)
+    low[:700] |= 0xFFFF
+    low[:300] = 0xFFFF
+    low[:300] += torch.arange(300) << 14
+    bits = low | 127 << 23
+    x = bits.to(torch.int32).view(torch.float32)
+    big = torch.tensor([torch.finfo(torch.float32).max, -torch.finfo(torch.float32).max, 3.3961e38])
+    y = _fa().linear(x[:, None].cuda(), x[:512, None].cuda()).double().cpu()
+    want = x.double()[:, None] * x.double()[None, :512]
+    assert ((y - want).abs() <= (2.0 ** -22 + 2.0 ** -23 + 2.0 ** -28) * want).all()
+    assert torch.equal(_fa().linear(big[:, None].cuda(), torch.ones(1, 1).cuda())[:, 0].cpu(), big)
