@@ -1210,7 +1210,8 @@ __global__ __launch_bounds__(LN_NT) void k_act_grad(const T *__restrict__ gy, co
 // before d is rounded: a workgroup takes 512 columns, eight a lane, each wave a
 // quarter of its rows, in the plan's order if GATHER (rows of no group have no
 // d).  [16384 x 2048] fp16: 54 us = 5.0 TB/s, 63 in two passes; bf16 in 24
-// groups 60 us.
+// groups 76 us (the workgroups of a row's columns on one XCD; 82 spread over
+// all, 93 with half as many workgroups).
 constexpr int AS_COLS = 8 * FL_WAVE;
 constexpr int AS_GROUPS = 2048;  // workgroups, where the rows give as many
 
@@ -1223,21 +1224,23 @@ __global__ __launch_bounds__(LN_NT) void k_act_sums(const T *__restrict__ gy, co
     constexpr int AHEAD = 4;
     constexpr int WAVES = LN_NT / FL_WAVE;
     __shared__ float sums[WAVES][AS_COLS];
-    const uint32_t blocks = (uint32_t)((N + AS_COLS - 1) / AS_COLS), item = blockIdx.x / blocks;
-    const int64_t c0 = (int64_t)(blockIdx.x % blocks) * AS_COLS, c = c0 + fl_lane() * 8;
+    const uint32_t w = GATHER ? (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x) : blockIdx.x;
+    const uint32_t blocks = (uint32_t)((N + AS_COLS - 1) / AS_COLS), item = w / blocks;
+    const int64_t c0 = (int64_t)(w % blocks) * AS_COLS, c = c0 + fl_lane() * 8;
     const int64_t g = GATHER ? item / parts : 0, part = GATHER ? item % parts : item;
     const int have = N - c < 8 ? (int)(N - c) : 8;
     int64_t begin, end;
     part_range(GATHER ? offsets : nullptr, M, g, parts * WAVES, (int)part * WAVES + fl_wave_id(), &begin, &end);
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    int rows = 0;  // lane j: the j-th of 64 in the order
     for (int64_t p = begin; p < end; p += AHEAD) {
         float v[AHEAD][8], q[AHEAD][8];
         int64_t row[AHEAD];
+        const int at = (int)(p - begin) % FL_WAVE;
+        if (GATHER && at == 0) rows = order[p + fl_lane() < end ? p + fl_lane() : end - 1];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            row[j] = p + j < end ? p + j : end - 1;
-            if constexpr (GATHER) row[j] = order[row[j]];
-        }
+        for (int j = 0; j < AHEAD; ++j)
+            row[j] = GATHER ? (int64_t)__builtin_amdgcn_readlane(rows, at + j) : p + j < end ? p + j : end - 1;
         if (have <= 0) continue;
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
