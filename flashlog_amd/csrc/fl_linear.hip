@@ -608,9 +608,9 @@ __global__ __launch_bounds__(LN_NT) void k_lin_finish(RowsArgs a) {
 }
 
 // Products whose C rows are the batch's rows (the forward, and dx): a tile is
-// BM rows of one group.  fp32 [1536 x 2048 -> 1645]: 76 us = 136 TFLOP/s, dx 97,
+// BM rows of one group.  fp32 [1536 x 2048 -> 1645]: 65 us = 159 TFLOP/s, dx 86,
 // bound by the six products' matrix instructions and the LDS reads before them;
-// [15000 x 128 -> 75] in 74 groups 16 us, four steps of latency.
+// [15000 x 128 -> 75] in 74 groups 17 us, four steps of latency.
 template <typename T, bool B_CONTIG, int BM, int BN, int BK>
 __global__ __launch_bounds__(LN_NT) void k_lin_rows(RowsArgs a) {
     using Prod = Product<T, BM, BN, BK>;
@@ -698,7 +698,7 @@ __device__ __forceinline__ void store_outer(const OuterArgs &a, const f32x4 (&ac
 }
 
 // dW_g = sum over the group's rows (a part of them) of d^T x.  fp32 [1645 x
-// 2048] over 1536 rows: 102 us; [75 x 128] over 15000 rows in 74 groups 21 us.
+// 2048] over 1536 rows: 86 us; [75 x 128] over 15000 rows in 74 groups 21 us.
 template <typename T, int BM, int BN, int BK>
 __global__ __launch_bounds__(LN_NT) void k_lin_outer(OuterArgs a) {
     using Prod = Product<T, BM, BN, BK>;
@@ -1095,11 +1095,11 @@ __device__ __forceinline__ void wide_store_outer(const OuterArgs &a, const f32x4
     });
 }
 
-// The forward (B_CONTIG) and dx.  [8192 x 8192 -> 8192] bf16: 888 us = 1238
-// TFLOP/s; [16384 x 2048 -> 2048] 127 us = 1083 TFLOP/s (two rounds of 256
-// tiles, whose first loads and last stores nothing overlaps), 186 us with silu,
-// a residual and the argument kept: its fp32 values go past the caches (210 us
-// through them).
+// The forward (B_CONTIG) and dx.  [8192 x 8192 -> 8192] bf16: 900 us = 1221
+// TFLOP/s; [16384 x 2048 -> 2048] 121 us = 1136 TFLOP/s (two rounds of 256
+// tiles, whose first loads and last stores nothing overlaps), 163 us in fp16 with
+// silu, a residual and the argument kept: its fp32 values go past the caches
+// (through them an eighth more).
 template <typename T, bool B_CONTIG, int BM, int BK, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_rows(RowsArgs a) {
     using TA = WideContig<BM, BK>;
@@ -1146,7 +1146,7 @@ __device__ __forceinline__ uint32_t outer_item(const OuterArgs &a) {
     return (j * FL_XCDS + (j & 1 ? FL_XCDS - 1 - x : x)) * unit + p % unit;
 }
 
-// dW.  [2048 x 2048] over 16384 fp16 rows: 144 us = 954 TFLOP/s in four parts
+// dW.  [2048 x 2048] over 16384 fp16 rows: 123 us = 1116 TFLOP/s in four parts
 // of the rows, that fold_parts joins in 12 us.
 template <typename T, bool GATHER, int BK, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
@@ -1209,7 +1209,7 @@ __global__ __launch_bounds__(LN_NT) void k_act_grad(const T *__restrict__ gy, co
 // The same and the column sums of a part of a group's rows in one pass, added
 // before d is rounded: a workgroup takes 512 columns, eight a lane, each wave a
 // quarter of its rows, in the plan's order if GATHER (rows of no group have no
-// d).  [16384 x 2048] fp16: 54 us = 5.0 TB/s, 63 in two passes; bf16 in 24
+// d).  [16384 x 2048] fp16: 55 us = 4.8 TB/s, 63 in two passes; bf16 in 24
 // groups 76 us (the workgroups of a row's columns on one XCD; 82 spread over
 // all, 93 with half as many workgroups).
 constexpr int AS_COLS = 8 * FL_WAVE;
@@ -1273,7 +1273,7 @@ __global__ __launch_bounds__(LN_NT) void k_act_sums(const T *__restrict__ gy, co
 }
 
 // Column sums of a group's rows (a part of them), one thread a column: [16384 x
-// 2048] fp16 18 us = 3.7 TB/s.  With an activation (ACT) d's terms are made
+// 2048] fp16 15 us = 4.5 TB/s.  With an activation (ACT) d's terms are made
 // again from the gradient gy and the argument, unrounded.
 template <typename T, bool ACT>
 __global__ __launch_bounds__(LN_NT) void k_col_sums(const T *__restrict__ d, const float *__restrict__ pre, int act,
@@ -1321,7 +1321,7 @@ struct Cut {
 // A 32-value step of a tile takes `alone` microseconds where CUs hold one
 // workgroup, `shared` times the workgroups of a CU where they hold more (fp32:
 // [1536 x 2048 -> 1645] takes 147 us in 156 tiles of 128, 101 us in 624 tiles
-// of 64; [8192 x 2048 -> 2048] 370 us in tiles of 128); joining parts takes a
+// of 64; [8192 x 2048 -> 2048] 383 us in tiles of 128); joining parts takes a
 // launch and their traffic.
 Cut best_cut(int64_t M, int64_t N, int64_t K, bool f32, bool small_tiles) {
     struct Tile {
