@@ -499,10 +499,13 @@ def constrain_logits(logits, allowed=None, group=None, bias=None, history=None, 
     allowed: a bool mask [n] or [groups, n], or its ``pack_allowed`` (keep
     that where the mask stays the same); bias [n] or [groups, n].  group: the
     table row of every row, integers of the logits' leading shape or of its
-    first dimensions (a query's steps then share it); a group outside the
-    tables has nothing allowed.  history: ids [..., h] for the logits' leading
-    shape or its first dimensions, padded with ids outside [0, n), or
-    (offsets, ids) with the ids offsets[i] .. offsets[i+1] of row i.
+    first dimensions (a query's steps then share it).  A table of one row is
+    every row's, whatever its group; a group outside a table of several has
+    nothing allowed.  history: ids [..., h] for the logits' leading shape or
+    its first dimensions, padded with ids outside [0, n), or (offsets, ids)
+    with the ids offsets[i] .. offsets[i+1] of row i; a column is counted up
+    to some 65,000 times.  The scalars are float32; repetition and temperature
+    lie in [2^-126, 2^126].
 
     Masked logits are not read into anything: they may be infinite or NaN.
     Gradients reach logits and bias; masked columns have none."""
@@ -515,6 +518,7 @@ def hop_attention(logits, allowed=None, group=None, bias=None, history=None, rep
     """A hop's attention: the softmax of ``constrain_logits`` over the allowed
     columns, float32 [..., n], with the same arguments.  Masked columns are
     exactly 0; a row with nothing left (no column allowed, or every allowed
-    logit -inf) is all zeros and has no gradient."""
+    logit -inf) is all zeros and has no gradient.  A NaN or +inf among a row's
+    allowed logits makes the row's other allowed weights NaN."""
     return _apply(logits, *_constraints("hop_attention", logits, allowed, group, bias, history, repetition, presence,
                                         frequency, temperature, 0.0), softmax=True)

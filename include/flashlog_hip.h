@@ -896,8 +896,8 @@ int fl_linear_backward(void *stream, const fl_linear *op, const void *gy,
  * a history of column ids, history_len of them
  * padded with ids outside [0, cols), or with history_ptr [owners + 1] the
  * ids of [ptr[o], ptr[o+1]) in a list of history_len.  An owner whose group
- * is outside a table has nothing allowed.  With c = how often a column is in
- * the history:
+ * is outside a table of several rows has nothing allowed.  With c = how often
+ * a column is in the history (up to some 65,000 times):
  *   u = x + bias; if c: u = u > 0 ? u / repetition : u * repetition,
  *   u -= presence + frequency c;  v = u / temperature; not allowed: fill. */
 typedef struct fl_logits {

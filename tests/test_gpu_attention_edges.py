@@ -254,3 +254,41 @@ def test_products_of_float32():
     want = x.double()[:, None] * x.double()[None, :512]
     assert ((y - want).abs() <= (2.0 ** -22 + 2.0 ** -23 + 2.0 ** -28) * want).all()
     assert torch.equal(_fa().linear(big[:, None].cuda(), torch.ones(1, 1).cuda())[:, 0].cpu(), big)
+
+
+@pytest.mark.parametrize("t", HALVES)
+def test_bias_gradient_of_groups_captured(t):
+    """Activation's gradient and column sums of gathered rows in one pass: the same bits every time, and in a graph
+    that is replayed on other rows and groups beside eager work."""
+    fa = _fa()
+    g = torch.Generator().manual_seed(6)
+    x, w = torch.randn(400, 40, generator=g).to(t).cuda(), (torch.randn(6, 515, 40, generator=g) / 6).to(t).cuda()
+    b, gy = torch.randn(6, 515, generator=g).cuda(), torch.randn(400, 515, generator=g).to(t).cuda()
+    index = torch.randint(-1, 7, (400,), generator=g).cuda()
+
+    def step():
+        leaves = [v.detach().requires_grad_(True) for v in (x, w, b)]
+        y = fa.relation_linear(leaves[0], fa.group_rows(index, 6), leaves[1], leaves[2], "gelu")
+        return [y.detach(), *torch.autograd.grad(y, leaves, gy)]
+
+    first = step()
+    for _ in range(2):
+        for p, q in zip(first, step()):
+            assert torch.equal(p, q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(3):
+        h = torch.Generator().manual_seed(60 + k)
+        x.copy_(torch.randn(400, 40, generator=h))
+        index.copy_(torch.randint(-1, 7, (400,), generator=h))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(want, out):
+            assert torch.equal(p, q)
