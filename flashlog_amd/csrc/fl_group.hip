@@ -140,7 +140,8 @@ __device__ __forceinline__ void write_tiles(const GroupArgs &a, int *lds) {
         int b = 0, n = 0;
         if (i < ng) {
             b = a.offsets[i];
-            n = ((i < a.groups ? a.offsets[i + 1] : (int)a.rows) - b + a.block - 1) / a.block;
+            const uint32_t rows = (uint32_t)((i < a.groups ? a.offsets[i + 1] : (int)a.rows) - b);
+            n = (int)((rows + a.block - 1) / a.block);  // rows + block may pass 2^31
         }
         int total;
         const int pre = fl_block_excl_scan<GR_NT>(n, lds, &total);

@@ -292,3 +292,20 @@ def test_bias_gradient_of_groups_captured(t):
         torch.cuda.synchronize()
         for p, q in zip(want, out):
             assert torch.equal(p, q)
+
+
+def test_as_many_rows_as_a_plan_takes():
+    """2^31 - 1 rows, all but three in one group: its tiles are counted past 2^31 - 256 rows too."""
+    fa = _fa()
+    rows = (1 << 31) - 1
+    index = torch.zeros(rows, dtype=torch.long, device="cuda")
+    index[[5, 1 << 30, rows - 1]] = -1
+    plan = fa.group_rows(index, 1)
+    del index
+    assert plan.offsets.tolist() == [0, rows - 3]
+    assert plan.order[-4:].tolist() == [rows - 2, 5, 1 << 30, rows - 1]
+    assert plan.order[4:6].tolist() == [4, 6]
+    tiles = plan.tiles.view(-1, 2)
+    n = (rows - 3 + 255) // 256
+    assert not tiles[:n, 0].any() and torch.equal(tiles[:n, 1].long(), 256 * torch.arange(n, device="cuda"))
+    assert tiles[n:].tolist()[0] == [1, rows - 3] and (tiles[n + 1:, 0] == -1).all()
