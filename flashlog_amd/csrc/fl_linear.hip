@@ -1027,11 +1027,21 @@ __device__ __forceinline__ void wide_rows_out(const f32x4 (&acc)[MT][4], float *
     }
 }
 
-// The first `have` of eight values as floats, the others 0.
-template <typename U>
+typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+
+// The first `have` of eight values as floats, the others 0.  PAST: past the
+// caches.
+template <bool PAST = false, typename U>
 __device__ __forceinline__ void load_eight(const U *p, int have, float (&out)[8]) {
     if (have >= 8) {
-        const Vec<U, 8> r = load_vec<U, 8>(p);
+        Vec<U, 8> r;
+        if constexpr (PAST) {
+            Words q[sizeof(r) / 16];
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(r) / 16; ++i)
+                q[i] = __builtin_nontemporal_load(reinterpret_cast<const Words *>(p) + i);
+            __builtin_memcpy(&r, q, sizeof(r));
+        } else r = load_vec<U, 8>(p);
 #pragma unroll
         for (int e = 0; e < 8; ++e) out[e] = (float)r.v[e];
     } else
@@ -1044,7 +1054,6 @@ __device__ __forceinline__ void store_eight(U *p, int have, const float (&v)[8])
 #pragma unroll
     for (int e = 0; e < 8; ++e) o.v[e] = (U)v[e];
     if (have >= 8) {
-        typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
         Words q[sizeof(o) / 16];
         __builtin_memcpy(q, &o, sizeof(o));
 #pragma unroll
@@ -1062,15 +1071,15 @@ __device__ __forceinline__ void wide_store_rows(const RowsArgs &a, const f32x4 (
     const int have = a.N - n < 8 ? (int)(a.N - n) : 8;
     float bias[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (a.bias && !t.none && have > 0) {
-        if (a.bias_f32) load_eight<float>((const float *)a.bias + t.g * a.bias_group + n, have, bias);
-        else load_eight<T>((const T *)a.bias + t.g * a.bias_group + n, have, bias);
+        if (a.bias_f32) load_eight<false, float>((const float *)a.bias + t.g * a.bias_group + n, have, bias);
+        else load_eight<false, T>((const T *)a.bias + t.g * a.bias_group + n, have, bias);
     }
     wide_rows_out<MT>(acc, slice, [&](int r, int, float (&v)[8]) {
         const int64_t p = pos + r;
         if (p >= t.end || have <= 0) return;
         const int64_t row = a.order ? (int64_t)a.order[p] : p;
         float res[8];
-        if (a.residual) load_eight<T>((const T *)a.residual + row * a.ldres + n, have, res);
+        if (a.residual) load_eight<false, T>((const T *)a.residual + row * a.ldres + n, have, res);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += bias[e];
         if (a.pre) store_eight<true, float>(a.pre + row * a.N + n, have, v);
@@ -1211,7 +1220,9 @@ __global__ __launch_bounds__(LN_NT) void k_act_grad(const T *__restrict__ gy, co
 // quarter of its rows, in the plan's order if GATHER (rows of no group have no
 // d).  [16384 x 2048] fp16: 55 us = 4.8 TB/s, 63 in two passes; bf16 in 24
 // groups 76 us (the workgroups of a row's columns on one XCD; 82 spread over
-// all, 93 with half as many workgroups).
+// all, 93 with half as many workgroups).  What it reads is not read again and
+// goes past the caches, which keep d for dx (there 114 -> 104 us) and dW
+// (113 -> 107).
 constexpr int AS_COLS = 8 * FL_WAVE;
 constexpr int AS_GROUPS = 2048;  // workgroups, where the rows give as many
 
@@ -1244,8 +1255,8 @@ __global__ __launch_bounds__(LN_NT) void k_act_sums(const T *__restrict__ gy, co
         if (have <= 0) continue;
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            load_eight<T>(gy + row[j] * N + c, have, v[j]);
-            load_eight<float>(pre + row[j] * N + c, have, q[j]);
+            load_eight<true, T>(gy + row[j] * N + c, have, v[j]);
+            load_eight<true, float>(pre + row[j] * N + c, have, q[j]);
         }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
