@@ -1155,7 +1155,7 @@ __device__ __forceinline__ uint32_t outer_item(const OuterArgs &a) {
     return (j * FL_XCDS + (j & 1 ? FL_XCDS - 1 - x : x)) * unit + p % unit;
 }
 
-// dW.  [2048 x 2048] over 16384 fp16 rows: 123 us = 1116 TFLOP/s in four parts
+// dW.  [2048 x 2048] over 16384 fp16 rows: 119 us = 1155 TFLOP/s in four parts
 // of the rows, that fold_parts joins in 12 us.
 template <typename T, bool GATHER, int BK, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_outer(OuterArgs a) {
@@ -1218,8 +1218,8 @@ __global__ __launch_bounds__(LN_NT) void k_act_grad(const T *__restrict__ gy, co
 // The same and the column sums of a part of a group's rows in one pass, added
 // before d is rounded: a workgroup takes 512 columns, eight a lane, each wave a
 // quarter of its rows, in the plan's order if GATHER (rows of no group have no
-// d).  [16384 x 2048] fp16: 55 us = 4.8 TB/s, 63 in two passes; bf16 in 24
-// groups 76 us (the workgroups of a row's columns on one XCD; 82 spread over
+// d).  [16384 x 2048] fp16: 51 us = 5.3 TB/s, 63 in two passes; bf16 in 24
+// groups 77 us (the workgroups of a row's columns on one XCD; 82 spread over
 // all, 93 with half as many workgroups).  What it reads is not read again and
 // goes past the caches, which keep d for dx (there 114 -> 104 us) and dW
 // (113 -> 107).
