@@ -110,6 +110,40 @@ class FlLogits(ctypes.Structure):
     ]
 
 
+class FlNorm(ctypes.Structure):
+    """Mirror of ``fl_norm`` (include/flashlog_hip.h)."""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("M", ctypes.c_int64), ("N", ctypes.c_int64), ("ldx", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+        ("eps", ctypes.c_float), ("dtype", ctypes.c_int32), ("wide", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class FlLists(ctypes.Structure):
+    """Mirror of ``fl_lists`` (include/flashlog_hip.h)."""
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("k", ctypes.c_int64), ("ids", ctypes.c_void_p), ("teacher", ctypes.c_void_p),
+        ("temperature", ctypes.c_float), ("reserved", ctypes.c_int32),
+    ]
+
+
+class FlScores(ctypes.Structure):
+    """Mirror of ``fl_scores`` (include/flashlog_hip.h)."""
+    _fields_ = [
+        ("lists", FlLists), ("logits", ctypes.c_void_p), ("cols", ctypes.c_int64), ("ld", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class FlVocab(ctypes.Structure):
+    """Mirror of ``fl_vocab`` (include/flashlog_hip.h)."""
+    _fields_ = [
+        ("lists", FlLists), ("M", ctypes.c_int64), ("V", ctypes.c_int64), ("K", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("weight", ctypes.c_void_p), ("ldw", ctypes.c_int64),
+        ("bias", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("bias_f32", ctypes.c_int32),
+    ]
+
+
 _SIGS = {
     "fl_last_error": (ctypes.c_char_p, []),
     "fl_abi_version": (ctypes.c_int, []),
@@ -270,6 +304,24 @@ _SIGS = {
     "fl_logits_grad_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLogits)] + [ctypes.c_int] * 3),
     "fl_logits_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlLogits)] + [ctypes.c_void_p] * 5 +
                        [ctypes.c_size_t]),
+    "fl_norm_op_bytes": (ctypes.c_size_t, []),
+    "fl_norm_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlNorm)] + [ctypes.c_void_p] * 2),
+    "fl_norm_backward_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlNorm), ctypes.c_int]),
+    "fl_norm_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlNorm)] + [ctypes.c_void_p] * 6 +
+                         [ctypes.c_size_t]),
+    "fl_lists_state_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlLists)]),
+    "fl_scores_op_bytes": (ctypes.c_size_t, []),
+    "fl_scores_forward_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlScores)]),
+    "fl_scores_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlScores)] + [ctypes.c_void_p] * 3 +
+                          [ctypes.c_size_t]),
+    "fl_scores_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlScores)] + [ctypes.c_void_p] * 3),
+    "fl_vocab_op_bytes": (ctypes.c_size_t, []),
+    "fl_vocab_forward_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlVocab)]),
+    "fl_vocab_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlVocab)] + [ctypes.c_void_p] * 3 +
+                         [ctypes.c_size_t]),
+    "fl_vocab_backward_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlVocab)] + [ctypes.c_int] * 3),
+    "fl_vocab_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlVocab)] + [ctypes.c_void_p] * 6 +
+                          [ctypes.c_size_t]),
     "fl_prof_enable": (ctypes.c_int, [ctypes.c_int]),
     "fl_prof_read": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),
                                     ctypes.POINTER(ctypes.c_int64)]),
@@ -296,7 +348,8 @@ def exported_symbols():
 # each argument struct and the entry point returning the library's sizeof
 STRUCT_SIZES = ((FlSide, "fl_side_bytes"), (FlSparseHop, "fl_sparse_hop_bytes"),
                 (FlGroundGraph, "fl_ground_graph_bytes"), (FlLinear, "fl_linear_op_bytes"),
-                (FlLogits, "fl_logits_op_bytes"))
+                (FlLogits, "fl_logits_op_bytes"), (FlNorm, "fl_norm_op_bytes"), (FlScores, "fl_scores_op_bytes"),
+                (FlVocab, "fl_vocab_op_bytes"))
 
 
 def lib():

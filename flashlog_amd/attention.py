@@ -7,6 +7,7 @@ evaluation takes score rows ``[Q, E]``.  The reference's model files make w
 with torch (linear layers, then ``softmax(w_all[:, t] / tau_1)``,
 src/model_DRUM_kernel.py:90-117); it has no constraints on either.  Here:
 
+  layer_norm       normalised rows, in front of the layers and heads;
   linear           act(x W^T + b) + residual in one pass: generator layers and
                    the head that makes relation logits;
   relation_linear  the same with weights of its own for every head relation,
@@ -20,11 +21,12 @@ src/model_DRUM_kernel.py:90-117); it has no constraints on either.  Here:
 
 Operands are float32, bfloat16 or float16 tensors on the GPU (CPU tensors
 raise); sums, softmax statistics and gradients of tables are float32.  All
-four are differentiable (once and backward: a second derivative and
+five are differentiable (once and backward: a second derivative and
 forward-mode tangents raise), run on torch's current stream, allocate with
 torch, and neither synchronise nor keep anything between calls, so they can be
 captured into a graph.  A captured backward needs leaves whose gradient graph
-was not begun outside the capture, as everywhere in torch.
+was not begun outside the capture, as everywhere in torch.  ``losses`` has what
+the logits and scores are trained with.
 """
 import math
 
@@ -34,10 +36,10 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import FlLinear, FlLogits, check
+from ._lib import FlLinear, FlLogits, FlNorm, check
 
-__all__ = ["RowGroups", "group_rows", "linear", "relation_linear", "pack_allowed", "history_from_pairs",
-           "constrain_logits", "hop_attention"]
+__all__ = ["RowGroups", "group_rows", "layer_norm", "linear", "relation_linear", "pack_allowed",
+           "history_from_pairs", "constrain_logits", "hop_attention"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3, "tanh": 4, "sigmoid": 5}
@@ -296,6 +298,84 @@ def relation_linear(x, groups, weight, bias=None, activation=None, residual=None
     if not isinstance(groups, RowGroups):
         raise TypeError("relation_linear: groups must come from group_rows")
     return _product("relation_linear", x, groups, weight, bias, activation, residual)
+
+
+# ---------------------------------------------------------------------------
+# Layer normalisation
+
+
+def _norm_op(x, weight, bias, eps, wide):
+    return FlNorm(x.data_ptr(), x.shape[0], x.shape[1], x.stride(0), _ptr(weight), _ptr(bias), eps, _TYPES[x.dtype],
+                  wide, 0)
+
+
+def _norm_forward(x, weight, bias, eps, wide, keep):
+    """(y, the laid out x, weight and bias, the rows' statistics or None)."""
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    x = _rows_of(x, x.shape[-1])
+    weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias))
+    stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device) if keep else None
+    _launch("layer_norm", _lib_handle().fl_norm_forward, x.device, _norm_op(x, weight, bias, eps, wide), y.data_ptr(),
+            _ptr(stats))
+    return y, x, weight, stats
+
+
+class _NormFunction(autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, wide):
+        y, x2, w2, stats = _norm_forward(x, weight, bias, eps, wide, True)
+        ctx.save_for_backward(x2, w2, stats)
+        ctx.eps, ctx.wide, ctx.shape, ctx.dtype = eps, wide, x.shape, torch.float32 if wide else x.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, stats = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dev, lib, grad = x.device, _lib_handle(), grad.contiguous()
+        make = torch.empty if x.shape[0] else torch.zeros  # the sums over no rows
+        dx = torch.empty(ctx.shape, dtype=x.dtype, device=dev) if need_x else None
+        dw = make(x.shape[1], dtype=ctx.dtype, device=dev) if need_w else None
+        db = make(x.shape[1], dtype=ctx.dtype, device=dev) if need_b else None
+        if x.numel():
+            op = _norm_op(x, weight, None, ctx.eps, ctx.wide)
+            nbytes = lib.fl_norm_backward_bytes(op, need_w or need_b)
+            ws = _workspace(nbytes, dev)
+            _launch("layer_norm", lib.fl_norm_backward, dev, op, grad.data_ptr(), stats.data_ptr(), _ptr(dx), _ptr(dw),
+                    _ptr(db), _ptr(ws), nbytes)
+        return dx, dw, db, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension.
+
+    x [..., n]; weight and bias [n] or None, both of x's type or both float32.
+    Mean and variance (of the n values, about their mean) and all sums are
+    float32, the result is rounded once.  Rows may be strided; x whose last
+    dimension is not contiguous is copied.  An infinity or NaN makes its row
+    NaN, and with it the gradients of weight and bias."""
+    _need_gpu("layer_norm", x, weight, bias)
+    if x.dtype not in _TYPES:
+        raise TypeError("layer_norm: x must be float32, bfloat16 or float16")
+    if x.dim() < 1:
+        raise ValueError("layer_norm: x must be [..., columns]")
+    wide = False
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            if t.dtype is not x.dtype and t.dtype is not torch.float32:
+                raise TypeError("layer_norm: %s must be of x's type or float32" % name)
+            if t.shape != x.shape[-1:]:
+                raise ValueError("layer_norm: %s must be [%d]" % (name, x.shape[-1]))
+            wide = x.dtype is not torch.float32 and t.dtype is torch.float32
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
+        raise TypeError("layer_norm: weight and bias must be of one type")
+    eps = float(eps)
+    if not 0.0 <= eps < math.inf:
+        raise ValueError("layer_norm: eps must be finite and not negative")
+    if _differentiated(x, weight, bias):
+        return _NormFunction.apply(x, weight, bias, eps, wide)
+    return _norm_forward(x, weight, bias, eps, wide, False)[0]
 
 
 # ---------------------------------------------------------------------------

@@ -939,6 +939,89 @@ int fl_logits_grad(void *stream, const fl_logits *op, const float *w,
                    const void *grad, void *dx, float *dbias, void *ws,
                    size_t ws_bytes);
 
+/* Layer normalisation: y = (x - mean) / sqrt(var + eps) * weight + bias over
+ * the columns of x [M, N] (row stride ldx, columns contiguous; y and the
+ * gradients contiguous).  weight and bias [N] of x's type, or fp32 if `wide`;
+ * either may be null. */
+typedef struct fl_norm {
+    const void *x;
+    int64_t M, N, ldx;
+    const void *weight, *bias;
+    float eps;
+    int32_t dtype, wide, reserved;
+} fl_norm;
+
+size_t fl_norm_op_bytes(void);
+/* stats [M][2], optional: a row's mean and 1 / sqrt(var + eps), for the
+ * backward. */
+int fl_norm_forward(void *stream, const fl_norm *op, void *y, float *stats);
+/* Those of the gradients that are not null: dx [M, N], dw and db [N] of the
+ * weight's type (M > 0; the sums over no rows are the caller's zeros). */
+size_t fl_norm_backward_bytes(const fl_norm *op, int with_dw);
+int fl_norm_backward(void *stream, const fl_norm *op, const void *gy,
+                     const float *stats, void *dx, void *dw, void *db,
+                     void *ws, size_t ws_bytes);
+
+/* What every row of logits is held to: k <= 4096 ids, those outside the
+ * vocabulary not listed, with a teacher's logits, or (teacher null, k = 1) a
+ * target.  With u = logits / temperature and q = softmax(teacher / temperature)
+ * over the listed ids whose u is not -inf,
+ *   loss = temperature^2 sum q (log q - u[id] + log sum exp u);
+ * a row in which nothing is listed or nothing is left has loss 0 and no
+ * gradient.  A target's loss is log sum exp u - u[id]. */
+typedef struct fl_lists {
+    int64_t rows, k;
+    const int64_t *ids;       /* [rows, k]                                 */
+    const float *teacher;     /* [rows, k] or null                         */
+    float temperature;        /* in [2^-100, 2^100]                        */
+    int32_t reserved;
+} fl_lists;
+
+/* Bytes of the state that a forward writes and its backward reads. */
+size_t fl_lists_state_bytes(const fl_lists *lists);
+
+/* Rows that are given. */
+typedef struct fl_scores {
+    fl_lists lists;
+    const void *logits;       /* [rows, cols], row stride ld               */
+    int64_t cols, ld;
+    int32_t dtype, reserved;
+} fl_scores;
+
+size_t fl_scores_op_bytes(void);
+size_t fl_scores_forward_bytes(const fl_scores *op);
+int fl_scores_forward(void *stream, const fl_scores *op, float *loss,
+                      void *state, void *ws, size_t ws_bytes);
+/* dx [rows, cols] of the logits' type; grad [rows] of the losses. */
+int fl_scores_backward(void *stream, const fl_scores *op, const float *grad,
+                       void *state, void *dx);
+
+/* Rows that are a product, x [M, K] weight [V, K]^T + bias [V], which is not
+ * kept: lists.rows = M. */
+typedef struct fl_vocab {
+    fl_lists lists;
+    int64_t M, V, K;
+    const void *x;            /* row stride ldx                            */
+    int64_t ldx;
+    const void *weight;       /* row stride ldw                            */
+    int64_t ldw;
+    const void *bias;         /* contiguous, or null                       */
+    int32_t dtype, bias_f32;
+} fl_vocab;
+
+size_t fl_vocab_op_bytes(void);
+size_t fl_vocab_forward_bytes(const fl_vocab *op);
+int fl_vocab_forward(void *stream, const fl_vocab *op, float *loss,
+                     void *state, void *ws, size_t ws_bytes);
+/* Those of the gradients that are not null: dx [M, K] and dw [V, K] of the
+ * operands' type, db [V] fp32 if bias_f32, else of the operands' type.  ws on
+ * a 16-byte boundary. */
+size_t fl_vocab_backward_bytes(const fl_vocab *op, int with_dx, int with_dw,
+                               int with_db);
+int fl_vocab_backward(void *stream, const fl_vocab *op, const float *grad,
+                      void *state, void *dx, void *dw, void *db, void *ws,
+                      size_t ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif
