@@ -317,10 +317,11 @@ _SIGS = {
     "fl_scores_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlScores)] + [ctypes.c_void_p] * 3),
     "fl_vocab_op_bytes": (ctypes.c_size_t, []),
     "fl_vocab_forward_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlVocab)]),
-    "fl_vocab_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlVocab)] + [ctypes.c_void_p] * 3 +
+    "fl_vocab_layout_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlVocab)]),
+    "fl_vocab_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlVocab)] + [ctypes.c_void_p] * 4 +
                          [ctypes.c_size_t]),
     "fl_vocab_backward_bytes": (ctypes.c_size_t, [ctypes.POINTER(FlVocab)] + [ctypes.c_int] * 3),
-    "fl_vocab_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlVocab)] + [ctypes.c_void_p] * 6 +
+    "fl_vocab_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(FlVocab)] + [ctypes.c_void_p] * 7 +
                           [ctypes.c_size_t]),
     "fl_prof_enable": (ctypes.c_int, [ctypes.c_int]),
     "fl_prof_read": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),

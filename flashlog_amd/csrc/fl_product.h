@@ -401,8 +401,17 @@ struct WideContig {
     }
 };
 
+// fp32 values as two fp16 planes, v s = v0 + v1 with a power of two s that brings
+// the largest to 2^13..2^14: v1 is the rest rounded, so that what is lost is below
+// 2^-22 of v or 2^-39 of the largest.  A row holds 32 values of the one plane, the
+// same 32 of the other, and so on: 64 values of a row are a step of 32 k, and the
+// three products v0 w0 + v0 w1 + v1 w0 are off by 2^-22 once more.
+__device__ __forceinline__ int64_t pair_at(int64_t c) { return c / 32 * 64 + c % 32; }
+
 // k-strided: the rows of k one after the other, or in an order if GATHER.
-template <int BR, int BK, bool GATHER>
+// PAIRS: of values held as two planes (pair_at), BK / 2 rows of the one
+// plane and then the same rows of the other.
+template <int BR, int BK, bool GATHER, bool PAIRS = false>
 struct WideStrided {
     static constexpr int CH = BR / 8;                // chunks a row of k
     static constexpr int RPL = FL_WAVE / CH;         // rows of k a load
@@ -416,15 +425,16 @@ struct WideStrided {
     // transposed read takes of each of 4 rows.
     static __device__ __forceinline__ int turn(int k) { return 2 * ((k & 3) | ((((k >> 3) ^ (k >> 4)) & 1) << 2)); }
     static __device__ __forceinline__ int row(int i) { return (fl_wave_id() * LOADS + i) * RPL + fl_lane() / CH; }
+    static __device__ __forceinline__ int row_of_k(int i) { return PAIRS ? row(i) % (BK / 2) : row(i); }
 
     __device__ __forceinline__ void init(const uint16_t *b, int64_t stride, int64_t R) {
         base = b;
         ld = stride;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int64_t c = ((fl_lane() % CH) ^ turn(row(i))) * 8;
-            at[i] = (uint32_t)((c <= R - 8 ? c : R - 8) * 2);
-            if constexpr (!GATHER) at[i] += (uint32_t)(row(i) * stride * 2);
+            const int64_t c0 = ((fl_lane() % CH) ^ turn(row(i))) * 8, c = c0 <= R - 8 ? c0 : R - 8;
+            at[i] = (uint32_t)((PAIRS ? pair_at(c) + row(i) / (BK / 2) * 32 : c) * 2);
+            if constexpr (!GATHER) at[i] += (uint32_t)(row_of_k(i) * stride * 2);
         }
     }
     // The next `count` rows of k, BK if WHOLE; r: this lane's, if GATHER.
@@ -434,7 +444,7 @@ struct WideStrided {
         for (int i = 0; i < LOADS; ++i) {
             const char *q = (const char *)base + at[i];
             if constexpr (GATHER) q += (int64_t)r[i] * ld * 2;
-            if (!WHOLE && row(i) >= count) q = (const char *)wd_zeros;
+            if (!WHOLE && row_of_k(i) >= count) q = (const char *)wd_zeros;
             load_lds(q, lds + (fl_wave_id() * LOADS + i) * 512);
         }
         if constexpr (!GATHER) base += count * ld;
@@ -592,6 +602,94 @@ struct WideProduct {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+};
+
+// Tiles one after the other as one sequence of steps, `steps` a tile: the loads
+// run ahead over the tiles' ends, and a half of the waves takes a tile's sums
+// out (out(tile)) while the other half still multiplies.  Tiles of BM rows and
+// WN x 64 columns, a step of 64 values (PAIRS: 32 of both planes).  The halves
+// take turns as in WideProduct.
+//
+// feed(lds_a, lds_b) issues the loads of the next step.
+template <typename T, bool PAIRS, int BM, int WN, int STAGES, typename TA, typename TB>
+struct WideTiles {
+    static constexpr int WM = WD_WAVES / WN, MT = BM / WM / 16, NTL = 4, BN = WN * 64;
+    static constexpr int ELEMS = TA::ELEMS + TB::ELEMS, LOADS = TA::LOADS + TB::LOADS;
+    using Waits = WideProduct<T, BM, 64, STAGES, TA, TB>;
+    f32x4 acc[MT][NTL];
+
+    static __device__ __forceinline__ int wave_m() { return (fl_wave_id() / WN) * (BM / WM); }
+    static __device__ __forceinline__ int wave_n() { return (fl_wave_id() % WN) * 64; }
+
+    template <bool FIRST>
+    __device__ __forceinline__ void multiply(const u32x4 (&fa)[2][MT], const u32x4 (&fb)[2][NTL]) {
+#pragma unroll
+        for (int p = 0; p < (PAIRS ? 3 : 2); ++p)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NTL; ++j) {
+                    const int ka = PAIRS ? p == 1 : p, kb = PAIRS ? p == 0 : p;
+                    const f32x4 c = FIRST && p == 0 ? f32x4{0, 0, 0, 0} : acc[i][j];
+                    acc[i][j] = mfma<T>(fb[kb][j], fa[ka][i], c);
+                }
+    }
+
+    template <typename F, typename O>
+    __device__ __forceinline__ void run(const TA &ta, const TB &tb, int64_t tiles, int steps, uint16_t *lds, F &&feed,
+                                        O &&out) {
+        const int64_t all = tiles * steps;
+        if (all <= 0) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NTL; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+            for (int64_t t = 0; t < tiles; ++t) out(t);
+            return;
+        }
+        const bool second = fl_wave_id() >= WD_WAVES / 2;
+        const auto load = [&](int64_t step) {
+            uint16_t *to = lds + (int)(step % STAGES) * ELEMS;
+            feed(to, to + TA::ELEMS);
+        };
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s)
+            if (s < all) load(s);
+        if (all < STAGES) Waits::template wait<0>();
+        else Waits::template wait<LOADS *(STAGES - 1)>();
+        Waits::meet();
+        if (second) Waits::meet();
+        int at = 0;
+        int64_t tile = 0;
+        for (int64_t s = 0; s < all; ++s) {
+            const uint16_t *la = lds + (int)(s % STAGES) * ELEMS, *lb = la + TA::ELEMS;
+            const bool full = s + STAGES - 1 < all;
+            if (!second && s > 0 && full) load(s + STAGES - 1);
+            if (second) {
+                if (full) Waits::template wait<LOADS *(STAGES - 2)>();
+                else Waits::template wait<0>();
+            }
+            if (at == 0 && s > 0) out(tile++);
+            u32x4 fa[2][MT], fb[2][NTL];
+            tb.read(lb, wave_n(), fb);
+            ta.read(la, wave_m(), fa);
+            Waits::wait_lds();
+            Waits::meet();
+            if (second && s + STAGES < all) load(s + STAGES);
+            __builtin_amdgcn_s_setprio(1);
+            if (at == 0) multiply<true>(fa, fb);
+            else multiply<false>(fa, fb);
+            __builtin_amdgcn_s_setprio(0);
+            if (!second) {
+                if (full) Waits::template wait<LOADS *(STAGES - 2)>();
+                else Waits::template wait<0>();
+            }
+            Waits::meet();
+            if (++at == steps) at = 0;
+        }
+        if (!second) Waits::meet();
+        out(tile);
     }
 };
 

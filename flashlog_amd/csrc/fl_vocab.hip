@@ -1,0 +1,1131 @@
+// The losses of rows that are a product z = x W^T + b, which is not kept: the
+// forward joins the tiles' maxima and sums of exponentials, and the backward
+// makes the tiles again with dz in place of z, for a piece of the vocabulary at
+// a time (fl_loss.hip has the formulas):
+//
+//   dx = dz W      dW = dz^T x      db = sum over the rows of dz
+//
+// The piece of dz is what a call holds of [rows x vocabulary], in the
+// operands' type (an operand of two products), small enough for the last level
+// cache.  The listed columns' own u comes from a dot product each; their
+// entries of dz are made apart, since p - q of values rounded before would
+// keep few bits where p is near 1.
+//
+// Bound by the matrix instructions: four products where logits that are kept
+// would need three.  Small products go by k_vocab_*, the others by k_wide_*:
+// tiles one after the other, so that the loads of a tile begin while the one
+// before it is finished, and exponentials of one half of the waves run beside
+// the products of the other.  There fp32 operands are held as two fp16 planes
+// (half the products of three bfloat16 planes), and 16-bit rows that do not lie
+// on 16 bytes as copies that do.
+#include "fl_abi.h"
+#include "fl_common.h"
+#include "fl_loss.h"
+#include "fl_product.h"
+#include <type_traits>
+
+namespace fl {
+namespace {
+
+constexpr int LS_NT = 256;
+constexpr int LS_WAVES = LS_NT / FL_WAVE;
+constexpr size_t LS_PIECE = 128u << 20;  // bytes of dz
+
+struct VocabArgs {
+    fl_vocab op;
+    float scale;          // log2(e) / tau
+    // the vocabulary's piece [v0, v0 + width)
+    int64_t v0, width;
+    uint32_t m_tiles, n_tiles, parts;
+    Running *part;        // [M][parts]
+    const float2 *rows;
+    float2 *listed;
+    const float *coef;    // tau g of every row (times a power of two), 0 where it has no gradient
+    void *d;              // dz of the piece: [M][ldd], columns behind the piece 0
+    int64_t ldd;
+    float *sums;          // dx: [parts][M][K]; dW: [parts][width][K]
+    void *dw;
+    const float *unscale;  // what undoes dz's power of two
+    int add;
+    // wide kernels: operands laid out (or as they are), columns, and what undoes the planes' powers of two (or null)
+    const uint16_t *x, *w;
+    int64_t ldx, ldw, cols, d_cols;
+    const float *undo;     // x's, weight's
+};
+
+// u of the listed columns: a wave a row and four of them.
+constexpr int DOT_IDS = 4;
+
+template <typename T>
+__global__ __launch_bounds__(LS_NT) void k_vocab_dots(VocabArgs a) {
+    const int64_t k = a.op.lists.k, quads = (k + DOT_IDS - 1) / DOT_IDS;
+    const int64_t item = fl_block() * LS_WAVES + fl_wave_id();
+    if (item >= a.op.M * quads) return;
+    const int64_t row = item / quads, j0 = item % quads * DOT_IDS, K = a.op.K;
+    const T *x = (const T *)a.op.x + row * a.op.ldx;
+    const T *w[DOT_IDS];
+    int64_t id[DOT_IDS];
+    float s[DOT_IDS] = {};
+#pragma unroll
+    for (int i = 0; i < DOT_IDS; ++i) {
+        id[i] = j0 + i < k ? a.op.lists.ids[row * k + j0 + i] : -1;
+        if (id[i] >= a.op.V) id[i] = -1;
+        w[i] = (const T *)a.op.weight + (id[i] < 0 ? 0 : id[i]) * a.op.ldw;
+    }
+    int64_t c = fl_lane() * 8;
+    for (; c + 8 <= K; c += FL_WAVE * 8) {
+        const Vec<T, 8> xv = load_vec<T, 8>(x + c);
+        Vec<T, 8> wv[DOT_IDS];
+#pragma unroll
+        for (int i = 0; i < DOT_IDS; ++i) wv[i] = load_vec<T, 8>(w[i] + c);
+#pragma unroll
+        for (int i = 0; i < DOT_IDS; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[i] = __builtin_fmaf((float)xv.v[e], (float)wv[i].v[e], s[i]);
+    }
+    for (int64_t e = c; e < K && e < c + 8; ++e)
+#pragma unroll
+        for (int i = 0; i < DOT_IDS; ++i) s[i] = __builtin_fmaf((float)x[e], (float)w[i][e], s[i]);
+#pragma unroll
+    for (int i = 0; i < DOT_IDS; ++i) {
+        s[i] = fl_wave_sum_f32(s[i]);
+        if (fl_lane() == 0 && j0 + i < k) {
+            float b = 0.0f;
+            if (a.op.bias && id[i] >= 0)
+                b = a.op.bias_f32 ? ((const float *)a.op.bias)[id[i]] : (float)((const T *)a.op.bias)[id[i]];
+            a.listed[row * k + j0 + i] = float2{(s[i] + b) * a.scale, 0.0f};
+        }
+    }
+}
+
+// The logits of a lane's tiles in units of log 2, -inf behind the vocabulary:
+// f(i, j, u[4]) of the row i * 16 + (lane & 15) and four columns from
+// col + j * 16 + (lane >> 4) * 4 on, both within the wave's part of the tile.
+template <typename T, int MT, int NTL, typename F>
+__device__ __forceinline__ void each_u(const VocabArgs &a, const f32x4 (&acc)[MT][NTL], int64_t col, int64_t end,
+                                       F &&f) {
+#pragma unroll
+    for (int j = 0; j < NTL; ++j) {
+        const int64_t n = col + j * 16 + (fl_lane() >> 4) * 4;
+        const int have = end - n < 0 ? 0 : end - n < 4 ? (int)(end - n) : 4;
+        float b[4] = {0, 0, 0, 0};
+        if (a.op.bias) {
+            if (a.op.bias_f32) load_some<float>((const float *)a.op.bias + n, have, b);
+            else load_some<T>((const T *)a.op.bias + n, have, b);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            float u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = e < have ? (acc[i][j][e] + b[e]) * a.scale : -INFINITY;
+            f(i, j, u);
+        }
+    }
+}
+
+// Joins the lanes' sums of a wave's rows and the waves' of a tile's columns,
+// and stores them as one part of the rows.
+template <int BM, int WAVES_N, int MT>
+__device__ __forceinline__ void store_running(const VocabArgs &a, Running (&r)[MT], Running *lds, int wave_row,
+                                              int wave_col, int64_t row0, uint32_t part) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        r[i] = joined(r[i], Running{__shfl_xor(r[i].m, 16), __shfl_xor(r[i].s, 16)});
+        r[i] = joined(r[i], Running{__shfl_xor(r[i].m, 32), __shfl_xor(r[i].s, 32)});
+        if (fl_lane() < 16) lds[wave_col * BM + wave_row + i * 16 + fl_lane()] = r[i];
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < BM; t += blockDim.x) {
+        Running s = lds[t];
+#pragma unroll
+        for (int w = 1; w < WAVES_N; ++w) s = joined(s, lds[w * BM + t]);
+        if (row0 + t < a.op.M) a.part[(row0 + t) * a.parts + part] = s;
+    }
+}
+
+template <typename T, int BM, int BN, int BK>
+__global__ __launch_bounds__(LN_NT) void k_vocab_stats(VocabArgs a) {
+    using Prod = Product<T, BM, BN, BK>;
+    __shared__ __align__(16) uint16_t lds[Prod::LDS_ELEMS];
+    __shared__ Running join[Prod::WAVES_N * BM];
+    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    const uint32_t mt = w % a.m_tiles, part = w / a.m_tiles;
+    const int64_t row0 = (int64_t)mt * BM, V = a.op.V;
+    const int64_t t0 = (int64_t)a.n_tiles * part / a.parts, t1 = (int64_t)a.n_tiles * (part + 1) / a.parts;
+    Running r[Prod::MT];
+#pragma unroll
+    for (int i = 0; i < Prod::MT; ++i) r[i] = Running{-INFINITY, 0.0f};
+    Prod prod;
+    for (int64_t t = t0; t < t1; ++t) {
+        const int64_t n0 = t * BN;
+        ContigTile<T, BM, BK> ta;
+        ContigTile<T, BN, BK> tb;
+        ta.init([&](int i) { return (const T *)a.op.x + (row0 + i < a.op.M ? row0 + i : a.op.M - 1) * a.op.ldx; });
+        tb.init([&](int i) { return (const T *)a.op.weight + (n0 + i < V ? n0 + i : V - 1) * a.op.ldw; });
+        prod.run(ta, tb, a.op.K, lds);
+        __syncthreads();
+        float u[Prod::MT][Prod::NTL * 4];
+        each_u<T>(a, prod.acc, n0 + prod.wave_n(), V, [&](int i, int j, const float (&v)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[i][j * 4 + e] = v[e];
+        });
+#pragma unroll
+        for (int i = 0; i < Prod::MT; ++i) {
+            float m = r[i].m, s = 0.0f;
+#pragma unroll
+            for (int e = 0; e < Prod::NTL * 4; ++e) m = fmaxf(m, u[i][e]);
+            const float at = base_of(m);
+#pragma unroll
+            for (int e = 0; e < Prod::NTL * 4; ++e) s += exp2_of(u[i][e] - at);
+            r[i] = Running{m, r[i].s * exp2_of(r[i].m - at) + s};
+        }
+    }
+    store_running<BM, Prod::WAVES_N>(a, r, join, prod.wave_m(), prod.wave_n() / (BN / Prod::WAVES_N), row0, part);
+}
+
+// What a row's gradients are multiplied by.  SCALED (half): times the power of
+// two that brings the largest to 2^14, so that small ones stay normal numbers.
+template <bool SCALED>
+__global__ __launch_bounds__(1024) void k_vocab_coef(const float2 *__restrict__ rows, const float *__restrict__ g,
+                                                     float tau, int64_t M, float *__restrict__ coef,
+                                                     float *__restrict__ unscale) {
+    __shared__ float most[16];
+    float scale = 1.0f;
+    if constexpr (SCALED) {
+        float m = 0.0f;
+        for (int64_t i = threadIdx.x; i < M; i += 1024) {
+            const float c = rows[i].y != 0.0f ? fabsf(tau * g[i]) : 0.0f;
+            m = fmaxf(m, c < INFINITY ? c : 0.0f);
+        }
+#pragma unroll
+        for (int o = FL_WAVE / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if (fl_lane() == 0) most[threadIdx.x / FL_WAVE] = m;
+        __syncthreads();
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, most[i]);
+        int e;
+        frexpf(m, &e);  // m < 2^e
+        e = e < -100 ? -100 : e;
+        scale = m > 0.0f ? ldexpf(1.0f, 14 - e) : 1.0f;
+        if (threadIdx.x == 0) *unscale = m > 0.0f ? ldexpf(1.0f, e - 14) : 1.0f;
+    } else if (fl_block() == 0 && threadIdx.x == 0) *unscale = 1.0f;
+    const int64_t step = SCALED ? 1024 : (int64_t)gridDim.x * 1024;
+    for (int64_t i = (SCALED ? 0 : (int64_t)blockIdx.x * 1024) + threadIdx.x; i < M; i += step)
+        coef[i] = rows[i].y != 0.0f ? tau * g[i] * scale : 0.0f;
+}
+
+// dz of a piece but for the listed columns.
+template <typename T, int BM, int BN, int BK>
+__global__ __launch_bounds__(LN_NT) void k_vocab_grad(VocabArgs a) {
+    using Prod = Product<T, BM, BN, BK>;
+    __shared__ __align__(16) uint16_t lds[Prod::LDS_ELEMS];
+    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    const int64_t row0 = (int64_t)(w % a.m_tiles) * BM, n0 = a.v0 + (int64_t)(w / a.m_tiles) * BN, V = a.op.V;
+    ContigTile<T, BM, BK> ta;
+    ContigTile<T, BN, BK> tb;
+    ta.init([&](int i) { return (const T *)a.op.x + (row0 + i < a.op.M ? row0 + i : a.op.M - 1) * a.op.ldx; });
+    tb.init([&](int i) { return (const T *)a.op.weight + (n0 + i < V ? n0 + i : V - 1) * a.op.ldw; });
+    Prod prod;
+    prod.run(ta, tb, a.op.K, lds);
+    const int64_t row = row0 + prod.wave_m() + (fl_lane() & 15), col = n0 + prod.wave_n();
+    float lse[Prod::MT], c[Prod::MT];
+#pragma unroll
+    for (int i = 0; i < Prod::MT; ++i) {
+        const int64_t m = row + i * 16 < a.op.M ? row + i * 16 : a.op.M - 1;
+        lse[i] = a.rows[m].x;
+        c[i] = a.coef[m];
+    }
+    each_u<T>(a, prod.acc, col, a.v0 + a.width, [&](int i, int j, const float (&u)[4]) {
+        const int64_t n = col + j * 16 + (fl_lane() >> 4) * 4 - a.v0;
+        if (row + i * 16 >= a.op.M || n >= a.ldd) return;
+        Vec<T, 4> o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o.v[e] = (T)(c[i] == 0.0f ? 0.0f : c[i] * exp2_of(u[e] - lse[i]));
+        store_vec<T, 4>((T *)a.d + (row + i * 16) * a.ldd + n, o);
+    });
+}
+
+// dz of the listed columns in the piece.
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
+    const int64_t i = fl_block() * LS_NT + threadIdx.x, k = a.op.lists.k;
+    if (i >= a.op.M * k) return;
+    const int64_t row = i / k, v = a.op.lists.ids[i] - a.v0;
+    const float c = a.coef[row];
+    if (v < 0 || v >= a.width || c == 0.0f) return;
+    const float2 l = a.listed[i];
+    const float d = c * (exp2_of(l.x - a.rows[row].x) - l.y);
+    if constexpr (WIDE && sizeof(T) == 4) {
+        _Float16 *to = (_Float16 *)a.d + row * a.ldd + pair_at(v);
+        to[0] = (_Float16)d;
+        to[32] = (_Float16)(d - (float)to[0]);
+    } else ((T *)a.d)[row * a.ldd + v] = (T)d;
+}
+
+// A piece's part of dx, added to what is there if `add`.
+template <typename T, int BM, int BN, int BK>
+__global__ __launch_bounds__(LN_NT) void k_vocab_dx(VocabArgs a) {
+    using Prod = Product<T, BM, BN, BK>;
+    __shared__ __align__(16) uint16_t lds[Prod::LDS_ELEMS];
+    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    const uint32_t tile = w / a.parts, part = w % a.parts;
+    const int64_t row0 = (int64_t)(tile / a.n_tiles) * BM, n0 = (int64_t)(tile % a.n_tiles) * BN, M = a.op.M;
+    const int64_t steps = (a.width + BK - 1) / BK, k0 = steps * part / a.parts * BK;
+    const int64_t k1 = part + 1 == a.parts ? a.width : steps * (part + 1) / a.parts * BK;
+    ContigTile<T, BM, BK> ta;
+    StridedTile<T, BN, BK> tb;
+    ta.init([&](int r) { return (const T *)a.d + (row0 + r < M ? row0 + r : M - 1) * a.ldd + k0; });
+    tb.init((const T *)a.op.weight + (a.v0 + k0) * a.op.ldw + n0, a.op.ldw, a.op.K - n0, nullptr);
+    Prod prod;
+    prod.run(ta, tb, k1 - k0, lds);
+#pragma unroll
+    for (int i = 0; i < Prod::MT; ++i) {
+        const int64_t row = row0 + prod.wave_m() + i * 16 + (fl_lane() & 15);
+        if (row >= M) continue;
+#pragma unroll
+        for (int j = 0; j < Prod::NTL; ++j) {
+            const int64_t n = n0 + prod.wave_n() + j * 16 + (fl_lane() >> 4) * 4;
+            if (n >= a.op.K) continue;
+            const int have = a.op.K - n < 4 ? (int)(a.op.K - n) : 4;
+            float *q = a.sums + ((int64_t)part * M + row) * a.op.K + n;
+            Vec<float, 4> f{{prod.acc[i][j][0], prod.acc[i][j][1], prod.acc[i][j][2], prod.acc[i][j][3]}};
+            if (a.add) {
+                float old[4];
+                load_some<float>(q, have, old);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f.v[e] += old[e];
+            }
+            if (have == 4) store_vec<float, 4>(q, f);
+            else store_some<float, 4>(q, f, have);
+        }
+    }
+}
+
+// The parts of a sum added in order and rounded: four values a thread.
+template <typename T>
+__global__ __launch_bounds__(LS_NT) void k_vocab_fold(const float *__restrict__ part, uint32_t parts, int64_t n,
+                                                      const float *__restrict__ unscale,
+                                                      const float *__restrict__ undo, T *__restrict__ out) {
+    const int64_t i = (fl_block() * LS_NT + threadIdx.x) * 4;
+    if (i >= n) return;
+    const int have = n - i < 4 ? (int)(n - i) : 4;
+    const float f = *unscale, f2 = undo ? *undo : 1.0f;
+    float s[4] = {0, 0, 0, 0}, v[4];
+    for (uint32_t p = 0; p < parts; ++p) {
+        load_some<float>(part + p * n + i, have, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+    }
+    Vec<T, 4> o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o.v[e] = (T)(s[e] * f * f2);
+    if (have == 4) store_vec<T, 4>(out + i, o);
+    else store_some<T, 4>(out + i, o, have);
+}
+
+// A piece's rows of dW, or of a part of the rows' sum.
+template <typename T, int BM, int BN, int BK>
+__global__ __launch_bounds__(LN_NT) void k_vocab_dw(VocabArgs a) {
+    using Prod = Product<T, BM, BN, BK>;
+    __shared__ __align__(16) uint16_t lds[Prod::LDS_ELEMS];
+    uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    const int64_t m0 = (int64_t)(w % a.m_tiles) * BM;
+    w /= a.m_tiles;
+    const int64_t c0 = (int64_t)(w % a.n_tiles) * BN;
+    const uint32_t part = w / a.n_tiles;
+    const int64_t begin = a.op.M * part / a.parts, end = a.op.M * (part + 1) / a.parts;
+    StridedTile<T, BM, BK> ta;
+    StridedTile<T, BN, BK> tb;
+    ta.init((const T *)a.d + begin * a.ldd + m0, a.ldd, a.ldd - m0, nullptr);
+    tb.init((const T *)a.op.x + begin * a.op.ldx + c0, a.op.ldx, a.op.K - c0, nullptr);
+    Prod prod;
+    prod.run(ta, tb, end - begin, lds);
+    const float f = a.sums ? 1.0f : *a.unscale;
+#pragma unroll
+    for (int i = 0; i < Prod::MT; ++i) {
+        const int64_t m = m0 + prod.wave_m() + i * 16 + (fl_lane() & 15);
+        if (m >= a.width) continue;
+#pragma unroll
+        for (int j = 0; j < Prod::NTL; ++j) {
+            const int64_t c = c0 + prod.wave_n() + j * 16 + (fl_lane() >> 4) * 4;
+            if (c >= a.op.K) continue;
+            const int n = a.op.K - c < 4 ? (int)(a.op.K - c) : 4;
+            if (a.sums) {
+                float *q = a.sums + ((int64_t)part * a.width + m) * a.op.K + c;
+                const Vec<float, 4> o{{prod.acc[i][j][0], prod.acc[i][j][1], prod.acc[i][j][2], prod.acc[i][j][3]}};
+                if (n == 4) store_vec<float, 4>(q, o);
+                else store_some<float, 4>(q, o, n);
+            } else {
+                T *q = (T *)a.dw + (a.v0 + m) * a.op.K + c;
+                Vec<T, 4> o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o.v[e] = (T)(prod.acc[i][j][e] * f);
+                if (n == 4) store_vec<T, 4>(q, o);
+                else store_some<T, 4>(q, o, n);
+            }
+        }
+    }
+}
+
+// Column sums of a part of the rows of dz, a thread a column.
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
+    const int64_t blocks = (a.width + LS_NT - 1) / LS_NT, item = fl_block(), part = item / blocks;
+    const int64_t c = item % blocks * LS_NT + threadIdx.x;
+    if (part >= a.parts || c >= a.width) return;
+    float s = 0.0f;
+    for (int64_t m = a.op.M * part / a.parts; m < a.op.M * (part + 1) / a.parts; ++m) {
+        if constexpr (WIDE && sizeof(T) == 4) {
+            const _Float16 *d = (const _Float16 *)a.d + m * a.ldd + pair_at(c);
+            s += (float)d[0] + (float)d[32];
+        } else s += (float)((const T *)a.d)[m * a.ldd + c];
+    }
+    a.sums[part * a.width + c] = s;
+}
+
+// ---------------------------------------------------------------------------
+// The same for large products
+
+// The largest finite magnitude of x and of weight, a part of them a workgroup.
+constexpr int LAY_PARTS = 512;
+
+__global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restrict__ most) {
+    __shared__ float waves[LS_WAVES];
+    const bool second = blockIdx.y;
+    const int64_t R = second ? a.op.V : a.op.M, ld = second ? a.op.ldw : a.op.ldx, quads = (a.op.K + 3) / 4;
+    const float *p = (const float *)(second ? a.op.weight : a.op.x);
+    float m = 0.0f;
+    for (int64_t i = (int64_t)blockIdx.x * LS_NT + threadIdx.x; i < R * quads; i += (int64_t)LAY_PARTS * LS_NT) {
+        const int64_t c = i % quads * 4;
+        float v[4];
+        load_some<float>(p + i / quads * ld + c, a.op.K - c < 4 ? (int)(a.op.K - c) : 4, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
+    }
+#pragma unroll
+    for (int o = FL_WAVE / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (fl_lane() == 0) waves[fl_wave_id()] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) most[blockIdx.y * LAY_PARTS + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+}
+
+// x and weight as rows of 16-bit values on 16 bytes: fp32 as two planes (pair_at), others copied; zeros behind a row.
+template <typename T>
+__global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restrict__ most, uint16_t *__restrict__ x,
+                                               uint16_t *__restrict__ w, float *__restrict__ undo) {
+    constexpr bool PAIRS = sizeof(T) == 4;
+    const bool second = blockIdx.y;
+    const int64_t R = second ? a.op.V : a.op.M, ld = second ? a.op.ldw : a.op.ldx, chunks = a.cols / 8, K = a.op.K;
+    const T *p = (const T *)(second ? a.op.weight : a.op.x);
+    uint16_t *out = second ? w : x;
+    float scale = 1.0f;
+    if constexpr (PAIRS) {
+        __shared__ float waves[LS_WAVES];
+        float m = 0.0f;
+        for (int i = threadIdx.x; i < LAY_PARTS; i += LS_NT) m = fmaxf(m, most[blockIdx.y * LAY_PARTS + i]);
+#pragma unroll
+        for (int o = FL_WAVE / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if (fl_lane() == 0) waves[fl_wave_id()] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+        int e;
+        frexpf(m, &e);  // m < 2^e
+        e = e < -100 ? -100 : e;
+        scale = ldexpf(1.0f, 14 - e);
+        if (blockIdx.x == 0 && threadIdx.x == 0) undo[blockIdx.y] = ldexpf(1.0f, e - 14);
+    }
+    for (int64_t i = (int64_t)blockIdx.x * LS_NT + threadIdx.x; i < R * chunks; i += (int64_t)gridDim.x * LS_NT) {
+        const int64_t r = i / chunks, c = i % chunks * 8;
+        Vec<T, 8> v;
+        if (c + 8 <= K) v = load_vec<T, 8>(p + r * ld + c);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v.v[e] = c + e < K ? p[r * ld + c + e] : (T)0.0f;
+        if constexpr (PAIRS) {
+            Vec<_Float16, 8> hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float s = v.v[e] * scale;
+                hi.v[e] = (_Float16)s;
+                lo.v[e] = (_Float16)(s - (float)hi.v[e]);
+            }
+            _Float16 *q = (_Float16 *)out + r * 2 * a.cols + pair_at(c);
+            store_vec<_Float16, 8>(q, hi);
+            store_vec<_Float16, 8>(q + 32, lo);
+        } else store_vec<T, 8>((T *)out + r * a.cols + c, v);
+    }
+}
+
+// The operands' 16-bit type.
+template <typename T>
+using Half = std::conditional_t<sizeof(T) == 4, _Float16, T>;
+template <typename T>
+constexpr bool is_pairs() {
+    return sizeof(T) == 4;
+}
+
+// Logit tiles: row tiles of x against row tiles of weight from n0 on, whose
+// order in LDS gives a lane 16 columns in a row (16 (lane / 16) .. of the
+// wave's 64).
+template <typename T, int BM, int WN, int STAGES>
+struct LogitTiles {
+    using TA = WideContig<BM, 64>;
+    using TB = WideContig<WN * 64, 64>;
+    using Run = WideTiles<Half<T>, is_pairs<T>(), BM, WN, STAGES, TA, TB>;
+    TA ta;
+    TB tb;
+    int steps, last, at;  // of a tile's row; values of the last step; the next step's
+    int64_t row_len, n_next;
+
+    static __device__ __forceinline__ int column(int r) {
+        return (r & ~63) + ((r >> 2) & 3) * 16 + ((r >> 4) & 3) * 4 + (r & 3);
+    }
+    __device__ __forceinline__ void aim(const VocabArgs &a) {
+        tb.init([&](int r) {
+            const int64_t n = n_next + column(r);
+            return a.w + (n < a.op.V ? n : a.op.V - 1) * a.ldw;
+        });
+    }
+    __device__ __forceinline__ void init(const VocabArgs &a, int64_t row0, int64_t n0) {
+        row_len = is_pairs<T>() ? 2 * a.cols : a.cols;
+        steps = (int)((row_len + 63) / 64);
+        last = (int)(row_len - (int64_t)(steps - 1) * 64);
+        at = 0;
+        n_next = n0;
+        ta.init([&](int r) { return a.x + (row0 + r < a.op.M ? row0 + r : a.op.M - 1) * a.ldx; });
+        aim(a);
+    }
+    __device__ __forceinline__ void feed(const VocabArgs &a, uint16_t *la, uint16_t *lb) {
+        if (at + 1 < steps || last == 64) {
+            ta.template issue<true>(la, 64);
+            tb.template issue<true>(lb, 64);
+        } else {
+            ta.template issue<false>(la, last);
+            tb.template issue<false>(lb, last);
+        }
+        if (++at < steps) return;
+        at = 0;
+#pragma unroll
+        for (int i = 0; i < TA::LOADS; ++i) ta.p[i] -= row_len;
+        n_next += WN * 64;
+        aim(a);
+    }
+};
+
+// A workgroup's row tile and part: eight row tiles and four parts are near each
+// other, so that an XCD's workgroups share both operands.
+__device__ __forceinline__ void row_and_part(const VocabArgs &a, uint32_t *mt, uint32_t *part) {
+    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    const uint32_t g = w / (8 * a.parts), n = a.m_tiles - 8 * g < 8 ? a.m_tiles - 8 * g : 8, l = w - g * 8 * a.parts;
+    *mt = 8 * g + l % n;
+    *part = l / n;
+}
+
+// A lane's bias for its 16 columns from n on, in units of log 2.
+template <typename T>
+__device__ __forceinline__ void lane_bias(const VocabArgs &a, int64_t n, float (&b)[16]) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+        const int64_t left = a.op.V - n - h * 4;
+        const int have = left < 0 ? 0 : left < 4 ? (int)left : 4;
+        float v[4];
+        if (a.op.bias_f32) load_some<float>((const float *)a.op.bias + n + h * 4, have, v);
+        else load_some<T>((const T *)a.op.bias + n + h * 4, have, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[h * 4 + e] = v[e] * a.scale;
+    }
+}
+
+template <typename T, int BM, int WN, int STAGES>
+__global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
+    using Tiles = LogitTiles<T, BM, WN, STAGES>;
+    using Run = typename Tiles::Run;
+    constexpr int MT = Run::MT;
+    extern __shared__ __align__(16) uint16_t wide_lds[];
+    uint32_t mt, part;
+    row_and_part(a, &mt, &part);
+    const int64_t row0 = (int64_t)mt * BM, V = a.op.V;
+    const int64_t t0 = (int64_t)a.n_tiles * part / a.parts, t1 = (int64_t)a.n_tiles * (part + 1) / a.parts;
+    // a lane's sums over its own columns, a pair a row
+    Running *state = reinterpret_cast<Running *>(wide_lds + STAGES * Run::ELEMS) + fl_wave_id() * MT * FL_WAVE + fl_lane();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) state[i * FL_WAVE] = Running{-INFINITY, 0.0f};
+    Tiles tiles;
+    tiles.init(a, row0, t0 * WN * 64);
+    const float scale = a.undo ? a.undo[0] * a.undo[1] * a.scale : a.scale;
+    Run run;
+    run.run(
+        tiles.ta, tiles.tb, t1 - t0, tiles.steps, wide_lds, [&](uint16_t *la, uint16_t *lb) { tiles.feed(a, la, lb); },
+        [&](int64_t t) {
+            const int64_t n = (t0 + t) * WN * 64 + run.wave_n() + (fl_lane() >> 4) * 16;
+            const int have = V - n < 16 ? (int)(V - n) : 16;
+            float b[16];
+            if (a.op.bias) lane_bias<T>(a, n, b);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                Running r = state[i * FL_WAVE];
+                float u[16], s = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    u[e] = run.acc[i][e / 4][e % 4] * scale;
+                    if (a.op.bias) u[e] += b[e];
+                }
+                if (__any(have < 16))
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) u[e] = e < have ? u[e] : -INFINITY;
+                // what the lane had first serves as the maximum, until a sum overflows or is not a number
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s += exp2_of(u[e] - r.m);
+                s += r.s;
+                if (__any(r.m == -INFINITY || !(s < INFINITY))) {
+                    float m = r.m;
+                    s = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) m = fmaxf(m, u[e]);
+                    const float at = base_of(m);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s += exp2_of(u[e] - at);
+                    s += r.s * exp2_of(r.m - at);
+                    r.m = m;
+                }
+                r.s = s;
+                state[i * FL_WAVE] = r;
+            }
+        });
+    Running r[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) r[i] = state[i * FL_WAVE];
+    __syncthreads();  // the operands in the LDS are read
+    store_running<BM, WN>(a, r, reinterpret_cast<Running *>(wide_lds), run.wave_m(), run.wave_n() / 64, row0, part);
+}
+
+// dz of a piece but for the listed columns.
+template <typename T, int BM, int WN, int STAGES>
+__global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
+    using Tiles = LogitTiles<T, BM, WN, STAGES>;
+    using Run = typename Tiles::Run;
+    constexpr int MT = Run::MT;
+    extern __shared__ __align__(16) uint16_t wide_lds[];
+    uint32_t mt, part;
+    row_and_part(a, &mt, &part);
+    const int64_t row0 = (int64_t)mt * BM, end = a.v0 + a.width;
+    const int64_t t0 = (int64_t)a.n_tiles * part / a.parts, t1 = (int64_t)a.n_tiles * (part + 1) / a.parts;
+    float2 *of = reinterpret_cast<float2 *>(wide_lds + STAGES * Run::ELEMS);  // (lse, coefficient) of the tile's rows
+    for (int t = threadIdx.x; t < BM; t += WD_NT) {
+        const int64_t m = row0 + t < a.op.M ? row0 + t : a.op.M - 1;
+        of[t] = float2{a.rows[m].x, a.coef[m]};
+    }
+    __syncthreads();
+    Tiles tiles;
+    tiles.init(a, row0, a.v0 + t0 * WN * 64);
+    const float scale = a.undo ? a.undo[0] * a.undo[1] * a.scale : a.scale;
+    Run run;
+    run.run(
+        tiles.ta, tiles.tb, t1 - t0, tiles.steps, wide_lds, [&](uint16_t *la, uint16_t *lb) { tiles.feed(a, la, lb); },
+        [&](int64_t t) {
+            const int64_t c = (t0 + t) * WN * 64 + run.wave_n() + (fl_lane() >> 4) * 16, n = a.v0 + c;
+            const int have = end - n < 16 ? (int)(end - n) : 16;
+            float b[16];
+            if (a.op.bias) lane_bias<T>(a, n, b);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int r = run.wave_m() + i * 16 + (fl_lane() & 15);
+                const float2 q = of[r];
+                float u[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    u[e] = run.acc[i][e / 4][e % 4] * scale;
+                    if (a.op.bias) u[e] += b[e];
+                    u[e] = q.y == 0.0f ? 0.0f : q.y * exp2_of(u[e] - q.x);
+                }
+                if (__any(have < 16))
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) u[e] = e < have ? u[e] : 0.0f;
+                if (row0 + r >= a.op.M) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (c + h * 8 >= a.d_cols) continue;
+                    Vec<Half<T>, 8> o;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o.v[e] = (Half<T>)u[h * 8 + e];
+                    Half<T> *to = (Half<T> *)a.d + (row0 + r) * a.ldd + (is_pairs<T>() ? pair_at(c + h * 8) : c + h * 8);
+                    store_vec<Half<T>, 8>(to, o);
+                    if constexpr (is_pairs<T>()) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o.v[e] = (Half<T>)(u[h * 8 + e] - (float)o.v[e]);
+                        store_vec<Half<T>, 8>(to + 32, o);
+                    }
+                }
+            }
+        });
+}
+
+// A piece's part of dx, added to what is there if `add`.
+template <typename T, int BM, int WN, int STAGES>
+__global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
+    constexpr bool PAIRS = is_pairs<T>();
+    constexpr int STEP = PAIRS ? 32 : 64;
+    using TA = WideContig<BM, 64>;
+    using TB = WideStrided<WN * 64, 64, false, PAIRS>;
+    using Run = WideTiles<Half<T>, PAIRS, BM, WN, STAGES, TA, TB>;
+    extern __shared__ __align__(16) uint16_t wide_lds[];
+    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x), tiles = a.m_tiles * a.n_tiles;
+    const uint32_t part = w / tiles, tile = w % tiles;
+    const int64_t row0 = (int64_t)(tile % a.m_tiles) * BM, n0 = (int64_t)(tile / a.m_tiles) * WN * 64, M = a.op.M;
+    const int64_t all = (a.width + STEP - 1) / STEP, s0 = all * part / a.parts, s1 = all * (part + 1) / a.parts;
+    TA ta;
+    TB tb;
+    ta.init([&](int r) { return (const uint16_t *)a.d + (row0 + r < M ? row0 + r : M - 1) * a.ldd + s0 * 64; });
+    tb.init(a.w + (a.v0 + s0 * STEP) * a.ldw + (PAIRS ? 2 * n0 : n0), a.ldw, a.cols - n0);
+    int64_t left = (s1 == all ? a.width : s1 * STEP) - s0 * STEP;
+    Run run;
+    run.run(
+        ta, tb, 1, (int)(s1 - s0), wide_lds,
+        [&](uint16_t *la, uint16_t *lb) {
+            if (left >= STEP) {
+                ta.template issue<true>(la, 64);
+                tb.template issue<true>(lb, STEP, {});
+            } else {  // the columns behind the piece are 0
+                if (PAIRS) ta.template issue<true>(la, 64);
+                else ta.template issue<false>(la, (int)left);
+                tb.template issue<false>(lb, (int)left, {});
+            }
+            left -= STEP;
+        },
+        [&](int64_t) {
+#pragma unroll
+            for (int i = 0; i < Run::MT; ++i) {
+                const int64_t row = row0 + run.wave_m() + i * 16 + (fl_lane() & 15);
+                if (row >= M) continue;
+#pragma unroll
+                for (int j = 0; j < Run::NTL; ++j) {
+                    const int64_t n = n0 + run.wave_n() + j * 16 + (fl_lane() >> 4) * 4;
+                    if (n >= a.op.K) continue;
+                    const int have = a.op.K - n < 4 ? (int)(a.op.K - n) : 4;
+                    float *q = a.sums + ((int64_t)part * M + row) * a.op.K + n;
+                    Vec<float, 4> f{{run.acc[i][j][0], run.acc[i][j][1], run.acc[i][j][2], run.acc[i][j][3]}};
+                    if (a.add) {
+                        float old[4];
+                        load_some<float>(q, have, old);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f.v[e] += old[e];
+                    }
+                    if (have == 4) store_vec<float, 4>(q, f);
+                    else store_some<float, 4>(q, f, have);
+                }
+            }
+        });
+}
+
+// A piece's rows of dW, or of a part of the rows' sum: tiles in a row.
+template <typename T, int WN, int STAGES>
+__global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
+    constexpr bool PAIRS = is_pairs<T>();
+    constexpr int STEP = PAIRS ? 32 : 64, BM = 256;
+    using TA = WideStrided<BM, 64, false, PAIRS>;
+    using TB = WideStrided<WN * 64, 64, false, PAIRS>;
+    using Run = WideTiles<Half<T>, PAIRS, BM, WN, STAGES, TA, TB>;
+    extern __shared__ __align__(16) uint16_t wide_lds[];
+    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x), walks = gridDim.x / a.parts;
+    const uint32_t part = w / walks, walk = w % walks;
+    const int64_t all = (int64_t)a.m_tiles * a.n_tiles, t0 = all * walk / walks, t1 = all * (walk + 1) / walks;
+    const int64_t begin = a.op.M * part / a.parts, len = a.op.M * (part + 1) / a.parts - begin;
+    const int steps = (int)((len + STEP - 1) / STEP);
+    TA ta;
+    TB tb;
+    int64_t next = t0, left = len;
+    const auto aim = [&]() {
+        const int64_t m0 = next / a.n_tiles * BM, c0 = next % a.n_tiles * (WN * 64);
+        ta.init((const uint16_t *)a.d + begin * a.ldd + (PAIRS ? 2 * m0 : m0), a.ldd, a.d_cols - m0);
+        tb.init(a.x + begin * a.ldx + (PAIRS ? 2 * c0 : c0), a.ldx, a.cols - c0);
+    };
+    aim();
+    const float f = a.sums ? 1.0f : *a.unscale, f2 = a.sums || !a.undo ? 1.0f : a.undo[0];
+    Run run;
+    run.run(
+        ta, tb, t1 - t0, steps, wide_lds,
+        [&](uint16_t *la, uint16_t *lb) {
+            if (left >= STEP) {
+                ta.template issue<true>(la, STEP, {});
+                tb.template issue<true>(lb, STEP, {});
+            } else {
+                ta.template issue<false>(la, (int)left, {});
+                tb.template issue<false>(lb, (int)left, {});
+            }
+            left -= STEP;
+            if (left > 0) return;
+            left = len;
+            if (++next < t1) aim();
+        },
+        [&](int64_t t) {
+            const int64_t m0 = (t0 + t) / a.n_tiles * BM, c0 = (t0 + t) % a.n_tiles * (WN * 64);
+#pragma unroll
+            for (int i = 0; i < Run::MT; ++i) {
+                const int64_t m = m0 + run.wave_m() + i * 16 + (fl_lane() & 15);
+                if (m >= a.width) continue;
+#pragma unroll
+                for (int j = 0; j < Run::NTL; ++j) {
+                    const int64_t c = c0 + run.wave_n() + j * 16 + (fl_lane() >> 4) * 4;
+                    if (c >= a.op.K) continue;
+                    const int n = a.op.K - c < 4 ? (int)(a.op.K - c) : 4;
+                    if (a.sums) {
+                        float *q = a.sums + ((int64_t)part * a.width + m) * a.op.K + c;
+                        const Vec<float, 4> o{{run.acc[i][j][0], run.acc[i][j][1], run.acc[i][j][2], run.acc[i][j][3]}};
+                        if (n == 4) store_vec<float, 4>(q, o);
+                        else store_some<float, 4>(q, o, n);
+                    } else {
+                        T *q = (T *)a.dw + (a.v0 + m) * a.op.K + c;
+                        Vec<T, 4> o;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o.v[e] = (T)(run.acc[i][j][e] * f * f2);
+                        if (n == 4) store_vec<T, 4>(q, o);
+                        else store_some<T, 4>(q, o, n);
+                    }
+                }
+            }
+        });
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+
+// How the products of a vocabulary are cut.
+struct VocabPlan {
+    bool wide, pairs, lay;             // wide kernels; two planes; operands laid out
+    int bm, bn;                        // tiles of the logits
+    uint32_t m_tiles, n_tiles, parts;  // parts: of the vocabulary, in the forward
+    int64_t piece, d_cols, ldd;        // columns of dz in the backward, with those that pad them, and its row stride
+    int64_t cols;                      // wide: inputs, with those that pad them
+    int64_t size;                      // bytes of a value of dz
+};
+
+VocabPlan vocab_plan(const fl_vocab *op) {
+    VocabPlan p{};
+    p.pairs = op->dtype == FL_F32;
+    p.wide = op->K >= 1 && op->K <= 1 << 20 && (double)op->M * op->V * op->K >= 1 << 27;
+    p.size = p.pairs ? 4 : 2;
+    if (p.wide) {
+        p.lay = p.pairs || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % 8;
+        p.cols = p.pairs ? ceil_div(op->K, 32) * 32 : ceil_div(op->K, 8) * 8;
+        const bool small = ceil_div(op->M, 256) * ceil_div(op->V, 256) < 192;
+        p.bm = small ? 128 : 256;
+        p.bn = small ? 128 : 256;
+    } else {
+        p.bm = op->M > 64 ? 128 : 64;
+        p.bn = p.bm;
+    }
+    p.m_tiles = (uint32_t)ceil_div(op->M, p.bm);
+    p.n_tiles = (uint32_t)ceil_div(op->V, p.bn);
+    const int64_t want = p.wide ? (p.m_tiles < 256 ? 256 / p.m_tiles : 1) : ceil_div(1024, p.m_tiles);
+    p.parts = (uint32_t)(want < p.n_tiles ? want : p.n_tiles);
+    int64_t piece = (int64_t)(LS_PIECE / p.size) / (op->M > 0 ? op->M : 1) / 256 * 256;
+    if (piece < 256) piece = 256;
+    if (piece > 1 << 22) piece = 1 << 22;  // 32-bit offsets of 64 rows of dz
+    p.piece = piece < op->V ? piece : op->V;
+    p.d_cols = p.wide && p.pairs ? ceil_div(p.piece, 32) * 32 : ceil_div(p.piece, 8) * 8;
+    p.ldd = p.wide && p.pairs ? 2 * p.d_cols : p.d_cols;
+    return p;
+}
+
+// The laid out operands: x, weight, what undoes their powers of two, parts of their maxima.
+struct VocabLayout {
+    size_t x, w, undo, most, bytes;
+};
+
+VocabLayout vocab_layout(const fl_vocab *op, const VocabPlan &p) {
+    VocabLayout l{};
+    if (!p.lay) return l;
+    l.w = rounded((size_t)op->M * p.cols * p.size);
+    l.undo = l.w + rounded((size_t)op->V * p.cols * p.size);
+    l.most = l.undo + 256;
+    l.bytes = l.most + (p.pairs ? 2 * LAY_PARTS * 4 : 0);
+    return l;
+}
+
+struct VocabSpace {
+    size_t coef, d, dx, dw, db, bytes;
+    int dx_parts, dw_parts, db_parts;
+    int dx_tile, dx_cols, dw_cols, dw_tile;
+    uint32_t dw_walks;
+};
+
+VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, bool with_dw, bool with_db) {
+    VocabSpace s{};
+    const auto take = [&](size_t n) {
+        const size_t at = s.bytes;
+        s.bytes += rounded(n);
+        return at;
+    };
+    const bool f32 = op->dtype == FL_F32;
+    s.coef = take((size_t)(op->M + 1) * 4);
+    s.d = take((size_t)op->M * p.ldd * (p.wide ? 2 : p.size));
+    const int narrow = op->K <= 128 ? 128 : 256;
+    if (with_dx) {
+        if (p.wide) {
+            s.dx_tile = ceil_div(op->M, 256) * ceil_div(op->K, narrow) < 16 ? 128 : 256;
+            s.dx_cols = s.dx_tile == 128 ? 128 : narrow;
+            const int64_t tiles = ceil_div(op->M, s.dx_tile) * ceil_div(op->K, s.dx_cols);
+            const int64_t want = 256 / tiles, most = p.piece / 256;
+            const int64_t n = want < most ? want : most;
+            s.dx_parts = (int)(n < 1 ? 1 : n > 32 ? 32 : n);
+        } else {
+            const Cut c = best_cut(op->M, op->K, p.piece, f32, false);
+            s.dx_parts = c.parts;
+            s.dx_tile = c.rows == 128 && op->K >= 2 ? 128 : 64;
+        }
+        s.dx = take((size_t)s.dx_parts * op->M * op->K * 4);
+    }
+    if (with_dw) {
+        if (p.wide) {
+            s.dw_cols = narrow;
+            const int64_t tiles = ceil_div(p.piece, 256) * ceil_div(op->K, narrow), want = 256 / tiles, most = op->M / 256;
+            const int64_t n = want < most ? want : most;
+            s.dw_parts = (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+            s.dw_walks = (uint32_t)(tiles < 256 ? tiles : 256);
+        } else {
+            const Cut c = best_cut(p.piece, op->K, op->M, f32, false);
+            s.dw_parts = c.parts;
+            s.dw_tile = c.rows == 128 && op->K >= 2 && p.piece >= 2 ? 128 : 64;
+        }
+        if (s.dw_parts > 1) s.dw = take((size_t)s.dw_parts * p.piece * op->K * 4);
+    }
+    if (with_db) {
+        const int64_t want = ceil_div(2048, ceil_div(p.piece, LS_NT)), most = op->M / 16;
+        const int64_t n = want < most ? want : most;
+        s.db_parts = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+        s.db = take((size_t)s.db_parts * p.piece * 4);
+    }
+    return s;
+}
+
+VocabArgs vocab_args(const fl_vocab *op, const VocabPlan &p, void *state, void *layout) {
+    VocabArgs a{};
+    a.op = *op;
+    a.scale = LOG2E / op->lists.temperature;
+    a.rows = state_rows(state);
+    a.listed = state_listed(&op->lists, state);
+    a.width = op->V;
+    a.cols = p.cols;
+    if (p.lay) {
+        const VocabLayout l = vocab_layout(op, p);
+        a.x = (const uint16_t *)((char *)layout + l.x);
+        a.w = (const uint16_t *)((char *)layout + l.w);
+        a.ldx = a.ldw = p.pairs ? 2 * p.cols : p.cols;
+        if (p.pairs) a.undo = (const float *)((char *)layout + l.undo);
+    } else {
+        a.x = (const uint16_t *)op->x;
+        a.w = (const uint16_t *)op->weight;
+        a.ldx = op->ldx;
+        a.ldw = op->ldw;
+    }
+    return a;
+}
+
+constexpr unsigned tiles_bytes(int bm, int bn, int stages) { return (unsigned)(stages * (bm + bn) * 64 * 2); }
+
+template <typename T>
+int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, void *layout, void *ws) {
+    constexpr int BK = sizeof(T) == 4 ? 32 : 64;
+    const VocabPlan p = vocab_plan(op);
+    VocabArgs a = vocab_args(op, p, state, layout);
+    a.m_tiles = p.m_tiles;
+    a.n_tiles = p.n_tiles;
+    a.parts = p.parts;
+    a.part = (Running *)ws;
+    const int64_t grid = (int64_t)p.m_tiles * p.parts;
+    if (!launch_fits(grid, WD_NT)) return fl_fail(FL_ERR_ARG, "linear_loss: too many tiles for one launch (shape)");
+    const dim3 g((unsigned)grid);
+    if (p.lay) {
+        const VocabLayout l = vocab_layout(op, p);
+        float *most = (float *)((char *)layout + l.most);
+        if (p.pairs) FL_LAUNCH("k_lay_max", k_lay_max, dim3(LAY_PARTS, 2), dim3(LS_NT), 0, st, a, most);
+        const int64_t chunks = (op->M > op->V ? op->M : op->V) * (p.cols / 8), want = ceil_div(chunks, LS_NT);
+        FL_LAUNCH("k_lay", k_lay<T>, dim3((unsigned)(want < 4096 ? want : 4096), 2), dim3(LS_NT), 0, st, a, most,
+                  (uint16_t *)a.x, (uint16_t *)a.w, (float *)a.undo);
+    }
+    if (op->lists.k)
+        FL_LAUNCH("k_vocab_dots", k_vocab_dots<T>,
+                  grid_of(ceil_div(op->M * ceil_div(op->lists.k, DOT_IDS), LS_WAVES)), dim3(LS_NT), 0, st, a);
+    if (p.wide) {
+        const auto extra = [](int, int mt) { return (unsigned)(WD_WAVES * mt * FL_WAVE * sizeof(Running)); };
+        if (p.bm == 256)
+            FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 256, 4, 2>), g, dim3(WD_NT), tiles_bytes(256, 256, 2) + extra(256, 8), st, a);
+        else
+            FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 128, 2, 4>), g, dim3(WD_NT), tiles_bytes(128, 128, 4) + extra(128, 2), st, a);
+    } else if (p.bm == 128)
+        FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 128, 128, BK>), g, dim3(LN_NT), 0, st, a);
+    else FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 64, 64, BK>), g, dim3(LN_NT), 0, st, a);
+    return join_listed(st, &op->lists, op->V, a.part, p.parts, state, loss, "linear_loss");
+}
+
+template <typename T>
+int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *state, void *layout, void *dx, void *dw,
+                   void *db, char *ws) {
+    constexpr int BK = sizeof(T) == 4 ? 32 : 64;
+    const VocabPlan p = vocab_plan(op);
+    const VocabSpace s = vocab_space(op, p, dx, dw, db);
+    VocabArgs a = vocab_args(op, p, state, layout);
+    float *coef = (float *)(ws + s.coef);
+    a.coef = coef;
+    a.unscale = coef + op->M;
+    a.d = ws + s.d;
+    a.ldd = p.ldd;
+    a.d_cols = p.d_cols;
+    const dim3 nt(LN_NT), wt(WD_NT);
+    const auto fits = [&](int64_t grid) { return launch_fits(grid, WD_NT); };
+    const auto fail = [&]() { return fl_fail(FL_ERR_ARG, "linear_loss: too many tiles for one launch (shape)"); };
+    if (std::is_same<T, _Float16>::value || (p.wide && p.pairs))
+        FL_LAUNCH("k_vocab_coef", k_vocab_coef<true>, dim3(1), dim3(1024), 0, st, a.rows, grad, op->lists.temperature,
+                  op->M, coef, coef + op->M);
+    else
+        FL_LAUNCH("k_vocab_coef", k_vocab_coef<false>, dim3((unsigned)(op->M > 65536 ? 64 : ceil_div(op->M, 1024))),
+                  dim3(1024), 0, st, a.rows, grad, op->lists.temperature, op->M, coef, coef + op->M);
+    for (a.v0 = 0; a.v0 < op->V; a.v0 += p.piece) {
+        a.width = op->V - a.v0 < p.piece ? op->V - a.v0 : p.piece;
+        a.m_tiles = p.m_tiles;
+        a.n_tiles = (uint32_t)ceil_div(a.width, p.bn);
+        if (p.wide) {
+            const int64_t want = p.m_tiles < 256 ? 256 / p.m_tiles : 1;
+            a.parts = (uint32_t)(want < a.n_tiles ? want : a.n_tiles);
+        } else a.parts = a.n_tiles;
+        int64_t grid = (int64_t)a.m_tiles * a.parts;
+        if (!fits(grid)) return fail();
+        if (p.wide) {
+            const auto extra = [](int bm) { return (unsigned)(bm * sizeof(float2)); };
+            if (p.bm == 256)
+                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 256, 4, 2>), dim3((unsigned)grid), wt, tiles_bytes(256, 256, 2) + extra(256), st, a);
+            else
+                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 128, 2, 4>), dim3((unsigned)grid), wt, tiles_bytes(128, 128, 4) + extra(128), st, a);
+        } else if (p.bm == 128)
+            FL_LAUNCH("k_vocab_grad", (k_vocab_grad<T, 128, 128, BK>), dim3((unsigned)grid), nt, 0, st, a);
+        else FL_LAUNCH("k_vocab_grad", (k_vocab_grad<T, 64, 64, BK>), dim3((unsigned)grid), nt, 0, st, a);
+        if (op->lists.k) {
+            const dim3 g = grid_of(ceil_div(op->M * op->lists.k, LS_NT));
+            if (p.wide) FL_LAUNCH("k_vocab_listed", (k_vocab_listed<T, true>), g, dim3(LS_NT), 0, st, a);
+            else FL_LAUNCH("k_vocab_listed", (k_vocab_listed<T, false>), g, dim3(LS_NT), 0, st, a);
+        }
+        if (dx && op->K) {
+            a.m_tiles = (uint32_t)ceil_div(op->M, s.dx_tile);
+            a.n_tiles = (uint32_t)ceil_div(op->K, p.wide ? s.dx_cols : s.dx_tile);
+            a.parts = (uint32_t)s.dx_parts;
+            a.sums = (float *)(ws + s.dx);
+            a.add = a.v0 > 0;
+            grid = (int64_t)a.m_tiles * a.n_tiles * a.parts;
+            if (!fits(grid)) return fail();
+            const dim3 g((unsigned)grid);
+            if (p.wide) {
+                if (s.dx_tile == 128)
+                    FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 128, 2, 4>), g, wt, tiles_bytes(128, 128, 4), st, a);
+                else if (s.dx_cols == 128)
+                    FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 256, 2, 3>), g, wt, tiles_bytes(256, 128, 3), st, a);
+                else
+                    FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 256, 4, 2>), g, wt, tiles_bytes(256, 256, 2), st, a);
+            } else if (s.dx_tile == 128)
+                FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 128, 128, BK>), g, nt, 0, st, a);
+            else FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 64, 64, BK>), g, nt, 0, st, a);
+        }
+        if (dw && op->K) {
+            const int rows = p.wide ? 256 : s.dw_tile, cols = p.wide ? s.dw_cols : s.dw_tile;
+            a.m_tiles = (uint32_t)ceil_div(a.width, rows);
+            a.n_tiles = (uint32_t)ceil_div(op->K, cols);
+            a.parts = (uint32_t)s.dw_parts;
+            a.sums = s.dw_parts > 1 ? (float *)(ws + s.dw) : nullptr;
+            a.dw = dw;
+            grid = (int64_t)a.m_tiles * a.n_tiles;
+            if (p.wide && grid > s.dw_walks) grid = s.dw_walks;
+            grid *= a.parts;
+            if (!fits(grid)) return fail();
+            const dim3 g((unsigned)grid);
+            if (p.wide) {
+                if (cols == 128) FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 2, 3>), g, wt, tiles_bytes(256, 128, 3), st, a);
+                else FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 4, 2>), g, wt, tiles_bytes(256, 256, 2), st, a);
+            } else if (rows == 128)
+                FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 128, 128, BK>), g, nt, 0, st, a);
+            else FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 64, 64, BK>), g, nt, 0, st, a);
+            if (a.sums)
+                FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(a.width * op->K, LS_NT * 4)), dim3(LS_NT),
+                          0, st, a.sums, a.parts, a.width * op->K, a.unscale, a.undo, (T *)dw + a.v0 * op->K);
+        }
+        if (db) {
+            a.parts = (uint32_t)s.db_parts;
+            a.sums = (float *)(ws + s.db);
+            const dim3 cg = grid_of(a.parts * ceil_div(a.width, LS_NT)), g = grid_of(ceil_div(a.width, LS_NT * 4));
+            if (p.wide) FL_LAUNCH("k_vocab_cols", (k_vocab_cols<T, true>), cg, dim3(LS_NT), 0, st, a);
+            else FL_LAUNCH("k_vocab_cols", (k_vocab_cols<T, false>), cg, dim3(LS_NT), 0, st, a);
+            const float *none = nullptr;
+            if (op->bias_f32)
+                FL_LAUNCH("k_vocab_fold", k_vocab_fold<float>, g, dim3(LS_NT), 0, st, a.sums, a.parts, a.width,
+                          a.unscale, none, (float *)db + a.v0);
+            else
+                FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, g, dim3(LS_NT), 0, st, a.sums, a.parts, a.width, a.unscale,
+                          none, (T *)db + a.v0);
+        }
+    }
+    if (dx && op->K)
+        FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(op->M * op->K, LS_NT * 4)), dim3(LS_NT), 0, st,
+                  (const float *)(ws + s.dx), (uint32_t)s.dx_parts, op->M * op->K, a.unscale,
+                  a.undo ? a.undo + 1 : nullptr, (T *)dx);
+    return fl_check_launch("linear_loss");
+}
+
+int check_vocab(const fl_vocab *op, const char *what) {
+    if (!op) return fl_fail(FL_ERR_ARG, "%s: null operator", what);
+    if (op->dtype < FL_F32 || op->dtype > FL_F16) return fl_fail(FL_ERR_ARG, "%s: unknown type", what);
+    if (op->M < 0 || op->V < 1 || op->K < 0 || op->V > 0x7fffffffll || op->K > 0x7fffffffll || op->M != op->lists.rows)
+        return fl_fail(FL_ERR_ARG, "%s: bad shape", what);
+    if (op->M && op->K && (!op->x || !op->weight)) return fl_fail(FL_ERR_ARG, "%s: null pointer", what);
+    return check_lists(&op->lists, what);
+}
+
+}  // namespace
+}  // namespace fl
+
+#define FL_BY_TYPE(dtype, call)                           \
+    switch (dtype) {                                      \
+        case FL_F32: { using T = float; return call; }    \
+        case FL_BF16: { using T = __bf16; return call; }  \
+        default: { using T = _Float16; return call; }     \
+    }
+
+extern "C" {
+
+size_t fl_vocab_op_bytes(void) { return sizeof(fl_vocab); }
+
+size_t fl_vocab_layout_bytes(const fl_vocab *op) {
+    if (!op || op->M < 1 || op->V < 1 || op->K < 0) return 0;
+    return fl::vocab_layout(op, fl::vocab_plan(op)).bytes;
+}
+
+size_t fl_vocab_forward_bytes(const fl_vocab *op) {
+    if (!op || op->M < 1 || op->V < 1 || op->K < 0) return 0;
+    return (size_t)op->M * fl::vocab_plan(op).parts * 8;
+}
+
+int fl_vocab_forward(void *stream, const fl_vocab *op, float *loss, void *state, void *layout, void *ws,
+                     size_t ws_bytes) {
+    const int rc = fl::check_vocab(op, "linear_loss");
+    if (rc) return rc;
+    if (op->M == 0) return FL_OK;
+    const size_t need = fl_vocab_forward_bytes(op);
+    if (!loss || !state || (!layout && fl_vocab_layout_bytes(op))) return fl::fl_fail(FL_ERR_ARG, "linear_loss: null pointer");
+    if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "linear_loss: workspace too small");
+    FL_BY_TYPE(op->dtype, fl::vocab_forward<T>((hipStream_t)stream, op, loss, state, layout, ws))
+}
+
+size_t fl_vocab_backward_bytes(const fl_vocab *op, int with_dx, int with_dw, int with_db) {
+    if (!op || op->M < 1 || op->V < 1 || op->K < 0) return 0;
+    return fl::vocab_space(op, fl::vocab_plan(op), with_dx, with_dw, with_db).bytes;
+}
+
+int fl_vocab_backward(void *stream, const fl_vocab *op, const float *grad, void *state, void *layout, void *dx,
+                      void *dw, void *db, void *ws, size_t ws_bytes) {
+    const int rc = fl::check_vocab(op, "linear_loss");
+    if (rc) return rc;
+    if (op->M == 0) return FL_OK;
+    if (!grad || !state || (!layout && fl_vocab_layout_bytes(op))) return fl::fl_fail(FL_ERR_ARG, "linear_loss: null pointer");
+    const size_t need = fl_vocab_backward_bytes(op, dx != nullptr, dw != nullptr, db != nullptr);
+    if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "linear_loss: workspace too small");
+    if ((uintptr_t)ws % 16) return fl::fl_fail(FL_ERR_ARG, "linear_loss: workspace must be 16-byte aligned");
+    FL_BY_TYPE(op->dtype, fl::vocab_backward<T>((hipStream_t)stream, op, grad, state, layout, dx, dw, db, (char *)ws))
+}
+
+}  // extern "C"

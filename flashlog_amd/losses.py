@@ -77,7 +77,7 @@ def _vocab_op(x, weight, bias, lists):
 
 
 def _vocab_forward(what, x, weight, bias, lists):
-    """(losses, the laid out x, weight and bias, the state for the backward)."""
+    """(losses, x, weight and bias as the call took them, the state and the layout for the backward)."""
     dev, lib = x.device, _lib_handle()
     loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     x = _rows_of(x, x.shape[-1])
@@ -87,24 +87,25 @@ def _vocab_forward(what, x, weight, bias, lists):
         bias = bias.contiguous()
     op = _vocab_op(x, weight, bias, lists)
     state = _workspace(lib.fl_lists_state_bytes(op.lists), dev)
+    layout = _workspace(lib.fl_vocab_layout_bytes(op), dev)
     nbytes = lib.fl_vocab_forward_bytes(op)
     ws = _workspace(nbytes, dev)
-    _launch(what, lib.fl_vocab_forward, dev, op, loss.data_ptr(), _ptr(state), _ptr(ws), nbytes)
-    return loss, x, weight, bias, state
+    _launch(what, lib.fl_vocab_forward, dev, op, loss.data_ptr(), _ptr(state), _ptr(layout), _ptr(ws), nbytes)
+    return loss, x, weight, bias, state, layout
 
 
 class _VocabFunction(autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, lists, what):
-        loss, x2, w2, b2, state = _vocab_forward(what, x, weight, bias, lists)
-        ctx.save_for_backward(x2, w2, b2, state, lists.ids, lists.teacher)
+        loss, x2, w2, b2, state, layout = _vocab_forward(what, x, weight, bias, lists)
+        ctx.save_for_backward(x2, w2, b2, state, layout, lists.ids, lists.teacher)
         ctx.lists, ctx.what, ctx.shape = lists, what, x.shape
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, weight, bias, state = ctx.saved_tensors[:4]
+        x, weight, bias, state, layout = ctx.saved_tensors[:5]
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev, lib, grad = x.device, _lib_handle(), grad.contiguous()
         make = torch.empty if x.shape[0] else torch.zeros  # the sums over no rows
@@ -115,8 +116,8 @@ class _VocabFunction(autograd.Function):
             op = _vocab_op(x, weight, bias, ctx.lists)
             nbytes = lib.fl_vocab_backward_bytes(op, need_x, need_w, need_b)
             ws = _workspace(nbytes, dev)
-            _launch(ctx.what, lib.fl_vocab_backward, dev, op, grad.data_ptr(), _ptr(state), _ptr(dx), _ptr(dw),
-                    _ptr(db), _ptr(ws), nbytes)
+            _launch(ctx.what, lib.fl_vocab_backward, dev, op, grad.data_ptr(), _ptr(state), _ptr(layout), _ptr(dx),
+                    _ptr(dw), _ptr(db), _ptr(ws), nbytes)
         return dx, dw, db, None, None
 
 

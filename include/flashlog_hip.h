@@ -1010,17 +1010,21 @@ typedef struct fl_vocab {
 } fl_vocab;
 
 size_t fl_vocab_op_bytes(void);
+/* Bytes of the operands as the products take them where they are laid out anew
+ * (fp32, rows not on 16 bytes; else 0): a forward writes them, its backward
+ * reads them. */
+size_t fl_vocab_layout_bytes(const fl_vocab *op);
 size_t fl_vocab_forward_bytes(const fl_vocab *op);
 int fl_vocab_forward(void *stream, const fl_vocab *op, float *loss,
-                     void *state, void *ws, size_t ws_bytes);
+                     void *state, void *layout, void *ws, size_t ws_bytes);
 /* Those of the gradients that are not null: dx [M, K] and dw [V, K] of the
  * operands' type, db [V] fp32 if bias_f32, else of the operands' type.  ws on
  * a 16-byte boundary. */
 size_t fl_vocab_backward_bytes(const fl_vocab *op, int with_dx, int with_dw,
                                int with_db);
 int fl_vocab_backward(void *stream, const fl_vocab *op, const float *grad,
-                      void *state, void *dx, void *dw, void *db, void *ws,
-                      size_t ws_bytes);
+                      void *state, void *layout, void *dx, void *dw, void *db,
+                      void *ws, size_t ws_bytes);
 
 #ifdef __cplusplus
 }

@@ -89,14 +89,18 @@ def test_vocab_arguments():
             setattr(p, k, v)
         return p
 
-    fwd = lambda p, loss=ONE, size=1 << 20: _error(lib.fl_vocab_forward(None, p, loss, ONE, ONE, size))
+    fwd = lambda p, loss=ONE, size=1 << 20: _error(lib.fl_vocab_forward(None, p, loss, ONE, None, ONE, size))
     for word, kw in LISTS:
         if kw != dict(rows=-1):
             assert word in fwd(op(_lists(**kw)))
     assert "type" in fwd(op(dtype=3)) and "shape" in fwd(op(V=0)) and "shape" in fwd(op(K=-1))
     assert "shape" in fwd(op(M=3)) and "null" in fwd(op(x=None)) and "null" in fwd(op(weight=None))
     assert "null" in fwd(op(), None) and "workspace" in fwd(op(), ONE, 0)
-    back = lambda p, ws=ONE, size=1 << 30, g=ONE: _error(lib.fl_vocab_backward(None, p, g, ONE, ONE, ONE, ONE, ws, size))
+    back = lambda p, ws=ONE, size=1 << 30, g=ONE: _error(
+        lib.fl_vocab_backward(None, p, g, ONE, None, ONE, ONE, ONE, ws, size))
     assert "null" in back(op(), g=None) and "workspace" in back(op(), size=16)
     assert "16-byte" in back(op(), ctypes.c_void_p(24))
-    assert lib.fl_vocab_backward(None, op(_lists(rows=0), M=0), None, None, None, None, None, None, 0) == 0
+    assert lib.fl_vocab_backward(None, op(_lists(rows=0), M=0), None, None, None, None, None, None, None, 0) == 0
+    large = op(_lists(rows=4096), M=4096, V=4096, K=64, ldx=64, ldw=64)
+    assert lib.fl_vocab_layout_bytes(large) > 4 * 2 * 4096 * 64 and lib.fl_vocab_layout_bytes(op()) == 0
+    assert "null" in fwd(large)
