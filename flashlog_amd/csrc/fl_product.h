@@ -401,6 +401,45 @@ struct WideContig {
     }
 };
 
+// A value that the compiler takes for new at this place, so that what is made of
+// it is not kept in registers over a loop.
+__device__ __forceinline__ int made_here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// The same for rows of whole steps, from a base that all lanes have and with
+// 32-bit offsets (half the registers): rows of less than 2^23 values.
+template <int BR>
+struct StepsContig {
+    using At = WideContig<BR, 64>;
+    static constexpr int LOADS = At::LOADS, ELEMS = At::ELEMS;
+    const uint16_t *base;  // of the next step
+    uint32_t at[LOADS];    // bytes
+
+    // Row r of the tile is row row_at(r) from b on.
+    template <typename F>
+    __device__ __forceinline__ void init(const uint16_t *b, int64_t ld, F &&row_at) {
+        const int lane = made_here(fl_lane());
+        base = b;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = (fl_wave_id() * LOADS + i) * 8 + lane / 8;
+            at[i] = (uint32_t)row_at(r) * (uint32_t)(ld * 2) + lds_at<64>(r, lane % 8) % 64 * 2;
+        }
+    }
+    __device__ __forceinline__ void issue(uint16_t *lds) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            load_lds((const char *)base + at[i], lds + (fl_wave_id() * LOADS + i) * 512);
+        base += 64;
+    }
+    template <int N>
+    __device__ __forceinline__ void read(const uint16_t *lds, int row0, u32x4 (&f)[2][N]) const {
+        At().read(lds, row0, f);
+    }
+};
+
 // fp32 values as two fp16 planes, v s = v0 + v1 with a power of two s that brings
 // the largest to 2^13..2^14: v1 is the rest rounded, so that what is lost is below
 // 2^-22 of v or 2^-39 of the largest.  A row holds 32 values of the one plane, the
@@ -409,9 +448,7 @@ struct WideContig {
 __device__ __forceinline__ int64_t pair_at(int64_t c) { return c / 32 * 64 + c % 32; }
 
 // k-strided: the rows of k one after the other, or in an order if GATHER.
-// PAIRS: of values held as two planes (pair_at), BK / 2 rows of the one
-// plane and then the same rows of the other.
-template <int BR, int BK, bool GATHER, bool PAIRS = false>
+template <int BR, int BK, bool GATHER>
 struct WideStrided {
     static constexpr int CH = BR / 8;                // chunks a row of k
     static constexpr int RPL = FL_WAVE / CH;         // rows of k a load
@@ -425,16 +462,15 @@ struct WideStrided {
     // transposed read takes of each of 4 rows.
     static __device__ __forceinline__ int turn(int k) { return 2 * ((k & 3) | ((((k >> 3) ^ (k >> 4)) & 1) << 2)); }
     static __device__ __forceinline__ int row(int i) { return (fl_wave_id() * LOADS + i) * RPL + fl_lane() / CH; }
-    static __device__ __forceinline__ int row_of_k(int i) { return PAIRS ? row(i) % (BK / 2) : row(i); }
 
     __device__ __forceinline__ void init(const uint16_t *b, int64_t stride, int64_t R) {
         base = b;
         ld = stride;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int64_t c0 = ((fl_lane() % CH) ^ turn(row(i))) * 8, c = c0 <= R - 8 ? c0 : R - 8;
-            at[i] = (uint32_t)((PAIRS ? pair_at(c) + row(i) / (BK / 2) * 32 : c) * 2);
-            if constexpr (!GATHER) at[i] += (uint32_t)(row_of_k(i) * stride * 2);
+            const int64_t c = ((fl_lane() % CH) ^ turn(row(i))) * 8;
+            at[i] = (uint32_t)((c <= R - 8 ? c : R - 8) * 2);
+            if constexpr (!GATHER) at[i] += (uint32_t)(row(i) * stride * 2);
         }
     }
     // The next `count` rows of k, BK if WHOLE; r: this lane's, if GATHER.
@@ -444,7 +480,7 @@ struct WideStrided {
         for (int i = 0; i < LOADS; ++i) {
             const char *q = (const char *)base + at[i];
             if constexpr (GATHER) q += (int64_t)r[i] * ld * 2;
-            if (!WHOLE && row_of_k(i) >= count) q = (const char *)wd_zeros;
+            if (!WHOLE && row(i) >= count) q = (const char *)wd_zeros;
             load_lds(q, lds + (fl_wave_id() * LOADS + i) * 512);
         }
         if constexpr (!GATHER) base += count * ld;
@@ -496,6 +532,43 @@ struct WideStrided {
                     f[ks][i + t] = u32x4{(uint32_t)v[t][2 * ks], (uint32_t)(v[t][2 * ks] >> 32),
                                          (uint32_t)v[t][2 * ks + 1], (uint32_t)(v[t][2 * ks + 1] >> 32)};
         }
+    }
+};
+
+// The same, k rows one after the other, without guards: rows behind the last one
+// read it again, so that the other operand has to be 0 there.  PAIRS: of values
+// held as two planes, 32 rows of the one and then the same rows of the other.
+template <int BR, bool PAIRS>
+struct StepsStrided {
+    using At = WideStrided<BR, 64, false>;
+    static constexpr int LOADS = At::LOADS, ELEMS = At::ELEMS, STEP = PAIRS ? 32 : 64;
+    const uint16_t *base;  // of the next step
+    int64_t ld;
+    uint32_t at[LOADS];  // bytes
+
+    // From column 0 of b on, R columns; `rows`: of k that there are, STEP at most.
+    __device__ __forceinline__ void init(const uint16_t *b, int64_t stride, int64_t R, int rows) {
+        const int lane = made_here(fl_lane());
+        base = b;
+        ld = stride;
+        const int most = R - 8 < BR ? (int)R - 8 : BR;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = (fl_wave_id() * LOADS + i) * At::RPL + lane / At::CH, k = PAIRS ? r % 32 : r;
+            const int c0 = ((lane % At::CH) ^ At::turn(r)) * 8, c = c0 < most ? c0 : most;
+            at[i] = (uint32_t)(PAIRS ? (int)pair_at(c) + r / 32 * 32 : c) * 2 +
+                    (uint32_t)(k < rows ? k : rows - 1) * (uint32_t)(stride * 2);
+        }
+    }
+    __device__ __forceinline__ void issue(uint16_t *lds) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            load_lds((const char *)base + at[i], lds + (fl_wave_id() * LOADS + i) * 512);
+        base += STEP * ld;
+    }
+    template <int N>
+    __device__ __forceinline__ void read(const uint16_t *lds, int col0, u32x4 (&f)[2][N]) const {
+        At().read(lds, col0, f);
     }
 };
 
@@ -622,7 +695,12 @@ struct WideTiles {
     static __device__ __forceinline__ int wave_m() { return (fl_wave_id() / WN) * (BM / WM); }
     static __device__ __forceinline__ int wave_n() { return (fl_wave_id() % WN) * 64; }
 
-    template <bool FIRST>
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    }
     __device__ __forceinline__ void multiply(const u32x4 (&fa)[2][MT], const u32x4 (&fb)[2][NTL]) {
 #pragma unroll
         for (int p = 0; p < (PAIRS ? 3 : 2); ++p)
@@ -631,62 +709,64 @@ struct WideTiles {
 #pragma unroll
                 for (int j = 0; j < NTL; ++j) {
                     const int ka = PAIRS ? p == 1 : p, kb = PAIRS ? p == 0 : p;
-                    const f32x4 c = FIRST && p == 0 ? f32x4{0, 0, 0, 0} : acc[i][j];
-                    acc[i][j] = mfma<T>(fb[kb][j], fa[ka][i], c);
+                    acc[i][j] = mfma<T>(fb[kb][j], fa[ka][i], acc[i][j]);
                 }
     }
 
-    template <typename F, typename O>
-    __device__ __forceinline__ void run(const TA &ta, const TB &tb, int64_t tiles, int steps, uint16_t *lds, F &&feed,
+    // ONE: a single tile.
+    template <bool ONE, typename F, typename O>
+    __device__ __forceinline__ void run(const TA &ta, const TB &tb, int tiles, int steps, uint16_t *lds, F &&feed,
                                         O &&out) {
-        const int64_t all = tiles * steps;
+        const int all = tiles * steps;
+        clear();
         if (all <= 0) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NTL; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-            for (int64_t t = 0; t < tiles; ++t) out(t);
+            for (int t = 0; t < tiles; ++t) out(t);
             return;
         }
         const bool second = fl_wave_id() >= WD_WAVES / 2;
-        const auto load = [&](int64_t step) {
-            uint16_t *to = lds + (int)(step % STAGES) * ELEMS;
+        uint16_t *to = lds;
+        const auto load = [&]() {
             feed(to, to + TA::ELEMS);
+            to = to == lds + (STAGES - 1) * ELEMS ? lds : to + ELEMS;
+        };
+        const auto arrive = [&](bool full) {  // the next step's loads have
+            if (full) Waits::template wait<LOADS *(STAGES - 2)>();
+            else Waits::template wait<0>();
         };
 #pragma unroll
         for (int s = 0; s < STAGES; ++s)
-            if (s < all) load(s);
+            if (s < all) load();
         if (all < STAGES) Waits::template wait<0>();
         else Waits::template wait<LOADS *(STAGES - 1)>();
         Waits::meet();
         if (second) Waits::meet();
-        int at = 0;
-        int64_t tile = 0;
-        for (int64_t s = 0; s < all; ++s) {
-            const uint16_t *la = lds + (int)(s % STAGES) * ELEMS, *lb = la + TA::ELEMS;
-            const bool full = s + STAGES - 1 < all;
-            if (!second && s > 0 && full) load(s + STAGES - 1);
-            if (second) {
-                if (full) Waits::template wait<LOADS *(STAGES - 2)>();
-                else Waits::template wait<0>();
+        const uint16_t *la = lds;
+        int at = 0, tile = 0;
+        for (int s = 0; !ONE || s < all; ++s) {
+            const bool full = s + STAGES - 1 < all, done = !ONE && at == steps;
+            if (!second && s > 0 && full) load();
+            if (done) {
+                if (s == all && !second) Waits::meet();
+                if (second && s < all) arrive(full);  // before out's stores are under way
+                out(tile++);
+                if (s == all) return;
+                clear();
+                at = 0;
             }
-            if (at == 0 && s > 0) out(tile++);
             u32x4 fa[2][MT], fb[2][NTL];
-            tb.read(lb, wave_n(), fb);
+            tb.read(la + TA::ELEMS, wave_n(), fb);
             ta.read(la, wave_m(), fa);
-            Waits::wait_lds();
+            la = la == lds + (STAGES - 1) * ELEMS ? lds : la + ELEMS;
+            if (second && !done) arrive(full);
+            else Waits::wait_lds();
             Waits::meet();
-            if (second && s + STAGES < all) load(s + STAGES);
+            if (second && s + STAGES < all) load();
             __builtin_amdgcn_s_setprio(1);
-            if (at == 0) multiply<true>(fa, fb);
-            else multiply<false>(fa, fb);
+            multiply(fa, fb);
             __builtin_amdgcn_s_setprio(0);
-            if (!second) {
-                if (full) Waits::template wait<LOADS *(STAGES - 2)>();
-                else Waits::template wait<0>();
-            }
+            if (!second) arrive(full);
             Waits::meet();
-            if (++at == steps) at = 0;
+            ++at;
         }
         if (!second) Waits::meet();
         out(tile);

@@ -41,15 +41,16 @@ struct VocabArgs {
     const float2 *rows;
     float2 *listed;
     const float *coef;    // tau g of every row (times a power of two), 0 where it has no gradient
-    void *d;              // dz of the piece: [M][ldd], columns behind the piece 0
+    void *d;              // dz of the piece: [M][ldd]
     int64_t ldd;
     float *sums;          // dx: [parts][M][K]; dW: [parts][width][K]
     void *dw;
     const float *unscale;  // what undoes dz's power of two
     int add;
-    // wide kernels: operands laid out (or as they are), columns, and what undoes the planes' powers of two (or null)
+    // wide kernels: operands laid out (or as they are), their columns and dz's with those that pad them to whole steps
+    // (dz: 0 there, and in the rows that pad it), and what undoes the planes' powers of two (or null)
     const uint16_t *x, *w;
-    int64_t ldx, ldw, cols, d_cols;
+    int64_t ldx, ldw, cols, d_cols, d_rows;
     const float *undo;     // x's, weight's
 };
 
@@ -468,44 +469,36 @@ constexpr bool is_pairs() {
 // wave's 64).
 template <typename T, int BM, int WN, int STAGES>
 struct LogitTiles {
-    using TA = WideContig<BM, 64>;
-    using TB = WideContig<WN * 64, 64>;
+    using TA = StepsContig<BM>;
+    using TB = StepsContig<WN * 64>;
     using Run = WideTiles<Half<T>, is_pairs<T>(), BM, WN, STAGES, TA, TB>;
     TA ta;
     TB tb;
-    int steps, last, at;  // of a tile's row; values of the last step; the next step's
-    int64_t row_len, n_next;
+    int steps, at;  // of a tile's row; of the next load
+    int64_t n_next;
 
     static __device__ __forceinline__ int column(int r) {
         return (r & ~63) + ((r >> 2) & 3) * 16 + ((r >> 4) & 3) * 4 + (r & 3);
     }
     __device__ __forceinline__ void aim(const VocabArgs &a) {
-        tb.init([&](int r) {
-            const int64_t n = n_next + column(r);
-            return a.w + (n < a.op.V ? n : a.op.V - 1) * a.ldw;
-        });
+        const int64_t n0 = n_next < a.op.V ? n_next : a.op.V - 1;
+        const int most = (int)(a.op.V - 1 - n0 < WN * 64 ? a.op.V - 1 - n0 : WN * 64);
+        tb.init(a.w + n0 * a.ldw, a.ldw, [&](int r) { return column(r) < most ? column(r) : most; });
     }
     __device__ __forceinline__ void init(const VocabArgs &a, int64_t row0, int64_t n0) {
-        row_len = is_pairs<T>() ? 2 * a.cols : a.cols;
-        steps = (int)((row_len + 63) / 64);
-        last = (int)(row_len - (int64_t)(steps - 1) * 64);
+        steps = (int)(a.cols / (is_pairs<T>() ? 32 : 64));
         at = 0;
         n_next = n0;
-        ta.init([&](int r) { return a.x + (row0 + r < a.op.M ? row0 + r : a.op.M - 1) * a.ldx; });
+        const int most = (int)(a.op.M - 1 - row0 < BM ? a.op.M - 1 - row0 : BM);
+        ta.init(a.x + row0 * a.ldx, a.ldx, [&](int r) { return r < most ? r : most; });
         aim(a);
     }
     __device__ __forceinline__ void feed(const VocabArgs &a, uint16_t *la, uint16_t *lb) {
-        if (at + 1 < steps || last == 64) {
-            ta.template issue<true>(la, 64);
-            tb.template issue<true>(lb, 64);
-        } else {
-            ta.template issue<false>(la, last);
-            tb.template issue<false>(lb, last);
-        }
+        ta.issue(la);
+        tb.issue(lb);
         if (++at < steps) return;
         at = 0;
-#pragma unroll
-        for (int i = 0; i < TA::LOADS; ++i) ta.p[i] -= row_len;
+        ta.base -= steps * 64;
         n_next += WN * 64;
         aim(a);
     }
@@ -516,8 +509,14 @@ struct LogitTiles {
 __device__ __forceinline__ void row_and_part(const VocabArgs &a, uint32_t *mt, uint32_t *part) {
     const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
     const uint32_t g = w / (8 * a.parts), n = a.m_tiles - 8 * g < 8 ? a.m_tiles - 8 * g : 8, l = w - g * 8 * a.parts;
-    *mt = 8 * g + l % n;
-    *part = l / n;
+    // quotients come in vector registers
+    *mt = (uint32_t)__builtin_amdgcn_readfirstlane((int)(8 * g + l % n));
+    *part = (uint32_t)__builtin_amdgcn_readfirstlane((int)(l / n));
+}
+
+// Where the part of `all` things begins.
+__device__ __forceinline__ int64_t part_begin(int64_t all, uint32_t part, uint32_t parts) {
+    return fl_uniform_i64(all * part / parts);
 }
 
 // A lane's bias for its 16 columns from n on, in units of log 2.
@@ -544,24 +543,27 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
     uint32_t mt, part;
     row_and_part(a, &mt, &part);
     const int64_t row0 = (int64_t)mt * BM, V = a.op.V;
-    const int64_t t0 = (int64_t)a.n_tiles * part / a.parts, t1 = (int64_t)a.n_tiles * (part + 1) / a.parts;
+    const int64_t t0 = part_begin(a.n_tiles, part, a.parts), t1 = part_begin(a.n_tiles, part + 1, a.parts);
     // a lane's sums over its own columns, a pair a row
-    Running *state = reinterpret_cast<Running *>(wide_lds + STAGES * Run::ELEMS) + fl_wave_id() * MT * FL_WAVE + fl_lane();
+    Running *sums = reinterpret_cast<Running *>(wide_lds + STAGES * Run::ELEMS) + fl_wave_id() * MT * FL_WAVE;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) state[i * FL_WAVE] = Running{-INFINITY, 0.0f};
+    for (int i = 0; i < MT; ++i) sums[i * FL_WAVE + fl_lane()] = Running{-INFINITY, 0.0f};
     Tiles tiles;
     tiles.init(a, row0, t0 * WN * 64);
     const float scale = a.undo ? a.undo[0] * a.undo[1] * a.scale : a.scale;
     Run run;
-    run.run(
-        tiles.ta, tiles.tb, t1 - t0, tiles.steps, wide_lds, [&](uint16_t *la, uint16_t *lb) { tiles.feed(a, la, lb); },
+    run.template run<false>(
+        tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](uint16_t *la, uint16_t *lb) { tiles.feed(a, la, lb); },
         [&](int64_t t) {
-            const int64_t n = (t0 + t) * WN * 64 + run.wave_n() + (fl_lane() >> 4) * 16;
+            const int lane = made_here(fl_lane());
+            Running *state = sums + lane;
+            const int64_t n = (t0 + t) * WN * 64 + run.wave_n() + (lane >> 4) * 16;
             const int have = V - n < 16 ? (int)(V - n) : 16;
             float b[16];
             if (a.op.bias) lane_bias<T>(a, n, b);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
+                __builtin_amdgcn_sched_barrier(0);  // a row's values at a time: few registers
                 Running r = state[i * FL_WAVE];
                 float u[16], s = 0.0f;
 #pragma unroll
@@ -593,7 +595,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
         });
     Running r[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) r[i] = state[i * FL_WAVE];
+    for (int i = 0; i < MT; ++i) r[i] = sums[i * FL_WAVE + fl_lane()];
     __syncthreads();  // the operands in the LDS are read
     store_running<BM, WN>(a, r, reinterpret_cast<Running *>(wide_lds), run.wave_m(), run.wave_n() / 64, row0, part);
 }
@@ -608,27 +610,29 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
     uint32_t mt, part;
     row_and_part(a, &mt, &part);
     const int64_t row0 = (int64_t)mt * BM, end = a.v0 + a.width;
-    const int64_t t0 = (int64_t)a.n_tiles * part / a.parts, t1 = (int64_t)a.n_tiles * (part + 1) / a.parts;
+    const int64_t t0 = part_begin(a.n_tiles, part, a.parts), t1 = part_begin(a.n_tiles, part + 1, a.parts);
     float2 *of = reinterpret_cast<float2 *>(wide_lds + STAGES * Run::ELEMS);  // (lse, coefficient) of the tile's rows
     for (int t = threadIdx.x; t < BM; t += WD_NT) {
         const int64_t m = row0 + t < a.op.M ? row0 + t : a.op.M - 1;
-        of[t] = float2{a.rows[m].x, a.coef[m]};
+        of[t] = float2{a.rows[m].x, row0 + t < a.op.M ? a.coef[m] : 0.0f};
     }
     __syncthreads();
     Tiles tiles;
     tiles.init(a, row0, a.v0 + t0 * WN * 64);
     const float scale = a.undo ? a.undo[0] * a.undo[1] * a.scale : a.scale;
     Run run;
-    run.run(
-        tiles.ta, tiles.tb, t1 - t0, tiles.steps, wide_lds, [&](uint16_t *la, uint16_t *lb) { tiles.feed(a, la, lb); },
+    run.template run<false>(
+        tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](uint16_t *la, uint16_t *lb) { tiles.feed(a, la, lb); },
         [&](int64_t t) {
-            const int64_t c = (t0 + t) * WN * 64 + run.wave_n() + (fl_lane() >> 4) * 16, n = a.v0 + c;
+            const int lane = made_here(fl_lane());
+            const int64_t c = (t0 + t) * WN * 64 + run.wave_n() + (lane >> 4) * 16, n = a.v0 + c;
             const int have = end - n < 16 ? (int)(end - n) : 16;
             float b[16];
             if (a.op.bias) lane_bias<T>(a, n, b);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const int r = run.wave_m() + i * 16 + (fl_lane() & 15);
+                __builtin_amdgcn_sched_barrier(0);
+                const int r = run.wave_m() + i * 16 + (lane & 15);
                 const float2 q = of[r];
                 float u[16];
 #pragma unroll
@@ -640,7 +644,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
                 if (__any(have < 16))
 #pragma unroll
                     for (int e = 0; e < 16; ++e) u[e] = e < have ? u[e] : 0.0f;
-                if (row0 + r >= a.op.M) continue;
+                if (row0 + r >= a.d_rows) continue;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (c + h * 8 >= a.d_cols) continue;
@@ -664,41 +668,45 @@ template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
     constexpr bool PAIRS = is_pairs<T>();
     constexpr int STEP = PAIRS ? 32 : 64;
-    using TA = WideContig<BM, 64>;
-    using TB = WideStrided<WN * 64, 64, false, PAIRS>;
+    using TA = StepsContig<BM>;
+    using TB = StepsStrided<WN * 64, PAIRS>;
     using Run = WideTiles<Half<T>, PAIRS, BM, WN, STAGES, TA, TB>;
     extern __shared__ __align__(16) uint16_t wide_lds[];
     const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x), tiles = a.m_tiles * a.n_tiles;
-    const uint32_t part = w / tiles, tile = w % tiles;
-    const int64_t row0 = (int64_t)(tile % a.m_tiles) * BM, n0 = (int64_t)(tile / a.m_tiles) * WN * 64, M = a.op.M;
-    const int64_t all = (a.width + STEP - 1) / STEP, s0 = all * part / a.parts, s1 = all * (part + 1) / a.parts;
+    const uint32_t part = (uint32_t)__builtin_amdgcn_readfirstlane((int)(w / tiles)), tile = w - part * tiles;
+    const uint32_t nt = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tile / a.m_tiles));
+    const int64_t row0 = (int64_t)(tile - nt * a.m_tiles) * BM, n0 = (int64_t)nt * WN * 64, M = a.op.M;
+    const int64_t all = (a.width + STEP - 1) / STEP;
+    const int64_t s0 = part_begin(all, part, a.parts), s1 = part_begin(all, part + 1, a.parts);
     TA ta;
     TB tb;
-    ta.init([&](int r) { return (const uint16_t *)a.d + (row0 + r < M ? row0 + r : M - 1) * a.ldd + s0 * 64; });
-    tb.init(a.w + (a.v0 + s0 * STEP) * a.ldw + (PAIRS ? 2 * n0 : n0), a.ldw, a.cols - n0);
-    int64_t left = (s1 == all ? a.width : s1 * STEP) - s0 * STEP;
+    const int most = (int)(M - 1 - row0 < BM ? M - 1 - row0 : BM);
+    ta.init((const uint16_t *)a.d + row0 * a.ldd + s0 * 64, a.ldd, [&](int r) { return r < most ? r : most; });
+    const auto aim = [&](int64_t step) {
+        const int64_t left = a.width - step * STEP;
+        tb.init(a.w + (a.v0 + step * STEP) * a.ldw + (PAIRS ? 2 * n0 : n0), a.ldw, a.cols - n0,
+                left < STEP ? (int)left : STEP);
+    };
+    int64_t next = s0;
+    aim(s0);
     Run run;
-    run.run(
+    run.template run<true>(
         ta, tb, 1, (int)(s1 - s0), wide_lds,
         [&](uint16_t *la, uint16_t *lb) {
-            if (left >= STEP) {
-                ta.template issue<true>(la, 64);
-                tb.template issue<true>(lb, STEP, {});
-            } else {  // the columns behind the piece are 0
-                if (PAIRS) ta.template issue<true>(la, 64);
-                else ta.template issue<false>(la, (int)left);
-                tb.template issue<false>(lb, (int)left, {});
-            }
-            left -= STEP;
+            ta.issue(la);
+            tb.issue(lb);
+            if (++next == all - 1) aim(next);  // dz is 0 behind the piece
         },
         [&](int64_t) {
+            const int lane = made_here(fl_lane());
 #pragma unroll
             for (int i = 0; i < Run::MT; ++i) {
-                const int64_t row = row0 + run.wave_m() + i * 16 + (fl_lane() & 15);
+                __builtin_amdgcn_sched_barrier(0);
+                const int64_t row = row0 + run.wave_m() + i * 16 + (lane & 15);
                 if (row >= M) continue;
 #pragma unroll
                 for (int j = 0; j < Run::NTL; ++j) {
-                    const int64_t n = n0 + run.wave_n() + j * 16 + (fl_lane() >> 4) * 4;
+                    const int64_t n = n0 + run.wave_n() + j * 16 + (lane >> 4) * 4;
                     if (n >= a.op.K) continue;
                     const int have = a.op.K - n < 4 ? (int)(a.op.K - n) : 4;
                     float *q = a.sums + ((int64_t)part * M + row) * a.op.K + n;
@@ -721,50 +729,57 @@ template <typename T, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
     constexpr bool PAIRS = is_pairs<T>();
     constexpr int STEP = PAIRS ? 32 : 64, BM = 256;
-    using TA = WideStrided<BM, 64, false, PAIRS>;
-    using TB = WideStrided<WN * 64, 64, false, PAIRS>;
+    using TA = StepsStrided<BM, PAIRS>;
+    using TB = StepsStrided<WN * 64, PAIRS>;
     using Run = WideTiles<Half<T>, PAIRS, BM, WN, STAGES, TA, TB>;
     extern __shared__ __align__(16) uint16_t wide_lds[];
-    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x), walks = gridDim.x / a.parts;
-    const uint32_t part = w / walks, walk = w % walks;
-    const int64_t all = (int64_t)a.m_tiles * a.n_tiles, t0 = all * walk / walks, t1 = all * (walk + 1) / walks;
-    const int64_t begin = a.op.M * part / a.parts, len = a.op.M * (part + 1) / a.parts - begin;
-    const int steps = (int)((len + STEP - 1) / STEP);
+    const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
+    const uint32_t walks = (uint32_t)__builtin_amdgcn_readfirstlane((int)(gridDim.x / a.parts));
+    const uint32_t part = (uint32_t)__builtin_amdgcn_readfirstlane((int)(w / walks)), walk = w - part * walks;
+    const int64_t all = (int64_t)a.m_tiles * a.n_tiles;
+    const int64_t t0 = part_begin(all, walk, walks), t1 = part_begin(all, walk + 1, walks);
+    const int64_t rows = (a.op.M + STEP - 1) / STEP, s0 = part_begin(rows, part, a.parts);
+    const int steps = (int)(part_begin(rows, part + 1, a.parts) - s0);
     TA ta;
     TB tb;
-    int64_t next = t0, left = len;
-    const auto aim = [&]() {
-        const int64_t m0 = next / a.n_tiles * BM, c0 = next % a.n_tiles * (WN * 64);
-        ta.init((const uint16_t *)a.d + begin * a.ldd + (PAIRS ? 2 * m0 : m0), a.ldd, a.d_cols - m0);
-        tb.init(a.x + begin * a.ldx + (PAIRS ? 2 * c0 : c0), a.ldx, a.cols - c0);
+    int64_t next = t0, m0, c0;
+    int at = 0;
+    const auto aim = [&](int step) {  // dz is 0 in the rows behind the last
+        const int64_t k = (s0 + step) * STEP, left = a.op.M - k;
+        ta.init((const uint16_t *)a.d + k * a.ldd + (PAIRS ? 2 * m0 : m0), a.ldd, a.d_cols - m0, STEP);
+        tb.init(a.x + k * a.ldx + (PAIRS ? 2 * c0 : c0), a.ldx, a.cols - c0, left < STEP ? (int)left : STEP);
     };
-    aim();
+    const auto aim_tile = [&]() {
+        const int64_t mt = fl_uniform_i64(next / a.n_tiles);
+        m0 = mt * BM;
+        c0 = (next - mt * a.n_tiles) * (WN * 64);
+        aim(0);
+    };
+    aim_tile();
     const float f = a.sums ? 1.0f : *a.unscale, f2 = a.sums || !a.undo ? 1.0f : a.undo[0];
     Run run;
-    run.run(
-        ta, tb, t1 - t0, steps, wide_lds,
+    run.template run<false>(
+        ta, tb, (int)(t1 - t0), steps, wide_lds,
         [&](uint16_t *la, uint16_t *lb) {
-            if (left >= STEP) {
-                ta.template issue<true>(la, STEP, {});
-                tb.template issue<true>(lb, STEP, {});
-            } else {
-                ta.template issue<false>(la, (int)left, {});
-                tb.template issue<false>(lb, (int)left, {});
-            }
-            left -= STEP;
-            if (left > 0) return;
-            left = len;
-            if (++next < t1) aim();
+            ta.issue(la);
+            tb.issue(lb);
+            if (++at == steps) {
+                at = 0;
+                if (++next < t1) aim_tile();
+            } else if (s0 + at == rows - 1 && a.op.M % STEP) aim(at);
         },
         [&](int64_t t) {
-            const int64_t m0 = (t0 + t) / a.n_tiles * BM, c0 = (t0 + t) % a.n_tiles * (WN * 64);
+            const int lane = made_here(fl_lane());
+            const int64_t mt = fl_uniform_i64((t0 + t) / a.n_tiles), m0 = mt * BM;
+            const int64_t c0 = (t0 + t - mt * a.n_tiles) * (WN * 64);
 #pragma unroll
             for (int i = 0; i < Run::MT; ++i) {
-                const int64_t m = m0 + run.wave_m() + i * 16 + (fl_lane() & 15);
+                __builtin_amdgcn_sched_barrier(0);
+                const int64_t m = m0 + run.wave_m() + i * 16 + (lane & 15);
                 if (m >= a.width) continue;
 #pragma unroll
                 for (int j = 0; j < Run::NTL; ++j) {
-                    const int64_t c = c0 + run.wave_n() + j * 16 + (fl_lane() >> 4) * 4;
+                    const int64_t c = c0 + run.wave_n() + j * 16 + (lane >> 4) * 4;
                     if (c >= a.op.K) continue;
                     const int n = a.op.K - c < 4 ? (int)(a.op.K - c) : 4;
                     if (a.sums) {
@@ -794,7 +809,7 @@ struct VocabPlan {
     int bm, bn;                        // tiles of the logits
     uint32_t m_tiles, n_tiles, parts;  // parts: of the vocabulary, in the forward
     int64_t piece, d_cols, ldd;        // columns of dz in the backward, with those that pad them, and its row stride
-    int64_t cols;                      // wide: inputs, with those that pad them
+    int64_t d_rows, cols;              // rows of dz and inputs, with those that pad them
     int64_t size;                      // bytes of a value of dz
 };
 
@@ -803,9 +818,11 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     p.pairs = op->dtype == FL_F32;
     p.wide = op->K >= 1 && op->K <= 1 << 20 && (double)op->M * op->V * op->K >= 1 << 27;
     p.size = p.pairs ? 4 : 2;
+    const int64_t step = p.pairs ? 32 : 64;  // values of a step of the wide kernels
     if (p.wide) {
-        p.lay = p.pairs || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % 8;
-        p.cols = p.pairs ? ceil_div(op->K, 32) * 32 : ceil_div(op->K, 8) * 8;
+        p.lay = p.pairs || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % 64 || op->ldx >= 1 << 23 ||
+                op->ldw >= 1 << 23;  // 32-bit offsets of 256 rows
+        p.cols = ceil_div(op->K, step) * step;
         const bool small = ceil_div(op->M, 256) * ceil_div(op->V, 256) < 192;
         p.bm = small ? 128 : 256;
         p.bn = small ? 128 : 256;
@@ -819,9 +836,10 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     p.parts = (uint32_t)(want < p.n_tiles ? want : p.n_tiles);
     int64_t piece = (int64_t)(LS_PIECE / p.size) / (op->M > 0 ? op->M : 1) / 256 * 256;
     if (piece < 256) piece = 256;
-    if (piece > 1 << 22) piece = 1 << 22;  // 32-bit offsets of 64 rows of dz
+    if (piece > 1 << 21) piece = 1 << 21;  // 32-bit offsets of 256 rows of dz
     p.piece = piece < op->V ? piece : op->V;
-    p.d_cols = p.wide && p.pairs ? ceil_div(p.piece, 32) * 32 : ceil_div(p.piece, 8) * 8;
+    p.d_cols = p.wide ? ceil_div(p.piece, step) * step : ceil_div(p.piece, 8) * 8;
+    p.d_rows = p.wide ? ceil_div(op->M, step) * step : op->M;
     p.ldd = p.wide && p.pairs ? 2 * p.d_cols : p.d_cols;
     return p;
 }
@@ -857,7 +875,7 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
     };
     const bool f32 = op->dtype == FL_F32;
     s.coef = take((size_t)(op->M + 1) * 4);
-    s.d = take((size_t)op->M * p.ldd * (p.wide ? 2 : p.size));
+    s.d = take((size_t)p.d_rows * p.ldd * (p.wide ? 2 : p.size));
     const int narrow = op->K <= 128 ? 128 : 256;
     if (with_dx) {
         if (p.wide) {
@@ -970,6 +988,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
     a.d = ws + s.d;
     a.ldd = p.ldd;
     a.d_cols = p.d_cols;
+    a.d_rows = p.d_rows;
     const dim3 nt(LN_NT), wt(WD_NT);
     const auto fits = [&](int64_t grid) { return launch_fits(grid, WD_NT); };
     const auto fail = [&]() { return fl_fail(FL_ERR_ARG, "linear_loss: too many tiles for one launch (shape)"); };
