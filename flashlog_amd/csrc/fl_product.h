@@ -428,15 +428,17 @@ struct StepsContig {
             at[i] = (uint32_t)row_at(r) * (uint32_t)(ld * 2) + lds_at<64>(r, lane % 8) % 64 * 2;
         }
     }
-    __device__ __forceinline__ void issue(uint16_t *lds) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            load_lds((const char *)base + at[i], lds + (fl_wave_id() * LOADS + i) * 512);
-        base += 64;
+    __device__ __forceinline__ void issue(uint16_t *lds, int i) {
+        load_lds((const char *)base + at[i], lds + (fl_wave_id() * LOADS + i) * 512);
     }
-    template <int N>
-    __device__ __forceinline__ void read(const uint16_t *lds, int row0, u32x4 (&f)[2][N]) const {
-        At().read(lds, row0, f);
+    __device__ __forceinline__ void next() { base += 64; }
+    // The operands of N 16-row tiles from row0 on, of the step's first or second 32 values.
+    template <int KS, int N>
+    __device__ __forceinline__ void read(const uint16_t *lds, int row0, u32x4 (&f)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            f[i] = *reinterpret_cast<const u32x4 *>(
+                lds + lds_at<64>(row0 + i * 16 + (fl_lane() & 15), KS * 4 + (fl_lane() >> 4)));
     }
 };
 
@@ -560,15 +562,56 @@ struct StepsStrided {
                     (uint32_t)(k < rows ? k : rows - 1) * (uint32_t)(stride * 2);
         }
     }
-    __device__ __forceinline__ void issue(uint16_t *lds) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            load_lds((const char *)base + at[i], lds + (fl_wave_id() * LOADS + i) * 512);
-        base += STEP * ld;
+    __device__ __forceinline__ void issue(uint16_t *lds, int i) {
+        load_lds((const char *)base + at[i], lds + (fl_wave_id() * LOADS + i) * 512);
     }
-    template <int N>
-    __device__ __forceinline__ void read(const uint16_t *lds, int col0, u32x4 (&f)[2][N]) const {
-        At().read(lds, col0, f);
+    __device__ __forceinline__ void next() { base += STEP * ld; }
+    // Of N 16-column tiles from col0 on, of the step's first or second 32 rows.  In
+    // asm, with the wait, as WideStrided's.
+    template <int KS, int N>
+    __device__ __forceinline__ void read(const uint16_t *lds, int col0, u32x4 (&f)[N]) const {
+        static_assert(N == 2 || N % 4 == 0, "two or four tiles a block");
+        const int s = fl_lane() & 15, k = (fl_lane() >> 4) * 8 + (s >> 2);
+        const uint32_t from =
+            (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t *)lds + k * (BR * 2) + (s & 1) * 8;
+        constexpr int LO = KS * 32 * BR * 2, HI = LO + 4 * BR * 2;
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            uint32_t a[4];
+            uint64_t v[4][2];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                a[t] = from + ((((col0 >> 3) + (i + t) * 2 + ((s & 3) >> 1)) ^ At::turn(k)) << 4);
+            if constexpr (N == 2)
+                asm volatile(
+                    "ds_read_b64_tr_b16 %0, %4 offset:%6\n"
+                    "ds_read_b64_tr_b16 %1, %4 offset:%7\n"
+                    "ds_read_b64_tr_b16 %2, %5 offset:%6\n"
+                    "ds_read_b64_tr_b16 %3, %5 offset:%7\n"
+                    "s_waitcnt lgkmcnt(0)"
+                    : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
+                    : "v"(a[0]), "v"(a[1]), "n"(LO), "n"(HI)
+                    : "memory");
+            else
+                asm volatile(
+                    "ds_read_b64_tr_b16 %0, %8 offset:%12\n"
+                    "ds_read_b64_tr_b16 %1, %8 offset:%13\n"
+                    "ds_read_b64_tr_b16 %2, %9 offset:%12\n"
+                    "ds_read_b64_tr_b16 %3, %9 offset:%13\n"
+                    "ds_read_b64_tr_b16 %4, %10 offset:%12\n"
+                    "ds_read_b64_tr_b16 %5, %10 offset:%13\n"
+                    "ds_read_b64_tr_b16 %6, %11 offset:%12\n"
+                    "ds_read_b64_tr_b16 %7, %11 offset:%13\n"
+                    "s_waitcnt lgkmcnt(0)"
+                    : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]),
+                      "=&v"(v[3][0]), "=&v"(v[3][1])
+                    : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(LO), "n"(HI)
+                    : "memory");
+#pragma unroll
+            for (int t = 0; t < (N < 4 ? N : 4); ++t)
+                f[i + t] = u32x4{(uint32_t)v[t][0], (uint32_t)(v[t][0] >> 32), (uint32_t)v[t][1],
+                                 (uint32_t)(v[t][1] >> 32)};
+        }
     }
 };
 
@@ -679,12 +722,20 @@ struct WideProduct {
 };
 
 // Tiles one after the other as one sequence of steps, `steps` a tile: the loads
-// run ahead over the tiles' ends, and a half of the waves takes a tile's sums
-// out (out(tile)) while the other half still multiplies.  Tiles of BM rows and
-// WN x 64 columns, a step of 64 values (PAIRS: 32 of both planes).  The halves
-// take turns as in WideProduct.
+// run ahead over the tiles' ends.  Tiles of BM rows and WN x 64 columns, a step of
+// 64 values (PAIRS: 32 of both planes).
 //
-// feed(lds_a, lds_b) issues the loads of the next step.
+// A step's operands come in two halves (of its values; PAIRS: the planes), and
+// one is read from LDS while the other is multiplied; a barrier a step, between
+// the halves, says that the step is read by all and the next one there, whose
+// first half is read beside the second products.  Loads of a later step are issued
+// one at a time between those.  (Read and multiplied in turns, by half the waves
+// each or by all together, the matrix unit was busy 46% of the time, whatever the
+// tile: 128 x 128, fp32 [1536 x 2048 -> 1645] 52 and 50 us.)
+//
+// feed(i, lds_a, lds_b) issues load i of the next step, and after the last one
+// goes on to the step behind it; behind the last step it may load anything that
+// can be read.  out(tile) takes a tile's sums.
 template <typename T, bool PAIRS, int BM, int WN, int STAGES, typename TA, typename TB>
 struct WideTiles {
     static constexpr int WM = WD_WAVES / WN, MT = BM / WM / 16, NTL = 4, BN = WN * 64;
@@ -701,16 +752,19 @@ struct WideTiles {
 #pragma unroll
             for (int j = 0; j < NTL; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
     }
-    __device__ __forceinline__ void multiply(const u32x4 (&fa)[2][MT], const u32x4 (&fb)[2][NTL]) {
+    // between(i) comes behind the i-th of LOADS equal parts.
+    template <typename F>
+    __device__ __forceinline__ void multiply(const u32x4 (&fa)[MT], const u32x4 (&fb)[NTL], F &&between) {
+        constexpr int ALL = MT * NTL, EACH = ALL / LOADS;
+        static_assert(EACH >= 1, "a load between matrix instructions");
 #pragma unroll
-        for (int p = 0; p < (PAIRS ? 3 : 2); ++p)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NTL; ++j) {
-                    const int ka = PAIRS ? p == 1 : p, kb = PAIRS ? p == 0 : p;
-                    acc[i][j] = mfma<T>(fb[kb][j], fa[ka][i], acc[i][j]);
-                }
+            for (int j = 0; j < NTL; ++j) {
+                acc[i][j] = mfma<T>(fb[j], fa[i], acc[i][j]);
+                const int n = i * NTL + j + 1;
+                if (n % EACH == 0 && n / EACH <= LOADS) between(n / EACH - 1);
+            }
     }
 
     // ONE: a single tile.
@@ -723,53 +777,58 @@ struct WideTiles {
             for (int t = 0; t < tiles; ++t) out(t);
             return;
         }
-        const bool second = fl_wave_id() >= WD_WAVES / 2;
         uint16_t *to = lds;
-        const auto load = [&]() {
-            feed(to, to + TA::ELEMS);
-            to = to == lds + (STAGES - 1) * ELEMS ? lds : to + ELEMS;
+        const auto load = [&](int i) {
+            feed(i, to, to + TA::ELEMS);
+            if (i == LOADS - 1) to = to == lds + (STAGES - 1) * ELEMS ? lds : to + ELEMS;
         };
-        const auto arrive = [&](bool full) {  // the next step's loads have
-            if (full) Waits::template wait<LOADS *(STAGES - 2)>();
-            else Waits::template wait<0>();
+        const auto load_between = [&](int i) {
+            __builtin_amdgcn_sched_barrier(0);
+            load(i);
         };
+        const auto none = [](int) {};
 #pragma unroll
         for (int s = 0; s < STAGES; ++s)
-            if (s < all) load();
-        if (all < STAGES) Waits::template wait<0>();
-        else Waits::template wait<LOADS *(STAGES - 1)>();
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) load(i);
+        Waits::template wait<LOADS *(STAGES - 1)>();
         Waits::meet();
-        if (second) Waits::meet();
         const uint16_t *la = lds;
         int at = 0, tile = 0;
-        for (int s = 0; !ONE || s < all; ++s) {
-            const bool full = s + STAGES - 1 < all, done = !ONE && at == steps;
-            if (!second && s > 0 && full) load();
-            if (done) {
-                if (s == all && !second) Waits::meet();
-                if (second && s < all) arrive(full);  // before out's stores are under way
+        u32x4 a0[MT], b0[NTL];
+        ta.template read<0>(la, wave_m(), a0);
+        tb.template read<0>(la + TA::ELEMS, wave_n(), b0);
+        for (int s = 0; s < all; ++s) {
+            u32x4 a1[MT], b1[NTL];
+            tb.template read<1>(la + TA::ELEMS, wave_n(), b1);
+            ta.template read<1>(la, wave_m(), a1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(a0, b0, none);
+            __builtin_amdgcn_sched_barrier(0);
+            Waits::template wait<LOADS *(STAGES - 2)>();
+            Waits::meet();
+            la = la == lds + (STAGES - 1) * ELEMS ? lds : la + ELEMS;
+            if constexpr (PAIRS) {
+                multiply(a0, b1, load_between);
+                __builtin_amdgcn_sched_barrier(0);
+                ta.template read<0>(la, wave_m(), a0);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(a1, b0, none);
+                tb.template read<0>(la + TA::ELEMS, wave_n(), b0);
+            } else {
+                tb.template read<0>(la + TA::ELEMS, wave_n(), b0);
+                ta.template read<0>(la, wave_m(), a0);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(a1, b1, load_between);
+            }
+            if (!ONE && ++at == steps) {
                 out(tile++);
-                if (s == all) return;
                 clear();
                 at = 0;
             }
-            u32x4 fa[2][MT], fb[2][NTL];
-            tb.read(la + TA::ELEMS, wave_n(), fb);
-            ta.read(la, wave_m(), fa);
-            la = la == lds + (STAGES - 1) * ELEMS ? lds : la + ELEMS;
-            if (second && !done) arrive(full);
-            else Waits::wait_lds();
-            Waits::meet();
-            if (second && s + STAGES < all) load();
-            __builtin_amdgcn_s_setprio(1);
-            multiply(fa, fb);
-            __builtin_amdgcn_s_setprio(0);
-            if (!second) arrive(full);
-            Waits::meet();
-            ++at;
         }
-        if (!second) Waits::meet();
-        out(tile);
+        Waits::template wait<0>();  // loads behind the last step
+        if (ONE) out(0);
     }
 };
 

@@ -45,6 +45,7 @@ struct VocabArgs {
     int64_t ldd;
     float *sums;          // dx: [parts][M][K]; dW: [parts][width][K]
     void *dw;
+    void *dx;             // where one part and one piece are all of it
     const float *unscale;  // what undoes dz's power of two
     int add;
     // wide kernels: operands laid out (or as they are), their columns and dz's with those that pad them to whole steps
@@ -493,9 +494,12 @@ struct LogitTiles {
         ta.init(a.x + row0 * a.ldx, a.ldx, [&](int r) { return r < most ? r : most; });
         aim(a);
     }
-    __device__ __forceinline__ void feed(const VocabArgs &a, uint16_t *la, uint16_t *lb) {
-        ta.issue(la);
-        tb.issue(lb);
+    __device__ __forceinline__ void feed(const VocabArgs &a, int i, uint16_t *la, uint16_t *lb) {
+        if (i < TA::LOADS) ta.issue(la, i);
+        else tb.issue(lb, i - TA::LOADS);
+        if (i < TA::LOADS + TB::LOADS - 1) return;
+        ta.next();
+        tb.next();
         if (++at < steps) return;
         at = 0;
         ta.base -= steps * 64;
@@ -553,7 +557,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
     const float scale = a.undo ? a.undo[0] * a.undo[1] * a.scale : a.scale;
     Run run;
     run.template run<false>(
-        tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](uint16_t *la, uint16_t *lb) { tiles.feed(a, la, lb); },
+        tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](int i, uint16_t *la, uint16_t *lb) { tiles.feed(a, i, la, lb); },
         [&](int64_t t) {
             const int lane = made_here(fl_lane());
             Running *state = sums + lane;
@@ -622,7 +626,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
     const float scale = a.undo ? a.undo[0] * a.undo[1] * a.scale : a.scale;
     Run run;
     run.template run<false>(
-        tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](uint16_t *la, uint16_t *lb) { tiles.feed(a, la, lb); },
+        tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](int i, uint16_t *la, uint16_t *lb) { tiles.feed(a, i, la, lb); },
         [&](int64_t t) {
             const int lane = made_here(fl_lane());
             const int64_t c = (t0 + t) * WN * 64 + run.wave_n() + (lane >> 4) * 16, n = a.v0 + c;
@@ -682,20 +686,23 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
     TB tb;
     const int most = (int)(M - 1 - row0 < BM ? M - 1 - row0 : BM);
     ta.init((const uint16_t *)a.d + row0 * a.ldd + s0 * 64, a.ldd, [&](int r) { return r < most ? r : most; });
-    const auto aim = [&](int64_t step) {
-        const int64_t left = a.width - step * STEP;
-        tb.init(a.w + (a.v0 + step * STEP) * a.ldw + (PAIRS ? 2 * n0 : n0), a.ldw, a.cols - n0,
-                left < STEP ? (int)left : STEP);
+    const auto aim = [&](int64_t step) {  // dz is 0 behind the piece
+        const int64_t v = step * STEP, left = a.width - v;
+        tb.init(a.w + (a.v0 + v) * a.ldw + (PAIRS ? 2 * n0 : n0), a.ldw, a.cols - n0, left < STEP ? (int)left : STEP);
     };
     int64_t next = s0;
-    aim(s0);
+    aim(next);
+    const float f1 = a.dx ? *a.unscale : 1.0f, f2 = a.dx && a.undo ? a.undo[1] : 1.0f;
     Run run;
     run.template run<true>(
         ta, tb, 1, (int)(s1 - s0), wide_lds,
-        [&](uint16_t *la, uint16_t *lb) {
-            ta.issue(la);
-            tb.issue(lb);
-            if (++next == all - 1) aim(next);  // dz is 0 behind the piece
+        [&](int i, uint16_t *la, uint16_t *lb) {
+            if (i < TA::LOADS) ta.issue(la, i);
+            else tb.issue(lb, i - TA::LOADS);
+            if (i < Run::LOADS - 1 || ++next >= s1) return;
+            ta.next();
+            tb.next();
+            if (next == all - 1) aim(next);
         },
         [&](int64_t) {
             const int lane = made_here(fl_lane());
@@ -709,6 +716,15 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
                     const int64_t n = n0 + run.wave_n() + j * 16 + (lane >> 4) * 4;
                     if (n >= a.op.K) continue;
                     const int have = a.op.K - n < 4 ? (int)(a.op.K - n) : 4;
+                    if (a.dx) {
+                        Vec<T, 4> o;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o.v[e] = (T)(run.acc[i][j][e] * f1 * f2);
+                        T *q = (T *)a.dx + row * a.op.K + n;
+                        if (have == 4) store_vec<T, 4>(q, o);
+                        else store_some<T, 4>(q, o, have);
+                        continue;
+                    }
                     float *q = a.sums + ((int64_t)part * M + row) * a.op.K + n;
                     Vec<float, 4> f{{run.acc[i][j][0], run.acc[i][j][1], run.acc[i][j][2], run.acc[i][j][3]}};
                     if (a.add) {
@@ -725,10 +741,10 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
 }
 
 // A piece's rows of dW, or of a part of the rows' sum: tiles in a row.
-template <typename T, int WN, int STAGES>
+template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
     constexpr bool PAIRS = is_pairs<T>();
-    constexpr int STEP = PAIRS ? 32 : 64, BM = 256;
+    constexpr int STEP = PAIRS ? 32 : 64;
     using TA = StepsStrided<BM, PAIRS>;
     using TB = StepsStrided<WN * 64, PAIRS>;
     using Run = WideTiles<Half<T>, PAIRS, BM, WN, STAGES, TA, TB>;
@@ -738,14 +754,15 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
     const uint32_t part = (uint32_t)__builtin_amdgcn_readfirstlane((int)(w / walks)), walk = w - part * walks;
     const int64_t all = (int64_t)a.m_tiles * a.n_tiles;
     const int64_t t0 = part_begin(all, walk, walks), t1 = part_begin(all, walk + 1, walks);
-    const int64_t rows = (a.op.M + STEP - 1) / STEP, s0 = part_begin(rows, part, a.parts);
+    const int64_t rows = (a.op.M + STEP - 1) / STEP;
+    const int64_t s0 = part_begin(rows, part, a.parts);
     const int steps = (int)(part_begin(rows, part + 1, a.parts) - s0);
     TA ta;
     TB tb;
     int64_t next = t0, m0, c0;
     int at = 0;
-    const auto aim = [&](int step) {  // dz is 0 in the rows behind the last
-        const int64_t k = (s0 + step) * STEP, left = a.op.M - k;
+    const auto aim = [&](int64_t step) {  // dz is 0 in the rows behind the last
+        const int64_t k = step * STEP, left = a.op.M - k;
         ta.init((const uint16_t *)a.d + k * a.ldd + (PAIRS ? 2 * m0 : m0), a.ldd, a.d_cols - m0, STEP);
         tb.init(a.x + k * a.ldx + (PAIRS ? 2 * c0 : c0), a.ldx, a.cols - c0, left < STEP ? (int)left : STEP);
     };
@@ -753,20 +770,25 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
         const int64_t mt = fl_uniform_i64(next / a.n_tiles);
         m0 = mt * BM;
         c0 = (next - mt * a.n_tiles) * (WN * 64);
-        aim(0);
+        aim(s0);
     };
     aim_tile();
     const float f = a.sums ? 1.0f : *a.unscale, f2 = a.sums || !a.undo ? 1.0f : a.undo[0];
     Run run;
     run.template run<false>(
         ta, tb, (int)(t1 - t0), steps, wide_lds,
-        [&](uint16_t *la, uint16_t *lb) {
-            ta.issue(la);
-            tb.issue(lb);
+        [&](int i, uint16_t *la, uint16_t *lb) {
+            if (i < TA::LOADS) ta.issue(la, i);
+            else tb.issue(lb, i - TA::LOADS);
+            if (i < Run::LOADS - 1 || next >= t1) return;
             if (++at == steps) {
                 at = 0;
                 if (++next < t1) aim_tile();
-            } else if (s0 + at == rows - 1 && a.op.M % STEP) aim(at);
+                return;
+            }
+            ta.next();
+            tb.next();
+            if (s0 + at == rows - 1 && a.op.M % STEP) aim(s0 + at);
         },
         [&](int64_t t) {
             const int lane = made_here(fl_lane());
@@ -806,6 +828,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
 // How the products of a vocabulary are cut.
 struct VocabPlan {
     bool wide, pairs, lay;             // wide kernels; two planes; operands laid out
+    bool small;                        // tiles of 128
     int bm, bn;                        // tiles of the logits
     uint32_t m_tiles, n_tiles, parts;  // parts: of the vocabulary, in the forward
     int64_t piece, d_cols, ldd;        // columns of dz in the backward, with those that pad them, and its row stride
@@ -818,14 +841,14 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     p.pairs = op->dtype == FL_F32;
     p.wide = op->K >= 1 && op->K <= 1 << 20 && (double)op->M * op->V * op->K >= 1 << 27;
     p.size = p.pairs ? 4 : 2;
-    const int64_t step = p.pairs ? 32 : 64;  // values of a step of the wide kernels
+    const int64_t step = p.pairs ? 32 : 64;  // inputs of a step of the wide kernels
     if (p.wide) {
-        p.lay = p.pairs || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % 64 || op->ldx >= 1 << 23 ||
+        p.small = ceil_div(op->M, 256) * ceil_div(op->V, 256) < 192;
+        p.lay = p.pairs || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % step || op->ldx >= 1 << 23 ||
                 op->ldw >= 1 << 23;  // 32-bit offsets of 256 rows
         p.cols = ceil_div(op->K, step) * step;
-        const bool small = ceil_div(op->M, 256) * ceil_div(op->V, 256) < 192;
-        p.bm = small ? 128 : 256;
-        p.bn = small ? 128 : 256;
+        p.bm = p.small ? 128 : 256;
+        p.bn = p.small || p.pairs ? 128 : 256;  // two planes of 256 x 256 have no registers
     } else {
         p.bm = op->M > 64 ? 128 : 64;
         p.bn = p.bm;
@@ -863,6 +886,7 @@ struct VocabSpace {
     size_t coef, d, dx, dw, db, bytes;
     int dx_parts, dw_parts, db_parts;
     int dx_tile, dx_cols, dw_cols, dw_tile;
+    bool dx_direct;
     uint32_t dw_walks;
 };
 
@@ -876,26 +900,28 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
     const bool f32 = op->dtype == FL_F32;
     s.coef = take((size_t)(op->M + 1) * 4);
     s.d = take((size_t)p.d_rows * p.ldd * (p.wide ? 2 : p.size));
-    const int narrow = op->K <= 128 ? 128 : 256;
+    const int narrow = op->K <= 128 || p.pairs ? 128 : 256;
     if (with_dx) {
         if (p.wide) {
-            s.dx_tile = ceil_div(op->M, 256) * ceil_div(op->K, narrow) < 16 ? 128 : 256;
+            s.dx_tile = p.small || ceil_div(op->M, 256) * ceil_div(op->K, narrow) < 16 ? 128 : 256;
             s.dx_cols = s.dx_tile == 128 ? 128 : narrow;
             const int64_t tiles = ceil_div(op->M, s.dx_tile) * ceil_div(op->K, s.dx_cols);
             const int64_t want = 256 / tiles, most = p.piece / 256;
             const int64_t n = want < most ? want : most;
-            s.dx_parts = (int)(n < 1 ? 1 : n > 32 ? 32 : n);
+            s.dx_parts = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
         } else {
             const Cut c = best_cut(op->M, op->K, p.piece, f32, false);
             s.dx_parts = c.parts;
             s.dx_tile = c.rows == 128 && op->K >= 2 ? 128 : 64;
         }
-        s.dx = take((size_t)s.dx_parts * op->M * op->K * 4);
+        s.dx_direct = p.wide && s.dx_parts == 1 && p.piece == op->V;
+        if (!s.dx_direct) s.dx = take((size_t)s.dx_parts * op->M * op->K * 4);
     }
     if (with_dw) {
         if (p.wide) {
-            s.dw_cols = narrow;
-            const int64_t tiles = ceil_div(p.piece, 256) * ceil_div(op->K, narrow), want = 256 / tiles, most = op->M / 256;
+            s.dw_tile = p.small ? 128 : 256;
+            s.dw_cols = p.small ? 128 : narrow;
+            const int64_t tiles = ceil_div(p.piece, s.dw_tile) * ceil_div(op->K, s.dw_cols), want = 256 / tiles, most = op->M / 256;
             const int64_t n = want < most ? want : most;
             s.dw_parts = (int)(n < 1 ? 1 : n > 16 ? 16 : n);
             s.dw_walks = (uint32_t)(tiles < 256 ? tiles : 256);
@@ -964,11 +990,13 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
         FL_LAUNCH("k_vocab_dots", k_vocab_dots<T>,
                   grid_of(ceil_div(op->M * ceil_div(op->lists.k, DOT_IDS), LS_WAVES)), dim3(LS_NT), 0, st, a);
     if (p.wide) {
-        const auto extra = [](int, int mt) { return (unsigned)(WD_WAVES * mt * FL_WAVE * sizeof(Running)); };
-        if (p.bm == 256)
-            FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 256, 4, 2>), g, dim3(WD_NT), tiles_bytes(256, 256, 2) + extra(256, 8), st, a);
+        const auto extra = [](int mt) { return (unsigned)(WD_WAVES * mt * FL_WAVE * sizeof(Running)); };
+        if (p.bm == 128)
+            FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 128, 2, 4>), g, dim3(WD_NT), tiles_bytes(128, 128, 4) + extra(2), st, a);
+        else if constexpr (is_pairs<T>())
+            FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 256, 2, 3>), g, dim3(WD_NT), tiles_bytes(256, 128, 3) + extra(4), st, a);
         else
-            FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 128, 2, 4>), g, dim3(WD_NT), tiles_bytes(128, 128, 4) + extra(128, 2), st, a);
+            FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 256, 4, 2>), g, dim3(WD_NT), tiles_bytes(256, 256, 2) + extra(8), st, a);
     } else if (p.bm == 128)
         FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 128, 128, BK>), g, dim3(LN_NT), 0, st, a);
     else FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 64, 64, BK>), g, dim3(LN_NT), 0, st, a);
@@ -1010,10 +1038,13 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
         if (!fits(grid)) return fail();
         if (p.wide) {
             const auto extra = [](int bm) { return (unsigned)(bm * sizeof(float2)); };
-            if (p.bm == 256)
-                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 256, 4, 2>), dim3((unsigned)grid), wt, tiles_bytes(256, 256, 2) + extra(256), st, a);
+            const dim3 g((unsigned)grid);
+            if (p.bm == 128)
+                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 128, 2, 4>), g, wt, tiles_bytes(128, 128, 4) + extra(128), st, a);
+            else if constexpr (is_pairs<T>())
+                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 256, 2, 3>), g, wt, tiles_bytes(256, 128, 3) + extra(256), st, a);
             else
-                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 128, 2, 4>), dim3((unsigned)grid), wt, tiles_bytes(128, 128, 4) + extra(128), st, a);
+                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 256, 4, 2>), g, wt, tiles_bytes(256, 256, 2) + extra(256), st, a);
         } else if (p.bm == 128)
             FL_LAUNCH("k_vocab_grad", (k_vocab_grad<T, 128, 128, BK>), dim3((unsigned)grid), nt, 0, st, a);
         else FL_LAUNCH("k_vocab_grad", (k_vocab_grad<T, 64, 64, BK>), dim3((unsigned)grid), nt, 0, st, a);
@@ -1027,6 +1058,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             a.n_tiles = (uint32_t)ceil_div(op->K, p.wide ? s.dx_cols : s.dx_tile);
             a.parts = (uint32_t)s.dx_parts;
             a.sums = (float *)(ws + s.dx);
+            a.dx = s.dx_direct ? dx : nullptr;
             a.add = a.v0 > 0;
             grid = (int64_t)a.m_tiles * a.n_tiles * a.parts;
             if (!fits(grid)) return fail();
@@ -1036,14 +1068,14 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
                     FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 128, 2, 4>), g, wt, tiles_bytes(128, 128, 4), st, a);
                 else if (s.dx_cols == 128)
                     FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 256, 2, 3>), g, wt, tiles_bytes(256, 128, 3), st, a);
-                else
+                else if constexpr (!is_pairs<T>())
                     FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 256, 4, 2>), g, wt, tiles_bytes(256, 256, 2), st, a);
             } else if (s.dx_tile == 128)
                 FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 128, 128, BK>), g, nt, 0, st, a);
             else FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 64, 64, BK>), g, nt, 0, st, a);
         }
         if (dw && op->K) {
-            const int rows = p.wide ? 256 : s.dw_tile, cols = p.wide ? s.dw_cols : s.dw_tile;
+            const int rows = s.dw_tile, cols = p.wide ? s.dw_cols : s.dw_tile;
             a.m_tiles = (uint32_t)ceil_div(a.width, rows);
             a.n_tiles = (uint32_t)ceil_div(op->K, cols);
             a.parts = (uint32_t)s.dw_parts;
@@ -1055,8 +1087,12 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             if (!fits(grid)) return fail();
             const dim3 g((unsigned)grid);
             if (p.wide) {
-                if (cols == 128) FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 2, 3>), g, wt, tiles_bytes(256, 128, 3), st, a);
-                else FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 4, 2>), g, wt, tiles_bytes(256, 256, 2), st, a);
+                if (rows == 128)
+                    FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 128, 2, 4>), g, wt, tiles_bytes(128, 128, 4), st, a);
+                else if (cols == 128)
+                    FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 256, 2, 3>), g, wt, tiles_bytes(256, 128, 3), st, a);
+                else if constexpr (!is_pairs<T>())
+                    FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 256, 4, 2>), g, wt, tiles_bytes(256, 256, 2), st, a);
             } else if (rows == 128)
                 FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 128, 128, BK>), g, nt, 0, st, a);
             else FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 64, 64, BK>), g, nt, 0, st, a);
@@ -1079,7 +1115,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
                           none, (T *)db + a.v0);
         }
     }
-    if (dx && op->K)
+    if (dx && op->K && !s.dx_direct)
         FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(op->M * op->K, LS_NT * 4)), dim3(LS_NT), 0, st,
                   (const float *)(ws + s.dx), (uint32_t)s.dx_parts, op->M * op->K, a.unscale,
                   a.undo ? a.undo + 1 : nullptr, (T *)dx);
