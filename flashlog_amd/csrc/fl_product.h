@@ -725,13 +725,13 @@ struct WideProduct {
 // run ahead over the tiles' ends.  Tiles of BM rows and WN x 64 columns, a step of
 // 64 values (PAIRS: 32 of both planes).
 //
-// A step's operands come in two halves (of its values; PAIRS: the planes), and
-// one is read from LDS while the other is multiplied; a barrier a step, between
-// the halves, says that the step is read by all and the next one there, whose
-// first half is read beside the second products.  Loads of a later step are issued
-// one at a time between those.  (Read and multiplied in turns, by half the waves
-// each or by all together, the matrix unit was busy 46% of the time, whatever the
-// tile: 128 x 128, fp32 [1536 x 2048 -> 1645] 52 and 50 us.)
+// Operands are read from LDS beside the products of others: of small tiles those
+// of the next step; of 256 x 256 tiles, whose sums leave fewer registers, a step's
+// come in two halves, the first of the next step's beside the second's products.
+// A barrier a step says that it is read by all and the next one there.  Loads of a
+// later step are issued one at a time between the products.  (Read and multiplied
+// in turns, by half the waves each or by all together, the matrix unit was busy 46%
+// of the time, whatever the tile: 128 x 128, fp32 [1536 x 2048 -> 1645] 52 and 50 us.)
 //
 // feed(i, lds_a, lds_b) issues load i of the next step, and after the last one
 // goes on to the step behind it; behind the last step it may load anything that
@@ -795,36 +795,71 @@ struct WideTiles {
         Waits::meet();
         const uint16_t *la = lds;
         int at = 0, tile = 0;
-        u32x4 a0[MT], b0[NTL];
-        ta.template read<0>(la, wave_m(), a0);
-        tb.template read<0>(la + TA::ELEMS, wave_n(), b0);
-        for (int s = 0; s < all; ++s) {
-            u32x4 a1[MT], b1[NTL];
-            tb.template read<1>(la + TA::ELEMS, wave_n(), b1);
-            ta.template read<1>(la, wave_m(), a1);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(a0, b0, none);
-            __builtin_amdgcn_sched_barrier(0);
-            Waits::template wait<LOADS *(STAGES - 2)>();
-            Waits::meet();
-            la = la == lds + (STAGES - 1) * ELEMS ? lds : la + ELEMS;
-            if constexpr (PAIRS) {
-                multiply(a0, b1, load_between);
+        const auto go_on = [&]() { la = la == lds + (STAGES - 1) * ELEMS ? lds : la + ELEMS; };
+        const auto finished = [&]() {
+            if (ONE || ++at < steps) return;
+            out(tile++);
+            clear();
+            at = 0;
+        };
+        if constexpr (MT * NTL <= 16) {
+            // a whole step's operands beside those that are multiplied; half the waves read first, half multiply first
+            struct Operands {
+                u32x4 a[2][MT], b[2][NTL];
+            };
+            const bool second = fl_wave_id() >= WD_WAVES / 2;
+            const auto read = [&](Operands &o) {
+                tb.template read<0>(la + TA::ELEMS, wave_n(), o.b[0]);
+                ta.template read<0>(la, wave_m(), o.a[0]);
+                tb.template read<1>(la + TA::ELEMS, wave_n(), o.b[1]);
+                ta.template read<1>(la, wave_m(), o.a[1]);
+            };
+            const auto step = [&](const Operands &now, Operands &next) {
+                Waits::template wait<LOADS *(STAGES - 2)>();
+                Waits::meet();
+                go_on();
+                if (!second) read(next);
                 __builtin_amdgcn_sched_barrier(0);
-                ta.template read<0>(la, wave_m(), a0);
+                if constexpr (PAIRS) {
+                    multiply(now.a[0], now.b[1], load_between);
+                    multiply(now.a[1], now.b[0], none);
+                    multiply(now.a[0], now.b[0], none);
+                } else {
+                    multiply(now.a[0], now.b[0], load_between);
+                    multiply(now.a[1], now.b[1], none);
+                }
                 __builtin_amdgcn_sched_barrier(0);
-                multiply(a1, b0, none);
-                tb.template read<0>(la + TA::ELEMS, wave_n(), b0);
-            } else {
+                if (second) read(next);
+                finished();
+            };
+            Operands even, odd;
+            read(even);
+            for (int s = 0;; s += 2) {
+                step(even, odd);
+                if (s + 1 >= all) break;
+                step(odd, even);
+                if (s + 2 >= all) break;
+            }
+        } else {
+            static_assert(!PAIRS, "two planes of such tiles have no registers");
+            u32x4 a0[MT], b0[NTL];
+            ta.template read<0>(la, wave_m(), a0);
+            tb.template read<0>(la + TA::ELEMS, wave_n(), b0);
+            for (int s = 0; s < all; ++s) {
+                u32x4 a1[MT], b1[NTL];
+                tb.template read<1>(la + TA::ELEMS, wave_n(), b1);
+                ta.template read<1>(la, wave_m(), a1);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(a0, b0, none);
+                __builtin_amdgcn_sched_barrier(0);
+                Waits::template wait<LOADS *(STAGES - 2)>();
+                Waits::meet();
+                go_on();
                 tb.template read<0>(la + TA::ELEMS, wave_n(), b0);
                 ta.template read<0>(la, wave_m(), a0);
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(a1, b1, load_between);
-            }
-            if (!ONE && ++at == steps) {
-                out(tile++);
-                clear();
-                at = 0;
+                finished();
             }
         }
         Waits::template wait<0>();  // loads behind the last step

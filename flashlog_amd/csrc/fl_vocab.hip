@@ -302,24 +302,42 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_dx(VocabArgs a) {
     }
 }
 
-// The parts of a sum added in order and rounded: four values a thread.
+// The parts of a sum added and rounded: four values a lane, a quarter of the
+// parts a wave, each in order and then the quarters.
 template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_vocab_fold(const float *__restrict__ part, uint32_t parts, int64_t n,
                                                       const float *__restrict__ unscale,
                                                       const float *__restrict__ undo, T *__restrict__ out) {
-    const int64_t i = (fl_block() * LS_NT + threadIdx.x) * 4;
-    if (i >= n) return;
-    const int have = n - i < 4 ? (int)(n - i) : 4;
-    const float f = *unscale, f2 = undo ? *undo : 1.0f;
-    float s[4] = {0, 0, 0, 0}, v[4];
-    for (uint32_t p = 0; p < parts; ++p) {
-        load_some<float>(part + p * n + i, have, v);
+    __shared__ float runs[LS_WAVES][4 * FL_WAVE];
+    const int64_t i = (fl_block() * FL_WAVE + fl_lane()) * 4;
+    const int have = n - i < 0 ? 0 : n - i < 4 ? (int)(n - i) : 4;
+    float s[4] = {0, 0, 0, 0};
+    uint32_t p = parts * fl_wave_id() / LS_WAVES;
+    const uint32_t p1 = parts * (fl_wave_id() + 1) / LS_WAVES;
+    const auto add = [&](auto many) {
+        constexpr int N = decltype(many)::value;
+        float v[N][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v[e];
-    }
+        for (int j = 0; j < N; ++j) load_some<float>(part + (p + j) * n + i, have, v[j]);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += v[j][e];
+        p += N;
+    };
+    while (p + 8 <= p1) add(std::integral_constant<int, 8>());
+    while (p < p1) add(std::integral_constant<int, 1>());
+#pragma unroll
+    for (int e = 0; e < 4; ++e) runs[fl_wave_id()][fl_lane() * 4 + e] = s[e];
+    __syncthreads();
+    if (fl_wave_id() || !have) return;
+    const float f = *unscale, f2 = undo ? *undo : 1.0f;
     Vec<T, 4> o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o.v[e] = (T)(s[e] * f * f2);
+    for (int e = 0; e < 4; ++e) {
+        const int at = fl_lane() * 4 + e;
+        o.v[e] = (T)(((runs[0][at] + runs[1][at]) + (runs[2][at] + runs[3][at])) * f * f2);
+    }
     if (have == 4) store_vec<T, 4>(out + i, o);
     else store_some<T, 4>(out + i, o, have);
 }
@@ -569,27 +587,32 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
             for (int i = 0; i < MT; ++i) {
                 __builtin_amdgcn_sched_barrier(0);  // a row's values at a time: few registers
                 Running r = state[i * FL_WAVE];
-                float u[16], s = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    u[e] = run.acc[i][e / 4][e % 4] * scale;
-                    if (a.op.bias) u[e] += b[e];
-                }
-                if (__any(have < 16))
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) u[e] = e < have ? u[e] : -INFINITY;
+                float s = 0.0f;
+                const auto u = [&](int e, float less) {
+                    const float v = run.acc[i][e / 4][e % 4];
+                    const float t = a.op.bias ? b[e] - less : -less;
+                    return e < have ? __builtin_fmaf(v, scale, t) : -INFINITY;
+                };
                 // what the lane had first serves as the maximum, until a sum overflows or is not a number
+                if (__any(have < 16)) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s += exp2_of(u[e] - r.m);
+                    for (int e = 0; e < 16; ++e) s += exp2_of(u(e, r.m));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float v = run.acc[i][e / 4][e % 4];
+                        s += exp2_of(__builtin_fmaf(v, scale, a.op.bias ? b[e] - r.m : -r.m));
+                    }
+                }
                 s += r.s;
                 if (__any(r.m == -INFINITY || !(s < INFINITY))) {
                     float m = r.m;
                     s = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) m = fmaxf(m, u[e]);
+                    for (int e = 0; e < 16; ++e) m = fmaxf(m, u(e, 0.0f));
                     const float at = base_of(m);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) s += exp2_of(u[e] - at);
+                    for (int e = 0; e < 16; ++e) s += exp2_of(u(e, at));
                     s += r.s * exp2_of(r.m - at);
                     r.m = m;
                 }
@@ -641,13 +664,12 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
                 float u[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    u[e] = run.acc[i][e / 4][e % 4] * scale;
-                    if (a.op.bias) u[e] += b[e];
-                    u[e] = q.y == 0.0f ? 0.0f : q.y * exp2_of(u[e] - q.x);
+                    const float v = run.acc[i][e / 4][e % 4];
+                    u[e] = q.y * exp2_of(__builtin_fmaf(v, scale, a.op.bias ? b[e] - q.x : -q.x));
                 }
-                if (__any(have < 16))
+                if (__any(q.y == 0.0f || have < 16))
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) u[e] = e < have ? u[e] : 0.0f;
+                    for (int e = 0; e < 16; ++e) u[e] = q.y != 0.0f && e < have ? u[e] : 0.0f;
                 if (row0 + r >= a.d_rows) continue;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -1097,13 +1119,13 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
                 FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 128, 128, BK>), g, nt, 0, st, a);
             else FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 64, 64, BK>), g, nt, 0, st, a);
             if (a.sums)
-                FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(a.width * op->K, LS_NT * 4)), dim3(LS_NT),
+                FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(a.width * op->K, FL_WAVE * 4)), dim3(LS_NT),
                           0, st, a.sums, a.parts, a.width * op->K, a.unscale, a.undo, (T *)dw + a.v0 * op->K);
         }
         if (db) {
             a.parts = (uint32_t)s.db_parts;
             a.sums = (float *)(ws + s.db);
-            const dim3 cg = grid_of(a.parts * ceil_div(a.width, LS_NT)), g = grid_of(ceil_div(a.width, LS_NT * 4));
+            const dim3 cg = grid_of(a.parts * ceil_div(a.width, LS_NT)), g = grid_of(ceil_div(a.width, FL_WAVE * 4));
             if (p.wide) FL_LAUNCH("k_vocab_cols", (k_vocab_cols<T, true>), cg, dim3(LS_NT), 0, st, a);
             else FL_LAUNCH("k_vocab_cols", (k_vocab_cols<T, false>), cg, dim3(LS_NT), 0, st, a);
             const float *none = nullptr;
@@ -1116,7 +1138,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
         }
     }
     if (dx && op->K && !s.dx_direct)
-        FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(op->M * op->K, LS_NT * 4)), dim3(LS_NT), 0, st,
+        FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(op->M * op->K, FL_WAVE * 4)), dim3(LS_NT), 0, st,
                   (const float *)(ws + s.dx), (uint32_t)s.dx_parts, op->M * op->K, a.unscale,
                   a.undo ? a.undo + 1 : nullptr, (T *)dx);
     return fl_check_launch("linear_loss");
