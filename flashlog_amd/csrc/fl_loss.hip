@@ -26,27 +26,6 @@ constexpr int LS_SEG = 2048;  // columns of a wave
 constexpr int LS_NT = 256;
 constexpr int LS_WAVES = LS_NT / FL_WAVE;
 
-__device__ __forceinline__ Running joined_over(Running r, int lanes) {
-#pragma unroll
-    for (int o = FL_WAVE / 2; o > 0; o >>= 1) {
-        if (o >= lanes) continue;
-        r = joined(r, Running{__shfl_xor(r.m, o), __shfl_xor(r.s, o)});
-    }
-    return r;
-}
-
-struct ListArgs {
-    fl_lists op;
-    float scale, tau2;  // log2(e) / tau, tau^2
-    int64_t cols;
-    const Running *part;  // [rows][parts]
-    int64_t parts;
-    const void *logits;   // scores; null: `listed` holds u
-    int64_t ld;
-    float *loss;
-    float2 *rows, *listed;  // (lse, whether the row counts), (u, sum of q at the id)
-};
-
 // ---------------------------------------------------------------------------
 // Rows that are given
 
@@ -173,62 +152,24 @@ __global__ __launch_bounds__(LS_NT) void k_score_grad(ScoreArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Rows' sums joined, their lists, their losses: a wave a row.
-template <typename T>
+// Rows' sums joined, their lists, their losses: a wave a row, or the four of a
+// workgroup where there are many parts (2247 of 32 rows: 25 us with one).
+template <typename T, int WPR>
 __global__ __launch_bounds__(LS_NT) void k_list_rows(ListArgs a) {
     extern __shared__ __align__(16) float2 list_lds[];
-    const int waves = blockDim.x / FL_WAVE;
-    const int64_t row = fl_block() * waves + fl_wave_id(), k = a.op.k;
+    __shared__ Running quarters[LS_WAVES];
+    const int64_t waves = blockDim.x / FL_WAVE, row = WPR == 1 ? fl_block() * waves + fl_wave_id() : fl_block();
     if (row >= a.op.rows) return;
-    Running r{-INFINITY, 0.0f};
-    for (int64_t p = fl_lane(); p < a.parts; p += FL_WAVE) r = joined(r, a.part[row * a.parts + p]);
-    r = joined_over(r, FL_WAVE);
-    const float lse = r.m + log2f(r.s);
-    const int64_t *ids = a.op.ids + row * k;
-    float2 *mine = list_lds + fl_wave_id() * k, *listed = a.listed + row * k;
-    // (id, teacher in units of log 2), -inf where it does not count
-    float top = -INFINITY;
-    bool any = false;
-    for (int64_t j = fl_lane(); j < k; j += FL_WAVE) {
-        const int64_t id = ids[j];
-        const bool in = id >= 0 && id < a.cols;
-        float u = 0.0f;
-        if (a.logits) u = in ? (float)((const T *)a.logits)[row * a.ld + id] * a.scale : 0.0f;
-        else if (in) u = listed[j].x;
-        float v = -INFINITY;
-        if (in && a.op.teacher && u != -INFINITY) v = a.op.teacher[row * k + j] * a.scale;
-        if (in && !a.op.teacher) v = 0.0f;
-        mine[j] = float2{__int_as_float(in ? (int)id : -1), v};
-        listed[j] = float2{u, 0.0f};
-        top = fmaxf(top, v);
-        any = any || v != -INFINITY;
+    Running r = joined_parts(a.part + row * a.parts, a.parts, WPR == 1 ? 0 : fl_wave_id(), WPR);
+    if constexpr (WPR > 1) {
+        if (fl_lane() == 0) quarters[fl_wave_id()] = r;
+        __syncthreads();
+        if (fl_wave_id()) return;
+        r = joined(joined(quarters[0], quarters[1]), joined(quarters[2], quarters[3]));
     }
-#pragma unroll
-    for (int o = FL_WAVE / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const bool live = __any(any) && r.s != 0.0f;  // no sum: every u is -inf
-    float total = 0.0f;
-    for (int64_t j = fl_lane(); j < k; j += FL_WAVE) total += exp2_of(mine[j].y - top);
-    total = fl_wave_sum_f32(total);
-    const float of_total = 1.0f / total, log_total = log2f(total);
-    float loss = 0.0f;
-    for (int64_t j = fl_lane(); j < k; j += FL_WAVE) {
-        const float v = mine[j].y, q = live ? exp2_of(v - top) * of_total : 0.0f;
-        if (q != 0.0f) loss += q * ((v - top - log_total) - (listed[j].x - lse));
-        mine[j].y = q;
-    }
-    loss = fl_wave_sum_f32(loss) * (a.tau2 * LN2);
-    if (fl_lane() == 0) {
-        a.loss[row] = live ? loss : 0.0f;
-        a.rows[row] = float2{lse, live ? 1.0f : 0.0f};
-    }
-    fl_wave_sync();
-    for (int64_t j = fl_lane(); j < k; j += FL_WAVE) {
-        const int id = __float_as_int(mine[j].x);
-        float q = 0.0f;
-        if (id >= 0)
-            for (int64_t i = 0; i < k; ++i) q += __float_as_int(mine[i].x) == id ? mine[i].y : 0.0f;
-        listed[j].y = q;
-    }
+    list_row(a, row, r, list_lds + (WPR == 1 ? fl_wave_id() * a.op.k : 0), [&](int64_t j, int64_t id) {
+        return a.logits ? (float)((const T *)a.logits)[row * a.ld + id] * a.scale : a.listed[row * a.op.k + j].x;
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -238,23 +179,14 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 template <typename T>
 int join_rows(hipStream_t st, ListArgs &a, const char *what) {
+    if (a.parts > 4 * FL_WAVE) {
+        FL_LAUNCH("k_list_rows", (k_list_rows<T, LS_WAVES>), grid_of(a.op.rows), dim3(LS_NT), (size_t)a.op.k * 8, st, a);
+        return fl_check_launch(what);
+    }
     const int64_t waves = a.op.k <= 512 ? LS_WAVES : 1;
-    const size_t lds = (size_t)waves * a.op.k * 8;
-    FL_LAUNCH("k_list_rows", k_list_rows<T>, grid_of(ceil_div(a.op.rows, waves)), dim3((unsigned)waves * FL_WAVE), lds,
-              st, a);
+    FL_LAUNCH("k_list_rows", (k_list_rows<T, 1>), grid_of(ceil_div(a.op.rows, waves)), dim3((unsigned)waves * FL_WAVE),
+              (size_t)waves * a.op.k * 8, st, a);
     return fl_check_launch(what);
-}
-
-ListArgs list_args(const fl_lists *l, int64_t cols, void *state, float *loss) {
-    ListArgs a{};
-    a.op = *l;
-    a.scale = LOG2E / l->temperature;
-    a.tau2 = l->temperature * l->temperature;
-    a.cols = cols;
-    a.loss = loss;
-    a.rows = state_rows(state);
-    a.listed = state_listed(l, state);
-    return a;
 }
 
 int64_t segments_of(int64_t cols) { return ceil_div(cols, LS_SEG); }

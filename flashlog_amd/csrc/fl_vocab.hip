@@ -55,23 +55,18 @@ struct VocabArgs {
     const float *undo;     // x's, weight's
 };
 
-// u of the listed columns: a wave a row and four of them.
+// u of four listed ids of a row (-1: none), by one wave; the same in all lanes.
 constexpr int DOT_IDS = 4;
 
 template <typename T>
-__global__ __launch_bounds__(LS_NT) void k_vocab_dots(VocabArgs a) {
-    const int64_t k = a.op.lists.k, quads = (k + DOT_IDS - 1) / DOT_IDS;
-    const int64_t item = fl_block() * LS_WAVES + fl_wave_id();
-    if (item >= a.op.M * quads) return;
-    const int64_t row = item / quads, j0 = item % quads * DOT_IDS, K = a.op.K;
+__device__ __forceinline__ void dots(const VocabArgs &a, int64_t row, const int64_t (&id)[DOT_IDS],
+                                     float (&s)[DOT_IDS]) {
+    const int64_t K = a.op.K;
     const T *x = (const T *)a.op.x + row * a.op.ldx;
     const T *w[DOT_IDS];
-    int64_t id[DOT_IDS];
-    float s[DOT_IDS] = {};
 #pragma unroll
     for (int i = 0; i < DOT_IDS; ++i) {
-        id[i] = j0 + i < k ? a.op.lists.ids[row * k + j0 + i] : -1;
-        if (id[i] >= a.op.V) id[i] = -1;
+        s[i] = 0.0f;
         w[i] = (const T *)a.op.weight + (id[i] < 0 ? 0 : id[i]) * a.op.ldw;
     }
     int64_t c = fl_lane() * 8;
@@ -90,14 +85,51 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_dots(VocabArgs a) {
         for (int i = 0; i < DOT_IDS; ++i) s[i] = __builtin_fmaf((float)x[e], (float)w[i][e], s[i]);
 #pragma unroll
     for (int i = 0; i < DOT_IDS; ++i) {
-        s[i] = fl_wave_sum_f32(s[i]);
-        if (fl_lane() == 0 && j0 + i < k) {
-            float b = 0.0f;
-            if (a.op.bias && id[i] >= 0)
-                b = a.op.bias_f32 ? ((const float *)a.op.bias)[id[i]] : (float)((const T *)a.op.bias)[id[i]];
-            a.listed[row * k + j0 + i] = float2{(s[i] + b) * a.scale, 0.0f};
-        }
+        float b = 0.0f;
+        if (a.op.bias && id[i] >= 0)
+            b = a.op.bias_f32 ? ((const float *)a.op.bias)[id[i]] : (float)((const T *)a.op.bias)[id[i]];
+        s[i] = (fl_wave_sum_f32(s[i]) + b) * a.scale;
     }
+}
+__device__ __forceinline__ void ids_of(const VocabArgs &a, int64_t row, int64_t j0, int64_t (&id)[DOT_IDS]) {
+#pragma unroll
+    for (int i = 0; i < DOT_IDS; ++i) {
+        id[i] = j0 + i < a.op.lists.k ? a.op.lists.ids[row * a.op.lists.k + j0 + i] : -1;
+        if (id[i] >= a.op.V) id[i] = -1;
+    }
+}
+
+// A wave a row and four of its ids.
+template <typename T>
+__global__ __launch_bounds__(LS_NT) void k_vocab_dots(VocabArgs a) {
+    const int64_t k = a.op.lists.k, quads = (k + DOT_IDS - 1) / DOT_IDS;
+    const int64_t item = fl_block() * LS_WAVES + fl_wave_id();
+    if (item >= a.op.M * quads) return;
+    const int64_t row = item / quads, j0 = item % quads * DOT_IDS;
+    int64_t id[DOT_IDS];
+    float s[DOT_IDS];
+    ids_of(a, row, j0, id);
+    dots<T>(a, row, id, s);
+#pragma unroll
+    for (int i = 0; i < DOT_IDS; ++i)
+        if (fl_lane() == i && j0 + i < k) a.listed[row * k + j0 + i] = float2{s[i], 0.0f};
+}
+
+// The rows' sums, dots and losses in one, for lists of up to four ids (a launch
+// less): a wave a row.
+template <typename T>
+__global__ __launch_bounds__(LS_NT) void k_vocab_rows(VocabArgs a, ListArgs l) {
+    __shared__ float2 lists[LS_WAVES][DOT_IDS];
+    const int64_t row = fl_block() * LS_WAVES + fl_wave_id();
+    if (row >= a.op.M) return;
+    const Running r = joined_parts(a.part + row * a.parts, a.parts, 0, 1);
+    int64_t id[DOT_IDS];
+    float s[DOT_IDS];
+    ids_of(a, row, 0, id);
+    dots<T>(a, row, id, s);
+    list_row(l, row, r, lists[fl_wave_id()], [&](int64_t j, int64_t) {
+        return j == 0 ? s[0] : j == 1 ? s[1] : j == 2 ? s[2] : s[3];
+    });
 }
 
 // The logits of a lane's tiles in units of log 2, -inf behind the vocabulary:
@@ -260,7 +292,8 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
         _Float16 *to = (_Float16 *)a.d + row * a.ldd + pair_at(v);
         to[0] = (_Float16)d;
         to[32] = (_Float16)(d - (float)to[0]);
-    } else ((T *)a.d)[row * a.ldd + v] = (T)d;
+    } else if constexpr (WIDE) ((_Float16 *)a.d)[row * a.ldd + v] = (_Float16)d;
+    else ((T *)a.d)[row * a.ldd + v] = (T)d;
 }
 
 // A piece's part of dx, added to what is there if `add`.
@@ -387,58 +420,85 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_dw(VocabArgs a) {
 }
 
 // Column sums of a part of the rows of dz, a thread a column.
-template <typename T, bool WIDE>
+template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
     const int64_t blocks = (a.width + LS_NT - 1) / LS_NT, item = fl_block(), part = item / blocks;
     const int64_t c = item % blocks * LS_NT + threadIdx.x;
     if (part >= a.parts || c >= a.width) return;
     float s = 0.0f;
-    for (int64_t m = a.op.M * part / a.parts; m < a.op.M * (part + 1) / a.parts; ++m) {
-        if constexpr (WIDE && sizeof(T) == 4) {
-            const _Float16 *d = (const _Float16 *)a.d + m * a.ldd + pair_at(c);
-            s += (float)d[0] + (float)d[32];
-        } else s += (float)((const T *)a.d)[m * a.ldd + c];
-    }
+    for (int64_t m = a.op.M * part / a.parts; m < a.op.M * (part + 1) / a.parts; ++m)
+        s += (float)((const T *)a.d)[m * a.ldd + c];
     a.sums[part * a.width + c] = s;
 }
 
 // ---------------------------------------------------------------------------
 // The same for large products
 
+// Whether the operands are two planes, and whether they are scaled.
+template <typename T>
+constexpr bool is_pairs() {
+    return sizeof(T) == 4;
+}
+template <typename T>
+constexpr bool is_scaled() {
+    return !std::is_same<T, _Float16>::value;
+}
+
 // The largest finite magnitude of x and of weight, a part of them a workgroup.
 constexpr int LAY_PARTS = 512;
 
+template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restrict__ most) {
+    constexpr int G = 16 / (int)sizeof(T);
     __shared__ float waves[LS_WAVES];
     const bool second = blockIdx.y;
-    const int64_t R = second ? a.op.V : a.op.M, ld = second ? a.op.ldw : a.op.ldx, quads = (a.op.K + 3) / 4;
-    const float *p = (const float *)(second ? a.op.weight : a.op.x);
+    const int64_t R = second ? a.op.V : a.op.M, ld = second ? a.op.ldw : a.op.ldx, K = a.op.K, groups = (K + G - 1) / G;
+    const T *p = (const T *)(second ? a.op.weight : a.op.x);
     float m = 0.0f;
-    for (int64_t i = (int64_t)blockIdx.x * LS_NT + threadIdx.x; i < R * quads; i += (int64_t)LAY_PARTS * LS_NT) {
-        const int64_t c = i % quads * 4;
-        float v[4];
-        load_some<float>(p + i / quads * ld + c, a.op.K - c < 4 ? (int)(a.op.K - c) : 4, v);
+    const auto see = [&](T t) {
+        const float v = fabsf((float)t);
+        m = fmaxf(m, v < INFINITY ? v : 0.0f);
+    };
+    const int64_t all = R * groups, step = (int64_t)LAY_PARTS * LS_NT;
+    const auto take = [&](int64_t i, Vec<T, G> &v) {
+        const int64_t r = i / groups, c = (i - r * groups) * G;
+        if (c + G <= K) v = load_vec<T, G>(p + r * ld + c);
+        else
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
+            for (int e = 0; e < G; ++e) v.v[e] = c + e < K ? p[r * ld + c + e] : (T)0.0f;
+    };
+    for (int64_t i = (int64_t)blockIdx.x * LS_NT + threadIdx.x; i < all; i += 4 * step) {
+        Vec<T, G> v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) take(i + j * step < all ? i + j * step : i, v[j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < G; ++e) see(v[j].v[e]);
     }
 #pragma unroll
     for (int o = FL_WAVE / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     if (fl_lane() == 0) waves[fl_wave_id()] = m;
     __syncthreads();
-    if (threadIdx.x == 0) most[blockIdx.y * LAY_PARTS + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+    if (threadIdx.x == 0)
+        most[blockIdx.y * LAY_PARTS + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
 }
 
-// x and weight as rows of 16-bit values on 16 bytes: fp32 as two planes (pair_at), others copied; zeros behind a row.
+// x and weight as rows of half values on 16 bytes: fp32 as two planes (pair_at),
+// bfloat16 times a power of two that brings the largest to 2^13..2^14 (what is
+// above 2^-31 of it is held exactly, and what is lost below 2^-39), half as it is;
+// zeros behind a row.  (dz, in half, is then rounded by 2^-12 of itself; by 2^-9 in
+// bfloat16 it made the gradients' error 1.4 to 1.5 times that of their own rounding.)
 template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restrict__ most, uint16_t *__restrict__ x,
                                                uint16_t *__restrict__ w, float *__restrict__ undo) {
-    constexpr bool PAIRS = sizeof(T) == 4;
+    constexpr bool PAIRS = is_pairs<T>();
     const bool second = blockIdx.y;
     const int64_t R = second ? a.op.V : a.op.M, ld = second ? a.op.ldw : a.op.ldx, chunks = a.cols / 8, K = a.op.K;
     const T *p = (const T *)(second ? a.op.weight : a.op.x);
     uint16_t *out = second ? w : x;
     float scale = 1.0f;
-    if constexpr (PAIRS) {
+    if constexpr (is_scaled<T>()) {
         __shared__ float waves[LS_WAVES];
         float m = 0.0f;
         for (int i = threadIdx.x; i < LAY_PARTS; i += LS_NT) m = fmaxf(m, most[blockIdx.y * LAY_PARTS + i]);
@@ -471,16 +531,16 @@ __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restr
             _Float16 *q = (_Float16 *)out + r * 2 * a.cols + pair_at(c);
             store_vec<_Float16, 8>(q, hi);
             store_vec<_Float16, 8>(q + 32, lo);
-        } else store_vec<T, 8>((T *)out + r * a.cols + c, v);
+        } else {
+            Vec<_Float16, 8> o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (is_scaled<T>()) o.v[e] = (_Float16)((float)v.v[e] * scale);
+                else o.v[e] = v.v[e];
+            }
+            store_vec<_Float16, 8>((_Float16 *)out + r * a.cols + c, o);
+        }
     }
-}
-
-// The operands' 16-bit type.
-template <typename T>
-using Half = std::conditional_t<sizeof(T) == 4, _Float16, T>;
-template <typename T>
-constexpr bool is_pairs() {
-    return sizeof(T) == 4;
 }
 
 // Logit tiles: row tiles of x against row tiles of weight from n0 on, whose
@@ -490,7 +550,7 @@ template <typename T, int BM, int WN, int STAGES>
 struct LogitTiles {
     using TA = StepsContig<BM>;
     using TB = StepsContig<WN * 64>;
-    using Run = WideTiles<Half<T>, is_pairs<T>(), BM, WN, STAGES, TA, TB>;
+    using Run = WideTiles<_Float16, is_pairs<T>(), BM, WN, STAGES, TA, TB>;
     TA ta;
     TB tb;
     int steps, at;  // of a tile's row; of the next load
@@ -638,10 +698,19 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
     row_and_part(a, &mt, &part);
     const int64_t row0 = (int64_t)mt * BM, end = a.v0 + a.width;
     const int64_t t0 = part_begin(a.n_tiles, part, a.parts), t1 = part_begin(a.n_tiles, part + 1, a.parts);
-    float2 *of = reinterpret_cast<float2 *>(wide_lds + STAGES * Run::ELEMS);  // (lse, coefficient) of the tile's rows
+    // (lse, coefficient, the row's only id or -1, its dz) of the tile's rows
+    float4 *of = reinterpret_cast<float4 *>(wide_lds + STAGES * Run::ELEMS);
     for (int t = threadIdx.x; t < BM; t += WD_NT) {
         const int64_t m = row0 + t < a.op.M ? row0 + t : a.op.M - 1;
-        of[t] = float2{a.rows[m].x, row0 + t < a.op.M ? a.coef[m] : 0.0f};
+        const float lse = a.rows[m].x, c = row0 + t < a.op.M ? a.coef[m] : 0.0f;
+        float id = __int_as_float(-1), d = 0.0f;
+        if (a.op.lists.k == 1 && c != 0.0f) {
+            const int64_t v = a.op.lists.ids[m];
+            const float2 l = a.listed[m];
+            if (v >= a.v0 && v < end) id = __int_as_float((int)(v - a.v0));
+            d = c * (exp2_of(l.x - lse) - l.y);
+        }
+        of[t] = float4{lse, c, id, d};
     }
     __syncthreads();
     Tiles tiles;
@@ -652,7 +721,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
         tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](int i, uint16_t *la, uint16_t *lb) { tiles.feed(a, i, la, lb); },
         [&](int64_t t) {
             const int lane = made_here(fl_lane());
-            const int64_t c = (t0 + t) * WN * 64 + run.wave_n() + (lane >> 4) * 16, n = a.v0 + c;
+            const int64_t c = (t0 + t) * WN * 64 + run.wave_n() + (lane >> 4) * 16, n = a.v0 + c;  // c: in the piece
             const int have = end - n < 16 ? (int)(end - n) : 16;
             float b[16];
             if (a.op.bias) lane_bias<T>(a, n, b);
@@ -660,7 +729,8 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
             for (int i = 0; i < MT; ++i) {
                 __builtin_amdgcn_sched_barrier(0);
                 const int r = run.wave_m() + i * 16 + (lane & 15);
-                const float2 q = of[r];
+                const float4 q = of[r];
+                const int64_t at = __float_as_int(q.z) - c;  // of the row's only id
                 float u[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -670,23 +740,64 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
                 if (__any(q.y == 0.0f || have < 16))
 #pragma unroll
                     for (int e = 0; e < 16; ++e) u[e] = q.y != 0.0f && e < have ? u[e] : 0.0f;
+                if (__any(at >= 0 && at < 16))
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) u[e] = at == e ? q.w : u[e];
                 if (row0 + r >= a.d_rows) continue;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (c + h * 8 >= a.d_cols) continue;
-                    Vec<Half<T>, 8> o;
+                    Vec<_Float16, 8> o;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) o.v[e] = (Half<T>)u[h * 8 + e];
-                    Half<T> *to = (Half<T> *)a.d + (row0 + r) * a.ldd + (is_pairs<T>() ? pair_at(c + h * 8) : c + h * 8);
-                    store_vec<Half<T>, 8>(to, o);
+                    for (int e = 0; e < 8; ++e) o.v[e] = (_Float16)u[h * 8 + e];
+                    _Float16 *to = (_Float16 *)a.d + (row0 + r) * a.ldd + (is_pairs<T>() ? pair_at(c + h * 8) : c + h * 8);
+                    store_vec<_Float16, 8>(to, o);
                     if constexpr (is_pairs<T>()) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) o.v[e] = (Half<T>)(u[h * 8 + e] - (float)o.v[e]);
-                        store_vec<Half<T>, 8>(to + 32, o);
+                        for (int e = 0; e < 8; ++e) o.v[e] = (_Float16)(u[h * 8 + e] - (float)o.v[e]);
+                        store_vec<_Float16, 8>(to + 32, o);
                     }
                 }
             }
         });
+}
+
+// Column sums of a part of the rows of dz: 512 columns a workgroup, eight a lane,
+// a quarter of the rows a wave.
+constexpr int COLS_WIDE = 8 * FL_WAVE;
+
+template <bool PAIRS>
+__global__ __launch_bounds__(LS_NT) void k_wide_cols(VocabArgs a) {
+    constexpr int AHEAD = 4;
+    __shared__ float sums[LS_WAVES][COLS_WIDE];
+    const int64_t blocks = (a.width + COLS_WIDE - 1) / COLS_WIDE, item = fl_block(), part = item / blocks;
+    if (part >= a.parts) return;
+    const int64_t c0 = item % blocks * COLS_WIDE, c = c0 + fl_lane() * 8;
+    const int64_t runs = (int64_t)a.parts * LS_WAVES, run = part * LS_WAVES + fl_wave_id();
+    const int64_t begin = a.op.M * run / runs, end = a.op.M * (run + 1) / runs;
+    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (c < a.d_cols)
+        for (int64_t m = begin; m < end; m += AHEAD) {
+            Vec<_Float16, 8> v[AHEAD], w[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int64_t r = m + j < end ? m + j : end - 1;
+                const _Float16 *d = (const _Float16 *)a.d + r * a.ldd + (PAIRS ? pair_at(c) : c);
+                v[j] = load_vec<_Float16, 8>(d);
+                if (PAIRS) w[j] = load_vec<_Float16, 8>(d + 32);
+            }
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                if (m + j >= end) break;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[e] += PAIRS ? (float)v[j].v[e] + (float)w[j].v[e] : (float)v[j].v[e];
+            }
+        }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[fl_wave_id()][fl_lane() * 8 + e] = s[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < COLS_WIDE && c0 + i < a.width; i += LS_NT)
+        a.sums[part * a.width + c0 + i] = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
 }
 
 // A piece's part of dx, added to what is there if `add`.
@@ -696,7 +807,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
     constexpr int STEP = PAIRS ? 32 : 64;
     using TA = StepsContig<BM>;
     using TB = StepsStrided<WN * 64, PAIRS>;
-    using Run = WideTiles<Half<T>, PAIRS, BM, WN, STAGES, TA, TB>;
+    using Run = WideTiles<_Float16, PAIRS, BM, WN, STAGES, TA, TB>;
     extern __shared__ __align__(16) uint16_t wide_lds[];
     const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x), tiles = a.m_tiles * a.n_tiles;
     const uint32_t part = (uint32_t)__builtin_amdgcn_readfirstlane((int)(w / tiles)), tile = w - part * tiles;
@@ -769,7 +880,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
     constexpr int STEP = PAIRS ? 32 : 64;
     using TA = StepsStrided<BM, PAIRS>;
     using TB = StepsStrided<WN * 64, PAIRS>;
-    using Run = WideTiles<Half<T>, PAIRS, BM, WN, STAGES, TA, TB>;
+    using Run = WideTiles<_Float16, PAIRS, BM, WN, STAGES, TA, TB>;
     extern __shared__ __align__(16) uint16_t wide_lds[];
     const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
     const uint32_t walks = (uint32_t)__builtin_amdgcn_readfirstlane((int)(gridDim.x / a.parts));
@@ -866,14 +977,25 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     const int64_t step = p.pairs ? 32 : 64;  // inputs of a step of the wide kernels
     if (p.wide) {
         p.small = ceil_div(op->M, 256) * ceil_div(op->V, 256) < 192;
-        p.lay = p.pairs || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % step || op->ldx >= 1 << 23 ||
+        p.lay = op->dtype != FL_F16 || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % step || op->ldx >= 1 << 23 ||
                 op->ldw >= 1 << 23;  // 32-bit offsets of 256 rows
         p.cols = ceil_div(op->K, step) * step;
         p.bm = p.small ? 128 : 256;
         p.bn = p.small || p.pairs ? 128 : 256;  // two planes of 256 x 256 have no registers
     } else {
-        p.bm = op->M > 64 ? 128 : 64;
-        p.bn = p.bm;
+        // tiles by the steps that the fullest CU takes: a step of 128 x 128 takes 2.3 us alone and 1.45 more a tile beside
+        // others, of 64 x 64 1.2 and 0.52, of 32 x 64 0.52 and 0.3 (fp32)
+        double least = 1e30;
+        const int rows[3] = {128, 64, 32}, cols[3] = {128, 64, 64};
+        const double alone[3] = {2.3, 1.2, 0.52}, beside[3] = {1.45, 0.52, 0.3};
+        for (int i = 0; i < 3; ++i) {
+            const double n = (double)ceil_div(ceil_div(op->M, rows[i]) * ceil_div(op->V, cols[i]), 256) * beside[i];
+            const double us = n > alone[i] ? n : alone[i];
+            if (us >= least) continue;
+            least = us;
+            p.bm = rows[i];
+            p.bn = cols[i];
+        }
     }
     p.m_tiles = (uint32_t)ceil_div(op->M, p.bm);
     p.n_tiles = (uint32_t)ceil_div(op->V, p.bn);
@@ -900,7 +1022,7 @@ VocabLayout vocab_layout(const fl_vocab *op, const VocabPlan &p) {
     l.w = rounded((size_t)op->M * p.cols * p.size);
     l.undo = l.w + rounded((size_t)op->V * p.cols * p.size);
     l.most = l.undo + 256;
-    l.bytes = l.most + (p.pairs ? 2 * LAY_PARTS * 4 : 0);
+    l.bytes = l.most + 2 * LAY_PARTS * 4;
     return l;
 }
 
@@ -955,7 +1077,8 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
         if (s.dw_parts > 1) s.dw = take((size_t)s.dw_parts * p.piece * op->K * 4);
     }
     if (with_db) {
-        const int64_t want = ceil_div(2048, ceil_div(p.piece, LS_NT)), most = op->M / 16;
+        const int64_t want = p.wide ? ceil_div(1024, ceil_div(p.piece, COLS_WIDE)) : ceil_div(2048, ceil_div(p.piece, LS_NT));
+        const int64_t most = op->M / 16;
         const int64_t n = want < most ? want : most;
         s.db_parts = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
         s.db = take((size_t)s.db_parts * p.piece * 4);
@@ -976,7 +1099,7 @@ VocabArgs vocab_args(const fl_vocab *op, const VocabPlan &p, void *state, void *
         a.x = (const uint16_t *)((char *)layout + l.x);
         a.w = (const uint16_t *)((char *)layout + l.w);
         a.ldx = a.ldw = p.pairs ? 2 * p.cols : p.cols;
-        if (p.pairs) a.undo = (const float *)((char *)layout + l.undo);
+        if (op->dtype != FL_F16) a.undo = (const float *)((char *)layout + l.undo);
     } else {
         a.x = (const uint16_t *)op->x;
         a.w = (const uint16_t *)op->weight;
@@ -1003,12 +1126,14 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
     if (p.lay) {
         const VocabLayout l = vocab_layout(op, p);
         float *most = (float *)((char *)layout + l.most);
-        if (p.pairs) FL_LAUNCH("k_lay_max", k_lay_max, dim3(LAY_PARTS, 2), dim3(LS_NT), 0, st, a, most);
+        if constexpr (is_scaled<T>())
+            FL_LAUNCH("k_lay_max", k_lay_max<T>, dim3(LAY_PARTS, 2), dim3(LS_NT), 0, st, a, most);
         const int64_t chunks = (op->M > op->V ? op->M : op->V) * (p.cols / 8), want = ceil_div(chunks, LS_NT);
         FL_LAUNCH("k_lay", k_lay<T>, dim3((unsigned)(want < 4096 ? want : 4096), 2), dim3(LS_NT), 0, st, a, most,
                   (uint16_t *)a.x, (uint16_t *)a.w, (float *)a.undo);
     }
-    if (op->lists.k)
+    const bool few = op->lists.k <= DOT_IDS && p.parts <= 4 * FL_WAVE;
+    if (!few)
         FL_LAUNCH("k_vocab_dots", k_vocab_dots<T>,
                   grid_of(ceil_div(op->M * ceil_div(op->lists.k, DOT_IDS), LS_WAVES)), dim3(LS_NT), 0, st, a);
     if (p.wide) {
@@ -1021,8 +1146,12 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
             FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 256, 4, 2>), g, dim3(WD_NT), tiles_bytes(256, 256, 2) + extra(8), st, a);
     } else if (p.bm == 128)
         FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 128, 128, BK>), g, dim3(LN_NT), 0, st, a);
-    else FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 64, 64, BK>), g, dim3(LN_NT), 0, st, a);
-    return join_listed(st, &op->lists, op->V, a.part, p.parts, state, loss, "linear_loss");
+    else if (p.bm == 64) FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 64, 64, BK>), g, dim3(LN_NT), 0, st, a);
+    else FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 32, 64, 64>), g, dim3(LN_NT), 0, st, a);
+    if (!few) return join_listed(st, &op->lists, op->V, a.part, p.parts, state, loss, "linear_loss");
+    FL_LAUNCH("k_vocab_rows", k_vocab_rows<T>, grid_of(ceil_div(op->M, LS_WAVES)), dim3(LS_NT), 0, st, a,
+              list_args(&op->lists, op->V, state, loss));
+    return fl_check_launch("linear_loss");
 }
 
 template <typename T>
@@ -1042,7 +1171,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
     const dim3 nt(LN_NT), wt(WD_NT);
     const auto fits = [&](int64_t grid) { return launch_fits(grid, WD_NT); };
     const auto fail = [&]() { return fl_fail(FL_ERR_ARG, "linear_loss: too many tiles for one launch (shape)"); };
-    if (std::is_same<T, _Float16>::value || (p.wide && p.pairs))
+    if (std::is_same<T, _Float16>::value || p.wide)
         FL_LAUNCH("k_vocab_coef", k_vocab_coef<true>, dim3(1), dim3(1024), 0, st, a.rows, grad, op->lists.temperature,
                   op->M, coef, coef + op->M);
     else
@@ -1059,7 +1188,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
         int64_t grid = (int64_t)a.m_tiles * a.parts;
         if (!fits(grid)) return fail();
         if (p.wide) {
-            const auto extra = [](int bm) { return (unsigned)(bm * sizeof(float2)); };
+            const auto extra = [](int bm) { return (unsigned)(bm * sizeof(float4)); };
             const dim3 g((unsigned)grid);
             if (p.bm == 128)
                 FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 128, 2, 4>), g, wt, tiles_bytes(128, 128, 4) + extra(128), st, a);
@@ -1069,8 +1198,9 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
                 FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 256, 4, 2>), g, wt, tiles_bytes(256, 256, 2) + extra(256), st, a);
         } else if (p.bm == 128)
             FL_LAUNCH("k_vocab_grad", (k_vocab_grad<T, 128, 128, BK>), dim3((unsigned)grid), nt, 0, st, a);
-        else FL_LAUNCH("k_vocab_grad", (k_vocab_grad<T, 64, 64, BK>), dim3((unsigned)grid), nt, 0, st, a);
-        if (op->lists.k) {
+        else if (p.bm == 64) FL_LAUNCH("k_vocab_grad", (k_vocab_grad<T, 64, 64, BK>), dim3((unsigned)grid), nt, 0, st, a);
+        else FL_LAUNCH("k_vocab_grad", (k_vocab_grad<T, 32, 64, 64>), dim3((unsigned)grid), nt, 0, st, a);
+        if (op->lists.k > 1 || (op->lists.k && !p.wide)) {
             const dim3 g = grid_of(ceil_div(op->M * op->lists.k, LS_NT));
             if (p.wide) FL_LAUNCH("k_vocab_listed", (k_vocab_listed<T, true>), g, dim3(LS_NT), 0, st, a);
             else FL_LAUNCH("k_vocab_listed", (k_vocab_listed<T, false>), g, dim3(LS_NT), 0, st, a);
@@ -1125,9 +1255,13 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
         if (db) {
             a.parts = (uint32_t)s.db_parts;
             a.sums = (float *)(ws + s.db);
-            const dim3 cg = grid_of(a.parts * ceil_div(a.width, LS_NT)), g = grid_of(ceil_div(a.width, FL_WAVE * 4));
-            if (p.wide) FL_LAUNCH("k_vocab_cols", (k_vocab_cols<T, true>), cg, dim3(LS_NT), 0, st, a);
-            else FL_LAUNCH("k_vocab_cols", (k_vocab_cols<T, false>), cg, dim3(LS_NT), 0, st, a);
+            const dim3 g = grid_of(ceil_div(a.width, FL_WAVE * 4));
+            if (p.wide)
+                FL_LAUNCH("k_wide_cols", k_wide_cols<is_pairs<T>()>, grid_of(a.parts * ceil_div(a.width, COLS_WIDE)),
+                          dim3(LS_NT), 0, st, a);
+            else
+                FL_LAUNCH("k_vocab_cols", k_vocab_cols<T>, grid_of(a.parts * ceil_div(a.width, LS_NT)), dim3(LS_NT), 0,
+                          st, a);
             const float *none = nullptr;
             if (op->bias_f32)
                 FL_LAUNCH("k_vocab_fold", k_vocab_fold<float>, g, dim3(LS_NT), 0, st, a.sums, a.parts, a.width,
