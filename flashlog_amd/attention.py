@@ -311,10 +311,13 @@ def _norm_op(x, weight, bias, eps, wide):
 
 def _norm_forward(x, weight, bias, eps, wide, keep):
     """(y, the laid out x, weight and bias, the rows' statistics or None)."""
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     x = _rows_of(x, x.shape[-1])
-    weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias))
-    stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device) if keep else None
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    stats = x.new_empty((x.shape[0], 2), dtype=torch.float32) if keep else None
     _launch("layer_norm", _lib_handle().fl_norm_forward, x.device, _norm_op(x, weight, bias, eps, wide), y.data_ptr(),
             _ptr(stats))
     return y, x, weight, stats
@@ -334,10 +337,10 @@ class _NormFunction(autograd.Function):
         x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev, lib, grad = x.device, _lib_handle(), grad.contiguous()
-        make = torch.empty if x.shape[0] else torch.zeros  # the sums over no rows
-        dx = torch.empty(ctx.shape, dtype=x.dtype, device=dev) if need_x else None
-        dw = make(x.shape[1], dtype=ctx.dtype, device=dev) if need_w else None
-        db = make(x.shape[1], dtype=ctx.dtype, device=dev) if need_b else None
+        make = x.new_empty if x.shape[0] else x.new_zeros  # the sums over no rows
+        dx = x.new_empty(ctx.shape) if need_x else None
+        dw = make(x.shape[1], dtype=ctx.dtype) if need_w else None
+        db = make(x.shape[1], dtype=ctx.dtype) if need_b else None
         if x.numel():
             op = _norm_op(x, weight, None, ctx.eps, ctx.wide)
             nbytes = lib.fl_norm_backward_bytes(op, need_w or need_b)

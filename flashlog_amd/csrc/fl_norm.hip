@@ -6,15 +6,20 @@
 //   dw = sum over the rows of gy h,      db = sum over the rows of gy
 //
 // HBM-bound: one read and one write of the rows forward, two reads and one
-// write backward.  A row is in the registers of one wave (up to 2048 columns)
-// or of a workgroup's four (up to 8192), 16 bytes a lane and load, so that the
-// mean is known before the deviations are squared (no cancellation, whatever
-// the mean); longer rows are read again for each sum.  mean and r are kept in
-// fp32 for the backward, 8 bytes a row.
+// write backward.  A row is in the registers of one wave (up to 512 columns) or
+// of a workgroup's four (up to 8192), 16 bytes a lane and load, so that the mean
+// is known before the deviations are squared (no cancellation, whatever the
+// mean); longer rows are read again for each sum.  mean and r are kept in fp32
+// for the backward, 8 bytes a row.  Waves walk the rows with the weight in
+// registers and the next row's loads under way.
 //
-// dw and db: a wave walks its share of the rows with the sums of its columns
-// in registers, the waves of a workgroup are added through LDS, and a second
-// launch adds the workgroups in a fixed order.
+// dw and db: the sums of a lane's columns stay in registers over the walk, waves
+// with rows of their own are added through LDS, and a second launch adds the
+// workgroups in a fixed order.
+//
+// [16384 x 2048] bf16: 33 us forward, 46 + 5 backward = 4.1 and 4.4 TB/s (a copy
+// 4.7 on the same card); with a wave a row of 2048 columns 35 and 60 + 4, without
+// the next row's loads 49 and 56 + 7.
 #include "fl_abi.h"
 #include "fl_common.h"
 
@@ -24,8 +29,13 @@ namespace {
 constexpr int NM_WAVES = 4;
 constexpr int NM_NT = NM_WAVES * FL_WAVE;
 constexpr int NM_LANE = 32;                     // most values of a row that a lane holds
-constexpr int NM_WAVE_COLS = NM_LANE * FL_WAVE;  // 2048
-constexpr int NM_ROW_COLS = NM_WAVE_COLS * NM_WAVES;
+constexpr int NM_WAVE_COLS = 512;
+constexpr int NM_ROW_COLS = NM_LANE * FL_WAVE * NM_WAVES;
+// Most workgroups that walk the rows: forward ([16384 x 2048] bf16, us with 512, 1024,
+// 1536, 4096 of them 53, 37, 31, 33) and backward, each of which leaves a row of sums
+// (with 512, 1024, 1536, 2048 of them 68 + 4, 46 + 5, 56 + 6, 51 + 8).
+constexpr int64_t NM_WALKS = 4096;
+constexpr int64_t NM_GRAD_WALKS = 1024;
 
 struct NormArgs {
     const void *x, *gy, *weight, *bias;
@@ -89,12 +99,25 @@ __device__ __forceinline__ void store_cols(U *row, int64_t c, int64_t N, const f
             if (c + e < N) row[c + e] = (U)v[e];
 }
 
+// A wave's sum, the same in all lanes: moves within the vector unit (through LDS,
+// as shuffles go, a row's two sums took longer than its loads).
+__device__ __forceinline__ float wave_sum(float v) {
+    const auto add = [&](int moved) { v += __int_as_float(moved); };
+    add(fl_dpp<0x111>(__float_as_int(v)));
+    add(fl_dpp<0x112>(__float_as_int(v)));
+    add(fl_dpp<0x114>(__float_as_int(v)));
+    add(fl_dpp<0x118>(__float_as_int(v)));
+    add(fl_dpp<0x142, 0xa>(__float_as_int(v)));
+    add(fl_dpp<0x143, 0xc>(__float_as_int(v)));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), FL_WAVE - 1));
+}
+
 // Sums of S values a thread over the WPR waves of a row.  `lds`: [2][NM_WAVES][S],
 // `turn` alternates, so that one barrier a sum is enough.
 template <int WPR, int S>
 __device__ __forceinline__ void row_sums(float (&v)[S], float *lds, int &turn) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) v[s] = fl_wave_sum_f32(v[s]);
+    for (int s = 0; s < S; ++s) v[s] = wave_sum(v[s]);
     if constexpr (WPR > 1) {
         float *at = lds + (turn & 1) * NM_WAVES * 2;
         ++turn;
@@ -107,55 +130,107 @@ __device__ __forceinline__ void row_sums(float (&v)[S], float *lds, int &turn) {
     }
 }
 
-// PER loads of a lane; WPR waves a row (1 or all).
+// A lane's part of a row as it lies in memory, so that the next row's can be under
+// way while this one's is worked on.
+template <typename T, int PER>
+struct RowPart {
+    static constexpr int G = 16 / (int)sizeof(T);
+    T v[PER][G];
+
+    // The columns c0 + p step .., 0 behind the last: loads without branches around
+    // them (each would be waited for by itself).  The group that a row ends in is
+    // read from its last G columns and moved.
+    __device__ __forceinline__ void load(const T *row, int c0, int step, int N) {
+        if (N < G) {
+#pragma unroll
+            for (int p = 0; p < PER; ++p)
+#pragma unroll
+                for (int e = 0; e < G; ++e) v[p][e] = c0 + p * step + e < N ? row[c0 + p * step + e] : (T)0.0f;
+            return;
+        }
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+            const int c = c0 + p * step;
+            __builtin_memcpy(v[p], row + (c < N - G ? c : N - G), sizeof(v[p]));
+        }
+        if (N % G == 0 && N == PER * step) return;
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+            const int over = c0 + p * step - (N - G);
+            if (over <= 0) continue;
+#pragma unroll
+            for (int d = 1; d < G; d *= 2)
+                if (over & d)
+#pragma unroll
+                    for (int e = 0; e < G; ++e) v[p][e] = e + d < G ? v[p][e + d] : (T)0.0f;
+            if (over >= G)
+#pragma unroll
+                for (int e = 0; e < G; ++e) v[p][e] = (T)0.0f;
+        }
+    }
+};
+
+// PER loads of a lane; WPR waves a row (1 or all), which walk the rows with the
+// weight and bias in registers.
 template <typename T, typename W, int PER, int WPR>
 __global__ __launch_bounds__(NM_NT) void k_norm_rows(NormArgs a) {
     constexpr int G = 16 / (int)sizeof(T);
     __shared__ float lds[2 * NM_WAVES * 2];
     int turn = 0;
-    const int64_t row = WPR == 1 ? fl_block() * NM_WAVES + fl_wave_id() : fl_block();
-    if (row >= a.M) return;
+    const int64_t first = WPR == 1 ? (int64_t)blockIdx.x * NM_WAVES + fl_wave_id() : blockIdx.x;
+    const int64_t stride = (int64_t)gridDim.x * (WPR == 1 ? NM_WAVES : 1);
+    if (first >= a.M) return;
     const int64_t N = a.N, c0 = (int64_t)(WPR == 1 ? fl_lane() : threadIdx.x) * G, step = (int64_t)WPR * FL_WAVE * G;
-    const T *x = (const T *)a.x + row * a.ldx;
-    float v[PER][G], s[1] = {0.0f};
-#pragma unroll
-    for (int p = 0; p < PER; ++p) load_cols<T, T>(x, c0 + p * step, N, v[p]);
-#pragma unroll
-    for (int p = 0; p < PER; ++p)
-#pragma unroll
-        for (int e = 0; e < G; ++e) s[0] += v[p][e];
-    row_sums<WPR, 1>(s, lds, turn);
-    const float inv = 1.0f / (float)N, mean = s[0] * inv;
-    s[0] = 0.0f;
-#pragma unroll
-    for (int p = 0; p < PER; ++p)
-#pragma unroll
-        for (int e = 0; e < G; ++e) {
-            v[p][e] = c0 + p * step + e < N ? v[p][e] - mean : 0.0f;
-            s[0] = __builtin_fmaf(v[p][e], v[p][e], s[0]);
-        }
-    row_sums<WPR, 1>(s, lds, turn);
-    const float r = 1.0f / sqrtf(s[0] * inv + a.eps);
-    if (a.stats && (WPR == 1 ? fl_lane() : (int)threadIdx.x) == 0) {
-        a.stats[row * 2] = mean;
-        a.stats[row * 2 + 1] = r;
-    }
-    T *y = (T *)a.y + row * N;
+    const T *x = (const T *)a.x;
+    const float inv = 1.0f / (float)N;
+    RowPart<T, PER> next;
+    next.load(x + first * a.ldx, (int)c0, (int)step, (int)N);
+    float w[PER][G], b[PER][G];
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
-        const int64_t c = c0 + p * step;
-        if (c >= N) continue;
-        float w[G], b[G];
-        if (a.weight) load_cols<T, W>((const W *)a.weight, c, N, w);
-        if (a.bias) load_cols<T, W>((const W *)a.bias, c, N, b);
+        if (a.weight) load_cols<T, W>((const W *)a.weight, c0 + p * step, N, w[p]);
+        if (a.bias) load_cols<T, W>((const W *)a.bias, c0 + p * step, N, b[p]);
+    }
+    for (int64_t row = first; row < a.M; row += stride) {
+        float v[PER][G], s[1] = {0.0f};
 #pragma unroll
-        for (int e = 0; e < G; ++e) {
-            float h = v[p][e] * r;
-            if (a.weight) h *= w[e];
-            if (a.bias) h += b[e];
-            v[p][e] = h;
+        for (int p = 0; p < PER; ++p)
+#pragma unroll
+            for (int e = 0; e < G; ++e) {
+                v[p][e] = (float)next.v[p][e];
+                s[0] += v[p][e];
+            }
+        if (row + stride < a.M) next.load(x + (row + stride) * a.ldx, (int)c0, (int)step, (int)N);
+        row_sums<WPR, 1>(s, lds, turn);
+        const float mean = s[0] * inv;
+        s[0] = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PER; ++p)
+#pragma unroll
+            for (int e = 0; e < G; ++e) {
+                v[p][e] = c0 + p * step + e < N ? v[p][e] - mean : 0.0f;
+                s[0] = __builtin_fmaf(v[p][e], v[p][e], s[0]);
+            }
+        row_sums<WPR, 1>(s, lds, turn);
+        const float r = 1.0f / sqrtf(s[0] * inv + a.eps);
+        if (a.stats && (WPR == 1 ? fl_lane() : (int)threadIdx.x) == 0) {
+            a.stats[row * 2] = mean;
+            a.stats[row * 2 + 1] = r;
         }
-        store_cols<T, T>(y, c, N, v[p]);
+        T *y = (T *)a.y + row * N;
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+            const int64_t c = c0 + p * step;
+            if (c >= N) continue;
+#pragma unroll
+            for (int e = 0; e < G; ++e) {
+                float h = v[p][e] * r;
+                if (a.weight) h *= w[p][e];
+                if (a.bias) h += b[p][e];
+                v[p][e] = h;
+            }
+            store_cols<T, T>(y, c, N, v[p]);
+        }
     }
 }
 
@@ -230,15 +305,25 @@ __global__ __launch_bounds__(NM_NT) void k_norm_grad(NormArgs a) {
             dw[p][e] = db[p][e] = 0.0f;
         }
     }
+    RowPart<T, PER> next_x, next_g;
+    float2 next_of = {0.0f, 0.0f};
+    const auto load = [&](int64_t row) {
+        next_x.load((const T *)a.x + row * a.ldx, (int)c0, (int)step, (int)N);
+        next_g.load((const T *)a.gy + row * N, (int)c0, (int)step, (int)N);
+        next_of = *reinterpret_cast<const float2 *>(a.stats_in + row * 2);
+    };
+    if (first < a.M) load(first);
     for (int64_t row = first; row < a.M; row += stride) {
-        const T *x = (const T *)a.x + row * a.ldx, *gy = (const T *)a.gy + row * N;
-        const float mean = a.stats_in[row * 2], r = a.stats_in[row * 2 + 1];
+        const float mean = next_of.x, r = next_of.y;
         float h[PER][G], g[PER][G], s[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int p = 0; p < PER; ++p) {
-            load_cols<T, T>(x, c0 + p * step, N, h[p]);
-            load_cols<T, T>(gy, c0 + p * step, N, g[p]);
-        }
+        for (int p = 0; p < PER; ++p)
+#pragma unroll
+            for (int e = 0; e < G; ++e) {
+                h[p][e] = (float)next_x.v[p][e];
+                g[p][e] = (float)next_g.v[p][e];
+            }
+        if (row + stride < a.M) load(row + stride);
 #pragma unroll
         for (int p = 0; p < PER; ++p)
 #pragma unroll
@@ -350,16 +435,19 @@ __global__ __launch_bounds__(NM_NT) void k_norm_cols(NormArgs a, int parts) {
     a.part[(part * 2 + 1) * a.N + c] = db;
 }
 
-// dw and db from the parts, in order: 64 columns and four runs of the parts a workgroup.
+// dw and db from the parts: 64 columns and sixteen runs of the parts a workgroup,
+// each in order, then the runs.
+constexpr int NM_FOLD = 16;
+
 template <typename W>
-__global__ __launch_bounds__(NM_NT) void k_norm_fold(const float *__restrict__ part, int parts, int64_t N,
-                                                     W *__restrict__ dw, W *__restrict__ db) {
-    __shared__ float runs[NM_WAVES][FL_WAVE];
+__global__ __launch_bounds__(NM_FOLD *FL_WAVE) void k_norm_fold(const float *__restrict__ part, int parts, int64_t N,
+                                                                 W *__restrict__ dw, W *__restrict__ db) {
+    __shared__ float runs[NM_FOLD][FL_WAVE];
     const int64_t i = fl_block() * FL_WAVE + fl_lane();
     float s = 0.0f;
     if (i < 2 * N) {
-        int p = parts * fl_wave_id() / NM_WAVES;
-        const int p1 = parts * (fl_wave_id() + 1) / NM_WAVES;
+        int p = parts * fl_wave_id() / NM_FOLD;
+        const int p1 = parts * (fl_wave_id() + 1) / NM_FOLD;
         for (; p + 8 <= p1; p += 8) {
             float v[8];
 #pragma unroll
@@ -373,7 +461,11 @@ __global__ __launch_bounds__(NM_NT) void k_norm_fold(const float *__restrict__ p
     __syncthreads();
     if (fl_wave_id() || i >= 2 * N) return;
     W *to = i < N ? dw : db;
-    if (to) to[i < N ? i : i - N] = (W)((runs[0][fl_lane()] + runs[1][fl_lane()]) + (runs[2][fl_lane()] + runs[3][fl_lane()]));
+    if (!to) return;
+    s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NM_FOLD; ++w) s += runs[w][fl_lane()];
+    to[i < N ? i : i - N] = (W)s;
 }
 
 // Workgroups that walk the rows for dw and db.
@@ -384,7 +476,7 @@ int grad_groups(const fl_norm *op, bool with_dw) {
         const int64_t p = op->M / 32;
         return (int)(p < 1 ? 1 : p > 64 ? 64 : p);
     }
-    const int64_t most = with_dw ? 512 : 1 << 22;
+    const int64_t most = with_dw ? NM_GRAD_WALKS : 1 << 22;
     return (int)(all < most ? all : most);
 }
 
@@ -436,8 +528,9 @@ int forward(hipStream_t st, const fl_norm *op, void *y, float *stats) {
     }
     by_cols<T>(op->N, [&](auto per, auto wpr) {
         constexpr int PER = decltype(per)::value, WPR = decltype(wpr)::value;
-        const int64_t rows = WPR == 1 ? NM_WAVES : 1;
-        FL_LAUNCH("k_norm_rows", (k_norm_rows<T, W, PER, WPR>), grid_of((op->M + rows - 1) / rows), dim3(NM_NT), 0, st, a);
+        const int64_t rows = WPR == 1 ? NM_WAVES : 1, all = (op->M + rows - 1) / rows;
+        FL_LAUNCH("k_norm_rows", (k_norm_rows<T, W, PER, WPR>), dim3((unsigned)(all < NM_WALKS ? all : NM_WALKS)),
+                  dim3(NM_NT), 0, st, a);
     });
     return fl_check_launch("layer_norm");
 }
@@ -463,7 +556,8 @@ int backward(hipStream_t st, const fl_norm *op, const void *gy, const float *sta
             FL_LAUNCH("k_norm_grad", (k_norm_grad<T, W, PER, WPR>), dim3(groups), dim3(NM_NT), 0, st, a);
         });
     if (a.with_dw)
-        FL_LAUNCH("k_norm_fold", k_norm_fold<W>, grid_of((2 * op->N + FL_WAVE - 1) / FL_WAVE), dim3(NM_NT), 0, st, ws,
+        FL_LAUNCH("k_norm_fold", k_norm_fold<W>, grid_of((2 * op->N + FL_WAVE - 1) / FL_WAVE),
+                  dim3(NM_FOLD * FL_WAVE), 0, st, ws,
                   groups, op->N, (W *)dw, (W *)db);
     return fl_check_launch("layer_norm");
 }

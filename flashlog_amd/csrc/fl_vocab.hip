@@ -445,36 +445,50 @@ constexpr bool is_scaled() {
 }
 
 // The largest finite magnitude of x and of weight, a part of them a workgroup.
-constexpr int LAY_PARTS = 512;
+constexpr int LAY_PARTS = 1024;
 
 template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restrict__ most) {
     constexpr int G = 16 / (int)sizeof(T);
     __shared__ float waves[LS_WAVES];
     const bool second = blockIdx.y;
-    const int64_t R = second ? a.op.V : a.op.M, ld = second ? a.op.ldw : a.op.ldx, K = a.op.K, groups = (K + G - 1) / G;
+    // rows without gaps are one
+    int64_t R = second ? a.op.V : a.op.M, K = a.op.K;
+    const int64_t ld = second ? a.op.ldw : a.op.ldx;
+    if (ld == K) {
+        K *= R;
+        R = 1;
+    }
     const T *p = (const T *)(second ? a.op.weight : a.op.x);
     float m = 0.0f;
-    const auto see = [&](T t) {
-        const float v = fabsf((float)t);
-        m = fmaxf(m, v < INFINITY ? v : 0.0f);
+    const auto see = [&](const Vec<T, G> &v) {
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+            const float t = fabsf((float)v.v[e]);
+            m = fmaxf(m, t < INFINITY ? t : 0.0f);
+        }
     };
-    const int64_t all = R * groups, step = (int64_t)LAY_PARTS * LS_NT;
-    const auto take = [&](int64_t i, Vec<T, G> &v) {
-        const int64_t r = i / groups, c = (i - r * groups) * G;
-        if (c + G <= K) v = load_vec<T, G>(p + r * ld + c);
-        else
+    // a row to a workgroup, or one to all of them
+    const int64_t step = (R == 1 ? LAY_PARTS : 1) * (int64_t)LS_NT * G;
+    const int64_t c0 = ((R == 1 ? (int64_t)blockIdx.x : 0) * LS_NT + threadIdx.x) * G;
+    for (int64_t r = R == 1 ? 0 : blockIdx.x; r < R; r += LAY_PARTS) {
+        const T *row = p + r * ld;
+        int64_t c = c0;
+        for (; c + 7 * step + G <= K; c += 8 * step) {
+            Vec<T, G> v[8];
 #pragma unroll
-            for (int e = 0; e < G; ++e) v.v[e] = c + e < K ? p[r * ld + c + e] : (T)0.0f;
-    };
-    for (int64_t i = (int64_t)blockIdx.x * LS_NT + threadIdx.x; i < all; i += 4 * step) {
-        Vec<T, G> v[4];
+            for (int j = 0; j < 8; ++j) v[j] = load_vec<T, G>(row + c + j * step);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) take(i + j * step < all ? i + j * step : i, v[j]);
+            for (int j = 0; j < 8; ++j) see(v[j]);
+        }
+        for (; c < K; c += step) {
+            Vec<T, G> v;
+            if (c + G <= K) v = load_vec<T, G>(row + c);
+            else
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < G; ++e) see(v[j].v[e]);
+                for (int e = 0; e < G; ++e) v.v[e] = c + e < K ? row[c + e] : (T)0.0f;
+            see(v);
+        }
     }
 #pragma unroll
     for (int o = FL_WAVE / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));

@@ -79,7 +79,7 @@ def _vocab_op(x, weight, bias, lists):
 def _vocab_forward(what, x, weight, bias, lists):
     """(losses, x, weight and bias as the call took them, the state and the layout for the backward)."""
     dev, lib = x.device, _lib_handle()
-    loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    loss = x.new_empty(x.shape[:-1], dtype=torch.float32)
     x = _rows_of(x, x.shape[-1])
     if weight.shape[1] > 1 and weight.stride(1) != 1:
         weight = weight.contiguous()
@@ -108,10 +108,10 @@ class _VocabFunction(autograd.Function):
         x, weight, bias, state, layout = ctx.saved_tensors[:5]
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev, lib, grad = x.device, _lib_handle(), grad.contiguous()
-        make = torch.empty if x.shape[0] else torch.zeros  # the sums over no rows
-        dx = torch.empty(ctx.shape, dtype=x.dtype, device=dev) if need_x else None
-        dw = make(weight.shape, dtype=x.dtype, device=dev) if need_w else None
-        db = make(weight.shape[0], dtype=bias.dtype, device=dev) if need_b else None
+        make = x.new_empty if x.shape[0] else x.new_zeros  # the sums over no rows
+        dx = x.new_empty(ctx.shape) if need_x else None
+        dw = make(weight.shape) if need_w else None
+        db = make(weight.shape[0], dtype=bias.dtype) if need_b else None
         if x.shape[0]:
             op = _vocab_op(x, weight, bias, ctx.lists)
             nbytes = lib.fl_vocab_backward_bytes(op, need_x, need_w, need_b)
@@ -186,7 +186,7 @@ def _scores_op(logits, lists):
 def _scores_forward(logits, lists):
     """(losses, the laid out logits, the state for the backward)."""
     dev, lib = logits.device, _lib_handle()
-    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+    loss = logits.new_empty(logits.shape[:-1], dtype=torch.float32)
     x = _rows_of(logits, logits.shape[-1])
     op = _scores_op(x, lists)
     state = _workspace(lib.fl_lists_state_bytes(op.lists), dev)
@@ -208,7 +208,7 @@ class _ScoresFunction(autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         x, state = ctx.saved_tensors[:2]
-        dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device)
+        dx = x.new_empty(ctx.shape)
         if dx.numel():
             _launch("distillation", _lib_handle().fl_scores_backward, x.device, _scores_op(x, ctx.lists),
                     grad.contiguous().data_ptr(), _ptr(state), dx.data_ptr())
