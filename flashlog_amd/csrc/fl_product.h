@@ -414,6 +414,7 @@ template <int BR>
 struct StepsContig {
     using At = WideContig<BR, 64>;
     static constexpr int LOADS = At::LOADS, ELEMS = At::ELEMS;
+    static constexpr bool BLOCKING = false;
     const uint16_t *base;  // of the next step
     uint32_t at[LOADS];    // bytes
 
@@ -544,6 +545,7 @@ template <int BR, bool PAIRS>
 struct StepsStrided {
     using At = WideStrided<BR, 64, false>;
     static constexpr int LOADS = At::LOADS, ELEMS = At::ELEMS, STEP = PAIRS ? 32 : 64;
+    static constexpr bool BLOCKING = true;
     const uint16_t *base;  // of the next step
     int64_t ld;
     uint32_t at[LOADS];  // bytes
@@ -842,23 +844,33 @@ struct WideTiles {
             }
         } else {
             static_assert(!PAIRS, "two planes of such tiles have no registers");
-            u32x4 a0[MT], b0[NTL];
+            // operands whose reads are waited for at once: half the waves read first, half multiply first
+            const bool later = TA::BLOCKING && TB::BLOCKING && fl_wave_id() >= WD_WAVES / 2;
+            u32x4 a0[MT], b0[NTL], a1[MT], b1[NTL];
             ta.template read<0>(la, wave_m(), a0);
             tb.template read<0>(la + TA::ELEMS, wave_n(), b0);
-            for (int s = 0; s < all; ++s) {
-                u32x4 a1[MT], b1[NTL];
+            const auto second_half = [&]() {
                 tb.template read<1>(la + TA::ELEMS, wave_n(), b1);
                 ta.template read<1>(la, wave_m(), a1);
+            };
+            const auto first_half = [&]() {
+                tb.template read<0>(la + TA::ELEMS, wave_n(), b0);
+                ta.template read<0>(la, wave_m(), a0);
+            };
+            for (int s = 0; s < all; ++s) {
+                if (!later) second_half();
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(a0, b0, none);
                 __builtin_amdgcn_sched_barrier(0);
+                if (later) second_half();
                 Waits::template wait<LOADS *(STAGES - 2)>();
                 Waits::meet();
                 go_on();
-                tb.template read<0>(la + TA::ELEMS, wave_n(), b0);
-                ta.template read<0>(la, wave_m(), a0);
+                if (!later) first_half();
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(a1, b1, load_between);
+                __builtin_amdgcn_sched_barrier(0);
+                if (later) first_half();
                 finished();
             }
         }

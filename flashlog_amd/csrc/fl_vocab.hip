@@ -5,9 +5,8 @@
 //
 //   dx = dz W      dW = dz^T x      db = sum over the rows of dz
 //
-// The piece of dz is what a call holds of [rows x vocabulary], in the
-// operands' type (an operand of two products), small enough for the last level
-// cache.  The listed columns' own u comes from a dot product each; their
+// The piece of dz is what a call holds of [rows x vocabulary], in 16 bits (an
+// operand of two products; fp32: two planes).  The listed columns' own u comes from a dot product each; their
 // entries of dz are made apart, since p - q of values rounded before would
 // keep few bits where p is near 1.
 //
@@ -29,7 +28,14 @@ namespace {
 
 constexpr int LS_NT = 256;
 constexpr int LS_WAVES = LS_NT / FL_WAVE;
-constexpr size_t LS_PIECE = 128u << 20;  // bytes of dz
+// Bytes of dz: with 128 MB, which the last level cache holds, [8192 x 512 -> 41000]
+// bf16 train takes 1850 us, with 512 MB and 1 GB 1640 ([512 x 128 -> 4.6M] 6480,
+// 6460 and 6100): fewer beginnings and ends of kernels.
+constexpr size_t LS_PIECE = 1u << 30;
+
+// The wide kernels' dz lies in blocks of so many columns, each row of a block
+// behind the one before it: a tile's rows are one piece of memory.
+constexpr int D_BLOCK = 256;
 
 struct VocabArgs {
     fl_vocab op;
@@ -41,8 +47,8 @@ struct VocabArgs {
     const float2 *rows;
     float2 *listed;
     const float *coef;    // tau g of every row (times a power of two), 0 where it has no gradient
-    void *d;              // dz of the piece: [M][ldd]
-    int64_t ldd;
+    void *d;              // dz of the piece: [M][ldd], wide: blocks of D_BLOCK columns, [d_rows][ldd] each
+    int64_t ldd, d_block;  // d_block: from one to the next
     float *sums;          // dx: [parts][M][K]; dW: [parts][width][K]
     void *dw;
     void *dx;             // where one part and one piece are all of it
@@ -130,6 +136,14 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_rows(VocabArgs a, ListArgs l) {
     list_row(l, row, r, lists[fl_wave_id()], [&](int64_t j, int64_t) {
         return j == 0 ? s[0] : j == 1 ? s[1] : j == 2 ? s[2] : s[3];
     });
+}
+
+// Where the wide kernels' dz of row m and column c (of the piece) is; PAIRS: its
+// first plane's, the second is 32 values behind it.
+template <bool PAIRS>
+__device__ __forceinline__ int64_t dz_at(const VocabArgs &a, int64_t m, int64_t c) {
+    const int in = (int)(c % D_BLOCK);
+    return c / D_BLOCK * a.d_block + m * a.ldd + (PAIRS ? pair_at(in) : in);
 }
 
 // The logits of a lane's tiles in units of log 2, -inf behind the vocabulary:
@@ -289,10 +303,10 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
     const float2 l = a.listed[i];
     const float d = c * (exp2_of(l.x - a.rows[row].x) - l.y);
     if constexpr (WIDE && sizeof(T) == 4) {
-        _Float16 *to = (_Float16 *)a.d + row * a.ldd + pair_at(v);
+        _Float16 *to = (_Float16 *)a.d + dz_at<true>(a, row, v);
         to[0] = (_Float16)d;
         to[32] = (_Float16)(d - (float)to[0]);
-    } else if constexpr (WIDE) ((_Float16 *)a.d)[row * a.ldd + v] = (_Float16)d;
+    } else if constexpr (WIDE) ((_Float16 *)a.d)[dz_at<false>(a, row, v)] = (_Float16)d;
     else ((T *)a.d)[row * a.ldd + v] = (T)d;
 }
 
@@ -764,7 +778,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
                     Vec<_Float16, 8> o;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) o.v[e] = (_Float16)u[h * 8 + e];
-                    _Float16 *to = (_Float16 *)a.d + (row0 + r) * a.ldd + (is_pairs<T>() ? pair_at(c + h * 8) : c + h * 8);
+                    _Float16 *to = (_Float16 *)a.d + dz_at<is_pairs<T>()>(a, row0 + r, c + h * 8);
                     store_vec<_Float16, 8>(to, o);
                     if constexpr (is_pairs<T>()) {
 #pragma unroll
@@ -796,7 +810,7 @@ __global__ __launch_bounds__(LS_NT) void k_wide_cols(VocabArgs a) {
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const int64_t r = m + j < end ? m + j : end - 1;
-                const _Float16 *d = (const _Float16 *)a.d + r * a.ldd + (PAIRS ? pair_at(c) : c);
+                const _Float16 *d = (const _Float16 *)a.d + dz_at<PAIRS>(a, r, c);
                 v[j] = load_vec<_Float16, 8>(d);
                 if (PAIRS) w[j] = load_vec<_Float16, 8>(d + 32);
             }
@@ -832,7 +846,9 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
     TA ta;
     TB tb;
     const int most = (int)(M - 1 - row0 < BM ? M - 1 - row0 : BM);
-    ta.init((const uint16_t *)a.d + row0 * a.ldd + s0 * 64, a.ldd, [&](int r) { return r < most ? r : most; });
+    constexpr int IN_BLOCK = D_BLOCK / STEP;  // steps
+    ta.init((const uint16_t *)a.d + s0 / IN_BLOCK * a.d_block + row0 * a.ldd + s0 % IN_BLOCK * 64, a.ldd,
+            [&](int r) { return r < most ? r : most; });
     const auto aim = [&](int64_t step) {  // dz is 0 behind the piece
         const int64_t v = step * STEP, left = a.width - v;
         tb.init(a.w + (a.v0 + v) * a.ldw + (PAIRS ? 2 * n0 : n0), a.ldw, a.cols - n0, left < STEP ? (int)left : STEP);
@@ -849,6 +865,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
             if (i < Run::LOADS - 1 || ++next >= s1) return;
             ta.next();
             tb.next();
+            if (next % IN_BLOCK == 0) ta.base += a.d_block - a.ldd;
             if (next == all - 1) aim(next);
         },
         [&](int64_t) {
@@ -910,7 +927,9 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
     int at = 0;
     const auto aim = [&](int64_t step) {  // dz is 0 in the rows behind the last
         const int64_t k = step * STEP, left = a.op.M - k;
-        ta.init((const uint16_t *)a.d + k * a.ldd + (PAIRS ? 2 * m0 : m0), a.ldd, a.d_cols - m0, STEP);
+        const int in = (int)(m0 % D_BLOCK);
+        ta.init((const uint16_t *)a.d + m0 / D_BLOCK * a.d_block + k * a.ldd + (PAIRS ? 2 * in : in), a.ldd, D_BLOCK - in,
+                STEP);
         tb.init(a.x + k * a.ldx + (PAIRS ? 2 * c0 : c0), a.ldx, a.cols - c0, left < STEP ? (int)left : STEP);
     };
     const auto aim_tile = [&]() {
@@ -979,6 +998,7 @@ struct VocabPlan {
     int bm, bn;                        // tiles of the logits
     uint32_t m_tiles, n_tiles, parts;  // parts: of the vocabulary, in the forward
     int64_t piece, d_cols, ldd;        // columns of dz in the backward, with those that pad them, and its row stride
+    int64_t d_block;                   // wide: from one block of its columns to the next
     int64_t d_rows, cols;              // rows of dz and inputs, with those that pad them
     int64_t size;                      // bytes of a value of dz
 };
@@ -1017,11 +1037,11 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     p.parts = (uint32_t)(want < p.n_tiles ? want : p.n_tiles);
     int64_t piece = (int64_t)(LS_PIECE / p.size) / (op->M > 0 ? op->M : 1) / 256 * 256;
     if (piece < 256) piece = 256;
-    if (piece > 1 << 21) piece = 1 << 21;  // 32-bit offsets of 256 rows of dz
     p.piece = piece < op->V ? piece : op->V;
-    p.d_cols = p.wide ? ceil_div(p.piece, step) * step : ceil_div(p.piece, 8) * 8;
+    p.d_cols = p.wide ? ceil_div(p.piece, D_BLOCK) * D_BLOCK : ceil_div(p.piece, 8) * 8;
     p.d_rows = p.wide ? ceil_div(op->M, step) * step : op->M;
-    p.ldd = p.wide && p.pairs ? 2 * p.d_cols : p.d_cols;
+    p.ldd = !p.wide ? p.d_cols : p.pairs ? 2 * D_BLOCK : D_BLOCK;
+    p.d_block = p.d_rows * p.ldd;
     return p;
 }
 
@@ -1057,7 +1077,7 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
     };
     const bool f32 = op->dtype == FL_F32;
     s.coef = take((size_t)(op->M + 1) * 4);
-    s.d = take((size_t)p.d_rows * p.ldd * (p.wide ? 2 : p.size));
+    s.d = take((size_t)p.d_rows * p.d_cols * p.size);
     const int narrow = op->K <= 128 || p.pairs ? 128 : 256;
     if (with_dx) {
         if (p.wide) {
@@ -1180,6 +1200,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
     a.unscale = coef + op->M;
     a.d = ws + s.d;
     a.ldd = p.ldd;
+    a.d_block = p.d_block;
     a.d_cols = p.d_cols;
     a.d_rows = p.d_rows;
     const dim3 nt(LN_NT), wt(WD_NT);

@@ -156,7 +156,7 @@ def linear_cross_entropy(x, weight, target, bias=None):
     of which nothing is left 0 without a gradient.
 
     No logits are kept: the backward computes them again, a piece of the
-    vocabulary at a time, in a workspace of some 128 MB.  Their gradient is
+    vocabulary at a time, in a workspace of up to 1 GB.  Their gradient is
     rounded to the operands' type as an operand of two products and a term of
     the bias's.  Products are as exact as ``attention.linear``'s, softmax terms
     are off by 2^-23 of themselves times 1 + their logit's distance from the
