@@ -141,6 +141,7 @@ class FlVocab(ctypes.Structure):
         ("lists", FlLists), ("M", ctypes.c_int64), ("V", ctypes.c_int64), ("K", ctypes.c_int64),
         ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("weight", ctypes.c_void_p), ("ldw", ctypes.c_int64),
         ("bias", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("bias_f32", ctypes.c_int32),
+        ("train", ctypes.c_int32), ("reserved", ctypes.c_int32),
     ]
 
 

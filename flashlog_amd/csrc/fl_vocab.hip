@@ -448,14 +448,10 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
 // ---------------------------------------------------------------------------
 // The same for large products
 
-// Whether the operands are two planes, and whether they are scaled.
+// Whether the operands are two planes.
 template <typename T>
 constexpr bool is_pairs() {
     return sizeof(T) == 4;
-}
-template <typename T>
-constexpr bool is_scaled() {
-    return !std::is_same<T, _Float16>::value;
 }
 
 // The largest finite magnitude of x and of weight, a part of them a workgroup.
@@ -514,10 +510,10 @@ __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restric
 
 // x and weight as rows of half values on 16 bytes: fp32 as two planes (pair_at),
 // bfloat16 times a power of two that brings the largest to 2^13..2^14 (what is
-// above 2^-31 of it is held exactly, and what is lost below 2^-39), half as it is;
-// zeros behind a row.  (dz, in half, is then rounded by 2^-12 of itself; by 2^-9 in
+// above 2^-31 of it is held exactly, and what is lost below 2^-39), half, and
+// bfloat16 that no backward follows, as they are; zeros behind a row.  (dz, in half, is then rounded by 2^-12 of itself; by 2^-9 in
 // bfloat16 it made the gradients' error 1.4 to 1.5 times that of their own rounding.)
-template <typename T>
+template <typename T, bool SCALED>
 __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restrict__ most, uint16_t *__restrict__ x,
                                                uint16_t *__restrict__ w, float *__restrict__ undo) {
     constexpr bool PAIRS = is_pairs<T>();
@@ -526,7 +522,7 @@ __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restr
     const T *p = (const T *)(second ? a.op.weight : a.op.x);
     uint16_t *out = second ? w : x;
     float scale = 1.0f;
-    if constexpr (is_scaled<T>()) {
+    if constexpr (SCALED) {
         __shared__ float waves[LS_WAVES];
         float m = 0.0f;
         for (int i = threadIdx.x; i < LAY_PARTS; i += LS_NT) m = fmaxf(m, most[blockIdx.y * LAY_PARTS + i]);
@@ -559,26 +555,23 @@ __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restr
             _Float16 *q = (_Float16 *)out + r * 2 * a.cols + pair_at(c);
             store_vec<_Float16, 8>(q, hi);
             store_vec<_Float16, 8>(q + 32, lo);
-        } else {
+        } else if constexpr (SCALED) {
             Vec<_Float16, 8> o;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (is_scaled<T>()) o.v[e] = (_Float16)((float)v.v[e] * scale);
-                else o.v[e] = v.v[e];
-            }
+            for (int e = 0; e < 8; ++e) o.v[e] = (_Float16)((float)v.v[e] * scale);
             store_vec<_Float16, 8>((_Float16 *)out + r * a.cols + c, o);
-        }
+        } else store_vec<T, 8>((T *)out + r * a.cols + c, v);
     }
 }
 
 // Logit tiles: row tiles of x against row tiles of weight from n0 on, whose
 // order in LDS gives a lane 16 columns in a row (16 (lane / 16) .. of the
 // wave's 64).
-template <typename T, int BM, int WN, int STAGES>
+template <typename T, typename H, int BM, int WN, int STAGES>
 struct LogitTiles {
     using TA = StepsContig<BM>;
     using TB = StepsContig<WN * 64>;
-    using Run = WideTiles<_Float16, is_pairs<T>(), BM, WN, STAGES, TA, TB>;
+    using Run = WideTiles<H, is_pairs<T>(), BM, WN, STAGES, TA, TB>;
     TA ta;
     TB tb;
     int steps, at;  // of a tile's row; of the next load
@@ -644,9 +637,9 @@ __device__ __forceinline__ void lane_bias(const VocabArgs &a, int64_t n, float (
     }
 }
 
-template <typename T, int BM, int WN, int STAGES>
+template <typename T, typename H, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
-    using Tiles = LogitTiles<T, BM, WN, STAGES>;
+    using Tiles = LogitTiles<T, H, BM, WN, STAGES>;
     using Run = typename Tiles::Run;
     constexpr int MT = Run::MT;
     extern __shared__ __align__(16) uint16_t wide_lds[];
@@ -718,7 +711,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
 // dz of a piece but for the listed columns.
 template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
-    using Tiles = LogitTiles<T, BM, WN, STAGES>;
+    using Tiles = LogitTiles<T, _Float16, BM, WN, STAGES>;
     using Run = typename Tiles::Run;
     constexpr int MT = Run::MT;
     extern __shared__ __align__(16) uint16_t wide_lds[];
@@ -993,7 +986,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
 
 // How the products of a vocabulary are cut.
 struct VocabPlan {
-    bool wide, pairs, lay;             // wide kernels; two planes; operands laid out
+    bool wide, pairs, lay, scaled;     // wide kernels; two planes; operands laid out, times powers of two
     bool small;                        // tiles of 128
     int bm, bn;                        // tiles of the logits
     uint32_t m_tiles, n_tiles, parts;  // parts: of the vocabulary, in the forward
@@ -1006,14 +999,25 @@ struct VocabPlan {
 VocabPlan vocab_plan(const fl_vocab *op) {
     VocabPlan p{};
     p.pairs = op->dtype == FL_F32;
-    p.wide = op->K >= 1 && op->K <= 1 << 20 && (double)op->M * op->V * op->K >= 1 << 27;
     p.size = p.pairs ? 4 : 2;
     const int64_t step = p.pairs ? 32 : 64;  // inputs of a step of the wide kernels
+    p.scaled = op->dtype == FL_F32 || (op->dtype == FL_BF16 && op->train);
+    p.lay = p.scaled || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % step ||
+            op->ldx >= 1 << 23 || op->ldw >= 1 << 23;  // 32-bit offsets of 256 rows
+    // Laying the weight out takes up to four passes over it, which few rows do not pay for: in units of 1e-12 s a value of
+    // it, fp32 3.5 and then 2 rows / 360 a product, against 2 rows / 150 (0.9 at least) from where it lies, with four
+    // products in training; 16-bit values 0.9 to 1.3 and 2 rows / 1000, against 2 rows / 430 (0.45 at least).  bfloat16 in
+    // training is laid out whatever it costs, so that dz is half.
+    int64_t least = 65;
+    if (op->dtype == FL_F32) least = op->train ? 144 : 448;
+    else if (op->dtype == FL_BF16 && op->train) least = 1;
+    else if (p.lay) least = op->train ? 128 : 384;
+    p.wide = op->K >= 1 && op->K <= 1 << 20 && op->M >= least && (double)op->M * op->V * op->K >= 1 << 27;
+    p.lay = p.lay && p.wide;
+    p.scaled = p.scaled && p.wide;
     if (p.wide) {
-        p.small = ceil_div(op->M, 256) * ceil_div(op->V, 256) < 192;
-        p.lay = op->dtype != FL_F16 || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % step || op->ldx >= 1 << 23 ||
-                op->ldw >= 1 << 23;  // 32-bit offsets of 256 rows
         p.cols = ceil_div(op->K, step) * step;
+        p.small = op->M <= 128 || ceil_div(op->M, 256) * ceil_div(op->V, 256) < 192;
         p.bm = p.small ? 128 : 256;
         p.bn = p.small || p.pairs ? 128 : 256;  // two planes of 256 x 256 have no registers
     } else {
@@ -1088,9 +1092,11 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
             const int64_t n = want < most ? want : most;
             s.dx_parts = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
         } else {
-            const Cut c = best_cut(op->M, op->K, p.piece, f32, false);
-            s.dx_parts = c.parts;
-            s.dx_tile = c.rows == 128 && op->K >= 2 ? 128 : 64;
+            // enough workgroups for the chip, of at least 512 columns
+            s.dx_tile = op->M > 64 && op->K > 64 ? 128 : 64;
+            const int64_t tiles = ceil_div(op->M, s.dx_tile) * ceil_div(op->K, s.dx_tile);
+            const int64_t want = ceil_div(1024, tiles > 0 ? tiles : 1), most = p.piece / 512, n = want < most ? want : most;
+            s.dx_parts = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
         }
         s.dx_direct = p.wide && s.dx_parts == 1 && p.piece == op->V;
         if (!s.dx_direct) s.dx = take((size_t)s.dx_parts * op->M * op->K * 4);
@@ -1133,7 +1139,7 @@ VocabArgs vocab_args(const fl_vocab *op, const VocabPlan &p, void *state, void *
         a.x = (const uint16_t *)((char *)layout + l.x);
         a.w = (const uint16_t *)((char *)layout + l.w);
         a.ldx = a.ldw = p.pairs ? 2 * p.cols : p.cols;
-        if (op->dtype != FL_F16) a.undo = (const float *)((char *)layout + l.undo);
+        if (p.scaled) a.undo = (const float *)((char *)layout + l.undo);
     } else {
         a.x = (const uint16_t *)op->x;
         a.w = (const uint16_t *)op->weight;
@@ -1160,11 +1166,18 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
     if (p.lay) {
         const VocabLayout l = vocab_layout(op, p);
         float *most = (float *)((char *)layout + l.most);
-        if constexpr (is_scaled<T>())
-            FL_LAUNCH("k_lay_max", k_lay_max<T>, dim3(LAY_PARTS, 2), dim3(LS_NT), 0, st, a, most);
         const int64_t chunks = (op->M > op->V ? op->M : op->V) * (p.cols / 8), want = ceil_div(chunks, LS_NT);
-        FL_LAUNCH("k_lay", k_lay<T>, dim3((unsigned)(want < 4096 ? want : 4096), 2), dim3(LS_NT), 0, st, a, most,
-                  (uint16_t *)a.x, (uint16_t *)a.w, (float *)a.undo);
+        const dim3 lg((unsigned)(want < 4096 ? want : 4096), 2);
+        if constexpr (!std::is_same<T, _Float16>::value)
+            if (p.scaled) {
+                FL_LAUNCH("k_lay_max", k_lay_max<T>, dim3(LAY_PARTS, 2), dim3(LS_NT), 0, st, a, most);
+                FL_LAUNCH("k_lay", (k_lay<T, true>), lg, dim3(LS_NT), 0, st, a, most, (uint16_t *)a.x, (uint16_t *)a.w,
+                          (float *)a.undo);
+            }
+        if constexpr (sizeof(T) == 2)
+            if (!p.scaled)
+                FL_LAUNCH("k_lay", (k_lay<T, false>), lg, dim3(LS_NT), 0, st, a, most, (uint16_t *)a.x, (uint16_t *)a.w,
+                          (float *)nullptr);
     }
     const bool few = op->lists.k <= DOT_IDS && p.parts <= 4 * FL_WAVE;
     if (!few)
@@ -1172,12 +1185,19 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
                   grid_of(ceil_div(op->M * ceil_div(op->lists.k, DOT_IDS), LS_WAVES)), dim3(LS_NT), 0, st, a);
     if (p.wide) {
         const auto extra = [](int mt) { return (unsigned)(WD_WAVES * mt * FL_WAVE * sizeof(Running)); };
-        if (p.bm == 128)
-            FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 128, 2, 4>), g, dim3(WD_NT), tiles_bytes(128, 128, 4) + extra(2), st, a);
-        else if constexpr (is_pairs<T>())
-            FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 256, 2, 3>), g, dim3(WD_NT), tiles_bytes(256, 128, 3) + extra(4), st, a);
-        else
-            FL_LAUNCH("k_wide_stats", (k_wide_stats<T, 256, 4, 2>), g, dim3(WD_NT), tiles_bytes(256, 256, 2) + extra(8), st, a);
+        const auto launch = [&](auto half) {
+            using H = decltype(half);
+            if (p.bm == 128)
+                FL_LAUNCH("k_wide_stats", (k_wide_stats<T, H, 128, 2, 4>), g, dim3(WD_NT), tiles_bytes(128, 128, 4) + extra(2), st, a);
+            else if constexpr (is_pairs<T>())
+                FL_LAUNCH("k_wide_stats", (k_wide_stats<T, H, 256, 2, 3>), g, dim3(WD_NT), tiles_bytes(256, 128, 3) + extra(4), st, a);
+            else
+                FL_LAUNCH("k_wide_stats", (k_wide_stats<T, H, 256, 4, 2>), g, dim3(WD_NT), tiles_bytes(256, 256, 2) + extra(8), st, a);
+        };
+        if constexpr (std::is_same<T, __bf16>::value) {
+            if (p.scaled) launch(_Float16());
+            else launch(T());
+        } else launch(_Float16());
     } else if (p.bm == 128)
         FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 128, 128, BK>), g, dim3(LN_NT), 0, st, a);
     else if (p.bm == 64) FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 64, 64, BK>), g, dim3(LN_NT), 0, st, a);

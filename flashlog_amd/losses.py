@@ -70,13 +70,13 @@ def _lists(what, lead, ids, teacher, temperature):
 # Rows that are a product
 
 
-def _vocab_op(x, weight, bias, lists):
+def _vocab_op(x, weight, bias, lists, train):
     return FlVocab(lists.op(), x.shape[0], weight.shape[0], weight.shape[1], x.data_ptr(), x.stride(0),
                    weight.data_ptr(), weight.stride(0), _ptr(bias), _TYPES[x.dtype],
-                   int(bias is not None and bias.dtype is torch.float32))
+                   int(bias is not None and bias.dtype is torch.float32), train, 0)
 
 
-def _vocab_forward(what, x, weight, bias, lists):
+def _vocab_forward(what, x, weight, bias, lists, train):
     """(losses, x, weight and bias as the call took them, the state and the layout for the backward)."""
     dev, lib = x.device, _lib_handle()
     loss = x.new_empty(x.shape[:-1], dtype=torch.float32)
@@ -85,7 +85,7 @@ def _vocab_forward(what, x, weight, bias, lists):
         weight = weight.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    op = _vocab_op(x, weight, bias, lists)
+    op = _vocab_op(x, weight, bias, lists, train)
     state = _workspace(lib.fl_lists_state_bytes(op.lists), dev)
     layout = _workspace(lib.fl_vocab_layout_bytes(op), dev)
     nbytes = lib.fl_vocab_forward_bytes(op)
@@ -97,7 +97,7 @@ def _vocab_forward(what, x, weight, bias, lists):
 class _VocabFunction(autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, lists, what):
-        loss, x2, w2, b2, state, layout = _vocab_forward(what, x, weight, bias, lists)
+        loss, x2, w2, b2, state, layout = _vocab_forward(what, x, weight, bias, lists, True)
         ctx.save_for_backward(x2, w2, b2, state, layout, lists.ids, lists.teacher)
         ctx.lists, ctx.what, ctx.shape = lists, what, x.shape
         return loss
@@ -113,7 +113,7 @@ class _VocabFunction(autograd.Function):
         dw = make(weight.shape) if need_w else None
         db = make(weight.shape[0], dtype=bias.dtype) if need_b else None
         if x.shape[0]:
-            op = _vocab_op(x, weight, bias, ctx.lists)
+            op = _vocab_op(x, weight, bias, ctx.lists, True)
             nbytes = lib.fl_vocab_backward_bytes(op, need_x, need_w, need_b)
             ws = _workspace(nbytes, dev)
             _launch(ctx.what, lib.fl_vocab_backward, dev, op, grad.data_ptr(), _ptr(state), _ptr(layout), _ptr(dx),
@@ -142,7 +142,7 @@ def _vocab_operands(what, x, weight, bias):
 def _vocab_loss(what, x, weight, bias, lists):
     if _differentiated(x, weight, bias):
         return _VocabFunction.apply(x, weight, bias, lists, what)
-    return _vocab_forward(what, x, weight, bias, lists)[0]
+    return _vocab_forward(what, x, weight, bias, lists, False)[0]
 
 
 def linear_cross_entropy(x, weight, target, bias=None):

@@ -1007,6 +1007,8 @@ typedef struct fl_vocab {
     int64_t ldw;
     const void *bias;         /* contiguous, or null                       */
     int32_t dtype, bias_f32;
+    int32_t train;            /* whether a backward follows the forward    */
+    int32_t reserved;
 } fl_vocab;
 
 size_t fl_vocab_op_bytes(void);
