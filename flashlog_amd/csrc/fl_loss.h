@@ -11,19 +11,23 @@ constexpr float LN2 = 0.69314718055994531f;
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// A running maximum and the sum of 2^(u - maximum).
+// A running maximum m of a row's u and the sum of 2^((u - m) unit): what unit is
+// depends on where u comes from.  Scores are held as they are given: their
+// distance from m is exact at any size (a mask of the type's lowest value in
+// every column leaves a uniform row).
 struct Running {
     float m, s;
 };
 // What exponents are taken from: the maximum, 0 where nothing is above -inf.
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
-__device__ __forceinline__ Running joined(Running a, Running b) {
+__device__ __forceinline__ Running joined(Running a, Running b, float unit = 1.0f) {
     const float m = fmaxf(a.m, b.m), at = base_of(m);
-    return Running{m, a.s * exp2_of(a.m - at) + b.s * exp2_of(b.m - at)};
+    return Running{m, a.s * exp2_of((a.m - at) * unit) + b.s * exp2_of((b.m - at) * unit)};
 }
 
-// The state that a forward leaves for the backward: rows [rows] (lse, whether
-// the row counts), listed [rows][k] (u of the id, the sum of q at it).
+// The state that a forward leaves for the backward: rows [rows] (the maximum, the
+// sum's logarithm; +inf where the row does not count), listed [rows][k] (u of the
+// id, the sum of q at it).
 inline size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 inline size_t state_bytes(const fl_lists *l) { return rounded((size_t)l->rows * 8) + (size_t)l->rows * l->k * 8; }
 inline float2 *state_rows(void *state) { return (float2 *)state; }
@@ -31,13 +35,14 @@ inline float2 *state_listed(const fl_lists *l, void *state) {
     return (float2 *)((char *)state + rounded((size_t)l->rows * 8));
 }
 
-__device__ __forceinline__ Running joined_over_lanes(Running r) {
+__device__ __forceinline__ Running joined_over_lanes(Running r, float unit) {
 #pragma unroll
-    for (int o = FL_WAVE / 2; o > 0; o >>= 1) r = joined(r, Running{__shfl_xor(r.m, o), __shfl_xor(r.s, o)});
+    for (int o = FL_WAVE / 2; o > 0; o >>= 1) r = joined(r, Running{__shfl_xor(r.m, o), __shfl_xor(r.s, o)}, unit);
     return r;
 }
 // Of the parts [count], a wave's share (every `waves`-th 64 of them): the same in all lanes.
-__device__ __forceinline__ Running joined_parts(const Running *part, int64_t count, int wave, int waves) {
+__device__ __forceinline__ Running joined_parts(const Running *part, int64_t count, int wave, int waves,
+                                                float unit) {
     Running r{-INFINITY, 0.0f};
     const int64_t step = (int64_t)waves * FL_WAVE;
     int64_t p = (int64_t)wave * FL_WAVE + fl_lane();
@@ -46,22 +51,23 @@ __device__ __forceinline__ Running joined_parts(const Running *part, int64_t cou
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = part[p + j * step];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r = joined(r, v[j]);
+        for (int j = 0; j < 8; ++j) r = joined(r, v[j], unit);
     }
-    for (; p < count; p += step) r = joined(r, part[p]);
-    return joined_over_lanes(r);
+    for (; p < count; p += step) r = joined(r, part[p], unit);
+    return joined_over_lanes(r, unit);
 }
 
 struct ListArgs {
     fl_lists op;
     float scale, tau2;  // log2(e) / tau, tau^2
+    float unit;         // of u: scale where logits are given, 1 where u is in units of log 2
     int64_t cols;
     const Running *part;  // [rows][parts]
     int64_t parts;
     const void *logits;   // scores; null: `listed` holds u
     int64_t ld;
     float *loss;
-    float2 *rows, *listed;  // (lse, whether the row counts), (u, sum of q at the id)
+    float2 *rows, *listed;  // the state
 };
 
 inline ListArgs list_args(const fl_lists *l, int64_t cols, void *state, float *loss) {
@@ -69,6 +75,7 @@ inline ListArgs list_args(const fl_lists *l, int64_t cols, void *state, float *l
     a.op = *l;
     a.scale = LOG2E / l->temperature;
     a.tau2 = l->temperature * l->temperature;
+    a.unit = 1.0f;
     a.cols = cols;
     a.loss = loss;
     a.rows = state_rows(state);
@@ -81,10 +88,10 @@ inline ListArgs list_args(const fl_lists *l, int64_t cols, void *state, float *l
 template <typename U>
 __device__ __forceinline__ void list_row(const ListArgs &a, int64_t row, Running r, float2 *mine, U &&u_of) {
     const int64_t k = a.op.k;
-    const float lse = r.m + log2f(r.s);
+    const float log_sum = log2f(r.s);
     const int64_t *ids = a.op.ids + row * k;
     float2 *listed = a.listed + row * k;
-    // (id, teacher in units of log 2), -inf where it does not count
+    // (id, teacher), -inf where it does not count
     float top = -INFINITY;
     bool any = false;
     for (int64_t j = fl_lane(); j < k; j += FL_WAVE) {
@@ -92,7 +99,7 @@ __device__ __forceinline__ void list_row(const ListArgs &a, int64_t row, Running
         const bool in = id >= 0 && id < a.cols;
         const float u = in ? u_of(j, id) : 0.0f;
         float v = -INFINITY;
-        if (in && a.op.teacher && u != -INFINITY) v = a.op.teacher[row * k + j] * a.scale;
+        if (in && a.op.teacher && u != -INFINITY) v = a.op.teacher[row * k + j];
         if (in && !a.op.teacher) v = 0.0f;
         mine[j] = float2{__int_as_float(in ? (int)id : -1), v};
         listed[j] = float2{u, 0.0f};
@@ -103,19 +110,19 @@ __device__ __forceinline__ void list_row(const ListArgs &a, int64_t row, Running
     for (int o = FL_WAVE / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     const bool live = __any(any) && r.s != 0.0f;  // no sum: every u is -inf
     float total = 0.0f;
-    for (int64_t j = fl_lane(); j < k; j += FL_WAVE) total += exp2_of(mine[j].y - top);
+    for (int64_t j = fl_lane(); j < k; j += FL_WAVE) total += exp2_of((mine[j].y - top) * a.scale);
     total = fl_wave_sum_f32(total);
     const float of_total = 1.0f / total, log_total = log2f(total);
     float loss = 0.0f;
     for (int64_t j = fl_lane(); j < k; j += FL_WAVE) {
-        const float v = mine[j].y, q = live ? exp2_of(v - top) * of_total : 0.0f;
-        if (q != 0.0f) loss += q * ((v - top - log_total) - (listed[j].x - lse));
+        const float v = (mine[j].y - top) * a.scale, q = live ? exp2_of(v) * of_total : 0.0f;
+        if (q != 0.0f) loss += q * ((v - log_total) - ((listed[j].x - r.m) * a.unit - log_sum));
         mine[j].y = q;
     }
     loss = fl_wave_sum_f32(loss) * (a.tau2 * LN2);
     if (fl_lane() == 0) {
         a.loss[row] = live ? loss : 0.0f;
-        a.rows[row] = float2{lse, live ? 1.0f : 0.0f};
+        a.rows[row] = float2{r.m, live ? log_sum : INFINITY};
     }
     fl_wave_sync();
     for (int64_t j = fl_lane(); j < k; j += FL_WAVE) {

@@ -13,8 +13,8 @@
 //
 // HBM-bound: one read forward, one read and one write backward.  A wave takes a
 // segment of a row in registers, a second launch joins the segments' maxima and
-// sums and looks at the lists.  u is held in units of log 2: exponentials are the
-// hardware's 2^x, off by 2^-24 |u| of themselves besides its own step.
+// sums and looks at the lists.  Exponentials are the hardware's 2^x of distances
+// from the row's maximum, off by 2^-23 of their exponent besides its own step.
 #include "fl_abi.h"
 #include "fl_common.h"
 #include "fl_loss.h"
@@ -101,12 +101,11 @@ __global__ __launch_bounds__(LS_NT) void k_score_stats(ScoreArgs a) {
         for (int e = 0; e < G; ++e) r.m = fmaxf(r.m, (float)s.v[i].v[e]);
 #pragma unroll
     for (int o = FL_WAVE / 2; o > 0; o >>= 1) r.m = fmaxf(r.m, __shfl_xor(r.m, o));
-    r.m *= a.scale;
     const float at = base_of(r.m);
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int e = 0; e < G; ++e) r.s += exp2_of((float)s.v[i].v[e] * a.scale - at);
+        for (int e = 0; e < G; ++e) r.s += exp2_of(((float)s.v[i].v[e] - at) * a.scale);
     r.s = fl_wave_sum_f32(r.s);
     if (fl_lane() == 0) a.part[row * a.segments + seg] = r;
 }
@@ -118,7 +117,7 @@ __global__ __launch_bounds__(LS_NT) void k_score_grad(ScoreArgs a) {
     if (item >= a.op.rows * a.segments) return;
     const int64_t row = item / a.segments, c0 = (item % a.segments) * LS_SEG;
     const float2 of = a.rows[row];
-    const float c = of.y != 0.0f ? a.op.temperature * a.grad[row] : 0.0f;
+    const float c = of.y != INFINITY ? a.op.temperature * a.grad[row] : 0.0f;
     T *out = (T *)a.dx + row * a.cols;
     Segment<T> s;
     s.load((const T *)a.logits + row * a.ld, c0, a.cols);
@@ -126,7 +125,7 @@ __global__ __launch_bounds__(LS_NT) void k_score_grad(ScoreArgs a) {
     for (int i = 0; i < N; ++i) {
 #pragma unroll
         for (int e = 0; e < G; ++e)
-            s.v[i].v[e] = (T)(c == 0.0f ? 0.0f : c * exp2_of((float)s.v[i].v[e] * a.scale - of.x));
+            s.v[i].v[e] = (T)(c == 0.0f ? 0.0f : c * exp2_of(__builtin_fmaf((float)s.v[i].v[e] - of.x, a.scale, -of.y)));
         const int64_t at = c0 + (i * FL_WAVE + fl_lane()) * G;
         if (at + G <= a.cols) store_cols<T, G>(out + at, s.v[i]);
         else store_first<T, G>(out + at, s.v[i], (int)(a.cols - at));
@@ -146,7 +145,7 @@ __global__ __launch_bounds__(LS_NT) void k_score_grad(ScoreArgs a) {
         waited = true;
         if (here) {
             const float2 l = a.listed[row * a.op.k + j];
-            out[id] = (T)(c * (exp2_of(l.x - of.x) - l.y));
+            out[id] = (T)(c * (exp2_of(__builtin_fmaf(l.x - of.x, a.scale, -of.y)) - l.y));
         }
     }
 }
@@ -160,15 +159,15 @@ __global__ __launch_bounds__(LS_NT) void k_list_rows(ListArgs a) {
     __shared__ Running quarters[LS_WAVES];
     const int64_t waves = blockDim.x / FL_WAVE, row = WPR == 1 ? fl_block() * waves + fl_wave_id() : fl_block();
     if (row >= a.op.rows) return;
-    Running r = joined_parts(a.part + row * a.parts, a.parts, WPR == 1 ? 0 : fl_wave_id(), WPR);
+    Running r = joined_parts(a.part + row * a.parts, a.parts, WPR == 1 ? 0 : fl_wave_id(), WPR, a.unit);
     if constexpr (WPR > 1) {
         if (fl_lane() == 0) quarters[fl_wave_id()] = r;
         __syncthreads();
         if (fl_wave_id()) return;
-        r = joined(joined(quarters[0], quarters[1]), joined(quarters[2], quarters[3]));
+        r = joined(joined(quarters[0], quarters[1], a.unit), joined(quarters[2], quarters[3], a.unit), a.unit);
     }
     list_row(a, row, r, list_lds + (WPR == 1 ? fl_wave_id() * a.op.k : 0), [&](int64_t j, int64_t id) {
-        return a.logits ? (float)((const T *)a.logits)[row * a.ld + id] * a.scale : a.listed[row * a.op.k + j].x;
+        return a.logits ? (float)((const T *)a.logits)[row * a.ld + id] : a.listed[row * a.op.k + j].x;
     });
 }
 
@@ -207,6 +206,7 @@ int score_forward(hipStream_t st, const fl_scores *op, float *loss, void *state,
     ListArgs a = list_args(&op->lists, op->cols, state, loss);
     a.part = s.part;
     a.parts = s.segments;
+    a.unit = a.scale;
     a.logits = op->logits;
     a.ld = op->ld;
     return join_rows<T>(st, a, "distillation");
@@ -248,8 +248,8 @@ int check_lists(const fl_lists *l, const char *what) {
         return fl_fail(FL_ERR_ARG, "%s: lists of more than %d ids (shape)", what, (int)LS_MOST_LISTED);
     if (l->rows && !l->teacher && l->k > 1) return fl_fail(FL_ERR_ARG, "%s: targets without a teacher are one a row (shape)", what);
     if (l->rows && l->k && !l->ids) return fl_fail(FL_ERR_ARG, "%s: null pointer", what);
-    if (!(l->temperature >= 0x1p-100f && l->temperature <= 0x1p100f))
-        return fl_fail(FL_ERR_ARG, "%s: temperature must be positive and finite", what);
+    if (!(l->temperature >= 0x1p-60f && l->temperature <= 0x1p60f))
+        return fl_fail(FL_ERR_ARG, "%s: temperature must be within 2^-60 and 2^60", what);
     return FL_OK;
 }
 

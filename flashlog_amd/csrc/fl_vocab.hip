@@ -128,7 +128,7 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_rows(VocabArgs a, ListArgs l) {
     __shared__ float2 lists[LS_WAVES][DOT_IDS];
     const int64_t row = fl_block() * LS_WAVES + fl_wave_id();
     if (row >= a.op.M) return;
-    const Running r = joined_parts(a.part + row * a.parts, a.parts, 0, 1);
+    const Running r = joined_parts(a.part + row * a.parts, a.parts, 0, 1, 1.0f);
     int64_t id[DOT_IDS];
     float s[DOT_IDS];
     ids_of(a, row, 0, id);
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(1024) void k_vocab_coef(const float2 *__restrict__ 
     if constexpr (SCALED) {
         float m = 0.0f;
         for (int64_t i = threadIdx.x; i < M; i += 1024) {
-            const float c = rows[i].y != 0.0f ? fabsf(tau * g[i]) : 0.0f;
+            const float c = rows[i].y != INFINITY ? fabsf(tau * g[i]) : 0.0f;
             m = fmaxf(m, c < INFINITY ? c : 0.0f);
         }
 #pragma unroll
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(1024) void k_vocab_coef(const float2 *__restrict__ 
     } else if (fl_block() == 0 && threadIdx.x == 0) *unscale = 1.0f;
     const int64_t step = SCALED ? 1024 : (int64_t)gridDim.x * 1024;
     for (int64_t i = (SCALED ? 0 : (int64_t)blockIdx.x * 1024) + threadIdx.x; i < M; i += step)
-        coef[i] = rows[i].y != 0.0f ? tau * g[i] * scale : 0.0f;
+        coef[i] = rows[i].y != INFINITY ? tau * g[i] * scale : 0.0f;
 }
 
 // dz of a piece but for the listed columns.
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_grad(VocabArgs a) {
 #pragma unroll
     for (int i = 0; i < Prod::MT; ++i) {
         const int64_t m = row + i * 16 < a.op.M ? row + i * 16 : a.op.M - 1;
-        lse[i] = a.rows[m].x;
+        lse[i] = a.rows[m].x + a.rows[m].y;
         c[i] = a.coef[m];
     }
     each_u<T>(a, prod.acc, col, a.v0 + a.width, [&](int i, int j, const float (&u)[4]) {
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
     const float c = a.coef[row];
     if (v < 0 || v >= a.width || c == 0.0f) return;
     const float2 l = a.listed[i];
-    const float d = c * (exp2_of(l.x - a.rows[row].x) - l.y);
+    const float d = c * (exp2_of((l.x - a.rows[row].x) - a.rows[row].y) - l.y);
     if constexpr (WIDE && sizeof(T) == 4) {
         _Float16 *to = (_Float16 *)a.d + dz_at<true>(a, row, v);
         to[0] = (_Float16)d;
@@ -455,21 +455,15 @@ constexpr bool is_pairs() {
 }
 
 // The largest finite magnitude of x and of weight, a part of them a workgroup.
+// Rows of x in which nothing is listed do not count and are laid out as zeros
+// (padded rows may hold anything), a wave a row; live: those that count.
 constexpr int LAY_PARTS = 1024;
 
 template <typename T>
-__global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restrict__ most) {
+__global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restrict__ most,
+                                                   uint8_t *__restrict__ live) {
     constexpr int G = 16 / (int)sizeof(T);
     __shared__ float waves[LS_WAVES];
-    const bool second = blockIdx.y;
-    // rows without gaps are one
-    int64_t R = second ? a.op.V : a.op.M, K = a.op.K;
-    const int64_t ld = second ? a.op.ldw : a.op.ldx;
-    if (ld == K) {
-        K *= R;
-        R = 1;
-    }
-    const T *p = (const T *)(second ? a.op.weight : a.op.x);
     float m = 0.0f;
     const auto see = [&](const Vec<T, G> &v) {
 #pragma unroll
@@ -478,12 +472,7 @@ __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restric
             m = fmaxf(m, t < INFINITY ? t : 0.0f);
         }
     };
-    // a row to a workgroup, or one to all of them
-    const int64_t step = (R == 1 ? LAY_PARTS : 1) * (int64_t)LS_NT * G;
-    const int64_t c0 = ((R == 1 ? (int64_t)blockIdx.x : 0) * LS_NT + threadIdx.x) * G;
-    for (int64_t r = R == 1 ? 0 : blockIdx.x; r < R; r += LAY_PARTS) {
-        const T *row = p + r * ld;
-        int64_t c = c0;
+    const auto see_row = [&](const T *row, int64_t c, int64_t step, int64_t K) {
         for (; c + 7 * step + G <= K; c += 8 * step) {
             Vec<T, G> v[8];
 #pragma unroll
@@ -499,6 +488,26 @@ __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restric
                 for (int e = 0; e < G; ++e) v.v[e] = c + e < K ? row[c + e] : (T)0.0f;
             see(v);
         }
+    };
+    if (blockIdx.y == 0) {
+        const int64_t k = a.op.lists.k;
+        for (int64_t r = (int64_t)blockIdx.x * LS_WAVES + fl_wave_id(); r < a.op.M; r += LAY_PARTS * LS_WAVES) {
+            bool any = false;
+            for (int64_t j = fl_lane(); j < k; j += FL_WAVE) {
+                const int64_t id = a.op.lists.ids[r * k + j];
+                any = any || (id >= 0 && id < a.op.V);
+            }
+            any = __any(any);
+            if (fl_lane() == 0) live[r] = any;
+            if (any) see_row((const T *)a.op.x + r * a.op.ldx, fl_lane() * G, FL_WAVE * G, a.op.K);
+        }
+    } else {
+        // rows without gaps are one, of all workgroups
+        const bool one = a.op.ldw == a.op.K;
+        const int64_t R = one ? 1 : a.op.V, K = one ? a.op.V * a.op.K : a.op.K;
+        const int64_t c0 = ((one ? (int64_t)blockIdx.x : 0) * LS_NT + threadIdx.x) * G;
+        for (int64_t r = one ? 0 : blockIdx.x; r < R; r += LAY_PARTS)
+            see_row((const T *)a.op.weight + r * a.op.ldw, c0, (one ? LAY_PARTS : 1) * (int64_t)LS_NT * G, K);
     }
 #pragma unroll
     for (int o = FL_WAVE / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -514,7 +523,8 @@ __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restric
 // bfloat16 that no backward follows, as they are; zeros behind a row.  (dz, in half, is then rounded by 2^-12 of itself; by 2^-9 in
 // bfloat16 it made the gradients' error 1.4 to 1.5 times that of their own rounding.)
 template <typename T, bool SCALED>
-__global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restrict__ most, uint16_t *__restrict__ x,
+__global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restrict__ most,
+                                               const uint8_t *__restrict__ live, uint16_t *__restrict__ x,
                                                uint16_t *__restrict__ w, float *__restrict__ undo) {
     constexpr bool PAIRS = is_pairs<T>();
     const bool second = blockIdx.y;
@@ -539,11 +549,12 @@ __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restr
     }
     for (int64_t i = (int64_t)blockIdx.x * LS_NT + threadIdx.x; i < R * chunks; i += (int64_t)gridDim.x * LS_NT) {
         const int64_t r = i / chunks, c = i % chunks * 8;
+        const int64_t have = SCALED && !second && !live[r] ? 0 : K;
         Vec<T, 8> v;
-        if (c + 8 <= K) v = load_vec<T, 8>(p + r * ld + c);
+        if (c + 8 <= have) v = load_vec<T, 8>(p + r * ld + c);
         else
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v.v[e] = c + e < K ? p[r * ld + c + e] : (T)0.0f;
+            for (int e = 0; e < 8; ++e) v.v[e] = c + e < have ? p[r * ld + c + e] : (T)0.0f;
         if constexpr (PAIRS) {
             Vec<_Float16, 8> hi, lo;
 #pragma unroll
@@ -622,6 +633,11 @@ __device__ __forceinline__ int64_t part_begin(int64_t all, uint32_t part, uint32
     return fl_uniform_i64(all * part / parts);
 }
 
+// What a product is multiplied by, in units of log 2 (finite: a product of 0 stays 0).
+__device__ __forceinline__ float product_scale(const VocabArgs &a) {
+    return a.undo ? fminf(a.undo[0] * a.undo[1] * a.scale, 0x1.fffffep127f) : a.scale;
+}
+
 // A lane's bias for its 16 columns from n on, in units of log 2.
 template <typename T>
 __device__ __forceinline__ void lane_bias(const VocabArgs &a, int64_t n, float (&b)[16]) {
@@ -653,7 +669,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
     for (int i = 0; i < MT; ++i) sums[i * FL_WAVE + fl_lane()] = Running{-INFINITY, 0.0f};
     Tiles tiles;
     tiles.init(a, row0, t0 * WN * 64);
-    const float scale = a.undo ? a.undo[0] * a.undo[1] * a.scale : a.scale;
+    const float scale = product_scale(a);
     Run run;
     run.template run<false>(
         tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](int i, uint16_t *la, uint16_t *lb) { tiles.feed(a, i, la, lb); },
@@ -686,7 +702,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
                     }
                 }
                 s += r.s;
-                if (__any(r.m == -INFINITY || !(s < INFINITY))) {
+                if (r.m == -INFINITY || !(s < INFINITY)) {  // a lane's own: rows do not touch each other's bits
                     float m = r.m;
                     s = 0.0f;
 #pragma unroll
@@ -723,20 +739,21 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
     float4 *of = reinterpret_cast<float4 *>(wide_lds + STAGES * Run::ELEMS);
     for (int t = threadIdx.x; t < BM; t += WD_NT) {
         const int64_t m = row0 + t < a.op.M ? row0 + t : a.op.M - 1;
-        const float lse = a.rows[m].x, c = row0 + t < a.op.M ? a.coef[m] : 0.0f;
+        const float2 sum = a.rows[m];
+        const float c = row0 + t < a.op.M ? a.coef[m] : 0.0f;
         float id = __int_as_float(-1), d = 0.0f;
         if (a.op.lists.k == 1 && c != 0.0f) {
             const int64_t v = a.op.lists.ids[m];
             const float2 l = a.listed[m];
             if (v >= a.v0 && v < end) id = __int_as_float((int)(v - a.v0));
-            d = c * (exp2_of(l.x - lse) - l.y);
+            d = c * (exp2_of((l.x - sum.x) - sum.y) - l.y);
         }
-        of[t] = float4{lse, c, id, d};
+        of[t] = float4{sum.x + sum.y, c, id, d};
     }
     __syncthreads();
     Tiles tiles;
     tiles.init(a, row0, a.v0 + t0 * WN * 64);
-    const float scale = a.undo ? a.undo[0] * a.undo[1] * a.scale : a.scale;
+    const float scale = product_scale(a);
     Run run;
     run.template run<false>(
         tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](int i, uint16_t *la, uint16_t *lb) { tiles.feed(a, i, la, lb); },
@@ -1049,9 +1066,9 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     return p;
 }
 
-// The laid out operands: x, weight, what undoes their powers of two, parts of their maxima.
+// The laid out operands: x, weight, what undoes their powers of two, parts of their maxima, x's rows that count.
 struct VocabLayout {
-    size_t x, w, undo, most, bytes;
+    size_t x, w, undo, most, live, bytes;
 };
 
 VocabLayout vocab_layout(const fl_vocab *op, const VocabPlan &p) {
@@ -1060,7 +1077,8 @@ VocabLayout vocab_layout(const fl_vocab *op, const VocabPlan &p) {
     l.w = rounded((size_t)op->M * p.cols * p.size);
     l.undo = l.w + rounded((size_t)op->V * p.cols * p.size);
     l.most = l.undo + 256;
-    l.bytes = l.most + 2 * LAY_PARTS * 4;
+    l.live = l.most + 2 * LAY_PARTS * 4;
+    l.bytes = l.live + rounded((size_t)op->M);
     return l;
 }
 
@@ -1166,18 +1184,19 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
     if (p.lay) {
         const VocabLayout l = vocab_layout(op, p);
         float *most = (float *)((char *)layout + l.most);
+        uint8_t *live = (uint8_t *)layout + l.live;
         const int64_t chunks = (op->M > op->V ? op->M : op->V) * (p.cols / 8), want = ceil_div(chunks, LS_NT);
         const dim3 lg((unsigned)(want < 4096 ? want : 4096), 2);
         if constexpr (!std::is_same<T, _Float16>::value)
             if (p.scaled) {
-                FL_LAUNCH("k_lay_max", k_lay_max<T>, dim3(LAY_PARTS, 2), dim3(LS_NT), 0, st, a, most);
-                FL_LAUNCH("k_lay", (k_lay<T, true>), lg, dim3(LS_NT), 0, st, a, most, (uint16_t *)a.x, (uint16_t *)a.w,
-                          (float *)a.undo);
+                FL_LAUNCH("k_lay_max", k_lay_max<T>, dim3(LAY_PARTS, 2), dim3(LS_NT), 0, st, a, most, live);
+                FL_LAUNCH("k_lay", (k_lay<T, true>), lg, dim3(LS_NT), 0, st, a, most, live, (uint16_t *)a.x,
+                          (uint16_t *)a.w, (float *)a.undo);
             }
         if constexpr (sizeof(T) == 2)
             if (!p.scaled)
-                FL_LAUNCH("k_lay", (k_lay<T, false>), lg, dim3(LS_NT), 0, st, a, most, (uint16_t *)a.x, (uint16_t *)a.w,
-                          (float *)nullptr);
+                FL_LAUNCH("k_lay", (k_lay<T, false>), lg, dim3(LS_NT), 0, st, a, most, live, (uint16_t *)a.x,
+                          (uint16_t *)a.w, (float *)nullptr);
     }
     const bool few = op->lists.k <= DOT_IDS && p.parts <= 4 * FL_WAVE;
     if (!few)
@@ -1387,6 +1406,7 @@ int fl_vocab_backward(void *stream, const fl_vocab *op, const float *grad, void 
     const int rc = fl::check_vocab(op, "linear_loss");
     if (rc) return rc;
     if (op->M == 0) return FL_OK;
+    if (!op->train) return fl::fl_fail(FL_ERR_ARG, "linear_loss: a forward without `train` has no backward");
     if (!grad || !state || (!layout && fl_vocab_layout_bytes(op))) return fl::fl_fail(FL_ERR_ARG, "linear_loss: null pointer");
     const size_t need = fl_vocab_backward_bytes(op, dx != nullptr, dw != nullptr, db != nullptr);
     if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "linear_loss: workspace too small");

@@ -58,8 +58,8 @@ def _lists(what, lead, ids, teacher, temperature):
     if teacher.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s: the teacher has no gradient; detach it" % what)
     temperature = float(temperature)
-    if not 2.0 ** -100 <= temperature <= 2.0 ** 100:
-        raise ValueError("%s: temperature must be finite and positive" % what)
+    if not 2.0 ** -60 <= temperature <= 2.0 ** 60:
+        raise ValueError("%s: temperature must be within 2^-60 and 2^60" % what)
     out = _Lists()
     out.ids, out.teacher, out.temperature = _integers(what, "ids", ids), teacher.float().contiguous(), temperature
     out.rows, out.k = math.prod(lead), ids.shape[-1]
@@ -114,6 +114,9 @@ class _VocabFunction(autograd.Function):
         db = make(weight.shape[0], dtype=bias.dtype) if need_b else None
         if x.shape[0]:
             op = _vocab_op(x, weight, bias, ctx.lists, True)
+            if lib.fl_vocab_layout_bytes(op) != (0 if layout is None else layout.numel()):
+                # a hook on saved tensors has them on other strides than the forward had
+                state, layout = _vocab_forward(ctx.what, x, weight, bias, ctx.lists, True)[4:]
             nbytes = lib.fl_vocab_backward_bytes(op, need_x, need_w, need_b)
             ws = _workspace(nbytes, dev)
             _launch(ctx.what, lib.fl_vocab_backward, dev, op, grad.data_ptr(), _ptr(state), _ptr(layout), _ptr(dx),

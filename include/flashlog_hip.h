@@ -973,7 +973,7 @@ typedef struct fl_lists {
     int64_t rows, k;
     const int64_t *ids;       /* [rows, k]                                 */
     const float *teacher;     /* [rows, k] or null                         */
-    float temperature;        /* in [2^-100, 2^100]                        */
+    float temperature;        /* in [2^-60, 2^60]                          */
     int32_t reserved;
 } fl_lists;
 
@@ -1007,14 +1007,15 @@ typedef struct fl_vocab {
     int64_t ldw;
     const void *bias;         /* contiguous, or null                       */
     int32_t dtype, bias_f32;
-    int32_t train;            /* whether a backward follows the forward    */
+    int32_t train;            /* whether a backward follows; set in it too */
     int32_t reserved;
 } fl_vocab;
 
 size_t fl_vocab_op_bytes(void);
-/* Bytes of the operands as the products take them where they are laid out anew
- * (fp32, rows not on 16 bytes; else 0): a forward writes them, its backward
- * reads them. */
+/* Bytes of the operands as the products take them where large products lay
+ * them out anew (fp32 as two fp16 planes, bf16 in training as scaled fp16, rows
+ * that do not lie on 16 bytes; else 0): a forward writes them, its backward, of
+ * the same operands on the same strides, reads them. */
 size_t fl_vocab_layout_bytes(const fl_vocab *op);
 size_t fl_vocab_forward_bytes(const fl_vocab *op);
 int fl_vocab_forward(void *stream, const fl_vocab *op, float *loss,

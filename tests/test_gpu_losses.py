@@ -10,8 +10,10 @@ columns, weighed by p, and by (80 + 2 |lse|) e for its sums, exponentials (off
 by 2 e times 1 + the distance from the maximum) and logarithm.  p is off by
 those errors and 8 e (1 + |u - lse|) relative to itself, a teacher's share q by
 16 e (1 + the range of its list).  dz = c (p - Q) is rounded to the operands'
-type (u, and for half, held at the scale of the largest |c|, 2^-38 of that) and
-enters sums of n terms with (n + 16) e."""
+type (u, and where it is held in half, at the scale of the largest |c|, 2^-38 of
+that) and enters sums of n terms with (n + 16) e.  Operands that are held in half
+at the scale of their largest (float32 as two planes, bfloat16 in training) lose
+up to 2^-38 of that."""
 import math
 
 import pytest
@@ -89,12 +91,16 @@ def vocab_reference(x, w, b, ids, teacher, tau, g):
     z, mag = x @ w.T, x.abs() @ w.abs().T
     if b is not None:
         z, mag = z + b.double(), mag + torch.nan_to_num(b.double().abs(), posinf=0)
-    loss, dloss, d, dd, c = _rows(z, (K + 16) * E * mag, ids, teacher, tau, g, t)
-    dd = dd + u * d.abs() + (c.abs().max() * 2.0 ** -38 if t is torch.float16 else _tiny(t))
+    live = ((ids >= 0) & (ids < V)).any(1, keepdim=True)
+    xm, wm = (x.abs() * live).max() if x.numel() else 0.0, w.abs().max() if w.numel() else 0.0
+    lost = 2.0 ** -38 * (xm * w.abs().sum(1)[None, :] + wm * x.abs().sum(1, keepdim=True))
+    loss, dloss, d, dd, c = _rows(z, (K + 16) * E * mag + lost, ids, teacher, tau, g, t)
+    dd = dd + u * d.abs() + c.abs().max() * 2.0 ** -38 + _tiny(t)
     dd = torch.where(c == 0, 0.0, dd)
     out = {"loss": (loss, dloss * 1.01 + 1e-30)}
     for name, a, v, n in (("dx", d, w, V), ("dw", d.T, x, M)):
-        out[name] = (a @ v, (dd if name == "dx" else dd.T) @ v.abs() + (n + 16) * E * (a.abs() @ v.abs()))
+        out[name] = (a @ v, (dd if name == "dx" else dd.T) @ v.abs() + (n + 16) * E * (a.abs() @ v.abs())
+                     + 2.0 ** -38 * (wm if name == "dx" else xm) * a.abs().sum(1, keepdim=True))
     if b is not None:
         out["db"] = (d.sum(0), dd.sum(0) + (M + 16) * E * d.abs().sum(0))
     for k in list(out)[1:]:
@@ -114,14 +120,17 @@ def _make(M, K, V, t, seed, k=None, bias=True, spread=2.0):
     return x, w, b, ids, teacher, grad
 
 
+def _loss_of(x, w, b, ids, teacher, tau):
+    if teacher is None:
+        return _losses().linear_cross_entropy(x, w, ids[..., 0], b)
+    return _losses().linear_distillation(x, w, ids, teacher.cuda(), b, temperature=tau)
+
+
 def _run(x, w, b, ids, teacher, tau, g):
     dev = [v.cuda() for v in (x, w)] + ([b.cuda()] if b is not None else [])
     leaves = [v.detach().requires_grad_(True) for v in dev]
     bias = leaves[2] if b is not None else None
-    if teacher is None:
-        loss = _losses().linear_cross_entropy(leaves[0], leaves[1], ids[..., 0].cuda(), bias)
-    else:
-        loss = _losses().linear_distillation(leaves[0], leaves[1], ids.cuda(), teacher.cuda(), bias, temperature=tau)
+    loss = _loss_of(leaves[0], leaves[1], bias, ids.cuda(), teacher, tau)
     grads = torch.autograd.grad(loss, leaves, g.cuda().reshape(loss.shape))
     return {"loss": loss.detach(), **dict(zip(("dx", "dw", "db"), grads))}
 
@@ -132,6 +141,9 @@ def _check(x, w, b, ids, teacher, tau, g):
     assert out["loss"].dtype is torch.float32 and set(out) == set(ref)
     for k, (value, bound) in ref.items():
         _held(out[k], value, bound, k)
+    with torch.no_grad():  # other kernels: no backward follows
+        ev = _loss_of(x.cuda(), w.cuda(), None if b is None else b.cuda(), ids.cuda(), teacher, tau)
+    _held(ev, *ref["loss"], "loss without gradients")
     return out
 
 
@@ -156,7 +168,8 @@ def test_linear_distillation(M, K, V, k, tau, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("M,K,V", [(300, 256, 1000), (257, 512, 2049), (1000, 64, 4096), (520, 200, 3333)])
+@pytest.mark.parametrize("M,K,V", [(300, 256, 1000), (257, 512, 2049), (1000, 64, 4096), (520, 200, 3333),
+                                   (2, 1024, 70000), (70, 512, 4096), (150, 200, 4500), (400, 100, 3400), (460, 64, 4600)])
 def test_many_tiles(M, K, V, t):
     """Sizes of several tiles in every direction, odd ends among them."""
     x, w, b, ids, _, g = (v.cuda() if v is not None else None for v in _make(M, K, V, t, M + K + V))
@@ -202,9 +215,10 @@ def test_fp32_bias(t):
 
 
 @pytest.mark.parametrize("t", TYPES)
-def test_columns_that_the_bias_takes_out(t):
-    x, w, b, ids, teacher, g = _make(40, 24, 150, t, 12, k=6)
-    b[torch.randperm(150, generator=torch.Generator().manual_seed(1))[:100]] = -math.inf
+@pytest.mark.parametrize("M,K,V", [(40, 24, 150), (300, 128, 4000)])
+def test_columns_that_the_bias_takes_out(M, K, V, t):
+    x, w, b, ids, teacher, g = _make(M, K, V, t, 12, k=6)
+    b[torch.randperm(V, generator=torch.Generator().manual_seed(1))[:2 * V // 3]] = -math.inf
     ids[3] = 0
     b[0] = -math.inf
     out = _check(x, w, b, ids, teacher, 1.0, g)  # listed ids that are out do not count
@@ -219,26 +233,70 @@ def test_columns_that_the_bias_takes_out(t):
     assert all((v == 0).all() for v in out.values())
 
 
-def test_rows_without_a_target():
-    x, w, b, ids, _, g = _make(50, 40, 90, torch.float32, 13)
-    ids[:, 0] = torch.tensor([-1, 90, 5, -100, 1 << 40])[torch.arange(50) % 5]
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,K,V", [(50, 40, 90), (300, 128, 4000)])
+def test_rows_without_a_target(M, K, V, t):
+    x, w, b, ids, _, g = _make(M, K, V, t, 13)
+    ids[:, 0] = torch.tensor([-1, V, 5, -100, 1 << 40])[torch.arange(M) % 5]
     out = _check(x, w, b, ids, None, 1.0, g)
-    off = torch.arange(50) % 5 != 2
+    off = torch.arange(M) % 5 != 2
+    # whatever such rows hold, as padded ones may, nothing else changes
+    pad = torch.where(off[:, None], torch.finfo(t).max / 2, x)
+    for k, v in _run(pad, w, b, ids, None, 1.0, g).items():
+        assert torch.equal(v, out[k]), k
     assert (out["loss"].cpu()[off] == 0).all() and (out["dx"].cpu()[off] == 0).all()
     ids.fill_(-1)
     assert all((v == 0).all() for v in _run(x, w, b, ids, None, 1.0, g).values())
 
 
-def test_not_finite_rows_stay_apart():
-    x, w, b, ids, _, g = _make(9, 40, 90, torch.float32, 14)
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,K,V", [(9, 40, 90), (300, 128, 4000)])
+def test_not_finite_rows_stay_apart(M, K, V, t):
+    x, w, b, ids, _, g = _make(M, K, V, t, 14)
     ids.clamp_(min=0)
     bad = x.clone()
     bad[2, 3] = float("nan")
     good, out = _run(x, w, b, ids, None, 1.0, g), _run(bad, w, b, ids, None, 1.0, g)
-    rows = [r for r in range(9) if r != 2]
+    rows = [r for r in range(M) if r != 2]
     assert out["loss"][2].isnan() and out["dx"][2].isnan().all()
     for k in ("loss", "dx"):
         assert torch.equal(out[k][rows], good[k][rows])
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_operands_of_many_magnitudes(t):
+    """Rows of x and of the weight over factors of 2^10, and operands of zeros."""
+    x, w, b, ids, _, g = _make(300, 128, 4000, t, 17)
+    x = x * 2.0 ** -(torch.arange(300) % 11)[:, None]
+    w = w * 2.0 ** -(torch.arange(4000) % 11)[:, None]
+    _check(x.to(t), w.to(t), b, ids, None, 1.0, g)
+    for a, c in ((x * 0, w), (x, w * 0), (x * 0, w * 0)):
+        _check(a.to(t), c.to(t), b, ids, None, 1.0, g)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_saved_tensors_on_other_strides(t):
+    """A hook may give the backward its operands on strides that the forward did not have."""
+    M, K, V = 300, 128, 4000
+    x, w, b, ids, _, g = _make(M, K, V, t, 18)
+    ref = vocab_reference(x, w, b, ids, None, 1.0, g)
+
+    def shifted(v):  # the same values on rows that begin 2 or 4 bytes behind 16
+        if v.dim() != 2 or v.dtype is not t:
+            return v
+        base = v.new_zeros(v.shape[0], v.shape[1] + 9)
+        base[:, 1:1 + v.shape[1]] = v
+        return base[:, 1:1 + v.shape[1]]
+
+    def straight(v):
+        return v.clone(memory_format=torch.contiguous_format) if v.dtype is t else v
+
+    for first, then in ((straight, shifted), (shifted, straight)):
+        leaves = [v.cuda().requires_grad_(True) for v in (x, w, b)]
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: v, then):
+            loss = _losses().linear_cross_entropy(first(leaves[0]), first(leaves[1]), ids[:, 0].cuda(), leaves[2])
+        for k, v in zip(("dx", "dw", "db"), torch.autograd.grad(loss, leaves, g.cuda())):
+            _held(v, *ref[k], k)
 
 
 def test_no_rows():
@@ -346,6 +404,25 @@ def test_masked_empty_and_padded_rows():
     assert (out["dx"].cpu()[torch.isneginf(z)] == 0).all()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tau", [1.0, 0.5])
+def test_masks_of_the_lowest_value(tau, t):
+    """Masks that are finite: a row of nothing else is uniform, as its distances from the largest are 0."""
+    z, ids, teacher, g = _make_scores(7, 4500, 9, t, 25)
+    low, far = torch.finfo(t).min, -math.inf
+    ids[1], ids[2] = 2 * torch.arange(9) + 1, 7
+    z[0], z[1, ::2], z[2] = low, low, low
+    z[2, 7] = 1.0
+    same, list_ = z.clone(), teacher.clone()
+    same[0], same[1, ::2], same[2] = 0.0, far, far  # in 64 bits: what differs by a constant or is as good as 0
+    same[2, 7] = 1.0
+    teacher[3], teacher[4, :4] = torch.finfo(torch.float32).min, torch.finfo(torch.float32).min
+    list_[3], list_[4, :4] = 0.0, far
+    ref, out = scores_reference(same, ids, list_, tau, g), _run_scores(z, ids, teacher, tau, g)
+    for name, (value, bound) in ref.items():
+        _held(out[name], value, bound, name)
+
+
 def test_not_finite_scores():
     z, ids, teacher, g = _make_scores(9, 2500, 6, torch.float32, 23)
     ids.clamp_(0, 2499)
@@ -426,8 +503,10 @@ def test_gradients_against_differences():
         assert (slope - got).abs() <= (ref[name][1] * way.abs()).sum() + 1e-8, name
 
 
-def test_same_bits_and_other_streams():
-    x, w, b, ids, teacher, g = _make(500, 128, 2000, torch.bfloat16, 32, k=7)
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("V", [1200, 2200])
+def test_same_bits_and_other_streams(V, t):
+    x, w, b, ids, teacher, g = _make(500, 128, V, t, 32, k=7)
     z, sids, steacher, sg = _make_scores(20, 9000, 30, torch.float16, 33)
     first = [_run(x, w, b, ids, teacher, 1.0, g), _run_scores(z, sids, steacher, 1.0, sg)]
     side = torch.cuda.Stream()
@@ -441,8 +520,9 @@ def test_same_bits_and_other_streams():
 
 
 @pytest.mark.parametrize("t", TYPES)
-def test_captured_forward_and_backward(t):
-    x, w, b, ids, teacher, g = (v.cuda() for v in _make(150, 72, 700, t, 34, k=5))
+@pytest.mark.parametrize("M,K,V", [(150, 72, 700), (300, 128, 4000)])
+def test_captured_forward_and_backward(M, K, V, t):
+    x, w, b, ids, teacher, g = (v.cuda() for v in _make(M, K, V, t, 34, k=5))
     z, sids, steacher, sg = (v.cuda() for v in _make_scores(10, 5000, 8, t, 35, 0.5))
     leaves = [v.detach().clone().requires_grad_(True) for v in (x, w, b, z)]
 

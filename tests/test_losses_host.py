@@ -57,7 +57,8 @@ def _lists(**kw):
 LISTS = [("shape", dict(k=4097)), ("shape", dict(k=-1)), ("shape", dict(rows=-1)), ("shape", dict(teacher=None)),
          ("null", dict(ids=None)), ("temperature", dict(temperature=0.0)),
          ("temperature", dict(temperature=float("nan"))), ("temperature", dict(temperature=float("inf"))),
-         ("temperature", dict(temperature=-1.0))]
+         ("temperature", dict(temperature=-1.0)), ("temperature", dict(temperature=2.0 ** -61)),
+         ("temperature", dict(temperature=2.0 ** 61))]
 
 
 def test_scores_arguments():
@@ -84,7 +85,7 @@ def test_vocab_arguments():
     lib = _lib.lib()
 
     def op(lists=None, **kw):
-        p = _lib.FlVocab(lists=lists or _lists(), M=4, V=6, K=3, x=16, ldx=3, weight=16, ldw=3)
+        p = _lib.FlVocab(lists=lists or _lists(), M=4, V=6, K=3, x=16, ldx=3, weight=16, ldw=3, train=1)
         for k, v in kw.items():
             setattr(p, k, v)
         return p
@@ -100,6 +101,7 @@ def test_vocab_arguments():
         lib.fl_vocab_backward(None, p, g, ONE, None, ONE, ONE, ONE, ws, size))
     assert "null" in back(op(), g=None) and "workspace" in back(op(), size=16)
     assert "16-byte" in back(op(), ctypes.c_void_p(24))
+    assert "train" in back(op(train=0))
     assert lib.fl_vocab_backward(None, op(_lists(rows=0), M=0), None, None, None, None, None, None, None, 0) == 0
     large = op(_lists(rows=4096), M=4096, V=4096, K=64, ldx=64, ldw=64)
     assert lib.fl_vocab_layout_bytes(large) > 4 * 2 * 4096 * 64 and lib.fl_vocab_layout_bytes(op()) == 0
