@@ -445,7 +445,7 @@ struct StepsContig {
 
 // fp32 values as two fp16 planes, v s = v0 + v1 with a power of two s that brings
 // the largest to 2^13..2^14: v1 is the rest rounded, so that what is lost is below
-// 2^-22 of v or 2^-39 of the largest.  A row holds 32 values of the one plane, the
+// 2^-22 of v or 2^-38 of the largest.  A row holds 32 values of the one plane, the
 // same 32 of the other, and so on: 64 values of a row are a step of 32 k, and the
 // three products v0 w0 + v0 w1 + v1 w0 are off by 2^-22 once more.
 __device__ __forceinline__ int64_t pair_at(int64_t c) { return c / 32 * 64 + c % 32; }

@@ -6,13 +6,13 @@
 //   dx = dz W      dW = dz^T x      db = sum over the rows of dz
 //
 // The piece of dz is what a call holds of [rows x vocabulary], in 16 bits (an
-// operand of two products; fp32: two planes).  The listed columns' own u comes from a dot product each; their
-// entries of dz are made apart, since p - q of values rounded before would
-// keep few bits where p is near 1.
+// operand of two products; fp32: two planes).  The listed columns' own u comes
+// from a dot product each; their entries of dz are made apart, since p - q of
+// values rounded before would keep few bits where p is near 1.
 //
 // Bound by the matrix instructions: four products where logits that are kept
-// would need three.  Small products go by k_vocab_*, the others by k_wide_*:
-// tiles one after the other, so that the loads of a tile begin while the one
+// would need three, beside 2 or 4 bytes of dz a logit written once and read twice.
+// Small products go by k_vocab_*, the others by k_wide_*: tiles one after the other, so that the loads of a tile begin while the one
 // before it is finished, and exponentials of one half of the waves run beside
 // the products of the other.  There fp32 operands are held as two fp16 planes
 // (half the products of three bfloat16 planes), and 16-bit rows that do not lie
@@ -62,6 +62,9 @@ struct VocabArgs {
 };
 
 // u of four listed ids of a row (-1: none), by one wave; the same in all lanes.
+// Four rows of the weight at once, since a wave's gathered rows are bound by the
+// time of a load: 4096 x 64 ids of 1024 fp16 values in 74 us, 7.2 TB/s of the
+// weight from the caches.
 constexpr int DOT_IDS = 4;
 
 template <typename T>
@@ -191,6 +194,10 @@ __device__ __forceinline__ void store_running(const VocabArgs &a, Running (&r)[M
     }
 }
 
+// The rows' running maxima and sums over a part of the vocabulary's tiles, a pair a
+// row and part.  Bound by a step's load time where there are few tiles: fp32
+// [96 x 256 -> 475] 7.7 us; by the fp32 planes' six products and LDS reads where
+// there are many: [128 x 256 -> 41000] 28 us = 96 TFLOP/s.
 template <typename T, int BM, int BN, int BK>
 __global__ __launch_bounds__(LN_NT) void k_vocab_stats(VocabArgs a) {
     using Prod = Product<T, BM, BN, BK>;
@@ -231,7 +238,7 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_stats(VocabArgs a) {
     store_running<BM, Prod::WAVES_N>(a, r, join, prod.wave_m(), prod.wave_n() / (BN / Prod::WAVES_N), row0, part);
 }
 
-// What a row's gradients are multiplied by.  SCALED (half): times the power of
+// What a row's gradients are multiplied by (2 to 11 us, 8192 rows in one workgroup).  SCALED (half): times the power of
 // two that brings the largest to 2^14, so that small ones stay normal numbers.
 template <bool SCALED>
 __global__ __launch_bounds__(1024) void k_vocab_coef(const float2 *__restrict__ rows, const float *__restrict__ g,
@@ -261,7 +268,8 @@ __global__ __launch_bounds__(1024) void k_vocab_coef(const float2 *__restrict__ 
         coef[i] = rows[i].y != INFINITY ? tau * g[i] * scale : 0.0f;
 }
 
-// dz of a piece but for the listed columns.
+// dz of a piece but for the listed columns: the product again, an exponential in
+// place of the sums.  fp32 [128 x 256 -> 41000] 32 us, bound as k_vocab_stats.
 template <typename T, int BM, int BN, int BK>
 __global__ __launch_bounds__(LN_NT) void k_vocab_grad(VocabArgs a) {
     using Prod = Product<T, BM, BN, BK>;
@@ -292,7 +300,8 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_grad(VocabArgs a) {
     });
 }
 
-// dz of the listed columns in the piece.
+// dz of the listed columns in the piece: scattered stores of 2 or 4 bytes, 4096 x 64
+// of them 12.5 us.
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
     const int64_t i = fl_block() * LS_NT + threadIdx.x, k = a.op.lists.k;
@@ -310,7 +319,9 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
     else ((T *)a.d)[row * a.ldd + v] = (T)d;
 }
 
-// A piece's part of dx, added to what is there if `add`.
+// A piece's part of dx, added to what is there if `add`: the vocabulary is the long
+// axis and is cut into parts.  fp32 [128 x 256 -> 41000] 35 us in 256 workgroups (46
+// in 160, of at least 512 columns each).
 template <typename T, int BM, int BN, int BK>
 __global__ __launch_bounds__(LN_NT) void k_vocab_dx(VocabArgs a) {
     using Prod = Product<T, BM, BN, BK>;
@@ -350,7 +361,8 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_dx(VocabArgs a) {
 }
 
 // The parts of a sum added and rounded: four values a lane, a quarter of the
-// parts a wave, each in order and then the quarters.
+// parts a wave, each in order and then the quarters.  HBM-bound: 67 MB of
+// parts in 17 us.
 template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_vocab_fold(const float *__restrict__ part, uint32_t parts, int64_t n,
                                                       const float *__restrict__ unscale,
@@ -389,7 +401,8 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_fold(const float *__restrict__ 
     else store_some<T, 4>(out + i, o, have);
 }
 
-// A piece's rows of dW, or of a part of the rows' sum.
+// A piece's rows of dW, or of a part of the rows' sum.  fp32 [128 x 256 -> 41000]
+// 40 us: four steps a tile, so that much of it is beginnings and stores.
 template <typename T, int BM, int BN, int BK>
 __global__ __launch_bounds__(LN_NT) void k_vocab_dw(VocabArgs a) {
     using Prod = Product<T, BM, BN, BK>;
@@ -433,7 +446,8 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_dw(VocabArgs a) {
     }
 }
 
-// Column sums of a part of the rows of dz, a thread a column.
+// Column sums of a part of the rows of dz, a thread a column: 21 MB in 7.7 us, from
+// the last level cache.
 template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
     const int64_t blocks = (a.width + LS_NT - 1) / LS_NT, item = fl_block(), part = item / blocks;
@@ -455,8 +469,9 @@ constexpr bool is_pairs() {
 }
 
 // The largest finite magnitude of x and of weight, a part of them a workgroup.
-// Rows of x in which nothing is listed do not count and are laid out as zeros
-// (padded rows may hold anything), a wave a row; live: those that count.
+// HBM-bound: 1.18 GB of bfloat16 in 263 us = 4.5 TB/s.  Rows of x in which nothing
+// is listed do not count and are laid out as zeros (padded rows may hold anything),
+// a wave a row; live: those that count.
 constexpr int LAY_PARTS = 1024;
 
 template <typename T>
@@ -519,9 +534,11 @@ __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restric
 
 // x and weight as rows of half values on 16 bytes: fp32 as two planes (pair_at),
 // bfloat16 times a power of two that brings the largest to 2^13..2^14 (what is
-// above 2^-31 of it is held exactly, and what is lost below 2^-39), half, and
-// bfloat16 that no backward follows, as they are; zeros behind a row.  (dz, in half, is then rounded by 2^-12 of itself; by 2^-9 in
-// bfloat16 it made the gradients' error 1.4 to 1.5 times that of their own rounding.)
+// above 2^-31 of it is held exactly, and what is lost below 2^-38), half, and
+// bfloat16 that no backward follows, as they are; zeros behind a row.  (dz, in
+// half, is then rounded by 2^-11 of itself; by 2^-8 in bfloat16 it made the
+// gradients' error 1.4 to 1.5 times that of their own rounding.)  HBM-bound: 1.18
+// GB of bfloat16 read and written in 443 us = 5.3 TB/s.
 template <typename T, bool SCALED>
 __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restrict__ most,
                                                const uint8_t *__restrict__ live, uint16_t *__restrict__ x,
@@ -653,6 +670,14 @@ __device__ __forceinline__ void lane_bias(const VocabArgs &a, int64_t n, float (
     }
 }
 
+// The rows' running maxima and sums over a part of the vocabulary's tiles: a lane
+// keeps those of its own columns in LDS over all tiles, and they are joined at the
+// end.  An exponent is one multiply-add from the product; the maximum is the
+// lane's first until a sum overflows, so that it is not looked for in every tile.
+// bf16 [8192 x 512 -> 41000] 339 us = 1014 TFLOP/s, fp16 [4096 x 1024 -> 123000]
+// 945 us = 1092 (a large library product 1313 and 1451 on the same card), fp32
+// [1536 x 2048 -> 1645] 46 us = 225 (153), in 156 tiles on 256 CUs; [512 x 128 ->
+// 4.6M] bf16 961 us = 627: of two steps a tile, the exponentials are half.
 template <typename T, typename H, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
     using Tiles = LogitTiles<T, H, BM, WN, STAGES>;
@@ -672,7 +697,8 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
     const float scale = product_scale(a);
     Run run;
     run.template run<false>(
-        tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](int i, uint16_t *la, uint16_t *lb) { tiles.feed(a, i, la, lb); },
+        tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds,
+        [&](int i, uint16_t *la, uint16_t *lb) { tiles.feed(a, i, la, lb); },
         [&](int64_t t) {
             const int lane = made_here(fl_lane());
             Running *state = sums + lane;
@@ -724,7 +750,9 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
     store_running<BM, WN>(a, r, reinterpret_cast<Running *>(wide_lds), run.wave_m(), run.wave_n() / 64, row0, part);
 }
 
-// dz of a piece but for the listed columns.
+// dz of a piece but for the listed columns (a row's only one is made in its tile).
+// 436, 1073 and 48 us where k_wide_stats takes 339, 945 and 46: what dz's stores
+// add, 672 MB of them in the first.
 template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
     using Tiles = LogitTiles<T, _Float16, BM, WN, STAGES>;
@@ -756,7 +784,8 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
     const float scale = product_scale(a);
     Run run;
     run.template run<false>(
-        tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds, [&](int i, uint16_t *la, uint16_t *lb) { tiles.feed(a, i, la, lb); },
+        tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds,
+        [&](int i, uint16_t *la, uint16_t *lb) { tiles.feed(a, i, la, lb); },
         [&](int64_t t) {
             const int lane = made_here(fl_lane());
             const int64_t c = (t0 + t) * WN * 64 + run.wave_n() + (lane >> 4) * 16, n = a.v0 + c;  // c: in the piece
@@ -801,7 +830,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
 }
 
 // Column sums of a part of the rows of dz: 512 columns a workgroup, eight a lane,
-// a quarter of the rows a wave.
+// a quarter of the rows a wave.  HBM-bound: 10 MB in 5.4 us, from the caches.
 constexpr int COLS_WIDE = 8 * FL_WAVE;
 
 template <bool PAIRS>
@@ -838,7 +867,10 @@ __global__ __launch_bounds__(LS_NT) void k_wide_cols(VocabArgs a) {
         a.sums[part * a.width + c0 + i] = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
 }
 
-// A piece's part of dx, added to what is there if `add`.
+// A piece's part of dx, added to what is there if `add`; with one part and one piece
+// the result itself.  bf16 [8192 x 512 -> 41000] 333 us = 1033 TFLOP/s, fp16
+// [4096 x 1024 -> 123000] 868 us = 1189; the weight's steps are read transposed
+// from LDS.
 template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
     constexpr bool PAIRS = is_pairs<T>();
@@ -914,7 +946,9 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
         });
 }
 
-// A piece's rows of dW, or of a part of the rows' sum: tiles in a row.
+// A piece's rows of dW, or of a part of the rows' sum: tiles in a row.  Both
+// operands are read transposed, with twice the LDS instructions of k_wide_dx: 468
+// us = 735 TFLOP/s and 1163 us = 887 in its cases.
 template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
     constexpr bool PAIRS = is_pairs<T>();
@@ -1110,10 +1144,10 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
             const int64_t n = want < most ? want : most;
             s.dx_parts = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
         } else {
-            // enough workgroups for the chip, of at least 512 columns
+            // enough workgroups for the chip, of at least 256 columns
             s.dx_tile = op->M > 64 && op->K > 64 ? 128 : 64;
             const int64_t tiles = ceil_div(op->M, s.dx_tile) * ceil_div(op->K, s.dx_tile);
-            const int64_t want = ceil_div(1024, tiles > 0 ? tiles : 1), most = p.piece / 512, n = want < most ? want : most;
+            const int64_t want = ceil_div(1024, tiles > 0 ? tiles : 1), most = p.piece / 256, n = want < most ? want : most;
             s.dx_parts = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
         }
         s.dx_direct = p.wide && s.dx_parts == 1 && p.piece == op->V;

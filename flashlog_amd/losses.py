@@ -154,16 +154,21 @@ def linear_cross_entropy(x, weight, target, bias=None):
     x [..., inputs], weight [vocabulary, inputs], bias [vocabulary] (x's type
     or float32; -inf takes a column out), target [...] integers; float32
     [...].  A row whose target is outside [0, vocabulary) has loss 0 and gives
-    no gradient; its x still has to be finite, since 0 times an infinity is NaN
+    no gradient; its x may be any finite values, but 0 times an infinity is NaN
     in weight's gradient.  A target that the bias takes out has loss inf, a row
     of which nothing is left 0 without a gradient.
 
     No logits are kept: the backward computes them again, a piece of the
-    vocabulary at a time, in a workspace of up to 1 GB.  Their gradient is
-    rounded to the operands' type as an operand of two products and a term of
-    the bias's.  Products are as exact as ``attention.linear``'s, softmax terms
-    are off by 2^-23 of themselves times 1 + their logit's distance from the
-    largest."""
+    vocabulary at a time, in a workspace of 1 GB (of 256 columns where there
+    are more rows than that holds).  Large products lay float32 operands out as
+    two half-precision planes, and bfloat16 ones in training as scaled half
+    (a copy of x's and weight's size, held for the backward): a value is off by
+    2^-22 of itself (bfloat16: by nothing) or by 2^-38 of the largest of its
+    tensor.  The logits' gradient is rounded to half the same way, or to the
+    operands' type, as an operand of two products and a term of the bias's.
+    Softmax terms are off by 2^-23 of themselves times 1 + their logit's
+    distance from the largest; a bias whose quotient by the temperature
+    overflows float32 counts as infinite."""
     _need_gpu("linear_cross_entropy", x, weight, target, bias)
     lead = _vocab_operands("linear_cross_entropy", x, weight, bias)
     return _vocab_loss("linear_cross_entropy", x, weight, bias, _targets("linear_cross_entropy", lead, target))
