@@ -446,6 +446,126 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_dw(VocabArgs a) {
     }
 }
 
+// dW of up to 32 KS rows, which is as good as a copy of W: HBM-bound by its stores.  A
+// wave keeps x's columns of its band in registers and walks the vocabulary, 16
+// columns of dz a tile, whose loads are a tile ahead.  The tile's values go through
+// the wave's own LDS, so that a store takes whole rows of the band; of rows of whole
+// 16 bytes nothing is masked, and lanes behind the end store what others do: where the
+// number of stores is known the wait for the loads leaves them in flight.  fp32 [23 x
+// 1152 -> 431394] 428 us = 4.6 TB/s (stores of 64 bytes of 16 rows, masked, 686; tiles
+// of 128 x 128 1011), fp16 [4 x 1024 -> 400000] 160 (363; 610), bf16 [16 x 512 ->
+// 200000] 45 (101; 160).
+// Up to 128 rows of 16-bit values and 64 of fp32 ([120 x 512 -> 200000] bf16 127 us,
+// 189 by k_wide_dw's tiles, fp32 319 and 303).
+inline int64_t few_rows(int dtype) { return dtype == FL_F32 ? 64 : 128; }
+constexpr int64_t FEW_WALKS = 512;  // workgroups
+
+template <typename T, int KS>
+constexpr int few_cols() {
+    return 512 / (int)sizeof(T) / KS;  // of x in registers: three planes of fp32
+}
+
+template <typename T, bool WIDE, int KS>
+__global__ __launch_bounds__(LS_NT) void k_few_dw(VocabArgs a) {
+    using H = typename std::conditional<WIDE, _Float16, T>::type;
+    constexpr int P = Planes<H>::N, PAIR = sizeof(T) == 2 ? 2 : 1, COLS = few_cols<T, KS>(), NT = COLS / 16;
+    using Out = Vec<T, 4 * PAIR>;
+    constexpr int G = 4 * PAIR, PITCH = COLS + G, STORES = 16 * COLS / G / FL_WAVE;
+    __shared__ __align__(16) T rows[LS_WAVES][16 * PITCH];
+    T *mine = rows[fl_wave_id()];
+    const int64_t M = a.op.M, K = a.op.K, bands = (K + COLS - 1) / COLS, tiles = (a.width + 15) / 16;
+    const int64_t item = (int64_t)blockIdx.x * LS_WAVES + fl_wave_id(), runs = (int64_t)gridDim.x * LS_WAVES / bands;
+    const int64_t run = item / bands, c0 = item % bands * COLS;
+    if (run >= runs || run >= tiles) return;
+    const int r = fl_lane() & 15, q = fl_lane() >> 4;
+    const H *xs = (const H *)(WIDE ? (const void *)a.x : a.op.x);
+    const int64_t ldx = WIDE ? a.ldx : a.op.ldx;
+    u32x4 x[KS][NT][P];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            // 16-bit tiles come in pairs whose columns alternate by fours: eight in a row a lane
+            const int64_t c = c0 + (PAIR == 1 ? j * 16 + r : j / 2 * 32 + (r >> 2) * 8 + (j & 1) * 4 + (r & 3));
+            H v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t m = s * 32 + q * 8 + i;
+                v[i] = m < M && c < K ? xs[m * ldx + c] : (H)0.0f;
+            }
+            chunk_planes<H>(v, x[s][j]);
+        }
+    H next[KS][8];
+    const auto load = [&](int64_t t) {
+        const int64_t v = t * 16 + r < a.width ? t * 16 + r : a.width - 1;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t m = s * 32 + q * 8 + i < M ? s * 32 + q * 8 + i : M - 1;
+                next[s][i] = ((const H *)a.d)[WIDE ? dz_at<false>(a, m, v) : m * a.ldd + v];
+            }
+    };
+    const float f = *a.unscale, f2 = a.undo ? a.undo[0] : 1.0f;
+    // the chunks of G columns that a lane stores
+    const int band = (int)(K - c0 < COLS ? K - c0 : COLS), chunks = (band + G - 1) / G;
+    const auto walk = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        load(run);
+        for (int64_t t = run; t < tiles; t += runs) {
+            u32x4 d[KS][P];
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (s * 32 + q * 8 + i >= M) next[s][i] = (H)0.0f;
+                chunk_planes<H>(next[s], d[s]);
+            }
+            load(t + runs < tiles ? t + runs : t);
+            fl_wave_sync();
+#pragma unroll
+            for (int p = 0; p < NT / PAIR; ++p) {
+                Vec<T, G> o;
+#pragma unroll
+                for (int h = 0; h < PAIR; ++h) {
+                    f32x4 acc{0, 0, 0, 0};
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        const u32x4(&b)[P] = x[s][p * PAIR + h];
+                        if constexpr (P == 3) {  // smallest products first
+                            acc = mfma<H>(b[2], d[s][0], acc);
+                            acc = mfma<H>(b[1], d[s][1], acc);
+                            acc = mfma<H>(b[0], d[s][2], acc);
+                            acc = mfma<H>(b[1], d[s][0], acc);
+                            acc = mfma<H>(b[0], d[s][1], acc);
+                        }
+                        acc = mfma<H>(b[0], d[s][0], acc);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o.v[h * 4 + e] = (T)(acc[e] * f * f2);
+                }
+                *reinterpret_cast<u32x4 *>(mine + r * PITCH + (p * 4 + q) * G) = __builtin_bit_cast(u32x4, o);
+            }
+            fl_wave_sync();
+            const int have = (int)(a.width - t * 16 < 16 ? a.width - t * 16 : 16) * chunks;
+            T *out = (T *)a.dw + (a.v0 + t * 16) * K + c0;
+#pragma unroll
+            for (int i = 0; i < STORES; ++i) {
+                int at = i * FL_WAVE + fl_lane();
+                if (!WHOLE && at >= have) continue;
+                at = at < have ? at : have - 1;
+                const int row = at / chunks, c = (at - row * chunks) * G;
+                const Vec<T, G> o = __builtin_bit_cast(
+                    Out, *reinterpret_cast<const u32x4 *>(mine + row * PITCH + c));
+                if (WHOLE || c + G <= band) store_vec<T, G>(out + row * K + c, o);
+                else store_some<T, G>(out + row * K + c, o, band - c);
+            }
+        }
+    };
+    if (K % G == 0) walk(std::true_type());
+    else walk(std::false_type());
+}
+
 // Column sums of a part of the rows of dz, a thread a column: 21 MB in 7.7 us, from
 // the last level cache.
 template <typename T>
@@ -1120,7 +1240,7 @@ struct VocabSpace {
     size_t coef, d, dx, dw, db, bytes;
     int dx_parts, dw_parts, db_parts;
     int dx_tile, dx_cols, dw_cols, dw_tile;
-    bool dx_direct;
+    bool dx_direct, few_dw;
     uint32_t dw_walks;
 };
 
@@ -1153,7 +1273,9 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
         s.dx_direct = p.wide && s.dx_parts == 1 && p.piece == op->V;
         if (!s.dx_direct) s.dx = take((size_t)s.dx_parts * op->M * op->K * 4);
     }
-    if (with_dw) {
+    s.few_dw = op->M <= few_rows(op->dtype);
+    if (with_dw && s.few_dw) s.dw_parts = 1;
+    else if (with_dw) {
         if (p.wide) {
             s.dw_tile = p.small ? 128 : 256;
             s.dw_cols = p.small ? 128 : narrow;
@@ -1334,7 +1456,25 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
                 FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 128, 128, BK>), g, nt, 0, st, a);
             else FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 64, 64, BK>), g, nt, 0, st, a);
         }
-        if (dw && op->K) {
+        if (dw && op->K && s.few_dw) {
+            const int cols = op->M <= 32 ? few_cols<T, 1>() : op->M <= 64 ? few_cols<T, 2>() : few_cols<T, 4>();
+            const int64_t bands = ceil_div(op->K, cols), all = ceil_div(bands * ceil_div(a.width, 16), LS_WAVES);
+            grid = ceil_div(bands, LS_WAVES);
+            if (grid < FEW_WALKS) grid = all < FEW_WALKS ? all : FEW_WALKS;
+            if (!fits(grid)) return fail();
+            a.dw = dw;
+            const dim3 g((unsigned)grid), t(LS_NT);
+            const auto launch = [&](auto wide) {
+                constexpr bool WIDE = decltype(wide)::value;
+                if (op->M <= 32) FL_LAUNCH("k_few_dw", (k_few_dw<T, WIDE, 1>), g, t, 0, st, a);
+                else if (op->M <= 64) FL_LAUNCH("k_few_dw", (k_few_dw<T, WIDE, 2>), g, t, 0, st, a);
+                else if constexpr (sizeof(T) == 2) FL_LAUNCH("k_few_dw", (k_few_dw<T, WIDE, 4>), g, t, 0, st, a);
+            };
+            if constexpr (sizeof(T) == 2) {
+                if (p.wide) launch(std::true_type());
+                else launch(std::false_type());
+            } else launch(std::false_type());
+        } else if (dw && op->K) {
             const int rows = s.dw_tile, cols = p.wide ? s.dw_cols : s.dw_tile;
             a.m_tiles = (uint32_t)ceil_div(a.width, rows);
             a.n_tiles = (uint32_t)ceil_div(op->K, cols);

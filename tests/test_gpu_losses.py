@@ -169,14 +169,15 @@ def test_linear_distillation(M, K, V, k, tau, t):
 
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("M,K,V", [(300, 256, 1000), (257, 512, 2049), (1000, 64, 4096), (520, 200, 3333),
-                                   (2, 1024, 70000), (70, 512, 4096), (150, 200, 4500), (400, 100, 3400), (460, 64, 4600)])
+                                   (2, 1024, 70000), (48, 600, 5000), (70, 512, 4096), (150, 200, 4500), (400, 100, 3400), (460, 64, 4600)])
 def test_many_tiles(M, K, V, t):
     """Sizes of several tiles in every direction, odd ends among them."""
     x, w, b, ids, _, g = (v.cuda() if v is not None else None for v in _make(M, K, V, t, M + K + V))
     _check(x, w, b, ids, None, 1.0, g)
 
 
-@pytest.mark.parametrize("t,M,K", [(torch.float32, 300, 16), (torch.bfloat16, 700, 8), (torch.float16, 700, 8)])
+@pytest.mark.parametrize("t,M,K", [(torch.float32, 300, 16), (torch.bfloat16, 700, 8), (torch.float16, 700, 8),
+                                   (torch.bfloat16, 128, 9)])
 def test_several_pieces_of_the_vocabulary(t, M, K):
     """More logits than a piece of 1 GB holds (in the last one a few columns), the bias's gradient among them."""
     V = (1 << 30) // (4 if t is torch.float32 else 2) // M // 256 * 256 + 300 + 11
