@@ -793,7 +793,7 @@ __device__ __forceinline__ void lane_bias(const VocabArgs &a, int64_t n, float (
 // The rows' running maxima and sums over a part of the vocabulary's tiles: a lane
 // keeps those of its own columns in LDS over all tiles, and they are joined at the
 // end.  An exponent is one multiply-add from the product; the maximum is the
-// lane's first until a sum overflows, so that it is not looked for in every tile.
+// lane's first until a sum passes 2^64, so that it is not looked for in every tile.
 // bf16 [8192 x 512 -> 41000] 339 us = 1014 TFLOP/s, fp16 [4096 x 1024 -> 123000]
 // 945 us = 1092 (a large library product 1313 and 1451 on the same card), fp32
 // [1536 x 2048 -> 1645] 46 us = 225 (153), in 156 tiles on 256 CUs; [512 x 128 ->
@@ -836,7 +836,8 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
                     const float t = a.op.bias ? b[e] - less : -less;
                     return e < have ? __builtin_fmaf(v, scale, t) : -INFINITY;
                 };
-                // what the lane had first serves as the maximum, until a sum overflows or is not a number
+                // what the lane had first serves as the maximum, until a sum passes 2^64 (joined with others of up to that it
+                // stays finite) or is not a number
                 if (__any(have < 16)) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s += exp2_of(u(e, r.m));
@@ -848,7 +849,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
                     }
                 }
                 s += r.s;
-                if (r.m == -INFINITY || !(s < INFINITY)) {  // a lane's own: rows do not touch each other's bits
+                if (r.m == -INFINITY || !(s < 0x1p64f)) {  // a lane's own: rows do not touch each other's bits
                     float m = r.m;
                     s = 0.0f;
 #pragma unroll

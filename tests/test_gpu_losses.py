@@ -195,6 +195,17 @@ def test_sharp_rows(t):
     _check(x, w, b, ids, None, 1.0, g)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("step", [84.0, 200.0])
+def test_columns_far_above_the_first(step, t):
+    """Large products in which a part's later columns are e^84 (within float32's range) or e^200 times its first ones."""
+    M, K, V = 300, 32, 40000
+    x, w, _, ids, _, g = (v.cuda() if v is not None else None for v in _make(M, K, V, t, 19, bias=False))
+    b = step * (torch.arange(V, device="cuda") // 256 % 2)
+    ids[::2, 0] = 256 + ids[::2, 0] % 256
+    _check(x, w, b, ids, None, 1.0, g)
+
+
 def test_small_gradients_in_half():
     """Weights of the rows' losses far below half's smallest number, in all rows or in some."""
     x, w, b, ids, _, g = _make(40, 64, 500, torch.float16, 10, bias=False)
