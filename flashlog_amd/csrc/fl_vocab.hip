@@ -49,7 +49,8 @@ struct VocabArgs {
     const float *coef;    // tau g of every row (times a power of two), 0 where it has no gradient
     void *d;              // dz of the piece: [M][ldd], wide: blocks of D_BLOCK columns, [d_rows][ldd] each
     int64_t ldd, d_block;  // d_block: from one to the next
-    float *sums;          // dx: [parts][M][K]; dW: [parts][width][K]
+    int64_t dz_rows;      // rows of dz: M, or 2 M where the second M are what rounding left of the first
+    float *sums;          // dx: [parts][dz_rows][K]; dW: [parts][width][K]
     void *dw;
     void *dx;             // where one part and one piece are all of it
     const float *unscale;  // what undoes dz's power of two
@@ -293,10 +294,15 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_grad(VocabArgs a) {
     each_u<T>(a, prod.acc, col, a.v0 + a.width, [&](int i, int j, const float (&u)[4]) {
         const int64_t n = col + j * 16 + (fl_lane() >> 4) * 4 - a.v0;
         if (row + i * 16 >= a.op.M || n >= a.ldd) return;
-        Vec<T, 4> o;
+        Vec<T, 4> o, rest;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o.v[e] = (T)(c[i] == 0.0f ? 0.0f : c[i] * exp2_of(u[e] - lse[i]));
+        for (int e = 0; e < 4; ++e) {
+            const float d = c[i] == 0.0f ? 0.0f : c[i] * exp2_of(u[e] - lse[i]);
+            o.v[e] = (T)d;
+            rest.v[e] = (T)(d - (float)o.v[e]);
+        }
         store_vec<T, 4>((T *)a.d + (row + i * 16) * a.ldd + n, o);
+        if (a.dz_rows > a.op.M) store_vec<T, 4>((T *)a.d + (a.op.M + row + i * 16) * a.ldd + n, rest);
     });
 }
 
@@ -316,7 +322,11 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
         to[0] = (_Float16)d;
         to[32] = (_Float16)(d - (float)to[0]);
     } else if constexpr (WIDE) ((_Float16 *)a.d)[dz_at<false>(a, row, v)] = (_Float16)d;
-    else ((T *)a.d)[row * a.ldd + v] = (T)d;
+    else {
+        const T o = (T)d;
+        ((T *)a.d)[row * a.ldd + v] = o;
+        if (a.dz_rows > a.op.M) ((T *)a.d)[(a.op.M + row) * a.ldd + v] = (T)(d - (float)o);
+    }
 }
 
 // A piece's part of dx, added to what is there if `add`: the vocabulary is the long
@@ -328,7 +338,7 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_dx(VocabArgs a) {
     __shared__ __align__(16) uint16_t lds[Prod::LDS_ELEMS];
     const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
     const uint32_t tile = w / a.parts, part = w % a.parts;
-    const int64_t row0 = (int64_t)(tile / a.n_tiles) * BM, n0 = (int64_t)(tile % a.n_tiles) * BN, M = a.op.M;
+    const int64_t row0 = (int64_t)(tile / a.n_tiles) * BM, n0 = (int64_t)(tile % a.n_tiles) * BN, M = a.dz_rows;
     const int64_t steps = (a.width + BK - 1) / BK, k0 = steps * part / a.parts * BK;
     const int64_t k1 = part + 1 == a.parts ? a.width : steps * (part + 1) / a.parts * BK;
     ContigTile<T, BM, BK> ta;
@@ -473,7 +483,7 @@ __global__ __launch_bounds__(LS_NT) void k_few_dw(VocabArgs a) {
     constexpr int G = 4 * PAIR, PITCH = COLS + G, STORES = 16 * COLS / G / FL_WAVE;
     __shared__ __align__(16) T rows[LS_WAVES][16 * PITCH];
     T *mine = rows[fl_wave_id()];
-    const int64_t M = a.op.M, K = a.op.K, bands = (K + COLS - 1) / COLS, tiles = (a.width + 15) / 16;
+    const int64_t M = a.dz_rows, K = a.op.K, bands = (K + COLS - 1) / COLS, tiles = (a.width + 15) / 16;
     const int64_t item = (int64_t)blockIdx.x * LS_WAVES + fl_wave_id(), runs = (int64_t)gridDim.x * LS_WAVES / bands;
     const int64_t run = item / bands, c0 = item % bands * COLS;
     if (run >= runs || run >= tiles) return;
@@ -491,7 +501,7 @@ __global__ __launch_bounds__(LS_NT) void k_few_dw(VocabArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int64_t m = s * 32 + q * 8 + i;
-                v[i] = m < M && c < K ? xs[m * ldx + c] : (H)0.0f;
+                v[i] = m < M && c < K ? xs[(m < a.op.M ? m : m - a.op.M) * ldx + c] : (H)0.0f;
             }
             chunk_planes<H>(v, x[s][j]);
         }
@@ -574,7 +584,7 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
     const int64_t c = item % blocks * LS_NT + threadIdx.x;
     if (part >= a.parts || c >= a.width) return;
     float s = 0.0f;
-    for (int64_t m = a.op.M * part / a.parts; m < a.op.M * (part + 1) / a.parts; ++m)
+    for (int64_t m = a.dz_rows * part / a.parts; m < a.dz_rows * (part + 1) / a.parts; ++m)
         s += (float)((const T *)a.d)[m * a.ldd + c];
     a.sums[part * a.width + c] = s;
 }
@@ -1164,7 +1174,7 @@ struct VocabPlan {
     uint32_t m_tiles, n_tiles, parts;  // parts: of the vocabulary, in the forward
     int64_t piece, d_cols, ldd;        // columns of dz in the backward, with those that pad them, and its row stride
     int64_t d_block;                   // wide: from one block of its columns to the next
-    int64_t d_rows, cols;              // rows of dz and inputs, with those that pad them
+    int64_t dz_rows, d_rows, cols;     // rows of dz; they and the inputs with those that pad them
     int64_t size;                      // bytes of a value of dz
 };
 
@@ -1179,12 +1189,13 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     // Laying the weight out takes up to four passes over it, which few rows do not pay for: in units of 1e-12 s a value of
     // it, fp32 3.5 and then 2 rows / 360 a product, against 2 rows / 150 (0.9 at least) from where it lies, with four
     // products in training; 16-bit values 0.9 to 1.3 and 2 rows / 1000, against 2 rows / 430 (0.45 at least).  bfloat16 in
-    // training is laid out whatever it costs, so that dz is half.
+    // training is laid out whatever it costs and at every size, so that dz is half.
     int64_t least = 65;
     if (op->dtype == FL_F32) least = op->train ? 144 : 448;
     else if (op->dtype == FL_BF16 && op->train) least = 1;
     else if (p.lay) least = op->train ? 128 : 384;
-    p.wide = op->K >= 1 && op->K <= 1 << 20 && op->M >= least && (double)op->M * op->V * op->K >= 1 << 27;
+    p.wide = op->K >= 1 && op->K <= 1 << 20 && op->M >= least &&
+             (least == 1 || (double)op->M * op->V * op->K >= 1 << 27);
     p.lay = p.lay && p.wide;
     p.scaled = p.scaled && p.wide;
     if (p.wide) {
@@ -1215,7 +1226,9 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     if (piece < 256) piece = 256;
     p.piece = piece < op->V ? piece : op->V;
     p.d_cols = p.wide ? ceil_div(p.piece, D_BLOCK) * D_BLOCK : ceil_div(p.piece, 8) * 8;
-    p.d_rows = p.wide ? ceil_div(op->M, step) * step : op->M;
+    // half: of few rows a gradient can be one term of dz, whose rounding would be as large as the gradient's own
+    p.dz_rows = op->dtype == FL_F16 && !p.wide && op->M <= 64 ? 2 * op->M : op->M;
+    p.d_rows = p.wide ? ceil_div(op->M, step) * step : p.dz_rows;
     p.ldd = !p.wide ? p.d_cols : p.pairs ? 2 * D_BLOCK : D_BLOCK;
     p.d_block = p.d_rows * p.ldd;
     return p;
@@ -1266,15 +1279,15 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
             s.dx_parts = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
         } else {
             // enough workgroups for the chip, of at least 256 columns
-            s.dx_tile = op->M > 64 && op->K > 64 ? 128 : 64;
-            const int64_t tiles = ceil_div(op->M, s.dx_tile) * ceil_div(op->K, s.dx_tile);
+            s.dx_tile = p.dz_rows > 64 && op->K > 64 ? 128 : 64;
+            const int64_t tiles = ceil_div(p.dz_rows, s.dx_tile) * ceil_div(op->K, s.dx_tile);
             const int64_t want = ceil_div(1024, tiles > 0 ? tiles : 1), most = p.piece / 256, n = want < most ? want : most;
             s.dx_parts = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
         }
         s.dx_direct = p.wide && s.dx_parts == 1 && p.piece == op->V;
-        if (!s.dx_direct) s.dx = take((size_t)s.dx_parts * op->M * op->K * 4);
+        if (!s.dx_direct) s.dx = take((size_t)s.dx_parts * p.dz_rows * op->K * 4);
     }
-    s.few_dw = op->M <= few_rows(op->dtype);
+    s.few_dw = p.dz_rows <= few_rows(op->dtype);
     if (with_dw && s.few_dw) s.dw_parts = 1;
     else if (with_dw) {
         if (p.wide) {
@@ -1399,6 +1412,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
     a.d_block = p.d_block;
     a.d_cols = p.d_cols;
     a.d_rows = p.d_rows;
+    a.dz_rows = p.dz_rows;
     const dim3 nt(LN_NT), wt(WD_NT);
     const auto fits = [&](int64_t grid) { return launch_fits(grid, WD_NT); };
     const auto fail = [&]() { return fl_fail(FL_ERR_ARG, "linear_loss: too many tiles for one launch (shape)"); };
@@ -1437,7 +1451,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             else FL_LAUNCH("k_vocab_listed", (k_vocab_listed<T, false>), g, dim3(LS_NT), 0, st, a);
         }
         if (dx && op->K) {
-            a.m_tiles = (uint32_t)ceil_div(op->M, s.dx_tile);
+            a.m_tiles = (uint32_t)ceil_div(p.dz_rows, s.dx_tile);
             a.n_tiles = (uint32_t)ceil_div(op->K, p.wide ? s.dx_cols : s.dx_tile);
             a.parts = (uint32_t)s.dx_parts;
             a.sums = (float *)(ws + s.dx);
@@ -1458,7 +1472,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             else FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 64, 64, BK>), g, nt, 0, st, a);
         }
         if (dw && op->K && s.few_dw) {
-            const int cols = op->M <= 32 ? few_cols<T, 1>() : op->M <= 64 ? few_cols<T, 2>() : few_cols<T, 4>();
+            const int cols = p.dz_rows <= 32 ? few_cols<T, 1>() : p.dz_rows <= 64 ? few_cols<T, 2>() : few_cols<T, 4>();
             const int64_t bands = ceil_div(op->K, cols), all = ceil_div(bands * ceil_div(a.width, 16), LS_WAVES);
             grid = ceil_div(bands, LS_WAVES);
             if (grid < FEW_WALKS) grid = all < FEW_WALKS ? all : FEW_WALKS;
@@ -1467,8 +1481,8 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             const dim3 g((unsigned)grid), t(LS_NT);
             const auto launch = [&](auto wide) {
                 constexpr bool WIDE = decltype(wide)::value;
-                if (op->M <= 32) FL_LAUNCH("k_few_dw", (k_few_dw<T, WIDE, 1>), g, t, 0, st, a);
-                else if (op->M <= 64) FL_LAUNCH("k_few_dw", (k_few_dw<T, WIDE, 2>), g, t, 0, st, a);
+                if (p.dz_rows <= 32) FL_LAUNCH("k_few_dw", (k_few_dw<T, WIDE, 1>), g, t, 0, st, a);
+                else if (p.dz_rows <= 64) FL_LAUNCH("k_few_dw", (k_few_dw<T, WIDE, 2>), g, t, 0, st, a);
                 else if constexpr (sizeof(T) == 2) FL_LAUNCH("k_few_dw", (k_few_dw<T, WIDE, 4>), g, t, 0, st, a);
             };
             if constexpr (sizeof(T) == 2) {
@@ -1522,7 +1536,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
     }
     if (dx && op->K && !s.dx_direct)
         FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(op->M * op->K, FL_WAVE * 4)), dim3(LS_NT), 0, st,
-                  (const float *)(ws + s.dx), (uint32_t)s.dx_parts, op->M * op->K, a.unscale,
+                  (const float *)(ws + s.dx), (uint32_t)(s.dx_parts * (p.dz_rows / op->M)), op->M * op->K, a.unscale,
                   a.undo ? a.undo + 1 : nullptr, (T *)dx);
     return fl_check_launch("linear_loss");
 }

@@ -164,8 +164,9 @@ def linear_cross_entropy(x, weight, target, bias=None):
     two half-precision planes, and bfloat16 ones in training as scaled half
     (a copy of x's and weight's size, held for the backward): a value is off by
     2^-22 of itself (bfloat16: by nothing) or by 2^-38 of the largest of its
-    tensor.  The logits' gradient is rounded to half the same way, or to the
-    operands' type, as an operand of two products and a term of the bias's.
+    tensor.  The logits' gradient is an operand of two products and a term of
+    the bias's: float32's is held as exactly, 16-bit ones' as half (of up to 64
+    rows of half with what its rounding leaves).
     Softmax terms are off by 2^-23 of themselves times 1 + their logit's
     distance from the largest; a bias whose quotient by the temperature
     overflows float32 counts as infinite."""

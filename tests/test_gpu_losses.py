@@ -10,7 +10,7 @@ columns, weighed by p, and by (80 + 2 |lse|) e for its sums, exponentials (off
 by 2 e times 1 + the distance from the maximum) and logarithm.  p is off by
 those errors and 8 e (1 + |u - lse|) relative to itself, a teacher's share q by
 16 e (1 + the range of its list).  dz = c (p - Q) is rounded to the operands'
-type (u, and where it is held in half, at the scale of the largest |c|, 2^-38 of
+type or to half (u, and where it is held in half, at the scale of the largest |c|, 2^-38 of
 that) and enters sums of n terms with (n + 16) e.  Operands that are held in half
 at the scale of their largest (float32 as two planes, bfloat16 in training) lose
 up to 2^-38 of that."""
@@ -95,6 +95,8 @@ def vocab_reference(x, w, b, ids, teacher, tau, g):
     xm, wm = (x.abs() * live).max() if x.numel() else 0.0, w.abs().max() if w.numel() else 0.0
     lost = 2.0 ** -38 * (xm * w.abs().sum(1)[None, :] + wm * x.abs().sum(1, keepdim=True))
     loss, dloss, d, dd, c = _rows(z, (K + 16) * E * mag + lost, ids, teacher, tau, g, t)
+    if K:  # bfloat16's is held in half, half's of few rows with what rounding leaves
+        u = 2.0 ** -22 if t is torch.float16 and M <= 64 else min(u, 2.0 ** -11)
     dd = dd + u * d.abs() + c.abs().max() * 2.0 ** -38 + _tiny(t)
     dd = torch.where(c == 0, 0.0, dd)
     out = {"loss": (loss, dloss * 1.01 + 1e-30)}
