@@ -1222,12 +1222,12 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     p.n_tiles = (uint32_t)ceil_div(op->V, p.bn);
     const int64_t want = p.wide ? (p.m_tiles < 256 ? 256 / p.m_tiles : 1) : ceil_div(1024, p.m_tiles);
     p.parts = (uint32_t)(want < p.n_tiles ? want : p.n_tiles);
-    int64_t piece = (int64_t)(LS_PIECE / p.size) / (op->M > 0 ? op->M : 1) / 256 * 256;
+    // half: of few rows a gradient can be one term of dz, whose rounding would be as large as the gradient's own
+    p.dz_rows = op->dtype == FL_F16 && !p.wide && op->M <= 64 ? 2 * op->M : op->M;
+    int64_t piece = (int64_t)(LS_PIECE / p.size) / (p.dz_rows > 0 ? p.dz_rows : 1) / 256 * 256;
     if (piece < 256) piece = 256;
     p.piece = piece < op->V ? piece : op->V;
     p.d_cols = p.wide ? ceil_div(p.piece, D_BLOCK) * D_BLOCK : ceil_div(p.piece, 8) * 8;
-    // half: of few rows a gradient can be one term of dz, whose rounding would be as large as the gradient's own
-    p.dz_rows = op->dtype == FL_F16 && !p.wide && op->M <= 64 ? 2 * op->M : op->M;
     p.d_rows = p.wide ? ceil_div(op->M, step) * step : p.dz_rows;
     p.ldd = !p.wide ? p.d_cols : p.pairs ? 2 * D_BLOCK : D_BLOCK;
     p.d_block = p.d_rows * p.ldd;
