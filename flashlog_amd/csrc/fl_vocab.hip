@@ -12,7 +12,8 @@
 //
 // Bound by the matrix instructions: four products where logits that are kept
 // would need three, beside 2 or 4 bytes of dz a logit written once and read twice.
-// Small products go by k_vocab_*, the others by k_wide_*: tiles one after the other, so that the loads of a tile begin while the one
+// Small products go by k_vocab_*, the others, and bfloat16 in training, by k_wide_*:
+// tiles one after the other, so that the loads of a tile begin while the one
 // before it is finished, and exponentials of one half of the waves run beside
 // the products of the other.  There fp32 operands are held as two fp16 planes
 // (half the products of three bfloat16 planes), and 16-bit rows that do not lie
@@ -1187,11 +1188,13 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     p.lay = p.scaled || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % step ||
             op->ldx >= 1 << 23 || op->ldw >= 1 << 23;  // 32-bit offsets of 256 rows
     // Laying the weight out takes up to four passes over it, which few rows do not pay for: in units of 1e-12 s a value of
-    // it, fp32 3.5 and then 2 rows / 360 a product, against 2 rows / 150 (0.9 at least) from where it lies, with four
-    // products in training; 16-bit values 0.9 to 1.3 and 2 rows / 1000, against 2 rows / 430 (0.45 at least).  bfloat16 in
-    // training is laid out whatever it costs and at every size, so that dz is half.
+    // it, fp32 3.5 and then 2 rows / 360 a product, against 2 rows / 150 (0.9 at least) from where it lies; 16-bit values
+    // 0.9 to 1.3 and 2 rows / 1000, against 2 rows / 430 (0.45 at least).  With the four products of training fp32 has
+    // [116 x 1176 -> 454586] in 4340 us laid out and 5220 as it is, [66 x 512 -> 200000] in 850 both ways, weights that
+    // the last level cache holds ([128 x 256 -> 41000]) in 170 and 167, but [143 x 512 -> 200000], past a tile of 128, in
+    // 1040 and 1360.  bfloat16 in training is laid out whatever it costs and at every size, so that dz is half.
     int64_t least = 65;
-    if (op->dtype == FL_F32) least = op->train ? 144 : 448;
+    if (op->dtype == FL_F32) least = !op->train ? 448 : (double)op->V * op->K >= 1 << 26 ? 65 : 129;
     else if (op->dtype == FL_BF16 && op->train) least = 1;
     else if (p.lay) least = op->train ? 128 : 384;
     p.wide = op->K >= 1 && op->K <= 1 << 20 && op->M >= least &&

@@ -159,8 +159,8 @@ def linear_cross_entropy(x, weight, target, bias=None):
     of which nothing is left 0 without a gradient.
 
     No logits are kept: the backward computes them again, a piece of the
-    vocabulary at a time, in a workspace of 1 GB (of 256 columns where there
-    are more rows than that holds).  Large products lay float32 operands out as
+    vocabulary at a time, in a workspace of up to 1 GB (of 256 columns
+    where there are more rows than that holds).  Large products lay float32 operands out as
     two half-precision planes, and bfloat16 ones in training as scaled half
     (a copy of x's and weight's size, held for the backward): a value is off by
     2^-22 of itself (bfloat16: by nothing) or by 2^-38 of the largest of its

@@ -171,7 +171,7 @@ def test_linear_distillation(M, K, V, k, tau, t):
 
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("M,K,V", [(300, 256, 1000), (257, 512, 2049), (1000, 64, 4096), (520, 200, 3333),
-                                   (2, 1024, 70000), (48, 600, 5000), (70, 512, 4096), (150, 200, 4500), (400, 100, 3400), (460, 64, 4600)])
+                                   (2, 1024, 70000), (48, 600, 5000), (66, 520, 140000), (130, 256, 4100), (70, 512, 4096), (150, 200, 4500), (400, 100, 3400), (460, 64, 4600)])
 def test_many_tiles(M, K, V, t):
     """Sizes of several tiles in every direction, odd ends among them."""
     x, w, b, ids, _, g = (v.cuda() if v is not None else None for v in _make(M, K, V, t, M + K + V))
