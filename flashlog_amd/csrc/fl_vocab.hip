@@ -14,10 +14,9 @@
 // would need three, beside 2 or 4 bytes of dz a logit written once and read twice.
 // Small products go by k_vocab_*, the others, and bfloat16 in training, by k_wide_*:
 // tiles one after the other, so that the loads of a tile begin while the one
-// before it is finished, and exponentials of one half of the waves run beside
-// the products of the other.  There fp32 operands are held as two fp16 planes
-// (half the products of three bfloat16 planes), and 16-bit rows that do not lie
-// on 16 bytes as copies that do.
+// before it is finished.  There fp32 operands are held as two fp16 planes (half the
+// products of three bfloat16 planes), and 16-bit rows that do not lie on 16 bytes
+// as copies that do.
 #include "fl_abi.h"
 #include "fl_common.h"
 #include "fl_loss.h"
