@@ -1371,7 +1371,7 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
                           (uint16_t *)a.w, (float *)nullptr);
     }
     const bool few = op->lists.k <= DOT_IDS && p.parts <= 4 * FL_WAVE;
-    if (!few)
+    if (!few && op->lists.k)
         FL_LAUNCH("k_vocab_dots", k_vocab_dots<T>,
                   grid_of(ceil_div(op->M * ceil_div(op->lists.k, DOT_IDS), LS_WAVES)), dim3(LS_NT), 0, st, a);
     if (p.wide) {
