@@ -1,4 +1,5 @@
 """Calls of the losses that the documentation allows at the ends of their ranges."""
+import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
