@@ -26,8 +26,10 @@ __device__ __forceinline__ Running joined(Running a, Running b, float unit = 1.0
 }
 
 // The state that a forward leaves for the backward: rows [rows] (the maximum, the
-// sum's logarithm; +inf where the row does not count), listed [rows][k] (u of the
-// id, the sum of q at it).
+// sum's reciprocal; 0 where the row does not count), listed [rows][k] (u of the
+// id, the sum of q at it).  A term's share is 2^((u - m) unit) times the reciprocal:
+// the two as one number, log sum exp u, would be rounded by 2^-24 of its size, an
+// error that all shares of the row have (sum(p) - 1 = 6e-4 at logits of 4000).
 inline size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 inline size_t state_bytes(const fl_lists *l) { return rounded((size_t)l->rows * 8) + (size_t)l->rows * l->k * 8; }
 inline float2 *state_rows(void *state) { return (float2 *)state; }
@@ -122,7 +124,7 @@ __device__ __forceinline__ void list_row(const ListArgs &a, int64_t row, Running
     loss = fl_wave_sum_f32(loss) * (a.tau2 * LN2);
     if (fl_lane() == 0) {
         a.loss[row] = live ? loss : 0.0f;
-        a.rows[row] = float2{r.m, live ? log_sum : INFINITY};
+        a.rows[row] = float2{r.m, live ? 1.0f / r.s : 0.0f};
     }
     fl_wave_sync();
     for (int64_t j = fl_lane(); j < k; j += FL_WAVE) {

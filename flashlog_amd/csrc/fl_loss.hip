@@ -121,7 +121,7 @@ __global__ __launch_bounds__(LS_NT) void k_score_grad(ScoreArgs a) {
     if (item >= a.op.rows * a.segments) return;
     const int64_t row = item / a.segments, c0 = (item % a.segments) * LS_SEG;
     const float2 of = a.rows[row];
-    const float c = of.y != INFINITY ? a.op.temperature * a.grad[row] : 0.0f;
+    const float c = of.y != 0.0f ? a.op.temperature * a.grad[row] : 0.0f, f = c * of.y;
     T *out = (T *)a.dx + row * a.cols;
     Segment<T> s;
     s.load((const T *)a.logits + row * a.ld, c0, a.cols);
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(LS_NT) void k_score_grad(ScoreArgs a) {
 #pragma unroll
         for (int e = 0; e < G; ++e)
             s.v[i].v[e] =
-                (T)(c == 0.0f ? 0.0f : c * exp2_of(__builtin_fmaf((float)s.v[i].v[e] - of.x, a.scale, -of.y)));
+                (T)(c == 0.0f ? 0.0f : f * exp2_of(((float)s.v[i].v[e] - of.x) * a.scale));
         const int64_t at = c0 + (i * FL_WAVE + fl_lane()) * G;
         if (at + G <= a.cols) store_cols<T, G>(out + at, s.v[i]);
         else store_first<T, G>(out + at, s.v[i], (int)(a.cols - at));
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(LS_NT) void k_score_grad(ScoreArgs a) {
         waited = true;
         if (here) {
             const float2 l = a.listed[row * a.op.k + j];
-            out[id] = (T)(c * (exp2_of(__builtin_fmaf(l.x - of.x, a.scale, -of.y)) - l.y));
+            out[id] = (T)(c * (exp2_of((l.x - of.x) * a.scale) * of.y - l.y));
         }
     }
 }

@@ -250,7 +250,7 @@ __global__ __launch_bounds__(1024) void k_vocab_coef(const float2 *__restrict__ 
     if constexpr (SCALED) {
         float m = 0.0f;
         for (int64_t i = threadIdx.x; i < M; i += 1024) {
-            const float c = rows[i].y != INFINITY ? fabsf(tau * g[i]) : 0.0f;
+            const float c = rows[i].y != 0.0f ? fabsf(tau * g[i]) : 0.0f;
             m = fmaxf(m, c < INFINITY ? c : 0.0f);
         }
 #pragma unroll
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(1024) void k_vocab_coef(const float2 *__restrict__ 
     } else if (fl_block() == 0 && threadIdx.x == 0) *unscale = 1.0f;
     const int64_t step = SCALED ? 1024 : (int64_t)gridDim.x * 1024;
     for (int64_t i = (SCALED ? 0 : (int64_t)blockIdx.x * 1024) + threadIdx.x; i < M; i += step)
-        coef[i] = rows[i].y != INFINITY ? tau * g[i] * scale : 0.0f;
+        coef[i] = rows[i].y != 0.0f ? tau * g[i] * scale : 0.0f;
 }
 
 // dz of a piece but for the listed columns: the product again, an exponential in
@@ -284,12 +284,13 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_grad(VocabArgs a) {
     Prod prod;
     prod.run(ta, tb, a.op.K, lds);
     const int64_t row = row0 + prod.wave_m() + (fl_lane() & 15), col = n0 + prod.wave_n();
-    float lse[Prod::MT], c[Prod::MT];
+    float top[Prod::MT], c[Prod::MT];  // c: times the sum's reciprocal
 #pragma unroll
     for (int i = 0; i < Prod::MT; ++i) {
         const int64_t m = row + i * 16 < a.op.M ? row + i * 16 : a.op.M - 1;
-        lse[i] = a.rows[m].x + a.rows[m].y;
-        c[i] = a.coef[m];
+        const float2 sum = a.rows[m];
+        top[i] = sum.x;
+        c[i] = a.coef[m] * sum.y;
     }
     each_u<T>(a, prod.acc, col, a.v0 + a.width, [&](int i, int j, const float (&u)[4]) {
         const int64_t n = col + j * 16 + (fl_lane() >> 4) * 4 - a.v0;
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_grad(VocabArgs a) {
         Vec<T, 4> o, rest;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float d = c[i] == 0.0f ? 0.0f : c[i] * exp2_of(u[e] - lse[i]);
+            const float d = c[i] == 0.0f ? 0.0f : c[i] * exp2_of(u[e] - top[i]);
             o.v[e] = (T)d;
             rest.v[e] = (T)(d - (float)o.v[e]);
         }
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
     const float c = a.coef[row];
     if (v < 0 || v >= a.width || c == 0.0f) return;
     const float2 l = a.listed[i];
-    const float d = c * (exp2_of((l.x - a.rows[row].x) - a.rows[row].y) - l.y);
+    const float d = c * (exp2_of(l.x - a.rows[row].x) * a.rows[row].y - l.y);
     if constexpr (WIDE && sizeof(T) == 4) {
         _Float16 *to = (_Float16 *)a.d + dz_at<true>(a, row, v);
         to[0] = (_Float16)d;
@@ -803,7 +804,8 @@ __device__ __forceinline__ void lane_bias(const VocabArgs &a, int64_t n, float (
 // The rows' running maxima and sums over a part of the vocabulary's tiles: a lane
 // keeps those of its own columns in LDS over all tiles, and they are joined at the
 // end.  An exponent is one multiply-add from the product; the maximum is the
-// lane's first until a sum passes 2^64, so that it is not looked for in every tile.
+// lane's first until a sum passes 2^20, so that it is not looked for in every tile
+// (and an exponent that counts is rounded by no more than 2^-20).
 // bf16 [8192 x 512 -> 41000] 339 us = 1014 TFLOP/s, fp16 [4096 x 1024 -> 123000]
 // 945 us = 1092 (a large library product 1313 and 1451 on the same card), fp32
 // [1536 x 2048 -> 1645] 46 us = 225 (153), in 156 tiles on 256 CUs; [512 x 128 ->
@@ -846,8 +848,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
                     const float t = a.op.bias ? b[e] - less : -less;
                     return e < have ? __builtin_fmaf(v, scale, t) : -INFINITY;
                 };
-                // what the lane had first serves as the maximum, until a sum passes 2^64 (joined with others of up to that it
-                // stays finite) or is not a number
+                // what the lane had first serves as the maximum, until a sum passes 2^20 or is not a number
                 if (__any(have < 16)) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s += exp2_of(u(e, r.m));
@@ -859,7 +860,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
                     }
                 }
                 s += r.s;
-                if (r.m == -INFINITY || !(s < 0x1p64f)) {  // a lane's own: rows do not touch each other's bits
+                if (r.m == -INFINITY || !(s < 0x1p20f)) {  // a lane's own: rows do not touch each other's bits
                     float m = r.m;
                     s = 0.0f;
 #pragma unroll
@@ -894,7 +895,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
     row_and_part(a, &mt, &part);
     const int64_t row0 = (int64_t)mt * BM, end = a.v0 + a.width;
     const int64_t t0 = part_begin(a.n_tiles, part, a.parts), t1 = part_begin(a.n_tiles, part + 1, a.parts);
-    // (lse, coefficient, the row's only id or -1, its dz) of the tile's rows
+    // (maximum, coefficient over the sum, the row's only id or -1, its dz) of the tile's rows
     float4 *of = reinterpret_cast<float4 *>(wide_lds + STAGES * Run::ELEMS);
     for (int t = threadIdx.x; t < BM; t += WD_NT) {
         const int64_t m = row0 + t < a.op.M ? row0 + t : a.op.M - 1;
@@ -905,9 +906,9 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
             const int64_t v = a.op.lists.ids[m];
             const float2 l = a.listed[m];
             if (v >= a.v0 && v < end) id = __int_as_float((int)(v - a.v0));
-            d = c * (exp2_of((l.x - sum.x) - sum.y) - l.y);
+            d = c * (exp2_of(l.x - sum.x) * sum.y - l.y);
         }
-        of[t] = float4{sum.x + sum.y, c, id, d};
+        of[t] = float4{sum.x, c * sum.y, id, d};
     }
     __syncthreads();
     Tiles tiles;

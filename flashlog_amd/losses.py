@@ -168,7 +168,8 @@ def linear_cross_entropy(x, weight, target, bias=None):
     the bias's: float32's is held as exactly, 16-bit ones' as half (of up to 64
     rows of half with what its rounding leaves).
     Softmax terms are off by 2^-23 of themselves times 1 + their logit's
-    distance from the largest; a bias whose quotient by the temperature
+    distance from the largest (at least 16 over large vocabularies), whatever
+    all logits have in common; a bias whose quotient by the temperature
     overflows float32 counts as infinite."""
     _need_gpu("linear_cross_entropy", x, weight, target, bias)
     lead = _vocab_operands("linear_cross_entropy", x, weight, bias)

@@ -45,3 +45,23 @@ def test_no_ids_over_a_large_vocabulary(M, K, V, t):
     with torch.no_grad():
         loss = _losses().linear_distillation(x.cuda(), w.cuda(), ids.cuda(), teacher.cuda())
     assert (loss == 0).all()
+
+
+#: By the plain tiles and by the wide ones (float32 in training from 129 rows on, bfloat16 always).
+ROWS = [(9, 40, 90), (60, 64, 500), (300, 128, 4000), (136, 256, 4100)]
+
+
+@pytest.mark.parametrize("M,K,V", ROWS)
+@pytest.mark.parametrize("offset", [0.0, 100.0, -4000.0, 4000.0])
+def test_shares_add_up_beside_a_common_offset(M, K, V, offset):
+    """sum(p) - 1 of every row, as the sum of the bias's gradient.  A share is off by 8 e (1 + its distance from the
+    largest) in the backward and once more in the forward's sum, of terms that are added by lanes (V / 16 at most one
+    after the other), waves and parts (64 steps); the column sums have M terms."""
+    x, w, b, ids, _, g = _make(M, K, V, torch.float32, 7)
+    b = b + offset  # rounded: the reference takes what is left
+    ref_z = x.double() @ w.double().T + b.double()
+    p = torch.softmax(ref_z, 1)
+    off = (p * 16 * E * (1 + ref_z.amax(1, keepdim=True) - ref_z)).sum(1) + (V / 16 + 64) * E
+    out = _run(x, w, b, ids, None, g)
+    bound = (g * off).sum() + (M + 16) * E * 2 * g.sum()
+    assert out["db"].double().sum().abs().item() <= bound.item()
