@@ -408,15 +408,22 @@ __device__ __forceinline__ int made_here(int v) {
     return v;
 }
 
+// fp32 values as three bfloat16 planes (chunk_planes): a row holds 32 values of the
+// first, the same 32 of the second and of the third, and so on.
+__device__ __forceinline__ int64_t plane_at(int64_t c) { return c / 32 * 96 + c % 32; }
+
 // The same for rows of whole steps, from a base that all lanes have and with
-// 32-bit offsets (half the registers): rows of less than 2^23 values.
-template <int BR>
+// 32-bit offsets (half the registers): rows of less than 2^23 values.  P: planes of
+// a value; a step is 64 k of one, 32 of three.  A plane's part of a step lies in LDS
+// as a tile of its own.
+template <int BR, int P>
 struct StepsContig {
-    using At = WideContig<BR, 64>;
-    static constexpr int LOADS = At::LOADS, ELEMS = At::ELEMS;
+    static constexpr int BK = P == 1 ? 64 : 32;
+    using At = WideContig<BR, BK>;
+    static constexpr int LOADS = P * At::LOADS, ELEMS = P * At::ELEMS;
     static constexpr bool BLOCKING = false;
-    const uint16_t *base;  // of the next step
-    uint32_t at[LOADS];    // bytes
+    const uint16_t *base;      // of the next step
+    uint32_t at[At::LOADS];    // bytes
 
     // Row r of the tile is row row_at(r) from b on.
     template <typename F>
@@ -424,31 +431,28 @@ struct StepsContig {
         const int lane = made_here(fl_lane());
         base = b;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int r = (fl_wave_id() * LOADS + i) * 8 + lane / 8;
-            at[i] = (uint32_t)row_at(r) * (uint32_t)(ld * 2) + lds_at<64>(r, lane % 8) % 64 * 2;
+        for (int i = 0; i < At::LOADS; ++i) {
+            const int r = (fl_wave_id() * At::LOADS + i) * At::RPL + lane / At::CPR;
+            at[i] = (uint32_t)row_at(r) * (uint32_t)(ld * 2) + lds_at<BK>(r, lane % At::CPR) % BK * 2;
         }
     }
     __device__ __forceinline__ void issue(uint16_t *lds, int i) {
-        load_lds((const char *)base + at[i], lds + (fl_wave_id() * LOADS + i) * 512);
+        const int p = i / At::LOADS, j = i % At::LOADS;
+        load_lds((const char *)base + p * (BK * 2) + at[j], lds + p * At::ELEMS + (fl_wave_id() * At::LOADS + j) * 512);
     }
-    __device__ __forceinline__ void next() { base += 64; }
-    // The operands of N 16-row tiles from row0 on, of the step's first or second 32 values.
+    __device__ __forceinline__ void next() { base += P * BK; }
+    // The operands of N 16-row tiles from row0 on: the step's first or second 32
+    // values, or those of a plane.
     template <int KS, int N>
     __device__ __forceinline__ void read(const uint16_t *lds, int row0, u32x4 (&f)[N]) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+        for (int i = 0; i < N; ++i) {
+            const int r = row0 + i * 16 + (fl_lane() & 15), c = fl_lane() >> 4;
             f[i] = *reinterpret_cast<const u32x4 *>(
-                lds + lds_at<64>(row0 + i * 16 + (fl_lane() & 15), KS * 4 + (fl_lane() >> 4)));
+                lds + (P == 1 ? lds_at<BK>(r, KS * 4 + c) : KS * At::ELEMS + lds_at<BK>(r, c)));
+        }
     }
 };
-
-// fp32 values as two fp16 planes, v s = v0 + v1 with a power of two s that brings
-// the largest to 2^13..2^14: v1 is the rest rounded, so that what is lost is below
-// 2^-22 of v or 2^-38 of the largest.  A row holds 32 values of the one plane, the
-// same 32 of the other, and so on: 64 values of a row are a step of 32 k, and the
-// three products v0 w0 + v0 w1 + v1 w0 are off by 2^-22 once more.
-__device__ __forceinline__ int64_t pair_at(int64_t c) { return c / 32 * 64 + c % 32; }
 
 // k-strided: the rows of k one after the other, or in an order if GATHER.
 template <int BR, int BK, bool GATHER>
@@ -539,16 +543,17 @@ struct WideStrided {
 };
 
 // The same, k rows one after the other, without guards: rows behind the last one
-// read it again, so that the other operand has to be 0 there.  PAIRS: of values
-// held as two planes, 32 rows of the one and then the same rows of the other.
-template <int BR, bool PAIRS>
+// read it again, so that the other operand has to be 0 there.  P: planes of a value,
+// each of which lies in LDS as a tile of its own.
+template <int BR, int P>
 struct StepsStrided {
-    using At = WideStrided<BR, 64, false>;
-    static constexpr int LOADS = At::LOADS, ELEMS = At::ELEMS, STEP = PAIRS ? 32 : 64;
+    static constexpr int STEP = P == 1 ? 64 : 32;
+    using At = WideStrided<BR, STEP, false>;
+    static constexpr int LOADS = P * At::LOADS, ELEMS = P * At::ELEMS;
     static constexpr bool BLOCKING = true;
     const uint16_t *base;  // of the next step
     int64_t ld;
-    uint32_t at[LOADS];  // bytes
+    uint32_t at[At::LOADS];  // bytes
 
     // From column 0 of b on, R columns; `rows`: of k that there are, STEP at most.
     __device__ __forceinline__ void init(const uint16_t *b, int64_t stride, int64_t R, int rows) {
@@ -557,19 +562,20 @@ struct StepsStrided {
         ld = stride;
         const int most = R - 8 < BR ? (int)R - 8 : BR;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int r = (fl_wave_id() * LOADS + i) * At::RPL + lane / At::CH, k = PAIRS ? r % 32 : r;
+        for (int i = 0; i < At::LOADS; ++i) {
+            const int r = (fl_wave_id() * At::LOADS + i) * At::RPL + lane / At::CH;
             const int c0 = ((lane % At::CH) ^ At::turn(r)) * 8, c = c0 < most ? c0 : most;
-            at[i] = (uint32_t)(PAIRS ? (int)pair_at(c) + r / 32 * 32 : c) * 2 +
-                    (uint32_t)(k < rows ? k : rows - 1) * (uint32_t)(stride * 2);
+            at[i] = (uint32_t)(P == 1 ? c : (int)plane_at(c)) * 2 +
+                    (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)(stride * 2);
         }
     }
     __device__ __forceinline__ void issue(uint16_t *lds, int i) {
-        load_lds((const char *)base + at[i], lds + (fl_wave_id() * LOADS + i) * 512);
+        const int p = i / At::LOADS, j = i % At::LOADS;
+        load_lds((const char *)base + p * 64 + at[j], lds + p * At::ELEMS + (fl_wave_id() * At::LOADS + j) * 512);
     }
     __device__ __forceinline__ void next() { base += STEP * ld; }
-    // Of N 16-column tiles from col0 on, of the step's first or second 32 rows.  In
-    // asm, with the wait, as WideStrided's.
+    // Of N 16-column tiles from col0 on: the step's first or second 32 rows, or those
+    // of a plane.  In asm, with the wait, as WideStrided's.
     template <int KS, int N>
     __device__ __forceinline__ void read(const uint16_t *lds, int col0, u32x4 (&f)[N]) const {
         static_assert(N == 2 || N % 4 == 0, "two or four tiles a block");
@@ -725,7 +731,7 @@ struct WideProduct {
 
 // Tiles one after the other as one sequence of steps, `steps` a tile: the loads
 // run ahead over the tiles' ends.  Tiles of BM rows and WN x 64 columns, a step of
-// 64 values (PAIRS: 32 of both planes).
+// 64 values (P = 3: 32 of three planes, six products).
 //
 // Operands are read from LDS beside the products of others: of small tiles those
 // of the next step; of 256 x 256 tiles, whose sums leave fewer registers, a step's
@@ -733,12 +739,12 @@ struct WideProduct {
 // A barrier a step says that it is read by all and the next one there.  Loads of a
 // later step are issued one at a time between the products.  (Read and multiplied
 // in turns, by half the waves each or by all together, the matrix unit was busy 46%
-// of the time, whatever the tile: 128 x 128, fp32 [1536 x 2048 -> 1645] 52 and 50 us.)
+// of the time, whatever the tile.)
 //
 // feed(i, lds_a, lds_b) issues load i of the next step, and after the last one
 // goes on to the step behind it; behind the last step it may load anything that
 // can be read.  out(tile) takes a tile's sums.
-template <typename T, bool PAIRS, int BM, int WN, int STAGES, typename TA, typename TB>
+template <typename T, int P, int BM, int WN, int STAGES, typename TA, typename TB>
 struct WideTiles {
     static constexpr int WM = WD_WAVES / WN, MT = BM / WM / 16, NTL = 4, BN = WN * 64;
     static constexpr int ELEMS = TA::ELEMS + TB::ELEMS, LOADS = TA::LOADS + TB::LOADS;
@@ -807,7 +813,7 @@ struct WideTiles {
         if constexpr (MT * NTL <= 16) {
             // a whole step's operands beside those that are multiplied; half the waves read first, half multiply first
             struct Operands {
-                u32x4 a[2][MT], b[2][NTL];
+                u32x4 a[P == 1 ? 2 : 3][MT], b[P == 1 ? 2 : 3][NTL];
             };
             const bool second = fl_wave_id() >= WD_WAVES / 2;
             const auto read = [&](Operands &o) {
@@ -815,6 +821,10 @@ struct WideTiles {
                 ta.template read<0>(la, wave_m(), o.a[0]);
                 tb.template read<1>(la + TA::ELEMS, wave_n(), o.b[1]);
                 ta.template read<1>(la, wave_m(), o.a[1]);
+                if constexpr (P == 3) {
+                    tb.template read<2>(la + TA::ELEMS, wave_n(), o.b[2]);
+                    ta.template read<2>(la, wave_m(), o.a[2]);
+                }
             };
             const auto step = [&](const Operands &now, Operands &next) {
                 Waits::template wait<LOADS *(STAGES - 2)>();
@@ -822,8 +832,11 @@ struct WideTiles {
                 go_on();
                 if (!second) read(next);
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (PAIRS) {
-                    multiply(now.a[0], now.b[1], load_between);
+                if constexpr (P == 3) {  // smallest products first
+                    multiply(now.a[0], now.b[2], load_between);
+                    multiply(now.a[1], now.b[1], none);
+                    multiply(now.a[2], now.b[0], none);
+                    multiply(now.a[0], now.b[1], none);
                     multiply(now.a[1], now.b[0], none);
                     multiply(now.a[0], now.b[0], none);
                 } else {
@@ -843,7 +856,7 @@ struct WideTiles {
                 if (s + 2 >= all) break;
             }
         } else {
-            static_assert(!PAIRS, "two planes of such tiles have no registers");
+            static_assert(P == 1, "three planes of such tiles have no registers");
             // operands whose reads are waited for at once: half the waves read first, half multiply first
             const bool later = TA::BLOCKING && TB::BLOCKING && fl_wave_id() >= WD_WAVES / 2;
             u32x4 a0[MT], b0[NTL], a1[MT], b1[NTL];

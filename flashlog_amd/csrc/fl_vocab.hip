@@ -6,7 +6,7 @@
 //   dx = dz W      dW = dz^T x      db = sum over the rows of dz
 //
 // The piece of dz is what a call holds of [rows x vocabulary], in 16 bits (an
-// operand of two products; fp32: two planes).  The listed columns' own u comes
+// operand of two products; fp32: as it is or in three bfloat16 planes).  The listed columns' own u comes
 // from a dot product each; their entries of dz are made apart, since p - q of
 // values rounded before would keep few bits where p is near 1.
 //
@@ -14,9 +14,8 @@
 // would need three, beside 2 or 4 bytes of dz a logit written once and read twice.
 // Small products go by k_vocab_*, the others, and bfloat16 in training, by k_wide_*:
 // tiles one after the other, so that the loads of a tile begin while the one
-// before it is finished.  There fp32 operands are held as two fp16 planes (half the
-// products of three bfloat16 planes), and 16-bit rows that do not lie on 16 bytes
-// as copies that do.
+// before it is finished.  There fp32 operands are laid out as their three bfloat16
+// planes, and 16-bit rows that do not lie on 16 bytes as copies that do.
 #include "fl_abi.h"
 #include "fl_common.h"
 #include "fl_loss.h"
@@ -142,12 +141,20 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_rows(VocabArgs a, ListArgs l) {
     });
 }
 
-// Where the wide kernels' dz of row m and column c (of the piece) is; PAIRS: its
-// first plane's, the second is 32 values behind it.
-template <bool PAIRS>
+// Planes of a value in the wide kernels' operands, what they are, and dz's.
+template <typename T>
+constexpr int planes_of() {
+    return sizeof(T) == 4 ? 3 : 1;
+}
+template <typename T>
+using WideDz = typename std::conditional<sizeof(T) == 4, __bf16, _Float16>::type;
+
+// Where the wide kernels' dz of row m and column c (of the piece) is; of three
+// planes the first one's, the others are each 32 values behind the one before.
+template <int P>
 __device__ __forceinline__ int64_t dz_at(const VocabArgs &a, int64_t m, int64_t c) {
     const int in = (int)(c % D_BLOCK);
-    return c / D_BLOCK * a.d_block + m * a.ldd + (PAIRS ? pair_at(in) : in);
+    return c / D_BLOCK * a.d_block + m * a.ldd + (P == 1 ? in : plane_at(in));
 }
 
 // The logits of a lane's tiles in units of log 2, -inf behind the vocabulary:
@@ -319,10 +326,13 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
     const float2 l = a.listed[i];
     const float d = c * (exp2_of(l.x - a.rows[row].x) * a.rows[row].y - l.y);
     if constexpr (WIDE && sizeof(T) == 4) {
-        _Float16 *to = (_Float16 *)a.d + dz_at<true>(a, row, v);
-        to[0] = (_Float16)d;
-        to[32] = (_Float16)(d - (float)to[0]);
-    } else if constexpr (WIDE) ((_Float16 *)a.d)[dz_at<false>(a, row, v)] = (_Float16)d;
+        const float chunk[8] = {d, 0, 0, 0, 0, 0, 0, 0};
+        u32x4 plane[3];
+        chunk_planes<float>(chunk, plane);
+        uint16_t *to = (uint16_t *)a.d + dz_at<3>(a, row, v);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) to[p * 32] = (uint16_t)plane[p][0];
+    } else if constexpr (WIDE) ((_Float16 *)a.d)[dz_at<1>(a, row, v)] = (_Float16)d;
     else {
         const T o = (T)d;
         ((T *)a.d)[row * a.ldd + v] = o;
@@ -514,7 +524,7 @@ __global__ __launch_bounds__(LS_NT) void k_few_dw(VocabArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int64_t m = s * 32 + q * 8 + i < M ? s * 32 + q * 8 + i : M - 1;
-                next[s][i] = ((const H *)a.d)[WIDE ? dz_at<false>(a, m, v) : m * a.ldd + v];
+                next[s][i] = ((const H *)a.d)[WIDE ? dz_at<1>(a, m, v) : m * a.ldd + v];
             }
     };
     const float f = *a.unscale, f2 = a.undo ? a.undo[0] : 1.0f;
@@ -593,12 +603,6 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
 // ---------------------------------------------------------------------------
 // The same for large products
 
-// Whether the operands are two planes.
-template <typename T>
-constexpr bool is_pairs() {
-    return sizeof(T) == 4;
-}
-
 // The largest finite magnitude of x and of weight, a part of them a workgroup.
 // HBM-bound: 1.18 GB of bfloat16 in 263 us = 4.5 TB/s.  Rows of x in which nothing
 // is listed do not count and are laid out as zeros (padded rows may hold anything),
@@ -663,8 +667,8 @@ __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restric
         most[blockIdx.y * LAY_PARTS + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
 }
 
-// x and weight as rows of half values on 16 bytes: fp32 as two planes (pair_at),
-// bfloat16 times a power of two that brings the largest to 2^13..2^14 (what is
+// x and weight as rows on 16 bytes: fp32 as its planes (plane_at), bfloat16 as half,
+// times a power of two that brings the largest to 2^13..2^14 (what is
 // above 2^-31 of it is held exactly, and what is lost below 2^-38), half, and
 // bfloat16 that no backward follows, as they are; zeros behind a row.  (dz, in
 // half, is then rounded by 2^-11 of itself; by 2^-8 in bfloat16 it made the
@@ -674,7 +678,6 @@ template <typename T, bool SCALED>
 __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restrict__ most,
                                                const uint8_t *__restrict__ live, uint16_t *__restrict__ x,
                                                uint16_t *__restrict__ w, float *__restrict__ undo) {
-    constexpr bool PAIRS = is_pairs<T>();
     const bool second = blockIdx.y;
     const int64_t R = second ? a.op.V : a.op.M, ld = second ? a.op.ldw : a.op.ldx, chunks = a.cols / 8, K = a.op.K;
     const T *p = (const T *)(second ? a.op.weight : a.op.x);
@@ -703,17 +706,12 @@ __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restr
         else
 #pragma unroll
             for (int e = 0; e < 8; ++e) v.v[e] = c + e < have ? p[r * ld + c + e] : (T)0.0f;
-        if constexpr (PAIRS) {
-            Vec<_Float16, 8> hi, lo;
+        if constexpr (sizeof(T) == 4) {
+            u32x4 plane[3];
+            chunk_planes<float>(v.v, plane);
+            uint16_t *q = out + r * 3 * a.cols + plane_at(c);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float s = v.v[e] * scale;
-                hi.v[e] = (_Float16)s;
-                lo.v[e] = (_Float16)(s - (float)hi.v[e]);
-            }
-            _Float16 *q = (_Float16 *)out + r * 2 * a.cols + pair_at(c);
-            store_vec<_Float16, 8>(q, hi);
-            store_vec<_Float16, 8>(q + 32, lo);
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(q + p * 32) = plane[p];
         } else if constexpr (SCALED) {
             Vec<_Float16, 8> o;
 #pragma unroll
@@ -728,9 +726,10 @@ __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restr
 // wave's 64).
 template <typename T, typename H, int BM, int WN, int STAGES>
 struct LogitTiles {
-    using TA = StepsContig<BM>;
-    using TB = StepsContig<WN * 64>;
-    using Run = WideTiles<H, is_pairs<T>(), BM, WN, STAGES, TA, TB>;
+    static constexpr int P = planes_of<T>();
+    using TA = StepsContig<BM, P>;
+    using TB = StepsContig<WN * 64, P>;
+    using Run = WideTiles<H, P, BM, WN, STAGES, TA, TB>;
     TA ta;
     TB tb;
     int steps, at;  // of a tile's row; of the next load
@@ -745,7 +744,7 @@ struct LogitTiles {
         tb.init(a.w + n0 * a.ldw, a.ldw, [&](int r) { return column(r) < most ? column(r) : most; });
     }
     __device__ __forceinline__ void init(const VocabArgs &a, int64_t row0, int64_t n0) {
-        steps = (int)(a.cols / (is_pairs<T>() ? 32 : 64));
+        steps = (int)(a.cols / TA::BK);
         at = 0;
         n_next = n0;
         const int most = (int)(a.op.M - 1 - row0 < BM ? a.op.M - 1 - row0 : BM);
@@ -760,7 +759,7 @@ struct LogitTiles {
         tb.next();
         if (++at < steps) return;
         at = 0;
-        ta.base -= steps * 64;
+        ta.base -= steps * (P * TA::BK);
         n_next += WN * 64;
         aim(a);
     }
@@ -808,8 +807,9 @@ __device__ __forceinline__ void lane_bias(const VocabArgs &a, int64_t n, float (
 // (and an exponent that counts is rounded by no more than 2^-20).
 // bf16 [8192 x 512 -> 41000] 339 us = 1014 TFLOP/s, fp16 [4096 x 1024 -> 123000]
 // 945 us = 1092 (a large library product 1313 and 1451 on the same card), fp32
-// [1536 x 2048 -> 1645] 46 us = 225 (153), in 156 tiles on 256 CUs; [512 x 128 ->
-// 4.6M] bf16 961 us = 627: of two steps a tile, the exponentials are half.
+// [1536 x 2048 -> 1645] 81 us = 128 (153), six products each in 156 tiles on 256
+// CUs; [512 x 128 -> 4.6M] bf16 961 us = 627: of two steps a tile, the exponentials
+// are half.
 template <typename T, typename H, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
     using Tiles = LogitTiles<T, H, BM, WN, STAGES>;
@@ -883,11 +883,11 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
 }
 
 // dz of a piece but for the listed columns (a row's only one is made in its tile).
-// 436, 1073 and 48 us where k_wide_stats takes 339, 945 and 46: what dz's stores
+// 436, 1073 and 83 us where k_wide_stats takes 339, 945 and 81: what dz's stores
 // add, 672 MB of them in the first.
 template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
-    using Tiles = LogitTiles<T, _Float16, BM, WN, STAGES>;
+    using Tiles = LogitTiles<T, WideDz<T>, BM, WN, STAGES>;
     using Run = typename Tiles::Run;
     constexpr int MT = Run::MT;
     extern __shared__ __align__(16) uint16_t wide_lds[];
@@ -946,15 +946,20 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (c + h * 8 >= a.d_cols) continue;
-                    Vec<_Float16, 8> o;
+                    uint16_t *to = (uint16_t *)a.d + dz_at<planes_of<T>()>(a, row0 + r, c + h * 8);
+                    if constexpr (sizeof(T) == 4) {
+                        float one[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) o.v[e] = (_Float16)u[h * 8 + e];
-                    _Float16 *to = (_Float16 *)a.d + dz_at<is_pairs<T>()>(a, row0 + r, c + h * 8);
-                    store_vec<_Float16, 8>(to, o);
-                    if constexpr (is_pairs<T>()) {
+                        for (int e = 0; e < 8; ++e) one[e] = u[h * 8 + e];
+                        u32x4 plane[3];
+                        chunk_planes<float>(one, plane);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) o.v[e] = (_Float16)(u[h * 8 + e] - (float)o.v[e]);
-                        store_vec<_Float16, 8>(to + 32, o);
+                        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(to + p * 32) = plane[p];
+                    } else {
+                        Vec<_Float16, 8> o;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o.v[e] = (_Float16)u[h * 8 + e];
+                        store_vec<_Float16, 8>((_Float16 *)to, o);
                     }
                 }
             }
@@ -962,12 +967,13 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
 }
 
 // Column sums of a part of the rows of dz: 512 columns a workgroup, eight a lane,
-// a quarter of the rows a wave.  HBM-bound: 10 MB in 5.4 us, from the caches.
+// a quarter of the rows a wave.  HBM-bound: 15 MB in 5.8 us, from the caches.
 constexpr int COLS_WIDE = 8 * FL_WAVE;
 
-template <bool PAIRS>
+template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_wide_cols(VocabArgs a) {
-    constexpr int AHEAD = 4;
+    constexpr int P = planes_of<T>(), AHEAD = P == 1 ? 4 : 2;
+    using D = WideDz<T>;
     __shared__ float sums[LS_WAVES][COLS_WIDE];
     const int64_t blocks = (a.width + COLS_WIDE - 1) / COLS_WIDE, item = fl_block(), part = item / blocks;
     if (part >= a.parts) return;
@@ -977,19 +983,24 @@ __global__ __launch_bounds__(LS_NT) void k_wide_cols(VocabArgs a) {
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (c < a.d_cols)
         for (int64_t m = begin; m < end; m += AHEAD) {
-            Vec<_Float16, 8> v[AHEAD], w[AHEAD];
+            Vec<D, 8> v[AHEAD][P];
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const int64_t r = m + j < end ? m + j : end - 1;
-                const _Float16 *d = (const _Float16 *)a.d + dz_at<PAIRS>(a, r, c);
-                v[j] = load_vec<_Float16, 8>(d);
-                if (PAIRS) w[j] = load_vec<_Float16, 8>(d + 32);
+                const D *d = (const D *)a.d + dz_at<P>(a, r, c);
+#pragma unroll
+                for (int p = 0; p < P; ++p) v[j][p] = load_vec<D, 8>(d + p * 32);
             }
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 if (m + j >= end) break;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s[e] += PAIRS ? (float)v[j].v[e] + (float)w[j].v[e] : (float)v[j].v[e];
+                for (int e = 0; e < 8; ++e) {
+                    float t = (float)v[j][P - 1].v[e];
+#pragma unroll
+                    for (int p = P - 2; p >= 0; --p) t += (float)v[j][p].v[e];
+                    s[e] += t;
+                }
             }
         }
 #pragma unroll
@@ -1005,11 +1016,11 @@ __global__ __launch_bounds__(LS_NT) void k_wide_cols(VocabArgs a) {
 // from LDS.
 template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
-    constexpr bool PAIRS = is_pairs<T>();
-    constexpr int STEP = PAIRS ? 32 : 64;
-    using TA = StepsContig<BM>;
-    using TB = StepsStrided<WN * 64, PAIRS>;
-    using Run = WideTiles<_Float16, PAIRS, BM, WN, STAGES, TA, TB>;
+    constexpr int P = planes_of<T>();
+    using TA = StepsContig<BM, P>;
+    using TB = StepsStrided<WN * 64, P>;
+    using Run = WideTiles<WideDz<T>, P, BM, WN, STAGES, TA, TB>;
+    constexpr int STEP = TB::STEP;
     extern __shared__ __align__(16) uint16_t wide_lds[];
     const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x), tiles = a.m_tiles * a.n_tiles;
     const uint32_t part = (uint32_t)__builtin_amdgcn_readfirstlane((int)(w / tiles)), tile = w - part * tiles;
@@ -1021,11 +1032,11 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
     TB tb;
     const int most = (int)(M - 1 - row0 < BM ? M - 1 - row0 : BM);
     constexpr int IN_BLOCK = D_BLOCK / STEP;  // steps
-    ta.init((const uint16_t *)a.d + s0 / IN_BLOCK * a.d_block + row0 * a.ldd + s0 % IN_BLOCK * 64, a.ldd,
+    ta.init((const uint16_t *)a.d + s0 / IN_BLOCK * a.d_block + row0 * a.ldd + s0 % IN_BLOCK * (P * STEP), a.ldd,
             [&](int r) { return r < most ? r : most; });
     const auto aim = [&](int64_t step) {  // dz is 0 behind the piece
         const int64_t v = step * STEP, left = a.width - v;
-        tb.init(a.w + (a.v0 + v) * a.ldw + (PAIRS ? 2 * n0 : n0), a.ldw, a.cols - n0, left < STEP ? (int)left : STEP);
+        tb.init(a.w + (a.v0 + v) * a.ldw + P * n0, a.ldw, a.cols - n0, left < STEP ? (int)left : STEP);
     };
     int64_t next = s0;
     aim(next);
@@ -1083,11 +1094,11 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
 // us = 735 TFLOP/s and 1163 us = 887 in its cases.
 template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
-    constexpr bool PAIRS = is_pairs<T>();
-    constexpr int STEP = PAIRS ? 32 : 64;
-    using TA = StepsStrided<BM, PAIRS>;
-    using TB = StepsStrided<WN * 64, PAIRS>;
-    using Run = WideTiles<_Float16, PAIRS, BM, WN, STAGES, TA, TB>;
+    constexpr int P = planes_of<T>();
+    using TA = StepsStrided<BM, P>;
+    using TB = StepsStrided<WN * 64, P>;
+    using Run = WideTiles<WideDz<T>, P, BM, WN, STAGES, TA, TB>;
+    constexpr int STEP = TB::STEP;
     extern __shared__ __align__(16) uint16_t wide_lds[];
     const uint32_t w = (uint32_t)fl_xcd_contig(blockIdx.x, gridDim.x);
     const uint32_t walks = (uint32_t)__builtin_amdgcn_readfirstlane((int)(gridDim.x / a.parts));
@@ -1104,9 +1115,9 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
     const auto aim = [&](int64_t step) {  // dz is 0 in the rows behind the last
         const int64_t k = step * STEP, left = a.op.M - k;
         const int in = (int)(m0 % D_BLOCK);
-        ta.init((const uint16_t *)a.d + m0 / D_BLOCK * a.d_block + k * a.ldd + (PAIRS ? 2 * in : in), a.ldd, D_BLOCK - in,
+        ta.init((const uint16_t *)a.d + m0 / D_BLOCK * a.d_block + k * a.ldd + P * in, a.ldd, D_BLOCK - in,
                 STEP);
-        tb.init(a.x + k * a.ldx + (PAIRS ? 2 * c0 : c0), a.ldx, a.cols - c0, left < STEP ? (int)left : STEP);
+        tb.init(a.x + k * a.ldx + P * c0, a.ldx, a.cols - c0, left < STEP ? (int)left : STEP);
     };
     const auto aim_tile = [&]() {
         const int64_t mt = fl_uniform_i64(next / a.n_tiles);
@@ -1169,7 +1180,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
 
 // How the products of a vocabulary are cut.
 struct VocabPlan {
-    bool wide, pairs, lay, scaled;     // wide kernels; two planes; operands laid out, times powers of two
+    bool wide, lay, scaled;            // wide kernels; operands laid out, times powers of two
     bool small;                        // tiles of 128
     int bm, bn;                        // tiles of the logits
     uint32_t m_tiles, n_tiles, parts;  // parts: of the vocabulary, in the forward
@@ -1181,31 +1192,35 @@ struct VocabPlan {
 
 VocabPlan vocab_plan(const fl_vocab *op) {
     VocabPlan p{};
-    p.pairs = op->dtype == FL_F32;
-    p.size = p.pairs ? 4 : 2;
-    const int64_t step = p.pairs ? 32 : 64;  // inputs of a step of the wide kernels
-    p.scaled = op->dtype == FL_F32 || (op->dtype == FL_BF16 && op->train);
-    p.lay = p.scaled || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % step ||
+    const bool f32 = op->dtype == FL_F32;
+    const int64_t step = f32 ? 32 : 64, planes = f32 ? 3 : 1;  // inputs of a step of the wide kernels
+    p.scaled = op->dtype == FL_BF16 && op->train;
+    p.lay = f32 || p.scaled || !aligned(op->x, op->ldx) || !aligned(op->weight, op->ldw) || op->K % step ||
             op->ldx >= 1 << 23 || op->ldw >= 1 << 23;  // 32-bit offsets of 256 rows
-    // Laying the weight out takes up to four passes over it, which few rows do not pay for: in units of 1e-12 s a value of
-    // it, fp32 3.5 and then 2 rows / 360 a product, against 2 rows / 150 (0.9 at least) from where it lies; 16-bit values
-    // 0.9 to 1.3 and 2 rows / 1000, against 2 rows / 430 (0.45 at least).  With the four products of training fp32 has
-    // [116 x 1176 -> 454586] in 4340 us laid out and 5220 as it is, [66 x 512 -> 200000] in 850 both ways, weights that
-    // the last level cache holds ([128 x 256 -> 41000]) in 170 and 167, but [143 x 512 -> 200000], past a tile of 128, in
-    // 1040 and 1360.  bfloat16 in training is laid out whatever it costs and at every size, so that dz is half.
+    // Laying the weight out takes a pass over it or two, which few rows do not pay for.  fp32 (us laid out and as it is):
+    // in training [1536 x 2048 -> 1645] 317 and 450, [4096 x 512 -> 4000] 414 and 463, [600 x 256 -> 41000] 414 and 468, but
+    // [200 x 256 -> 41000] 214 and 216, [300 x 64 -> 41000] 161 and 133, [143 x 512 -> 200000] 1411 and 1304; in evaluation
+    // 91 and 148, 99 and 102, 100 and 101, but [200 x 512 -> 8000] 45 and 26.  16-bit values, in units of 1e-12 s a value of
+    // the weight: 0.9 to 1.3 and 2 rows / 1000 a product, against 2 rows / 430 (0.45 at least) from where it lies.  bfloat16
+    // in training is laid out whatever it costs and at every size, so that dz is half.
     int64_t least = 65;
-    if (op->dtype == FL_F32) least = !op->train ? 448 : (double)op->V * op->K >= 1 << 26 ? 65 : 129;
-    else if (op->dtype == FL_BF16 && op->train) least = 1;
-    else if (p.lay) least = op->train ? 128 : 384;
-    p.wide = op->K >= 1 && op->K <= 1 << 20 && op->M >= least &&
-             (least == 1 || (double)op->M * op->V * op->K >= 1 << 27);
+    double work = 1 << 27;
+    if (f32) {
+        least = op->train ? 256 : 512;
+        work = op->train ? 1 << 30 : 1ll << 31;
+    } else if (op->dtype == FL_BF16 && op->train) {
+        least = 1;
+        work = 0;
+    } else if (p.lay) least = op->train ? 128 : 384;
+    p.wide = op->K >= 1 && op->K <= 1 << 20 && op->M >= least && (double)op->M * op->V * op->K >= work;
     p.lay = p.lay && p.wide;
     p.scaled = p.scaled && p.wide;
+    p.size = !f32 ? 2 : p.wide ? 6 : 4;
     if (p.wide) {
         p.cols = ceil_div(op->K, step) * step;
-        p.small = op->M <= 128 || ceil_div(op->M, 256) * ceil_div(op->V, 256) < 192;
+        p.small = f32 || op->M <= 128 || ceil_div(op->M, 256) * ceil_div(op->V, 256) < 192;
         p.bm = p.small ? 128 : 256;
-        p.bn = p.small || p.pairs ? 128 : 256;  // two planes of 256 x 256 have no registers
+        p.bn = p.bm;  // three planes of 256 x 256 have no registers
     } else {
         // tiles by the steps that the fullest CU takes: a step of 128 x 128 takes 2.3 us alone and 1.45 more a tile beside
         // others, of 64 x 64 1.2 and 0.52, of 32 x 64 0.52 and 0.3 (fp32)
@@ -1232,7 +1247,7 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     p.piece = piece < op->V ? piece : op->V;
     p.d_cols = p.wide ? ceil_div(p.piece, D_BLOCK) * D_BLOCK : ceil_div(p.piece, 8) * 8;
     p.d_rows = p.wide ? ceil_div(op->M, step) * step : p.dz_rows;
-    p.ldd = !p.wide ? p.d_cols : p.pairs ? 2 * D_BLOCK : D_BLOCK;
+    p.ldd = !p.wide ? p.d_cols : planes * D_BLOCK;
     p.d_block = p.d_rows * p.ldd;
     return p;
 }
@@ -1271,7 +1286,7 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
     const bool f32 = op->dtype == FL_F32;
     s.coef = take((size_t)(op->M + 1) * 4);
     s.d = take((size_t)p.d_rows * p.d_cols * p.size);
-    const int narrow = op->K <= 128 || p.pairs ? 128 : 256;
+    const int narrow = op->K <= 128 ? 128 : 256;
     if (with_dx) {
         if (p.wide) {
             s.dx_tile = p.small || ceil_div(op->M, 256) * ceil_div(op->K, narrow) < 16 ? 128 : 256;
@@ -1329,7 +1344,7 @@ VocabArgs vocab_args(const fl_vocab *op, const VocabPlan &p, void *state, void *
         const VocabLayout l = vocab_layout(op, p);
         a.x = (const uint16_t *)((char *)layout + l.x);
         a.w = (const uint16_t *)((char *)layout + l.w);
-        a.ldx = a.ldw = p.pairs ? 2 * p.cols : p.cols;
+        a.ldx = a.ldw = op->dtype == FL_F32 ? 3 * p.cols : p.cols;
         if (p.scaled) a.undo = (const float *)((char *)layout + l.undo);
     } else {
         a.x = (const uint16_t *)op->x;
@@ -1340,11 +1355,19 @@ VocabArgs vocab_args(const fl_vocab *op, const VocabPlan &p, void *state, void *
     return a;
 }
 
-constexpr unsigned tiles_bytes(int bm, int bn, int stages) { return (unsigned)(stages * (bm + bn) * 64 * 2); }
+// Of tiles of 128 x 128, 256 x 128 and 256 x 256: stages, and bytes of LDS.
+template <typename T>
+constexpr int small_stages() {
+    return planes_of<T>() == 1 ? 4 : 3;
+}
+template <typename T>
+constexpr unsigned tiles_bytes(int bm, int bn, int stages) {
+    return (unsigned)(stages * (bm + bn) * (planes_of<T>() == 1 ? 64 : 96) * 2);
+}
 
 template <typename T>
 int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, void *layout, void *ws) {
-    constexpr int BK = sizeof(T) == 4 ? 32 : 64;
+    constexpr int BK = sizeof(T) == 4 ? 32 : 64, S = small_stages<T>();
     const VocabPlan p = vocab_plan(op);
     VocabArgs a = vocab_args(op, p, state, layout);
     a.m_tiles = p.m_tiles;
@@ -1360,16 +1383,15 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
         uint8_t *live = (uint8_t *)layout + l.live;
         const int64_t chunks = (op->M > op->V ? op->M : op->V) * (p.cols / 8), want = ceil_div(chunks, LS_NT);
         const dim3 lg((unsigned)(want < 4096 ? want : 4096), 2);
-        if constexpr (!std::is_same<T, _Float16>::value)
+        if constexpr (std::is_same<T, __bf16>::value)
             if (p.scaled) {
                 FL_LAUNCH("k_lay_max", k_lay_max<T>, dim3(LAY_PARTS, 2), dim3(LS_NT), 0, st, a, most, live);
                 FL_LAUNCH("k_lay", (k_lay<T, true>), lg, dim3(LS_NT), 0, st, a, most, live, (uint16_t *)a.x,
                           (uint16_t *)a.w, (float *)a.undo);
             }
-        if constexpr (sizeof(T) == 2)
-            if (!p.scaled)
-                FL_LAUNCH("k_lay", (k_lay<T, false>), lg, dim3(LS_NT), 0, st, a, most, live, (uint16_t *)a.x,
-                          (uint16_t *)a.w, (float *)nullptr);
+        if (!p.scaled)
+            FL_LAUNCH("k_lay", (k_lay<T, false>), lg, dim3(LS_NT), 0, st, a, most, live, (uint16_t *)a.x,
+                      (uint16_t *)a.w, (float *)nullptr);
     }
     const bool few = op->lists.k <= DOT_IDS && p.parts <= 4 * FL_WAVE;
     if (!few && op->lists.k)
@@ -1380,16 +1402,14 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
         const auto launch = [&](auto half) {
             using H = decltype(half);
             if (p.bm == 128)
-                FL_LAUNCH("k_wide_stats", (k_wide_stats<T, H, 128, 2, 4>), g, dim3(WD_NT), tiles_bytes(128, 128, 4) + extra(2), st, a);
-            else if constexpr (is_pairs<T>())
-                FL_LAUNCH("k_wide_stats", (k_wide_stats<T, H, 256, 2, 3>), g, dim3(WD_NT), tiles_bytes(256, 128, 3) + extra(4), st, a);
-            else
-                FL_LAUNCH("k_wide_stats", (k_wide_stats<T, H, 256, 4, 2>), g, dim3(WD_NT), tiles_bytes(256, 256, 2) + extra(8), st, a);
+                FL_LAUNCH("k_wide_stats", (k_wide_stats<T, H, 128, 2, S>), g, dim3(WD_NT), tiles_bytes<T>(128, 128, S) + extra(2), st, a);
+            else if constexpr (planes_of<T>() == 1)
+                FL_LAUNCH("k_wide_stats", (k_wide_stats<T, H, 256, 4, 2>), g, dim3(WD_NT), tiles_bytes<T>(256, 256, 2) + extra(8), st, a);
         };
         if constexpr (std::is_same<T, __bf16>::value) {
             if (p.scaled) launch(_Float16());
             else launch(T());
-        } else launch(_Float16());
+        } else launch(WideDz<T>());
     } else if (p.bm == 128)
         FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 128, 128, BK>), g, dim3(LN_NT), 0, st, a);
     else if (p.bm == 64) FL_LAUNCH("k_vocab_stats", (k_vocab_stats<T, 64, 64, BK>), g, dim3(LN_NT), 0, st, a);
@@ -1403,7 +1423,7 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
 template <typename T>
 int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *state, void *layout, void *dx, void *dw,
                    void *db, char *ws) {
-    constexpr int BK = sizeof(T) == 4 ? 32 : 64;
+    constexpr int BK = sizeof(T) == 4 ? 32 : 64, S = small_stages<T>();
     const VocabPlan p = vocab_plan(op);
     const VocabSpace s = vocab_space(op, p, dx, dw, db);
     VocabArgs a = vocab_args(op, p, state, layout);
@@ -1419,7 +1439,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
     const dim3 nt(LN_NT), wt(WD_NT);
     const auto fits = [&](int64_t grid) { return launch_fits(grid, WD_NT); };
     const auto fail = [&]() { return fl_fail(FL_ERR_ARG, "linear_loss: too many tiles for one launch (shape)"); };
-    if (std::is_same<T, _Float16>::value || p.wide)
+    if (std::is_same<T, _Float16>::value || (sizeof(T) == 2 && p.wide))
         FL_LAUNCH("k_vocab_coef", k_vocab_coef<true>, dim3(1), dim3(1024), 0, st, a.rows, grad, op->lists.temperature,
                   op->M, coef, coef + op->M);
     else
@@ -1439,11 +1459,9 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             const auto extra = [](int bm) { return (unsigned)(bm * sizeof(float4)); };
             const dim3 g((unsigned)grid);
             if (p.bm == 128)
-                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 128, 2, 4>), g, wt, tiles_bytes(128, 128, 4) + extra(128), st, a);
-            else if constexpr (is_pairs<T>())
-                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 256, 2, 3>), g, wt, tiles_bytes(256, 128, 3) + extra(256), st, a);
-            else
-                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 256, 4, 2>), g, wt, tiles_bytes(256, 256, 2) + extra(256), st, a);
+                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 128, 2, S>), g, wt, tiles_bytes<T>(128, 128, S) + extra(128), st, a);
+            else if constexpr (planes_of<T>() == 1)
+                FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 256, 4, 2>), g, wt, tiles_bytes<T>(256, 256, 2) + extra(256), st, a);
         } else if (p.bm == 128)
             FL_LAUNCH("k_vocab_grad", (k_vocab_grad<T, 128, 128, BK>), dim3((unsigned)grid), nt, 0, st, a);
         else if (p.bm == 64) FL_LAUNCH("k_vocab_grad", (k_vocab_grad<T, 64, 64, BK>), dim3((unsigned)grid), nt, 0, st, a);
@@ -1465,11 +1483,13 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             const dim3 g((unsigned)grid);
             if (p.wide) {
                 if (s.dx_tile == 128)
-                    FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 128, 2, 4>), g, wt, tiles_bytes(128, 128, 4), st, a);
-                else if (s.dx_cols == 128)
-                    FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 256, 2, 3>), g, wt, tiles_bytes(256, 128, 3), st, a);
-                else if constexpr (!is_pairs<T>())
-                    FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 256, 4, 2>), g, wt, tiles_bytes(256, 256, 2), st, a);
+                    FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 128, 2, S>), g, wt, tiles_bytes<T>(128, 128, S), st, a);
+                else if constexpr (planes_of<T>() == 1) {
+                    if (s.dx_cols == 128)
+                        FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 256, 2, 3>), g, wt, tiles_bytes<T>(256, 128, 3), st, a);
+                    else
+                        FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 256, 4, 2>), g, wt, tiles_bytes<T>(256, 256, 2), st, a);
+                }
             } else if (s.dx_tile == 128)
                 FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 128, 128, BK>), g, nt, 0, st, a);
             else FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 64, 64, BK>), g, nt, 0, st, a);
@@ -1506,11 +1526,13 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             const dim3 g((unsigned)grid);
             if (p.wide) {
                 if (rows == 128)
-                    FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 128, 2, 4>), g, wt, tiles_bytes(128, 128, 4), st, a);
-                else if (cols == 128)
-                    FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 256, 2, 3>), g, wt, tiles_bytes(256, 128, 3), st, a);
-                else if constexpr (!is_pairs<T>())
-                    FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 256, 4, 2>), g, wt, tiles_bytes(256, 256, 2), st, a);
+                    FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 128, 2, S>), g, wt, tiles_bytes<T>(128, 128, S), st, a);
+                else if constexpr (planes_of<T>() == 1) {
+                    if (cols == 128)
+                        FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 256, 2, 3>), g, wt, tiles_bytes<T>(256, 128, 3), st, a);
+                    else
+                        FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 256, 4, 2>), g, wt, tiles_bytes<T>(256, 256, 2), st, a);
+                }
             } else if (rows == 128)
                 FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 128, 128, BK>), g, nt, 0, st, a);
             else FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 64, 64, BK>), g, nt, 0, st, a);
@@ -1523,7 +1545,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             a.sums = (float *)(ws + s.db);
             const dim3 g = grid_of(ceil_div(a.width, FL_WAVE * 4));
             if (p.wide)
-                FL_LAUNCH("k_wide_cols", k_wide_cols<is_pairs<T>()>, grid_of(a.parts * ceil_div(a.width, COLS_WIDE)),
+                FL_LAUNCH("k_wide_cols", k_wide_cols<T>, grid_of(a.parts * ceil_div(a.width, COLS_WIDE)),
                           dim3(LS_NT), 0, st, a);
             else
                 FL_LAUNCH("k_vocab_cols", k_vocab_cols<T>, grid_of(a.parts * ceil_div(a.width, LS_NT)), dim3(LS_NT), 0,

@@ -161,12 +161,13 @@ def linear_cross_entropy(x, weight, target, bias=None):
     No logits are kept: the backward computes them again, a piece of the
     vocabulary at a time, in a workspace of up to 1 GB (of 256 columns
     where there are more rows than that holds).  Large products lay float32 operands out as
-    two half-precision planes, and bfloat16 ones in training as scaled half
-    (a copy of x's and weight's size, held for the backward): a value is off by
-    2^-22 of itself (bfloat16: by nothing) or by 2^-38 of the largest of its
-    tensor.  The logits' gradient is an operand of two products and a term of
-    the bias's: float32's is held as exactly, 16-bit ones' as half (of up to 64
-    rows of half with what its rounding leaves).
+    three bfloat16 planes (1.5 times their size; all of their 24 bits, at
+    float32's range), and bfloat16 ones in training as scaled half
+    (a copy of x and weight, held for the backward): bfloat16 values are off by
+    nothing or by 2^-38 of the largest of their tensor.  The logits' gradient is
+    an operand of two products and a term of the bias's: float32's is held as
+    such, 16-bit ones' as half (of up to 64 rows of half with what its rounding
+    leaves).
     Softmax terms are off by 2^-23 of themselves times 1 + their logit's
     distance from the largest (at least 16 over large vocabularies), whatever
     all logits have in common; a bias whose quotient by the temperature

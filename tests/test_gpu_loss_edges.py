@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from test_gpu_losses import _held, _rows, _tiny
+
 pytestmark = pytest.mark.gpu
 
 E = 2.0 ** -24
@@ -47,8 +49,9 @@ def test_no_ids_over_a_large_vocabulary(M, K, V, t):
     assert (loss == 0).all()
 
 
-#: By the plain tiles and by the wide ones (float32 in training from 129 rows on, bfloat16 always).
-ROWS = [(9, 40, 90), (60, 64, 500), (300, 128, 4000), (136, 256, 4100)]
+#: By the plain tiles and by the wide ones (float32 in training from 256 rows and 2^30 products of two values on,
+#: bfloat16 always).
+ROWS = [(9, 40, 90), (60, 64, 500), (300, 128, 4000), (136, 256, 4100), (300, 256, 14100)]
 
 
 @pytest.mark.parametrize("M,K,V", ROWS)
@@ -65,3 +68,66 @@ def test_shares_add_up_beside_a_common_offset(M, K, V, offset):
     out = _run(x, w, b, ids, None, g)
     bound = (g * off).sum() + (M + 16) * E * 2 * g.sum()
     assert out["db"].double().sum().abs().item() <= bound.item()
+
+
+def _reference(x, w, b, ids, g):
+    """{name: (value, bound)} of cross entropy in 64 bits.  As in test_gpu_losses, but that nothing is lost relative to
+    another row's or another column's values: what float32 holds is off by 2^-23 of itself; what 16-bit types hold of a
+    row's p - q by 2^-11 of itself or 2^-39, and of weight's gradient's other operand 2^-38 of its largest value."""
+    t, (M, K) = x.dtype, x.shape
+    x, w = x.double(), w.double()
+    z, mag = x @ w.T, x.abs() @ w.abs().T
+    if b is not None:
+        z, mag = z + b.double(), mag + b.double().abs()
+    loss, dloss, d, dd, c = _rows(z, (K + 16) * E * mag, ids, None, 1.0, g, t)
+    if t is torch.float32:
+        dd = dd + 2.0 ** -23 * d.abs() + _tiny(t)
+        lost = 0.0
+    else:
+        dd = dd + 2.0 ** -11 * d.abs() + 2.0 ** -39 * c.abs()
+        share = torch.where(c == 0, 0.0, d / torch.where(c == 0, 1.0, c)).abs()
+        lost = 2.0 ** -38 * 2 * (c.abs() * x.abs().amax(1, keepdim=True)).max() * share.sum(0)[:, None]
+    out = {"loss": (loss, dloss * 1.01 + 1e-30)}
+    for name, a, da, v, n in (("dx", d, dd, w, w.shape[0]), ("dw", d.T, dd.T, x, M)):
+        out[name] = (a @ v, da @ v.abs() + (n + 16) * E * (a.abs() @ v.abs()) + (lost if name == "dw" else 0.0))
+    if b is not None:
+        out["db"] = (d.sum(0), dd.sum(0) + (M + 16) * E * d.abs().sum(0))
+    for k in list(out)[1:]:
+        tt = b.dtype if k == "db" else t
+        out[k] = (out[k][0], (out[k][1] + torch.finfo(tt).eps / 2 * out[k][0].abs()) * 1.01 + _tiny(tt))
+    return out
+
+
+def _check(x, w, b, ids, g):
+    ref, out = _reference(x, w, b, ids, g), _run(x, w, b, ids, None, g)
+    for k, (value, bound) in ref.items():
+        _held(out[k], value, bound, k)
+
+
+
+@pytest.mark.parametrize("M,K,V", ROWS)
+@pytest.mark.parametrize("spread", [2.0, 6.0])
+def test_small_terms_in_float32(M, K, V, spread):
+    """Softmax terms down to 2^-60, in rows whose losses weigh 1 and 2^-30: every entry is a float32 one."""
+    x, w, b, ids, _, g = _make(M, K, V, torch.float32, 2, spread=spread)
+    _check(x, w, b, ids, torch.where(torch.arange(M) % 3 == 0, g, g * 2.0 ** -30))
+
+
+@pytest.mark.parametrize("M,K,V", ROWS)
+def test_large_rows_beside_others_in_float32(M, K, V):
+    """A row of x, then a row of the weight, 2^26 times the others' size."""
+    x, w, b, ids, _, g = _make(M, K, V, torch.float32, 3)
+    big = x.clone()
+    big[5] *= 2.0 ** 26
+    _check(big, w, b, ids, g)
+    far = w.clone()
+    far[7] *= 2.0 ** 26
+    _check(x, far, b, ids, g)
+
+
+@pytest.mark.parametrize("M,K,V", [(257, 520, 8100), (1100, 72, 14000), (256, 1030, 4150), (2000, 300, 1900)])
+def test_wide_products_in_float32(M, K, V):
+    """Several tiles in every direction, odd ends among them."""
+    x, w, b, ids, _, g = _make(M, K, V, torch.float32, 11)
+    ids[::7] = -1
+    _check(x, w, b, ids, g)
