@@ -45,14 +45,18 @@ struct VocabArgs {
     Running *part;        // [M][parts]
     const float2 *rows;
     float2 *listed;
-    const float *coef;    // tau g of every row (times a power of two), 0 where it has no gradient
+    const float *coef;    // tau g of every row, 0 where it has no gradient; over a power of two where dz is half:
+    const float *factor;  // that power, or null
     void *d;              // dz of the piece: [M][ldd], wide: blocks of D_BLOCK columns, [d_rows][ldd] each
     int64_t ldd, d_block;  // d_block: from one to the next
     int64_t dz_rows;      // rows of dz: M, or 2 M where the second M are what rounding left of the first
     float *sums;          // dx: [parts][dz_rows][K]; dW: [parts][width][K]
     void *dw;
     void *dx;             // where one part and one piece are all of it
-    const float *unscale;  // what undoes dz's power of two
+    // x as dW takes it, and the exponent of what undoes its power of two, or null
+    const void *y;
+    int64_t ldy;
+    const int *y_exp;
     int add;
     // wide kernels: operands laid out (or as they are), their columns and dz's with those that pad them to whole steps
     // (dz: 0 there, and in the rows that pad it), and what undoes the planes' powers of two (or null)
@@ -246,34 +250,109 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_stats(VocabArgs a) {
     store_running<BM, Prod::WAVES_N>(a, r, join, prod.wave_m(), prod.wave_n() / (BN / Prod::WAVES_N), row0, part);
 }
 
-// What a row's gradients are multiplied by (2 to 11 us, 8192 rows in one workgroup).  SCALED (half): times the power of
-// two that brings the largest to 2^14, so that small ones stay normal numbers.
-template <bool SCALED>
+// What a row's dz is multiplied by.
 __global__ __launch_bounds__(1024) void k_vocab_coef(const float2 *__restrict__ rows, const float *__restrict__ g,
-                                                     float tau, int64_t M, float *__restrict__ coef,
-                                                     float *__restrict__ unscale) {
-    __shared__ float most[16];
-    float scale = 1.0f;
-    if constexpr (SCALED) {
+                                                     float tau, int64_t M, float *__restrict__ coef) {
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < M; i += (int64_t)gridDim.x * 1024)
+        coef[i] = rows[i].y != 0.0f ? tau * g[i] : 0.0f;
+}
+
+// Where dz is half: a row's tau g as a number of 2^14..2^15, which its dz is multiplied
+// by, and a power of two, which its row of dx, its terms of db and its row of dW's
+// other operand are multiplied by.  So what half can hold is that of p - q, 2^-39
+// absolute, in every row, whatever the rows' gradients are to each other.  A wave a row;
+// most: the largest exponent of a workgroup's rows of x times that power.
+constexpr int LAY_PARTS = 1024;
+constexpr int NO_EXP = -(1 << 20);
+
+template <typename T>
+__global__ __launch_bounds__(LS_NT) void k_row_scale(VocabArgs a, const float *__restrict__ g, float tau, int with_y,
+                                                     float *__restrict__ coef, float *__restrict__ factor,
+                                                     int *__restrict__ most) {
+    __shared__ int waves[LS_WAVES];
+    int top = NO_EXP;
+    for (int64_t r = (int64_t)blockIdx.x * LS_WAVES + fl_wave_id(); r < a.op.M; r += (int64_t)gridDim.x * LS_WAVES) {
+        float c = a.rows[r].y != 0.0f ? tau * g[r] : 0.0f;
+        int e = 15;
+        const bool some = c != 0.0f && fabsf(c) < INFINITY;
+        if (some) {
+            frexpf(c, &e);  // |c| < 2^e
+            e = e < -110 ? -110 : e;
+            c = ldexpf(c, 15 - e);
+        }
+        if (fl_lane() == 0) {
+            coef[r] = c;
+            factor[r] = ldexpf(1.0f, e - 15);
+        }
+        if (!with_y || !some) continue;
+        const T *x = (const T *)a.op.x + r * a.op.ldx;
         float m = 0.0f;
-        for (int64_t i = threadIdx.x; i < M; i += 1024) {
-            const float c = rows[i].y != 0.0f ? fabsf(tau * g[i]) : 0.0f;
-            m = fmaxf(m, c < INFINITY ? c : 0.0f);
+        const auto see = [&](T v) {
+            const float t = fabsf((float)v);
+            m = fmaxf(m, t < INFINITY ? t : 0.0f);
+        };
+        for (int64_t k = fl_lane() * 8; k < a.op.K; k += FL_WAVE * 8) {
+            if (k + 8 <= a.op.K) {
+                const Vec<T, 8> v = load_vec<T, 8>(x + k);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) see(v.v[i]);
+            } else
+                for (int64_t i = k; i < a.op.K; ++i) see(x[i]);
         }
 #pragma unroll
         for (int o = FL_WAVE / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        if (fl_lane() == 0) most[threadIdx.x / FL_WAVE] = m;
-        __syncthreads();
-        for (int i = 0; i < 16; ++i) m = fmaxf(m, most[i]);
+        int xe;
+        frexpf(m, &xe);
+        if (m > 0.0f && xe + e - 15 > top) top = xe + e - 15;
+    }
+    if (fl_lane() == 0) waves[fl_wave_id()] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < LS_WAVES; ++w) top = waves[w] > top ? waves[w] : top;
+        most[blockIdx.x] = top;
+    }
+}
+
+// dW's other operand in half: rows of x times their power of two and one of all rows,
+// which brings the largest value to 2^13..2^14; 0 in rows without a gradient.
+template <typename T>
+__global__ __launch_bounds__(LS_NT) void k_lay_y(VocabArgs a, const int *__restrict__ most, int parts,
+                                                 _Float16 *__restrict__ y, int *__restrict__ y_exp) {
+    __shared__ int waves[LS_WAVES];
+    int top = NO_EXP;
+    for (int i = threadIdx.x; i < parts; i += LS_NT) top = most[i] > top ? most[i] : top;
+#pragma unroll
+    for (int o = FL_WAVE / 2; o > 0; o >>= 1) {
+        const int t = __shfl_xor(top, o);
+        top = t > top ? t : top;
+    }
+    if (fl_lane() == 0) waves[fl_wave_id()] = top;
+    __syncthreads();
+    for (int w = 0; w < LS_WAVES; ++w) top = waves[w] > top ? waves[w] : top;
+    if (top == NO_EXP) top = 14;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *y_exp = top - 14;
+    const int64_t chunks = a.ldy / 8;
+    for (int64_t i = (int64_t)blockIdx.x * LS_NT + threadIdx.x; i < a.op.M * chunks; i += (int64_t)gridDim.x * LS_NT) {
+        const int64_t r = i / chunks, c = i % chunks * 8, have = a.coef[r] != 0.0f ? a.op.K : 0;
+        const T *x = (const T *)a.op.x + r * a.op.ldx;
+        Vec<T, 8> v;
+        if (c + 8 <= have) v = load_vec<T, 8>(x + c);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v.v[e] = c + e < have ? x[c + e] : (T)0.0f;
         int e;
-        frexpf(m, &e);  // m < 2^e
-        e = e < -100 ? -100 : e;
-        scale = m > 0.0f ? ldexpf(1.0f, 14 - e) : 1.0f;
-        if (threadIdx.x == 0) *unscale = m > 0.0f ? ldexpf(1.0f, e - 14) : 1.0f;
-    } else if (fl_block() == 0 && threadIdx.x == 0) *unscale = 1.0f;
-    const int64_t step = SCALED ? 1024 : (int64_t)gridDim.x * 1024;
-    for (int64_t i = (SCALED ? 0 : (int64_t)blockIdx.x * 1024) + threadIdx.x; i < M; i += step)
-        coef[i] = rows[i].y != 0.0f ? tau * g[i] * scale : 0.0f;
+        frexpf(a.factor[r], &e);  // its power plus 1
+        Vec<_Float16, 8> o;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o.v[k] = (_Float16)ldexpf((float)v.v[k], e - 1 + 14 - top);
+        store_vec<_Float16, 8>(y + r * a.ldy + c, o);
+    }
+}
+
+// A value of dW from its sum.
+template <typename T>
+__device__ __forceinline__ T dw_of(float sum, int y_exp) {
+    return (T)(sizeof(T) == 2 ? ldexpf(sum, y_exp) : sum);
 }
 
 // dz of a piece but for the listed columns: the product again, an exponential in
@@ -314,6 +393,14 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_grad(VocabArgs a) {
     });
 }
 
+// A listed column's p from its u and the row's sums, 1 at most (its product is not the
+// one in the sums: where logits are so large that their rounding passes 1, it could be
+// anything above, and nothing that half holds).
+__device__ __forceinline__ float listed_share(float u, float2 sum) {
+    const float p = exp2_of(u - sum.x) * sum.y;
+    return p > 1.0f ? 1.0f : p;
+}
+
 // dz of the listed columns in the piece: scattered stores of 2 or 4 bytes, 4096 x 64
 // of them 12.5 us.
 template <typename T, bool WIDE>
@@ -324,7 +411,7 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
     const float c = a.coef[row];
     if (v < 0 || v >= a.width || c == 0.0f) return;
     const float2 l = a.listed[i];
-    const float d = c * (exp2_of(l.x - a.rows[row].x) * a.rows[row].y - l.y);
+    const float d = c * (listed_share(l.x, a.rows[row]) - l.y);
     if constexpr (WIDE && sizeof(T) == 4) {
         const float chunk[8] = {d, 0, 0, 0, 0, 0, 0, 0};
         u32x4 plane[3];
@@ -384,10 +471,12 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_dx(VocabArgs a) {
 // The parts of a sum added and rounded: four values a lane, a quarter of the
 // parts a wave, each in order and then the quarters.  HBM-bound: 67 MB of
 // parts in 17 us.
+// undo, factor (of rows of K values), exponent: what the sum is multiplied by, or null.
 template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_vocab_fold(const float *__restrict__ part, uint32_t parts, int64_t n,
-                                                      const float *__restrict__ unscale,
-                                                      const float *__restrict__ undo, T *__restrict__ out) {
+                                                      const float *__restrict__ undo,
+                                                      const float *__restrict__ factor, int64_t K,
+                                                      const int *__restrict__ exponent, T *__restrict__ out) {
     __shared__ float runs[LS_WAVES][4 * FL_WAVE];
     const int64_t i = (fl_block() * FL_WAVE + fl_lane()) * 4;
     const int have = n - i < 0 ? 0 : n - i < 4 ? (int)(n - i) : 4;
@@ -411,12 +500,15 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_fold(const float *__restrict__ 
     for (int e = 0; e < 4; ++e) runs[fl_wave_id()][fl_lane() * 4 + e] = s[e];
     __syncthreads();
     if (fl_wave_id() || !have) return;
-    const float f = *unscale, f2 = undo ? *undo : 1.0f;
+    const float f = undo ? *undo : 1.0f;
+    const int e2 = exponent ? *exponent : 0;
     Vec<T, 4> o;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int at = fl_lane() * 4 + e;
-        o.v[e] = (T)(((runs[0][at] + runs[1][at]) + (runs[2][at] + runs[3][at])) * f * f2);
+        float v = ((runs[0][at] + runs[1][at]) + (runs[2][at] + runs[3][at])) * f;
+        if (factor) v *= factor[(i + (e < have ? e : 0)) / K];
+        o.v[e] = (T)(exponent ? ldexpf(v, e2) : v);
     }
     if (have == 4) store_vec<T, 4>(out + i, o);
     else store_some<T, 4>(out + i, o, have);
@@ -437,10 +529,10 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_dw(VocabArgs a) {
     StridedTile<T, BM, BK> ta;
     StridedTile<T, BN, BK> tb;
     ta.init((const T *)a.d + begin * a.ldd + m0, a.ldd, a.ldd - m0, nullptr);
-    tb.init((const T *)a.op.x + begin * a.op.ldx + c0, a.op.ldx, a.op.K - c0, nullptr);
+    tb.init((const T *)a.y + begin * a.ldy + c0, a.ldy, a.op.K - c0, nullptr);
     Prod prod;
     prod.run(ta, tb, end - begin, lds);
-    const float f = a.sums ? 1.0f : *a.unscale;
+    const int y_exp = a.y_exp ? *a.y_exp : 0;
 #pragma unroll
     for (int i = 0; i < Prod::MT; ++i) {
         const int64_t m = m0 + prod.wave_m() + i * 16 + (fl_lane() & 15);
@@ -459,7 +551,7 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_dw(VocabArgs a) {
                 T *q = (T *)a.dw + (a.v0 + m) * a.op.K + c;
                 Vec<T, 4> o;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o.v[e] = (T)(prod.acc[i][j][e] * f);
+                for (int e = 0; e < 4; ++e) o.v[e] = dw_of<T>(prod.acc[i][j][e], y_exp);
                 if (n == 4) store_vec<T, 4>(q, o);
                 else store_some<T, 4>(q, o, n);
             }
@@ -499,8 +591,7 @@ __global__ __launch_bounds__(LS_NT) void k_few_dw(VocabArgs a) {
     const int64_t run = item / bands, c0 = item % bands * COLS;
     if (run >= runs || run >= tiles) return;
     const int r = fl_lane() & 15, q = fl_lane() >> 4;
-    const H *xs = (const H *)(WIDE ? (const void *)a.x : a.op.x);
-    const int64_t ldx = WIDE ? a.ldx : a.op.ldx;
+    const H *xs = (const H *)a.y;
     u32x4 x[KS][NT][P];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -508,11 +599,14 @@ __global__ __launch_bounds__(LS_NT) void k_few_dw(VocabArgs a) {
         for (int j = 0; j < NT; ++j) {
             // 16-bit tiles come in pairs whose columns alternate by fours: eight in a row a lane
             const int64_t c = c0 + (PAIR == 1 ? j * 16 + r : j / 2 * 32 + (r >> 2) * 8 + (j & 1) * 4 + (r & 3));
+            // loads without branches around them, from places that there are: the compiler moved values of earlier rows to
+            // other registers within the last branch, for the lanes that took it alone
             H v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int64_t m = s * 32 + q * 8 + i;
-                v[i] = m < M && c < K ? xs[(m < a.op.M ? m : m - a.op.M) * ldx + c] : (H)0.0f;
+                const int64_t m = s * 32 + q * 8 + i, row = m < M ? m : M - 1;
+                v[i] = xs[(row < a.op.M ? row : row - a.op.M) * a.ldy + (c < K ? c : K - 1)];
+                if (m >= M || c >= K) v[i] = (H)0.0f;
             }
             chunk_planes<H>(v, x[s][j]);
         }
@@ -527,7 +621,7 @@ __global__ __launch_bounds__(LS_NT) void k_few_dw(VocabArgs a) {
                 next[s][i] = ((const H *)a.d)[WIDE ? dz_at<1>(a, m, v) : m * a.ldd + v];
             }
     };
-    const float f = *a.unscale, f2 = a.undo ? a.undo[0] : 1.0f;
+    const int y_exp = a.y_exp ? *a.y_exp : 0;
     // the chunks of G columns that a lane stores
     const int band = (int)(K - c0 < COLS ? K - c0 : COLS), chunks = (band + G - 1) / G;
     const auto walk = [&](auto whole) {
@@ -563,7 +657,7 @@ __global__ __launch_bounds__(LS_NT) void k_few_dw(VocabArgs a) {
                         acc = mfma<H>(b[0], d[s][0], acc);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o.v[h * 4 + e] = (T)(acc[e] * f * f2);
+                    for (int e = 0; e < 4; ++e) o.v[h * 4 + e] = dw_of<T>(acc[e], y_exp);
                 }
                 *reinterpret_cast<u32x4 *>(mine + r * PITCH + (p * 4 + q) * G) = __builtin_bit_cast(u32x4, o);
             }
@@ -595,8 +689,10 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
     const int64_t c = item % blocks * LS_NT + threadIdx.x;
     if (part >= a.parts || c >= a.width) return;
     float s = 0.0f;
-    for (int64_t m = a.dz_rows * part / a.parts; m < a.dz_rows * (part + 1) / a.parts; ++m)
-        s += (float)((const T *)a.d)[m * a.ldd + c];
+    for (int64_t m = a.dz_rows * part / a.parts; m < a.dz_rows * (part + 1) / a.parts; ++m) {
+        const float d = (float)((const T *)a.d)[m * a.ldd + c];
+        s += a.factor ? d * a.factor[m < a.op.M ? m : m - a.op.M] : d;
+    }
     a.sums[part * a.width + c] = s;
 }
 
@@ -607,8 +703,6 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
 // HBM-bound: 1.18 GB of bfloat16 in 263 us = 4.5 TB/s.  Rows of x in which nothing
 // is listed do not count and are laid out as zeros (padded rows may hold anything),
 // a wave a row; live: those that count.
-constexpr int LAY_PARTS = 1024;
-
 template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restrict__ most,
                                                    uint8_t *__restrict__ live) {
@@ -906,7 +1000,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
             const int64_t v = a.op.lists.ids[m];
             const float2 l = a.listed[m];
             if (v >= a.v0 && v < end) id = __int_as_float((int)(v - a.v0));
-            d = c * (exp2_of(l.x - sum.x) * sum.y - l.y);
+            d = c * (listed_share(l.x, sum) - l.y);
         }
         of[t] = float4{sum.x, c * sum.y, id, d};
     }
@@ -994,12 +1088,13 @@ __global__ __launch_bounds__(LS_NT) void k_wide_cols(VocabArgs a) {
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 if (m + j >= end) break;
+                const float f = P == 1 ? a.factor[m + j] : 1.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float t = (float)v[j][P - 1].v[e];
 #pragma unroll
                     for (int p = P - 2; p >= 0; --p) t += (float)v[j][p].v[e];
-                    s[e] += t;
+                    s[e] += t * f;
                 }
             }
         }
@@ -1040,7 +1135,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
     };
     int64_t next = s0;
     aim(next);
-    const float f1 = a.dx ? *a.unscale : 1.0f, f2 = a.dx && a.undo ? a.undo[1] : 1.0f;
+    const float f = a.dx && a.undo ? a.undo[1] : 1.0f;
     Run run;
     run.template run<true>(
         ta, tb, 1, (int)(s1 - s0), wide_lds,
@@ -1060,6 +1155,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
                 __builtin_amdgcn_sched_barrier(0);
                 const int64_t row = row0 + run.wave_m() + i * 16 + (lane & 15);
                 if (row >= M) continue;
+                const float f2 = a.dx && P == 1 ? a.factor[row] : 1.0f;
 #pragma unroll
                 for (int j = 0; j < Run::NTL; ++j) {
                     const int64_t n = n0 + run.wave_n() + j * 16 + (lane >> 4) * 4;
@@ -1068,7 +1164,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
                     if (a.dx) {
                         Vec<T, 4> o;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o.v[e] = (T)(run.acc[i][j][e] * f1 * f2);
+                        for (int e = 0; e < 4; ++e) o.v[e] = (T)(run.acc[i][j][e] * f * f2);
                         T *q = (T *)a.dx + row * a.op.K + n;
                         if (have == 4) store_vec<T, 4>(q, o);
                         else store_some<T, 4>(q, o, have);
@@ -1117,7 +1213,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
         const int in = (int)(m0 % D_BLOCK);
         ta.init((const uint16_t *)a.d + m0 / D_BLOCK * a.d_block + k * a.ldd + P * in, a.ldd, D_BLOCK - in,
                 STEP);
-        tb.init(a.x + k * a.ldx + P * c0, a.ldx, a.cols - c0, left < STEP ? (int)left : STEP);
+        tb.init((const uint16_t *)a.y + k * a.ldy + P * c0, a.ldy, a.cols - c0, left < STEP ? (int)left : STEP);
     };
     const auto aim_tile = [&]() {
         const int64_t mt = fl_uniform_i64(next / a.n_tiles);
@@ -1126,7 +1222,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
         aim(s0);
     };
     aim_tile();
-    const float f = a.sums ? 1.0f : *a.unscale, f2 = a.sums || !a.undo ? 1.0f : a.undo[0];
+    const int y_exp = a.y_exp ? *a.y_exp : 0;
     Run run;
     run.template run<false>(
         ta, tb, (int)(t1 - t0), steps, wide_lds,
@@ -1166,7 +1262,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
                         T *q = (T *)a.dw + (a.v0 + m) * a.op.K + c;
                         Vec<T, 4> o;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o.v[e] = (T)(run.acc[i][j][e] * f * f2);
+                        for (int e = 0; e < 4; ++e) o.v[e] = dw_of<T>(run.acc[i][j][e], y_exp);
                         if (n == 4) store_vec<T, 4>(q, o);
                         else store_some<T, 4>(q, o, n);
                     }
@@ -1269,7 +1365,9 @@ VocabLayout vocab_layout(const fl_vocab *op, const VocabPlan &p) {
 }
 
 struct VocabSpace {
-    size_t coef, d, dx, dw, db, bytes;
+    size_t coef, factor, most, y_exp, y, d, dx, dw, db, bytes;
+    bool half;  // dz: its rows' gradients as a number and a power of two
+    int64_t ldy;
     int dx_parts, dw_parts, db_parts;
     int dx_tile, dx_cols, dw_cols, dw_tile;
     bool dx_direct, few_dw;
@@ -1284,7 +1382,15 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
         return at;
     };
     const bool f32 = op->dtype == FL_F32;
-    s.coef = take((size_t)(op->M + 1) * 4);
+    s.coef = take((size_t)op->M * 4);
+    s.half = op->dtype == FL_F16 || (op->dtype == FL_BF16 && p.wide);
+    if (s.half) {
+        s.factor = take((size_t)op->M * 4);
+        s.most = take(LAY_PARTS * 4);
+        s.y_exp = take(4);
+        s.ldy = ceil_div(op->K, 64) * 64;
+        if (with_dw) s.y = take((size_t)op->M * s.ldy * 2);
+    }
     s.d = take((size_t)p.d_rows * p.d_cols * p.size);
     const int narrow = op->K <= 128 ? 128 : 256;
     if (with_dx) {
@@ -1429,7 +1535,6 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
     VocabArgs a = vocab_args(op, p, state, layout);
     float *coef = (float *)(ws + s.coef);
     a.coef = coef;
-    a.unscale = coef + op->M;
     a.d = ws + s.d;
     a.ldd = p.ldd;
     a.d_block = p.d_block;
@@ -1437,14 +1542,32 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
     a.d_rows = p.d_rows;
     a.dz_rows = p.dz_rows;
     const dim3 nt(LN_NT), wt(WD_NT);
+    const float *none = nullptr;
     const auto fits = [&](int64_t grid) { return launch_fits(grid, WD_NT); };
     const auto fail = [&]() { return fl_fail(FL_ERR_ARG, "linear_loss: too many tiles for one launch (shape)"); };
-    if (std::is_same<T, _Float16>::value || (sizeof(T) == 2 && p.wide))
-        FL_LAUNCH("k_vocab_coef", k_vocab_coef<true>, dim3(1), dim3(1024), 0, st, a.rows, grad, op->lists.temperature,
-                  op->M, coef, coef + op->M);
-    else
-        FL_LAUNCH("k_vocab_coef", k_vocab_coef<false>, dim3((unsigned)(op->M > 65536 ? 64 : ceil_div(op->M, 1024))),
-                  dim3(1024), 0, st, a.rows, grad, op->lists.temperature, op->M, coef, coef + op->M);
+    a.y = p.wide ? (const void *)a.x : op->x;
+    a.ldy = p.wide ? a.ldx : op->ldx;
+    if (!s.half)
+        FL_LAUNCH("k_vocab_coef", k_vocab_coef, dim3((unsigned)(op->M > 65536 ? 64 : ceil_div(op->M, 1024))), dim3(1024),
+                  0, st, a.rows, grad, op->lists.temperature, op->M, coef);
+    if constexpr (sizeof(T) == 2)
+        if (s.half) {
+            float *factor = (float *)(ws + s.factor);
+            int *most = (int *)(ws + s.most), *y_exp = (int *)(ws + s.y_exp);
+            const int64_t all = ceil_div(op->M, LS_WAVES);
+            const int parts = (int)(all < LAY_PARTS ? all : LAY_PARTS);
+            a.factor = factor;
+            FL_LAUNCH("k_row_scale", k_row_scale<T>, dim3(parts), dim3(LS_NT), 0, st, a, grad, op->lists.temperature,
+                      dw && op->K, coef, factor, most);
+            a.y = ws + s.y;
+            a.ldy = s.ldy;
+            a.y_exp = y_exp;
+            if (dw && op->K) {
+                const int64_t want = ceil_div(op->M * (s.ldy / 8), LS_NT);
+                FL_LAUNCH("k_lay_y", k_lay_y<T>, dim3((unsigned)(want < 2048 ? want : 2048)), dim3(LS_NT), 0, st, a, most,
+                          parts, (_Float16 *)(ws + s.y), y_exp);
+            }
+        }
     for (a.v0 = 0; a.v0 < op->V; a.v0 += p.piece) {
         a.width = op->V - a.v0 < p.piece ? op->V - a.v0 : p.piece;
         a.m_tiles = p.m_tiles;
@@ -1538,7 +1661,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             else FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 64, 64, BK>), g, nt, 0, st, a);
             if (a.sums)
                 FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(a.width * op->K, FL_WAVE * 4)), dim3(LS_NT),
-                          0, st, a.sums, a.parts, a.width * op->K, a.unscale, a.undo, (T *)dw + a.v0 * op->K);
+                          0, st, a.sums, a.parts, a.width * op->K, none, none, (int64_t)1, a.y_exp, (T *)dw + a.v0 * op->K);
         }
         if (db) {
             a.parts = (uint32_t)s.db_parts;
@@ -1550,19 +1673,18 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
             else
                 FL_LAUNCH("k_vocab_cols", k_vocab_cols<T>, grid_of(a.parts * ceil_div(a.width, LS_NT)), dim3(LS_NT), 0,
                           st, a);
-            const float *none = nullptr;
             if (op->bias_f32)
                 FL_LAUNCH("k_vocab_fold", k_vocab_fold<float>, g, dim3(LS_NT), 0, st, a.sums, a.parts, a.width,
-                          a.unscale, none, (float *)db + a.v0);
+                          none, none, (int64_t)1, (const int *)nullptr, (float *)db + a.v0);
             else
-                FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, g, dim3(LS_NT), 0, st, a.sums, a.parts, a.width, a.unscale,
-                          none, (T *)db + a.v0);
+                FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, g, dim3(LS_NT), 0, st, a.sums, a.parts, a.width, none,
+                          none, (int64_t)1, (const int *)nullptr, (T *)db + a.v0);
         }
     }
     if (dx && op->K && !s.dx_direct)
         FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(op->M * op->K, FL_WAVE * 4)), dim3(LS_NT), 0, st,
-                  (const float *)(ws + s.dx), (uint32_t)(s.dx_parts * (p.dz_rows / op->M)), op->M * op->K, a.unscale,
-                  a.undo ? a.undo + 1 : nullptr, (T *)dx);
+                  (const float *)(ws + s.dx), (uint32_t)(s.dx_parts * (p.dz_rows / op->M)), op->M * op->K,
+                  a.undo ? a.undo + 1 : none, a.factor, op->K, (const int *)nullptr, (T *)dx);
     return fl_check_launch("linear_loss");
 }
 

@@ -166,8 +166,11 @@ def linear_cross_entropy(x, weight, target, bias=None):
     (a copy of x and weight, held for the backward): bfloat16 values are off by
     nothing or by 2^-38 of the largest of their tensor.  The logits' gradient is
     an operand of two products and a term of the bias's: float32's is held as
-    such, 16-bit ones' as half (of up to 64 rows of half with what its rounding
-    leaves).
+    such; of 16-bit operands the softmax's terms less what the row is held to
+    are held as half (2^-11 of themselves or 2^-39; of up to 64 rows of half
+    with what rounding leaves), whatever the losses' gradients are, and in
+    weight's gradient each row's input times its loss's (2^-38 of the largest
+    of all rows).
     Softmax terms are off by 2^-23 of themselves times 1 + their logit's
     distance from the largest (at least 16 over large vocabularies), whatever
     all logits have in common; a bias whose quotient by the temperature

@@ -131,3 +131,29 @@ def test_wide_products_in_float32(M, K, V):
     x, w, b, ids, _, g = _make(M, K, V, torch.float32, 11)
     ids[::7] = -1
     _check(x, w, b, ids, g)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,K,V", ROWS)
+def test_weights_of_losses_stay_with_their_rows(M, K, V, t):
+    """The gradient of one row's loss, of any size, changes no bit of another row's dx."""
+    x, w, b, ids, _, g = _make(M, K, V, t, 4)
+    one = _run(x, w, b, ids, None, g)
+    rows = torch.arange(M) != 2
+    for factor in (2.0 ** 45, 2.0 ** -45, -3.0, 0.0):
+        other = _run(x, w, b, ids, None, torch.where(rows, g, g * factor))
+        assert torch.equal(other["dx"][rows], one["dx"][rows]), factor
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,K,V", ROWS)
+def test_gradients_of_losses_of_different_weights(M, K, V, t):
+    """Rows' losses weigh 1 and 2^-45 (half: 2^14 and 2^-10): every row's dx is within its own row's bound."""
+    x, w, b, ids, _, g = _make(M, K, V, t, 5)
+    large, small = (2.0 ** 14, 2.0 ** -10) if t is torch.float16 else (1.0, 2.0 ** -45)
+    g = torch.where(torch.arange(M) % 3 == 0, g * large, g * small)
+    ref, out = _reference(x, w, b.float(), ids, g), _run(x, w, b.float(), ids, None, g)
+    for k in ("loss", "dx", "db"):
+        _held(out[k], *ref[k], k)
+    fits = ref["dw"][0].abs() + ref["dw"][1] < torch.finfo(t).max  # half: what overflows is infinite
+    _held(torch.where(fits, out["dw"].double().cpu(), 0.0), torch.where(fits, ref["dw"][0], 0.0), ref["dw"][1], "dw")
