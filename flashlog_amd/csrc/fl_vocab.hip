@@ -59,10 +59,10 @@ struct VocabArgs {
     const int *y_exp;
     int add;
     // wide kernels: operands laid out (or as they are), their columns and dz's with those that pad them to whole steps
-    // (dz: 0 there, and in the rows that pad it), and what undoes the planes' powers of two (or null)
+    // (dz: 0 there, and in the rows that pad it), and what undoes the powers of two of x's rows and of weight (or null)
     const uint16_t *x, *w;
     int64_t ldx, ldw, cols, d_cols, d_rows;
-    const float *undo;     // x's, weight's
+    const float *undo_x, *undo_w;
 };
 
 // u of four listed ids of a row (-1: none), by one wave; the same in all lanes.
@@ -699,13 +699,22 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
 // ---------------------------------------------------------------------------
 // The same for large products
 
-// The largest finite magnitude of x and of weight, a part of them a workgroup.
-// HBM-bound: 1.18 GB of bfloat16 in 263 us = 4.5 TB/s.  Rows of x in which nothing
-// is listed do not count and are laid out as zeros (padded rows may hold anything),
-// a wave a row; live: those that count.
+// bfloat16 in training: rows of x laid out, a wave each (blockIdx.y 0), and the largest
+// finite magnitude of weight, a part of it a workgroup.  HBM-bound: 1.18 GB of weight in
+// 263 us = 4.5 TB/s.  A row of x is multiplied by a power of two of its own, so that rows
+// of any sizes keep their bits beside each other (as operands of the logits: dW takes
+// them from k_lay_y); one in which nothing is listed is zeros (padded rows may hold
+// anything).
+// The power of two that brings m to 2^13..2^14 is 2^(14 - e).
+__device__ __forceinline__ int exponent_of(float m) {
+    int e;
+    frexpf(m, &e);  // m < 2^e
+    return e < -100 ? -100 : e;
+}
+
 template <typename T>
-__global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restrict__ most,
-                                                   uint8_t *__restrict__ live) {
+__global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restrict__ most, _Float16 *__restrict__ out,
+                                                   float *__restrict__ undo_x) {
     constexpr int G = 16 / (int)sizeof(T);
     __shared__ float waves[LS_WAVES];
     float m = 0.0f;
@@ -742,9 +751,28 @@ __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restric
                 any = any || (id >= 0 && id < a.op.V);
             }
             any = __any(any);
-            if (fl_lane() == 0) live[r] = any;
-            if (any) see_row((const T *)a.op.x + r * a.op.ldx, fl_lane() * G, FL_WAVE * G, a.op.K);
+            const T *row = (const T *)a.op.x + r * a.op.ldx;
+            m = 0.0f;
+            if (any) see_row(row, fl_lane() * G, FL_WAVE * G, a.op.K);
+#pragma unroll
+            for (int o = FL_WAVE / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+            const int e = exponent_of(m);
+            const float scale = ldexpf(1.0f, 14 - e);
+            if (fl_lane() == 0) undo_x[r] = ldexpf(1.0f, e - 14);
+            const int64_t have = any ? a.op.K : 0;
+            for (int64_t c = fl_lane() * 8; c < a.cols; c += FL_WAVE * 8) {
+                Vec<T, 8> v;
+                if (c + 8 <= have) v = load_vec<T, 8>(row + c);
+                else
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v.v[i] = c + i < have ? row[c + i] : (T)0.0f;
+                Vec<_Float16, 8> o;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o.v[i] = (_Float16)((float)v.v[i] * scale);
+                store_vec<_Float16, 8>(out + r * a.cols + c, o);
+            }
         }
+        return;
     } else {
         // rows without gaps are one, of all workgroups
         const bool one = a.op.ldw == a.op.K;
@@ -758,21 +786,20 @@ __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restric
     if (fl_lane() == 0) waves[fl_wave_id()] = m;
     __syncthreads();
     if (threadIdx.x == 0)
-        most[blockIdx.y * LAY_PARTS + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+        most[blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
 }
 
-// x and weight as rows on 16 bytes: fp32 as its planes (plane_at), bfloat16 as half,
-// times a power of two that brings the largest to 2^13..2^14 (what is
-// above 2^-31 of it is held exactly, and what is lost below 2^-38), half, and
-// bfloat16 that no backward follows, as they are; zeros behind a row.  (dz, in
+// x and weight as rows on 16 bytes: fp32 as its planes (plane_at), half, and bfloat16
+// that no backward follows, as they are; SCALED, bfloat16 in training: weight as half
+// times a power of two that brings the largest to 2^13..2^14 (what is above 2^-31 of
+// it is held exactly, and what is lost below 2^-38).  Zeros behind a row.  (dz, in
 // half, is then rounded by 2^-11 of itself; by 2^-8 in bfloat16 it made the
 // gradients' error 1.4 to 1.5 times that of their own rounding.)  HBM-bound: 1.18
 // GB of bfloat16 read and written in 443 us = 5.3 TB/s.
 template <typename T, bool SCALED>
-__global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restrict__ most,
-                                               const uint8_t *__restrict__ live, uint16_t *__restrict__ x,
+__global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restrict__ most, uint16_t *__restrict__ x,
                                                uint16_t *__restrict__ w, float *__restrict__ undo) {
-    const bool second = blockIdx.y;
+    const bool second = SCALED || blockIdx.y;
     const int64_t R = second ? a.op.V : a.op.M, ld = second ? a.op.ldw : a.op.ldx, chunks = a.cols / 8, K = a.op.K;
     const T *p = (const T *)(second ? a.op.weight : a.op.x);
     uint16_t *out = second ? w : x;
@@ -780,26 +807,22 @@ __global__ __launch_bounds__(LS_NT) void k_lay(VocabArgs a, const float *__restr
     if constexpr (SCALED) {
         __shared__ float waves[LS_WAVES];
         float m = 0.0f;
-        for (int i = threadIdx.x; i < LAY_PARTS; i += LS_NT) m = fmaxf(m, most[blockIdx.y * LAY_PARTS + i]);
+        for (int i = threadIdx.x; i < LAY_PARTS; i += LS_NT) m = fmaxf(m, most[i]);
 #pragma unroll
         for (int o = FL_WAVE / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
         if (fl_lane() == 0) waves[fl_wave_id()] = m;
         __syncthreads();
-        m = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
-        int e;
-        frexpf(m, &e);  // m < 2^e
-        e = e < -100 ? -100 : e;
+        const int e = exponent_of(fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3])));
         scale = ldexpf(1.0f, 14 - e);
-        if (blockIdx.x == 0 && threadIdx.x == 0) undo[blockIdx.y] = ldexpf(1.0f, e - 14);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *undo = ldexpf(1.0f, e - 14);
     }
     for (int64_t i = (int64_t)blockIdx.x * LS_NT + threadIdx.x; i < R * chunks; i += (int64_t)gridDim.x * LS_NT) {
         const int64_t r = i / chunks, c = i % chunks * 8;
-        const int64_t have = SCALED && !second && !live[r] ? 0 : K;
         Vec<T, 8> v;
-        if (c + 8 <= have) v = load_vec<T, 8>(p + r * ld + c);
+        if (c + 8 <= K) v = load_vec<T, 8>(p + r * ld + c);
         else
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v.v[e] = c + e < have ? p[r * ld + c + e] : (T)0.0f;
+            for (int e = 0; e < 8; ++e) v.v[e] = c + e < K ? p[r * ld + c + e] : (T)0.0f;
         if constexpr (sizeof(T) == 4) {
             u32x4 plane[3];
             chunk_planes<float>(v.v, plane);
@@ -874,9 +897,15 @@ __device__ __forceinline__ int64_t part_begin(int64_t all, uint32_t part, uint32
     return fl_uniform_i64(all * part / parts);
 }
 
-// What a product is multiplied by, in units of log 2 (finite: a product of 0 stays 0).
-__device__ __forceinline__ float product_scale(const VocabArgs &a) {
-    return a.undo ? fminf(a.undo[0] * a.undo[1] * a.scale, 0x1.fffffep127f) : a.scale;
+// What a row's products are multiplied by, in units of log 2 (finite: a product of 0 stays 0).
+__device__ __forceinline__ float product_scale(const VocabArgs &a, int64_t row) {
+    if (!a.undo_x) return a.scale;
+    return fminf(a.undo_x[row < a.op.M ? row : a.op.M - 1] * *a.undo_w * a.scale, 0x1.fffffep127f);
+}
+// Whether the operands' rows have powers of two.
+template <typename T, typename H>
+constexpr bool is_scaled() {
+    return std::is_same<T, __bf16>::value && std::is_same<H, _Float16>::value;
 }
 
 // A lane's bias for its 16 columns from n on, in units of log 2.
@@ -920,8 +949,12 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
     for (int i = 0; i < MT; ++i) sums[i * FL_WAVE + fl_lane()] = Running{-INFINITY, 0.0f};
     Tiles tiles;
     tiles.init(a, row0, t0 * WN * 64);
-    const float scale = product_scale(a);
+    constexpr bool SCALED = is_scaled<T, H>();
+    float scales[(MT + 3) / 4];  // of the wave's rows, one a lane
     Run run;
+    if constexpr (SCALED)
+#pragma unroll
+        for (int h = 0; h < (MT + 3) / 4; ++h) scales[h] = product_scale(a, row0 + run.wave_m() + h * FL_WAVE + fl_lane());
     run.template run<false>(
         tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds,
         [&](int i, uint16_t *la, uint16_t *lb) { tiles.feed(a, i, la, lb); },
@@ -936,7 +969,8 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
             for (int i = 0; i < MT; ++i) {
                 __builtin_amdgcn_sched_barrier(0);  // a row's values at a time: few registers
                 Running r = state[i * FL_WAVE];
-                float s = 0.0f;
+                float s = 0.0f, scale = a.scale;
+                if constexpr (SCALED) scale = __shfl(scales[i / 4], i % 4 * 16 + (lane & 15));
                 const auto u = [&](int e, float less) {
                     const float v = run.acc[i][e / 4][e % 4];
                     const float t = a.op.bias ? b[e] - less : -less;
@@ -1004,10 +1038,13 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
         }
         of[t] = float4{sum.x, c * sum.y, id, d};
     }
+    constexpr bool SCALED = is_scaled<T, WideDz<T>>();
+    float *scales = reinterpret_cast<float *>(of + BM);
+    if constexpr (SCALED)
+        for (int t = threadIdx.x; t < BM; t += WD_NT) scales[t] = product_scale(a, row0 + t);
     __syncthreads();
     Tiles tiles;
     tiles.init(a, row0, a.v0 + t0 * WN * 64);
-    const float scale = product_scale(a);
     Run run;
     run.template run<false>(
         tiles.ta, tiles.tb, (int)(t1 - t0), tiles.steps, wide_lds,
@@ -1023,6 +1060,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
                 __builtin_amdgcn_sched_barrier(0);
                 const int r = run.wave_m() + i * 16 + (lane & 15);
                 const float4 q = of[r];
+                const float scale = SCALED ? scales[r] : a.scale;
                 const int64_t at = __float_as_int(q.z) - c;  // of the row's only id
                 float u[16];
 #pragma unroll
@@ -1135,7 +1173,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
     };
     int64_t next = s0;
     aim(next);
-    const float f = a.dx && a.undo ? a.undo[1] : 1.0f;
+    const float f = a.dx && a.undo_w ? *a.undo_w : 1.0f;
     Run run;
     run.template run<true>(
         ta, tb, 1, (int)(s1 - s0), wide_lds,
@@ -1348,19 +1386,22 @@ VocabPlan vocab_plan(const fl_vocab *op) {
     return p;
 }
 
-// The laid out operands: x, weight, what undoes their powers of two, parts of their maxima, x's rows that count.
+// The laid out operands: x, weight, what undoes the powers of two of x's rows and of weight, parts of weight's maximum.
 struct VocabLayout {
-    size_t x, w, undo, most, live, bytes;
+    size_t x, w, undo_x, undo_w, most, bytes;
 };
 
 VocabLayout vocab_layout(const fl_vocab *op, const VocabPlan &p) {
     VocabLayout l{};
     if (!p.lay) return l;
     l.w = rounded((size_t)op->M * p.cols * p.size);
-    l.undo = l.w + rounded((size_t)op->V * p.cols * p.size);
-    l.most = l.undo + 256;
-    l.live = l.most + 2 * LAY_PARTS * 4;
-    l.bytes = l.live + rounded((size_t)op->M);
+    l.bytes = l.w + rounded((size_t)op->V * p.cols * p.size);
+    if (p.scaled) {
+        l.undo_x = l.bytes;
+        l.undo_w = l.undo_x + rounded((size_t)op->M * 4);
+        l.most = l.undo_w + 256;
+        l.bytes = l.most + LAY_PARTS * 4;
+    }
     return l;
 }
 
@@ -1451,7 +1492,10 @@ VocabArgs vocab_args(const fl_vocab *op, const VocabPlan &p, void *state, void *
         a.x = (const uint16_t *)((char *)layout + l.x);
         a.w = (const uint16_t *)((char *)layout + l.w);
         a.ldx = a.ldw = op->dtype == FL_F32 ? 3 * p.cols : p.cols;
-        if (p.scaled) a.undo = (const float *)((char *)layout + l.undo);
+        if (p.scaled) {
+            a.undo_x = (const float *)((char *)layout + l.undo_x);
+            a.undo_w = (const float *)((char *)layout + l.undo_w);
+        }
     } else {
         a.x = (const uint16_t *)op->x;
         a.w = (const uint16_t *)op->weight;
@@ -1485,19 +1529,19 @@ int vocab_forward(hipStream_t st, const fl_vocab *op, float *loss, void *state, 
     const dim3 g((unsigned)grid);
     if (p.lay) {
         const VocabLayout l = vocab_layout(op, p);
-        float *most = (float *)((char *)layout + l.most);
-        uint8_t *live = (uint8_t *)layout + l.live;
-        const int64_t chunks = (op->M > op->V ? op->M : op->V) * (p.cols / 8), want = ceil_div(chunks, LS_NT);
-        const dim3 lg((unsigned)(want < 4096 ? want : 4096), 2);
+        const int64_t chunks = (op->M > op->V && !p.scaled ? op->M : op->V) * (p.cols / 8), want = ceil_div(chunks, LS_NT);
+        const unsigned lg = (unsigned)(want < 4096 ? want : 4096);
         if constexpr (std::is_same<T, __bf16>::value)
             if (p.scaled) {
-                FL_LAUNCH("k_lay_max", k_lay_max<T>, dim3(LAY_PARTS, 2), dim3(LS_NT), 0, st, a, most, live);
-                FL_LAUNCH("k_lay", (k_lay<T, true>), lg, dim3(LS_NT), 0, st, a, most, live, (uint16_t *)a.x,
-                          (uint16_t *)a.w, (float *)a.undo);
+                float *most = (float *)((char *)layout + l.most);
+                FL_LAUNCH("k_lay_max", k_lay_max<T>, dim3(LAY_PARTS, 2), dim3(LS_NT), 0, st, a, most, (_Float16 *)a.x,
+                          (float *)a.undo_x);
+                FL_LAUNCH("k_lay", (k_lay<T, true>), dim3(lg), dim3(LS_NT), 0, st, a, most, (uint16_t *)a.x,
+                          (uint16_t *)a.w, (float *)a.undo_w);
             }
         if (!p.scaled)
-            FL_LAUNCH("k_lay", (k_lay<T, false>), lg, dim3(LS_NT), 0, st, a, most, live, (uint16_t *)a.x,
-                      (uint16_t *)a.w, (float *)nullptr);
+            FL_LAUNCH("k_lay", (k_lay<T, false>), dim3(lg, 2), dim3(LS_NT), 0, st, a, (const float *)nullptr,
+                      (uint16_t *)a.x, (uint16_t *)a.w, (float *)nullptr);
     }
     const bool few = op->lists.k <= DOT_IDS && p.parts <= 4 * FL_WAVE;
     if (!few && op->lists.k)
@@ -1579,7 +1623,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
         int64_t grid = (int64_t)a.m_tiles * a.parts;
         if (!fits(grid)) return fail();
         if (p.wide) {
-            const auto extra = [](int bm) { return (unsigned)(bm * sizeof(float4)); };
+            const auto extra = [](int bm) { return (unsigned)(bm * (sizeof(float4) + sizeof(float))); };
             const dim3 g((unsigned)grid);
             if (p.bm == 128)
                 FL_LAUNCH("k_wide_grad", (k_wide_grad<T, 128, 2, S>), g, wt, tiles_bytes<T>(128, 128, S) + extra(128), st, a);
@@ -1684,7 +1728,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
     if (dx && op->K && !s.dx_direct)
         FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(op->M * op->K, FL_WAVE * 4)), dim3(LS_NT), 0, st,
                   (const float *)(ws + s.dx), (uint32_t)(s.dx_parts * (p.dz_rows / op->M)), op->M * op->K,
-                  a.undo ? a.undo + 1 : none, a.factor, op->K, (const int *)nullptr, (T *)dx);
+                  a.undo_w, a.factor, op->K, (const int *)nullptr, (T *)dx);
     return fl_check_launch("linear_loss");
 }
 

@@ -163,8 +163,8 @@ def linear_cross_entropy(x, weight, target, bias=None):
     where there are more rows than that holds).  Large products lay float32 operands out as
     three bfloat16 planes (1.5 times their size; all of their 24 bits, at
     float32's range), and bfloat16 ones in training as scaled half
-    (a copy of x and weight, held for the backward): bfloat16 values are off by
-    nothing or by 2^-38 of the largest of their tensor.  The logits' gradient is
+    (a copy of x and weight, held for the backward): a bfloat16 value is off by
+    nothing, or by 2^-38 of the largest of its row of x or of weight.  The logits' gradient is
     an operand of two products and a term of the bias's: float32's is held as
     such; of 16-bit operands the softmax's terms less what the row is held to
     are held as half (2^-11 of themselves or 2^-39; of up to 64 rows of half

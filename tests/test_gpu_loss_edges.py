@@ -157,3 +157,17 @@ def test_gradients_of_losses_of_different_weights(M, K, V, t):
         _held(out[k], *ref[k], k)
     fits = ref["dw"][0].abs() + ref["dw"][1] < torch.finfo(t).max  # half: what overflows is infinite
     _held(torch.where(fits, out["dw"].double().cpu(), 0.0), torch.where(fits, ref["dw"][0], 0.0), ref["dw"][1], "dw")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,K,V", ROWS)
+def test_sizes_of_rows_stay_with_them(M, K, V, t):
+    """One row of x, of any size, changes no bit of another row's loss and dx."""
+    x, w, b, ids, _, g = _make(M, K, V, t, 6)
+    one = _run(x, w, b, ids, None, g)
+    rows = torch.arange(M) != 2
+    for factor in ((2.0 ** 10, 2.0 ** -10) if t is torch.float16 else (2.0 ** 50, 2.0 ** 10, 2.0 ** -50)):
+        y = torch.where(rows[:, None], x, x * factor)
+        other = _run(y, w, b, ids, None, g)
+        for k in ("loss", "dx"):
+            assert torch.equal(other[k][rows], one[k][rows]), (k, factor)
