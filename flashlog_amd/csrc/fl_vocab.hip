@@ -145,13 +145,16 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_rows(VocabArgs a, ListArgs l) {
     });
 }
 
-// Planes of a value in the wide kernels' operands, what they are, and dz's.
+// Planes of a value in the wide kernels' operands, and what they and dz are; dz in
+// the others.
 template <typename T>
 constexpr int planes_of() {
     return sizeof(T) == 4 ? 3 : 1;
 }
 template <typename T>
 using WideDz = typename std::conditional<sizeof(T) == 4, __bf16, _Float16>::type;
+template <typename T>
+using PlainDz = typename std::conditional<sizeof(T) == 4, float, _Float16>::type;
 
 // Where the wide kernels' dz of row m and column c (of the piece) is; of three
 // planes the first one's, the others are each 32 values behind the one before.
@@ -381,15 +384,16 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_grad(VocabArgs a) {
     each_u<T>(a, prod.acc, col, a.v0 + a.width, [&](int i, int j, const float (&u)[4]) {
         const int64_t n = col + j * 16 + (fl_lane() >> 4) * 4 - a.v0;
         if (row + i * 16 >= a.op.M || n >= a.ldd) return;
-        Vec<T, 4> o, rest;
+        using D = PlainDz<T>;
+        Vec<D, 4> o, rest;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float d = c[i] == 0.0f ? 0.0f : c[i] * exp2_of(u[e] - top[i]);
-            o.v[e] = (T)d;
-            rest.v[e] = (T)(d - (float)o.v[e]);
+            o.v[e] = (D)d;
+            rest.v[e] = (D)(d - (float)o.v[e]);
         }
-        store_vec<T, 4>((T *)a.d + (row + i * 16) * a.ldd + n, o);
-        if (a.dz_rows > a.op.M) store_vec<T, 4>((T *)a.d + (a.op.M + row + i * 16) * a.ldd + n, rest);
+        store_vec<D, 4>((D *)a.d + (row + i * 16) * a.ldd + n, o);
+        if (a.dz_rows > a.op.M) store_vec<D, 4>((D *)a.d + (a.op.M + row + i * 16) * a.ldd + n, rest);
     });
 }
 
@@ -421,9 +425,10 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_listed(VocabArgs a) {
         for (int p = 0; p < 3; ++p) to[p * 32] = (uint16_t)plane[p][0];
     } else if constexpr (WIDE) ((_Float16 *)a.d)[dz_at<1>(a, row, v)] = (_Float16)d;
     else {
-        const T o = (T)d;
-        ((T *)a.d)[row * a.ldd + v] = o;
-        if (a.dz_rows > a.op.M) ((T *)a.d)[(a.op.M + row) * a.ldd + v] = (T)(d - (float)o);
+        using D = PlainDz<T>;
+        const D o = (D)d;
+        ((D *)a.d)[row * a.ldd + v] = o;
+        if (a.dz_rows > a.op.M) ((D *)a.d)[(a.op.M + row) * a.ldd + v] = (D)(d - (float)o);
     }
 }
 
@@ -690,7 +695,7 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
     if (part >= a.parts || c >= a.width) return;
     float s = 0.0f;
     for (int64_t m = a.dz_rows * part / a.parts; m < a.dz_rows * (part + 1) / a.parts; ++m) {
-        const float d = (float)((const T *)a.d)[m * a.ldd + c];
+        const float d = (float)((const PlainDz<T> *)a.d)[m * a.ldd + c];
         s += a.factor ? d * a.factor[m < a.op.M ? m : m - a.op.M] : d;
     }
     a.sums[part * a.width + c] = s;
@@ -1324,6 +1329,9 @@ struct VocabPlan {
     int64_t size;                      // bytes of a value of dz
 };
 
+// Inputs whose laid out rows have 32-bit offsets over a tile (255 and 127 of them, 2 and 6 bytes a value).
+constexpr int64_t most_inputs(bool f32) { return f32 ? 1 << 22 : 1 << 23; }
+
 VocabPlan vocab_plan(const fl_vocab *op) {
     VocabPlan p{};
     const bool f32 = op->dtype == FL_F32;
@@ -1346,7 +1354,7 @@ VocabPlan vocab_plan(const fl_vocab *op) {
         least = 1;
         work = 0;
     } else if (p.lay) least = op->train ? 128 : 384;
-    p.wide = op->K >= 1 && op->K <= 1 << 20 && op->M >= least && (double)op->M * op->V * op->K >= work;
+    p.wide = op->K >= 1 && op->K <= most_inputs(f32) && op->M >= least && (double)op->M * op->V * op->K >= work;
     p.lay = p.lay && p.wide;
     p.scaled = p.scaled && p.wide;
     p.size = !f32 ? 2 : p.wide ? 6 : 4;
@@ -1424,7 +1432,7 @@ VocabSpace vocab_space(const fl_vocab *op, const VocabPlan &p, bool with_dx, boo
     };
     const bool f32 = op->dtype == FL_F32;
     s.coef = take((size_t)op->M * 4);
-    s.half = op->dtype == FL_F16 || (op->dtype == FL_BF16 && p.wide);
+    s.half = !f32;
     if (s.half) {
         s.factor = take((size_t)op->M * 4);
         s.most = take(LAY_PARTS * 4);
@@ -1574,6 +1582,8 @@ template <typename T>
 int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *state, void *layout, void *dx, void *dw,
                    void *db, char *ws) {
     constexpr int BK = sizeof(T) == 4 ? 32 : 64, S = small_stages<T>();
+    // dx and dW by the plain tiles: bfloat16 in training has them only where there are no inputs, and so neither
+    constexpr bool PLAIN = !std::is_same<T, __bf16>::value;
     const VocabPlan p = vocab_plan(op);
     const VocabSpace s = vocab_space(op, p, dx, dw, db);
     VocabArgs a = vocab_args(op, p, state, layout);
@@ -1595,7 +1605,7 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
         FL_LAUNCH("k_vocab_coef", k_vocab_coef, dim3((unsigned)(op->M > 65536 ? 64 : ceil_div(op->M, 1024))), dim3(1024),
                   0, st, a.rows, grad, op->lists.temperature, op->M, coef);
     if constexpr (sizeof(T) == 2)
-        if (s.half) {
+        {
             float *factor = (float *)(ws + s.factor);
             int *most = (int *)(ws + s.most), *y_exp = (int *)(ws + s.y_exp);
             const int64_t all = ceil_div(op->M, LS_WAVES);
@@ -1657,9 +1667,10 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
                     else
                         FL_LAUNCH("k_wide_dx", (k_wide_dx<T, 256, 4, 2>), g, wt, tiles_bytes<T>(256, 256, 2), st, a);
                 }
-            } else if (s.dx_tile == 128)
-                FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 128, 128, BK>), g, nt, 0, st, a);
-            else FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 64, 64, BK>), g, nt, 0, st, a);
+            } else if constexpr (PLAIN) {
+                if (s.dx_tile == 128) FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 128, 128, BK>), g, nt, 0, st, a);
+                else FL_LAUNCH("k_vocab_dx", (k_vocab_dx<T, 64, 64, BK>), g, nt, 0, st, a);
+            }
         }
         if (dw && op->K && s.few_dw) {
             const int cols = p.dz_rows <= 32 ? few_cols<T, 1>() : p.dz_rows <= 64 ? few_cols<T, 2>() : few_cols<T, 4>();
@@ -1675,10 +1686,10 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
                 else if (p.dz_rows <= 64) FL_LAUNCH("k_few_dw", (k_few_dw<T, WIDE, 2>), g, t, 0, st, a);
                 else if constexpr (sizeof(T) == 2) FL_LAUNCH("k_few_dw", (k_few_dw<T, WIDE, 4>), g, t, 0, st, a);
             };
-            if constexpr (sizeof(T) == 2) {
+            if constexpr (sizeof(T) == 2)
                 if (p.wide) launch(std::true_type());
-                else launch(std::false_type());
-            } else launch(std::false_type());
+            if constexpr (PLAIN)
+                if (!p.wide) launch(std::false_type());
         } else if (dw && op->K) {
             const int rows = s.dw_tile, cols = p.wide ? s.dw_cols : s.dw_tile;
             a.m_tiles = (uint32_t)ceil_div(a.width, rows);
@@ -1700,9 +1711,10 @@ int vocab_backward(hipStream_t st, const fl_vocab *op, const float *grad, void *
                     else
                         FL_LAUNCH("k_wide_dw", (k_wide_dw<T, 256, 4, 2>), g, wt, tiles_bytes<T>(256, 256, 2), st, a);
                 }
-            } else if (rows == 128)
-                FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 128, 128, BK>), g, nt, 0, st, a);
-            else FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 64, 64, BK>), g, nt, 0, st, a);
+            } else if constexpr (PLAIN) {
+                if (rows == 128) FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 128, 128, BK>), g, nt, 0, st, a);
+                else FL_LAUNCH("k_vocab_dw", (k_vocab_dw<T, 64, 64, BK>), g, nt, 0, st, a);
+            }
             if (a.sums)
                 FL_LAUNCH("k_vocab_fold", k_vocab_fold<T>, grid_of(ceil_div(a.width * op->K, FL_WAVE * 4)), dim3(LS_NT),
                           0, st, a.sums, a.parts, a.width * op->K, none, none, (int64_t)1, a.y_exp, (T *)dw + a.v0 * op->K);
@@ -1738,6 +1750,8 @@ int check_vocab(const fl_vocab *op, const char *what) {
     if (op->M < 0 || op->V < 1 || op->K < 0 || op->V > 0x7fffffffll || op->K > 0x7fffffffll || op->M != op->lists.rows)
         return fl_fail(FL_ERR_ARG, "%s: bad shape", what);
     if (op->M && op->K && (!op->x || !op->weight)) return fl_fail(FL_ERR_ARG, "%s: null pointer", what);
+    if (op->dtype == FL_BF16 && op->train && op->K > most_inputs(false))
+        return fl_fail(FL_ERR_ARG, "%s: bfloat16 in training has up to %d inputs (shape)", what, (int)most_inputs(false));
     return check_lists(&op->lists, what);
 }
 

@@ -158,6 +158,8 @@ def linear_cross_entropy(x, weight, target, bias=None):
     in weight's gradient.  A target that the bias takes out has loss inf, a row
     of which nothing is left 0 without a gradient.
 
+    In training, bfloat16 has up to 2^23 inputs.
+
     No logits are kept: the backward computes them again, a piece of the
     vocabulary at a time, in a workspace of up to 1 GB (of 256 columns
     where there are more rows than that holds).  Large products lay float32 operands out as

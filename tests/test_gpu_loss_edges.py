@@ -86,7 +86,7 @@ def _reference(x, w, b, ids, g):
     else:
         dd = dd + 2.0 ** -11 * d.abs() + 2.0 ** -39 * c.abs()
         share = torch.where(c == 0, 0.0, d / torch.where(c == 0, 1.0, c)).abs()
-        lost = 2.0 ** -38 * 2 * (c.abs() * x.abs().amax(1, keepdim=True)).max() * share.sum(0)[:, None]
+        lost = 2.0 ** -38 * 2 * (c.abs() * (x.abs().amax(1, keepdim=True) if K else 0.0)).max() * share.sum(0)[:, None]
     out = {"loss": (loss, dloss * 1.01 + 1e-30)}
     for name, a, da, v, n in (("dx", d, dd, w, w.shape[0]), ("dw", d.T, dd.T, x, M)):
         out[name] = (a @ v, da @ v.abs() + (n + 16) * E * (a.abs() @ v.abs()) + (lost if name == "dw" else 0.0))
@@ -171,3 +171,28 @@ def test_sizes_of_rows_stay_with_them(M, K, V, t):
         other = _run(y, w, b, ids, None, g)
         for k in ("loss", "dx"):
             assert torch.equal(other[k][rows], one[k][rows]), (k, factor)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M", [3, 70])
+def test_no_inputs(M, t):
+    """The logits are the bias: its gradient is all there is."""
+    x, w, b, ids, _, g = _make(M, 0, 300, t, 8)
+    _check(x, w, b.float(), ids, g)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_more_than_a_million_inputs(t):
+    """x is 0 but for some inputs at both ends, so that the others add nothing and lose nothing."""
+    M, K, V = 3, (1 << 20) + 72, 5
+    some = torch.cat((torch.arange(40), torch.arange(K - 40, K)))
+    x, w, b, ids, _, g = _make(M, len(some), V, t, 9)
+    long_x = torch.zeros(M, K, dtype=t)
+    long_x[:, some] = x
+    long_w = torch.randn(V, K, generator=torch.Generator().manual_seed(10)).to(t)
+    long_w[:, some] = w
+    ref, out = _reference(x, w, b, ids, g), _run(long_x, long_w, b, ids, None, g)
+    for k, (value, bound) in ref.items():
+        got = out[k][:, some] if k in ("dx", "dw") else out[k]
+        _held(got, value, bound, k)
+    assert (out["dw"][:, 40:K - 40] == 0).all()

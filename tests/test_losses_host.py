@@ -106,3 +106,12 @@ def test_vocab_arguments():
     large = op(_lists(rows=4096), M=4096, V=4096, K=64, ldx=64, ldw=64)
     assert lib.fl_vocab_layout_bytes(large) > 4 * 2 * 4096 * 64 and lib.fl_vocab_layout_bytes(op()) == 0
     assert "null" in fwd(large)
+
+
+def test_many_bfloat16_inputs_in_training():
+    lib = _lib.lib()
+    op = lambda K, **kw: _lib.FlVocab(lists=_lists(), M=4, V=6, K=K, x=16, ldx=K, weight=16, ldw=K, dtype=1, **kw)
+    fwd = lambda p: _error(lib.fl_vocab_forward(None, p, ONE, ONE, ONE, ONE, 0))
+    assert "inputs" in fwd(op((1 << 23) + 1, train=1))
+    assert "inputs" not in fwd(op(1 << 23, train=1)) and "inputs" not in fwd(op((1 << 23) + 1))
+    assert lib.fl_vocab_layout_bytes(op(1 << 23, train=1)) > 2 * 10 << 23
