@@ -1787,6 +1787,7 @@ int fl_vocab_forward(void *stream, const fl_vocab *op, float *loss, void *state,
     const size_t need = fl_vocab_forward_bytes(op);
     if (!loss || !state || (!layout && fl_vocab_layout_bytes(op))) return fl::fl_fail(FL_ERR_ARG, "linear_loss: null pointer");
     if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "linear_loss: workspace too small");
+    if ((uintptr_t)layout % 16) return fl::fl_fail(FL_ERR_ARG, "linear_loss: layout must be 16-byte aligned");
     FL_BY_TYPE(op->dtype, fl::vocab_forward<T>((hipStream_t)stream, op, loss, state, layout, ws))
 }
 
@@ -1805,6 +1806,7 @@ int fl_vocab_backward(void *stream, const fl_vocab *op, const float *grad, void 
     const size_t need = fl_vocab_backward_bytes(op, dx != nullptr, dw != nullptr, db != nullptr);
     if (ws_bytes < need || (need && !ws)) return fl::fl_fail(FL_ERR_ARG, "linear_loss: workspace too small");
     if ((uintptr_t)ws % 16) return fl::fl_fail(FL_ERR_ARG, "linear_loss: workspace must be 16-byte aligned");
+    if ((uintptr_t)layout % 16) return fl::fl_fail(FL_ERR_ARG, "linear_loss: layout must be 16-byte aligned");
     FL_BY_TYPE(op->dtype, fl::vocab_backward<T>((hipStream_t)stream, op, grad, state, layout, dx, dw, db, (char *)ws))
 }
 

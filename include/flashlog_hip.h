@@ -1013,9 +1013,10 @@ typedef struct fl_vocab {
 
 size_t fl_vocab_op_bytes(void);
 /* Bytes of the operands as the products take them where large products lay
- * them out anew (fp32 as two fp16 planes, bf16 in training as scaled fp16, rows
- * that do not lie on 16 bytes; else 0): a forward writes them, its backward, of
- * the same operands on the same strides, reads them. */
+ * them out anew (fp32 as three bf16 planes, bf16 in training as scaled fp16,
+ * 16-bit rows that do not lie on 16 bytes; else 0): a forward writes them, its
+ * backward, of the same operands on the same strides, reads them.  layout on a
+ * 16-byte boundary. */
 size_t fl_vocab_layout_bytes(const fl_vocab *op);
 size_t fl_vocab_forward_bytes(const fl_vocab *op);
 int fl_vocab_forward(void *stream, const fl_vocab *op, float *loss,

@@ -115,3 +115,12 @@ def test_many_bfloat16_inputs_in_training():
     assert "inputs" in fwd(op((1 << 23) + 1, train=1))
     assert "inputs" not in fwd(op(1 << 23, train=1)) and "inputs" not in fwd(op((1 << 23) + 1))
     assert lib.fl_vocab_layout_bytes(op(1 << 23, train=1)) > 2 * 10 << 23
+
+
+def test_layouts_lie_on_16_bytes():
+    lib = _lib.lib()
+    op = _lib.FlVocab(lists=_lists(), M=4, V=6, K=64, x=16, ldx=64, weight=16, ldw=64, dtype=1, train=1)
+    assert lib.fl_vocab_layout_bytes(op) > 0
+    off = ctypes.c_void_p(24)
+    assert "layout" in _error(lib.fl_vocab_forward(None, op, ONE, ONE, off, ONE, 1 << 20))
+    assert "layout" in _error(lib.fl_vocab_backward(None, op, ONE, ONE, off, ONE, ONE, ONE, ONE, 1 << 30))
