@@ -161,18 +161,22 @@ def linear_cross_entropy(x, weight, target, bias=None):
     In training, bfloat16 has up to 2^23 inputs.
 
     No logits are kept: the backward computes them again, a piece of the
-    vocabulary at a time, in a workspace of up to 1 GB (of 256 columns
-    where there are more rows than that holds).  Large products lay float32 operands out as
-    three bfloat16 planes (1.5 times their size; all of their 24 bits, at
-    float32's range), and bfloat16 ones in training as scaled half
-    (a copy of x and weight, held for the backward): a bfloat16 value is off by
-    nothing, or by 2^-38 of the largest of its row of x or of weight.  The logits' gradient is
-    an operand of two products and a term of the bias's: float32's is held as
-    such; of 16-bit operands the softmax's terms less what the row is held to
-    are held as half (2^-11 of themselves or 2^-39; of up to 64 rows of half
-    with what rounding leaves), whatever the losses' gradients are, and in
-    weight's gradient each row's input times its loss's (2^-38 of the largest
-    of all rows).
+    vocabulary at a time.  Its workspace is up to 1 GB of their gradient (256
+    columns where there are more rows than that holds), float32 sums of x's
+    gradient (of its size where the vocabulary takes several pieces, else up to
+    64 MB) and of weight's (up to 64 MB), and a copy of 16-bit x.  Held from the
+    forward to the backward are copies of x and weight, where large products
+    lay them out: float32 as three bfloat16 planes (1.5 times their size; all
+    of their 24 bits, at float32's range), half whose rows are not whole steps
+    of 64 inputs on 16 bytes, and bfloat16, always, as scaled half (a value is
+    off by nothing, or by 2^-38 of the largest of its row of x or of weight).
+
+    The logits' gradient is an operand of two products and a term of the
+    bias's: float32's is held as such; of 16-bit operands the softmax's terms
+    less what the row is held to are held as half (2^-11 of themselves or
+    2^-39; of up to 64 rows of half with what rounding leaves), whatever the
+    losses' gradients are, and in weight's gradient each row's input times its
+    loss's (2^-38 of the largest of all rows).
     Softmax terms are off by 2^-23 of themselves times 1 + their logit's
     distance from the largest (at least 16 over large vocabularies), whatever
     all logits have in common; a bias whose quotient by the temperature
