@@ -130,7 +130,9 @@ __global__ __launch_bounds__(LS_NT) void k_score_grad(ScoreArgs a) {
 #pragma unroll
         for (int e = 0; e < G; ++e)
             s.v[i].v[e] =
-                (T)(c == 0.0f ? 0.0f : f * exp2_of(((float)s.v[i].v[e] - of.x) * a.scale));
+                (T)(c == 0.0f || (float)s.v[i].v[e] == -INFINITY
+                        ? 0.0f  // masked, whatever its row holds
+                        : f * exp2_of(((float)s.v[i].v[e] - of.x) * a.scale));
         const int64_t at = c0 + (i * FL_WAVE + fl_lane()) * G;
         if (at + G <= a.cols) store_cols<T, G>(out + at, s.v[i]);
         else store_first<T, G>(out + at, s.v[i], (int)(a.cols - at));
@@ -150,7 +152,7 @@ __global__ __launch_bounds__(LS_NT) void k_score_grad(ScoreArgs a) {
         waited = true;
         if (here) {
             const float2 l = a.listed[row * a.op.k + j];
-            out[id] = (T)(c * (exp2_of((l.x - of.x) * a.scale) * of.y - l.y));
+            if (l.x != -INFINITY) out[id] = (T)(c * (exp2_of((l.x - of.x) * a.scale) * of.y - l.y));
         }
     }
 }

@@ -196,3 +196,22 @@ def test_more_than_a_million_inputs(t):
         got = out[k][:, some] if k in ("dx", "dw") else out[k]
         _held(got, value, bound, k)
     assert (out["dw"][:, 40:K - 40] == 0).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_masked_columns_beside_what_is_not_finite(t):
+    """Their gradient is 0 in rows with a NaN or an infinity, and where the loss's own gradient is one."""
+    g = torch.Generator().manual_seed(12)
+    z = torch.randn(5, 3000, generator=g).to(t)
+    masked = torch.rand(5, 3000, generator=g) < 0.5
+    ids = torch.randint(0, 3000, (5, 9), generator=g)
+    z[masked] = -float("inf")
+    z[0, ~masked[0]] = float("nan")
+    z[1, ids[1, 0]] = float("inf")
+    masked[1, ids[1, 0]] = False
+    grad = torch.tensor([1.0, 1.0, float("inf"), float("nan"), 1.0])
+    leaf = z.cuda().requires_grad_(True)
+    loss = _losses().distillation(leaf, ids.cuda(), torch.randn(5, 9, generator=g).cuda())
+    dx = torch.autograd.grad(loss, leaf, grad.cuda())[0].cpu()
+    assert (dx[masked] == 0).all()
+    assert dx[0][~masked[0]].isnan().all() and dx[4].isfinite().all() and (dx[4] != 0).any()
