@@ -568,11 +568,12 @@ __global__ __launch_bounds__(LN_NT) void k_vocab_dw(VocabArgs a) {
 // wave keeps x's columns of its band in registers and walks the vocabulary, 16
 // columns of dz a tile, whose loads are a tile ahead.  The tile's values go through
 // the wave's own LDS, so that a store takes whole rows of the band; of rows of whole
-// 16 bytes nothing is masked, and lanes behind the end store what others do: where the
-// number of stores is known the wait for the loads leaves them in flight.  fp32 [23 x
-// 1152 -> 431394] 428 us = 4.6 TB/s (stores of 64 bytes of 16 rows, masked, 686; tiles
-// of 128 x 128 1011), fp16 [4 x 1024 -> 400000] 160 (363; 610), bf16 [16 x 512 ->
-// 200000] 45 (101; 160).
+// 16 bytes nothing is masked, and lanes behind the end store what others do.  fp32 [23
+// x 1152 -> 431394] 420 us = 4.7 TB/s (stores of 64 bytes of 16 rows, masked, 686;
+// tiles of 128 x 128 1011), fp16 [4 x 1024 -> 400000] 167 (363; 610), bf16 [16 x 512 ->
+// 200000] 46 (101; 160).  The stores of a tile are waited for with the next one's loads:
+// left in flight 474 for 420, [17 x 544 -> 1001465] 583 for 510 and bf16 [60 x 512 ->
+// 200000] 72 for 64, against 162 for 167, 42 for 46 and [120 x 512 -> 200000] 119 for 127.
 // Up to 128 rows of 16-bit values and 64 of fp32 ([120 x 512 -> 200000] bf16 127 us,
 // 189 by k_wide_dw's tiles, fp32 319 and 303).
 inline int64_t few_rows(int dtype) { return dtype == FL_F32 ? 64 : 128; }
@@ -633,6 +634,7 @@ __global__ __launch_bounds__(LS_NT) void k_few_dw(VocabArgs a) {
         constexpr bool WHOLE = decltype(whole)::value;
         load(run);
         for (int64_t t = run; t < tiles; t += runs) {
+            if constexpr (WHOLE) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
             u32x4 d[KS][P];
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
