@@ -33,7 +33,8 @@ constexpr int NM_WAVE_COLS = 512;
 constexpr int NM_ROW_COLS = NM_LANE * FL_WAVE * NM_WAVES;
 // Most workgroups that walk the rows: forward ([16384 x 2048] bf16, us with 512, 1024,
 // 1536, 4096 of them 53, 37, 31, 33) and backward, each of which leaves a row of sums
-// (with 512, 1024, 1536, 2048 of them 68 + 4, 46 + 5, 56 + 6, 51 + 8).
+// (with 512, 1024, 1536, 2048 of them 68 + 4, 46 + 5, 56 + 6, 51 + 8).  Of fewer rows
+// not chosen apart: 1536 are one or two a workgroup, 12 + 5 us of 2048 fp32 columns for 8.
 constexpr int64_t NM_WALKS = 4096;
 constexpr int64_t NM_GRAD_WALKS = 1024;
 
@@ -234,7 +235,9 @@ __global__ __launch_bounds__(NM_NT) void k_norm_rows(NormArgs a) {
     }
 }
 
-// Rows of any length: a workgroup a row, read once for each sum and once more.
+// Rows of any length: a workgroup a row, read once for each sum and once more, from the
+// caches but for the first: [1024 x 20000] fp32 60 us = 2.7 TB/s of one read and one
+// write, bf16 42.
 template <typename T, typename W>
 __global__ __launch_bounds__(NM_NT) void k_norm_long(NormArgs a) {
     __shared__ float lds[2 * NM_WAVES * 2];
@@ -377,7 +380,8 @@ __global__ __launch_bounds__(NM_NT) void k_norm_grad(NormArgs a) {
     }
 }
 
-// dx of rows of any length.
+// dx of rows of any length: [1024 x 20000] fp32 64 us = 3.8 TB/s of two reads and one
+// write, bf16 49.
 template <typename T, typename W>
 __global__ __launch_bounds__(NM_NT) void k_norm_long_grad(NormArgs a) {
     __shared__ float lds[2 * NM_WAVES * 2];
@@ -419,7 +423,8 @@ __global__ __launch_bounds__(NM_NT) void k_norm_long_grad(NormArgs a) {
     }
 }
 
-// The sums over a part of the rows, a column a thread.
+// The sums over a part of the rows, a column a thread: [1024 x 20000] fp32 29 us = 5.6
+// TB/s, bf16 24.
 template <typename T>
 __global__ __launch_bounds__(NM_NT) void k_norm_cols(NormArgs a, int parts) {
     const int64_t blocks = (a.N + NM_NT - 1) / NM_NT, item = fl_block();

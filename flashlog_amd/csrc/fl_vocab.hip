@@ -263,8 +263,8 @@ __global__ __launch_bounds__(1024) void k_vocab_coef(const float2 *__restrict__ 
 // Where dz is half: a row's tau g as a number of 2^14..2^15, which its dz is multiplied
 // by, and a power of two, which its row of dx, its terms of db and its row of dW's
 // other operand are multiplied by.  So what half can hold is that of p - q, 2^-39
-// absolute, in every row, whatever the rows' gradients are to each other.  A wave a row;
-// most: the largest exponent of a workgroup's rows of x times that power.
+// absolute, in every row, whatever the rows' gradients are to each other.  A wave a row:
+// [8192 x 512] bf16 5.7 us; most: the largest exponent of a workgroup's rows of x times that power.
 constexpr int LAY_PARTS = 1024;
 constexpr int NO_EXP = -(1 << 20);
 
@@ -318,6 +318,7 @@ __global__ __launch_bounds__(LS_NT) void k_row_scale(VocabArgs a, const float *_
 
 // dW's other operand in half: rows of x times their power of two and one of all rows,
 // which brings the largest value to 2^13..2^14; 0 in rows without a gradient.
+// HBM-bound: [8192 x 512] bf16 6.6 us.
 template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_lay_y(VocabArgs a, const int *__restrict__ most, int parts,
                                                  _Float16 *__restrict__ y, int *__restrict__ y_exp) {
@@ -935,10 +936,10 @@ __device__ __forceinline__ void lane_bias(const VocabArgs &a, int64_t n, float (
 // end.  An exponent is one multiply-add from the product; the maximum is the
 // lane's first until a sum passes 2^20, so that it is not looked for in every tile
 // (and an exponent that counts is rounded by no more than 2^-20).
-// bf16 [8192 x 512 -> 41000] 339 us = 1014 TFLOP/s, fp16 [4096 x 1024 -> 123000]
-// 945 us = 1092 (a large library product 1313 and 1451 on the same card), fp32
-// [1536 x 2048 -> 1645] 81 us = 128 (153), six products each in 156 tiles on 256
-// CUs; [512 x 128 -> 4.6M] bf16 961 us = 627: of two steps a tile, the exponentials
+// bf16 [8192 x 512 -> 41000] 339 to 348 us = 988 to 1014 TFLOP/s, fp16 [4096 x 1024
+// -> 123000] 945 to 994 us = 1038 to 1092 (a large library product 1313 and 1451 on the same card), fp32
+// [1536 x 2048 -> 1645] 78 us = 132 (153), six products each in 156 tiles on 256
+// CUs; [512 x 128 -> 4.6M] bf16 954 us = 632: of two steps a tile, the exponentials
 // are half.
 template <typename T, typename H, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
@@ -1018,7 +1019,7 @@ __global__ __launch_bounds__(WD_NT) void k_wide_stats(VocabArgs a) {
 }
 
 // dz of a piece but for the listed columns (a row's only one is made in its tile).
-// 436, 1073 and 83 us where k_wide_stats takes 339, 945 and 81: what dz's stores
+// 443, 1085 and 80 us where k_wide_stats takes 348, 994 and 78: what dz's stores
 // add, 672 MB of them in the first.
 template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_grad(VocabArgs a) {
@@ -1152,7 +1153,8 @@ __global__ __launch_bounds__(LS_NT) void k_wide_cols(VocabArgs a) {
 
 // A piece's part of dx, added to what is there if `add`; with one part and one piece
 // the result itself.  bf16 [8192 x 512 -> 41000] 333 us = 1033 TFLOP/s, fp16
-// [4096 x 1024 -> 123000] 868 us = 1189; the weight's steps are read transposed
+// [4096 x 1024 -> 123000] 860 us = 1200, fp32 [1536 x 2048 -> 1645] 75 us = 138; the
+// weight's steps are read transposed
 // from LDS.
 template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
@@ -1231,8 +1233,10 @@ __global__ __launch_bounds__(WD_NT) void k_wide_dx(VocabArgs a) {
 }
 
 // A piece's rows of dW, or of a part of the rows' sum: tiles in a row.  Both
-// operands are read transposed, with twice the LDS instructions of k_wide_dx: 468
-// us = 735 TFLOP/s and 1163 us = 887 in its cases.
+// operands lie with the rows of x one after the other and are read transposed, with
+// twice the LDS instructions of k_wide_dx: 463 us = 743 TFLOP/s and 1172 us = 880 in
+// its cases, fp32 [1536 x 2048 -> 1645] 76 us = 137.  (x could be laid out the other
+// way round; it is not.)
 template <typename T, int BM, int WN, int STAGES>
 __global__ __launch_bounds__(WD_NT) void k_wide_dw(VocabArgs a) {
     constexpr int P = planes_of<T>();
