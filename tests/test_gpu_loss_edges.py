@@ -215,3 +215,24 @@ def test_masked_columns_beside_what_is_not_finite(t):
     dx = torch.autograd.grad(loss, leaf, grad.cuda())[0].cpu()
     assert (dx[masked] == 0).all()
     assert dx[0][~masked[0]].isnan().all() and dx[4].isfinite().all() and (dx[4] != 0).any()
+
+
+def test_bfloat16_rows_of_the_most_inputs():
+    """2^23 of them, in so many rows of the weight that a tile's offsets reach the end of 32 bits."""
+    M, K, V = 2, 1 << 23, 300
+    some = torch.cat((torch.arange(40), torch.arange(K - 40, K)))
+    x, w, b, ids, _, g = _make(M, len(some), V, torch.bfloat16, 13)
+    ids[0] = V - 1
+    long_x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    long_x[:, some] = x.cuda()
+    long_w = torch.full((V, K), 0.5, dtype=torch.bfloat16, device="cuda")
+    long_w[:, some] = w.cuda()
+    ref, out = _reference(x, w, b, ids, g), _run(long_x, long_w, b, ids, None, g)
+    for k, (value, bound) in ref.items():
+        got = out[k][:, some] if k in ("dx", "dw") else out[k]
+        _held(got, value, bound, k)
+    # where x is 0: a weight of 1/2 times the sum of a row's gradients, which is 0 within their bound
+    d = torch.softmax(x.double() @ w.double().T + b.double(), 1).scatter_add_(1, ids, -torch.ones(M, 1).double())
+    bound = 0.5 * g.double() * (2.0 ** -11 + 2.0 ** -16) * d.abs().sum(1) + 2.0 ** -39 * V
+    assert (out["dx"][:, 40:K - 40].abs().amax(1).double().cpu() <= bound * (1 + 2.0 ** -8)).all()
+    assert (out["dw"][:, 40:K - 40] == 0).all()
