@@ -6,9 +6,10 @@
 //   dx = dz W      dW = dz^T x      db = sum over the rows of dz
 //
 // The piece of dz is what a call holds of [rows x vocabulary], in 16 bits (an
-// operand of two products; fp32: as it is or in three bfloat16 planes).  The listed columns' own u comes
-// from a dot product each; their entries of dz are made apart, since p - q of
-// values rounded before would keep few bits where p is near 1.
+// operand of two products; fp32: as it is or in three bfloat16 planes).  The
+// listed columns' own u comes from a dot product each; their entries of dz are
+// made apart, since p - q of values rounded before would keep few bits where p is
+// near 1.
 //
 // Bound by the matrix instructions: four products where logits that are kept
 // would need three, beside 2 or 4 bytes of dz a logit written once and read twice.
@@ -263,8 +264,9 @@ __global__ __launch_bounds__(1024) void k_vocab_coef(const float2 *__restrict__ 
 // Where dz is half: a row's tau g as a number of 2^14..2^15, which its dz is multiplied
 // by, and a power of two, which its row of dx, its terms of db and its row of dW's
 // other operand are multiplied by.  So what half can hold is that of p - q, 2^-39
-// absolute, in every row, whatever the rows' gradients are to each other.  A wave a row:
-// [8192 x 512] bf16 5.7 us; most: the largest exponent of a workgroup's rows of x times that power.
+// absolute, in every row, whatever the rows' gradients are to each other.  A wave a
+// row, [8192 x 512] bf16 5.7 us; most: the largest exponent of a workgroup's rows of x
+// times that power.
 constexpr int LAY_PARTS = 1024;
 constexpr int NO_EXP = -(1 << 20);
 
@@ -707,12 +709,6 @@ __global__ __launch_bounds__(LS_NT) void k_vocab_cols(VocabArgs a) {
 // ---------------------------------------------------------------------------
 // The same for large products
 
-// bfloat16 in training: rows of x laid out, a wave each (blockIdx.y 0), and the largest
-// finite magnitude of weight, a part of it a workgroup.  HBM-bound: 1.18 GB of weight in
-// 263 us = 4.5 TB/s.  A row of x is multiplied by a power of two of its own, so that rows
-// of any sizes keep their bits beside each other (as operands of the logits: dW takes
-// them from k_lay_y); one in which nothing is listed is zeros (padded rows may hold
-// anything).
 // The power of two that brings m to 2^13..2^14 is 2^(14 - e).
 __device__ __forceinline__ int exponent_of(float m) {
     int e;
@@ -720,6 +716,12 @@ __device__ __forceinline__ int exponent_of(float m) {
     return e < -100 ? -100 : e;
 }
 
+// bfloat16 in training: rows of x laid out, a wave each (blockIdx.y 0), and the largest
+// finite magnitude of weight, a part of it a workgroup.  HBM-bound: 1.18 GB of weight in
+// 263 us = 4.5 TB/s.  A row of x is multiplied by a power of two of its own, so that rows
+// of any sizes keep their bits beside each other (as operands of the logits: dW takes
+// them from k_lay_y); one in which nothing is listed is zeros (padded rows may hold
+// anything).
 template <typename T>
 __global__ __launch_bounds__(LS_NT) void k_lay_max(VocabArgs a, float *__restrict__ most, _Float16 *__restrict__ out,
                                                    float *__restrict__ undo_x) {
